@@ -52,6 +52,22 @@ class Epilogue(ctypes.Structure):
 
 _EPI = ctypes.POINTER(Epilogue)
 
+
+CT_ATTENTION_FORWARD, CT_ATTENTION_ROWS, CT_ATTENTION_KEYS = 0, 1, 2
+
+
+class Attention(ctypes.Structure):
+    """Mirror of `ct_attention`: the operands of attention over packed records."""
+
+    _fields_ = [
+        ("q", _P), ("k", _P), ("v", _P), ("q_token", _I64), ("q_head", _I64), ("k_token", _I64), ("k_head", _I64),
+        ("v_token", _I64), ("v_head", _I64), ("records", _P), ("heads", _I32), ("kv_heads", _I32),
+        ("head_dim", _I32), ("dtype", _I32), ("causal", _I32), ("scale", ctypes.c_float),
+    ]
+
+
+_ATT = ctypes.POINTER(Attention)
+
 _SIGNATURES = {
     "ct_abi_version": (ctypes.c_int, []),
     "ct_init_device": (ctypes.c_int, []),
@@ -96,6 +112,11 @@ _SIGNATURES = {
     "ct_cast_f32_bf16": (ctypes.c_int, [_P, _P, _P, _I32, _P]),
     "ct_adamw_step": (ctypes.c_int, [_P, _I64, _P, _I64, _I64, _I32, ctypes.c_double, ctypes.c_double,
                                      ctypes.c_double, ctypes.c_double, ctypes.c_double, _I32, _I32, _P]),
+    "ct_attention_plan": (ctypes.c_int, [_I32, _P, _I64, _I32, _I32, _I32, _I32, _P, _I64, _P]),
+    "ct_attention_workspace": (_I64, [_I32, _I64, _I32, _I32]),
+    "ct_attention_forward": (ctypes.c_int, [_ATT, _P, _P, _P, _P, _P, _I64, _P]),
+    "ct_attention_backward": (ctypes.c_int, [_ATT, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _I64,
+                                             _P]),
     "ct_profile_begin": (ctypes.c_int, [_I32, _I32]),
     "ct_profile_read": (ctypes.c_int, [_I32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_I64),
                                        ctypes.POINTER(ctypes.c_double)]),

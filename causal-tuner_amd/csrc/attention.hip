@@ -1,0 +1,981 @@
+// Attention over packed records on gfx950: forward, and the backward that recomputes the
+// probabilities. Per record and head, with query i and key j of the record,
+//   s_ij = scale q_i . k_j          visible: j < limit_i = keys (plain) or
+//                                   min(keys, i + 1 + keys - queries) (causal)
+//   p_ij = exp(s_ij - lse_i),  lse_i = log sum_j exp(s_ij),  o_i = sum_j p_ij v_j
+//   delta_i = do_i . o_i,  ds_ij = p_ij (do_i . v_j - delta_i)
+//   dv_j = sum_i p_ij do_i,  dk_j = scale sum_i ds_ij q_i,  dq_i = scale sum_j ds_ij k_j
+// (the place of the reference's kernels/attention.py:58-93, which calls a library).
+//
+// Rows. The `group` query heads of one key/value head are rows of one matrix: row r of a
+// record is token r / group, head r % group. One tile of keys then serves all heads of the
+// group, a single token of a shared head already fills rows, and the key gradients' sum
+// over heads is the sum over rows.
+//
+// Matrix products. Every product is v_mfma_*_32x32x* with the wave's own rows (forward and
+// dq) or keys (dk, dv) as the column index, so lane l holds column l % 32 of the scores and
+// 16 of their 32 rows: softmax statistics are one register per lane, the probabilities go
+// from the accumulators straight into the next product's B operand (rounded to bf16 in
+// pairs; the operands' k order follows the accumulator's), and the outputs o^T, dq^T, dk^T
+// and dv^T accumulate 32 rows of the head dimension at a time. The A operands come from
+// LDS: rows as stored (ds_read_b128) for the scores, transposed (ds_read_b64_tr_b16) for
+// the outputs.
+//
+// Rounding. Scores, statistics, delta and all sums are fp32. bf16 inputs round p and ds to
+// bf16 for the second products (half a unit in the last place each, 2^-9 relative, below
+// the 2^-9 of the output's own rounding once averaged over the keys); float32 inputs round
+// nothing.
+//
+// dq and dk/dv are two kernels that each recompute s (7 products instead of 5): the one-pass
+// form would add dq over workgroups by atomics, whose order changes results from run to run.
+
+#include <math.h>
+
+#include <algorithm>
+#include <type_traits>
+#include <vector>
+
+#include "gemm_common.hpp"
+
+namespace ct {
+namespace {
+
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
+
+constexpr int kThreads = 256;   // 4 waves
+constexpr int kWaveCols = 32;   // rows (forward, dq) or keys (dk, dv) per wave
+constexpr int kTile = 128;      // per workgroup
+constexpr int kEntry = 8;       // int32 per plan entry
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Record {
+    int64_t q_start, q_len, k_start, k_len;
+};
+
+struct Item {
+    int32_t record, begin, lo, hi, slot, pad0, pad1, pad2;
+};
+
+struct AttnParams {
+    const char *q, *k, *v, *out, *dout;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;  // bytes
+    int64_t o_token, o_head;                                    // bytes: out, dq (contiguous)
+    int64_t do_token, do_head;                                  // bytes
+    const Record *records;
+    const Item *items;
+    char *dst0, *dst1;    // out | dq | dk, dv
+    int64_t d_token;      // bytes between tokens of dst0 and dst1
+    float *stats;         // [tokens, heads] lse * log2(e), +inf where a row sees no key
+    float *delta;         // [tokens, heads]
+    float *part0, *part1; // split partials
+    int32_t heads, kv_heads, group, head_dim, causal;
+    uint32_t magic;       // r / group = (r * magic) >> shift for r < 2^31
+    int32_t shift;
+    float scale, scale2;  // scale, scale * log2(e)
+};
+
+__device__ __forceinline__ uint32_t div_group(const AttnParams &a, uint32_t r) {
+    return (uint32_t)(((uint64_t)r * a.magic) >> a.shift);
+}
+
+// ------------------------------------------------------------------ LDS tiles
+// A tile holds rows of DP elements (DP * sizeof(T) = 128, 256 or 512 bytes) in 16-byte
+// chunks. ds_read_b128 serves lanes {0-7, 24-31}, {8-15, 16-23}, ... in one pass each over
+// 16 units, and the fragment reads take 32 rows at one chunk; the transposing reads take
+// four consecutive rows at four chunks. XORing the chunk with the row's low four bits, its
+// two pairs exchanged, makes both conflict-free; 128-byte rows share a 256-byte line in
+// pairs and use the line number the same way.
+template <typename T, int DP>
+struct Tile {
+    static constexpr int kBytes = DP * (int)sizeof(T);
+    static constexpr int kChunks = kBytes / 16;
+    static constexpr int kFrags = kChunks / 2;   // 16-byte fragments of a row per lane half
+    __device__ static __forceinline__ int addr(int r, int c) {
+        if constexpr (kBytes == 128) {
+            const int line = r >> 1;
+            return line * 256 + (((((r & 1) << 3) | c) ^ (((line & 1) << 2) | ((line >> 1) & 3))) << 4);
+        } else {
+            return r * kBytes + ((c ^ (((r & 3) << 2) | ((r >> 2) & 3))) << 4);
+        }
+    }
+};
+
+typedef const __attribute__((address_space(3))) char lds_char;
+
+__device__ __forceinline__ lds_char *lds_of(const uint4 *p) { return (lds_char *)p; }
+
+__device__ __forceinline__ uint4 lds_read16(lds_char *p) {
+    return __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) u32x4 *)p);
+}
+
+// acc[row, col] += sum_d tile[row0 + row][d] * frag[col][d]
+template <typename T, int DP>
+__device__ __forceinline__ void scores(f32x16 &acc, const uint4 *tile, int row0, const uint4 (&frag)[Tile<T, DP>::kFrags],
+                                       int lane) {
+    lds_char *base = lds_of(tile);
+    const int h = lane >> 5, row = lane & 31;
+#pragma unroll
+    for (int s = 0; s < Tile<T, DP>::kFrags; ++s) {
+        const uint4 a = lds_read16(base + row0 * Tile<T, DP>::kBytes + Tile<T, DP>::addr(row, 2 * s + h));
+        if constexpr (sizeof(T) == 2) {
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                          __builtin_bit_cast(bf16x8, frag[s]), acc, 0, 0, 0);
+        } else {
+            const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, frag[s]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], acc, 0, 0, 0);
+        }
+    }
+}
+
+// acc[b][d, col] += sum_row tile[row0 + row][32 b + d] * p[row, col], p as `scores` leaves it:
+// register i of lane half h is row 8 (i / 4) + 4 h + i % 4.
+template <typename T, int DP>
+__device__ __forceinline__ void outer(f32x16 (&acc)[DP / 32], const uint4 *tile, int row0, const f32x16 &p, int lane) {
+    lds_char *base = lds_of(tile) + row0 * Tile<T, DP>::kBytes;
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+        const int row = 4 * h + ((lane & 15) >> 2);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            uint4 b;
+            b.x = pack_bf16x2(p[8 * s], p[8 * s + 1]);
+            b.y = pack_bf16x2(p[8 * s + 2], p[8 * s + 3]);
+            b.z = pack_bf16x2(p[8 * s + 4], p[8 * s + 5]);
+            b.w = pack_bf16x2(p[8 * s + 6], p[8 * s + 7]);
+#pragma unroll
+            for (int n = 0; n < DP / 32; ++n) {
+                const int c = 4 * n + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), o = (lane & 1) * 8;
+                lds_char *lo = base + 16 * s * Tile<T, DP>::kBytes + Tile<T, DP>::addr(row, c) + o;
+                lds_char *hi = base + 16 * s * Tile<T, DP>::kBytes + Tile<T, DP>::addr(row + 8, c) + o;
+                const uint2 l2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_kt_v4s *)lo));
+                const uint2 h2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_kt_v4s *)hi));
+                const uint4 a = make_uint4(l2.x, l2.y, h2.x, h2.y);
+                acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                                 __builtin_bit_cast(bf16x8, b), acc[n], 0, 0, 0);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int row = 8 * (i >> 2) + 4 * h + (i & 3);
+#pragma unroll
+            for (int n = 0; n < DP / 32; ++n) {
+                const float a = *(const __attribute__((address_space(3))) float *)(
+                    base + Tile<T, DP>::addr(row, 8 * n + ((lane & 31) >> 2)) + (lane & 3) * 4);
+                acc[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[i], acc[n], 0, 0, 0);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ global -> LDS
+// One thread's share of a tile of ROWS rows, held in registers between the load and the
+// LDS store. `at(row)` gives the byte offset of a row from the base, or kOOB: an offset
+// past the buffer's range reads zeros, so nothing behind a record's end enters a product
+// (a masked zero times a NaN there would be NaN).
+template <typename T, int DP, int ROWS>
+struct Stage {
+    static constexpr int kChunks = Tile<T, DP>::kChunks;
+    static constexpr int kLoads = ROWS * kChunks / kThreads;
+    uint4 r[kLoads];
+    template <typename At>
+    __device__ __forceinline__ void load(const char *base, int chunks, At at) {
+        const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(base, 0x7fffffff);
+#pragma unroll
+        for (int p = 0; p < kLoads; ++p) {
+            const int i = p * kThreads + (int)threadIdx.x, row = i / kChunks, c = i % kChunks;
+            const uint32_t off = at(row);
+            r[p] = buf_load16(rsrc, c < chunks && off != kOOB ? off + 16u * (uint32_t)c : kOOB);
+        }
+    }
+    __device__ __forceinline__ void store(uint4 *tile) const {
+#pragma unroll
+        for (int p = 0; p < kLoads; ++p) {
+            const int i = p * kThreads + (int)threadIdx.x, row = i / kChunks, c = i % kChunks;
+            *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(tile) + Tile<T, DP>::addr(row, c)) = r[p];
+        }
+    }
+};
+
+// A row's fragments as the B operand holds them: chunks 2 s + h of the row at `p`.
+template <typename T, int DP>
+__device__ __forceinline__ void row_fragments(const char *p, uint4 (&frag)[Tile<T, DP>::kFrags], bool valid,
+                                              int chunks, int lane) {
+#pragma unroll
+    for (int s = 0; s < Tile<T, DP>::kFrags; ++s) {
+        const int c = 2 * s + (lane >> 5);
+        frag[s] = valid && c < chunks ? *reinterpret_cast<const uint4 *>(p + 16 * c) : zero4();
+    }
+}
+
+__device__ __forceinline__ f32x16 splat(float v) {
+    f32x16 r;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = v;
+    return r;
+}
+
+// Value of the same column in the other half of the wave.
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+// Four consecutive elements of a row at element d.
+template <typename T>
+__device__ __forceinline__ void store4(char *row, int d, float x, float y, float z, float w) {
+    if constexpr (sizeof(T) == 2)
+        *reinterpret_cast<uint2 *>(row + 2 * d) = make_uint2(pack_bf16x2(x, y), pack_bf16x2(z, w));
+    else
+        *reinterpret_cast<float4 *>(row + 4 * d) = make_float4(x, y, z, w);
+}
+
+// ------------------------------------------------------------------ rows of a forward or dq tile
+struct RowOf {
+    bool valid;
+    int64_t token;    // in the whole tensor
+    int head;
+    int limit;        // keys the row sees
+    __device__ __forceinline__ RowOf(const AttnParams &a, const Record &rec, int kv_head, int64_t r) {
+        valid = r < rec.q_len * a.group;
+        const uint32_t t = valid ? div_group(a, (uint32_t)r) : 0;
+        token = rec.q_start + t;
+        head = kv_head * a.group + (valid ? (int)((uint32_t)r - t * (uint32_t)a.group) : 0);
+        const int64_t seen = a.causal ? (int64_t)t + 1 + rec.k_len - rec.q_len : rec.k_len;
+        limit = seen < 0 ? 0 : (int)(seen < rec.k_len ? seen : rec.k_len);
+    }
+};
+
+// Smallest and largest `limit` over the wave's valid rows (INT_MAX and 0 without any).
+__device__ __forceinline__ void wave_limits(const RowOf &row, int &least, int &most) {
+    least = row.valid ? row.limit : 0x7fffffff;
+    most = row.valid ? row.limit : 0;
+#pragma unroll
+    for (int m = 16; m; m >>= 1) {
+        least = min(least, __shfl_xor(least, m, 64));
+        most = max(most, __shfl_xor(most, m, 64));
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+}
+
+template <typename T>
+constexpr int kKeyTile = sizeof(T) == 2 ? 64 : 32;
+
+// Running softmax of a wave's 32 rows over their keys; m2 is the reference exponent of base
+// 2 that p and the sums are relative to.
+struct Running {
+    float m2 = -INFINITY, sum = 0.0f;
+};
+
+// ------------------------------------------------------------------ forward
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_forward(AttnParams a) {
+    constexpr int KT = kKeyTile<T>;
+    constexpr int kUnits = KT * Tile<T, DP>::kChunks;
+    __shared__ uint4 sk[2][kUnits], sv[2][kUnits];
+    const Item item = a.items[blockIdx.x / a.kv_heads];
+    const int kv_head = blockIdx.x % a.kv_heads;
+    const Record rec = a.records[item.record];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chunks = a.head_dim * (int)sizeof(T) / 16;
+
+    const RowOf row(a, rec, kv_head, (int64_t)item.begin + wave * kWaveCols + (lane & 31));
+    int least, most;
+    wave_limits(row, least, most);
+    uint4 qf[Tile<T, DP>::kFrags];
+    row_fragments<T, DP>(a.q + row.token * a.q_token + row.head * a.q_head, qf, row.valid, chunks, lane);
+
+    const char *k0 = a.k + rec.k_start * a.k_token + kv_head * a.k_head;
+    const char *v0 = a.v + rec.k_start * a.v_token + kv_head * a.v_head;
+    Stage<T, DP, KT> ks, vs;
+    auto load = [&](int key) {
+        const int left = (int)rec.k_len - key;
+        ks.load(k0 + key * a.k_token, chunks, [&](int r) { return r < left ? (uint32_t)(r * a.k_token) : kOOB; });
+        vs.load(v0 + key * a.v_token, chunks, [&](int r) { return r < left ? (uint32_t)(r * a.v_token) : kOOB; });
+    };
+
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) o[n] = splat(0.0f);
+    Running run;
+    int buf = 0;
+    if (item.lo < item.hi) {
+        load(item.lo);
+        ks.store(sk[0]);
+        vs.store(sv[0]);
+    }
+    __syncthreads();
+    for (int key = item.lo; key < item.hi; key += KT) {
+        const bool more = key + KT < item.hi;
+        if (more) load(key + KT);
+        if (key < most) {
+            f32x16 s[KT / 32];
+#pragma unroll
+            for (int t = 0; t < KT / 32; ++t) {
+                s[t] = splat(0.0f);
+                scores<T, DP>(s[t], sk[buf], 32 * t, qf, lane);
+            }
+            if (key + KT > least) {
+                const int left = row.limit - key - 4 * (lane >> 5);
+#pragma unroll
+                for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s[t][i] = 32 * t + 8 * (i >> 2) + (i & 3) < left ? s[t][i] : -INFINITY;
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
+            top = fmaxf(top, other_half(top)) * a.scale2;
+            // The reference moves only when a row's maximum has grown by more than 2^8: p then
+            // stays below 2^8, o and the sum are exact in that scale, and most tiles skip the
+            // rescaling of o.
+            if (__any(top > run.m2 + 8.0f)) {
+                const float next = fmaxf(run.m2, top);
+                const float shrink = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run.m2 - next);
+                run.m2 = next;
+                run.sum *= shrink;
+#pragma unroll
+                for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[n][i] *= shrink;
+            }
+            const float ref = run.m2 == -INFINITY ? 0.0f : run.m2;
+#pragma unroll
+            for (int t = 0; t < KT / 32; ++t) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.scale2, -ref));
+                    run.sum += s[t][i];
+                }
+                outer<T, DP>(o, sv[buf], 32 * t, s[t], lane);
+            }
+        }
+        if (more) {
+            ks.store(sk[buf ^ 1]);
+            vs.store(sv[buf ^ 1]);
+        }
+        __syncthreads();
+        buf ^= 1;
+    }
+
+    const float sum = run.sum + other_half(run.sum);
+    const int d0 = 4 * (lane >> 5);
+    if (!row.valid) return;
+    if (item.slot < 0) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        char *dst = a.dst0 + row.token * a.o_token + row.head * a.o_head;
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int d = 32 * n + 2 * i + d0;
+                if (d < a.head_dim)
+                    store4<T>(dst, d, o[n][i] * inv, o[n][i + 1] * inv, o[n][i + 2] * inv, o[n][i + 3] * inv);
+            }
+        if (lane < 32)
+            a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : run.m2 + __builtin_amdgcn_logf(sum);
+    } else {
+        const int64_t at = ((int64_t)item.slot * a.kv_heads + kv_head) * kTile + wave * kWaveCols + (lane & 31);
+        float *dst = a.part0 + at * DP;
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float4 *>(dst + 32 * n + 2 * i + d0) =
+                    make_float4(o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3]);
+        if (lane < 32) *reinterpret_cast<float2 *>(a.part1 + 2 * at) = make_float2(run.m2, sum);
+    }
+}
+
+// Joins the key ranges of split rows: with M = max_s m_s, o = sum_s 2^(m_s - M) o_s over
+// sum_s 2^(m_s - M) sum_s. One wave per row, the parts in order.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void attention_join(AttnParams a, const Item *joins) {
+    const Item join = joins[blockIdx.x / (a.kv_heads * (kTile / 4))];
+    const int rest = blockIdx.x % (a.kv_heads * (kTile / 4));
+    const int kv_head = rest % a.kv_heads, lane = threadIdx.x & 63;
+    const int r = rest / a.kv_heads * 4 + (threadIdx.x >> 6);
+    const Record rec = a.records[join.record];
+    const RowOf row(a, rec, kv_head, (int64_t)join.begin + r);
+    if (!row.valid) return;
+    const int64_t first = ((int64_t)join.lo * a.kv_heads + kv_head) * kTile + r, step = (int64_t)a.kv_heads * kTile;
+    float top = -INFINITY;
+    for (int s = 0; s < join.hi; ++s) top = fmaxf(top, a.part1[2 * (first + s * step)]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, acc[DP / 64];
+#pragma unroll
+    for (int j = 0; j < DP / 64; ++j) acc[j] = 0.0f;
+    for (int s = 0; s < join.hi; ++s) {
+        const int64_t at = first + s * step;
+        const float w = __builtin_amdgcn_exp2f(a.part1[2 * at] - ref);
+        sum = __builtin_fmaf(w, a.part1[2 * at + 1], sum);
+#pragma unroll
+        for (int j = 0; j < DP / 64; ++j) acc[j] = __builtin_fmaf(w, a.part0[at * DP + lane * (DP / 64) + j], acc[j]);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    char *dst = a.dst0 + row.token * a.o_token + row.head * a.o_head;
+#pragma unroll
+    for (int j = 0; j < DP / 64; ++j) {
+        const int d = lane * (DP / 64) + j;
+        if (d < a.head_dim) {
+            if constexpr (sizeof(T) == 2) reinterpret_cast<uint16_t *>(dst)[d] = bf16_bits(acc[j] * inv);
+            else reinterpret_cast<float *>(dst)[d] = acc[j] * inv;
+        }
+    }
+    if (lane == 0) a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+}
+
+// ------------------------------------------------------------------ dq (and delta)
+template <typename T>
+__device__ __forceinline__ float dot_chunk(const uint4 &x, const uint4 &y, float acc) {
+    const uint32_t p[4] = {x.x, x.y, x.z, x.w}, q[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 2) {
+            acc = __builtin_fmaf(__builtin_bit_cast(float, p[j] << 16), __builtin_bit_cast(float, q[j] << 16), acc);
+            acc = __builtin_fmaf(__builtin_bit_cast(float, p[j] & 0xffff0000u),
+                                 __builtin_bit_cast(float, q[j] & 0xffff0000u), acc);
+        } else {
+            acc = __builtin_fmaf(__builtin_bit_cast(float, p[j]), __builtin_bit_cast(float, q[j]), acc);
+        }
+    }
+    return acc;
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq(AttnParams a) {
+    constexpr int KT = kKeyTile<T>;
+    constexpr int kUnits = KT * Tile<T, DP>::kChunks;
+    __shared__ uint4 sk[2][kUnits], sv[2][kUnits];
+    const Item item = a.items[blockIdx.x / a.kv_heads];
+    const int kv_head = blockIdx.x % a.kv_heads;
+    const Record rec = a.records[item.record];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chunks = a.head_dim * (int)sizeof(T) / 16;
+
+    const RowOf row(a, rec, kv_head, (int64_t)item.begin + wave * kWaveCols + (lane & 31));
+    int least, most;
+    wave_limits(row, least, most);
+    uint4 qf[Tile<T, DP>::kFrags], gf[Tile<T, DP>::kFrags];
+    row_fragments<T, DP>(a.dout + row.token * a.do_token + row.head * a.do_head, gf, row.valid, chunks, lane);
+    row_fragments<T, DP>(a.out + row.token * a.o_token + row.head * a.o_head, qf, row.valid, chunks, lane);
+    float delta = 0.0f;
+#pragma unroll
+    for (int s = 0; s < Tile<T, DP>::kFrags; ++s) delta = dot_chunk<T>(gf[s], qf[s], delta);
+    delta += other_half(delta);
+    float lse = INFINITY;
+    if (row.valid) {
+        const int64_t at = row.token * a.heads + row.head;
+        lse = a.stats[at];
+        if (lane < 32) a.delta[at] = delta;
+    }
+    row_fragments<T, DP>(a.q + row.token * a.q_token + row.head * a.q_head, qf, row.valid, chunks, lane);
+
+    const char *k0 = a.k + rec.k_start * a.k_token + kv_head * a.k_head;
+    const char *v0 = a.v + rec.k_start * a.v_token + kv_head * a.v_head;
+    Stage<T, DP, KT> ks, vs;
+    auto load = [&](int key) {
+        const int left = (int)rec.k_len - key;
+        ks.load(k0 + key * a.k_token, chunks, [&](int r) { return r < left ? (uint32_t)(r * a.k_token) : kOOB; });
+        vs.load(v0 + key * a.v_token, chunks, [&](int r) { return r < left ? (uint32_t)(r * a.v_token) : kOOB; });
+    };
+
+    f32x16 o[DP / 32];
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) o[n] = splat(0.0f);
+    int buf = 0;
+    if (item.lo < item.hi) {
+        load(item.lo);
+        ks.store(sk[0]);
+        vs.store(sv[0]);
+    }
+    __syncthreads();
+    for (int key = item.lo; key < item.hi; key += KT) {
+        const bool more = key + KT < item.hi;
+        if (more) load(key + KT);
+        if (key < most) {
+            const bool masked = key + KT > least;
+            const int left = row.limit - key - 4 * (lane >> 5);
+#pragma unroll
+            for (int t = 0; t < KT / 32; ++t) {
+                f32x16 s = splat(0.0f), g = splat(-delta);
+                scores<T, DP>(s, sk[buf], 32 * t, qf, lane);
+                scores<T, DP>(g, sv[buf], 32 * t, gf, lane);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse)) * g[i];
+                if (masked)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = 32 * t + 8 * (i >> 2) + (i & 3) < left ? s[i] : 0.0f;
+                outer<T, DP>(o, sk[buf], 32 * t, s, lane);
+            }
+        }
+        if (more) {
+            ks.store(sk[buf ^ 1]);
+            vs.store(sv[buf ^ 1]);
+        }
+        __syncthreads();
+        buf ^= 1;
+    }
+    if (!row.valid) return;
+    char *dst = a.dst0 + row.token * a.d_token + (int64_t)row.head * a.head_dim * (int)sizeof(T);
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = 32 * n + 2 * i + 4 * (lane >> 5);
+            if (d < a.head_dim)
+                store4<T>(dst, d, o[n][i] * a.scale, o[n][i + 1] * a.scale, o[n][i + 2] * a.scale,
+                          o[n][i + 3] * a.scale);
+        }
+}
+
+// ------------------------------------------------------------------ dk, dv
+template <typename T>
+constexpr int kRowTile = sizeof(T) == 2 ? 64 : 32;
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads, 1) void attention_dkv(AttnParams a) {
+    constexpr int RT = kRowTile<T>;
+    constexpr int kUnits = RT * Tile<T, DP>::kChunks;
+    __shared__ uint4 sq[2][kUnits], sg[2][kUnits];
+    __shared__ float slse[2][RT], sdelta[2][RT];
+    const Item item = a.items[blockIdx.x / a.kv_heads];
+    const int kv_head = blockIdx.x % a.kv_heads;
+    const Record rec = a.records[item.record];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chunks = a.head_dim * (int)sizeof(T) / 16;
+
+    const int key0 = item.begin + wave * kWaveCols, key = key0 + (lane & 31);
+    const bool valid = key < rec.k_len;
+    const int64_t kv = rec.k_start + (valid ? key : 0);
+    uint4 kf[Tile<T, DP>::kFrags], vf[Tile<T, DP>::kFrags];
+    row_fragments<T, DP>(a.k + kv * a.k_token + kv_head * a.k_head, kf, valid, chunks, lane);
+    row_fragments<T, DP>(a.v + kv * a.v_token + kv_head * a.v_head, vf, valid, chunks, lane);
+
+    const int nrows = (int)(rec.q_len * a.group);
+    // Row r sees key j when r >= first(j); tokens before key j - (keys - queries) do not.
+    auto first = [&](int j) -> int64_t {
+        const int64_t t = a.causal ? j - (rec.k_len - rec.q_len) : 0;
+        return t < 0 ? 0 : t * a.group;
+    };
+    const int64_t mine = first(key), wave_first = first(key0), wave_last = first(key0 + kWaveCols - 1);
+
+    Stage<T, DP, RT> qs, gs;
+    float lse_r, delta_r;
+    auto load = [&](int r0) {
+        const uint32_t t0 = div_group(a, (uint32_t)r0);
+        const int64_t token = rec.q_start + t0;
+        auto at = [&](int row, int64_t by_token, int64_t by_head) -> uint32_t {
+            const uint32_t r = (uint32_t)(r0 + row);
+            if ((int)r >= nrows) return kOOB;
+            const uint32_t t = div_group(a, r);
+            return (uint32_t)((t - t0) * by_token + (r - t * (uint32_t)a.group) * by_head);
+        };
+        qs.load(a.q + token * a.q_token + (int64_t)kv_head * a.group * a.q_head, chunks,
+                [&](int row) { return at(row, a.q_token, a.q_head); });
+        gs.load(a.dout + token * a.do_token + (int64_t)kv_head * a.group * a.do_head, chunks,
+                [&](int row) { return at(row, a.do_token, a.do_head); });
+        if ((int)threadIdx.x < RT) {
+            const uint32_t r = (uint32_t)(r0 + (int)threadIdx.x);
+            lse_r = INFINITY;
+            delta_r = 0.0f;
+            if ((int)r < nrows) {
+                const uint32_t t = div_group(a, r);
+                const int64_t at = (rec.q_start + t) * a.heads + kv_head * a.group + (int)(r - t * (uint32_t)a.group);
+                lse_r = a.stats[at];
+                delta_r = a.delta[at];
+            }
+        }
+    };
+    auto store = [&](int buf) {
+        qs.store(sq[buf]);
+        gs.store(sg[buf]);
+        if ((int)threadIdx.x < RT) {
+            slse[buf][threadIdx.x] = lse_r;
+            sdelta[buf][threadIdx.x] = delta_r;
+        }
+    };
+
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) dk[n] = dv[n] = splat(0.0f);
+    int buf = 0;
+    if (item.lo < item.hi) {
+        load(item.lo);
+        store(0);
+    }
+    __syncthreads();
+    for (int r0 = item.lo; r0 < item.hi; r0 += RT) {
+        const bool more = r0 + RT < item.hi;
+        if (more) load(r0 + RT);
+        if (r0 + RT > wave_first) {
+            const bool masked = r0 < wave_last;
+#pragma unroll
+            for (int t = 0; t < RT / 32; ++t) {
+                f32x16 s = splat(0.0f), g, p;
+                float lse[16];
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const int at = 32 * t + 2 * i + 4 * (lane >> 5);
+                    const float4 l4 = *reinterpret_cast<const float4 *>(&slse[buf][at]);
+                    const float4 d4 = *reinterpret_cast<const float4 *>(&sdelta[buf][at]);
+                    lse[i] = l4.x; lse[i + 1] = l4.y; lse[i + 2] = l4.z; lse[i + 3] = l4.w;
+                    g[i] = -d4.x; g[i + 1] = -d4.y; g[i + 2] = -d4.z; g[i + 3] = -d4.w;
+                }
+                scores<T, DP>(s, sq[buf], 32 * t, kf, lane);
+                scores<T, DP>(g, sg[buf], 32 * t, vf, lane);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse[i]));
+                    s[i] = p[i] * g[i];
+                }
+                if (masked) {
+                    const int64_t hidden = mine - r0 - 4 * (lane >> 5);   // rows below it do not see the key
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const bool seen = 32 * t + 8 * (i >> 2) + (i & 3) >= hidden;
+                        p[i] = seen ? p[i] : 0.0f;
+                        s[i] = seen ? s[i] : 0.0f;
+                    }
+                }
+                outer<T, DP>(dv, sg[buf], 32 * t, p, lane);
+                outer<T, DP>(dk, sq[buf], 32 * t, s, lane);
+            }
+        }
+        if (more) store(buf ^ 1);
+        __syncthreads();
+        buf ^= 1;
+    }
+    const int d0 = 4 * (lane >> 5);
+    if (item.slot < 0) {
+        if (!valid) return;
+        const int64_t off = kv * a.d_token + (int64_t)kv_head * a.head_dim * (int)sizeof(T);
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int d = 32 * n + 2 * i + d0;
+                if (d < a.head_dim) {
+                    store4<T>(a.dst0 + off, d, dk[n][i] * a.scale, dk[n][i + 1] * a.scale, dk[n][i + 2] * a.scale,
+                              dk[n][i + 3] * a.scale);
+                    store4<T>(a.dst1 + off, d, dv[n][i], dv[n][i + 1], dv[n][i + 2], dv[n][i + 3]);
+                }
+            }
+    } else {
+        const int64_t at = (((int64_t)item.slot * a.kv_heads + kv_head) * kTile + wave * kWaveCols + (lane & 31)) * DP;
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                *reinterpret_cast<float4 *>(a.part0 + at + 32 * n + 2 * i + d0) =
+                    make_float4(dk[n][i], dk[n][i + 1], dk[n][i + 2], dk[n][i + 3]);
+                *reinterpret_cast<float4 *>(a.part1 + at + 32 * n + 2 * i + d0) =
+                    make_float4(dv[n][i], dv[n][i + 1], dv[n][i + 2], dv[n][i + 3]);
+            }
+    }
+}
+
+// Sums the row ranges of split key tiles in order: one thread per four elements of a key.
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void attention_dkv_join(AttnParams a, const Item *joins) {
+    constexpr int kPer = kThreads * 4 / DP;   // keys per workgroup
+    const int blocks = kTile / kPer * a.kv_heads;
+    const Item join = joins[blockIdx.x / blocks];
+    const int rest = blockIdx.x % blocks, kv_head = rest % a.kv_heads;
+    const int j = rest / a.kv_heads * kPer + threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
+    const Record rec = a.records[join.record];
+    const int64_t key = (int64_t)join.begin + j;
+    if (key >= rec.k_len || d >= a.head_dim) return;
+    const int64_t step = (int64_t)a.kv_heads * kTile * DP;
+    int64_t at = (((int64_t)join.lo * a.kv_heads + kv_head) * kTile + j) * DP + d;
+    float4 dk = make_float4(0, 0, 0, 0), dv = dk;
+    for (int s = 0; s < join.hi; ++s, at += step) {
+        const float4 x = *reinterpret_cast<const float4 *>(a.part0 + at), y = *reinterpret_cast<const float4 *>(a.part1 + at);
+        dk.x += x.x; dk.y += x.y; dk.z += x.z; dk.w += x.w;
+        dv.x += y.x; dv.y += y.y; dv.z += y.z; dv.w += y.w;
+    }
+    const int64_t off = (rec.k_start + key) * a.d_token + (int64_t)kv_head * a.head_dim * (int)sizeof(T);
+    store4<T>(a.dst0 + off, d, dk.x * a.scale, dk.y * a.scale, dk.z * a.scale, dk.w * a.scale);
+    store4<T>(a.dst1 + off, d, dv.x, dv.y, dv.z, dv.w);
+}
+
+// ------------------------------------------------------------------ host side
+constexpr int64_t kMaxRows = 0x7fffffff - 2 * kTile;
+
+constexpr int64_t kMaxPitch = (int64_t)1 << 24;   // bytes between tokens of k and v
+
+// 64 packed rows span at most 64 / group + 2 tokens and all heads of the group.
+bool row_span_ok(int64_t token, int64_t head, int64_t group) {
+    return (64 / group + 2) * (double)token + (double)group * (double)head < 2147483647.0 - 1024;
+}
+
+int padded_dim(int64_t head_dim) { return head_dim <= 64 ? 64 : 128; }
+
+bool dims_ok(int64_t heads, int64_t kv_heads, int64_t head_dim) {
+    return heads > 0 && kv_heads > 0 && heads <= 65536 && heads % kv_heads == 0 && head_dim >= 8 && head_dim <= 128 &&
+           head_dim % 8 == 0;
+}
+
+int fill_params(const ct_attention *c, AttnParams &a) {
+    if (!c) return -CT_EINVAL_POINTER;
+    if (c->dtype != CT_BF16 && c->dtype != CT_F32) return -CT_EINVAL_DTYPE;
+    if (!dims_ok(c->heads, c->kv_heads, c->head_dim) || !(c->scale > 0.0f) || !(c->scale < INFINITY))
+        return -CT_EINVAL_SHAPE;
+    if (!c->q || !c->k || !c->v || !c->records) return -CT_EINVAL_POINTER;
+    const int64_t size = c->dtype == CT_BF16 ? 2 : 4;
+    const int64_t strides[6] = {c->q_token, c->q_head, c->k_token, c->k_head, c->v_token, c->v_head};
+    for (int64_t s : strides)
+        if (s < 0 || s * size % 16 || s > (int64_t)1 << 40) return -CT_EINVAL_SHAPE;
+    if (((uintptr_t)c->q | (uintptr_t)c->k | (uintptr_t)c->v) % 16) return -CT_EINVAL_POINTER;
+    a = AttnParams{};
+    a.q = (const char *)c->q;
+    a.k = (const char *)c->k;
+    a.v = (const char *)c->v;
+    a.q_token = c->q_token * size;
+    a.q_head = c->q_head * size;
+    a.k_token = c->k_token * size;
+    a.k_head = c->k_head * size;
+    a.v_token = c->v_token * size;
+    a.v_head = c->v_head * size;
+    a.o_head = c->head_dim * size;
+    a.o_token = c->heads * a.o_head;
+    a.records = (const Record *)c->records;
+    a.heads = c->heads;
+    a.kv_heads = c->kv_heads;
+    a.group = c->heads / c->kv_heads;
+    a.head_dim = c->head_dim;
+    a.causal = c->causal ? 1 : 0;
+    a.scale = c->scale;
+    a.scale2 = c->scale * kLog2e;
+    // r / group for r < 2^31: with 2^s >= group and M = floor(2^(31+s) / group) + 1,
+    // r M / 2^(31+s) exceeds r / group by less than 1 / group.
+    int s = 0;
+    while ((1 << s) < a.group) ++s;
+    a.magic = (uint32_t)(((uint64_t)1 << (31 + s)) / (uint64_t)a.group + 1);
+    a.shift = 31 + s;
+    // 32-bit offsets inside a tile: 64 rows of keys, and the tokens and heads of 64 packed rows.
+    if (a.k_token > kMaxPitch || a.v_token > kMaxPitch) return -CT_EINVAL_SHAPE;
+    if (!row_span_ok(a.q_token, a.q_head, a.group)) return -CT_EINVAL_SHAPE;
+    return 0;
+}
+
+int status_of_last_launch() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : (int)e;
+}
+
+template <typename F>
+int by_type(int dtype, int dp, F f) {
+    if (dtype == CT_BF16) return dp == 64 ? f((uint16_t)0, std::integral_constant<int, 64>()) : f((uint16_t)0, std::integral_constant<int, 128>());
+    return dp == 64 ? f(0.0f, std::integral_constant<int, 64>()) : f(0.0f, std::integral_constant<int, 128>());
+}
+
+int64_t parts_per_item(int32_t pass, int dp) {   // floats
+    return pass == CT_ATTENTION_KEYS ? 2 * (int64_t)kTile * dp : (int64_t)kTile * (dp + 2);
+}
+
+// Workgroups that keep the card busy: two per CU in the forward, one (of twice the
+// registers) in the dk, dv kernel, and some more, since the ranges end at different times.
+constexpr int64_t kForwardGroups = 512, kKeyGroups = 512;
+
+void plan_items(int32_t pass, const Record *rec, int64_t n, int64_t kv_heads, int64_t group, bool causal,
+                std::vector<Item> &items, std::vector<Item> &joins, int64_t &slots) {
+    const bool keys = pass == CT_ATTENTION_KEYS;
+    constexpr int64_t kUnit = 64;   // ranges are cut at multiples of a tile
+    int64_t work = 0;
+    for (int64_t i = 0; i < n; ++i) {
+        const int64_t rows = rec[i].q_len * group, span = keys ? rec[i].k_len : rows;
+        for (int64_t b = 0; b < span; b += kTile) {
+            Item it = {};
+            it.record = (int32_t)i;
+            it.begin = (int32_t)b;
+            it.slot = -1;
+            const int64_t shift = rec[i].k_len - rec[i].q_len;
+            if (keys) {   // rows that see the tile's first key, from a whole tile of rows on
+                const int64_t t = causal ? std::max<int64_t>(0, b - shift) : 0;
+                it.lo = (int32_t)std::min(t * group / kUnit * kUnit, rows);
+                it.hi = (int32_t)rows;
+            } else {      // keys that the tile's last row sees
+                const int64_t t = (std::min(rows, b + kTile) - 1) / group;
+                it.hi = (int32_t)(causal ? std::min(rec[i].k_len, std::max<int64_t>(0, t + 1 + shift)) : rec[i].k_len);
+            }
+            work += cdiv(it.hi - it.lo, kUnit);
+            items.push_back(it);
+        }
+    }
+    slots = 0;
+    if (pass != CT_ATTENTION_ROWS) {
+        const int64_t target = std::max<int64_t>(1, (keys ? kKeyGroups : kForwardGroups) / kv_heads);
+        const int64_t range = std::max<int64_t>(keys ? 4 : 2, cdiv(work, target)) * kUnit;
+        const bool enough = !keys && (int64_t)items.size() >= target;
+        std::vector<Item> whole;
+        whole.swap(items);
+        for (const Item &it : whole) {
+            const int64_t parts = enough ? 1 : std::max<int64_t>(1, cdiv(it.hi - it.lo, range));
+            if (parts == 1) {
+                items.push_back(it);
+                continue;
+            }
+            const int64_t step = cdiv(cdiv(it.hi - it.lo, parts), kUnit) * kUnit;
+            Item join = it;
+            join.lo = (int32_t)slots;
+            for (int64_t lo = it.lo; lo < it.hi; lo += step) {
+                Item part = it;
+                part.lo = (int32_t)lo;
+                part.hi = (int32_t)std::min<int64_t>(it.hi, lo + step);
+                part.slot = (int32_t)slots++;
+                items.push_back(part);
+            }
+            join.hi = (int32_t)(slots - join.lo);
+            joins.push_back(join);
+        }
+    }
+    // Longest first: what starts last then ends soon.
+    std::stable_sort(items.begin(), items.end(),
+                     [](const Item &x, const Item &y) { return x.hi - x.lo > y.hi - y.lo; });
+}
+
+bool items_ok(int64_t items, int64_t joins, int64_t slots, int64_t kv_heads) {
+    const int64_t most = 0x7fffffff / (kTile * kv_heads);
+    return items >= 0 && joins >= 0 && slots >= 0 && items <= most && joins <= most && slots <= most;
+}
+
+}  // namespace
+}  // namespace ct
+
+using namespace ct;
+
+extern "C" int ct_attention_plan(int32_t pass, const int64_t *records, int64_t n_records, int32_t heads,
+                                 int32_t kv_heads, int32_t head_dim, int32_t causal, int32_t *entries,
+                                 int64_t capacity, int64_t *counts) {
+    if (pass < CT_ATTENTION_FORWARD || pass > CT_ATTENTION_KEYS || n_records < 0 || n_records > 0x7fffffff ||
+        !dims_ok(heads, kv_heads, head_dim))
+        return -CT_EINVAL_SHAPE;
+    if (!counts || (n_records && !records)) return -CT_EINVAL_POINTER;
+    const int64_t group = heads / kv_heads;
+    const Record *rec = reinterpret_cast<const Record *>(records);
+    int64_t tiles = 0;
+    for (int64_t i = 0; i < n_records; ++i) {
+        const Record &r = rec[i];
+        if (r.q_start < 0 || r.q_len < 0 || r.k_start < 0 || r.k_len < 0 || r.k_len > kMaxRows ||
+            r.q_len > kMaxRows / group)
+            return -CT_EINVAL_SHAPE;
+        tiles += cdiv(r.q_len * group, kTile) + cdiv(r.k_len, kTile);
+    }
+    if (tiles > 0x7fffffff / (4 * kTile * kv_heads)) return -CT_EINVAL_SHAPE;
+    try {
+        std::vector<Item> items, joins;
+        int64_t slots = 0;
+        plan_items(pass, rec, n_records, kv_heads, group, causal != 0, items, joins, slots);
+        counts[0] = (int64_t)items.size();
+        counts[1] = (int64_t)joins.size();
+        counts[2] = slots;
+        if (!items_ok(counts[0], counts[1], counts[2], kv_heads)) return -CT_EINVAL_SHAPE;
+        if (!entries) return 0;
+        if (capacity < counts[0] + counts[1]) return -CT_EINVAL_WORKSPACE;
+        std::copy(items.begin(), items.end(), reinterpret_cast<Item *>(entries));
+        std::copy(joins.begin(), joins.end(), reinterpret_cast<Item *>(entries) + items.size());
+    } catch (...) {
+        return (int)hipErrorOutOfMemory;
+    }
+    return 0;
+}
+
+extern "C" int64_t ct_attention_workspace(int32_t pass, int64_t slots, int32_t kv_heads, int32_t head_dim) {
+    if (slots <= 0 || kv_heads <= 0 || head_dim <= 0 || head_dim > 128) return 0;
+    return slots * kv_heads * parts_per_item(pass, padded_dim(head_dim)) * (int64_t)sizeof(float);
+}
+
+extern "C" int ct_attention_forward(const ct_attention *c, const int32_t *plan, const int64_t *counts, void *out,
+                                    float *stats, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
+    AttnParams a;
+    if (const int status = fill_params(c, a)) return status;
+    if (!counts) return -CT_EINVAL_POINTER;
+    const int64_t n = counts[0], joins = counts[1], slots = counts[2];
+    if (!items_ok(n, joins, slots, c->kv_heads)) return -CT_EINVAL_SHAPE;
+    if (n == 0) return 0;
+    if (!plan || !out || !stats || (uintptr_t)plan % 16 || (uintptr_t)out % 16) return -CT_EINVAL_POINTER;
+    if (slots && (!workspace || (uintptr_t)workspace % 16 ||
+                  workspace_bytes < ct_attention_workspace(CT_ATTENTION_FORWARD, slots, c->kv_heads, c->head_dim)))
+        return -CT_EINVAL_WORKSPACE;
+    const int dp = padded_dim(c->head_dim);
+    a.items = reinterpret_cast<const Item *>(plan);
+    a.dst0 = (char *)out;
+    a.stats = stats;
+    a.part0 = (float *)workspace;
+    a.part1 = a.part0 + slots * c->kv_heads * kTile * dp;
+    return by_type(c->dtype, dp, [&](auto type, auto dim) {
+        typedef decltype(type) T;
+        constexpr int DP = decltype(dim)::value;
+        attention_forward<T, DP><<<dim3((unsigned)(n * c->kv_heads)), dim3(kThreads), 0, stream>>>(a);
+        if (const int status = status_of_last_launch()) return status;
+        if (joins) {
+            attention_join<T, DP><<<dim3((unsigned)(joins * c->kv_heads * (kTile / 4))), dim3(kThreads), 0, stream>>>(
+                a, a.items + n);
+            return status_of_last_launch();
+        }
+        return 0;
+    });
+}
+
+extern "C" int ct_attention_backward(const ct_attention *c, const int32_t *row_plan, const int64_t *row_counts,
+                                     const int32_t *key_plan, const int64_t *key_counts, const void *out,
+                                     const float *stats, const void *dout, int64_t dout_token, int64_t dout_head,
+                                     float *delta, void *dq, void *dk, void *dv, void *workspace,
+                                     int64_t workspace_bytes, hipStream_t stream) {
+    AttnParams a;
+    if (const int status = fill_params(c, a)) return status;
+    if (!row_counts || !key_counts) return -CT_EINVAL_POINTER;
+    const int64_t rows = row_counts[0], keys = key_counts[0], joins = key_counts[1], slots = key_counts[2];
+    if (!items_ok(rows, row_counts[1], row_counts[2], c->kv_heads) || !items_ok(keys, joins, slots, c->kv_heads) ||
+        row_counts[1] || row_counts[2])
+        return -CT_EINVAL_SHAPE;
+    const int64_t size = c->dtype == CT_BF16 ? 2 : 4;
+    if (rows) {
+        if (!row_plan || !out || !stats || !dout || !delta || !dq ||
+            ((uintptr_t)row_plan | (uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq) % 16)
+            return -CT_EINVAL_POINTER;
+        if (dout_token < 0 || dout_head < 0 || dout_token * size % 16 || dout_head * size % 16 ||
+            dout_token > (int64_t)1 << 40 || dout_head > (int64_t)1 << 40)
+            return -CT_EINVAL_SHAPE;
+        if (!row_span_ok(dout_token * size, dout_head * size, a.group)) return -CT_EINVAL_SHAPE;
+    }
+    if (keys && (!key_plan || !dk || !dv || ((uintptr_t)key_plan | (uintptr_t)dk | (uintptr_t)dv) % 16))
+        return -CT_EINVAL_POINTER;
+    if (slots && (!workspace || (uintptr_t)workspace % 16 ||
+                  workspace_bytes < ct_attention_workspace(CT_ATTENTION_KEYS, slots, c->kv_heads, c->head_dim)))
+        return -CT_EINVAL_WORKSPACE;
+    const int dp = padded_dim(c->head_dim);
+    a.out = (const char *)out;
+    a.dout = (const char *)dout;
+    a.do_token = dout_token * size;
+    a.do_head = dout_head * size;
+    a.stats = const_cast<float *>(stats);
+    a.delta = delta;
+    return by_type(c->dtype, dp, [&](auto type, auto dim) {
+        typedef decltype(type) T;
+        constexpr int DP = decltype(dim)::value;
+        if (rows) {   // dq first: it leaves delta for the other kernel
+            AttnParams r = a;
+            r.items = reinterpret_cast<const Item *>(row_plan);
+            r.dst0 = (char *)dq;
+            r.d_token = a.o_token;
+            attention_dq<T, DP><<<dim3((unsigned)(rows * c->kv_heads)), dim3(kThreads), 0, stream>>>(r);
+            if (const int status = status_of_last_launch()) return status;
+        }
+        if (!keys) return 0;
+        AttnParams r = a;
+        r.items = reinterpret_cast<const Item *>(key_plan);
+        r.dst0 = (char *)dk;
+        r.dst1 = (char *)dv;
+        r.d_token = c->kv_heads * a.o_head;
+        r.part0 = (float *)workspace;
+        r.part1 = r.part0 + slots * c->kv_heads * kTile * DP;
+        attention_dkv<T, DP><<<dim3((unsigned)(keys * c->kv_heads)), dim3(kThreads), 0, stream>>>(r);
+        if (const int status = status_of_last_launch()) return status;
+        if (!joins) return 0;
+        attention_dkv_join<T, DP><<<dim3((unsigned)(joins * c->kv_heads * (kTile * DP / (4 * kThreads)))),
+                                    dim3(kThreads), 0, stream>>>(r, r.items + keys);
+        return status_of_last_launch();
+    });
+}

@@ -518,6 +518,71 @@ int ct_rope(const void *x, void *y, const void *cosine, const void *sine, int64_
             int32_t dtype, int32_t trig_dtype, hipStream_t stream);
 
 /*
+ * Attention over packed records (in the place of the reference's kernels/attention.py:58-93,
+ * which calls a library): per record and head, softmax(scale q k^T) v over the keys a query
+ * sees, all of the record's or, when `causal`, those up to its own position, the queries being
+ * the last of the keys (query i of L_q sees key j of L_k when j <= i + L_k - L_q). A query that
+ * sees no key gives zeros and takes no part in the gradients.
+ * q [tokens, heads, head_dim], k and v [key tokens, kv_heads, head_dim] of `dtype` (CT_BF16 or
+ * CT_F32); `*_token` and `*_head` are element strides, each 16 bytes' multiple, elements of a
+ * head contiguous, pointers 16-byte aligned; heads a multiple of kv_heads (query head h reads
+ * key/value head h / (heads / kv_heads)); head_dim a multiple of 8 up to 128; 0 < scale < inf.
+ * The bytes between two tokens of k and v are at most 2^24; 64 / group + 2 tokens and `group`
+ * heads of q (and of dout), group = heads / kv_heads, span less than 2^31 bytes.
+ * `records` int64 [n][4] on the device: first query, queries, first key, keys. Records must not
+ * share queries; for the backward they must not share keys.
+ */
+typedef struct ct_attention {
+    const void *q;
+    const void *k;
+    const void *v;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+    const int64_t *records;
+    int32_t heads;
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t dtype;
+    int32_t causal;
+    float scale;
+} ct_attention;
+
+#define CT_ATTENTION_FORWARD 0  /* ct_attention_forward */
+#define CT_ATTENTION_ROWS    1  /* dq of ct_attention_backward */
+#define CT_ATTENTION_KEYS    2  /* dk and dv of ct_attention_backward */
+
+/*
+ * The work of one pass over `records` (host copy of the table above), cut into workgroups'
+ * shares: 32-byte entries, counts[0] shares and then counts[1] joins, over counts[2] partial
+ * results. With entries = null only counts is written; capacity counts entries. A plan holds
+ * for every call with these records, heads, head_dim and causal; the caller copies its entries
+ * to the device (16-byte aligned) and hands them and counts to the calls.
+ */
+int ct_attention_plan(int32_t pass, const int64_t *records, int64_t n_records, int32_t heads, int32_t kv_heads,
+                      int32_t head_dim, int32_t causal, int32_t *entries, int64_t capacity, int64_t *counts);
+/* Bytes of workspace that a plan with counts[2] = slots needs (CT_ATTENTION_FORWARD or _KEYS). */
+int64_t ct_attention_workspace(int32_t pass, int64_t slots, int32_t kv_heads, int32_t head_dim);
+
+/*
+ * out [tokens, heads, head_dim] contiguous; stats float32 [tokens, heads] for the backward:
+ * log2 of the softmax's denominator with its maximum (+inf for a query that sees no key).
+ * Rows of no record are left as they are.
+ */
+int ct_attention_forward(const ct_attention *attention, const int32_t *plan, const int64_t *counts, void *out,
+                         float *stats, void *workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/*
+ * dq [tokens, heads, head_dim], dk and dv [key tokens, kv_heads, head_dim], contiguous, from
+ * dout (strides as for q), the forward's out and stats; delta float32 [tokens, heads] is
+ * scratch. The probabilities are recomputed; sums run in a fixed order, so repeated calls are
+ * bit-identical. Rows of no record are left as they are. row_plan and key_plan are the plans
+ * of CT_ATTENTION_ROWS and CT_ATTENTION_KEYS.
+ */
+int ct_attention_backward(const ct_attention *attention, const int32_t *row_plan, const int64_t *row_counts,
+                          const int32_t *key_plan, const int64_t *key_counts, const void *out, const float *stats,
+                          const void *dout, int64_t dout_token, int64_t dout_head, float *delta, void *dq, void *dk,
+                          void *dv, void *workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/*
  * Kernel timing for benchmarks; no counterpart in the reference (which publishes no kernel
  * timings). ct_profile_begin enables the families in `families` and creates `capacity`
  * HIP event pairs; each later launch of an enabled family is bracketed by one pair
