@@ -68,6 +68,25 @@ class Attention(ctypes.Structure):
 
 _ATT = ctypes.POINTER(Attention)
 
+
+class MuonMatrix(ctypes.Structure):
+    """Mirror of `ct_muon_matrix`: one matrix of an orthogonalising call."""
+
+    _fields_ = [
+        ("param", _P), ("grad", _P), ("momentum", _P), ("rows", _I64), ("cols", _I64), ("scratch", _I64),
+        ("parts", _I64), ("adjust", ctypes.c_float), ("splits", _I32),
+    ]
+
+
+class MuonOptions(ctypes.Structure):
+    """Mirror of `ct_muon_options`."""
+
+    _fields_ = [(name, ctypes.c_double) for name in ("lr", "weight_decay", "momentum", "a", "b", "c", "eps")] + [
+        ("nesterov", _I32), ("steps", _I32), ("update", _I32)]
+
+
+_MUON = ctypes.POINTER(MuonMatrix)
+
 _SIGNATURES = {
     "ct_abi_version": (ctypes.c_int, []),
     "ct_init_device": (ctypes.c_int, []),
@@ -117,6 +136,8 @@ _SIGNATURES = {
     "ct_attention_forward": (ctypes.c_int, [_ATT, _P, _P, _P, _P, _P, _I64, _P]),
     "ct_attention_backward": (ctypes.c_int, [_ATT, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _I64,
                                              _P]),
+    "ct_muon_plan": (ctypes.c_int, [_MUON, _I64, _P, _I64, _P, _P]),
+    "ct_muon": (ctypes.c_int, [_MUON, _I64, _P, _P, _I32, ctypes.POINTER(MuonOptions), _P, _I64, _I64, _P]),
     "ct_profile_begin": (ctypes.c_int, [_I32, _I32]),
     "ct_profile_read": (ctypes.c_int, [_I32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_I64),
                                        ctypes.POINTER(ctypes.c_double)]),

@@ -11,7 +11,17 @@ and every tensor is updated from a device-side table of (param, grad, exp_avg,
 exp_avg_sq, step, numel) rows and a list of fixed-size chunks. Parameters must live on
 the HIP device in fp32 or bf16 with dense gradients of the same dtype; amsgrad is not
 supported (the reference does not use it).
+
+Beside it stands an optimizer for parameters that are all matrices, as LoRA adapters are:
+`FusedMuon` takes torch.optim.Muon's arguments and keeps its state key (`momentum_buffer`; in
+float32 whatever the parameter's type), and `orthogonalize` is its iteration alone. Both run
+ct_muon: the Newton-Schulz steps in double on the short side's Gram matrix, all matrices of one
+type in one set of launches, results rounded once (torch's runs the steps in bfloat16).
 """
+
+import ctypes
+import functools
+import math
 
 import torch
 
@@ -104,4 +114,194 @@ class FusedAdamW(torch.optim.Optimizer):
                         float(group["eps"]), float(group["weight_decay"]), int(bool(group["maximize"])), 1,
                         _native.stream_of(members[0][0]))
                 _native.check(status, "ct_adamw_step")
+        return loss
+
+
+class _MuonPlan:
+    """The shares of work of one list of shapes on one device: kept between steps."""
+
+    def __init__(self, shapes, device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("orthogonalize/FusedMuon: the first call with a list of shapes makes its plan and cannot "
+                               "be captured; run it once before the capture")
+        lib = _native.library()
+        table = (_native.MuonMatrix * len(shapes))()
+        for row, (rows, cols, adjust) in zip(table, shapes):
+            row.rows, row.cols, row.adjust = rows, cols, adjust
+        self.counts, needed = (ctypes.c_int64 * 3)(), ctypes.c_int64()
+        _native.check(lib.ct_muon_plan(table, len(shapes), None, 0, self.counts, ctypes.byref(needed)), "ct_muon_plan")
+        size = sum(self.counts)
+        entries = torch.empty(size, 8, dtype=torch.int32)
+        _native.check(lib.ct_muon_plan(table, len(shapes), entries.data_ptr(), size, self.counts, ctypes.byref(needed)),
+                      "ct_muon_plan")
+        # A copy that the host waits for: complete for every stream.
+        with torch.cuda.device(device):
+            self.entries = entries.to(device)
+            self.stream = _native.stream_of(self.entries)
+        self.table, self.workspace = bytes(table), needed.value
+
+    def run(self, pointers, dtype, options):
+        """One call over `pointers`, a list of (param, grad, momentum) addresses in the shapes' order."""
+        device, stream = self.entries.device, _native.stream_of(self.entries)
+        table = (_native.MuonMatrix * len(pointers)).from_buffer_copy(self.table)
+        for row, (param, grad, momentum) in zip(table, pointers):
+            row.param, row.grad, row.momentum = param, grad, momentum
+        if stream != self.stream and not torch.cuda.is_current_stream_capturing():
+            self.entries.record_stream(torch.cuda.current_stream(device))
+        workspace = torch.empty(self.workspace, dtype=torch.uint8, device=device)
+        with _native.device_of(self.entries):
+            status = _native.library().ct_muon(
+                table, len(pointers), self.entries.data_ptr(), self.counts, _native.dtype_code(dtype),
+                ctypes.byref(options), workspace.data_ptr(), self.workspace, self.workspace, stream)
+        _native.check(status, "ct_muon")
+
+
+@functools.lru_cache(maxsize=64)
+def _muon_plan(shapes, device):
+    return _MuonPlan(shapes, device)
+
+
+def _muon_numbers(coefficients, steps, eps):
+    """Checked (a, b, c), steps and eps of the iteration."""
+    a, b, c = (float(x) for x in coefficients)
+    if not all(math.isfinite(x) for x in (a, b, c)):
+        raise ValueError(f"Invalid Newton-Schulz coefficients: {coefficients}")
+    if not 1 <= int(steps) <= 100 or int(steps) != steps:
+        raise ValueError(f"Invalid number of Newton-Schulz steps: {steps}")
+    if not float(eps) >= 0.0:
+        raise ValueError(f"Invalid epsilon value: {eps}")
+    return (a, b, c), int(steps), float(eps)
+
+
+def _newton_schulz(matrix, coefficients, steps, eps):
+    """The iteration in torch operations, in double: host tensors."""
+    a, b, c = coefficients
+    x = matrix.double()
+    x = x.T if x.shape[0] > x.shape[1] else x
+    x = x / x.norm().clamp(min=eps)
+    for _ in range(steps):
+        gram = x @ x.T
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return (x.T if matrix.shape[0] > matrix.shape[1] else x).to(matrix.dtype).contiguous()
+
+
+@torch.no_grad()
+def orthogonalize(matrices, *, coefficients=(3.4445, -4.7750, 2.0315), steps=5, eps=1e-7):
+    """Matrices with their singular values driven towards one by Newton-Schulz steps:
+    X = M / max(|M|, eps), then `steps` times X = a X + (b A + c A^2) X with A = X X^T (of the
+    transposed matrix where it has more rows than columns).
+
+    `matrices` is a 2-D tensor or a list of them, float32 or bfloat16 on the device (any
+    shapes and strides, types and devices mixed); returns new contiguous tensors of the same
+    shapes and types, one or a list. Empty matrices come back empty, zero ones zero."""
+    coefficients, steps, eps = _muon_numbers(coefficients, steps, eps)
+    single = isinstance(matrices, torch.Tensor)
+    inputs = [matrices] if single else list(matrices)
+    buckets, results = {}, []
+    for index, m in enumerate(inputs):
+        if m.dim() != 2:
+            raise ValueError(f"orthogonalize: a tensor of shape {tuple(m.shape)} is not a matrix")
+        if m.is_cuda and m.dtype not in (torch.float32, torch.bfloat16):
+            raise NotImplementedError("orthogonalize: the HIP kernels take float32 or bfloat16")
+        if not m.is_floating_point():
+            raise ValueError("orthogonalize: matrices of a floating type required")
+        if not m.is_cuda:
+            results.append(_newton_schulz(m, coefficients, steps, eps) if m.numel() else m.clone())
+            continue
+        results.append(torch.empty(m.shape, dtype=m.dtype, device=m.device))
+        if m.numel():
+            buckets.setdefault((m.device, m.dtype), []).append(index)
+    options = _native.MuonOptions(a=coefficients[0], b=coefficients[1], c=coefficients[2], eps=eps, steps=steps)
+    for (device, dtype), members in buckets.items():
+        sources = [inputs[i].contiguous() for i in members]
+        plan = _muon_plan(tuple((m.shape[0], m.shape[1], 1.0) for m in sources), device)
+        plan.run([(results[i].data_ptr(), m.data_ptr(), None) for i, m in zip(members, sources)], dtype, options)
+    return results[0] if single else results
+
+
+def _adjusted(adjust_lr_fn, rows, cols):
+    """Factor on the learning rate of a [rows, cols] matrix."""
+    if adjust_lr_fn == "match_rms_adamw":
+        return 0.2 * math.sqrt(max(rows, cols))
+    return math.sqrt(max(1.0, rows / cols))
+
+
+class FusedMuon(torch.optim.Optimizer):
+    """Muon over matrices on the device; torch.optim.Muon's arguments.
+
+    Each step: momentum = mu momentum + (1 - mu) grad, M = mu momentum + (1 - mu) grad (nesterov)
+    or momentum, param = param (1 - lr weight_decay) - lr adjust orthogonalize(M), with adjust =
+    sqrt(max(1, rows / cols)) ("original", the default) or 0.2 sqrt(max(rows, cols))
+    ("match_rms_adamw")."""
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
+                 ns_coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, ns_steps=5, adjust_lr_fn=None):
+        if not 0.0 <= float(lr):
+            raise ValueError(f"Invalid learning rate: {lr}")
+        if not 0.0 <= momentum <= 1.0:
+            raise ValueError(f"Invalid momentum value: {momentum}")
+        if not 0.0 <= weight_decay:
+            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
+        if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
+            raise ValueError(f"Invalid learning rate adjustment: {adjust_lr_fn}")
+        _muon_numbers(ns_coefficients, ns_steps, eps)
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
+                                      ns_coefficients=ns_coefficients, eps=eps, ns_steps=ns_steps,
+                                      adjust_lr_fn=adjust_lr_fn))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2:
+                raise ValueError(f"FusedMuon takes matrices only, not a parameter of shape {tuple(p.shape)}")
+
+    def load_state_dict(self, state_dict):
+        """Loads a state dict (this class's or torch.optim.Muon's); the buffers stay float32,
+        which the base class would round to a bfloat16 parameter's type."""
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        for group, given in zip(self.param_groups, state_dict["param_groups"]):
+            for p, key in zip(group["params"], given["params"]):
+                if "momentum_buffer" in saved.get(key, ()):
+                    self.state[p]["momentum_buffer"] = saved[key]["momentum_buffer"].to(
+                        device=p.device, dtype=torch.float32, copy=True).contiguous()
+
+    def _buffer_of(self, p):
+        state = self.state[p]
+        if "momentum_buffer" not in state:
+            state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        buffer = state["momentum_buffer"]
+        if (buffer.dtype != torch.float32 or buffer.shape != p.shape or buffer.device != p.device
+                or not buffer.is_contiguous()):
+            raise RuntimeError("FusedMuon: momentum_buffer must be a contiguous float32 tensor of the parameter's shape")
+        return buffer
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            coefficients, steps, eps = _muon_numbers(group["ns_coefficients"], group["ns_steps"], group["eps"])
+            buckets = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("FusedMuon does not support sparse gradients")
+                if not p.is_cuda or p.dtype not in (torch.float32, torch.bfloat16):
+                    raise NotImplementedError("FusedMuon: parameters must be fp32 or bf16 device tensors")
+                if p.grad.dtype != p.dtype or not p.is_contiguous() or not p.grad.is_contiguous():
+                    raise NotImplementedError("FusedMuon: contiguous gradients of the parameter's dtype required")
+                if p.numel():
+                    buckets.setdefault((p.device, p.dtype), []).append((p, self._buffer_of(p)))
+            options = _native.MuonOptions(
+                lr=float(group["lr"]), weight_decay=float(group["weight_decay"]), momentum=float(group["momentum"]),
+                a=coefficients[0], b=coefficients[1], c=coefficients[2], eps=eps,
+                nesterov=int(bool(group["nesterov"])), steps=steps, update=1)
+            for (device, dtype), members in buckets.items():
+                plan = _muon_plan(tuple((*p.shape, _adjusted(group["adjust_lr_fn"], *p.shape)) for p, _ in members),
+                                  device)
+                plan.run([(p.data_ptr(), p.grad.data_ptr(), m.data_ptr()) for p, m in members], dtype, options)
         return loss

@@ -583,6 +583,51 @@ int ct_attention_backward(const ct_attention *attention, const int32_t *row_plan
                           void *dv, void *workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /*
+ * Orthogonalising matrices by Newton-Schulz products, and the Muon step around it (no
+ * counterpart in the reference, whose optimizer is AdamW; the arguments are those of
+ * torch.optim.Muon). Each matrix M, taken with its short side first:
+ *   X_0 = M / max(|M|_F, eps),  X_{i+1} = a X_i + (b A + c A^2) X_i,  A = X_i X_i^T,  `steps` times
+ * update = 0: param = X_steps of grad (momentum unused; param must not be grad).
+ * update = 1: momentum = mu momentum + (1 - mu) grad, M = nesterov ? mu momentum + (1 - mu)
+ *   grad : momentum, param = param (1 - lr weight_decay) - lr adjust X_steps.
+ * param and grad are [rows, cols] contiguous of `dtype` (CT_F32 or CT_BF16), momentum float32.
+ * The iteration runs in double on the short side's Gram matrix, the last product in float32;
+ * results are rounded once. Sums run in a fixed order.
+ */
+typedef struct ct_muon_matrix {
+    void *param;
+    const void *grad;
+    float *momentum;
+    int64_t rows;
+    int64_t cols;
+    int64_t scratch;  /* written by ct_muon_plan */
+    int64_t parts;    /* written by ct_muon_plan */
+    float adjust;
+    int32_t splits;   /* written by ct_muon_plan */
+} ct_muon_matrix;
+
+typedef struct ct_muon_options {
+    double lr, weight_decay, momentum, a, b, c, eps;
+    int32_t nesterov;
+    int32_t steps;
+    int32_t update;
+} ct_muon_options;
+
+/*
+ * The work over `count` matrices (host table, whose scratch, parts and splits are filled in),
+ * cut into workgroups' shares: 32-byte entries of three kinds, counts[0..2], and the bytes of
+ * workspace. With entries = null only counts, the table and workspace_bytes are written. The
+ * caller copies the entries to the device (16-byte aligned); they hold for every call with
+ * these shapes. Empty matrices are refused: the caller leaves them out. ct_muon reads the
+ * host table while it runs and passes it to the device in kernel arguments.
+ */
+int ct_muon_plan(ct_muon_matrix *matrices, int64_t count, int32_t *entries, int64_t capacity, int64_t *counts,
+                 int64_t *workspace_bytes);
+int ct_muon(const ct_muon_matrix *matrices, int64_t count, const int32_t *plan, const int64_t *counts,
+            int32_t dtype, const ct_muon_options *options, void *workspace, int64_t workspace_bytes,
+            int64_t workspace_needed, hipStream_t stream);
+
+/*
  * Kernel timing for benchmarks; no counterpart in the reference (which publishes no kernel
  * timings). ct_profile_begin enables the families in `families` and creates `capacity`
  * HIP event pairs; each later launch of an enabled family is bracketed by one pair

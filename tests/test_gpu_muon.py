@@ -1,0 +1,168 @@
+"""orthogonalize and FusedMuon (ct_muon) against the iteration in float64.
+
+Bounds. The steps run in double, so what is left is the float32 product of the final r x r
+matrix Q (rounded once, e = 2^-24) with M / |M|: (r + 4) e |Q| |M| / |M|_F, doubled for second
+order and the double steps, and half a step u of the result's type. In a step, M itself is a
+float32 combination: three roundings, which the iteration (slope at most a^steps) carries to
+3 e a^steps in norm; the update and the parameter are rounded in float32 and stored in their type."""
+
+import copy
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+A, B, C = 3.4445, -4.7750, 2.0315
+E32 = 2.0 ** -24
+
+
+def _reference(m, steps=5, eps=1e-7, coefficients=(A, B, C)):
+    """(X_steps, elementwise bound before the output's own rounding) in float64."""
+    a, b, c = coefficients
+    x = m.double()
+    wide = x.T if x.shape[0] > x.shape[1] else x
+    x0 = wide / wide.norm().clamp(min=eps)
+    x, q = x0, torch.eye(len(x0), dtype=torch.float64, device=m.device)
+    for _ in range(steps):
+        g = x @ x.T
+        p = a * torch.eye(len(x0), dtype=torch.float64, device=m.device) + b * g + c * (g @ g)
+        x, q = p @ x, p @ q
+    bound = 2 * (len(x0) + 4) * E32 * (q.abs() @ x0.abs())
+    return (x.T, bound.T) if m.shape[0] > m.shape[1] else (x, bound)
+
+
+def _check(got, m, **kw):
+    want, bound = _reference(m, **kw)
+    u = torch.finfo(m.dtype).eps / 2
+    assert got.shape == m.shape and got.dtype == m.dtype and torch.isfinite(got).all()
+    over = (got.double() - want).abs() - bound - u * (want.abs() + bound) - 1e-37
+    assert over.max() <= 0, f"{tuple(m.shape)} {m.dtype}: {over.max()} over a bound of {bound.max()}"
+
+
+def _matrix(shape, dtype, decades=None, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(*shape, generator=g, dtype=torch.float64)
+    if decades is not None:
+        u, _, v = torch.linalg.svd(x, full_matrices=False)
+        x = (u * torch.logspace(0, -decades, min(shape), dtype=torch.float64)) @ v
+    return (x * 1e-3).to("cuda", dtype)
+
+
+SHAPES = [(1, 1), (1, 7), (5, 1), (3, 3), (16, 1024), (1024, 16), (31, 33), (33, 31), (64, 64), (65, 200), (130, 1111),
+          (2049, 64), (255, 257), (256, 4096), (4100, 128), (8, 3001), (300, 513), (700, 290)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_orthogonalize(shape, dtype):
+    from causal_tuner.optim import orthogonalize
+    m = _matrix(shape, dtype)
+    kept = m.clone()
+    _check(orthogonalize(m), m)
+    assert torch.equal(m, kept)
+
+
+@pytest.mark.parametrize("decades", [1, 2, 3, 5])
+def test_spectra_over_decades(decades):
+    from causal_tuner.optim import orthogonalize
+    m = _matrix((96, 500), torch.float32, decades)
+    _check(orthogonalize(m), m)
+
+
+def test_many_matrices_of_mixed_kinds_in_one_call():
+    from causal_tuner.optim import orthogonalize
+    inputs = [_matrix(s, t, seed=i) for i, (s, t) in enumerate(
+        [((16, 100), torch.float32), ((100, 16), torch.bfloat16), ((70, 70), torch.float32), ((0, 5), torch.float32),
+         ((256, 300), torch.bfloat16)] * 12)]
+    strided = _matrix((64, 90), torch.float32).T
+    inputs.append(strided)
+    results = orthogonalize(inputs)
+    assert len(results) == len(inputs)
+    for got, m in zip(results, inputs):
+        if m.numel():
+            _check(got, m)
+        assert got.shape == m.shape
+    again = orthogonalize(inputs)
+    assert all(torch.equal(x, y) for x, y in zip(results, again))
+
+
+def test_zero_tiny_and_infinite_matrices():
+    from causal_tuner.optim import orthogonalize
+    zero, tiny = torch.zeros(20, 30, device="cuda"), _matrix((20, 30), torch.float32) * 1e-6
+    bad = _matrix((20, 30), torch.float32)
+    bad[3, 4] = float("inf")
+    x, y, z = orthogonalize([zero, tiny, bad])
+    assert not x.any()
+    _check(y, tiny)
+    assert torch.isnan(z).all()
+
+
+@pytest.mark.parametrize("steps,coefficients", [(1, (2.0, -1.5, 0.5)), (2, (A, B, C)), (3, (1.875, -1.25, 0.375)),
+                                                (8, (A, B, C))])
+def test_steps_and_coefficients(steps, coefficients):
+    from causal_tuner.optim import orthogonalize
+    m = _matrix((40, 100), torch.float32)
+    _check(orthogonalize(m, steps=steps, coefficients=coefficients), m, steps=steps, coefficients=coefficients)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("adjust", [None, "match_rms_adamw"])
+def test_muon_steps(dtype, nesterov, adjust):
+    from causal_tuner.optim import FusedMuon
+    shapes = [(16, 256), (256, 16), (128, 300), (40, 40)]
+    params = [torch.nn.Parameter(_matrix(s, dtype, seed=i) * 20) for i, s in enumerate(shapes)]
+    skipped = torch.nn.Parameter(_matrix((4, 4), dtype))
+    lr, decay, mu = 0.02, 0.1, 0.9
+    optimizer = FusedMuon([*params, skipped], lr=lr, weight_decay=decay, momentum=mu, nesterov=nesterov,
+                          adjust_lr_fn=adjust)
+    unchanged = skipped.detach().clone()
+    momentum = [torch.zeros(s, dtype=torch.float64, device="cuda") for s in shapes]
+    u = torch.finfo(dtype).eps / 2
+    for step in range(3):
+        before = [p.detach().double() for p in params]
+        for i, p in enumerate(params):
+            p.grad = _matrix(shapes[i], dtype, seed=100 * step + i)
+        optimizer.step()
+        for p, old, m in zip(params, before, momentum):
+            buffer = optimizer.state[p]["momentum_buffer"]
+            m.mul_(mu).add_(p.grad.double(), alpha=1 - mu)
+            assert buffer.dtype == torch.float32
+            assert ((buffer.double() - m).abs() <= 4 * (step + 1) * E32 * (m.abs() + p.grad.abs().max())).all()
+            m.copy_(buffer)   # from here on with what the optimizer holds
+            direction, bound = _reference(mu * m + (1 - mu) * p.grad.double() if nesterov else m)
+            rows, cols = p.shape
+            factor = lr * (0.2 * max(rows, cols) ** 0.5 if adjust else max(1.0, rows / cols) ** 0.5)
+            want = old * (1 - lr * decay) - factor * direction
+            allowed = factor * (bound + 3 * E32 * A ** 5 + 4 * E32 * direction.abs()) + 4 * E32 * old.abs()
+            over = (p.double() - want).abs() - allowed - u * (want.abs() + allowed)
+            assert over.max() <= 0, f"{tuple(p.shape)}: {over.max()} over"
+    assert torch.equal(skipped, unchanged) and "momentum_buffer" not in optimizer.state[skipped]
+
+
+def test_muon_against_torch_and_its_state():
+    """torch.optim.Muon runs its steps in bfloat16: parameters agree to that (each step's update
+    within 2^-8 a few times over its norm), momenta to float32."""
+    from causal_tuner.optim import FusedMuon
+    start = [_matrix(s, torch.float32, seed=i) for i, s in enumerate([(32, 200), (200, 32)])]
+    ours, theirs = ([torch.nn.Parameter(m.clone()) for m in start] for _ in range(2))
+    a, b = FusedMuon(ours, lr=0.02), torch.optim.Muon(theirs, lr=0.02)
+    for step in range(2):
+        for x, y in zip(ours, theirs):
+            x.grad = _matrix(tuple(x.shape), torch.float32, seed=step + 7)
+            y.grad = x.grad.clone()
+        a.step()
+        b.step()
+    for x, y, m in zip(ours, theirs, start):
+        moved = (y - m).norm()
+        assert (x - y).norm() <= 0.05 * moved
+        torch.testing.assert_close(a.state[x]["momentum_buffer"], b.state[y]["momentum_buffer"], rtol=1e-6, atol=1e-9)
+    fresh = FusedMuon([torch.nn.Parameter(m.clone().bfloat16()) for m in start])
+    fresh.load_state_dict(copy.deepcopy(b.state_dict()))
+    for p, y in zip(fresh.param_groups[0]["params"], theirs):
+        assert fresh.state[p]["momentum_buffer"].dtype == torch.float32
+        assert torch.equal(fresh.state[p]["momentum_buffer"], b.state[y]["momentum_buffer"])
+        p.grad = torch.ones_like(p)
+    fresh.step()
+    assert fresh.param_groups[0]["lr"] == 0.02
