@@ -69,6 +69,9 @@ class Attention(ctypes.Structure):
 _ATT = ctypes.POINTER(Attention)
 
 
+CT_MUON_KINDS = 7  # kinds of plan entries of ct_muon_plan
+
+
 class MuonMatrix(ctypes.Structure):
     """Mirror of `ct_muon_matrix`: one matrix of an orthogonalising call."""
 

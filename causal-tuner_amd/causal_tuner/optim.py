@@ -128,7 +128,7 @@ class _MuonPlan:
         table = (_native.MuonMatrix * len(shapes))()
         for row, (rows, cols, adjust) in zip(table, shapes):
             row.rows, row.cols, row.adjust = rows, cols, adjust
-        self.counts, needed = (ctypes.c_int64 * 3)(), ctypes.c_int64()
+        self.counts, needed = (ctypes.c_int64 * _native.CT_MUON_KINDS)(), ctypes.c_int64()
         _native.check(lib.ct_muon_plan(table, len(shapes), None, 0, self.counts, ctypes.byref(needed)), "ct_muon_plan")
         size = sum(self.counts)
         entries = torch.empty(size, 8, dtype=torch.int32)

@@ -34,8 +34,10 @@ typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
 
 constexpr int kThreads = 256;
 constexpr int kPad = 32;        // r x r matrices are stored with r rounded up to this
-constexpr int kGramTile = 64;   // rows of M per side of a Gram share
-constexpr int kCols = 64;       // long-side elements per share of the last product
+constexpr int kSmall = 64;      // short sides up to this iterate inside one workgroup
+constexpr int kOnePass = 256;   // short sides up to this make their Gram matrix in one pass over M
+constexpr int kGramTile = 64;   // rows of M per side of a Gram share past kOnePass
+constexpr int kChunk = 32;      // long-side elements per LDS stage
 constexpr int kEntry = 8;       // int32 per plan entry
 
 struct Matrix {                 // ct_muon_matrix
@@ -43,38 +45,89 @@ struct Matrix {                 // ct_muon_matrix
     const void *grad;
     float *momentum;
     int64_t rows, cols;
-    int64_t scratch;            // doubles from the workspace's start
-    int64_t parts;              // partial Gram tiles of this matrix: first, in tiles of 64 x 64 doubles
+    int64_t scratch;            // doubles from the workspace's start: the r x r buffers
+    int64_t parts;              // and the partial Gram matrices
     float adjust;
-    int32_t splits;
+    int32_t splits;             // partial Gram matrices
 };
 
 struct Item {
-    int32_t matrix, i, j, lo, hi, pad0, pad1, pad2;
+    int32_t matrix, i, j, lo, hi, slot, pad0, pad1;
 };
 
 struct Hyper {
     float lr, mu, rest, keep;   // rest = 1 - mu, keep = 1 - lr decay
-    int nesterov, step;   // step: 0 = orthogonalize grad into param
+    int nesterov, step;         // step: 0 = orthogonalize grad into param
     double a, b, c, eps;
 };
 
-__device__ __forceinline__ int short_side(const Matrix &m) { return (int)(m.rows < m.cols ? m.rows : m.cols); }
-__device__ __forceinline__ int padded(int r) { return (r + kPad - 1) / kPad * kPad; }
+__host__ __device__ __forceinline__ int64_t least(int64_t x, int64_t y) { return x < y ? x : y; }
+__device__ __forceinline__ int short_side(const Matrix &m) { return (int)least(m.rows, m.cols); }
+__host__ __device__ __forceinline__ int padded(int r) { return (r + kPad - 1) / kPad * kPad; }
+__host__ __device__ __forceinline__ int tiles16(int r) { return (r + 15) / 16; }
+
+// A partial Gram matrix: the squared norms of its part of M (one, or one per 64 rows), then
+// the 16 x 16 tiles (i, j), i >= j, row by row.
+__host__ __device__ __forceinline__ int part_head(int r) {
+    return r <= kOnePass ? 2 : (r + kGramTile - 1) / kGramTile + 1 & ~1;
+}
+__host__ __device__ __forceinline__ int64_t part_size(int r) {
+    const int64_t t = tiles16(r);
+    return part_head(r) + t * (t + 1) / 2 * 256;
+}
+__device__ __forceinline__ double *part_of(const Matrix &m, double *ws, int slot) {
+    return ws + m.parts + slot * part_size(short_side(m));
+}
+__device__ __forceinline__ int64_t tile_of(int i, int j) { return ((int64_t)i * (i + 1) / 2 + j) * 256; }
+
+// The buffers of one matrix: 1 / |M|, then G, P, T and two Q (doubles; not for small ones)
+// and the final float Q.
+enum { kG = 0, kP = 1, kT = 2, kQ = 3, kBuffers = 5 };
+__device__ __forceinline__ double *buffer(const Matrix &m, double *ws, int which) {
+    const int64_t rp = padded(short_side(m));
+    return ws + m.scratch + 2 + which * rp * rp;
+}
+__device__ __forceinline__ float *final_q(const Matrix &m, double *ws) {
+    return reinterpret_cast<float *>(short_side(m) <= kSmall ? ws + m.scratch + 2 : buffer(m, ws, kBuffers));
+}
+// Element (row, k) of the final Q, ordered as the last product's lanes read it: lane (row, h)
+// takes k = 8 s + 4 h .. + 3 in one 16-byte load, 64 lanes 1 KB in a row.
+__device__ __forceinline__ int64_t final_at(int rp, int row, int k) {
+    return (((int64_t)(k >> 3) * rp + row) * 2 + ((k >> 2) & 1)) * 4 + (k & 3);
+}
 
 template <typename T>
 __device__ __forceinline__ float load_elem(const void *p, int64_t i) {
     if constexpr (sizeof(T) == 2) return bf16_to_f32(static_cast<const uint16_t *>(p)[i]);
     else return static_cast<const float *>(p)[i];
 }
+// Four elements from a multiple of four.
+template <typename T>
+__device__ __forceinline__ float4 load_four(const void *p, int64_t i) {
+    if constexpr (sizeof(T) == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i);
+        return make_float4(__builtin_bit_cast(float, v.x << 16), __builtin_bit_cast(float, v.x & 0xffff0000u),
+                           __builtin_bit_cast(float, v.y << 16), __builtin_bit_cast(float, v.y & 0xffff0000u));
+    } else {
+        return *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+    }
+}
 
-// Element of M: the gradient, or the step's combination of it with the updated momentum.
+// M from the gradient and the updated momentum.
+__device__ __forceinline__ float combine(const Hyper &h, float g, float m) {
+    return !h.step ? g : h.nesterov ? __builtin_fmaf(h.mu, m, h.rest * g) : m;
+}
 template <typename T>
 __device__ __forceinline__ float source(const Matrix &m, const Hyper &h, int64_t i) {
     const float g = load_elem<T>(m.grad, i);
-    if (!h.step) return g;
-    const float v = m.momentum[i];
-    return h.nesterov ? __builtin_fmaf(h.mu, v, h.rest * g) : v;
+    return h.step ? combine(h, g, m.momentum[i]) : g;
+}
+
+// Whether groups of four along a row can be loaded at once.
+template <typename T>
+__device__ __forceinline__ bool by_four(const Matrix &m, bool step) {
+    const uintptr_t p = (uintptr_t)m.grad | (uintptr_t)m.param, q = step ? (uintptr_t)m.momentum : 0;
+    return m.cols % 4 == 0 && p % (4 * sizeof(T)) == 0 && q % 16 == 0;
 }
 
 // ------------------------------------------------------------------ the table
@@ -90,29 +143,199 @@ __global__ __launch_bounds__(64) void muon_table(Matrix *dst, TableChunk chunk, 
     if ((int)threadIdx.x < count) dst[threadIdx.x] = chunk.m[threadIdx.x];
 }
 
-// ------------------------------------------------------------------ momentum
-template <typename T>
-__global__ __launch_bounds__(kThreads) void muon_momentum(const Matrix *matrices, const Item *items, Hyper h) {
-    const Item it = items[blockIdx.x];
-    const Matrix m = matrices[it.matrix];
-    const int r = short_side(m);
-    const int64_t width = m.rows * m.cols / r;
-    const int64_t end = (int64_t)it.hi < width ? (int64_t)it.hi * r : width * r;
-    for (int64_t i = (int64_t)it.lo * r + threadIdx.x; i < end; i += kThreads)
-        m.momentum[i] = __builtin_fmaf(h.mu, m.momentum[i], h.rest * load_elem<T>(m.grad, i));
-}
-
-// ------------------------------------------------------------------ Gram matrix
 // D[4 i + l / 16][l % 16] for i = 0..3 of A[l % 16][l / 16] B[l / 16][l % 16].
 __device__ __forceinline__ f64x4 mfma_f64(double a, double b, f64x4 c) {
     return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0);
 }
 
+// ------------------------------------------------------------------ Gram matrix, one pass
+// A workgroup of 8 waves reads its range of the long side once, with every row of the short
+// side, updates the momentum there, and holds the lower triangle of its partial Gram matrix
+// in registers: NT tiles of 16 rows, strips w and NT - 1 - w to one wave (NT + 1 tiles
+// each); where that takes fewer than 8 waves, groups of waves share out the k-steps and
+// leave partials of their own. Reading M once costs 12 bytes an element (4 in orthogonalize);
+// the products, 64 cycles for 16 x 16 x 4, bound it from rank 256 on.
+constexpr int kGramThreads = 512;
+
+struct Four {
+    float4 g, m;
+};
+
+template <typename T, int NT, bool TALL>
+__device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, const Hyper &h, double *ws, float *lds) {
+    constexpr int kRows = 16 * NT, kUnits = kRows * kChunk / 4;
+    constexpr int kPasses = (kUnits + kGramThreads - 1) / kGramThreads;
+    constexpr int kPitch = TALL ? (NT == 1 ? 16 : kRows + 16) : kChunk + 4;
+    constexpr int kStage = TALL ? kPitch * kChunk : kPitch * kRows;
+    constexpr int kWaves = NT < 2 ? 1 : NT / 2, kGroups = 8 / kWaves;
+    const int r = short_side(m), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int w = wave % kWaves, group = wave / kWaves, top = NT - 1 - w;
+    const bool four = by_four<T>(m, h.step);
+    const int64_t cols = m.cols;
+    f64x4 acc[NT + 1] = {};
+    double norm = 0.0;
+    Four held[kPasses];
+
+    // element (s, l) of a unit: four along the stored rows
+    auto place = [&](int p, int &s, int &l) -> bool {
+        const int u = p * kGramThreads + tid;
+        if (kUnits % kGramThreads && u >= kUnits) return false;
+        if constexpr (TALL) {
+            s = u % (kRows / 4) * 4;
+            l = u / (kRows / 4);
+        } else {
+            s = u / (kChunk / 4);
+            l = u % (kChunk / 4) * 4;
+        }
+        return true;
+    };
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+            int s, l;
+            held[p] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+            if (!place(p, s, l)) continue;
+            const int64_t at = TALL ? (int64_t)(k0 + l) * r + s : (int64_t)s * cols + k0 + l;
+            const int left = TALL ? (k0 + l < it.hi ? r - s : 0) : (s < r ? it.hi - k0 - l : 0);
+            if (four && left >= 4) {
+                held[p].g = load_four<T>(m.grad, at);
+                if (h.step) held[p].m = *reinterpret_cast<const float4 *>(m.momentum + at);
+            } else {
+                float *g = &held[p].g.x, *v = &held[p].m.x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (e < left) {
+                        g[e] = load_elem<T>(m.grad, at + e);
+                        if (h.step) v[e] = m.momentum[at + e];
+                    }
+            }
+        }
+    };
+    auto store = [&](int k0, float *stage) {
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+            int s, l;
+            if (!place(p, s, l)) continue;
+            float *g = &held[p].g.x, *v = &held[p].m.x;
+            if (h.step) {
+                const int64_t at = TALL ? (int64_t)(k0 + l) * r + s : (int64_t)s * cols + k0 + l;
+                const int left = TALL ? (k0 + l < it.hi ? r - s : 0) : (s < r ? it.hi - k0 - l : 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(h.mu, v[e], h.rest * g[e]);
+                if (four && left >= 4) {
+                    *reinterpret_cast<float4 *>(m.momentum + at) = held[p].m;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e < left) m.momentum[at + e] = v[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) g[e] = combine(h, g[e], v[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) norm = __builtin_fma((double)g[e], (double)g[e], norm);
+            *reinterpret_cast<float4 *>(stage + (TALL ? l * kPitch + s : s * kPitch + l)) = held[p].g;
+        }
+    };
+
+    int buf = 0;
+    if (it.lo < it.hi) {
+        load(it.lo);
+        store(it.lo, lds);
+    }
+    __syncthreads();
+    for (int k0 = it.lo; k0 < it.hi; k0 += kChunk) {
+        const bool more = k0 + kChunk < it.hi;
+        if (more) load(k0 + kChunk);
+        const float *stage = lds + buf * kStage + (TALL ? (lane >> 4) * kPitch + (lane & 15)
+                                                        : (lane & 15) * kPitch + (lane >> 4));
+        auto at = [&](int tile, int step) -> double {
+            return stage[tile * (TALL ? 16 : 16 * kPitch) + step * (TALL ? 4 * kPitch : 4)];
+        };
+#pragma unroll 1
+        for (int step = group; step < kChunk / 4; step += kGroups) {
+            const double high = at(top, step), low = at(NT < 2 ? 0 : w, step);
+#pragma unroll
+            for (int t = 0; t <= NT; ++t) {   // tiles 0 .. top of strip top, then w .. 0 of strip w
+                if (NT == 1 && t == 1) break;
+                const bool upper = t <= top;
+                acc[t] = mfma_f64(upper ? high : low, at(upper ? t : NT - t, step), acc[t]);
+            }
+        }
+        if (more) store(k0 + kChunk, lds + (buf ^ 1) * kStage);
+        __syncthreads();
+        buf ^= 1;
+    }
+
+    double *sums = reinterpret_cast<double *>(lds);
+    sums[tid] = norm;
+    __syncthreads();
+    for (int n = kGramThreads / 2; n; n >>= 1) {
+        if (tid < n) sums[tid] += sums[tid + n];
+        __syncthreads();
+    }
+    double *part = part_of(m, ws, it.slot * kGroups + group);
+    if (lane == 0 && w == 0) part[0] = group ? 0.0 : sums[0];
+    double *tiles = part + part_head(r);
+    const int have = tiles16(r);
+#pragma unroll
+    for (int t = 0; t <= NT; ++t) {
+        if (NT == 1 && t == 1) break;
+        const bool upper = t <= top;
+        const int i = upper ? top : w, j = upper ? t : NT - t;
+        if (i >= have) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tiles[tile_of(i, j) + (4 * e + (lane >> 4)) * 16 + (lane & 15)] = acc[t][e];
+    }
+}
+
+// NT for a short side: tiles of 16 rows, rounded up to a power of two.
+__host__ __device__ __forceinline__ int one_pass_tiles(int r) {
+    return r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : r <= 128 ? 8 : 16;
+}
+__host__ __forceinline__ int one_pass_groups(int r) {
+    const int nt = one_pass_tiles(r);
+    return nt < 2 ? 8 : 16 / nt;
+}
+
+template <typename T, bool TALL>
+__device__ __forceinline__ void gram_by_size(const Matrix &m, const Item &it, const Hyper &h, double *ws, float *lds) {
+    switch (one_pass_tiles(short_side(m))) {
+        case 1: return gram_one_pass<T, 1, TALL>(m, it, h, ws, lds);
+        case 2: return gram_one_pass<T, 2, TALL>(m, it, h, ws, lds);
+        case 4: return gram_one_pass<T, 4, TALL>(m, it, h, ws, lds);
+        case 8: return gram_one_pass<T, 8, TALL>(m, it, h, ws, lds);
+        default: return gram_one_pass<T, 16, TALL>(m, it, h, ws, lds);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kGramThreads, 2) void muon_gram(const Matrix *matrices, const Item *items, Hyper h,
+                                                            double *ws) {
+    __shared__ __align__(16) float lds[2 * (kChunk + 4) * kOnePass];
+    const Item it = items[blockIdx.x];
+    const Matrix m = matrices[it.matrix];
+    if (m.rows > m.cols) gram_by_size<T, true>(m, it, h, ws, lds);
+    else gram_by_size<T, false>(m, it, h, ws, lds);
+}
+
+// ------------------------------------------------------------------ Gram matrix, any short side
+template <typename T>
+__global__ __launch_bounds__(kThreads) void muon_momentum(const Matrix *matrices, const Item *items, Hyper h) {
+    const Item it = items[blockIdx.x];
+    const Matrix m = matrices[it.matrix];
+    const int r = short_side(m);
+    for (int64_t i = (int64_t)it.lo * r + threadIdx.x; i < (int64_t)it.hi * r; i += kThreads)
+        m.momentum[i] = __builtin_fmaf(h.mu, m.momentum[i], h.rest * load_elem<T>(m.grad, i));
+}
+
 // One 64 x 64 tile (i >= j) of M M^T over the columns lo .. hi - 1: 4 waves of 32 x 32.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void muon_gram(const Matrix *matrices, const Item *items, Hyper h, double *ws) {
+__global__ __launch_bounds__(kThreads) void muon_gram_tiles(const Matrix *matrices, const Item *items, Hyper h,
+                                                           double *ws) {
     constexpr int KC = 16, kPitch = KC + 4;
     __shared__ float sa[kGramTile * kPitch], sb[kGramTile * kPitch];
+    __shared__ double diagonal[kGramTile];
     const Item it = items[blockIdx.x];
     const Matrix m = matrices[it.matrix];
     const int r = short_side(m), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -146,58 +369,132 @@ __global__ __launch_bounds__(kThreads) void muon_gram(const Matrix *matrices, co
                 for (int y = 0; y < 2; ++y) acc[x][y] = mfma_f64(a[x], b[y], acc[x][y]);
         }
     }
-    double *dst = ws + (m.parts + it.pad0) * (kGramTile * kGramTile);
+    double *part = part_of(m, ws, it.slot), *tiles = part + part_head(r);
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+        for (int y = 0; y < 2; ++y) {
+            const int i = it.i * 4 + wi / 16 + x, j = it.j * 4 + wj / 16 + y;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                dst[(wi + 16 * x + 4 * i + (lane >> 4)) * kGramTile + wj + 16 * y + (lane & 15)] = acc[x][y][i];
+            for (int e = 0; e < 4; ++e) {
+                const int row = 4 * e + (lane >> 4), col = lane & 15;
+                if (i >= j && i < tiles16(r)) tiles[tile_of(i, j) + row * 16 + col] = acc[x][y][e];
+                if (i == j && row == col) diagonal[wi + 16 * x + row] = acc[x][y][e];
+            }
+        }
+    if (it.i != it.j) return;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double sum = 0.0;
+        for (int e = 0; e < kGramTile; ++e) sum += diagonal[e];
+        part[it.i] = sum;
+    }
 }
 
-// Buffers of one matrix in the workspace: G, P, T, two Q (doubles) and the final float Q.
-__device__ __forceinline__ double *buffer(const Matrix &m, double *ws, int which) {
-    const int64_t rp = padded(short_side(m));
-    return ws + m.scratch + 2 + which * rp * rp;   // [0] holds 1 / |M|
-}
-enum { kG = 0, kP = 1, kT = 2, kQ = 3, kFinal = 5 };
-
-// Partial tile that covers element (i, j), i >= j, split s.
-__device__ __forceinline__ double part(const Matrix &m, const double *ws, int i, int j, int s) {
-    const int ti = i / kGramTile, tj = j / kGramTile;
-    return ws[(m.parts + (ti * (ti + 1) / 2 + tj) * (int64_t)m.splits + s) * (kGramTile * kGramTile) +
-              (i % kGramTile) * kGramTile + j % kGramTile];
+// 1 / max(|M|, eps) from the parts' squared norms, in order.
+__device__ __forceinline__ double inverse_norm(const Matrix &m, double *ws, double eps) {
+    const int r = short_side(m), n = r <= kOnePass ? 1 : (r + kGramTile - 1) / kGramTile;
+    double sum = 0.0;
+    for (int s = 0; s < m.splits; ++s)
+        for (int e = 0; e < n; ++e) sum += part_of(m, ws, s)[e];
+    const double norm = sqrt(sum);
+    return 1.0 / (norm < eps ? eps : norm);
 }
 
-// G of a 32 x 32 tile: the partial sums in order, over the squared norm (G's trace, which
-// every workgroup sums for itself in one order).
+// Element `e` of tile (i, j): the parts in order.
+__device__ __forceinline__ double join_tile(const Matrix &m, double *ws, int i, int j, int e) {
+    const double *p = part_of(m, ws, 0) + part_head(short_side(m)) + tile_of(i, j) + e;
+    const int64_t step = part_size(short_side(m));
+    double v = 0.0;
+    for (int s = 0; s < m.splits; ++s) v += p[s * step];
+    return v;
+}
+
+// One 16 x 16 tile of G.
 __global__ __launch_bounds__(kThreads) void muon_join(const Matrix *matrices, const Item *items, Hyper h, double *ws) {
-    __shared__ double sums[kThreads];
     const Item it = items[blockIdx.x];
     const Matrix m = matrices[it.matrix];
-    const int r = short_side(m), rp = padded(r);
-    double trace = 0.0;
-    for (int i = threadIdx.x; i < r; i += kThreads)
-        for (int s = 0; s < m.splits; ++s) trace += part(m, ws, i, i, s);
-    sums[threadIdx.x] = trace;
-    __syncthreads();
-    for (int n = kThreads / 2; n; n >>= 1) {
-        if ((int)threadIdx.x < n) sums[threadIdx.x] += sums[threadIdx.x + n];
-        __syncthreads();
-    }
-    const double norm = sqrt(sums[0]), inv = 1.0 / (norm < h.eps ? h.eps : norm);
+    const int rp = padded(short_side(m)), row = threadIdx.x >> 4, col = threadIdx.x & 15;
+    const double inv = inverse_norm(m, ws, h.eps);
     if (it.i == 0 && threadIdx.x == 0) ws[m.scratch] = inv;
     double *g = buffer(m, ws, kG);
-    for (int e = threadIdx.x; e < kPad * kPad; e += kThreads) {
-        const int i = it.i * kPad + e / kPad, j = it.j * kPad + e % kPad;
-        if (i < j) continue;
-        double v = 0.0;
-        if (i < r)
-            for (int s = 0; s < m.splits; ++s) v += part(m, ws, i, j, s);
-        v *= inv * inv;
-        g[(int64_t)i * rp + j] = v;
-        g[(int64_t)j * rp + i] = v;
+    const int64_t i = it.i * 16 + row, j = it.j * 16 + col;
+    if (it.i >= tiles16(short_side(m))) {   // padding rows
+        g[i * rp + j] = g[j * rp + i] = 0.0;
+        return;
+    }
+    const double v = join_tile(m, ws, it.i, it.j, threadIdx.x) * (inv * inv);
+    if (i >= j) g[i * rp + j] = g[j * rp + i] = v;
+}
+
+// ------------------------------------------------------------------ short sides up to 64
+// All steps in one workgroup, G, P, T and Q in LDS. Symmetric operands are read along rows
+// for both sides of a product.
+__global__ __launch_bounds__(kThreads) void muon_small(const Matrix *matrices, const Item *items, Hyper h, double *ws,
+                                                      int steps) {
+    constexpr int kPitch = kSmall + 8;
+    __shared__ double sg[kSmall * kPitch], sp[kSmall * kPitch], st[kSmall * kPitch], sq[kSmall * kPitch];
+    const Item it = items[blockIdx.x];
+    const Matrix m = matrices[it.matrix];
+    const int r = short_side(m), n = tiles16(r), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const double inv = inverse_norm(m, ws, h.eps);
+    for (int t = 0, i = 0, j = 0; t < n * (n + 1) / 2; ++t) {
+        const double v = join_tile(m, ws, i, j, tid) * (inv * inv);
+        const int row = i * 16 + (tid >> 4), col = j * 16 + (tid & 15);
+        if (row >= col) sg[row * kPitch + col] = sg[col * kPitch + row] = v;
+        if (++j > i) ++i, j = 0;
+    }
+    __syncthreads();
+
+    // dst = left right, or a I + b left + c left right; dst may be an operand.
+    auto product = [&](const double *left, const double *right, double *dst, bool polynomial) {
+        constexpr int kMost = 3;   // of the ten tiles (i >= j) per wave
+        f64x4 acc[kMost] = {};
+        int ti[kMost], tj[kMost];
+#pragma unroll
+        for (int x = 0; x < kMost; ++x) {
+            const int t = wave + 4 * x;
+            ti[x] = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3;
+            tj[x] = t - ti[x] * (ti[x] + 1) / 2;
+        }
+        for (int k = lane >> 4; k < 16 * n; k += 4)
+#pragma unroll
+            for (int x = 0; x < kMost; ++x)
+                if (ti[x] < n && tj[x] <= ti[x])
+                    acc[x] = mfma_f64(left[k * kPitch + 16 * ti[x] + (lane & 15)],
+                                      right[k * kPitch + 16 * tj[x] + (lane & 15)], acc[x]);
+        if (polynomial) {
+#pragma unroll
+            for (int x = 0; x < kMost; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 16 * ti[x] + 4 * e + (lane >> 4), j = 16 * tj[x] + (lane & 15);
+                    if (ti[x] < n && tj[x] <= ti[x])
+                        acc[x][e] = h.c * acc[x][e] + h.b * left[i * kPitch + j] + (i == j && i < r ? h.a : 0.0);
+                }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < kMost; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 16 * ti[x] + 4 * e + (lane >> 4), j = 16 * tj[x] + (lane & 15);
+                if (ti[x] < n && tj[x] <= ti[x] && i >= j) dst[i * kPitch + j] = dst[j * kPitch + i] = acc[x][e];
+            }
+        __syncthreads();
+    };
+    for (int i = 0; i < steps; ++i) {
+        double *p = i == 0 ? sq : sp;   // the first P is the first Q
+        product(sg, sg, p, true);
+        if (i + 1 < steps) product(p, sg, st, false);
+        if (i) product(p, sq, sq, false);
+        if (i + 1 < steps) product(p, st, sg, false);
+    }
+    const int rp = padded(r);
+    float *final = final_q(m, ws);
+    for (int e = tid; e < rp * rp; e += kThreads) {
+        const int row = e % rp, k = e / rp;
+        final[final_at(rp, row, k)] = row < 16 * n && k < 16 * n ? (float)(sq[row * kPitch + k] * inv) : 0.0f;
     }
 }
 
@@ -209,137 +506,261 @@ struct StageOp {
 };
 
 // One 32 x 32 tile (i >= j) of left right, both symmetric and commuting, so their product is
-// symmetric too and the tile's mirror image is its transpose. kMakeP: a I + b G + c G G.
+// symmetric too and the tile's mirror image is its transpose. kMakeP: a I + b G + c G G. Each
+// of the 4 waves takes a quarter of the reduction over the whole tile (one load per product
+// instead of two) straight from L2, operand rows read along k's rows (symmetry), and the
+// quarters are added in LDS in order.
 __global__ __launch_bounds__(kThreads) void muon_stage(const Matrix *matrices, const Item *items, Hyper h, double *ws,
                                                       StageOp op0, StageOp op1) {
-    constexpr int KC = 32, kPitch = KC + 4;
-    __shared__ double sa[kPad * kPitch], sb[kPad * kPitch];
+    constexpr int kPitch = kPad + 1;
+    __shared__ double sums[4][kPad * kPitch];
     const StageOp op = blockIdx.y ? op1 : op0;
     const Item it = items[blockIdx.x];
     const Matrix m = matrices[it.matrix];
     const int r = short_side(m), rp = padded(r), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const double *left = buffer(m, ws, op.left) + (int64_t)it.i * kPad * rp;
-    const double *right = buffer(m, ws, op.right) + (int64_t)it.j * kPad * rp;
-    const int wi = (wave >> 1) * 16, wj = (wave & 1) * 16;
-    f64x4 acc = {};
-    for (int k0 = 0; k0 < rp; k0 += KC) {
-        __syncthreads();
-        for (int e = threadIdx.x; e < kPad * KC; e += kThreads) {
-            sa[e / KC * kPitch + e % KC] = left[(int64_t)(e / KC) * rp + k0 + e % KC];
-            sb[e / KC * kPitch + e % KC] = right[(int64_t)(e / KC) * rp + k0 + e % KC];
-        }
-        __syncthreads();
+    const double *left = buffer(m, ws, op.left) + it.i * kPad + (lane & 15) + (int64_t)(lane >> 4) * rp;
+    const double *right = buffer(m, ws, op.right) + it.j * kPad + (lane & 15) + (int64_t)(lane >> 4) * rp;
+    f64x4 acc[2][2] = {};
+    // rp is a multiple of 32: a quarter is a multiple of 8 rows
+    const int64_t first = (int64_t)wave * (rp / 4) * rp, step = 4 * (int64_t)rp;
+    const double *a = left + first, *b = right + first;
+    for (int k = 0; k < rp / 4; k += 8) {
+        double x[2][2], y[2][2];
 #pragma unroll
-        for (int s = 0; s < KC; s += 4)
-            acc = mfma_f64(sa[(wi + (lane & 15)) * kPitch + s + (lane >> 4)],
-                           sb[(wj + (lane & 15)) * kPitch + s + (lane >> 4)], acc);
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                x[u][t] = a[u * step + 16 * t];
+                y[u][t] = b[u * step + 16 * t];
+            }
+        a += 2 * step;
+        b += 2 * step;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = mfma_f64(x[u][i], y[u][j], acc[i][j]);
     }
-    const double inv = op.last ? ws[m.scratch] : 1.0;
-    double *dst = buffer(m, ws, op.dst);
-    float *final = reinterpret_cast<float *>(buffer(m, ws, kFinal));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int i = it.i * kPad + wi + 4 * e + (lane >> 4), j = it.j * kPad + wj + (lane & 15);
-        if (i < j) continue;
-        double v = acc[e];
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                sums[wave][(16 * i + 4 * e + (lane >> 4)) * kPitch + 16 * j + (lane & 15)] = acc[i][j][e];
+    __syncthreads();
+    const double inv = op.last ? ws[m.scratch] : 1.0;
+    const double *g = buffer(m, ws, op.left);
+    double *dst = buffer(m, ws, op.dst);
+    float *final = final_q(m, ws);
+    auto value = [&](int row, int col) -> double {
+        const int at = row * kPitch + col;
+        double v = ((sums[0][at] + sums[1][at]) + sums[2][at]) + sums[3][at];
         if (op.kind == kMakeP) {
-            v = h.c * v + h.b * left[(int64_t)(i - it.i * kPad) * rp + j];
+            const int i = it.i * kPad + row, j = it.j * kPad + col;
+            v = h.c * v + h.b * g[(int64_t)i * rp + j];
             if (i == j && i < r) v += h.a;
         }
-        const int64_t x = (int64_t)i * rp + j, y = (int64_t)j * rp + i;
-        if (op.last) {
-            final[x] = final[y] = (float)(v * inv);
-        } else {
-            dst[x] = v;
-            dst[y] = v;
+        return v;
+    };
+    for (int e = threadIdx.x; e < kPad * kPad; e += kThreads) {
+        const int row = e / kPad, col = e % kPad;
+        // (row, col) of the tile itself, then of its mirror image, both stored along rows
+        const double v = it.i == it.j && row < col ? value(col, row) : value(row, col);
+        const int i = it.i * kPad + row, j = it.j * kPad + col;
+        if (op.last) final[final_at(rp, i, j)] = (float)(v * inv);
+        else dst[(int64_t)i * rp + j] = v;
+        if (it.i != it.j) {
+            const double u = value(col, row);
+            const int x = it.j * kPad + row, y = it.i * kPad + col;
+            if (op.last) final[final_at(rp, x, y)] = (float)(u * inv);
+            else dst[(int64_t)x * rp + y] = u;
         }
     }
 }
 
 // ------------------------------------------------------------------ the last product
-// 64 elements of the long side, all of the short side in blocks of 128: 4 waves of 32 x 64
-// (wide) or 64 x 32 (tall), v_mfma_f32_32x32x2.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void muon_apply(const Matrix *matrices, const Item *items, Hyper h, double *ws) {
-    constexpr int KC = 32, kPitch = KC + 1;
-    __shared__ float sx[kCols * kPitch];   // [long][short]
-    const Item it = items[blockIdx.x];
-    const Matrix m = matrices[it.matrix];
-    const int r = short_side(m), rp = padded(r), lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-    const bool tall = m.rows > m.cols;
-    const int64_t width = tall ? m.rows : m.cols, col0 = (int64_t)it.i * kCols;
-    const float *q = reinterpret_cast<const float *>(buffer(m, ws, kFinal));
-    for (int r0 = 0; r0 < rp; r0 += 128) {
-        const int row = r0 + wave * 32 + (lane & 31);
+// Q M by 8 waves: each takes 32 rows of the short side and 64 elements of the long side
+// (v_mfma_f32_32x32x2, 2 x 32), so a workgroup covers 64, 128, 256 or 512 elements of the long
+// side with short sides up to 256, 128, 64 or 32. Its part of M (combined from gradient and
+// momentum on the way) stays in LDS, Q comes from L2 in the order that final_at gives it.
+// Short sides past 256 go in blocks of 256 rows and 256 of the reduction.
+constexpr int kApplyThreads = 512;
+
+__host__ __device__ __forceinline__ int apply_blocks(int r) { return r <= 32 ? 1 : r <= 64 ? 2 : r <= 128 ? 4 : 8; }
+
+template <typename T, int NB, bool TALL>
+__device__ __forceinline__ void apply_slab(const Matrix &m, const Item &it, const Hyper &h, double *ws, float *sx) {
+    constexpr int kLong = 64 * (8 / NB), kShort = 32 * NB;
+    constexpr int kPitch = TALL ? kShort + 4 : kLong + 8;
+    constexpr int kUnits = kLong * kShort / 4 / kApplyThreads;   // 8
+    const int r = short_side(m), rp = padded(r), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+    const int block = wave % NB, part = wave / NB * 64;
+    const int64_t width = TALL ? m.rows : m.cols, col0 = it.lo;
+    const bool four = by_four<T>(m, h.step);
+    const float *q = final_q(m, ws);
+    for (int r0 = 0; r0 < rp; r0 += kShort) {
+        const int row = r0 + 32 * block;   // this wave's short rows
         f32x16 acc[2] = {};
-        for (int k0 = 0; k0 < rp; k0 += KC) {
+        for (int k0 = 0; k0 < rp; k0 += kShort) {
             __syncthreads();
-            for (int e = threadIdx.x; e < kCols * KC; e += kThreads) {
-                const int c = tall ? e / KC : e % kCols, k = tall ? e % KC : e / kCols;
-                float v = 0.0f;
-                if (k0 + k < r && col0 + c < width)
-                    v = source<T>(m, h, tall ? (col0 + c) * r + k0 + k : (int64_t)(k0 + k) * m.cols + col0 + c);
-                sx[c * kPitch + k] = v;
+#pragma unroll
+            for (int p = 0; p < kUnits; ++p) {
+                const int u = p * kApplyThreads + tid;
+                const int s = TALL ? u % (kShort / 4) * 4 : u / (kLong / 4), l = TALL ? u / (kShort / 4) : u % (kLong / 4) * 4;
+                const int64_t at = TALL ? (col0 + l) * r + k0 + s : (int64_t)(k0 + s) * m.cols + col0 + l;
+                const int64_t left = TALL ? (col0 + l < width ? r - k0 - s : 0) : (k0 + s < r ? width - col0 - l : 0);
+                float4 v = make_float4(0, 0, 0, 0);
+                if (four && left >= 4) {
+                    v = load_four<T>(m.grad, at);
+                    if (h.step) {
+                        const float4 b = *reinterpret_cast<const float4 *>(m.momentum + at);
+                        v = make_float4(combine(h, v.x, b.x), combine(h, v.y, b.y), combine(h, v.z, b.z),
+                                        combine(h, v.w, b.w));
+                    }
+                } else {
+                    float *x = &v.x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e < left) x[e] = source<T>(m, h, at + e);
+                }
+                *reinterpret_cast<float4 *>(sx + (TALL ? l * kPitch + s : s * kPitch + l)) = v;
             }
             __syncthreads();
-            if (r0 + wave * 32 < rp) {
+            if (row >= rp) continue;
+            const int depth = rp - k0 < kShort ? rp - k0 : kShort;
+            const float4 *w = reinterpret_cast<const float4 *>(q) + ((int64_t)(k0 / 8) * rp + row + (lane & 31)) * 2 + half;
+#pragma unroll 2
+            for (int s = 0; s < depth; s += 8) {
+                const float4 w4 = w[(int64_t)(s / 8) * rp * 2];
+                const float wv[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-                for (int k = 0; k < KC; k += 2) {
-                    const float w = q[(int64_t)(k0 + k + half) * rp + row];
+                for (int t = 0; t < 2; ++t) {
+                    float xv[4];
+                    if constexpr (TALL) {
+                        const float4 x4 = *reinterpret_cast<const float4 *>(
+                            sx + (part + 32 * t + (lane & 31)) * kPitch + s + 4 * half);
+                        xv[0] = x4.x; xv[1] = x4.y; xv[2] = x4.z; xv[3] = x4.w;
+                    } else {
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const float x = sx[(32 * t + (lane & 31)) * kPitch + k + half];
-                        acc[t] = tall ? __builtin_amdgcn_mfma_f32_32x32x2f32(x, w, acc[t], 0, 0, 0)
-                                      : __builtin_amdgcn_mfma_f32_32x32x2f32(w, x, acc[t], 0, 0, 0);
+                        for (int e = 0; e < 4; ++e) xv[e] = sx[(s + 4 * half + e) * kPitch + part + 32 * t + (lane & 31)];
                     }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[t] = TALL ? __builtin_amdgcn_mfma_f32_32x32x2f32(xv[e], wv[e], acc[t], 0, 0, 0)
+                                      : __builtin_amdgcn_mfma_f32_32x32x2f32(wv[e], xv[e], acc[t], 0, 0, 0);
                 }
             }
         }
-        if (r0 + wave * 32 >= rp) continue;
+        if (row >= rp) continue;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
+            // register i is `8 (i / 4) + i % 4` rows of the stored matrix below the lane's first
+            const int s = row + (TALL ? lane & 31 : 4 * half);
+            const int64_t l = col0 + part + 32 * t + (TALL ? 4 * half : lane & 31);
+            const int64_t stride = TALL ? r : m.cols, at = TALL ? l * r + s : (int64_t)s * m.cols + l;
+            const int64_t below = TALL ? (s < r ? width - l : 0) : (l < width ? r - s : 0);
+            const int limit = below > 32 ? 32 : (int)below;
+            T *lane_param = static_cast<T *>(m.param) + at;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int down = 8 * (i >> 2) + 4 * half + (i & 3), across = lane & 31;
-                const int s = r0 + wave * 32 + (tall ? across : down);
-                const int64_t l = col0 + 32 * t + (tall ? down : across);
-                if (s >= r || l >= width) continue;
-                const int64_t at = tall ? l * r + s : (int64_t)s * m.cols + l;
+                const int down = 8 * (i >> 2) + (i & 3);
+                if (down >= limit) continue;
+                T *dst = lane_param + down * stride;
                 float v = acc[t][i];
-                if (h.step) {
-                    const float p = load_elem<T>(m.param, at);
-                    v = __builtin_fmaf(-h.lr * m.adjust, v, p * h.keep);
-                }
-                if constexpr (sizeof(T) == 2) static_cast<uint16_t *>(m.param)[at] = bf16_bits(v);
-                else static_cast<float *>(m.param)[at] = v;
+                if (h.step) v = __builtin_fmaf(-h.lr * m.adjust, v, load_elem<T>(dst, 0) * h.keep);
+                if constexpr (sizeof(T) == 2) *dst = bf16_bits(v);
+                else *dst = v;
             }
+        }
     }
+}
+
+template <typename T, bool TALL>
+__device__ __forceinline__ void apply_by_size(const Matrix &m, const Item &it, const Hyper &h, double *ws, float *sx) {
+    switch (apply_blocks(short_side(m))) {
+        case 1: return apply_slab<T, 1, TALL>(m, it, h, ws, sx);
+        case 2: return apply_slab<T, 2, TALL>(m, it, h, ws, sx);
+        case 4: return apply_slab<T, 4, TALL>(m, it, h, ws, sx);
+        default: return apply_slab<T, 8, TALL>(m, it, h, ws, sx);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kApplyThreads, 4) void muon_apply(const Matrix *matrices, const Item *items, Hyper h,
+                                                              double *ws) {
+    __shared__ __align__(16) float sx[18432];   // 256 x 72, 128 x 136, 64 x 264, 32 x 520 and their transposes
+    const Item it = items[blockIdx.x];
+    const Matrix m = matrices[it.matrix];
+    if (m.rows > m.cols) apply_by_size<T, true>(m, it, h, ws, sx);
+    else apply_by_size<T, false>(m, it, h, ws, sx);
 }
 
 // ------------------------------------------------------------------ host side
 constexpr int64_t kMaxShort = 16384, kMaxLong = (int64_t)1 << 30;
+constexpr int64_t kGroupsWanted = 256;   // one Gram workgroup per CU
+
+enum { kItemsGram = 0, kItemsTiles, kItemsMomentum, kItemsJoin, kItemsStage, kItemsSmall, kItemsApply, kKinds };
 
 struct Shape {
-    int64_t r, width, rp, pairs, splits;
+    int r, rp;
+    int64_t width;
 };
 
 bool shape_of(int64_t rows, int64_t cols, Shape &s) {
     if (rows <= 0 || cols <= 0) return false;
-    s.r = std::min(rows, cols);
     s.width = std::max(rows, cols);
-    if (s.r > kMaxShort || s.width > kMaxLong) return false;
-    s.rp = cdiv(s.r, kPad) * kPad;
-    const int64_t tiles = cdiv(s.r, kGramTile);
-    s.pairs = tiles * (tiles + 1) / 2;
-    s.splits = std::max<int64_t>(1, std::min<int64_t>(cdiv(s.width, 512), 32));
+    if (std::min(rows, cols) > kMaxShort || s.width > kMaxLong) return false;
+    s.r = (int)std::min(rows, cols);
+    s.rp = padded(s.r);
     return true;
 }
 
-int64_t scratch_doubles(const Shape &s) { return 2 + 5 * s.rp * s.rp + s.rp * s.rp / 2; }
+int64_t scratch_doubles(const Shape &s) {
+    const int64_t square = (int64_t)s.rp * s.rp;
+    return 2 + (s.r <= kSmall ? 0 : kBuffers * square) + square / 2;
+}
 
 int status_of_last_launch() {
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : (int)e;
+}
+
+// A matrix's items and partials, whose Gram products are `share` of kGroupsWanted workgroups.
+void plan_matrix(int32_t index, const Shape &s, double share, std::vector<Item> (&items)[kKinds], int32_t &splits) {
+    const int64_t most = cdiv(s.width, 2 * kChunk);
+    const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)(share * kGroupsWanted + 0.5)));
+    const bool one_pass = s.r <= kOnePass;
+    const int64_t parts = one_pass ? wanted : std::max<int64_t>(1, std::min<int64_t>(cdiv(s.width, 512), 32));
+    const int64_t step = cdiv(cdiv(s.width, parts), kChunk) * kChunk;
+    const int64_t count = cdiv(s.width, step);
+    auto range = [&](int64_t k, int32_t i, int32_t j) -> Item {
+        return {index, i, j, (int32_t)(k * step), (int32_t)std::min(s.width, (k + 1) * step), (int32_t)k, 0, 0};
+    };
+    if (one_pass) {
+        for (int64_t k = 0; k < count; ++k) items[kItemsGram].push_back(range(k, 0, 0));
+        splits = (int32_t)count * one_pass_groups(s.r);
+    } else {
+        const int tiles = (s.r + kGramTile - 1) / kGramTile;
+        for (int64_t k = 0; k < count; ++k)
+            for (int a = 0; a < tiles; ++a)
+                for (int b = 0; b <= a; ++b) items[kItemsTiles].push_back(range(k, a, b));
+        for (int64_t c = 0; c < s.width; c += 64)
+            items[kItemsMomentum].push_back({index, 0, 0, (int32_t)c, (int32_t)std::min(s.width, c + 64), 0, 0, 0});
+        splits = (int32_t)count;
+    }
+    if (s.r <= kSmall) {
+        items[kItemsSmall].push_back({index, 0, 0, 0, 0, 0, 0, 0});
+    } else {
+        for (int a = 0; a < s.rp / 16; ++a)
+            for (int b = 0; b <= a; ++b) items[kItemsJoin].push_back({index, a, b, 0, 0, 0, 0, 0});
+        for (int a = 0; a < s.rp / kPad; ++a)
+            for (int b = 0; b <= a; ++b) items[kItemsStage].push_back({index, a, b, 0, 0, 0, 0, 0});
+    }
+    const int64_t slab = 64 * (8 / apply_blocks(s.r));
+    for (int64_t c = 0; c < s.width; c += slab)
+        items[kItemsApply].push_back({index, 0, 0, (int32_t)c, (int32_t)std::min(s.width, c + slab), 0, 0, 0});
 }
 
 }  // namespace
@@ -347,130 +768,133 @@ int status_of_last_launch() {
 
 using namespace ct;
 
-static_assert(kGramTile * kGramTile * sizeof(double) == 32768 && sizeof(TableChunk) < 4000, "table");
-static_assert(sizeof(Matrix) == sizeof(ct_muon_matrix), "ct_muon_matrix");
+static_assert(sizeof(Matrix) == sizeof(ct_muon_matrix) && sizeof(Matrix) % 8 == 0, "ct_muon_matrix");
+static_assert(sizeof(TableChunk) < 3600, "kernel arguments");
+static_assert(kKinds == CT_MUON_KINDS, "counts");
 
 extern "C" int ct_muon_plan(ct_muon_matrix *matrices, int64_t count, int32_t *entries, int64_t capacity,
                             int64_t *counts, int64_t *workspace_bytes) {
-    if (count < 0 || count > 0x7fffffff) return -CT_EINVAL_SHAPE;
+    if (count < 0 || count > 1 << 24) return -CT_EINVAL_SHAPE;
     if (!counts || !workspace_bytes || (count && !matrices)) return -CT_EINVAL_POINTER;
     try {
-        std::vector<Item> gram, stage, apply;
-        int64_t doubles = 0, parts = 0;
+        std::vector<Item> items[kKinds];
+        double total = 0.0;
+        auto weight = [](const Shape &s) { return (double)s.width * tiles16(s.r) * (tiles16(s.r) + 1); };
+        Shape s;
         for (int64_t i = 0; i < count; ++i) {
-            Shape s;
             if (!shape_of(matrices[i].rows, matrices[i].cols, s)) return -CT_EINVAL_SHAPE;
-            matrices[i].parts = parts;
-            matrices[i].splits = (int32_t)s.splits;
-            parts += s.pairs * s.splits;
-            const int64_t step = cdiv(cdiv(s.width, s.splits), 16) * 16, tiles = cdiv(s.r, kGramTile);
-            int32_t slot = 0;
-            for (int64_t a = 0; a < tiles; ++a)
-                for (int64_t b = 0; b <= a; ++b)
-                    for (int64_t k = 0; k < s.splits; ++k)
-                        gram.push_back({(int32_t)i, (int32_t)a, (int32_t)b, (int32_t)std::min(s.width, k * step),
-                                        (int32_t)std::min(s.width, (k + 1) * step), slot++, 0, 0});
-            for (int64_t a = 0; a < s.rp / kPad; ++a)
-                for (int64_t b = 0; b <= a; ++b) stage.push_back({(int32_t)i, (int32_t)a, (int32_t)b, 0, 0, 0, 0, 0});
-            for (int64_t c = 0; c < cdiv(s.width, kCols); ++c)
-                apply.push_back({(int32_t)i, (int32_t)c, 0, (int32_t)(c * kCols),
-                                 (int32_t)std::min(s.width, (c + 1) * kCols), 0, 0, 0});
+            if (s.r <= kOnePass) total += weight(s);
         }
-        for (int64_t i = 0; i < count; ++i) matrices[i].parts += cdiv(count * (int64_t)sizeof(Matrix), 32768);
-        // the table first, then the partial tiles, then each matrix's buffers
-        doubles = (parts + cdiv(count * (int64_t)sizeof(Matrix), 32768)) * kGramTile * kGramTile;
+        // the table, then each matrix's partials and buffers, all 16-byte aligned
+        int64_t doubles = cdiv(count * (int64_t)sizeof(Matrix), 16) * 2;
         for (int64_t i = 0; i < count; ++i) {
-            Shape s;
             shape_of(matrices[i].rows, matrices[i].cols, s);
+            plan_matrix((int32_t)i, s, total > 0.0 ? weight(s) / total : 0.0, items, matrices[i].splits);
+            matrices[i].parts = doubles;
+            doubles += matrices[i].splits * part_size(s.r);
             matrices[i].scratch = doubles;
             doubles += scratch_doubles(s);
         }
-        counts[0] = (int64_t)gram.size();
-        counts[1] = (int64_t)stage.size();
-        counts[2] = (int64_t)apply.size();
+        int64_t size = 0;
+        for (int k = 0; k < kKinds; ++k) {
+            counts[k] = (int64_t)items[k].size();
+            if (counts[k] > 0x7fffffff / kGramThreads) return -CT_EINVAL_SHAPE;
+            size += counts[k];
+        }
         *workspace_bytes = doubles * (int64_t)sizeof(double);
-        for (int i = 0; i < 3; ++i)
-            if (counts[i] > 0x7fffffff / kThreads) return -CT_EINVAL_SHAPE;
         if (!entries) return 0;
-        if (capacity < counts[0] + counts[1] + counts[2]) return -CT_EINVAL_WORKSPACE;
+        if (capacity < size) return -CT_EINVAL_WORKSPACE;
         Item *dst = reinterpret_cast<Item *>(entries);
-        dst = std::copy(gram.begin(), gram.end(), dst);
-        dst = std::copy(stage.begin(), stage.end(), dst);
-        std::copy(apply.begin(), apply.end(), dst);
+        for (int k = 0; k < kKinds; ++k) dst = std::copy(items[k].begin(), items[k].end(), dst);
     } catch (...) {
         return (int)hipErrorOutOfMemory;
     }
     return 0;
 }
 
-extern "C" int ct_muon(const ct_muon_matrix *matrices, int64_t count, const int32_t *plan, const int64_t *counts, int32_t dtype,
-                       const ct_muon_options *o, void *workspace, int64_t workspace_bytes, int64_t workspace_needed,
-                       hipStream_t stream) {
+extern "C" int ct_muon(const ct_muon_matrix *matrices, int64_t count, const int32_t *plan, const int64_t *counts,
+                       int32_t dtype, const ct_muon_options *o, void *workspace, int64_t workspace_bytes,
+                       int64_t workspace_needed, hipStream_t stream) {
     if (!counts || !o) return -CT_EINVAL_POINTER;
     if (dtype != CT_F32 && dtype != CT_BF16) return -CT_EINVAL_DTYPE;
-    if (o->steps < 1 || o->steps > 100 || counts[0] < 0 || counts[1] < 0 || counts[2] < 0 || counts[0] > 0x7fffffff ||
-        counts[1] > 0x7fffffff || counts[2] > 0x7fffffff)
-        return -CT_EINVAL_SHAPE;
-    if (count <= 0 || counts[0] == 0) return count < 0 ? -CT_EINVAL_SHAPE : 0;
+    if (o->steps < 1 || o->steps > 100 || count < 0) return -CT_EINVAL_SHAPE;
+    for (int k = 0; k < kKinds; ++k)
+        if (counts[k] < 0 || counts[k] > 0x7fffffff) return -CT_EINVAL_SHAPE;
+    if (count == 0) return 0;
     if (!matrices || !plan || (uintptr_t)plan % 16) return -CT_EINVAL_POINTER;
     for (int64_t i = 0; i < count; ++i)
         if (!matrices[i].param || !matrices[i].grad || (o->update && !matrices[i].momentum)) return -CT_EINVAL_POINTER;
     if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < workspace_needed) return -CT_EINVAL_WORKSPACE;
-    const Matrix *mats = static_cast<const Matrix *>(workspace);
-    const Item *gram = reinterpret_cast<const Item *>(plan), *stage = gram + counts[0], *apply = stage + counts[1];
-    double *ws = static_cast<double *>(workspace);
     Hyper h;
     h.lr = (float)o->lr;
-    h.keep = (float)(1.0 - o->lr * o->weight_decay);
     h.mu = (float)o->momentum;
     h.rest = (float)(1.0 - o->momentum);
+    h.keep = (float)(1.0 - o->lr * o->weight_decay);
     h.nesterov = o->nesterov ? 1 : 0;
     h.step = o->update ? 1 : 0;
     h.a = o->a;
     h.b = o->b;
     h.c = o->c;
     h.eps = o->eps;
-    const dim3 threads(kThreads);
+    const Matrix *mats = static_cast<const Matrix *>(workspace);
+    const Item *items[kKinds];
+    items[0] = reinterpret_cast<const Item *>(plan);
+    for (int k = 1; k < kKinds; ++k) items[k] = items[k - 1] + counts[k - 1];
+    double *ws = static_cast<double *>(workspace);
+    auto grid = [&](int kind, unsigned y = 1) { return dim3((unsigned)counts[kind], y); };
+    const bool half = dtype == CT_BF16;
     int status = 0;
     auto ok = [&]() { return (status = status_of_last_launch()) == 0; };
     for (int64_t i = 0; i < count; i += kTableChunk) {
-        TableChunk chunk;
+        TableChunk chunk = {};
         const int n = (int)std::min<int64_t>(kTableChunk, count - i);
         std::copy_n(reinterpret_cast<const Matrix *>(matrices) + i, n, chunk.m);
         muon_table<<<dim3(1), dim3(64), 0, stream>>>(static_cast<Matrix *>(workspace) + i, chunk, n);
         if (!ok()) return status;
     }
-    if (h.step) {
-        if (dtype == CT_BF16) muon_momentum<uint16_t><<<dim3((unsigned)counts[2]), threads, 0, stream>>>(mats, apply, h);
-        else muon_momentum<float><<<dim3((unsigned)counts[2]), threads, 0, stream>>>(mats, apply, h);
+    if (counts[kItemsGram]) {
+        const auto kernel = half ? muon_gram<uint16_t> : muon_gram<float>;
+        kernel<<<grid(kItemsGram), dim3(kGramThreads), 0, stream>>>(mats, items[kItemsGram], h, ws);
         if (!ok()) return status;
     }
-    if (dtype == CT_BF16) muon_gram<uint16_t><<<dim3((unsigned)counts[0]), threads, 0, stream>>>(mats, gram, h, ws);
-    else muon_gram<float><<<dim3((unsigned)counts[0]), threads, 0, stream>>>(mats, gram, h, ws);
-    if (!ok()) return status;
-    muon_join<<<dim3((unsigned)counts[1]), threads, 0, stream>>>(mats, stage, h, ws);
-    if (!ok()) return status;
-    const dim3 one((unsigned)counts[1], 1), two((unsigned)counts[1], 2);
-    int q = kP;   // the product of the P so far
-    for (int i = 0; i < o->steps; ++i) {
-        const bool first = i == 0, last = i + 1 == o->steps;
-        // the first P is the first Q and is not overwritten before the second step has read it
-        const int p = first ? kQ : kP;
-        muon_stage<<<one, threads, 0, stream>>>(mats, stage, h, ws, {kMakeP, kG, kG, p, first && last}, {});
-        if (!ok()) return status;
-        const int next = q == kQ ? kQ + 1 : kQ;
-        const StageOp extend = {kMultiply, p, q, next, last}, shift = {kMultiply, p, kG, kT, 0};
-        if (!last) {
-            muon_stage<<<first ? one : two, threads, 0, stream>>>(mats, stage, h, ws, shift, extend);
+    if (counts[kItemsTiles]) {
+        if (h.step) {
+            const auto kernel = half ? muon_momentum<uint16_t> : muon_momentum<float>;
+            kernel<<<grid(kItemsMomentum), dim3(kThreads), 0, stream>>>(mats, items[kItemsMomentum], h);
             if (!ok()) return status;
-            muon_stage<<<one, threads, 0, stream>>>(mats, stage, h, ws, {kMultiply, p, kT, kG, 0}, {});
-        } else if (!first) {
-            muon_stage<<<one, threads, 0, stream>>>(mats, stage, h, ws, extend, {});
         }
+        const auto kernel = half ? muon_gram_tiles<uint16_t> : muon_gram_tiles<float>;
+        kernel<<<grid(kItemsTiles), dim3(kThreads), 0, stream>>>(mats, items[kItemsTiles], h, ws);
         if (!ok()) return status;
-        q = first ? kQ : next;
     }
-    if (dtype == CT_BF16) muon_apply<uint16_t><<<dim3((unsigned)counts[2]), threads, 0, stream>>>(mats, apply, h, ws);
-    else muon_apply<float><<<dim3((unsigned)counts[2]), threads, 0, stream>>>(mats, apply, h, ws);
+    if (counts[kItemsSmall]) {
+        muon_small<<<grid(kItemsSmall), dim3(kThreads), 0, stream>>>(mats, items[kItemsSmall], h, ws, o->steps);
+        if (!ok()) return status;
+    }
+    if (counts[kItemsStage]) {
+        muon_join<<<grid(kItemsJoin), dim3(kThreads), 0, stream>>>(mats, items[kItemsJoin], h, ws);
+        if (!ok()) return status;
+        auto stage = [&](const StageOp &op0, const StageOp *op1) {
+            muon_stage<<<grid(kItemsStage, op1 ? 2 : 1), dim3(kThreads), 0, stream>>>(mats, items[kItemsStage], h, ws,
+                                                                                     op0, op1 ? *op1 : op0);
+            return ok();
+        };
+        int q = kQ;   // the product of the P so far; the first P is the first Q
+        for (int i = 0; i < o->steps; ++i) {
+            const bool first = i == 0, last = i + 1 == o->steps;
+            const int p = first ? kQ : kP, next = q == kQ ? kQ + 1 : kQ;
+            if (!stage({kMakeP, kG, kG, p, first && last}, nullptr)) return status;
+            const StageOp extend = {kMultiply, p, q, next, last};
+            if (!last) {
+                if (!stage({kMultiply, p, kG, kT, 0}, first ? nullptr : &extend)) return status;
+                if (!stage({kMultiply, p, kT, kG, 0}, nullptr)) return status;
+            } else if (!first) {
+                if (!stage(extend, nullptr)) return status;
+            }
+            if (!first) q = next;
+        }
+    }
+    const auto kernel = half ? muon_apply<uint16_t> : muon_apply<float>;
+    kernel<<<grid(kItemsApply), dim3(kApplyThreads), 0, stream>>>(mats, items[kItemsApply], h, ws);
     return status_of_last_launch();
 }

@@ -594,6 +594,8 @@ int ct_attention_backward(const ct_attention *attention, const int32_t *row_plan
  * The iteration runs in double on the short side's Gram matrix, the last product in float32;
  * results are rounded once. Sums run in a fixed order.
  */
+#define CT_MUON_KINDS 7
+
 typedef struct ct_muon_matrix {
     void *param;
     const void *grad;
@@ -615,10 +617,10 @@ typedef struct ct_muon_options {
 
 /*
  * The work over `count` matrices (host table, whose scratch, parts and splits are filled in),
- * cut into workgroups' shares: 32-byte entries of three kinds, counts[0..2], and the bytes of
- * workspace. With entries = null only counts, the table and workspace_bytes are written. The
- * caller copies the entries to the device (16-byte aligned); they hold for every call with
- * these shapes. Empty matrices are refused: the caller leaves them out. ct_muon reads the
+ * cut into workgroups' shares: 32-byte entries of CT_MUON_KINDS kinds, counts[0 ..
+ * CT_MUON_KINDS - 1] of them one kind after the other, and the bytes of workspace. With
+ * entries = null only counts, the table and workspace_bytes are written. The caller copies the
+ * entries to the device (16-byte aligned); they hold for every call with these shapes. Empty matrices are refused: the caller leaves them out. ct_muon reads the
  * host table while it runs and passes it to the device in kernel arguments.
  */
 int ct_muon_plan(ct_muon_matrix *matrices, int64_t count, int32_t *entries, int64_t capacity, int64_t *counts,
