@@ -151,10 +151,13 @@ __device__ __forceinline__ f64x4 mfma_f64(double a, double b, f64x4 c) {
 // ------------------------------------------------------------------ Gram matrix, one pass
 // A workgroup of 8 waves reads its range of the long side once, with every row of the short
 // side, updates the momentum there, and holds the lower triangle of its partial Gram matrix
-// in registers: NT tiles of 16 rows, strips w and NT - 1 - w to one wave (NT + 1 tiles
-// each); where that takes fewer than 8 waves, groups of waves share out the k-steps and
-// leave partials of their own. Reading M once costs 12 bytes an element (4 in orthogonalize);
-// the products, 64 cycles for 16 x 16 x 4, bound it from rank 256 on.
+// in registers, in blocks of 64 x 64: a wave has one block below the diagonal (16 tiles of 16 x
+// 16 from 8 operand reads) or two on it (2 x 10 tiles). With 256 rows that makes 6 + 2 waves,
+// 36 tiles on the fullest SIMD of 34 on average; with fewer rows groups of 2 waves or single
+// waves share out the k-steps and add their sums in LDS at the end. (One strip of tiles from
+// each end of the triangle per wave is even, but takes 19 operand reads and conversions for 17
+// products: 281 against ... us over two layers' adapters.) Reading M once costs 12 bytes an
+// element (4 in orthogonalize); the products, 64 cycles for 16 x 16 x 4, bound it from rank 256 on.
 constexpr int kGramThreads = 512;
 
 struct Four {
@@ -165,14 +168,19 @@ template <typename T, int NT, bool TALL>
 __device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, const Hyper &h, double *ws, float *lds) {
     constexpr int kRows = 16 * NT, kUnits = kRows * kChunk / 4;
     constexpr int kPasses = (kUnits + kGramThreads - 1) / kGramThreads;
-    constexpr int kPitch = TALL ? (NT == 1 ? 16 : kRows + 16) : kChunk + 4;
+    constexpr int kPitch = TALL ? kRows + 16 : kChunk + 4;
     constexpr int kStage = TALL ? kPitch * kChunk : kPitch * kRows;
-    constexpr int kWaves = NT < 2 ? 1 : NT / 2, kGroups = 8 / kWaves;
+    constexpr int kWaves = NT == 16 ? 8 : NT == 8 ? 2 : 1, kGroups = 8 / kWaves, kMost = 20;
     const int r = short_side(m), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int w = wave % kWaves, group = wave / kWaves, top = NT - 1 - w;
+    const int w = wave % kWaves, group = wave / kWaves;
+    // Blocks (bi, bj) below the diagonal: (1, 0), (2, 0), (2, 1), (3, 0), ...; or bi = bj and bi + 1.
+    constexpr int kBelow = NT == 16 ? 6 : NT == 8 ? 1 : 0;
+    const bool below = w < kBelow;
+    const int bi = below ? (w < 1 ? 1 : w < 3 ? 2 : 3) : 2 * (w - kBelow);
+    const int bj = below ? w - bi * (bi - 1) / 2 : bi;
     const bool four = by_four<T>(m, h.step);
     const int64_t cols = m.cols;
-    f64x4 acc[NT + 1] = {};
+    f64x4 acc[kMost] = {};
     double norm = 0.0;
     Four held[kPasses];
 
@@ -249,17 +257,50 @@ __device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, c
         if (more) load(k0 + kChunk);
         const float *stage = lds + buf * kStage + (TALL ? (lane >> 4) * kPitch + (lane & 15)
                                                         : (lane & 15) * kPitch + (lane >> 4));
-        auto at = [&](int tile, int step) -> double {
-            return stage[tile * (TALL ? 16 : 16 * kPitch) + step * (TALL ? 4 * kPitch : 4)];
+        // operands x of the first block's rows and y of the second's (or of the next diagonal block)
+        const float *xs = stage + 4 * bi * (TALL ? 16 : 16 * kPitch);
+        const float *ys = stage + 4 * (below ? bj : bi + 1) * (TALL ? 16 : 16 * kPitch);
+        constexpr bool kSecond = NT > 4;
+        float xn[4], yn[4] = {};
+        auto fetch = [&](int step) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int at = t * (TALL ? 16 : 16 * kPitch) + step * (TALL ? 4 * kPitch : 4);
+                if (t < NT) xn[t] = xs[at];
+                if constexpr (kSecond) yn[t] = ys[at];
+            }
         };
+        fetch(group);
 #pragma unroll 1
         for (int step = group; step < kChunk / 4; step += kGroups) {
-            const double high = at(top, step), low = at(NT < 2 ? 0 : w, step);
+            double x[4], y[4];
 #pragma unroll
-            for (int t = 0; t <= NT; ++t) {   // tiles 0 .. top of strip top, then w .. 0 of strip w
-                if (NT == 1 && t == 1) break;
-                const bool upper = t <= top;
-                acc[t] = mfma_f64(upper ? high : low, at(upper ? t : NT - t, step), acc[t]);
+            for (int t = 0; t < 4; ++t) {
+                x[t] = xn[t];
+                y[t] = yn[t];
+            }
+            if (step + kGroups < kChunk / 4) fetch(step + kGroups);
+            if (below) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (64 * bi + 16 * i < r)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[4 * i + j] = mfma_f64(x[i], y[j], acc[4 * i + j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < (NT < 4 ? NT : 4); ++i)
+                    if (64 * bi + 16 * i < r)
+#pragma unroll
+                        for (int j = 0; j <= i; ++j)
+                            acc[i * (i + 1) / 2 + j] = mfma_f64(x[i], x[j], acc[i * (i + 1) / 2 + j]);
+                if constexpr (kSecond) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (64 * (bi + 1) + 16 * i < r)
+#pragma unroll
+                            for (int j = 0; j <= i; ++j)
+                                acc[10 + i * (i + 1) / 2 + j] = mfma_f64(y[i], y[j], acc[10 + i * (i + 1) / 2 + j]);
+                }
             }
         }
         if (more) store(k0 + kChunk, lds + (buf ^ 1) * kStage);
@@ -274,28 +315,58 @@ __device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, c
         if (tid < n) sums[tid] += sums[tid + n];
         __syncthreads();
     }
-    double *part = part_of(m, ws, it.slot * kGroups + group);
-    if (lane == 0 && w == 0) part[0] = group ? 0.0 : sums[0];
-    double *tiles = part + part_head(r);
+    double *part = part_of(m, ws, it.slot);
+    if (tid == 0) part[0] = sums[0];
+    // the groups' sums, in order, into the first group's registers
+    constexpr int kTiles = NT == 1 ? 1 : NT == 2 ? 3 : NT == 4 ? 10 : kMost;
+    static_assert(kGroups == 1 || (16 * kBelow + kTiles) * 2048 <= 2 * (kChunk + 4) * kOnePass * 4, "LDS");
+    const int mine = below ? 16 : kTiles;
+    double *shared = sums + (below ? 16 * w : 16 * kBelow) * 256 + lane;
+    for (int g = 1; g < kGroups; ++g) {
+        __syncthreads();
+        if (group == g) {
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+                if (t < mine)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) shared[t * 256 + e * 64] = acc[t][e];
+        }
+        __syncthreads();
+        if (group == 0) {
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+                if (t < mine)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[t][e] += shared[t * 256 + e * 64];
+        }
+    }
+    if (group) return;
+    double *tiles = part + part_head(r) + (lane >> 4) * 16 + (lane & 15);
     const int have = tiles16(r);
+    auto write = [&](int i, int j, const f64x4 &v) {
+        if (i >= have) return;
 #pragma unroll
-    for (int t = 0; t <= NT; ++t) {
-        if (NT == 1 && t == 1) break;
-        const bool upper = t <= top;
-        const int i = upper ? top : w, j = upper ? t : NT - t;
-        if (i >= have) continue;
+        for (int e = 0; e < 4; ++e) tiles[tile_of(i, j) + 64 * e] = v[e];
+    };
+    if (below) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) tiles[tile_of(i, j) + (4 * e + (lane >> 4)) * 16 + (lane & 15)] = acc[t][e];
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) write(4 * bi + i, 4 * bj + j, acc[4 * i + j]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j <= i; ++j) {
+                write(4 * bi + i, 4 * bi + j, acc[i * (i + 1) / 2 + j]);
+                if constexpr (NT > 4) write(4 * bi + 4 + i, 4 * bi + 4 + j, acc[10 + i * (i + 1) / 2 + j]);
+            }
     }
 }
 
 // NT for a short side: tiles of 16 rows, rounded up to a power of two.
 __host__ __device__ __forceinline__ int one_pass_tiles(int r) {
     return r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : r <= 128 ? 8 : 16;
-}
-__host__ __forceinline__ int one_pass_groups(int r) {
-    const int nt = one_pass_tiles(r);
-    return nt < 2 ? 8 : 16 / nt;
 }
 
 template <typename T, bool TALL>
@@ -391,12 +462,13 @@ __global__ __launch_bounds__(kThreads) void muon_gram_tiles(const Matrix *matric
     }
 }
 
-// 1 / max(|M|, eps) from the parts' squared norms, in order.
+// 1 / max(|M|, eps) from the parts' squared norms: every wave for itself, in one fixed order.
 __device__ __forceinline__ double inverse_norm(const Matrix &m, double *ws, double eps) {
-    const int r = short_side(m), n = r <= kOnePass ? 1 : (r + kGramTile - 1) / kGramTile;
+    const int r = short_side(m), heads = r <= kOnePass ? 1 : (r + kGramTile - 1) / kGramTile;
     double sum = 0.0;
-    for (int s = 0; s < m.splits; ++s)
-        for (int e = 0; e < n; ++e) sum += part_of(m, ws, s)[e];
+    for (int i = threadIdx.x & 63; i < m.splits * heads; i += 64) sum += part_of(m, ws, i / heads)[i % heads];
+#pragma unroll
+    for (int n = 32; n; n >>= 1) sum += __shfl_xor(sum, n, 64);
     const double norm = sqrt(sum);
     return 1.0 / (norm < eps ? eps : norm);
 }
@@ -406,6 +478,7 @@ __device__ __forceinline__ double join_tile(const Matrix &m, double *ws, int i, 
     const double *p = part_of(m, ws, 0) + part_head(short_side(m)) + tile_of(i, j) + e;
     const int64_t step = part_size(short_side(m));
     double v = 0.0;
+#pragma unroll 8
     for (int s = 0; s < m.splits; ++s) v += p[s * step];
     return v;
 }
@@ -507,49 +580,61 @@ struct StageOp {
 
 // One 32 x 32 tile (i >= j) of left right, both symmetric and commuting, so their product is
 // symmetric too and the tile's mirror image is its transpose. kMakeP: a I + b G + c G G. Each
-// of the 4 waves takes a quarter of the reduction over the whole tile (one load per product
-// instead of two) straight from L2, operand rows read along k's rows (symmetry), and the
-// quarters are added in LDS in order.
-__global__ __launch_bounds__(kThreads) void muon_stage(const Matrix *matrices, const Item *items, Hyper h, double *ws,
-                                                      StageOp op0, StageOp op1) {
-    constexpr int kPitch = kPad + 1;
+// of the 8 waves takes an eighth of the reduction over the whole tile (one load per product
+// instead of two) straight from L2, all loads of up to 8 k-steps in flight at once, operand
+// rows read along k's rows (symmetry), and the sums are added in LDS in order.
+constexpr int kStageThreads = 512;
+
+__global__ __launch_bounds__(kStageThreads) void muon_stage(const Matrix *matrices, const Item *items, Hyper h,
+                                                           double *ws, StageOp op0, StageOp op1) {
+    constexpr int kPitch = kPad + 1, kSteps = 8;
     __shared__ double sums[4][kPad * kPitch];
     const StageOp op = blockIdx.y ? op1 : op0;
     const Item it = items[blockIdx.x];
+    if (it.matrix < 0) return;
     const Matrix m = matrices[it.matrix];
     const int r = short_side(m), rp = padded(r), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const double *left = buffer(m, ws, op.left) + it.i * kPad + (lane & 15) + (int64_t)(lane >> 4) * rp;
-    const double *right = buffer(m, ws, op.right) + it.j * kPad + (lane & 15) + (int64_t)(lane >> 4) * rp;
+    const int64_t lane_at = (lane & 15) + (int64_t)(lane >> 4) * rp;
+    const double *left = buffer(m, ws, op.left) + it.i * kPad + lane_at;
+    const double *right = buffer(m, ws, op.right) + it.j * kPad + lane_at;
     f64x4 acc[2][2] = {};
-    // rp is a multiple of 32: a quarter is a multiple of 8 rows
-    const int64_t first = (int64_t)wave * (rp / 4) * rp, step = 4 * (int64_t)rp;
-    const double *a = left + first, *b = right + first;
-    for (int k = 0; k < rp / 4; k += 8) {
-        double x[2][2], y[2][2];
+    const int steps = rp / 32, first = wave * steps;   // k-steps of 4 rows
+    for (int s0 = 0; s0 < steps; s0 += kSteps) {
+        double x[kSteps][2], y[kSteps][2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < kSteps; ++u)
+            if (s0 + u < steps) {
+                const int64_t at = (int64_t)(first + s0 + u) * 4 * rp;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                x[u][t] = a[u * step + 16 * t];
-                y[u][t] = b[u * step + 16 * t];
+                for (int t = 0; t < 2; ++t) {
+                    x[u][t] = left[at + 16 * t];
+                    y[u][t] = right[at + 16 * t];
+                }
             }
-        a += 2 * step;
-        b += 2 * step;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < kSteps; ++u)
+            if (s0 + u < steps)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[i][j] = mfma_f64(x[u][i], y[u][j], acc[i][j]);
+    }
+    // waves 4 - 7, then 0 - 3 on top of them
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+        if (wave >> 2 != pass) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = mfma_f64(x[u][i], y[u][j], acc[i][j]);
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        double *dst = &sums[wave & 3][(16 * i + 4 * e + (lane >> 4)) * kPitch + 16 * j + (lane & 15)];
+                        *dst = pass ? *dst + acc[i][j][e] : acc[i][j][e];
+                    }
+        }
+        __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                sums[wave][(16 * i + 4 * e + (lane >> 4)) * kPitch + 16 * j + (lane & 15)] = acc[i][j][e];
-    __syncthreads();
     const double inv = op.last ? ws[m.scratch] : 1.0;
     const double *g = buffer(m, ws, op.left);
     double *dst = buffer(m, ws, op.dst);
@@ -564,7 +649,7 @@ __global__ __launch_bounds__(kThreads) void muon_stage(const Matrix *matrices, c
         }
         return v;
     };
-    for (int e = threadIdx.x; e < kPad * kPad; e += kThreads) {
+    for (int e = threadIdx.x; e < kPad * kPad; e += kStageThreads) {
         const int row = e / kPad, col = e % kPad;
         // (row, col) of the tile itself, then of its mirror image, both stored along rows
         const double v = it.i == it.j && row < col ? value(col, row) : value(row, col);
@@ -717,6 +802,19 @@ bool shape_of(int64_t rows, int64_t cols, Shape &s) {
     return true;
 }
 
+// Workgroups go to the 8 XCDs in turn: hands each XCD one run of neighbouring items, so that
+// what they share stays in its L2. Padded with items of no matrix to whole turns.
+void by_xcd(std::vector<Item> &items) {
+    constexpr int64_t kXcds = 8;
+    const int64_t n = (int64_t)items.size(), run = cdiv(n, kXcds);
+    std::vector<Item> ordered((size_t)(run * kXcds), Item{-1, 0, 0, 0, 0, 0, 0, 0});
+    for (int64_t x = 0, from = 0; x < kXcds; ++x) {
+        const int64_t to = n * (x + 1) / kXcds;
+        for (int64_t k = 0; from < to; ++k, ++from) ordered[(size_t)(k * kXcds + x)] = items[(size_t)from];
+    }
+    items.swap(ordered);
+}
+
 int64_t scratch_doubles(const Shape &s) {
     const int64_t square = (int64_t)s.rp * s.rp;
     return 2 + (s.r <= kSmall ? 0 : kBuffers * square) + square / 2;
@@ -727,20 +825,47 @@ int status_of_last_launch() {
     return e == hipSuccess ? 0 : (int)e;
 }
 
-// A matrix's items and partials, whose Gram products are `share` of kGroupsWanted workgroups.
-void plan_matrix(int32_t index, const Shape &s, double share, std::vector<Item> (&items)[kKinds], int32_t &splits) {
-    const int64_t most = cdiv(s.width, 2 * kChunk);
-    const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(most, (int64_t)(share * kGroupsWanted + 0.5)));
+// Cost of a chunk of the long side in the one-pass Gram kernel, in its unit of time: a tile's
+// product on one of four SIMDs, and no less than about 4 for reading the chunk.
+int64_t chunk_cost(int r) {
+    const int64_t t = one_pass_tiles(r);
+    return std::max<int64_t>(4, t * (t + 1) / 2);
+}
+
+// Long-side elements per workgroup so that none takes longer than `cap`, in whole chunks; at
+// least two, which pays for the partial result.
+int64_t gram_step(int r, int64_t cap) { return std::max<int64_t>(2, cap / chunk_cost(r)) * kChunk; }
+
+// The smallest cap with which all the one-pass Gram items run at once.
+int64_t gram_cap(const std::vector<Shape> &shapes) {
+    int64_t low = 1, high = 1;
+    auto fits = [&](int64_t cap) {
+        int64_t n = 0;
+        for (const Shape &s : shapes)
+            if (s.r <= kOnePass) n += cdiv(s.width, gram_step(s.r, cap));
+        return n <= std::max<int64_t>(kGroupsWanted, (int64_t)shapes.size());
+    };
+    while (!fits(high) && high < (int64_t)1 << 40) high *= 2;
+    while (low < high) {
+        const int64_t mid = (low + high) / 2;
+        if (fits(mid)) high = mid;
+        else low = mid + 1;
+    }
+    return high;
+}
+
+// A matrix's items and its number of partial Gram matrices.
+void plan_matrix(int32_t index, const Shape &s, int64_t cap, std::vector<Item> (&items)[kKinds], int32_t &splits) {
     const bool one_pass = s.r <= kOnePass;
-    const int64_t parts = one_pass ? wanted : std::max<int64_t>(1, std::min<int64_t>(cdiv(s.width, 512), 32));
-    const int64_t step = cdiv(cdiv(s.width, parts), kChunk) * kChunk;
+    const int64_t parts = one_pass ? cdiv(s.width, gram_step(s.r, cap))
+                                   : std::max<int64_t>(1, std::min<int64_t>(cdiv(s.width, 512), 32));
+    const int64_t step = cdiv(cdiv(s.width, parts), kChunk) * kChunk;   // even parts
     const int64_t count = cdiv(s.width, step);
     auto range = [&](int64_t k, int32_t i, int32_t j) -> Item {
         return {index, i, j, (int32_t)(k * step), (int32_t)std::min(s.width, (k + 1) * step), (int32_t)k, 0, 0};
     };
     if (one_pass) {
         for (int64_t k = 0; k < count; ++k) items[kItemsGram].push_back(range(k, 0, 0));
-        splits = (int32_t)count * one_pass_groups(s.r);
     } else {
         const int tiles = (s.r + kGramTile - 1) / kGramTile;
         for (int64_t k = 0; k < count; ++k)
@@ -748,8 +873,8 @@ void plan_matrix(int32_t index, const Shape &s, double share, std::vector<Item> 
                 for (int b = 0; b <= a; ++b) items[kItemsTiles].push_back(range(k, a, b));
         for (int64_t c = 0; c < s.width; c += 64)
             items[kItemsMomentum].push_back({index, 0, 0, (int32_t)c, (int32_t)std::min(s.width, c + 64), 0, 0, 0});
-        splits = (int32_t)count;
     }
+    splits = (int32_t)count;
     if (s.r <= kSmall) {
         items[kItemsSmall].push_back({index, 0, 0, 0, 0, 0, 0, 0});
     } else {
@@ -778,23 +903,21 @@ extern "C" int ct_muon_plan(ct_muon_matrix *matrices, int64_t count, int32_t *en
     if (!counts || !workspace_bytes || (count && !matrices)) return -CT_EINVAL_POINTER;
     try {
         std::vector<Item> items[kKinds];
-        double total = 0.0;
-        auto weight = [](const Shape &s) { return (double)s.width * tiles16(s.r) * (tiles16(s.r) + 1); };
-        Shape s;
-        for (int64_t i = 0; i < count; ++i) {
-            if (!shape_of(matrices[i].rows, matrices[i].cols, s)) return -CT_EINVAL_SHAPE;
-            if (s.r <= kOnePass) total += weight(s);
-        }
+        std::vector<Shape> shapes((size_t)count);
+        for (int64_t i = 0; i < count; ++i)
+            if (!shape_of(matrices[i].rows, matrices[i].cols, shapes[(size_t)i])) return -CT_EINVAL_SHAPE;
+        const int64_t cap = gram_cap(shapes);
         // the table, then each matrix's partials and buffers, all 16-byte aligned
         int64_t doubles = cdiv(count * (int64_t)sizeof(Matrix), 16) * 2;
         for (int64_t i = 0; i < count; ++i) {
-            shape_of(matrices[i].rows, matrices[i].cols, s);
-            plan_matrix((int32_t)i, s, total > 0.0 ? weight(s) / total : 0.0, items, matrices[i].splits);
+            const Shape &s = shapes[(size_t)i];
+            plan_matrix((int32_t)i, s, cap, items, matrices[i].splits);
             matrices[i].parts = doubles;
             doubles += matrices[i].splits * part_size(s.r);
             matrices[i].scratch = doubles;
             doubles += scratch_doubles(s);
         }
+        by_xcd(items[kItemsStage]);
         int64_t size = 0;
         for (int k = 0; k < kKinds; ++k) {
             counts[k] = (int64_t)items[k].size();
@@ -875,7 +998,7 @@ extern "C" int ct_muon(const ct_muon_matrix *matrices, int64_t count, const int3
         muon_join<<<grid(kItemsJoin), dim3(kThreads), 0, stream>>>(mats, items[kItemsJoin], h, ws);
         if (!ok()) return status;
         auto stage = [&](const StageOp &op0, const StageOp *op1) {
-            muon_stage<<<grid(kItemsStage, op1 ? 2 : 1), dim3(kThreads), 0, stream>>>(mats, items[kItemsStage], h, ws,
+            muon_stage<<<grid(kItemsStage, op1 ? 2 : 1), dim3(kStageThreads), 0, stream>>>(mats, items[kItemsStage], h, ws,
                                                                                      op0, op1 ? *op1 : op0);
             return ok();
         };
