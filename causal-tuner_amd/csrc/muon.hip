@@ -154,21 +154,21 @@ __device__ __forceinline__ f64x4 mfma_f64(double a, double b, f64x4 c) {
 // in registers, in blocks of 64 x 64: a wave has one block below the diagonal (16 tiles of 16 x
 // 16 from 8 operand reads) or two on it (2 x 10 tiles). With 256 rows that makes 6 + 2 waves,
 // 36 tiles on the fullest SIMD of 34 on average; with fewer rows groups of 2 waves or single
-// waves share out the k-steps and add their sums in LDS at the end. (One strip of tiles from
-// each end of the triangle per wave is even, but takes 19 operand reads and conversions for 17
-// products: 281 against ... us over two layers' adapters.) Reading M once costs 12 bytes an
+// waves share out the k-steps and add their sums in LDS at the end. M goes to LDS as doubles: converting
+// at the operand reads does it four times over, in the pipe that the products need. Reading M once costs 12 bytes an
 // element (4 in orthogonalize); the products, 64 cycles for 16 x 16 x 4, bound it from rank 256 on.
 constexpr int kGramThreads = 512;
+constexpr int kGramLds = 2 * kChunk * (kOnePass + 16);   // doubles: two stages, 139 KB
 
 struct Four {
     float4 g, m;
 };
 
 template <typename T, int NT, bool TALL>
-__device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, const Hyper &h, double *ws, float *lds) {
+__device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, const Hyper &h, double *ws, double *lds) {
     constexpr int kRows = 16 * NT, kUnits = kRows * kChunk / 4;
     constexpr int kPasses = (kUnits + kGramThreads - 1) / kGramThreads;
-    constexpr int kPitch = TALL ? kRows + 16 : kChunk + 4;
+    constexpr int kPitch = TALL ? kRows + 16 : kChunk + 2;
     constexpr int kStage = TALL ? kPitch * kChunk : kPitch * kRows;
     constexpr int kWaves = NT == 16 ? 8 : NT == 8 ? 2 : 1, kGroups = 8 / kWaves, kMost = 20;
     const int r = short_side(m), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -181,30 +181,27 @@ __device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, c
     const bool four = by_four<T>(m, h.step);
     const int64_t cols = m.cols;
     f64x4 acc[kMost] = {};
-    double norm = 0.0;
     Four held[kPasses];
 
-    // element (s, l) of a unit: four along the stored rows
-    auto place = [&](int p, int &s, int &l) -> bool {
-        const int u = p * kGramThreads + tid;
-        if (kUnits % kGramThreads && u >= kUnits) return false;
-        if constexpr (TALL) {
-            s = u % (kRows / 4) * 4;
-            l = u / (kRows / 4);
-        } else {
-            s = u / (kChunk / 4);
-            l = u % (kChunk / 4) * 4;
-        }
-        return true;
+    // A unit is four elements along a stored row; a thread's units are `gap` rows apart.
+    constexpr int kRowUnits = TALL ? kRows / 4 : kChunk / 4, kGap = kGramThreads / kRowUnits;
+    const bool active = kUnits >= kGramThreads || tid < kUnits;
+    const int along = tid % kRowUnits * 4, across = tid / kRowUnits;
+    const int64_t gap = kGap * (TALL ? (int64_t)r : cols);
+    int64_t at0 = TALL ? (int64_t)(it.lo + across) * r + along : (int64_t)across * cols + it.lo + along;
+    const int64_t next_chunk = TALL ? (int64_t)kChunk * r : kChunk;
+    // elements of unit p inside the matrix and the range, in the chunk at k0
+    auto left_of = [&](int p, int k0) -> int {
+        const int row = across + p * kGap;
+        return TALL ? (k0 + row < it.hi ? r - along : 0) : (row < r ? it.hi - k0 - along : 0);
     };
     auto load = [&](int k0) {
 #pragma unroll
         for (int p = 0; p < kPasses; ++p) {
-            int s, l;
             held[p] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
-            if (!place(p, s, l)) continue;
-            const int64_t at = TALL ? (int64_t)(k0 + l) * r + s : (int64_t)s * cols + k0 + l;
-            const int left = TALL ? (k0 + l < it.hi ? r - s : 0) : (s < r ? it.hi - k0 - l : 0);
+            if (!active) continue;
+            const int64_t at = at0 + p * gap;
+            const int left = left_of(p, k0);
             if (four && left >= 4) {
                 held[p].g = load_four<T>(m.grad, at);
                 if (h.step) held[p].m = *reinterpret_cast<const float4 *>(m.momentum + at);
@@ -219,15 +216,14 @@ __device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, c
             }
         }
     };
-    auto store = [&](int k0, float *stage) {
+    auto store = [&](int k0, double *stage) {
 #pragma unroll
         for (int p = 0; p < kPasses; ++p) {
-            int s, l;
-            if (!place(p, s, l)) continue;
+            if (!active) continue;
             float *g = &held[p].g.x, *v = &held[p].m.x;
             if (h.step) {
-                const int64_t at = TALL ? (int64_t)(k0 + l) * r + s : (int64_t)s * cols + k0 + l;
-                const int left = TALL ? (k0 + l < it.hi ? r - s : 0) : (s < r ? it.hi - k0 - l : 0);
+                const int64_t at = at0 + p * gap;
+                const int left = left_of(p, k0);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(h.mu, v[e], h.rest * g[e]);
                 if (four && left >= 4) {
@@ -240,10 +236,12 @@ __device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, c
 #pragma unroll
                 for (int e = 0; e < 4; ++e) g[e] = combine(h, g[e], v[e]);
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) norm = __builtin_fma((double)g[e], (double)g[e], norm);
-            *reinterpret_cast<float4 *>(stage + (TALL ? l * kPitch + s : s * kPitch + l)) = held[p].g;
+            const int row = across + p * kGap;
+            double2 *dst = reinterpret_cast<double2 *>(stage + row * kPitch + along);
+            dst[0] = make_double2(g[0], g[1]);
+            dst[1] = make_double2(g[2], g[3]);
         }
+        at0 += next_chunk;
     };
 
     int buf = 0;
@@ -255,31 +253,21 @@ __device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, c
     for (int k0 = it.lo; k0 < it.hi; k0 += kChunk) {
         const bool more = k0 + kChunk < it.hi;
         if (more) load(k0 + kChunk);
-        const float *stage = lds + buf * kStage + (TALL ? (lane >> 4) * kPitch + (lane & 15)
-                                                        : (lane & 15) * kPitch + (lane >> 4));
+        const double *stage = lds + buf * kStage + (TALL ? (lane >> 4) * kPitch + (lane & 15)
+                                                         : (lane & 15) * kPitch + (lane >> 4));
         // operands x of the first block's rows and y of the second's (or of the next diagonal block)
-        const float *xs = stage + 4 * bi * (TALL ? 16 : 16 * kPitch);
-        const float *ys = stage + 4 * (below ? bj : bi + 1) * (TALL ? 16 : 16 * kPitch);
+        const double *xs = stage + 4 * bi * (TALL ? 16 : 16 * kPitch);
+        const double *ys = stage + 4 * (below ? bj : bi + 1) * (TALL ? 16 : 16 * kPitch);
         constexpr bool kSecond = NT > 4;
-        float xn[4], yn[4] = {};
-        auto fetch = [&](int step) {
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int at = t * (TALL ? 16 : 16 * kPitch) + step * (TALL ? 4 * kPitch : 4);
-                if (t < NT) xn[t] = xs[at];
-                if constexpr (kSecond) yn[t] = ys[at];
-            }
-        };
-        fetch(group);
 #pragma unroll 1
         for (int step = group; step < kChunk / 4; step += kGroups) {
             double x[4], y[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                x[t] = xn[t];
-                y[t] = yn[t];
+                const int at = t * (TALL ? 16 : 16 * kPitch) + step * (TALL ? 4 * kPitch : 4);
+                if (t < NT) x[t] = xs[at];
+                if constexpr (kSecond) y[t] = ys[at];
             }
-            if (step + kGroups < kChunk / 4) fetch(step + kGroups);
             if (below) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -308,7 +296,19 @@ __device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, c
         buf ^= 1;
     }
 
-    double *sums = reinterpret_cast<double *>(lds);
+    // the squared norm is the trace
+    double norm = 0.0;
+    if (!below) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (4 * e + (lane >> 4) == (lane & 15)) {
+                    norm += acc[i * (i + 1) / 2 + i][e];
+                    if constexpr (NT > 4) norm += acc[10 + i * (i + 1) / 2 + i][e];
+                }
+    }
+    double *sums = lds;
     sums[tid] = norm;
     __syncthreads();
     for (int n = kGramThreads / 2; n; n >>= 1) {
@@ -317,49 +317,48 @@ __device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, c
     }
     double *part = part_of(m, ws, it.slot);
     if (tid == 0) part[0] = sums[0];
-    // the groups' sums, in order, into the first group's registers
+    __syncthreads();
+    // the groups' sums, one group after the other, in LDS
     constexpr int kTiles = NT == 1 ? 1 : NT == 2 ? 3 : NT == 4 ? 10 : kMost;
-    static_assert(kGroups == 1 || (16 * kBelow + kTiles) * 2048 <= 2 * (kChunk + 4) * kOnePass * 4, "LDS");
-    const int mine = below ? 16 : kTiles;
+    static_assert(kGroups == 1 || (16 * kBelow + kTiles) * 256 <= kGramLds, "LDS");
+    static_assert(2 * kStage <= kGramLds && kGramThreads <= kGramLds, "LDS");
     double *shared = sums + (below ? 16 * w : 16 * kBelow) * 256 + lane;
-    for (int g = 1; g < kGroups; ++g) {
-        __syncthreads();
-        if (group == g) {
+    if constexpr (kGroups > 1) {
+#pragma unroll 1
+        for (int g = 0; g < kGroups; ++g) {
+            if (group == g) {
 #pragma unroll
-            for (int t = 0; t < kTiles; ++t)
-                if (t < mine)
+                for (int t = 0; t < kTiles; ++t)
+                    if (t < 16 || !below)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) shared[t * 256 + e * 64] = acc[t][e];
+                        for (int e = 0; e < 4; ++e) {
+                            double *dst = shared + t * 256 + e * 64;
+                            *dst = g ? *dst + acc[t][e] : acc[t][e];
+                        }
+            }
+            __syncthreads();
         }
-        __syncthreads();
-        if (group == 0) {
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t)
-                if (t < mine)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[t][e] += shared[t * 256 + e * 64];
-        }
+        if (group) return;
     }
-    if (group) return;
     double *tiles = part + part_head(r) + (lane >> 4) * 16 + (lane & 15);
     const int have = tiles16(r);
-    auto write = [&](int i, int j, const f64x4 &v) {
+    auto write = [&](int i, int j, int t) {
         if (i >= have) return;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) tiles[tile_of(i, j) + 64 * e] = v[e];
+        for (int e = 0; e < 4; ++e) tiles[tile_of(i, j) + 64 * e] = kGroups > 1 ? shared[t * 256 + e * 64] : acc[t][e];
     };
     if (below) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) write(4 * bi + i, 4 * bj + j, acc[4 * i + j]);
+            for (int j = 0; j < 4; ++j) write(4 * bi + i, 4 * bj + j, 4 * i + j);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < (NT < 4 ? NT : 4); ++i)
 #pragma unroll
             for (int j = 0; j <= i; ++j) {
-                write(4 * bi + i, 4 * bi + j, acc[i * (i + 1) / 2 + j]);
-                if constexpr (NT > 4) write(4 * bi + 4 + i, 4 * bi + 4 + j, acc[10 + i * (i + 1) / 2 + j]);
+                write(4 * bi + i, 4 * bi + j, i * (i + 1) / 2 + j);
+                if constexpr (NT > 4) write(4 * bi + 4 + i, 4 * bi + 4 + j, 10 + i * (i + 1) / 2 + j);
             }
     }
 }
@@ -370,7 +369,7 @@ __host__ __device__ __forceinline__ int one_pass_tiles(int r) {
 }
 
 template <typename T, bool TALL>
-__device__ __forceinline__ void gram_by_size(const Matrix &m, const Item &it, const Hyper &h, double *ws, float *lds) {
+__device__ __forceinline__ void gram_by_size(const Matrix &m, const Item &it, const Hyper &h, double *ws, double *lds) {
     switch (one_pass_tiles(short_side(m))) {
         case 1: return gram_one_pass<T, 1, TALL>(m, it, h, ws, lds);
         case 2: return gram_one_pass<T, 2, TALL>(m, it, h, ws, lds);
@@ -383,7 +382,7 @@ __device__ __forceinline__ void gram_by_size(const Matrix &m, const Item &it, co
 template <typename T>
 __global__ __launch_bounds__(kGramThreads, 2) void muon_gram(const Matrix *matrices, const Item *items, Hyper h,
                                                             double *ws) {
-    __shared__ __align__(16) float lds[2 * (kChunk + 4) * kOnePass];
+    __shared__ __align__(16) double lds[kGramLds];
     const Item it = items[blockIdx.x];
     const Matrix m = matrices[it.matrix];
     if (m.rows > m.cols) gram_by_size<T, true>(m, it, h, ws, lds);
@@ -501,59 +500,84 @@ __global__ __launch_bounds__(kThreads) void muon_join(const Matrix *matrices, co
 }
 
 // ------------------------------------------------------------------ short sides up to 64
-// All steps in one workgroup, G, P, T and Q in LDS. Symmetric operands are read along rows
-// for both sides of a product.
-__global__ __launch_bounds__(kThreads) void muon_small(const Matrix *matrices, const Item *items, Hyper h, double *ws,
-                                                      int steps) {
-    constexpr int kPitch = kSmall + 8;
+// All steps in one workgroup of 8 waves, G, P, T and Q in LDS. Symmetric operands are read
+// along rows for both sides of a product; the ten tiles (i >= j) of rank 64 go to the waves in
+// turn, each in two chains of products.
+constexpr int kSmallThreads = 512;
+
+__global__ __launch_bounds__(kSmallThreads) void muon_small(const Matrix *matrices, const Item *items, Hyper h,
+                                                           double *ws, int steps) {
+    constexpr int kPitch = kSmall + 8, kMost = 10 * 256 / kSmallThreads;
     __shared__ double sg[kSmall * kPitch], sp[kSmall * kPitch], st[kSmall * kPitch], sq[kSmall * kPitch];
     const Item it = items[blockIdx.x];
     const Matrix m = matrices[it.matrix];
-    const int r = short_side(m), n = tiles16(r), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int r = short_side(m), n = tiles16(r), count = n * (n + 1) / 2, tid = threadIdx.x, lane = tid & 63,
+              wave = tid >> 6;
     const double inv = inverse_norm(m, ws, h.eps);
-    for (int t = 0, i = 0, j = 0; t < n * (n + 1) / 2; ++t) {
-        const double v = join_tile(m, ws, i, j, tid) * (inv * inv);
-        const int row = i * 16 + (tid >> 4), col = j * 16 + (tid & 15);
-        if (row >= col) sg[row * kPitch + col] = sg[col * kPitch + row] = v;
-        if (++j > i) ++i, j = 0;
+    {
+        // the parts in order, all of a thread's elements at once
+        const double *p = part_of(m, ws, 0) + part_head(r) + tid;
+        const int64_t step = part_size(r);
+        double v[kMost] = {};
+#pragma unroll 4
+        for (int s = 0; s < m.splits; ++s)
+#pragma unroll
+            for (int x = 0; x < kMost; ++x)
+                if (x * kSmallThreads + tid < count * 256) v[x] += p[s * step + x * kSmallThreads];
+#pragma unroll
+        for (int x = 0; x < kMost; ++x) {
+            const int t = (x * kSmallThreads + tid) >> 8, i = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, j = t - i * (i + 1) / 2;
+            const int row = i * 16 + ((tid & 255) >> 4), col = j * 16 + (tid & 15);
+            if (t < count && row >= col) sg[row * kPitch + col] = sg[col * kPitch + row] = v[x] * (inv * inv);
+        }
     }
     __syncthreads();
 
     // dst = left right, or a I + b left + c left right; dst may be an operand.
     auto product = [&](const double *left, const double *right, double *dst, bool polynomial) {
-        constexpr int kMost = 3;   // of the ten tiles (i >= j) per wave
-        f64x4 acc[kMost] = {};
-        int ti[kMost], tj[kMost];
+        f64x4 result[2];
 #pragma unroll
-        for (int x = 0; x < kMost; ++x) {
-            const int t = wave + 4 * x;
-            ti[x] = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3;
-            tj[x] = t - ti[x] * (ti[x] + 1) / 2;
-        }
-        for (int k = lane >> 4; k < 16 * n; k += 4)
+        for (int x = 0; x < 2; ++x) {
+            const int t = wave + 8 * x;
+            if (t >= count) continue;
+            const int i = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, j = t - i * (i + 1) / 2;
+            const double *a = left + (lane >> 4) * kPitch + 16 * i + (lane & 15);
+            const double *b = right + (lane >> 4) * kPitch + 16 * j + (lane & 15);
+            f64x4 even = {}, odd = {};
+            for (int k = 0; k < 16 * n; k += 16) {
+                double p[4], q[4];
 #pragma unroll
-            for (int x = 0; x < kMost; ++x)
-                if (ti[x] < n && tj[x] <= ti[x])
-                    acc[x] = mfma_f64(left[k * kPitch + 16 * ti[x] + (lane & 15)],
-                                      right[k * kPitch + 16 * tj[x] + (lane & 15)], acc[x]);
-        if (polynomial) {
-#pragma unroll
-            for (int x = 0; x < kMost; ++x)
+                for (int u = 0; u < 4; ++u) {
+                    p[u] = a[(k + 4 * u) * kPitch];
+                    q[u] = b[(k + 4 * u) * kPitch];
+                }
+                even = mfma_f64(p[0], q[0], even);
+                odd = mfma_f64(p[1], q[1], odd);
+                even = mfma_f64(p[2], q[2], even);
+                odd = mfma_f64(p[3], q[3], odd);
+            }
+            result[x] = even + odd;
+            if (polynomial) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int i = 16 * ti[x] + 4 * e + (lane >> 4), j = 16 * tj[x] + (lane & 15);
-                    if (ti[x] < n && tj[x] <= ti[x])
-                        acc[x][e] = h.c * acc[x][e] + h.b * left[i * kPitch + j] + (i == j && i < r ? h.a : 0.0);
+                    const int row = 16 * i + 4 * e + (lane >> 4), col = 16 * j + (lane & 15);
+                    result[x][e] = h.c * result[x][e] + h.b * left[row * kPitch + col] +
+                                   (row == col && row < r ? h.a : 0.0);
                 }
+            }
         }
         __syncthreads();
 #pragma unroll
-        for (int x = 0; x < kMost; ++x)
+        for (int x = 0; x < 2; ++x) {
+            const int t = wave + 8 * x;
+            if (t >= count) continue;
+            const int i = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, j = t - i * (i + 1) / 2;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int i = 16 * ti[x] + 4 * e + (lane >> 4), j = 16 * tj[x] + (lane & 15);
-                if (ti[x] < n && tj[x] <= ti[x] && i >= j) dst[i * kPitch + j] = dst[j * kPitch + i] = acc[x][e];
+                const int row = 16 * i + 4 * e + (lane >> 4), col = 16 * j + (lane & 15);
+                if (row >= col) dst[row * kPitch + col] = dst[col * kPitch + row] = result[x][e];
             }
+        }
         __syncthreads();
     };
     for (int i = 0; i < steps; ++i) {
@@ -565,7 +589,7 @@ __global__ __launch_bounds__(kThreads) void muon_small(const Matrix *matrices, c
     }
     const int rp = padded(r);
     float *final = final_q(m, ws);
-    for (int e = tid; e < rp * rp; e += kThreads) {
+    for (int e = tid; e < rp * rp; e += kSmallThreads) {
         const int row = e % rp, k = e / rp;
         final[final_at(rp, row, k)] = row < 16 * n && k < 16 * n ? (float)(sq[row * kPitch + k] * inv) : 0.0f;
     }
@@ -587,7 +611,7 @@ constexpr int kStageThreads = 512;
 
 __global__ __launch_bounds__(kStageThreads) void muon_stage(const Matrix *matrices, const Item *items, Hyper h,
                                                            double *ws, StageOp op0, StageOp op1) {
-    constexpr int kPitch = kPad + 1, kSteps = 8;
+    constexpr int kPitch = kPad + 1, kSteps = 4;
     __shared__ double sums[4][kPad * kPitch];
     const StageOp op = blockIdx.y ? op1 : op0;
     const Item it = items[blockIdx.x];
@@ -991,7 +1015,7 @@ extern "C" int ct_muon(const ct_muon_matrix *matrices, int64_t count, const int3
         if (!ok()) return status;
     }
     if (counts[kItemsSmall]) {
-        muon_small<<<grid(kItemsSmall), dim3(kThreads), 0, stream>>>(mats, items[kItemsSmall], h, ws, o->steps);
+        muon_small<<<grid(kItemsSmall), dim3(kSmallThreads), 0, stream>>>(mats, items[kItemsSmall], h, ws, o->steps);
         if (!ok()) return status;
     }
     if (counts[kItemsStage]) {
