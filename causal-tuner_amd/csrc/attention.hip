@@ -171,30 +171,35 @@ __device__ __forceinline__ void outer(f32x16 (&acc)[DP / 32], const uint4 *tile,
 
 // ------------------------------------------------------------------ global -> LDS
 // One thread's share of a tile of ROWS rows, held in registers between the load and the
-// LDS store. `at(row)` gives the byte offset of a row from the base, or kOOB: an offset
-// past the buffer's range reads zeros, so nothing behind a record's end enters a product
-// (a masked zero times a NaN there would be NaN).
-template <typename T, int DP, int ROWS>
+// LDS store. Rows that `valid` refuses are loaded from an offset past the buffer's range,
+// which reads zeros: nothing behind a record's end enters a product (a masked zero times a NaN
+// there would be NaN).
+template <typename T, int DP, int ROWS, int THREADS>
 struct Stage {
     static constexpr int kChunks = Tile<T, DP>::kChunks;
-    static constexpr int kLoads = ROWS * kChunks / kThreads;
+    static constexpr int kLoads = (ROWS * kChunks + THREADS - 1) / THREADS;
+    static_assert(ROWS * kChunks % THREADS == 0 || kLoads == 1, "whole loads");
+    static constexpr bool kPart = ROWS * kChunks < THREADS;   // some threads have none
     uint4 r[kLoads];
-    template <typename At>
-    __device__ __forceinline__ void load(const char *base, int chunks, At at) {
+    __device__ static __forceinline__ int row_of(int p) { return (p * THREADS + (int)threadIdx.x) / kChunks; }
+    __device__ static __forceinline__ int chunk_of() { return (int)threadIdx.x % kChunks; }   // THREADS % kChunks == 0
+    // offset(p): bytes from base to the row of load p; valid(row): whether it exists.
+    template <typename Offset, typename Valid>
+    __device__ __forceinline__ void load(const char *base, int chunks, Offset offset, Valid valid) {
         const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(base, 0x7fffffff);
+        const bool wanted = chunk_of() < chunks;
 #pragma unroll
         for (int p = 0; p < kLoads; ++p) {
-            const int i = p * kThreads + (int)threadIdx.x, row = i / kChunks, c = i % kChunks;
-            const uint32_t off = at(row);
-            r[p] = buf_load16(rsrc, c < chunks && off != kOOB ? off + 16u * (uint32_t)c : kOOB);
+            const bool ok = wanted & valid(row_of(p)) & (!kPart || row_of(p) < ROWS);
+            r[p] = buf_load16(rsrc, ok ? offset(p) + 16u * (uint32_t)chunk_of() : kOOB);
         }
     }
     __device__ __forceinline__ void store(uint4 *tile) const {
 #pragma unroll
-        for (int p = 0; p < kLoads; ++p) {
-            const int i = p * kThreads + (int)threadIdx.x, row = i / kChunks, c = i % kChunks;
-            *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(tile) + Tile<T, DP>::addr(row, c)) = r[p];
-        }
+        for (int p = 0; p < kLoads; ++p)
+            if (!kPart || row_of(p) < ROWS)
+                *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(tile) + Tile<T, DP>::addr(row_of(p), chunk_of())) =
+                    r[p];
     }
 };
 
@@ -215,6 +220,9 @@ __device__ __forceinline__ f32x16 splat(float v) {
     for (int i = 0; i < 16; ++i) r[i] = v;
     return r;
 }
+
+// The wave's number in its workgroup, known to be the same in all its lanes.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
 
 // Value of the same column in the other half of the wave.
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
@@ -257,8 +265,26 @@ __device__ __forceinline__ void wave_limits(const RowOf &row, int &least, int &m
     most = __builtin_amdgcn_readfirstlane(most);
 }
 
-template <typename T>
-constexpr int kKeyTile = sizeof(T) == 2 ? 64 : 32;
+// ------------------------------------------------------------------ the key loop
+// Forward and dq run over 32-key steps, dk/dv over 32-row steps, all in one rhythm: step t
+// multiplies with tile t (the second products) while it makes the scores of tile t + 1, so
+// that a wave always has matrix instructions beside its exponentials; tile t + 2 goes from
+// registers to LDS and tile t + 3 from memory to registers. Three LDS stages, one barrier a step.
+constexpr int kStep = 32, kStages = 3;
+
+// Runs f(stage, next, then) over consecutive steps with the stages as constants, so that LDS
+// addresses are one register per lane pattern and immediate offsets.
+template <typename F>
+__device__ __forceinline__ void by_stage(int from, int to, F f) {
+    typedef std::integral_constant<int, 0> Zero;
+    typedef std::integral_constant<int, 1> One;
+    typedef std::integral_constant<int, 2> Two;
+    for (int at = from; at < to; at += 3 * kStep) {
+        f(at, Zero(), One(), Two());
+        if (at + kStep < to) f(at + kStep, One(), Two(), Zero());
+        if (at + 2 * kStep < to) f(at + 2 * kStep, Two(), Zero(), One());
+    }
+}
 
 // Running softmax of a wave's 32 rows over their keys; m2 is the reference exponent of base
 // 2 that p and the sums are relative to.
@@ -267,15 +293,17 @@ struct Running {
 };
 
 // ------------------------------------------------------------------ forward
-template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_forward(AttnParams a) {
-    constexpr int KT = kKeyTile<T>;
-    constexpr int kUnits = KT * Tile<T, DP>::kChunks;
+template <typename T>
+constexpr int kKeyTile = sizeof(T) == 2 ? 64 : 32;
+
+template <typename T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) void attention_forward(AttnParams a) {
+    constexpr int KT = kKeyTile<T>, kUnits = KT * Tile<T, DP>::kChunks;
     __shared__ uint4 sk[2][kUnits], sv[2][kUnits];
     const Item item = a.items[blockIdx.x / a.kv_heads];
     const int kv_head = blockIdx.x % a.kv_heads;
     const Record rec = a.records[item.record];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chunks = a.head_dim * (int)sizeof(T) / 16;
+    const int lane = threadIdx.x & 63, wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
 
     const RowOf row(a, rec, kv_head, (int64_t)item.begin + wave * kWaveCols + (lane & 31));
     int least, most;
@@ -285,25 +313,26 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fo
 
     const char *k0 = a.k + rec.k_start * a.k_token + kv_head * a.k_head;
     const char *v0 = a.v + rec.k_start * a.v_token + kv_head * a.v_head;
-    Stage<T, DP, KT> ks, vs;
+    Stage<T, DP, KT, 64 * WAVES> ks, vs;
     auto load = [&](int key) {
         const int left = (int)rec.k_len - key;
-        ks.load(k0 + key * a.k_token, chunks, [&](int r) { return r < left ? (uint32_t)(r * a.k_token) : kOOB; });
-        vs.load(v0 + key * a.v_token, chunks, [&](int r) { return r < left ? (uint32_t)(r * a.v_token) : kOOB; });
+        auto valid = [&](int r) { return r < left; };
+        ks.load(k0 + key * a.k_token, chunks, [&](int p) { return (uint32_t)ks.row_of(p) * (uint32_t)a.k_token; }, valid);
+        vs.load(v0 + key * a.v_token, chunks, [&](int p) { return (uint32_t)vs.row_of(p) * (uint32_t)a.v_token; }, valid);
     };
 
     f32x16 o[DP / 32];
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) o[n] = splat(0.0f);
     Running run;
-    int buf = 0;
     if (item.lo < item.hi) {
         load(item.lo);
         ks.store(sk[0]);
         vs.store(sv[0]);
     }
     __syncthreads();
-    for (int key = item.lo; key < item.hi; key += KT) {
+    auto step = [&](int key, auto stage) {
+        constexpr int buf = decltype(stage)::value;
         const bool more = key + KT < item.hi;
         if (more) load(key + KT);
         if (key < most) {
@@ -331,9 +360,9 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fo
             // stays below 2^8, o and the sum are exact in that scale, and most tiles skip the
             // rescaling of o.
             if (__any(top > run.m2 + 8.0f)) {
-                const float next = fmaxf(run.m2, top);
-                const float shrink = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run.m2 - next);
-                run.m2 = next;
+                const float grown = fmaxf(run.m2, top);
+                const float shrink = grown == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run.m2 - grown);
+                run.m2 = grown;
                 run.sum *= shrink;
 #pragma unroll
                 for (int n = 0; n < DP / 32; ++n)
@@ -356,7 +385,10 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fo
             vs.store(sv[buf ^ 1]);
         }
         __syncthreads();
-        buf ^= 1;
+    };
+    for (int key = item.lo; key < item.hi; key += 2 * KT) {
+        step(key, std::integral_constant<int, 0>());
+        if (key + KT < item.hi) step(key + KT, std::integral_constant<int, 1>());
     }
 
     const float sum = run.sum + other_half(run.sum);
@@ -376,7 +408,7 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fo
         if (lane < 32)
             a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : run.m2 + __builtin_amdgcn_logf(sum);
     } else {
-        const int64_t at = ((int64_t)item.slot * a.kv_heads + kv_head) * kTile + wave * kWaveCols + (lane & 31);
+        const int64_t at = ((int64_t)item.slot * a.kv_heads + kv_head) * (32 * WAVES) + wave * kWaveCols + (lane & 31);
         float *dst = a.part0 + at * DP;
 #pragma unroll
         for (int n = 0; n < DP / 32; ++n)
@@ -391,15 +423,15 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_fo
 // Joins the key ranges of split rows: with M = max_s m_s, o = sum_s 2^(m_s - M) o_s over
 // sum_s 2^(m_s - M) sum_s. One wave per row, the parts in order.
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads) void attention_join(AttnParams a, const Item *joins) {
-    const Item join = joins[blockIdx.x / (a.kv_heads * (kTile / 4))];
-    const int rest = blockIdx.x % (a.kv_heads * (kTile / 4));
+__global__ __launch_bounds__(kThreads) void attention_join(AttnParams a, const Item *joins, int tile) {
+    const Item join = joins[blockIdx.x / (a.kv_heads * (tile / 4))];
+    const int rest = blockIdx.x % (a.kv_heads * (tile / 4));
     const int kv_head = rest % a.kv_heads, lane = threadIdx.x & 63;
     const int r = rest / a.kv_heads * 4 + (threadIdx.x >> 6);
     const Record rec = a.records[join.record];
     const RowOf row(a, rec, kv_head, (int64_t)join.begin + r);
     if (!row.valid) return;
-    const int64_t first = ((int64_t)join.lo * a.kv_heads + kv_head) * kTile + r, step = (int64_t)a.kv_heads * kTile;
+    const int64_t first = ((int64_t)join.lo * a.kv_heads + kv_head) * tile + r, step = (int64_t)a.kv_heads * tile;
     float top = -INFINITY;
     for (int s = 0; s < join.hi; ++s) top = fmaxf(top, a.part1[2 * (first + s * step)]);
     const float ref = top == -INFINITY ? 0.0f : top;
@@ -443,19 +475,19 @@ __device__ __forceinline__ float dot_chunk(const uint4 &x, const uint4 &y, float
     return acc;
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq(AttnParams a) {
-    constexpr int KT = kKeyTile<T>;
-    constexpr int kUnits = KT * Tile<T, DP>::kChunks;
-    __shared__ uint4 sk[2][kUnits], sv[2][kUnits];
+template <typename T, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) void attention_dq(AttnParams a) {
+    constexpr int kUnits = kStep * Tile<T, DP>::kChunks;
+    __shared__ uint4 sk[kStages][kUnits], sv[kStages][kUnits];
     const Item item = a.items[blockIdx.x / a.kv_heads];
     const int kv_head = blockIdx.x % a.kv_heads;
     const Record rec = a.records[item.record];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chunks = a.head_dim * (int)sizeof(T) / 16;
+    const int lane = threadIdx.x & 63, wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
 
     const RowOf row(a, rec, kv_head, (int64_t)item.begin + wave * kWaveCols + (lane & 31));
     int least, most;
     wave_limits(row, least, most);
+    most = min(most, item.hi);
     uint4 qf[Tile<T, DP>::kFrags], gf[Tile<T, DP>::kFrags];
     row_fragments<T, DP>(a.dout + row.token * a.do_token + row.head * a.do_head, gf, row.valid, chunks, lane);
     row_fragments<T, DP>(a.out + row.token * a.o_token + row.head * a.o_head, qf, row.valid, chunks, lane);
@@ -473,50 +505,59 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
 
     const char *k0 = a.k + rec.k_start * a.k_token + kv_head * a.k_head;
     const char *v0 = a.v + rec.k_start * a.v_token + kv_head * a.v_head;
-    Stage<T, DP, KT> ks, vs;
+    Stage<T, DP, kStep, 64 * WAVES> ks, vs;
     auto load = [&](int key) {
         const int left = (int)rec.k_len - key;
-        ks.load(k0 + key * a.k_token, chunks, [&](int r) { return r < left ? (uint32_t)(r * a.k_token) : kOOB; });
-        vs.load(v0 + key * a.v_token, chunks, [&](int r) { return r < left ? (uint32_t)(r * a.v_token) : kOOB; });
+        auto valid = [&](int r) { return r < left; };
+        ks.load(k0 + key * a.k_token, chunks, [&](int p) { return (uint32_t)ks.row_of(p) * (uint32_t)a.k_token; }, valid);
+        vs.load(v0 + key * a.v_token, chunks, [&](int p) { return (uint32_t)vs.row_of(p) * (uint32_t)a.v_token; }, valid);
+    };
+    auto store = [&](int buf) {
+        ks.store(sk[buf]);
+        vs.store(sv[buf]);
     };
 
-    f32x16 o[DP / 32];
+    f32x16 o[DP / 32], s, g;
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) o[n] = splat(0.0f);
-    int buf = 0;
     if (item.lo < item.hi) {
         load(item.lo);
-        ks.store(sk[0]);
-        vs.store(sv[0]);
+        store(0);
+        if (item.lo + kStep < item.hi) {
+            load(item.lo + kStep);
+            store(1);
+            if (item.lo + 2 * kStep < item.hi) load(item.lo + 2 * kStep);
+        }
     }
     __syncthreads();
-    for (int key = item.lo; key < item.hi; key += KT) {
-        const bool more = key + KT < item.hi;
-        if (more) load(key + KT);
-        if (key < most) {
-            const bool masked = key + KT > least;
-            const int left = row.limit - key - 4 * (lane >> 5);
-#pragma unroll
-            for (int t = 0; t < KT / 32; ++t) {
-                f32x16 s = splat(0.0f), g = splat(-delta);
-                scores<T, DP>(s, sk[buf], 32 * t, qf, lane);
-                scores<T, DP>(g, sv[buf], 32 * t, gf, lane);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse)) * g[i];
-                if (masked)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[i] = 32 * t + 8 * (i >> 2) + (i & 3) < left ? s[i] : 0.0f;
-                outer<T, DP>(o, sk[buf], 32 * t, s, lane);
-            }
+    auto both = [&](int buf) {
+        s = splat(0.0f);
+        g = splat(-delta);
+        scores<T, DP>(s, sk[buf], 0, qf, lane);
+        scores<T, DP>(g, sv[buf], 0, gf, lane);
+    };
+    if (item.lo < most) both(0);
+    by_stage(item.lo, item.hi, [&](int key, auto now_, auto next_, auto then_) {
+        constexpr int now = decltype(now_)::value, next = decltype(next_)::value, then = decltype(then_)::value;
+        if (key + 2 * kStep < item.hi) {
+            store(then);
+            if (key + 3 * kStep < item.hi) load(key + 3 * kStep);
         }
-        if (more) {
-            ks.store(sk[buf ^ 1]);
-            vs.store(sv[buf ^ 1]);
+        if (key < most) {
+            f32x16 ds;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                ds[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse)) * g[i];
+            if (key + kStep > least) {
+                const int left = row.limit - key - 4 * (lane >> 5);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) ds[i] = 8 * (i >> 2) + (i & 3) < left ? ds[i] : 0.0f;
+            }
+            if (key + kStep < most) both(next);
+            outer<T, DP>(o, sk[now], 0, ds, lane);
         }
         __syncthreads();
-        buf ^= 1;
-    }
+    });
     if (!row.valid) return;
     char *dst = a.dst0 + row.token * a.d_token + (int64_t)row.head * a.head_dim * (int)sizeof(T);
 #pragma unroll
@@ -531,26 +572,33 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 2 ? 2 : 1) void attention_dq
 }
 
 // ------------------------------------------------------------------ dk, dv
-template <typename T>
-constexpr int kRowTile = sizeof(T) == 2 ? 64 : 32;
+// Two waves share 32 keys. One makes the probabilities p = exp(s - lse) and dv += p^T do, the
+// other do . v - delta, ds = p (do . v - delta) with the first one's p through LDS (lane by
+// lane: both hold the same layout) and dk += ds^T q. Each then holds one operand of keys and
+// one accumulator, which leaves room for two waves per SIMD; a single wave with both needs
+// 490 registers and ran at 25% of the matrix instructions' rate (2633 against ... us at 8192
+// rows of 32 heads of 128).
+constexpr int kKeyWaves = 8;
 
 template <typename T, int DP>
-__global__ __launch_bounds__(kThreads, 1) void attention_dkv(AttnParams a) {
-    constexpr int RT = kRowTile<T>;
-    constexpr int kUnits = RT * Tile<T, DP>::kChunks;
-    __shared__ uint4 sq[2][kUnits], sg[2][kUnits];
-    __shared__ float slse[2][RT], sdelta[2][RT];
+__global__ __launch_bounds__(64 * kKeyWaves, 2) void attention_dkv(AttnParams a) {
+    constexpr int kUnits = kStep * Tile<T, DP>::kChunks, kAll = 64 * kKeyWaves;
+    __shared__ uint4 sq[kStages][kUnits], sg[kStages][kUnits];
+    __shared__ float slse[kStages][kStep], sdelta[kStages][kStep];   // negated
+    __shared__ f32x4 sp[2][kKeyWaves / 2][4][64];
     const Item item = a.items[blockIdx.x / a.kv_heads];
     const int kv_head = blockIdx.x % a.kv_heads;
     const Record rec = a.records[item.record];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chunks = a.head_dim * (int)sizeof(T) / 16;
+    const int lane = threadIdx.x & 63, wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
+    const int pair = wave & 3;                // waves w and w + 4 run on one SIMD
+    const bool for_dv = wave < kKeyWaves / 2;
 
-    const int key0 = item.begin + wave * kWaveCols, key = key0 + (lane & 31);
+    const int key0 = item.begin + pair * kWaveCols, key = key0 + (lane & 31);
     const bool valid = key < rec.k_len;
     const int64_t kv = rec.k_start + (valid ? key : 0);
-    uint4 kf[Tile<T, DP>::kFrags], vf[Tile<T, DP>::kFrags];
-    row_fragments<T, DP>(a.k + kv * a.k_token + kv_head * a.k_head, kf, valid, chunks, lane);
-    row_fragments<T, DP>(a.v + kv * a.v_token + kv_head * a.v_head, vf, valid, chunks, lane);
+    uint4 frag[Tile<T, DP>::kFrags];
+    row_fragments<T, DP>(for_dv ? a.k + kv * a.k_token + kv_head * a.k_head : a.v + kv * a.v_token + kv_head * a.v_head,
+                         frag, valid, chunks, lane);
 
     const int nrows = (int)(rec.q_len * a.group);
     // Row r sees key j when r >= first(j); tokens before key j - (keys - queries) do not.
@@ -560,118 +608,147 @@ __global__ __launch_bounds__(kThreads, 1) void attention_dkv(AttnParams a) {
     };
     const int64_t mine = first(key), wave_first = first(key0), wave_last = first(key0 + kWaveCols - 1);
 
-    Stage<T, DP, RT> qs, gs;
-    float lse_r, delta_r;
+    Stage<T, DP, kStep, kAll> qs, gs;
+    float stat_r = 0.0f;
+    // A group that divides the step makes a row's token and head the same in every step; the
+    // others are divided out each time.
+    const bool regular = kStep % a.group == 0;
+    const int stat_row = (int)threadIdx.x % kStep;
+    struct Place {
+        uint32_t q, g;
+        int32_t stat;
+    };
+    auto place = [&](int row, uint32_t base) -> Place {   // row after the first token of the step
+        const uint32_t r = base + (uint32_t)row, t = div_group(a, r), h = r - t * (uint32_t)a.group;
+        return {t * (uint32_t)a.q_token + h * (uint32_t)a.q_head, t * (uint32_t)a.do_token + h * (uint32_t)a.do_head,
+                (int32_t)(t * (uint32_t)a.heads + h)};
+    };
+    constexpr int kLoads = Stage<T, DP, kStep, kAll>::kLoads;
+    Place fixed[kLoads];
+#pragma unroll
+    for (int p = 0; p < kLoads; ++p) fixed[p] = place(qs.row_of(p), 0);
+    const int32_t fixed_stat = place(stat_row, 0).stat;
     auto load = [&](int r0) {
-        const uint32_t t0 = div_group(a, (uint32_t)r0);
+        const uint32_t t0 = div_group(a, (uint32_t)r0), base = (uint32_t)r0 - t0 * (uint32_t)a.group;
         const int64_t token = rec.q_start + t0;
-        auto at = [&](int row, int64_t by_token, int64_t by_head) -> uint32_t {
-            const uint32_t r = (uint32_t)(r0 + row);
-            if ((int)r >= nrows) return kOOB;
-            const uint32_t t = div_group(a, r);
-            return (uint32_t)((t - t0) * by_token + (r - t * (uint32_t)a.group) * by_head);
-        };
-        qs.load(a.q + token * a.q_token + (int64_t)kv_head * a.group * a.q_head, chunks,
-                [&](int row) { return at(row, a.q_token, a.q_head); });
+        const int left = nrows - r0;
+        Place at[kLoads];
+        int32_t stat = fixed_stat;
+#pragma unroll
+        for (int p = 0; p < kLoads; ++p) at[p] = fixed[p];
+        if (!regular) {
+#pragma unroll
+            for (int p = 0; p < kLoads; ++p) at[p] = place(qs.row_of(p), base);
+            stat = place(stat_row, base).stat;
+        }
+        auto exists = [&](int row) { return row < left; };
+        qs.load(a.q + token * a.q_token + (int64_t)kv_head * a.group * a.q_head, chunks, [&](int p) { return at[p].q; },
+                exists);
         gs.load(a.dout + token * a.do_token + (int64_t)kv_head * a.group * a.do_head, chunks,
-                [&](int row) { return at(row, a.do_token, a.do_head); });
-        if ((int)threadIdx.x < RT) {
-            const uint32_t r = (uint32_t)(r0 + (int)threadIdx.x);
-            lse_r = INFINITY;
-            delta_r = 0.0f;
-            if ((int)r < nrows) {
-                const uint32_t t = div_group(a, r);
-                const int64_t at = (rec.q_start + t) * a.heads + kv_head * a.group + (int)(r - t * (uint32_t)a.group);
-                lse_r = a.stats[at];
-                delta_r = a.delta[at];
-            }
+                [&](int p) { return at[p].g; }, exists);
+        if (wave == 0) {   // lanes 0 - 31 the statistics, 32 - 63 delta; rows behind the last: p = 0
+            const float *from = (lane < kStep ? a.stats : a.delta) + token * a.heads + kv_head * a.group;
+            stat_r = stat_row < left ? from[stat] : lane < kStep ? INFINITY : 0.0f;
         }
     };
     auto store = [&](int buf) {
         qs.store(sq[buf]);
         gs.store(sg[buf]);
-        if ((int)threadIdx.x < RT) {
-            slse[buf][threadIdx.x] = lse_r;
-            sdelta[buf][threadIdx.x] = delta_r;
-        }
+        if (wave == 0) (lane < kStep ? slse : sdelta)[buf][stat_row] = -stat_r;
     };
 
-    f32x16 dk[DP / 32], dv[DP / 32];
+    f32x16 acc[DP / 32], s = splat(0.0f);
 #pragma unroll
-    for (int n = 0; n < DP / 32; ++n) dk[n] = dv[n] = splat(0.0f);
-    int buf = 0;
+    for (int n = 0; n < DP / 32; ++n) acc[n] = splat(0.0f);
+    // Probabilities (for dv, shared) or do . v - delta of the rows at r0 in stage `buf`.
+    auto make = [&](int r0, int buf, int turn) {
+        const float *stat = (for_dv ? slse : sdelta)[buf] + 4 * (lane >> 5);
+        f32x16 st;
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(stat + 2 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st[i + e] = v[e];
+        }
+        if (for_dv) {
+            s = splat(0.0f);
+            scores<T, DP>(s, sq[buf], 0, frag, lane);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, st[i]));
+            if (r0 < wave_last) {
+                const int hidden = (int)(mine < nrows ? mine : nrows) - r0 - 4 * (lane >> 5);   // rows below do not see the key
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) >= hidden ? s[i] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sp[turn][pair][i][lane] = f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
+        } else {
+            s = st;
+            scores<T, DP>(s, sg[buf], 0, frag, lane);
+        }
+    };
     if (item.lo < item.hi) {
         load(item.lo);
         store(0);
+        if (item.lo + kStep < item.hi) {
+            load(item.lo + kStep);
+            store(1);
+            if (item.lo + 2 * kStep < item.hi) load(item.lo + 2 * kStep);
+        }
     }
     __syncthreads();
-    for (int r0 = item.lo; r0 < item.hi; r0 += RT) {
-        const bool more = r0 + RT < item.hi;
-        if (more) load(r0 + RT);
-        if (r0 + RT > wave_first) {
-            const bool masked = r0 < wave_last;
+    int turn = 0;
+    if (item.lo < item.hi && item.lo + kStep > wave_first) make(item.lo, 0, 0);
+    __syncthreads();
+    by_stage(item.lo, item.hi, [&](int r0, auto now_, auto next_, auto then_) {
+        constexpr int now = decltype(now_)::value, next = decltype(next_)::value, then = decltype(then_)::value;
+        if (r0 + 2 * kStep < item.hi) {
+            store(then);
+            if (r0 + 3 * kStep < item.hi) load(r0 + 3 * kStep);
+        }
+        const bool seen = r0 + kStep > wave_first, more = r0 + kStep < item.hi && r0 + 2 * kStep > wave_first;
+        f32x16 z = s;
+        if (seen && !for_dv) {
 #pragma unroll
-            for (int t = 0; t < RT / 32; ++t) {
-                f32x16 s = splat(0.0f), g, p;
-                float lse[16];
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 p = sp[turn][pair][i][lane];
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const int at = 32 * t + 2 * i + 4 * (lane >> 5);
-                    const float4 l4 = *reinterpret_cast<const float4 *>(&slse[buf][at]);
-                    const float4 d4 = *reinterpret_cast<const float4 *>(&sdelta[buf][at]);
-                    lse[i] = l4.x; lse[i + 1] = l4.y; lse[i + 2] = l4.z; lse[i + 3] = l4.w;
-                    g[i] = -d4.x; g[i + 1] = -d4.y; g[i + 2] = -d4.z; g[i + 3] = -d4.w;
-                }
-                scores<T, DP>(s, sq[buf], 32 * t, kf, lane);
-                scores<T, DP>(g, sg[buf], 32 * t, vf, lane);
+                for (int e = 0; e < 4; ++e) z[4 * i + e] *= p[e];
+            }
+            if (r0 < wave_last) {   // 0 x inf
+                const int hidden = (int)(mine < nrows ? mine : nrows) - r0 - 4 * (lane >> 5);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse[i]));
-                    s[i] = p[i] * g[i];
-                }
-                if (masked) {
-                    const int64_t hidden = mine - r0 - 4 * (lane >> 5);   // rows below it do not see the key
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const bool seen = 32 * t + 8 * (i >> 2) + (i & 3) >= hidden;
-                        p[i] = seen ? p[i] : 0.0f;
-                        s[i] = seen ? s[i] : 0.0f;
-                    }
-                }
-                outer<T, DP>(dv, sg[buf], 32 * t, p, lane);
-                outer<T, DP>(dk, sq[buf], 32 * t, s, lane);
+                for (int i = 0; i < 16; ++i) z[i] = 8 * (i >> 2) + (i & 3) >= hidden ? z[i] : 0.0f;
             }
         }
-        if (more) store(buf ^ 1);
+        if (more) make(r0 + kStep, next, turn ^ 1);
+        if (seen) outer<T, DP>(acc, for_dv ? sg[now] : sq[now], 0, z, lane);
         __syncthreads();
-        buf ^= 1;
-    }
+        turn ^= 1;
+    });
     const int d0 = 4 * (lane >> 5);
+    const float scale = for_dv ? 1.0f : a.scale;
     if (item.slot < 0) {
         if (!valid) return;
-        const int64_t off = kv * a.d_token + (int64_t)kv_head * a.head_dim * (int)sizeof(T);
+        char *dst = (for_dv ? a.dst1 : a.dst0) + kv * a.d_token + (int64_t)kv_head * a.head_dim * (int)sizeof(T);
 #pragma unroll
         for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const int d = 32 * n + 2 * i + d0;
-                if (d < a.head_dim) {
-                    store4<T>(a.dst0 + off, d, dk[n][i] * a.scale, dk[n][i + 1] * a.scale, dk[n][i + 2] * a.scale,
-                              dk[n][i + 3] * a.scale);
-                    store4<T>(a.dst1 + off, d, dv[n][i], dv[n][i + 1], dv[n][i + 2], dv[n][i + 3]);
-                }
+                if (d < a.head_dim)
+                    store4<T>(dst, d, acc[n][i] * scale, acc[n][i + 1] * scale, acc[n][i + 2] * scale,
+                              acc[n][i + 3] * scale);
             }
     } else {
-        const int64_t at = (((int64_t)item.slot * a.kv_heads + kv_head) * kTile + wave * kWaveCols + (lane & 31)) * DP;
+        float *dst = (for_dv ? a.part1 : a.part0) +
+                     (((int64_t)item.slot * a.kv_heads + kv_head) * kTile + pair * kWaveCols + (lane & 31)) * DP;
 #pragma unroll
         for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                *reinterpret_cast<float4 *>(a.part0 + at + 32 * n + 2 * i + d0) =
-                    make_float4(dk[n][i], dk[n][i + 1], dk[n][i + 2], dk[n][i + 3]);
-                *reinterpret_cast<float4 *>(a.part1 + at + 32 * n + 2 * i + d0) =
-                    make_float4(dv[n][i], dv[n][i + 1], dv[n][i + 2], dv[n][i + 3]);
-            }
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float4 *>(dst + 32 * n + 2 * i + d0) =
+                    make_float4(acc[n][i], acc[n][i + 1], acc[n][i + 2], acc[n][i + 3]);
     }
 }
 
@@ -700,6 +777,10 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_join(AttnParams a, con
 }
 
 // ------------------------------------------------------------------ host side
+#ifndef RW
+#define RW 4
+#endif
+constexpr int kRowWaves = RW, kRowTile = 32 * kRowWaves;
 constexpr int64_t kMaxRows = 0x7fffffff - 2 * kTile;
 
 constexpr int64_t kMaxPitch = (int64_t)1 << 24;   // bytes between tokens of k and v
@@ -771,7 +852,7 @@ int by_type(int dtype, int dp, F f) {
 }
 
 int64_t parts_per_item(int32_t pass, int dp) {   // floats
-    return pass == CT_ATTENTION_KEYS ? 2 * (int64_t)kTile * dp : (int64_t)kTile * (dp + 2);
+    return pass == CT_ATTENTION_KEYS ? 2 * (int64_t)kTile * dp : (int64_t)kRowTile * (dp + 2);
 }
 
 // Workgroups that keep the card busy: two per CU in the forward, one (of twice the
@@ -781,11 +862,12 @@ constexpr int64_t kForwardGroups = 512, kKeyGroups = 512;
 void plan_items(int32_t pass, const Record *rec, int64_t n, int64_t kv_heads, int64_t group, bool causal,
                 std::vector<Item> &items, std::vector<Item> &joins, int64_t &slots) {
     const bool keys = pass == CT_ATTENTION_KEYS;
+    const int64_t tile = keys ? kTile : kRowTile;
     constexpr int64_t kUnit = 64;   // ranges are cut at multiples of a tile
     int64_t work = 0;
     for (int64_t i = 0; i < n; ++i) {
         const int64_t rows = rec[i].q_len * group, span = keys ? rec[i].k_len : rows;
-        for (int64_t b = 0; b < span; b += kTile) {
+        for (int64_t b = 0; b < span; b += tile) {
             Item it = {};
             it.record = (int32_t)i;
             it.begin = (int32_t)b;
@@ -796,7 +878,7 @@ void plan_items(int32_t pass, const Record *rec, int64_t n, int64_t kv_heads, in
                 it.lo = (int32_t)std::min(t * group / kUnit * kUnit, rows);
                 it.hi = (int32_t)rows;
             } else {      // keys that the tile's last row sees
-                const int64_t t = (std::min(rows, b + kTile) - 1) / group;
+                const int64_t t = (std::min(rows, b + tile) - 1) / group;
                 it.hi = (int32_t)(causal ? std::min(rec[i].k_len, std::max<int64_t>(0, t + 1 + shift)) : rec[i].k_len);
             }
             work += cdiv(it.hi - it.lo, kUnit);
@@ -903,15 +985,15 @@ extern "C" int ct_attention_forward(const ct_attention *c, const int32_t *plan, 
     a.dst0 = (char *)out;
     a.stats = stats;
     a.part0 = (float *)workspace;
-    a.part1 = a.part0 + slots * c->kv_heads * kTile * dp;
+    a.part1 = a.part0 + slots * c->kv_heads * kRowTile * dp;
     return by_type(c->dtype, dp, [&](auto type, auto dim) {
         typedef decltype(type) T;
         constexpr int DP = decltype(dim)::value;
-        attention_forward<T, DP><<<dim3((unsigned)(n * c->kv_heads)), dim3(kThreads), 0, stream>>>(a);
+        attention_forward<T, DP, kRowWaves><<<dim3((unsigned)(n * c->kv_heads)), dim3(64 * kRowWaves), 0, stream>>>(a);
         if (const int status = status_of_last_launch()) return status;
         if (joins) {
-            attention_join<T, DP><<<dim3((unsigned)(joins * c->kv_heads * (kTile / 4))), dim3(kThreads), 0, stream>>>(
-                a, a.items + n);
+            attention_join<T, DP><<<dim3((unsigned)(joins * c->kv_heads * (kRowTile / 4))), dim3(kThreads), 0, stream>>>(
+                a, a.items + n, kRowTile);
             return status_of_last_launch();
         }
         return 0;
@@ -960,7 +1042,7 @@ extern "C" int ct_attention_backward(const ct_attention *c, const int32_t *row_p
             r.items = reinterpret_cast<const Item *>(row_plan);
             r.dst0 = (char *)dq;
             r.d_token = a.o_token;
-            attention_dq<T, DP><<<dim3((unsigned)(rows * c->kv_heads)), dim3(kThreads), 0, stream>>>(r);
+            attention_dq<T, DP, kRowWaves><<<dim3((unsigned)(rows * c->kv_heads)), dim3(64 * kRowWaves), 0, stream>>>(r);
             if (const int status = status_of_last_launch()) return status;
         }
         if (!keys) return 0;
@@ -971,7 +1053,7 @@ extern "C" int ct_attention_backward(const ct_attention *c, const int32_t *row_p
         r.d_token = c->kv_heads * a.o_head;
         r.part0 = (float *)workspace;
         r.part1 = r.part0 + slots * c->kv_heads * kTile * DP;
-        attention_dkv<T, DP><<<dim3((unsigned)(keys * c->kv_heads)), dim3(kThreads), 0, stream>>>(r);
+        attention_dkv<T, DP><<<dim3((unsigned)(keys * c->kv_heads)), dim3(64 * kKeyWaves), 0, stream>>>(r);
         if (const int status = status_of_last_launch()) return status;
         if (!joins) return 0;
         attention_dkv_join<T, DP><<<dim3((unsigned)(joins * c->kv_heads * (kTile * DP / (4 * kThreads)))),
