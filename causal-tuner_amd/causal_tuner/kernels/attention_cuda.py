@@ -121,10 +121,10 @@ class AttentionLayout:
         lib = _native.library()
         parts, plans, at = [self._host.view(torch.int32).reshape(-1, _ENTRY)], {}, len(self._host)
         for name, code in _PASSES.items():
-            counts = (ctypes.c_int64 * 3)()
+            counts = (ctypes.c_int64 * 4)()
             fixed = (code, _native.ptr(self._host), len(self._host), heads, kv_heads, head_dim, int(causal))
             _native.check(lib.ct_attention_plan(*fixed, None, 0, counts), "ct_attention_plan")
-            size = counts[0] + counts[1]
+            size = counts[0] + counts[1] + counts[3]
             entries = torch.empty(size, _ENTRY, dtype=torch.int32)
             if size:
                 _native.check(lib.ct_attention_plan(*fixed, _native.ptr(entries), size, counts), "ct_attention_plan")
@@ -214,12 +214,13 @@ class _PackedAttention(torch.autograd.Function):
             rows, keys, stream = tables.rows, tables.keys, _native.stream_of(q)
             tables.use(stream)
             delta = torch.empty_like(stats)
-            workspace = _workspace(keys.workspace, q.device)
+            nbytes = max(rows.workspace, keys.workspace)   # one pass after the other
+            workspace = _workspace(nbytes, q.device)
             with _native.device_of(q):
                 status = _native.library().ct_attention_backward(
                     _operands(q, k, v, tables, causal, scale), rows.entries, rows.counts, keys.entries, keys.counts,
                     out.data_ptr(), stats.data_ptr(), dout.data_ptr(), dout.stride(0), dout.stride(1), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                    _native.ptr(workspace), keys.workspace, stream)
+                    _native.ptr(workspace), nbytes, stream)
             _native.check(status, "ct_attention_backward")
         return dq, dk, dv, None, None, None
 

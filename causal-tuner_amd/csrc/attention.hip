@@ -52,8 +52,17 @@ struct Record {
     int64_t q_start, q_len, k_start, k_len;
 };
 
+// A plan: pieces of work, joins of what was cut, and the workgroups' lists of pieces.
 struct Item {
-    int32_t record, begin, lo, hi, slot, pad0, pad1, pad2;
+    int32_t record, begin;  // first row (forward, dq) or key (dk, dv) of the tile
+    int32_t lo, hi;         // piece: its keys or rows; join: its first partial and their number
+    int32_t slot;           // piece: its partial, or -1 for the whole tile; join: first row in the tile
+    int32_t rows;           // join: rows or keys
+    int32_t pad0, pad1;
+};
+
+struct Group {
+    int32_t first, count, pad[6];
 };
 
 struct AttnParams {
@@ -63,6 +72,7 @@ struct AttnParams {
     int64_t do_token, do_head;                                  // bytes
     const Record *records;
     const Item *items;
+    const Group *groups;
     char *dst0, *dst1;    // out | dq | dk, dv
     int64_t d_token;      // bytes between tokens of dst0 and dst1
     float *stats;         // [tokens, heads] lse * log2(e), +inf where a row sees no key
@@ -224,6 +234,14 @@ __device__ __forceinline__ f32x16 splat(float v) {
 // The wave's number in its workgroup, known to be the same in all its lanes.
 __device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
 
+// The lane, as a value that the compiler cannot carry from one piece of work to the next: what
+// depends on it is made anew instead of filling registers through the main loop.
+__device__ __forceinline__ int fresh_lane() {
+    int lane = (int)threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
 // Value of the same column in the other half of the wave.
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 
@@ -300,10 +318,12 @@ template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) void attention_forward(AttnParams a) {
     constexpr int KT = kKeyTile<T>, kUnits = KT * Tile<T, DP>::kChunks;
     __shared__ uint4 sk[2][kUnits], sv[2][kUnits];
-    const Item item = a.items[blockIdx.x / a.kv_heads];
+    const Group group = a.groups[blockIdx.x / a.kv_heads];
     const int kv_head = blockIdx.x % a.kv_heads;
+    for (int piece = 0; piece < group.count; ++piece) {
+    const Item item = a.items[group.first + piece];
     const Record rec = a.records[item.record];
-    const int lane = threadIdx.x & 63, wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
+    const int lane = fresh_lane(), wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
 
     const RowOf row(a, rec, kv_head, (int64_t)item.begin + wave * kWaveCols + (lane & 31));
     int least, most;
@@ -393,7 +413,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
 
     const float sum = run.sum + other_half(run.sum);
     const int d0 = 4 * (lane >> 5);
-    if (!row.valid) return;
+    if (!row.valid) continue;
     if (item.slot < 0) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         char *dst = a.dst0 + row.token * a.o_token + row.head * a.o_head;
@@ -418,44 +438,82 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
                     make_float4(o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3]);
         if (lane < 32) *reinterpret_cast<float2 *>(a.part1 + 2 * at) = make_float2(run.m2, sum);
     }
+    }
 }
 
 // Joins the key ranges of split rows: with M = max_s m_s, o = sum_s 2^(m_s - M) o_s over
-// sum_s 2^(m_s - M) sum_s. One wave per row, the parts in order.
+// sum_s 2^(m_s - M) sum_s. DP / 4 threads per row and part; parts past the fourth of a row are
+// shared out over up to 8 such teams, whose sums are added in order.
+__host__ __device__ __forceinline__ int join_teams(int parts) { return parts <= 4 ? 1 : parts <= 8 ? 2 : parts <= 16 ? 4 : 8; }
+__host__ __device__ __forceinline__ int join_rows(int parts, int dp) { return kThreads / (dp / 4) / join_teams(parts); }
+
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads) void attention_join(AttnParams a, const Item *joins, int tile) {
-    const Item join = joins[blockIdx.x / (a.kv_heads * (tile / 4))];
-    const int rest = blockIdx.x % (a.kv_heads * (tile / 4));
-    const int kv_head = rest % a.kv_heads, lane = threadIdx.x & 63;
-    const int r = rest / a.kv_heads * 4 + (threadIdx.x >> 6);
-    const Record rec = a.records[join.record];
-    const RowOf row(a, rec, kv_head, (int64_t)join.begin + r);
-    if (!row.valid) return;
-    const int64_t first = ((int64_t)join.lo * a.kv_heads + kv_head) * tile + r, step = (int64_t)a.kv_heads * tile;
+    constexpr int kLanes = DP / 4;
+    __shared__ float4 steams[kThreads];
+    __shared__ float ssum[kThreads / kLanes];
+    const Item join = joins[blockIdx.x / a.kv_heads];
+    const int kv_head = blockIdx.x % a.kv_heads, teams = join_teams(join.hi);
+    const int place = threadIdx.x / kLanes, lane = threadIdx.x % kLanes, team = place % teams;
+    const int r = join.slot + place / teams;
+    const bool wanted = r < join.slot + join.rows;
+    const int64_t first = ((int64_t)join.lo * a.kv_heads + kv_head) * tile + (wanted ? r : 0);
+    const int64_t step = (int64_t)a.kv_heads * tile;
     float top = -INFINITY;
+#pragma unroll 4
     for (int s = 0; s < join.hi; ++s) top = fmaxf(top, a.part1[2 * (first + s * step)]);
     const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, acc[DP / 64];
-#pragma unroll
-    for (int j = 0; j < DP / 64; ++j) acc[j] = 0.0f;
-    for (int s = 0; s < join.hi; ++s) {
+    float sum = 0.0f;
+    float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int s = team; s < join.hi; s += teams) {
         const int64_t at = first + s * step;
-        const float w = __builtin_amdgcn_exp2f(a.part1[2 * at] - ref);
-        sum = __builtin_fmaf(w, a.part1[2 * at + 1], sum);
-#pragma unroll
-        for (int j = 0; j < DP / 64; ++j) acc[j] = __builtin_fmaf(w, a.part0[at * DP + lane * (DP / 64) + j], acc[j]);
+        const float2 ms = *reinterpret_cast<const float2 *>(a.part1 + 2 * at);
+        const float4 x = *reinterpret_cast<const float4 *>(a.part0 + at * DP + 4 * lane);
+        const float w = __builtin_amdgcn_exp2f(ms.x - ref);
+        sum = __builtin_fmaf(w, ms.y, sum);
+        acc.x = __builtin_fmaf(w, x.x, acc.x);
+        acc.y = __builtin_fmaf(w, x.y, acc.y);
+        acc.z = __builtin_fmaf(w, x.z, acc.z);
+        acc.w = __builtin_fmaf(w, x.w, acc.w);
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    char *dst = a.dst0 + row.token * a.o_token + row.head * a.o_head;
-#pragma unroll
-    for (int j = 0; j < DP / 64; ++j) {
-        const int d = lane * (DP / 64) + j;
-        if (d < a.head_dim) {
-            if constexpr (sizeof(T) == 2) reinterpret_cast<uint16_t *>(dst)[d] = bf16_bits(acc[j] * inv);
-            else reinterpret_cast<float *>(dst)[d] = acc[j] * inv;
+    if (teams > 1) {
+        steams[threadIdx.x] = acc;
+        if (lane == 0) ssum[place] = sum;
+        __syncthreads();
+        if (team) return;
+        for (int t = 1; t < teams; ++t) {
+            const float4 x = steams[threadIdx.x + t * kLanes];
+            sum += ssum[place + t];
+            acc.x += x.x;
+            acc.y += x.y;
+            acc.z += x.z;
+            acc.w += x.w;
         }
     }
+    if (!wanted) return;
+    const Record rec = a.records[join.record];
+    const RowOf row(a, rec, kv_head, (int64_t)join.begin + r);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (4 * lane < a.head_dim)
+        store4<T>(a.dst0 + row.token * a.o_token + row.head * a.o_head, 4 * lane, acc.x * inv, acc.y * inv, acc.z * inv,
+                  acc.w * inv);
     if (lane == 0) a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+}
+
+// Sum of the parts of one row or key, in order, for four elements.
+template <int DP>
+__device__ __forceinline__ float4 sum_parts(const float *part, int64_t at, int64_t step, int count) {
+    float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int s = 0; s < count; ++s) {
+        const float4 x = *reinterpret_cast<const float4 *>(part + (at + s * step) * DP);
+        v.x += x.x;
+        v.y += x.y;
+        v.z += x.z;
+        v.w += x.w;
+    }
+    return v;
 }
 
 // ------------------------------------------------------------------ dq (and delta)
@@ -479,10 +537,12 @@ template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) void attention_dq(AttnParams a) {
     constexpr int kUnits = kStep * Tile<T, DP>::kChunks;
     __shared__ uint4 sk[kStages][kUnits], sv[kStages][kUnits];
-    const Item item = a.items[blockIdx.x / a.kv_heads];
+    const Group group = a.groups[blockIdx.x / a.kv_heads];
     const int kv_head = blockIdx.x % a.kv_heads;
+    for (int piece = 0; piece < group.count; ++piece) {
+    const Item item = a.items[group.first + piece];
     const Record rec = a.records[item.record];
-    const int lane = threadIdx.x & 63, wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
+    const int lane = fresh_lane(), wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
 
     const RowOf row(a, rec, kv_head, (int64_t)item.begin + wave * kWaveCols + (lane & 31));
     int least, most;
@@ -499,7 +559,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
     if (row.valid) {
         const int64_t at = row.token * a.heads + row.head;
         lse = a.stats[at];
-        if (lane < 32) a.delta[at] = delta;
+        if (lane < 32 && item.lo == 0) a.delta[at] = delta;
     }
     row_fragments<T, DP>(a.q + row.token * a.q_token + row.head * a.q_head, qf, row.valid, chunks, lane);
 
@@ -558,17 +618,44 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
         }
         __syncthreads();
     });
-    if (!row.valid) return;
-    char *dst = a.dst0 + row.token * a.d_token + (int64_t)row.head * a.head_dim * (int)sizeof(T);
+    if (!row.valid) continue;
+    const int d0 = 4 * (lane >> 5);
+    if (item.slot < 0) {
+        char *dst = a.dst0 + row.token * a.d_token + (int64_t)row.head * a.head_dim * (int)sizeof(T);
 #pragma unroll
-    for (int n = 0; n < DP / 32; ++n)
+        for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const int d = 32 * n + 2 * i + 4 * (lane >> 5);
-            if (d < a.head_dim)
-                store4<T>(dst, d, o[n][i] * a.scale, o[n][i + 1] * a.scale, o[n][i + 2] * a.scale,
-                          o[n][i + 3] * a.scale);
-        }
+            for (int i = 0; i < 16; i += 4) {
+                const int d = 32 * n + 2 * i + d0;
+                if (d < a.head_dim)
+                    store4<T>(dst, d, o[n][i] * a.scale, o[n][i + 1] * a.scale, o[n][i + 2] * a.scale,
+                              o[n][i + 3] * a.scale);
+            }
+    } else {
+        float *dst = a.part0 + (((int64_t)item.slot * a.kv_heads + kv_head) * (32 * WAVES) + wave * kWaveCols +
+                                (lane & 31)) * DP;
+#pragma unroll
+        for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float4 *>(dst + 32 * n + 2 * i + d0) =
+                    make_float4(o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3]);
+    }
+    }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kThreads) void attention_dq_join(AttnParams a, const Item *joins, int tile) {
+    const Item join = joins[blockIdx.x / a.kv_heads];
+    const int kv_head = blockIdx.x % a.kv_heads, place = threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
+    if (place >= join.rows || d >= a.head_dim) return;
+    const int64_t step = (int64_t)a.kv_heads * tile;
+    const float4 v = sum_parts<DP>(a.part0 + d, ((int64_t)join.lo * a.kv_heads + kv_head) * tile + join.slot + place, step,
+                                   join.hi);
+    const Record rec = a.records[join.record];
+    const RowOf row(a, rec, kv_head, (int64_t)join.begin + join.slot + place);
+    store4<T>(a.dst0 + row.token * a.d_token + (int64_t)row.head * a.head_dim * (int)sizeof(T), d, v.x * a.scale,
+              v.y * a.scale, v.z * a.scale, v.w * a.scale);
 }
 
 // ------------------------------------------------------------------ dk, dv
@@ -586,10 +673,12 @@ __global__ __launch_bounds__(64 * kKeyWaves, 2) void attention_dkv(AttnParams a)
     __shared__ uint4 sq[kStages][kUnits], sg[kStages][kUnits];
     __shared__ float slse[kStages][kStep], sdelta[kStages][kStep];   // negated
     __shared__ f32x4 sp[2][kKeyWaves / 2][4][64];
-    const Item item = a.items[blockIdx.x / a.kv_heads];
+    const Group group = a.groups[blockIdx.x / a.kv_heads];
     const int kv_head = blockIdx.x % a.kv_heads;
+    for (int piece = 0; piece < group.count; ++piece) {
+    const Item item = a.items[group.first + piece];
     const Record rec = a.records[item.record];
-    const int lane = threadIdx.x & 63, wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
+    const int lane = fresh_lane(), wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
     const int pair = wave & 3;                // waves w and w + 4 run on one SIMD
     const bool for_dv = wave < kKeyWaves / 2;
 
@@ -729,7 +818,7 @@ __global__ __launch_bounds__(64 * kKeyWaves, 2) void attention_dkv(AttnParams a)
     const int d0 = 4 * (lane >> 5);
     const float scale = for_dv ? 1.0f : a.scale;
     if (item.slot < 0) {
-        if (!valid) return;
+        if (!valid) continue;
         char *dst = (for_dv ? a.dst1 : a.dst0) + kv * a.d_token + (int64_t)kv_head * a.head_dim * (int)sizeof(T);
 #pragma unroll
         for (int n = 0; n < DP / 32; ++n)
@@ -750,28 +839,20 @@ __global__ __launch_bounds__(64 * kKeyWaves, 2) void attention_dkv(AttnParams a)
                 *reinterpret_cast<float4 *>(dst + 32 * n + 2 * i + d0) =
                     make_float4(acc[n][i], acc[n][i + 1], acc[n][i + 2], acc[n][i + 3]);
     }
+    }
 }
 
 // Sums the row ranges of split key tiles in order: one thread per four elements of a key.
 template <typename T, int DP>
 __global__ __launch_bounds__(kThreads) void attention_dkv_join(AttnParams a, const Item *joins) {
-    constexpr int kPer = kThreads * 4 / DP;   // keys per workgroup
-    const int blocks = kTile / kPer * a.kv_heads;
-    const Item join = joins[blockIdx.x / blocks];
-    const int rest = blockIdx.x % blocks, kv_head = rest % a.kv_heads;
-    const int j = rest / a.kv_heads * kPer + threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
-    const Record rec = a.records[join.record];
-    const int64_t key = (int64_t)join.begin + j;
-    if (key >= rec.k_len || d >= a.head_dim) return;
-    const int64_t step = (int64_t)a.kv_heads * kTile * DP;
-    int64_t at = (((int64_t)join.lo * a.kv_heads + kv_head) * kTile + j) * DP + d;
-    float4 dk = make_float4(0, 0, 0, 0), dv = dk;
-    for (int s = 0; s < join.hi; ++s, at += step) {
-        const float4 x = *reinterpret_cast<const float4 *>(a.part0 + at), y = *reinterpret_cast<const float4 *>(a.part1 + at);
-        dk.x += x.x; dk.y += x.y; dk.z += x.z; dk.w += x.w;
-        dv.x += y.x; dv.y += y.y; dv.z += y.z; dv.w += y.w;
-    }
-    const int64_t off = (rec.k_start + key) * a.d_token + (int64_t)kv_head * a.head_dim * (int)sizeof(T);
+    const Item join = joins[blockIdx.x / a.kv_heads];
+    const int kv_head = blockIdx.x % a.kv_heads, place = threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
+    if (place >= join.rows || d >= a.head_dim) return;
+    const int64_t step = (int64_t)a.kv_heads * kTile;
+    const int64_t at = ((int64_t)join.lo * a.kv_heads + kv_head) * kTile + join.slot + place;
+    const float4 dk = sum_parts<DP>(a.part0 + d, at, step, join.hi), dv = sum_parts<DP>(a.part1 + d, at, step, join.hi);
+    const int64_t key = a.records[join.record].k_start + join.begin + join.slot + place;
+    const int64_t off = key * a.d_token + (int64_t)kv_head * a.head_dim * (int)sizeof(T);
     store4<T>(a.dst0 + off, d, dk.x * a.scale, dk.y * a.scale, dk.z * a.scale, dk.w * a.scale);
     store4<T>(a.dst1 + off, d, dv.x, dv.y, dv.z, dv.w);
 }
@@ -783,6 +864,7 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_join(AttnParams a, con
 constexpr int kRowWaves = RW, kRowTile = 32 * kRowWaves;
 constexpr int64_t kMaxRows = 0x7fffffff - 2 * kTile;
 
+constexpr int64_t kRowFixed = 3, kKeyFixed = 6;   // a piece's fixed cost in units of kUnit
 constexpr int64_t kMaxPitch = (int64_t)1 << 24;   // bytes between tokens of k and v
 
 // 64 packed rows span at most 64 / group + 2 tokens and all heads of the group.
@@ -852,80 +934,149 @@ int by_type(int dtype, int dp, F f) {
 }
 
 int64_t parts_per_item(int32_t pass, int dp) {   // floats
-    return pass == CT_ATTENTION_KEYS ? 2 * (int64_t)kTile * dp : (int64_t)kRowTile * (dp + 2);
+    return pass == CT_ATTENTION_KEYS ? 2 * (int64_t)kTile * dp
+                                     : (int64_t)kRowTile * (dp + (pass == CT_ATTENTION_FORWARD ? 2 : 0));
 }
 
-// Workgroups that keep the card busy: two per CU in the forward, one (of twice the
-// registers) in the dk, dv kernel, and some more, since the ranges end at different times.
-constexpr int64_t kForwardGroups = 512, kKeyGroups = 512;
+// Workgroups that the card runs at once: two of 4 waves per CU in the forward and dq, one of 8
+// waves (two with heads up to 64) in the dk, dv kernel.
+int64_t groups_at_once(int32_t pass, int dp) { return pass == CT_ATTENTION_KEYS && dp > 64 ? 256 : 512; }
 
-void plan_items(int32_t pass, const Record *rec, int64_t n, int64_t kv_heads, int64_t group, bool causal,
-                std::vector<Item> &items, std::vector<Item> &joins, int64_t &slots) {
+constexpr int64_t kUnit = 64;   // keys or rows: pieces are cut at its multiples
+
+int64_t units_of(const Item &it) { return cdiv(it.hi - it.lo, kUnit); }
+
+// Fills workgroups one after the other with the tiles' units until each has taken `cap`, where
+// a piece costs its units and `fixed` (its rows' or keys' load, its result's store). Returns the
+// number of workgroups; with `groups`, writes them and their pieces down.
+int64_t fill(const std::vector<Item> &tiles, int64_t cap, int64_t fixed, std::vector<Item> *pieces,
+             std::vector<Group> *groups) {
+    int64_t count = 0, left = 0;
+    for (const Item &tile : tiles) {
+        for (int64_t lo = tile.lo;;) {
+            const int64_t units = cdiv(tile.hi - lo, kUnit);
+            // a workgroup's rest that is too short for its fixed cost stays unused
+            if (left < fixed + std::min<int64_t>(units, fixed)) {
+                left = cap;
+                ++count;
+                if (groups) groups->push_back({(int32_t)pieces->size(), 0, {}});
+            }
+            const int64_t take = std::min<int64_t>(units, std::max<int64_t>(1, left - fixed));
+            left -= take + fixed;
+            if (groups) {
+                Item piece = tile;
+                piece.lo = (int32_t)lo;
+                piece.hi = (int32_t)std::min<int64_t>(tile.hi, lo + take * kUnit);
+                piece.slot = piece.lo == tile.lo && piece.hi == tile.hi ? -1 : 0;
+                pieces->push_back(piece);
+                ++groups->back().count;
+            }
+            lo += take * kUnit;
+            if (lo >= tile.hi) break;
+        }
+    }
+    return count;
+}
+
+struct Plan {
+    std::vector<Item> pieces, joins;
+    std::vector<Group> groups;
+    int64_t slots = 0;
+};
+
+void make_plan(int32_t pass, const Record *rec, int64_t n, int64_t kv_heads, int64_t group, int dp, bool causal, Plan &plan) {
     const bool keys = pass == CT_ATTENTION_KEYS;
     const int64_t tile = keys ? kTile : kRowTile;
-    constexpr int64_t kUnit = 64;   // ranges are cut at multiples of a tile
-    int64_t work = 0;
+    std::vector<Item> tiles;
+    int64_t work = 0, longest = 0;
     for (int64_t i = 0; i < n; ++i) {
-        const int64_t rows = rec[i].q_len * group, span = keys ? rec[i].k_len : rows;
+        const int64_t rows = rec[i].q_len * group, span = keys ? rec[i].k_len : rows, shift = rec[i].k_len - rec[i].q_len;
         for (int64_t b = 0; b < span; b += tile) {
             Item it = {};
             it.record = (int32_t)i;
             it.begin = (int32_t)b;
             it.slot = -1;
-            const int64_t shift = rec[i].k_len - rec[i].q_len;
+            it.rows = (int32_t)std::min(tile, span - b);
             if (keys) {   // rows that see the tile's first key, from a whole tile of rows on
                 const int64_t t = causal ? std::max<int64_t>(0, b - shift) : 0;
                 it.lo = (int32_t)std::min(t * group / kUnit * kUnit, rows);
                 it.hi = (int32_t)rows;
             } else {      // keys that the tile's last row sees
-                const int64_t t = (std::min(rows, b + tile) - 1) / group;
+                const int64_t t = (b + it.rows - 1) / group;
                 it.hi = (int32_t)(causal ? std::min(rec[i].k_len, std::max<int64_t>(0, t + 1 + shift)) : rec[i].k_len);
             }
-            work += cdiv(it.hi - it.lo, kUnit);
-            items.push_back(it);
+            work += units_of(it);
+            longest = std::max(longest, units_of(it));
+            tiles.push_back(it);
         }
     }
-    slots = 0;
-    if (pass != CT_ATTENTION_ROWS) {
-        const int64_t target = std::max<int64_t>(1, (keys ? kKeyGroups : kForwardGroups) / kv_heads);
-        const int64_t range = std::max<int64_t>(keys ? 4 : 2, cdiv(work, target)) * kUnit;
-        const bool enough = !keys && (int64_t)items.size() >= target;
-        std::vector<Item> whole;
-        whole.swap(items);
-        for (const Item &it : whole) {
-            const int64_t parts = enough ? 1 : std::max<int64_t>(1, cdiv(it.hi - it.lo, range));
-            if (parts == 1) {
-                items.push_back(it);
-                continue;
-            }
-            const int64_t step = cdiv(cdiv(it.hi - it.lo, parts), kUnit) * kUnit;
-            Item join = it;
-            join.lo = (int32_t)slots;
-            for (int64_t lo = it.lo; lo < it.hi; lo += step) {
-                Item part = it;
-                part.lo = (int32_t)lo;
-                part.hi = (int32_t)std::min<int64_t>(it.hi, lo + step);
-                part.slot = (int32_t)slots++;
-                items.push_back(part);
-            }
-            join.hi = (int32_t)(slots - join.lo);
-            joins.push_back(join);
+    const int64_t at_once = std::max<int64_t>(1, groups_at_once(pass, dp) / kv_heads);
+    if ((int64_t)tiles.size() >= 2 * at_once && longest * at_once <= work) {
+        // Enough whole tiles, none of them longer than a workgroup's share: longest first, so
+        // that what starts last ends soon.
+        std::stable_sort(tiles.begin(), tiles.end(),
+                         [](const Item &x, const Item &y) { return units_of(x) > units_of(y); });
+        for (const Item &it : tiles) {
+            plan.groups.push_back({(int32_t)plan.pieces.size(), 1, {}});
+            plan.pieces.push_back(it);
+        }
+        return;
+    }
+    // Otherwise every workgroup gets the same share of all units, cutting tiles where it ends.
+    const int64_t fixed = keys ? kKeyFixed : kRowFixed;
+    int64_t low = 2 * fixed, high = std::max<int64_t>(low, work + fixed * (int64_t)tiles.size());
+    while (low < high) {
+        const int64_t mid = (low + high) / 2;
+        if (fill(tiles, mid, fixed, nullptr, nullptr) <= at_once) high = mid;
+        else low = mid + 1;
+    }
+    fill(tiles, high, fixed, &plan.pieces, &plan.groups);
+    for (size_t k = 0; k < plan.pieces.size();) {
+        if (plan.pieces[k].slot < 0) {
+            ++k;
+            continue;
+        }
+        Item join = plan.pieces[k];
+        join.lo = (int32_t)plan.slots;
+        const size_t from = k;
+        for (; k < plan.pieces.size() && plan.pieces[k].record == join.record && plan.pieces[k].begin == join.begin; ++k)
+            plan.pieces[k].slot = (int32_t)plan.slots++;
+        join.hi = (int32_t)(k - from);
+        const int at_a_time = pass == CT_ATTENTION_FORWARD ? join_rows(join.hi, dp) : kThreads / (dp / 4);
+        const int32_t rows = join.rows;
+        for (int32_t r = 0; r < rows; r += at_a_time) {
+            join.slot = r;
+            join.rows = std::min(at_a_time, rows - r);
+            plan.joins.push_back(join);
         }
     }
-    // Longest first: what starts last then ends soon.
-    std::stable_sort(items.begin(), items.end(),
-                     [](const Item &x, const Item &y) { return x.hi - x.lo > y.hi - y.lo; });
+    // The pieces keep their order; the workgroups with most to do start first.
+    auto cost = [&](const Group &g) {
+        int64_t c = 0;
+        for (int32_t k = 0; k < g.count; ++k) c += units_of(plan.pieces[(size_t)(g.first + k)]) + fixed;
+        return c;
+    };
+    std::stable_sort(plan.groups.begin(), plan.groups.end(), [&](const Group &x, const Group &y) { return cost(x) > cost(y); });
 }
 
-bool items_ok(int64_t items, int64_t joins, int64_t slots, int64_t kv_heads) {
-    const int64_t most = 0x7fffffff / (kTile * kv_heads);
-    return items >= 0 && joins >= 0 && slots >= 0 && items <= most && joins <= most && slots <= most;
+// counts: pieces, joins, partials, workgroups.
+bool counts_ok(const int64_t *counts, int64_t kv_heads) {
+    for (int i = 0; i < 4; ++i)
+        if (counts[i] < 0 || counts[i] > 0x7fffffff / (kTile * kv_heads)) return false;
+    return true;
+}
+
+void set_plan(AttnParams &a, const int32_t *plan, const int64_t *counts) {
+    a.items = reinterpret_cast<const Item *>(plan);
+    a.groups = reinterpret_cast<const Group *>(a.items + counts[0] + counts[1]);
 }
 
 }  // namespace
 }  // namespace ct
 
 using namespace ct;
+
+static_assert(sizeof(Item) == 4 * kEntry && sizeof(Group) == 4 * kEntry, "plan entries");
 
 extern "C" int ct_attention_plan(int32_t pass, const int64_t *records, int64_t n_records, int32_t heads,
                                  int32_t kv_heads, int32_t head_dim, int32_t causal, int32_t *entries,
@@ -946,17 +1097,18 @@ extern "C" int ct_attention_plan(int32_t pass, const int64_t *records, int64_t n
     }
     if (tiles > 0x7fffffff / (4 * kTile * kv_heads)) return -CT_EINVAL_SHAPE;
     try {
-        std::vector<Item> items, joins;
-        int64_t slots = 0;
-        plan_items(pass, rec, n_records, kv_heads, group, causal != 0, items, joins, slots);
-        counts[0] = (int64_t)items.size();
-        counts[1] = (int64_t)joins.size();
-        counts[2] = slots;
-        if (!items_ok(counts[0], counts[1], counts[2], kv_heads)) return -CT_EINVAL_SHAPE;
+        Plan made;
+        make_plan(pass, rec, n_records, kv_heads, group, padded_dim(head_dim), causal != 0, made);
+        counts[0] = (int64_t)made.pieces.size();
+        counts[1] = (int64_t)made.joins.size();
+        counts[2] = made.slots;
+        counts[3] = (int64_t)made.groups.size();
+        if (!counts_ok(counts, kv_heads)) return -CT_EINVAL_SHAPE;
         if (!entries) return 0;
-        if (capacity < counts[0] + counts[1]) return -CT_EINVAL_WORKSPACE;
-        std::copy(items.begin(), items.end(), reinterpret_cast<Item *>(entries));
-        std::copy(joins.begin(), joins.end(), reinterpret_cast<Item *>(entries) + items.size());
+        if (capacity < counts[0] + counts[1] + counts[3]) return -CT_EINVAL_WORKSPACE;
+        Item *dst = std::copy(made.pieces.begin(), made.pieces.end(), reinterpret_cast<Item *>(entries));
+        dst = std::copy(made.joins.begin(), made.joins.end(), dst);
+        std::copy(made.groups.begin(), made.groups.end(), reinterpret_cast<Group *>(dst));
     } catch (...) {
         return (int)hipErrorOutOfMemory;
     }
@@ -973,15 +1125,15 @@ extern "C" int ct_attention_forward(const ct_attention *c, const int32_t *plan, 
     AttnParams a;
     if (const int status = fill_params(c, a)) return status;
     if (!counts) return -CT_EINVAL_POINTER;
-    const int64_t n = counts[0], joins = counts[1], slots = counts[2];
-    if (!items_ok(n, joins, slots, c->kv_heads)) return -CT_EINVAL_SHAPE;
-    if (n == 0) return 0;
+    if (!counts_ok(counts, c->kv_heads)) return -CT_EINVAL_SHAPE;
+    const int64_t joins = counts[1], slots = counts[2], groups = counts[3];
+    if (groups == 0) return 0;
     if (!plan || !out || !stats || (uintptr_t)plan % 16 || (uintptr_t)out % 16) return -CT_EINVAL_POINTER;
     if (slots && (!workspace || (uintptr_t)workspace % 16 ||
                   workspace_bytes < ct_attention_workspace(CT_ATTENTION_FORWARD, slots, c->kv_heads, c->head_dim)))
         return -CT_EINVAL_WORKSPACE;
     const int dp = padded_dim(c->head_dim);
-    a.items = reinterpret_cast<const Item *>(plan);
+    set_plan(a, plan, counts);
     a.dst0 = (char *)out;
     a.stats = stats;
     a.part0 = (float *)workspace;
@@ -989,14 +1141,13 @@ extern "C" int ct_attention_forward(const ct_attention *c, const int32_t *plan, 
     return by_type(c->dtype, dp, [&](auto type, auto dim) {
         typedef decltype(type) T;
         constexpr int DP = decltype(dim)::value;
-        attention_forward<T, DP, kRowWaves><<<dim3((unsigned)(n * c->kv_heads)), dim3(64 * kRowWaves), 0, stream>>>(a);
+        attention_forward<T, DP, kRowWaves>
+            <<<dim3((unsigned)(groups * c->kv_heads)), dim3(64 * kRowWaves), 0, stream>>>(a);
         if (const int status = status_of_last_launch()) return status;
-        if (joins) {
-            attention_join<T, DP><<<dim3((unsigned)(joins * c->kv_heads * (kRowTile / 4))), dim3(kThreads), 0, stream>>>(
-                a, a.items + n, kRowTile);
-            return status_of_last_launch();
-        }
-        return 0;
+        if (!joins) return 0;
+        attention_join<T, DP><<<dim3((unsigned)(joins * c->kv_heads)), dim3(kThreads), 0, stream>>>(
+            a, a.items + counts[0], kRowTile);
+        return status_of_last_launch();
     });
 }
 
@@ -1008,10 +1159,8 @@ extern "C" int ct_attention_backward(const ct_attention *c, const int32_t *row_p
     AttnParams a;
     if (const int status = fill_params(c, a)) return status;
     if (!row_counts || !key_counts) return -CT_EINVAL_POINTER;
-    const int64_t rows = row_counts[0], keys = key_counts[0], joins = key_counts[1], slots = key_counts[2];
-    if (!items_ok(rows, row_counts[1], row_counts[2], c->kv_heads) || !items_ok(keys, joins, slots, c->kv_heads) ||
-        row_counts[1] || row_counts[2])
-        return -CT_EINVAL_SHAPE;
+    if (!counts_ok(row_counts, c->kv_heads) || !counts_ok(key_counts, c->kv_heads)) return -CT_EINVAL_SHAPE;
+    const int64_t rows = row_counts[3], keys = key_counts[3], row_slots = row_counts[2], key_slots = key_counts[2];
     const int64_t size = c->dtype == CT_BF16 ? 2 : 4;
     if (rows) {
         if (!row_plan || !out || !stats || !dout || !delta || !dq ||
@@ -1024,9 +1173,10 @@ extern "C" int ct_attention_backward(const ct_attention *c, const int32_t *row_p
     }
     if (keys && (!key_plan || !dk || !dv || ((uintptr_t)key_plan | (uintptr_t)dk | (uintptr_t)dv) % 16))
         return -CT_EINVAL_POINTER;
-    if (slots && (!workspace || (uintptr_t)workspace % 16 ||
-                  workspace_bytes < ct_attention_workspace(CT_ATTENTION_KEYS, slots, c->kv_heads, c->head_dim)))
-        return -CT_EINVAL_WORKSPACE;
+    // the two passes use the workspace one after the other
+    const int64_t needed = std::max(ct_attention_workspace(CT_ATTENTION_ROWS, row_slots, c->kv_heads, c->head_dim),
+                                    ct_attention_workspace(CT_ATTENTION_KEYS, key_slots, c->kv_heads, c->head_dim));
+    if (needed && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < needed)) return -CT_EINVAL_WORKSPACE;
     const int dp = padded_dim(c->head_dim);
     a.out = (const char *)out;
     a.dout = (const char *)dout;
@@ -1037,27 +1187,32 @@ extern "C" int ct_attention_backward(const ct_attention *c, const int32_t *row_p
     return by_type(c->dtype, dp, [&](auto type, auto dim) {
         typedef decltype(type) T;
         constexpr int DP = decltype(dim)::value;
+        AttnParams r = a;
+        r.part0 = (float *)workspace;
         if (rows) {   // dq first: it leaves delta for the other kernel
-            AttnParams r = a;
-            r.items = reinterpret_cast<const Item *>(row_plan);
+            set_plan(r, row_plan, row_counts);
             r.dst0 = (char *)dq;
             r.d_token = a.o_token;
-            attention_dq<T, DP, kRowWaves><<<dim3((unsigned)(rows * c->kv_heads)), dim3(64 * kRowWaves), 0, stream>>>(r);
+            attention_dq<T, DP, kRowWaves>
+                <<<dim3((unsigned)(rows * c->kv_heads)), dim3(64 * kRowWaves), 0, stream>>>(r);
             if (const int status = status_of_last_launch()) return status;
+            if (row_counts[1]) {
+                attention_dq_join<T, DP><<<dim3((unsigned)(row_counts[1] * c->kv_heads)), dim3(kThreads), 0, stream>>>(
+                    r, r.items + row_counts[0], kRowTile);
+                if (const int status = status_of_last_launch()) return status;
+            }
         }
         if (!keys) return 0;
-        AttnParams r = a;
-        r.items = reinterpret_cast<const Item *>(key_plan);
+        set_plan(r, key_plan, key_counts);
         r.dst0 = (char *)dk;
         r.dst1 = (char *)dv;
         r.d_token = c->kv_heads * a.o_head;
-        r.part0 = (float *)workspace;
-        r.part1 = r.part0 + slots * c->kv_heads * kTile * DP;
+        r.part1 = r.part0 + key_slots * c->kv_heads * kTile * DP;
         attention_dkv<T, DP><<<dim3((unsigned)(keys * c->kv_heads)), dim3(64 * kKeyWaves), 0, stream>>>(r);
         if (const int status = status_of_last_launch()) return status;
-        if (!joins) return 0;
-        attention_dkv_join<T, DP><<<dim3((unsigned)(joins * c->kv_heads * (kTile * DP / (4 * kThreads)))),
-                                    dim3(kThreads), 0, stream>>>(r, r.items + keys);
+        if (!key_counts[1]) return 0;
+        attention_dkv_join<T, DP><<<dim3((unsigned)(key_counts[1] * c->kv_heads)), dim3(kThreads), 0, stream>>>(
+            r, r.items + key_counts[0]);
         return status_of_last_launch();
     });
 }
