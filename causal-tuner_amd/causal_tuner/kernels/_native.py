@@ -134,7 +134,7 @@ _SIGNATURES = {
     "ct_cast_f32_bf16": (ctypes.c_int, [_P, _P, _P, _I32, _P]),
     "ct_adamw_step": (ctypes.c_int, [_P, _I64, _P, _I64, _I64, _I32, ctypes.c_double, ctypes.c_double,
                                      ctypes.c_double, ctypes.c_double, ctypes.c_double, _I32, _I32, _P]),
-    "ct_attention_plan": (ctypes.c_int, [_I32, _P, _I64, _I32, _I32, _I32, _I32, _P, _I64, _P]),
+    "ct_attention_plan": (ctypes.c_int, [_I32, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _I64, _P]),
     "ct_attention_workspace": (_I64, [_I32, _I64, _I32, _I32]),
     "ct_attention_forward": (ctypes.c_int, [_ATT, _P, _P, _P, _P, _P, _I64, _P]),
     "ct_attention_backward": (ctypes.c_int, [_ATT, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _I64,

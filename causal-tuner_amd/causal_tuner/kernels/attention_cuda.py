@@ -107,14 +107,14 @@ class AttentionLayout:
                                   dtype=torch.int64).reshape(-1, 4)
         self._tables = {}
 
-    def tables(self, heads, kv_heads, head_dim, causal):
-        key = (heads, kv_heads, head_dim, causal)
+    def tables(self, heads, kv_heads, head_dim, dtype, causal):
+        key = (heads, kv_heads, head_dim, dtype, causal)
         tables = self._tables.get(key)
         if tables is None:
             tables = self._tables[key] = self._make_tables(*key)
         return tables
 
-    def _make_tables(self, heads, kv_heads, head_dim, causal):
+    def _make_tables(self, heads, kv_heads, head_dim, dtype, causal):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AttentionLayout: the first call with a head layout makes its tables and cannot be "
                                "captured; run it once before the capture")
@@ -122,7 +122,8 @@ class AttentionLayout:
         parts, plans, at = [self._host.view(torch.int32).reshape(-1, _ENTRY)], {}, len(self._host)
         for name, code in _PASSES.items():
             counts = (ctypes.c_int64 * 4)()
-            fixed = (code, _native.ptr(self._host), len(self._host), heads, kv_heads, head_dim, int(causal))
+            fixed = (code, _native.ptr(self._host), len(self._host), heads, kv_heads, head_dim, _native.dtype_code(dtype),
+                     int(causal))
             _native.check(lib.ct_attention_plan(*fixed, None, 0, counts), "ct_attention_plan")
             size = counts[0] + counts[1] + counts[3]
             entries = torch.empty(size, _ENTRY, dtype=torch.int32)
@@ -180,7 +181,7 @@ class _PackedAttention(torch.autograd.Function):
         out = (torch.empty if whole else torch.zeros)(tokens, heads, head_dim, dtype=q.dtype, device=q.device)
         stats = torch.empty(tokens, heads, dtype=torch.float32, device=q.device)
         if tokens:
-            tables = layout.tables(heads, kv_heads, head_dim, causal)
+            tables = layout.tables(heads, kv_heads, head_dim, q.dtype, causal)
             plan, stream = tables.forward, _native.stream_of(q)
             tables.use(stream)
             workspace = _workspace(plan.workspace, q.device)
@@ -210,7 +211,7 @@ class _PackedAttention(torch.autograd.Function):
         dq = (torch.empty if whole else torch.zeros)(q.shape, **fresh)
         dk, dv = ((torch.empty if keys_whole else torch.zeros)(k.shape, **fresh) for _ in range(2))
         if tokens or key_tokens:
-            tables = layout.tables(heads, kv_heads, head_dim, causal)
+            tables = layout.tables(heads, kv_heads, head_dim, q.dtype, causal)
             rows, keys, stream = tables.rows, tables.keys, _native.stream_of(q)
             tables.use(stream)
             delta = torch.empty_like(stats)

@@ -112,21 +112,54 @@ struct Tile {
 
 typedef const __attribute__((address_space(3))) char lds_char;
 
-__device__ __forceinline__ lds_char *lds_of(const uint4 *p) { return (lds_char *)p; }
+__device__ __forceinline__ uint32_t lds_of(const uint4 *p) { return (uint32_t)(uintptr_t)(lds_char *)p; }
 
-__device__ __forceinline__ uint4 lds_read16(lds_char *p) {
-    return __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) u32x4 *)p);
+__device__ __forceinline__ uint4 lds_read16(uint32_t at) {
+    return __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)at);
 }
+__device__ __forceinline__ uint2 lds_read_transposed(uint32_t at) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_kt_v4s *)(uintptr_t)at));
+}
+
+// A lane's byte offsets in a tile: of the chunks it reads as rows, and of those it reads
+// transposed. `refresh` once a step keeps the sums with a stage's constant address out of
+// registers: they become immediate offsets of the reads.
+template <typename T, int DP>
+struct Lanes {
+    static constexpr int kFrags = Tile<T, DP>::kFrags, kCols = sizeof(T) == 2 ? DP / 16 : 1;
+    uint32_t row[kFrags], col[kCols];
+    __device__ __forceinline__ explicit Lanes(int lane) {
+        const int h = lane >> 5;
+#pragma unroll
+        for (int s = 0; s < kFrags; ++s) row[s] = (uint32_t)Tile<T, DP>::addr(lane & 31, 2 * s + h);
+        if constexpr (sizeof(T) == 2) {
+            const int r = 4 * h + ((lane & 15) >> 2);
+#pragma unroll
+            for (int n = 0; n < DP / 32; ++n) {
+                const int c = 4 * n + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), o = (lane & 1) * 8;
+                col[2 * n] = (uint32_t)(Tile<T, DP>::addr(r, c) + o);
+                col[2 * n + 1] = (uint32_t)(Tile<T, DP>::addr(r + 8, c) + o);
+            }
+        } else {
+            col[0] = (uint32_t)lane;
+        }
+    }
+    __device__ __forceinline__ void refresh() {
+#pragma unroll
+        for (int s = 0; s < kFrags; ++s) asm volatile("" : "+v"(row[s]));
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) asm volatile("" : "+v"(col[n]));
+    }
+};
 
 // acc[row, col] += sum_d tile[row0 + row][d] * frag[col][d]
 template <typename T, int DP>
 __device__ __forceinline__ void scores(f32x16 &acc, const uint4 *tile, int row0, const uint4 (&frag)[Tile<T, DP>::kFrags],
-                                       int lane) {
-    lds_char *base = lds_of(tile);
-    const int h = lane >> 5, row = lane & 31;
+                                       const Lanes<T, DP> &at) {
+    const uint32_t base = lds_of(tile) + row0 * Tile<T, DP>::kBytes;
 #pragma unroll
     for (int s = 0; s < Tile<T, DP>::kFrags; ++s) {
-        const uint4 a = lds_read16(base + row0 * Tile<T, DP>::kBytes + Tile<T, DP>::addr(row, 2 * s + h));
+        const uint4 a = lds_read16(at.row[s] + base);
         if constexpr (sizeof(T) == 2) {
             acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                           __builtin_bit_cast(bf16x8, frag[s]), acc, 0, 0, 0);
@@ -141,11 +174,10 @@ __device__ __forceinline__ void scores(f32x16 &acc, const uint4 *tile, int row0,
 // acc[b][d, col] += sum_row tile[row0 + row][32 b + d] * p[row, col], p as `scores` leaves it:
 // register i of lane half h is row 8 (i / 4) + 4 h + i % 4.
 template <typename T, int DP>
-__device__ __forceinline__ void outer(f32x16 (&acc)[DP / 32], const uint4 *tile, int row0, const f32x16 &p, int lane) {
-    lds_char *base = lds_of(tile) + row0 * Tile<T, DP>::kBytes;
-    const int h = lane >> 5;
+__device__ __forceinline__ void outer(f32x16 (&acc)[DP / 32], const uint4 *tile, int row0, const f32x16 &p,
+                                      const Lanes<T, DP> &at) {
+    const uint32_t base = lds_of(tile) + row0 * Tile<T, DP>::kBytes;
     if constexpr (sizeof(T) == 2) {
-        const int row = 4 * h + ((lane & 15) >> 2);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             uint4 b;
@@ -155,23 +187,21 @@ __device__ __forceinline__ void outer(f32x16 (&acc)[DP / 32], const uint4 *tile,
             b.w = pack_bf16x2(p[8 * s + 6], p[8 * s + 7]);
 #pragma unroll
             for (int n = 0; n < DP / 32; ++n) {
-                const int c = 4 * n + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), o = (lane & 1) * 8;
-                lds_char *lo = base + 16 * s * Tile<T, DP>::kBytes + Tile<T, DP>::addr(row, c) + o;
-                lds_char *hi = base + 16 * s * Tile<T, DP>::kBytes + Tile<T, DP>::addr(row + 8, c) + o;
-                const uint2 l2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_kt_v4s *)lo));
-                const uint2 h2 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_kt_v4s *)hi));
+                const uint2 l2 = lds_read_transposed(at.col[2 * n] + base + 16 * s * Tile<T, DP>::kBytes);
+                const uint2 h2 = lds_read_transposed(at.col[2 * n + 1] + base + 16 * s * Tile<T, DP>::kBytes);
                 const uint4 a = make_uint4(l2.x, l2.y, h2.x, h2.y);
                 acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                                  __builtin_bit_cast(bf16x8, b), acc[n], 0, 0, 0);
             }
         }
     } else {
+        const int lane = (int)at.col[0], h = lane >> 5;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int row = 8 * (i >> 2) + 4 * h + (i & 3);
 #pragma unroll
             for (int n = 0; n < DP / 32; ++n) {
-                const float a = *(const __attribute__((address_space(3))) float *)(
+                const float a = *(const __attribute__((address_space(3))) float *)(uintptr_t)(
                     base + Tile<T, DP>::addr(row, 8 * n + ((lane & 31) >> 2)) + (lane & 3) * 4);
                 acc[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[i], acc[n], 0, 0, 0);
             }
@@ -351,8 +381,10 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
         vs.store(sv[0]);
     }
     __syncthreads();
+    Lanes<T, DP> at(lane);
     auto step = [&](int key, auto stage) {
         constexpr int buf = decltype(stage)::value;
+        at.refresh();
         const bool more = key + KT < item.hi;
         if (more) load(key + KT);
         if (key < most) {
@@ -360,7 +392,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
 #pragma unroll
             for (int t = 0; t < KT / 32; ++t) {
                 s[t] = splat(0.0f);
-                scores<T, DP>(s[t], sk[buf], 32 * t, qf, lane);
+                scores<T, DP>(s[t], sk[buf], 32 * t, qf, at);
             }
             if (key + KT > least) {
                 const int left = row.limit - key - 4 * (lane >> 5);
@@ -397,7 +429,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
                     s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.scale2, -ref));
                     run.sum += s[t][i];
                 }
-                outer<T, DP>(o, sv[buf], 32 * t, s[t], lane);
+                outer<T, DP>(o, sv[buf], 32 * t, s[t], at);
             }
         }
         if (more) {
@@ -590,11 +622,12 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
         }
     }
     __syncthreads();
+    Lanes<T, DP> at(lane);
     auto both = [&](int buf) {
         s = splat(0.0f);
         g = splat(-delta);
-        scores<T, DP>(s, sk[buf], 0, qf, lane);
-        scores<T, DP>(g, sv[buf], 0, gf, lane);
+        scores<T, DP>(s, sk[buf], 0, qf, at);
+        scores<T, DP>(g, sv[buf], 0, gf, at);
     };
     if (item.lo < most) both(0);
     by_stage(item.lo, item.hi, [&](int key, auto now_, auto next_, auto then_) {
@@ -604,6 +637,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
             if (key + 3 * kStep < item.hi) load(key + 3 * kStep);
         }
         if (key < most) {
+            at.refresh();
             f32x16 ds;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -614,7 +648,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
                 for (int i = 0; i < 16; ++i) ds[i] = 8 * (i >> 2) + (i & 3) < left ? ds[i] : 0.0f;
             }
             if (key + kStep < most) both(next);
-            outer<T, DP>(o, sk[now], 0, ds, lane);
+            outer<T, DP>(o, sk[now], 0, ds, at);
         }
         __syncthreads();
     });
@@ -749,6 +783,7 @@ __global__ __launch_bounds__(64 * kKeyWaves, 2) void attention_dkv(AttnParams a)
     f32x16 acc[DP / 32], s = splat(0.0f);
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) acc[n] = splat(0.0f);
+    Lanes<T, DP> at(lane);
     // Probabilities (for dv, shared) or do . v - delta of the rows at r0 in stage `buf`.
     auto make = [&](int r0, int buf, int turn) {
         const float *stat = (for_dv ? slse : sdelta)[buf] + 4 * (lane >> 5);
@@ -761,7 +796,7 @@ __global__ __launch_bounds__(64 * kKeyWaves, 2) void attention_dkv(AttnParams a)
         }
         if (for_dv) {
             s = splat(0.0f);
-            scores<T, DP>(s, sq[buf], 0, frag, lane);
+            scores<T, DP>(s, sq[buf], 0, frag, at);
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, st[i]));
             if (r0 < wave_last) {
@@ -773,7 +808,7 @@ __global__ __launch_bounds__(64 * kKeyWaves, 2) void attention_dkv(AttnParams a)
             for (int i = 0; i < 4; ++i) sp[turn][pair][i][lane] = f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
         } else {
             s = st;
-            scores<T, DP>(s, sg[buf], 0, frag, lane);
+            scores<T, DP>(s, sg[buf], 0, frag, at);
         }
     };
     if (item.lo < item.hi) {
@@ -795,6 +830,7 @@ __global__ __launch_bounds__(64 * kKeyWaves, 2) void attention_dkv(AttnParams a)
             store(then);
             if (r0 + 3 * kStep < item.hi) load(r0 + 3 * kStep);
         }
+        at.refresh();
         const bool seen = r0 + kStep > wave_first, more = r0 + kStep < item.hi && r0 + 2 * kStep > wave_first;
         f32x16 z = s;
         if (seen && !for_dv) {
@@ -811,7 +847,7 @@ __global__ __launch_bounds__(64 * kKeyWaves, 2) void attention_dkv(AttnParams a)
             }
         }
         if (more) make(r0 + kStep, next, turn ^ 1);
-        if (seen) outer<T, DP>(acc, for_dv ? sg[now] : sq[now], 0, z, lane);
+        if (seen) outer<T, DP>(acc, for_dv ? sg[now] : sq[now], 0, z, at);
         __syncthreads();
         turn ^= 1;
     });
@@ -864,7 +900,8 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_join(AttnParams a, con
 constexpr int kRowWaves = RW, kRowTile = 32 * kRowWaves;
 constexpr int64_t kMaxRows = 0x7fffffff - 2 * kTile;
 
-constexpr int64_t kRowFixed = 3, kKeyFixed = 6;   // a piece's fixed cost in units of kUnit
+// A piece's fixed cost (its rows' or keys' load, its result's store) in units of kUnit.
+constexpr int64_t kRowFixed = 3, kKeyFixed = 6, kF32Fixed = 1;
 constexpr int64_t kMaxPitch = (int64_t)1 << 24;   // bytes between tokens of k and v
 
 // 64 packed rows span at most 64 / group + 2 tokens and all heads of the group.
@@ -984,7 +1021,8 @@ struct Plan {
     int64_t slots = 0;
 };
 
-void make_plan(int32_t pass, const Record *rec, int64_t n, int64_t kv_heads, int64_t group, int dp, bool causal, Plan &plan) {
+void make_plan(int32_t pass, const Record *rec, int64_t n, int64_t kv_heads, int64_t group, int dp, bool causal, int dtype,
+               Plan &plan) {
     const bool keys = pass == CT_ATTENTION_KEYS;
     const int64_t tile = keys ? kTile : kRowTile;
     std::vector<Item> tiles;
@@ -1023,7 +1061,7 @@ void make_plan(int32_t pass, const Record *rec, int64_t n, int64_t kv_heads, int
         return;
     }
     // Otherwise every workgroup gets the same share of all units, cutting tiles where it ends.
-    const int64_t fixed = keys ? kKeyFixed : kRowFixed;
+    const int64_t fixed = dtype == CT_F32 ? kF32Fixed : keys ? kKeyFixed : kRowFixed;
     int64_t low = 2 * fixed, high = std::max<int64_t>(low, work + fixed * (int64_t)tiles.size());
     while (low < high) {
         const int64_t mid = (low + high) / 2;
@@ -1079,11 +1117,12 @@ using namespace ct;
 static_assert(sizeof(Item) == 4 * kEntry && sizeof(Group) == 4 * kEntry, "plan entries");
 
 extern "C" int ct_attention_plan(int32_t pass, const int64_t *records, int64_t n_records, int32_t heads,
-                                 int32_t kv_heads, int32_t head_dim, int32_t causal, int32_t *entries,
-                                 int64_t capacity, int64_t *counts) {
+                                 int32_t kv_heads, int32_t head_dim, int32_t dtype, int32_t causal,
+                                 int32_t *entries, int64_t capacity, int64_t *counts) {
     if (pass < CT_ATTENTION_FORWARD || pass > CT_ATTENTION_KEYS || n_records < 0 || n_records > 0x7fffffff ||
         !dims_ok(heads, kv_heads, head_dim))
         return -CT_EINVAL_SHAPE;
+    if (dtype != CT_BF16 && dtype != CT_F32) return -CT_EINVAL_DTYPE;
     if (!counts || (n_records && !records)) return -CT_EINVAL_POINTER;
     const int64_t group = heads / kv_heads;
     const Record *rec = reinterpret_cast<const Record *>(records);
@@ -1098,7 +1137,7 @@ extern "C" int ct_attention_plan(int32_t pass, const int64_t *records, int64_t n
     if (tiles > 0x7fffffff / (4 * kTile * kv_heads)) return -CT_EINVAL_SHAPE;
     try {
         Plan made;
-        make_plan(pass, rec, n_records, kv_heads, group, padded_dim(head_dim), causal != 0, made);
+        make_plan(pass, rec, n_records, kv_heads, group, padded_dim(head_dim), causal != 0, dtype, made);
         counts[0] = (int64_t)made.pieces.size();
         counts[1] = (int64_t)made.joins.size();
         counts[2] = made.slots;

@@ -555,11 +555,12 @@ typedef struct ct_attention {
  * lists of pieces: 32-byte entries, counts[0] pieces, counts[1] joins of what was cut into
  * counts[2] partial results, counts[3] workgroups; counts holds 4. With entries = null only counts
  * is written; capacity counts entries. A plan holds
- * for every call with these records, heads, head_dim and causal; the caller copies its entries
+ * for every call with these records, heads, head_dim, dtype and causal; the caller copies its entries
  * to the device (16-byte aligned) and hands them and counts to the calls.
  */
 int ct_attention_plan(int32_t pass, const int64_t *records, int64_t n_records, int32_t heads, int32_t kv_heads,
-                      int32_t head_dim, int32_t causal, int32_t *entries, int64_t capacity, int64_t *counts);
+                      int32_t head_dim, int32_t dtype, int32_t causal, int32_t *entries, int64_t capacity,
+                      int64_t *counts);
 /* Bytes of workspace that a plan with counts[2] = slots needs; the backward, whose passes follow
  * one another, the larger of its two plans'. */
 int64_t ct_attention_workspace(int32_t pass, int64_t slots, int32_t kv_heads, int32_t head_dim);
