@@ -142,29 +142,48 @@ class AttentionLayout:
         return tables
 
 
-def _strided(t, *, tokens_at_once, heads):
+def _strided(t, tokens_at_once, heads):
     """`t` [tokens, heads, head_dim] in a form that the kernels take: itself, or a contiguous
     copy where an element stride, an alignment or a span of strides is not theirs."""
     size = t.element_size()
     token, head, unit = t.stride()
     if (unit != 1 or token * size % 16 or head * size % 16 or t.data_ptr() % 16 or token < 0 or head < 0
             or token * size > _MAX_PITCH or tokens_at_once * token * size + heads * head * size >= _MAX_SPAN):
-        return t.contiguous()
+        return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _operands(q, k, v, tables, causal, scale):
-    heads, head_dim = q.shape[1:]
+    q_token, q_head, _ = q.stride()
+    k_token, k_head, _ = k.stride()
+    v_token, v_head, _ = v.stride()
+    return _native.Attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_token, q_head, k_token, k_head, v_token, v_head,
+                             tables.records, q.shape[1], k.shape[1], q.shape[2], _native.dtype_code(q.dtype), causal,
+                             scale)
+
+
+def _forward(q, k, v, layout, causal, scale, keep_stats):
+    """(q, k, v as the kernels read them, out, stats or None)."""
+    tokens, heads, head_dim = q.shape
     kv_heads = k.shape[1]
-    return _native.Attention(
-        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_token=q.stride(0), q_head=q.stride(1),
-        k_token=k.stride(0), k_head=k.stride(1), v_token=v.stride(0), v_head=v.stride(1),
-        records=tables.records, heads=heads, kv_heads=kv_heads, head_dim=head_dim,
-        dtype=_native.dtype_code(q.dtype), causal=int(causal), scale=scale)
-
-
-def _workspace(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    group = heads // kv_heads
+    q, k, v = _strided(q, 64 // group + 2, group), _strided(k, 64, 0), _strided(v, 64, 0)
+    work = layout.tokens and layout.key_tokens   # else there is nothing but zeros
+    fresh = torch.empty if work and layout.whole and layout.tokens == tokens else torch.zeros
+    out = fresh((tokens, heads, head_dim), dtype=q.dtype, device=q.device)
+    stats = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if keep_stats else None
+    if work:
+        tables = layout.tables(heads, kv_heads, head_dim, q.dtype, causal)
+        plan, stream = tables.forward, _native.stream_of(q)
+        tables.use(stream)
+        nbytes = plan.workspace
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+        with _native.device_of(q):
+            status = _native.library().ct_attention_forward(
+                _operands(q, k, v, tables, causal, scale), plan.entries, plan.counts, out.data_ptr(),
+                _native.ptr(stats), _native.ptr(workspace), nbytes, stream)
+        _native.check(status, "ct_attention_forward")
+    return q, k, v, out, stats
 
 
 class _PackedAttention(torch.autograd.Function):
@@ -172,24 +191,7 @@ class _PackedAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, layout, causal, scale):
-        tokens, heads, head_dim = q.shape
-        kv_heads = k.shape[1]
-        group = heads // kv_heads
-        q = _strided(q, tokens_at_once=64 // group + 2, heads=group)
-        k, v = (_strided(t, tokens_at_once=64, heads=0) for t in (k, v))
-        whole = layout.whole and layout.tokens == tokens
-        out = (torch.empty if whole else torch.zeros)(tokens, heads, head_dim, dtype=q.dtype, device=q.device)
-        stats = torch.empty(tokens, heads, dtype=torch.float32, device=q.device)
-        if tokens:
-            tables = layout.tables(heads, kv_heads, head_dim, q.dtype, causal)
-            plan, stream = tables.forward, _native.stream_of(q)
-            tables.use(stream)
-            workspace = _workspace(plan.workspace, q.device)
-            with _native.device_of(q):
-                status = _native.library().ct_attention_forward(
-                    _operands(q, k, v, tables, causal, scale), plan.entries, plan.counts, out.data_ptr(),
-                    stats.data_ptr(), _native.ptr(workspace), plan.workspace, stream)
-            _native.check(status, "ct_attention_forward")
+        q, k, v, out, stats = _forward(q, k, v, layout, causal, scale, True)
         ctx.save_for_backward(q, k, v, out, stats)
         ctx.layout, ctx.causal, ctx.scale = layout, causal, scale
         return out
@@ -202,26 +204,29 @@ class _PackedAttention(torch.autograd.Function):
         if not layout.keys_disjoint:
             raise RuntimeError("packed_attention: key_records that overlap have no backward")
         tokens, heads, head_dim = q.shape
-        key_tokens, kv_heads = k.shape[:2]
-        group = heads // kv_heads
-        dout = _strided(dout, tokens_at_once=64 // group + 2, heads=group)
-        whole = layout.whole and layout.tokens == tokens
-        keys_whole = layout.keys_whole and layout.key_tokens == key_tokens
-        fresh = dict(dtype=q.dtype, device=q.device)
-        dq = (torch.empty if whole else torch.zeros)(q.shape, **fresh)
-        dk, dv = ((torch.empty if keys_whole else torch.zeros)(k.shape, **fresh) for _ in range(2))
-        if tokens or key_tokens:
-            tables = layout.tables(heads, kv_heads, head_dim, q.dtype, causal)
+        key_tokens, kv_heads, _ = k.shape
+        group, dtype, device = heads // kv_heads, q.dtype, q.device
+        dout = _strided(dout, 64 // group + 2, group)
+        work = layout.tokens and layout.key_tokens
+        fresh = torch.empty if work and layout.whole and layout.tokens == tokens else torch.zeros
+        dq = fresh((tokens, heads, head_dim), dtype=dtype, device=device)
+        fresh = torch.empty if work and layout.keys_whole and layout.key_tokens == key_tokens else torch.zeros
+        dk, dv = (fresh((key_tokens, kv_heads, head_dim), dtype=dtype, device=device) for _ in range(2))
+        if work:
+            tables = layout.tables(heads, kv_heads, head_dim, dtype, causal)
             rows, keys, stream = tables.rows, tables.keys, _native.stream_of(q)
             tables.use(stream)
-            delta = torch.empty_like(stats)
-            nbytes = max(rows.workspace, keys.workspace)   # one pass after the other
-            workspace = _workspace(nbytes, q.device)
+            # delta, then the partial results of one pass after the other
+            delta = -(-4 * tokens * heads // 256) * 256
+            nbytes = max(rows.workspace, keys.workspace)
+            scratch = torch.empty(max(delta + nbytes, 1), dtype=torch.uint8, device=device)
+            at = scratch.data_ptr()
+            dout_token, dout_head, _ = dout.stride()
             with _native.device_of(q):
                 status = _native.library().ct_attention_backward(
                     _operands(q, k, v, tables, causal, scale), rows.entries, rows.counts, keys.entries, keys.counts,
-                    out.data_ptr(), stats.data_ptr(), dout.data_ptr(), dout.stride(0), dout.stride(1), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                    _native.ptr(workspace), nbytes, stream)
+                    out.data_ptr(), stats.data_ptr(), dout.data_ptr(), dout_token, dout_head, at, dq.data_ptr(),
+                    dk.data_ptr(), dv.data_ptr(), at + delta if nbytes else None, nbytes, stream)
             _native.check(status, "ct_attention_backward")
         return dq, dk, dv, None, None, None
 
@@ -285,4 +290,6 @@ def packed_attention(q, k, v, records, *, causal=True, scale=None):
         raise NotImplementedError("packed_attention: the HIP kernels take bfloat16 or float32")
     if head_dim % 8 or head_dim > 128:
         raise ValueError(f"packed_attention: head_dim {head_dim} is not a multiple of 8 up to 128")
-    return _PackedAttention.apply(q, k, v, layout, causal, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _PackedAttention.apply(q, k, v, layout, causal, scale)
+    return _forward(q, k, v, layout, causal, scale, False)[3]

@@ -6,10 +6,11 @@ Every projection is a `Projection` with a frozen NF4 base and a unit-scale LoRA 
 driven through the reference's group operators: q/k/v share their input in
 `project_group` with the partial RoPE applied to q and k (`rotary=`), o_proj adds the
 residual, the MLP is `tiled_lora_mlp` with the residual; RMSNorm runs the HIP kernels,
-and the loss is `projection_loss` over the supervised rows. Attention is PyTorch-ROCm's
+and the loss is `projection_loss` over the supervised rows. Attention is causal within each
+packed record, the single key/value head shared by the query heads: PyTorch-ROCm's
 scaled-dot-product attention (memory-efficient backend, flash as the deterministic
-choice), causal within each packed record, with the
-single key/value head broadcast to the query heads. The MLP cache budget
+choice) or, with `DecoderConfig(attention="packed")`, the HIP kernels of
+`kernels.attention_cuda.packed_attention`, which are deterministic. The MLP cache budget
 (`mlp_cache_bytes`) is the reference's runtime option: layers from the last one back keep
 their gate/up outputs and xa while the budget lasts (modeling/model.py:227-237), so their
 backward skips the gate/up recompute. Not here (the reference's other runtime options):
@@ -39,6 +40,11 @@ class DecoderConfig:
     rope_theta: float = 10000.0
     partial_rotary_factor: float = 0.5
     rms_norm_eps: float = 1e-6
+    attention: str = "sdpa"   # or "packed"
+
+    def __post_init__(self):
+        if self.attention not in ("sdpa", "packed"):
+            raise ValueError(f"attention is 'sdpa' or 'packed', not {self.attention!r}")
 
     @property
     def rotary_dim(self):
@@ -47,7 +53,8 @@ class DecoderConfig:
 
 def record_positions(records, device):
     """Token positions restarting at every packed record: records are (start, stop) spans
-    covering the sequence in order."""
+    covering the sequence in order, or an AttentionLayout of them."""
+    records = getattr(records, "records", records)
     return torch.cat([torch.arange(stop - start, device=device) for start, stop in records])
 
 
@@ -75,9 +82,25 @@ def attention_backends():
     return names
 
 
-def _attention(q, k, v, records):
+def packed_records(records, config, device):
+    """`records` as the layers take them: for the packed kernels their layout, made once for all
+    layers, otherwise the spans themselves."""
+    from ..kernels.attention_cuda import AttentionLayout
+    if config.attention != "packed":
+        return getattr(records, "records", records)
+    return records if isinstance(records, AttentionLayout) else AttentionLayout(records, device)
+
+
+def _attention(q, k, v, records, config):
     """Causal attention inside each record. q [1, S, H, D]; k, v [1, S, 1, D]."""
+    if config.attention == "packed":
+        from ..kernels.attention_cuda import packed_attention
+        layout = packed_records(records, config, q.device)
+        if not layout.whole or layout.tokens != q.shape[1]:
+            raise ValueError("records must cover the sequence")
+        return packed_attention(q, k, v, layout)
     from torch.nn.attention import SDPBackend, sdpa_kernel
+    records = packed_records(records, config, q.device)
     heads = q.shape[2]
     sizes = [stop - start for start, stop in records]
     if sum(sizes) != q.shape[1]:
@@ -112,7 +135,7 @@ class Attention(nn.Module):
         q, k, v = project_group((self.q_proj, self.k_proj, self.v_proj), x, rotary=(cosine, sine, c.head_dim))
         q = q.reshape(b, s, c.num_attention_heads, c.head_dim)
         k, v = k.reshape(b, s, 1, c.head_dim), v.reshape(b, s, 1, c.head_dim)
-        y = _attention(q, k, v, records).reshape(b, s, -1)
+        y = _attention(q, k, v, records, c).reshape(b, s, -1)
         return project_group((self.o_proj,), y, residual=residual)[0]
 
 
@@ -174,6 +197,7 @@ class Decoder(nn.Module):
         cosine, sine = rotary_values(positions, self.config, torch.bfloat16)
         x = self.embed_tokens(ids)
         self.plan_mlp_cache(ids.numel() if ids.is_cuda else 0, mlp_cache_bytes)
+        records = packed_records(records, self.config, ids.device)
         with projection_budget(projection_bytes):
             for layer in self.layers:
                 x = layer(x, cosine, sine, records)

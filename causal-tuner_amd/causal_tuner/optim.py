@@ -117,6 +117,9 @@ class FusedAdamW(torch.optim.Optimizer):
         return loss
 
 
+_captured_plans = set()   # plans that a captured graph reads: never dropped
+
+
 class _MuonPlan:
     """The shares of work of one list of shapes on one device: kept between steps."""
 
@@ -126,8 +129,8 @@ class _MuonPlan:
                                "be captured; run it once before the capture")
         lib = _native.library()
         table = (_native.MuonMatrix * len(shapes))()
-        for row, (rows, cols, adjust) in zip(table, shapes):
-            row.rows, row.cols, row.adjust = rows, cols, adjust
+        for row, (rows, cols) in zip(table, shapes):
+            row.rows, row.cols = rows, cols
         self.counts, needed = (ctypes.c_int64 * _native.CT_MUON_KINDS)(), ctypes.c_int64()
         _native.check(lib.ct_muon_plan(table, len(shapes), None, 0, self.counts, ctypes.byref(needed)), "ct_muon_plan")
         size = sum(self.counts)
@@ -140,18 +143,22 @@ class _MuonPlan:
             self.stream = _native.stream_of(self.entries)
         self.table, self.workspace = bytes(table), needed.value
 
-    def run(self, pointers, dtype, options):
-        """One call over `pointers`, a list of (param, grad, momentum) addresses in the shapes' order."""
+    def run(self, matrices, dtype, options):
+        """One call over `matrices`, a list of (param, grad, momentum) addresses and the factor on
+        the learning rate, in the shapes' order."""
         device, stream = self.entries.device, _native.stream_of(self.entries)
-        table = (_native.MuonMatrix * len(pointers)).from_buffer_copy(self.table)
-        for row, (param, grad, momentum) in zip(table, pointers):
-            row.param, row.grad, row.momentum = param, grad, momentum
-        if stream != self.stream and not torch.cuda.is_current_stream_capturing():
-            self.entries.record_stream(torch.cuda.current_stream(device))
+        table = (_native.MuonMatrix * len(matrices)).from_buffer_copy(self.table)
+        for row, (param, grad, momentum, adjust) in zip(table, matrices):
+            row.param, row.grad, row.momentum, row.adjust = param, grad, momentum, adjust
+        if stream != self.stream:
+            if torch.cuda.is_current_stream_capturing():
+                _captured_plans.add(self)
+            else:
+                self.entries.record_stream(torch.cuda.current_stream(device))
         workspace = torch.empty(self.workspace, dtype=torch.uint8, device=device)
         with _native.device_of(self.entries):
             status = _native.library().ct_muon(
-                table, len(pointers), self.entries.data_ptr(), self.counts, _native.dtype_code(dtype),
+                table, len(matrices), self.entries.data_ptr(), self.counts, _native.dtype_code(dtype),
                 ctypes.byref(options), workspace.data_ptr(), self.workspace, self.workspace, stream)
         _native.check(status, "ct_muon")
 
@@ -214,8 +221,8 @@ def orthogonalize(matrices, *, coefficients=(3.4445, -4.7750, 2.0315), steps=5, 
     options = _native.MuonOptions(a=coefficients[0], b=coefficients[1], c=coefficients[2], eps=eps, steps=steps)
     for (device, dtype), members in buckets.items():
         sources = [inputs[i].contiguous() for i in members]
-        plan = _muon_plan(tuple((m.shape[0], m.shape[1], 1.0) for m in sources), device)
-        plan.run([(results[i].data_ptr(), m.data_ptr(), None) for i, m in zip(members, sources)], dtype, options)
+        plan = _muon_plan(tuple(tuple(m.shape) for m in sources), device)
+        plan.run([(results[i].data_ptr(), m.data_ptr(), None, 1.0) for i, m in zip(members, sources)], dtype, options)
     return results[0] if single else results
 
 
@@ -301,7 +308,7 @@ class FusedMuon(torch.optim.Optimizer):
                 a=coefficients[0], b=coefficients[1], c=coefficients[2], eps=eps,
                 nesterov=int(bool(group["nesterov"])), steps=steps, update=1)
             for (device, dtype), members in buckets.items():
-                plan = _muon_plan(tuple((*p.shape, _adjusted(group["adjust_lr_fn"], *p.shape)) for p, _ in members),
-                                  device)
-                plan.run([(p.data_ptr(), p.grad.data_ptr(), m.data_ptr()) for p, m in members], dtype, options)
+                plan = _muon_plan(tuple(tuple(p.shape) for p, _ in members), device)
+                plan.run([(p.data_ptr(), p.grad.data_ptr(), m.data_ptr(), _adjusted(group["adjust_lr_fn"], *p.shape))
+                          for p, m in members], dtype, options)
         return loss

@@ -112,7 +112,7 @@ struct Tile {
 
 typedef const __attribute__((address_space(3))) char lds_char;
 
-__device__ __forceinline__ uint32_t lds_of(const uint4 *p) { return (uint32_t)(uintptr_t)(lds_char *)p; }
+__device__ __forceinline__ uint32_t lds_of(const void *p) { return (uint32_t)(uintptr_t)(lds_char *)p; }
 
 __device__ __forceinline__ uint4 lds_read16(uint32_t at) {
     return __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)at);
@@ -144,6 +144,18 @@ struct Lanes {
             col[0] = (uint32_t)lane;
         }
     }
+    uint32_t moved = 0;   // float32: of the transposed reads
+    // Reads from so many bytes further on.
+    __device__ __forceinline__ void shift(uint32_t rows, uint32_t transposed) {
+#pragma unroll
+        for (int s = 0; s < kFrags; ++s) row[s] += rows;
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int n = 0; n < kCols; ++n) col[n] += transposed;
+        } else {
+            moved = transposed;
+        }
+    }
     __device__ __forceinline__ void refresh() {
 #pragma unroll
         for (int s = 0; s < kFrags; ++s) asm volatile("" : "+v"(row[s]));
@@ -154,9 +166,9 @@ struct Lanes {
 
 // acc[row, col] += sum_d tile[row0 + row][d] * frag[col][d]
 template <typename T, int DP>
-__device__ __forceinline__ void scores(f32x16 &acc, const uint4 *tile, int row0, const uint4 (&frag)[Tile<T, DP>::kFrags],
+__device__ __forceinline__ void scores(f32x16 &acc, uint32_t tile, int row0, const uint4 (&frag)[Tile<T, DP>::kFrags],
                                        const Lanes<T, DP> &at) {
-    const uint32_t base = lds_of(tile) + row0 * Tile<T, DP>::kBytes;
+    const uint32_t base = tile + row0 * Tile<T, DP>::kBytes;
 #pragma unroll
     for (int s = 0; s < Tile<T, DP>::kFrags; ++s) {
         const uint4 a = lds_read16(at.row[s] + base);
@@ -174,9 +186,9 @@ __device__ __forceinline__ void scores(f32x16 &acc, const uint4 *tile, int row0,
 // acc[b][d, col] += sum_row tile[row0 + row][32 b + d] * p[row, col], p as `scores` leaves it:
 // register i of lane half h is row 8 (i / 4) + 4 h + i % 4.
 template <typename T, int DP>
-__device__ __forceinline__ void outer(f32x16 (&acc)[DP / 32], const uint4 *tile, int row0, const f32x16 &p,
+__device__ __forceinline__ void outer(f32x16 (&acc)[DP / 32], uint32_t tile, int row0, const f32x16 &p,
                                       const Lanes<T, DP> &at) {
-    const uint32_t base = lds_of(tile) + row0 * Tile<T, DP>::kBytes;
+    const uint32_t base = tile + row0 * Tile<T, DP>::kBytes;
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -202,7 +214,7 @@ __device__ __forceinline__ void outer(f32x16 (&acc)[DP / 32], const uint4 *tile,
 #pragma unroll
             for (int n = 0; n < DP / 32; ++n) {
                 const float a = *(const __attribute__((address_space(3))) float *)(uintptr_t)(
-                    base + Tile<T, DP>::addr(row, 8 * n + ((lane & 31) >> 2)) + (lane & 3) * 4);
+                    base + at.moved + Tile<T, DP>::addr(row, 8 * n + ((lane & 31) >> 2)) + (lane & 3) * 4);
                 acc[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[i], acc[n], 0, 0, 0);
             }
         }
@@ -392,7 +404,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
 #pragma unroll
             for (int t = 0; t < KT / 32; ++t) {
                 s[t] = splat(0.0f);
-                scores<T, DP>(s[t], sk[buf], 32 * t, qf, at);
+                scores<T, DP>(s[t], lds_of(sk) + buf * (uint32_t)sizeof(sk[0]), 32 * t, qf, at);
             }
             if (key + KT > least) {
                 const int left = row.limit - key - 4 * (lane >> 5);
@@ -429,7 +441,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
                     s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.scale2, -ref));
                     run.sum += s[t][i];
                 }
-                outer<T, DP>(o, sv[buf], 32 * t, s[t], at);
+                outer<T, DP>(o, lds_of(sv) + buf * (uint32_t)sizeof(sv[0]), 32 * t, s[t], at);
             }
         }
         if (more) {
@@ -457,7 +469,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
                 if (d < a.head_dim)
                     store4<T>(dst, d, o[n][i] * inv, o[n][i + 1] * inv, o[n][i + 2] * inv, o[n][i + 3] * inv);
             }
-        if (lane < 32)
+        if (a.stats && lane < 32)
             a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : run.m2 + __builtin_amdgcn_logf(sum);
     } else {
         const int64_t at = ((int64_t)item.slot * a.kv_heads + kv_head) * (32 * WAVES) + wave * kWaveCols + (lane & 31);
@@ -530,7 +542,7 @@ __global__ __launch_bounds__(kThreads) void attention_join(AttnParams a, const I
     if (4 * lane < a.head_dim)
         store4<T>(a.dst0 + row.token * a.o_token + row.head * a.o_head, 4 * lane, acc.x * inv, acc.y * inv, acc.z * inv,
                   acc.w * inv);
-    if (lane == 0) a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+    if (a.stats && lane == 0) a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
 // Sum of the parts of one row or key, in order, for four elements.
@@ -626,8 +638,8 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
     auto both = [&](int buf) {
         s = splat(0.0f);
         g = splat(-delta);
-        scores<T, DP>(s, sk[buf], 0, qf, at);
-        scores<T, DP>(g, sv[buf], 0, gf, at);
+        scores<T, DP>(s, lds_of(sk) + buf * (uint32_t)sizeof(sk[0]), 0, qf, at);
+        scores<T, DP>(g, lds_of(sv) + buf * (uint32_t)sizeof(sv[0]), 0, gf, at);
     };
     if (item.lo < most) both(0);
     by_stage(item.lo, item.hi, [&](int key, auto now_, auto next_, auto then_) {
@@ -648,7 +660,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
                 for (int i = 0; i < 16; ++i) ds[i] = 8 * (i >> 2) + (i & 3) < left ? ds[i] : 0.0f;
             }
             if (key + kStep < most) both(next);
-            outer<T, DP>(o, sk[now], 0, ds, at);
+            outer<T, DP>(o, lds_of(sk) + now * (uint32_t)sizeof(sk[0]), 0, ds, at);
         }
         __syncthreads();
     });
@@ -702,10 +714,11 @@ __global__ __launch_bounds__(kThreads) void attention_dq_join(AttnParams a, cons
 constexpr int kKeyWaves = 8;
 
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * kKeyWaves, 2) void attention_dkv(AttnParams a) {
+__global__ __launch_bounds__(64 * kKeyWaves, sizeof(T) == 2 && DP == 64 ? 4 : 2) void attention_dkv(AttnParams a) {
     constexpr int kUnits = kStep * Tile<T, DP>::kChunks, kAll = 64 * kKeyWaves;
-    __shared__ uint4 sq[kStages][kUnits], sg[kStages][kUnits];
-    __shared__ float slse[kStages][kStep], sdelta[kStages][kStep];   // negated
+    __shared__ uint4 st[2][kStages][kUnits];                     // q, dout
+    __shared__ __align__(16) float sstat[2][kStages][kStep];   // -lse, -delta
+    __shared__ __align__(16) float szero[kStep];
     __shared__ f32x4 sp[2][kKeyWaves / 2][4][64];
     const Group group = a.groups[blockIdx.x / a.kv_heads];
     const int kv_head = blockIdx.x % a.kv_heads;
@@ -775,30 +788,39 @@ __global__ __launch_bounds__(64 * kKeyWaves, 2) void attention_dkv(AttnParams a)
         }
     };
     auto store = [&](int buf) {
-        qs.store(sq[buf]);
-        gs.store(sg[buf]);
-        if (wave == 0) (lane < kStep ? slse : sdelta)[buf][stat_row] = -stat_r;
+        qs.store(st[0][buf]);
+        gs.store(st[1][buf]);
+        if (wave == 0) sstat[lane < kStep ? 0 : 1][buf][stat_row] = -stat_r;
     };
 
     f32x16 acc[DP / 32], s = splat(0.0f);
 #pragma unroll
     for (int n = 0; n < DP / 32; ++n) acc[n] = splat(0.0f);
+    // Both roles run the same reads, from places of their own: scores with q, from zero, and the
+    // second product with dout, or the other way round and from -delta.
+    constexpr uint32_t kOther = sizeof(st[0]), kStage = sizeof(st[0][0]), kStat = sizeof(sstat[0][0]);
     Lanes<T, DP> at(lane);
+    at.shift(for_dv ? 0 : kOther, for_dv ? kOther : 0);
+    const uint32_t start = 16 * (lane >> 5) + (for_dv ? lds_of(szero) : lds_of(sstat) + kStages * kStat);
+    const uint32_t start_step = for_dv ? 0 : kStat;
+    if (threadIdx.x < kStep) szero[threadIdx.x] = 0.0f;
     // Probabilities (for dv, shared) or do . v - delta of the rows at r0 in stage `buf`.
     auto make = [&](int r0, int buf, int turn) {
-        const float *stat = (for_dv ? slse : sdelta)[buf] + 4 * (lane >> 5);
-        f32x16 st;
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const f32x4 v = *reinterpret_cast<const f32x4 *>(stat + 2 * i);
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 v = __builtin_bit_cast(f32x4, lds_read16(start + buf * start_step + 32 * i));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) st[i + e] = v[e];
+            for (int e = 0; e < 4; ++e) s[4 * i + e] = v[e];
         }
+        scores<T, DP>(s, lds_of(st) + buf * kStage, 0, frag, at);
         if (for_dv) {
-            s = splat(0.0f);
-            scores<T, DP>(s, sq[buf], 0, frag, at);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, st[i]));
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 v = __builtin_bit_cast(f32x4, lds_read16(lds_of(sstat) + buf * kStat + 16 * (lane >> 5) + 32 * i));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    s[4 * i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + e], a.scale2, v[e]));
+            }
             if (r0 < wave_last) {
                 const int hidden = (int)(mine < nrows ? mine : nrows) - r0 - 4 * (lane >> 5);   // rows below do not see the key
 #pragma unroll
@@ -806,9 +828,6 @@ __global__ __launch_bounds__(64 * kKeyWaves, 2) void attention_dkv(AttnParams a)
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) sp[turn][pair][i][lane] = f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
-        } else {
-            s = st;
-            scores<T, DP>(s, sg[buf], 0, frag, at);
         }
     };
     if (item.lo < item.hi) {
@@ -847,7 +866,7 @@ __global__ __launch_bounds__(64 * kKeyWaves, 2) void attention_dkv(AttnParams a)
             }
         }
         if (more) make(r0 + kStep, next, turn ^ 1);
-        if (seen) outer<T, DP>(acc, for_dv ? sg[now] : sq[now], 0, z, at);
+        if (seen) outer<T, DP>(acc, lds_of(st) + now * kStage, 0, z, at);
         __syncthreads();
         turn ^= 1;
     });
@@ -975,9 +994,13 @@ int64_t parts_per_item(int32_t pass, int dp) {   // floats
                                      : (int64_t)kRowTile * (dp + (pass == CT_ATTENTION_FORWARD ? 2 : 0));
 }
 
-// Workgroups that the card runs at once: two of 4 waves per CU in the forward and dq, one of 8
-// waves (two with heads up to 64) in the dk, dv kernel.
-int64_t groups_at_once(int32_t pass, int dp) { return pass == CT_ATTENTION_KEYS && dp > 64 ? 256 : 512; }
+// Workgroups that the card runs at once, by their registers: two of 4 waves per CU in the
+// forward and dq (one for float32 with heads past 64), one of 8 waves in the dk, dv kernel (two
+// for bf16 with heads up to 64).
+int64_t groups_at_once(int32_t pass, int dp, int dtype) {
+    if (pass == CT_ATTENTION_KEYS) return dp > 64 || dtype == CT_F32 ? 256 : 512;
+    return dp > 64 && dtype == CT_F32 ? 256 : 512;
+}
 
 constexpr int64_t kUnit = 64;   // keys or rows: pieces are cut at its multiples
 
@@ -1048,7 +1071,7 @@ void make_plan(int32_t pass, const Record *rec, int64_t n, int64_t kv_heads, int
             tiles.push_back(it);
         }
     }
-    const int64_t at_once = std::max<int64_t>(1, groups_at_once(pass, dp) / kv_heads);
+    const int64_t at_once = std::max<int64_t>(1, groups_at_once(pass, dp, dtype) / kv_heads);
     if ((int64_t)tiles.size() >= 2 * at_once && longest * at_once <= work) {
         // Enough whole tiles, none of them longer than a workgroup's share: longest first, so
         // that what starts last ends soon.
@@ -1167,7 +1190,7 @@ extern "C" int ct_attention_forward(const ct_attention *c, const int32_t *plan, 
     if (!counts_ok(counts, c->kv_heads)) return -CT_EINVAL_SHAPE;
     const int64_t joins = counts[1], slots = counts[2], groups = counts[3];
     if (groups == 0) return 0;
-    if (!plan || !out || !stats || (uintptr_t)plan % 16 || (uintptr_t)out % 16) return -CT_EINVAL_POINTER;
+    if (!plan || !out || (uintptr_t)plan % 16 || (uintptr_t)out % 16) return -CT_EINVAL_POINTER;
     if (slots && (!workspace || (uintptr_t)workspace % 16 ||
                   workspace_bytes < ct_attention_workspace(CT_ATTENTION_FORWARD, slots, c->kv_heads, c->head_dim)))
         return -CT_EINVAL_WORKSPACE;

@@ -566,8 +566,8 @@ int ct_attention_plan(int32_t pass, const int64_t *records, int64_t n_records, i
 int64_t ct_attention_workspace(int32_t pass, int64_t slots, int32_t kv_heads, int32_t head_dim);
 
 /*
- * out [tokens, heads, head_dim] contiguous; stats float32 [tokens, heads] for the backward:
- * log2 of the softmax's denominator with its maximum (+inf for a query that sees no key).
+ * out [tokens, heads, head_dim] contiguous; stats float32 [tokens, heads] for the backward (null:
+ * none): log2 of the softmax's denominator with its maximum (+inf for a query that sees no key).
  * Rows of no record are left as they are.
  */
 int ct_attention_forward(const ct_attention *attention, const int32_t *plan, const int64_t *counts, void *out,

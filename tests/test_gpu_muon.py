@@ -166,3 +166,69 @@ def test_muon_against_torch_and_its_state():
         p.grad = torch.ones_like(p)
     fresh.step()
     assert fresh.param_groups[0]["lr"] == 0.02
+
+
+def test_captured_steps_replay():
+    """orthogonalize and a step in a graph, replayed with new gradients between eager work; the
+    plan of unseen shapes is refused inside a capture."""
+    from causal_tuner.optim import FusedMuon, orthogonalize
+    shapes = [(24, 200), (200, 24), (100, 300)]
+    params, twins = ([torch.nn.Parameter(_matrix(s, torch.float32, seed=i)) for i, s in enumerate(shapes)]
+                     for _ in range(2))
+    a, b = FusedMuon(params, lr=0.01), FusedMuon(twins, lr=0.01)
+    for p, t in zip(params, twins):
+        p.grad, t.grad = torch.zeros_like(p), torch.zeros_like(t)
+    a.step()   # buffers and plan exist; zero gradients leave only the decay
+    b.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+        made = orthogonalize([p.grad for p in params])
+    for seed in range(3):
+        for i, (p, t) in enumerate(zip(params, twins)):
+            p.grad.copy_(_matrix(shapes[i], torch.float32, seed=50 + 3 * seed + i))
+            t.grad.copy_(p.grad)
+        graph.replay()
+        b.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, t) for p, t in zip(params, twins))
+        assert all(torch.equal(x, y) for x, y in zip(made, orthogonalize([t.grad for t in twins])))
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            orthogonalize(torch.ones(11, 13, device="cuda"))
+    torch.cuda.synchronize()
+    _check(orthogonalize(params[0].detach()), params[0].detach())
+
+
+def test_other_streams_and_unaligned_storage():
+    from causal_tuner.optim import orthogonalize
+    inputs = [_matrix((64, 301), torch.float32), _matrix((300, 130), torch.bfloat16)]
+    shifted = []
+    for m in inputs:   # contiguous, but no 16-byte start
+        buffer = torch.empty(m.numel() + 1, device="cuda", dtype=m.dtype)
+        shifted.append(buffer[1:].view(m.shape).copy_(m))
+    torch.cuda.synchronize()
+    results = []
+    for stream in (torch.cuda.Stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(stream):
+            results.append(orthogonalize(shifted))
+    torch.cuda.synchronize()
+    for result in results:
+        for got, m in zip(result, inputs):
+            _check(got, m)
+
+
+def test_device_refusals():
+    from causal_tuner.optim import FusedMuon, orthogonalize
+    with pytest.raises(NotImplementedError):
+        orthogonalize(torch.zeros(3, 3, device="cuda", dtype=torch.float16))
+    p = torch.nn.Parameter(torch.zeros(6, 4, device="cuda"))
+    p.grad = torch.zeros(4, 6, device="cuda").T
+    with pytest.raises(NotImplementedError, match="contiguous"):
+        FusedMuon([p]).step()
+    p.grad = torch.zeros(6, 4, device="cuda")
+    optimizer = FusedMuon([p])
+    optimizer.state[p]["momentum_buffer"] = torch.zeros(6, 4, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="momentum_buffer"):
+        optimizer.step()
