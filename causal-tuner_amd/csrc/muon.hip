@@ -501,34 +501,38 @@ __global__ __launch_bounds__(kThreads) void muon_join(const Matrix *matrices, co
 
 // ------------------------------------------------------------------ short sides up to 64
 // All steps in one workgroup of 8 waves, G, P, T and Q in LDS. Symmetric operands are read
-// along rows for both sides of a product; the ten tiles (i >= j) of rank 64 go to the waves in
-// turn, each in two chains of products.
+// along rows for both sides of a product (16 columns of 4 rows a load: odd rows are stored with
+// their blocks of 16 columns exchanged in pairs, so two rows fill the banks); the ten tiles (i
+// >= j) of rank 64 go to the waves in turn, all of a tile's loads in flight at once and its
+// products in two chains.
 constexpr int kSmallThreads = 512;
 
 __global__ __launch_bounds__(kSmallThreads) void muon_small(const Matrix *matrices, const Item *items, Hyper h,
                                                            double *ws, int steps) {
-    constexpr int kPitch = kSmall + 8, kMost = 10 * 256 / kSmallThreads;
-    __shared__ double sg[kSmall * kPitch], sp[kSmall * kPitch], st[kSmall * kPitch], sq[kSmall * kPitch];
+    constexpr int kMost = 10 * 256 / kSmallThreads;
+    __shared__ double sg[kSmall * kSmall], sp[kSmall * kSmall], st[kSmall * kSmall], sq[kSmall * kSmall];
     const Item it = items[blockIdx.x];
     const Matrix m = matrices[it.matrix];
     const int r = short_side(m), n = tiles16(r), count = n * (n + 1) / 2, tid = threadIdx.x, lane = tid & 63,
-              wave = tid >> 6;
+              wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    auto at = [](int row, int col) { return row * kSmall + (col ^ ((row & 1) << 4)); };
+    auto tile_row = [](int t) { return t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3; };
     const double inv = inverse_norm(m, ws, h.eps);
     {
         // the parts in order, all of a thread's elements at once
         const double *p = part_of(m, ws, 0) + part_head(r) + tid;
         const int64_t step = part_size(r);
         double v[kMost] = {};
-#pragma unroll 4
+#pragma unroll 8
         for (int s = 0; s < m.splits; ++s)
 #pragma unroll
             for (int x = 0; x < kMost; ++x)
                 if (x * kSmallThreads + tid < count * 256) v[x] += p[s * step + x * kSmallThreads];
 #pragma unroll
         for (int x = 0; x < kMost; ++x) {
-            const int t = (x * kSmallThreads + tid) >> 8, i = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, j = t - i * (i + 1) / 2;
+            const int t = (x * kSmallThreads + tid) >> 8, i = tile_row(t), j = t - i * (i + 1) / 2;
             const int row = i * 16 + ((tid & 255) >> 4), col = j * 16 + (tid & 15);
-            if (t < count && row >= col) sg[row * kPitch + col] = sg[col * kPitch + row] = v[x] * (inv * inv);
+            if (t < count && row >= col) sg[at(row, col)] = sg[at(col, row)] = v[x] * (inv * inv);
         }
     }
     __syncthreads();
@@ -540,29 +544,28 @@ __global__ __launch_bounds__(kSmallThreads) void muon_small(const Matrix *matric
         for (int x = 0; x < 2; ++x) {
             const int t = wave + 8 * x;
             if (t >= count) continue;
-            const int i = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, j = t - i * (i + 1) / 2;
-            const double *a = left + (lane >> 4) * kPitch + 16 * i + (lane & 15);
-            const double *b = right + (lane >> 4) * kPitch + 16 * j + (lane & 15);
-            f64x4 even = {}, odd = {};
-            for (int k = 0; k < 16 * n; k += 16) {
-                double p[4], q[4];
+            const int i = tile_row(t), j = t - i * (i + 1) / 2;
+            const int a = at(lane >> 4, 16 * i + (lane & 15)), b = at(lane >> 4, 16 * j + (lane & 15));
+            double p[16], q[16];   // k = 4 u + lane / 16
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    p[u] = a[(k + 4 * u) * kPitch];
-                    q[u] = b[(k + 4 * u) * kPitch];
+            for (int u = 0; u < 16; ++u)
+                if (u < 4 * n) {
+                    p[u] = left[a + 4 * u * kSmall];
+                    q[u] = right[b + 4 * u * kSmall];
                 }
-                even = mfma_f64(p[0], q[0], even);
-                odd = mfma_f64(p[1], q[1], odd);
-                even = mfma_f64(p[2], q[2], even);
-                odd = mfma_f64(p[3], q[3], odd);
-            }
+            f64x4 even = {}, odd = {};
+#pragma unroll
+            for (int u = 0; u < 16; u += 2)
+                if (u < 4 * n) {
+                    even = mfma_f64(p[u], q[u], even);
+                    odd = mfma_f64(p[u + 1], q[u + 1], odd);
+                }
             result[x] = even + odd;
             if (polynomial) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int row = 16 * i + 4 * e + (lane >> 4), col = 16 * j + (lane & 15);
-                    result[x][e] = h.c * result[x][e] + h.b * left[row * kPitch + col] +
-                                   (row == col && row < r ? h.a : 0.0);
+                    result[x][e] = h.c * result[x][e] + h.b * left[at(row, col)] + (row == col && row < r ? h.a : 0.0);
                 }
             }
         }
@@ -571,11 +574,11 @@ __global__ __launch_bounds__(kSmallThreads) void muon_small(const Matrix *matric
         for (int x = 0; x < 2; ++x) {
             const int t = wave + 8 * x;
             if (t >= count) continue;
-            const int i = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, j = t - i * (i + 1) / 2;
+            const int i = tile_row(t), j = t - i * (i + 1) / 2;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int row = 16 * i + 4 * e + (lane >> 4), col = 16 * j + (lane & 15);
-                if (row >= col) dst[row * kPitch + col] = dst[col * kPitch + row] = result[x][e];
+                if (row >= col) dst[at(row, col)] = dst[at(col, row)] = result[x][e];
             }
         }
         __syncthreads();
@@ -591,7 +594,7 @@ __global__ __launch_bounds__(kSmallThreads) void muon_small(const Matrix *matric
     float *final = final_q(m, ws);
     for (int e = tid; e < rp * rp; e += kSmallThreads) {
         const int row = e % rp, k = e / rp;
-        final[final_at(rp, row, k)] = row < 16 * n && k < 16 * n ? (float)(sq[row * kPitch + k] * inv) : 0.0f;
+        final[final_at(rp, row, k)] = row < 16 * n && k < 16 * n ? (float)(sq[at(row, k)] * inv) : 0.0f;
     }
 }
 
@@ -857,8 +860,14 @@ int64_t chunk_cost(int r) {
 }
 
 // Long-side elements per workgroup so that none takes longer than `cap`, in whole chunks; at
-// least two, which pays for the partial result.
-int64_t gram_step(int r, int64_t cap) { return std::max<int64_t>(2, cap / chunk_cost(r)) * kChunk; }
+// least two, which pays for the partial result, and for short sides up to kSmall, whose one
+// workgroup adds all parts, so many that a chunk's time (0.7 us) and a part's (1.1 us) balance:
+// 2049 x 64 in 33 parts 10 + 96 us, in 7 17 + 64.
+int64_t gram_step(const Shape &s, int64_t cap) {
+    int64_t chunks = std::max<int64_t>(2, cap / chunk_cost(s.r));
+    if (s.r <= kSmall) chunks = std::max<int64_t>(chunks, (int64_t)sqrt(1.6 * (double)cdiv(s.width, kChunk)));
+    return chunks * kChunk;
+}
 
 // The smallest cap with which all the one-pass Gram items run at once.
 int64_t gram_cap(const std::vector<Shape> &shapes) {
@@ -866,7 +875,7 @@ int64_t gram_cap(const std::vector<Shape> &shapes) {
     auto fits = [&](int64_t cap) {
         int64_t n = 0;
         for (const Shape &s : shapes)
-            if (s.r <= kOnePass) n += cdiv(s.width, gram_step(s.r, cap));
+            if (s.r <= kOnePass) n += cdiv(s.width, gram_step(s, cap));
         return n <= std::max<int64_t>(kGroupsWanted, (int64_t)shapes.size());
     };
     while (!fits(high) && high < (int64_t)1 << 40) high *= 2;
@@ -881,7 +890,7 @@ int64_t gram_cap(const std::vector<Shape> &shapes) {
 // A matrix's items and its number of partial Gram matrices.
 void plan_matrix(int32_t index, const Shape &s, int64_t cap, std::vector<Item> (&items)[kKinds], int32_t &splits) {
     const bool one_pass = s.r <= kOnePass;
-    const int64_t parts = one_pass ? cdiv(s.width, gram_step(s.r, cap))
+    const int64_t parts = one_pass ? cdiv(s.width, gram_step(s, cap))
                                    : std::max<int64_t>(1, std::min<int64_t>(cdiv(s.width, 512), 32));
     const int64_t step = cdiv(cdiv(s.width, parts), kChunk) * kChunk;   // even parts
     const int64_t count = cdiv(s.width, step);
