@@ -408,7 +408,8 @@ __global__ __launch_bounds__(kThreads) void muon_gram_tiles(const Matrix *matric
     __shared__ double diagonal[kGramTile];
     const Item it = items[blockIdx.x];
     const Matrix m = matrices[it.matrix];
-    const int r = short_side(m), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r = short_side(m), lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const bool tall = m.rows > m.cols;
     const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
     f64x4 acc[2][2] = {};
@@ -620,7 +621,8 @@ __global__ __launch_bounds__(kStageThreads) void muon_stage(const Matrix *matric
     const Item it = items[blockIdx.x];
     if (it.matrix < 0) return;
     const Matrix m = matrices[it.matrix];
-    const int r = short_side(m), rp = padded(r), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r = short_side(m), rp = padded(r), lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);   // scalar, as all that follows from it
     const int64_t lane_at = (lane & 15) + (int64_t)(lane >> 4) * rp;
     const double *left = buffer(m, ws, op.left) + it.i * kPad + lane_at;
     const double *right = buffer(m, ws, op.right) + it.j * kPad + lane_at;
