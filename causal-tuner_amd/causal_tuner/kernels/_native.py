@@ -171,7 +171,10 @@ def library():
             raise RuntimeError(f"The HIP library {path} is not built; run `python causal-tuner_amd/build.py`")
         lib = ctypes.CDLL(path)
         for name, (restype, argtypes) in _SIGNATURES.items():
-            fn = getattr(lib, name)
+            fn = getattr(lib, name, None)
+            if fn is None:
+                raise RuntimeError(f"The HIP library {path} has no {name}; rebuild it with "
+                                   "`python causal-tuner_amd/build.py`")
             fn.restype, fn.argtypes = restype, argtypes
         if lib.ct_abi_version() != ABI_VERSION:
             raise RuntimeError(f"The HIP library {path} has ABI {lib.ct_abi_version()}, this binding needs "

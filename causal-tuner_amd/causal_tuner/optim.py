@@ -150,11 +150,10 @@ class _MuonPlan:
         table = (_native.MuonMatrix * len(matrices)).from_buffer_copy(self.table)
         for row, (param, grad, momentum, adjust) in zip(table, matrices):
             row.param, row.grad, row.momentum, row.adjust = param, grad, momentum, adjust
-        if stream != self.stream:
-            if torch.cuda.is_current_stream_capturing():
-                _captured_plans.add(self)
-            else:
-                self.entries.record_stream(torch.cuda.current_stream(device))
+        if torch.cuda.is_current_stream_capturing():
+            _captured_plans.add(self)
+        elif stream != self.stream:
+            self.entries.record_stream(torch.cuda.current_stream(device))
         workspace = torch.empty(self.workspace, dtype=torch.uint8, device=device)
         with _native.device_of(self.entries):
             status = _native.library().ct_muon(

@@ -22,12 +22,24 @@
 // the outputs.
 //
 // Rounding. Scores, statistics, delta and all sums are fp32. bf16 inputs round p and ds to
-// bf16 for the second products (half a unit in the last place each, 2^-9 relative, below
-// the 2^-9 of the output's own rounding once averaged over the keys); float32 inputs round
-// nothing.
+// bf16 for the second products, which take bf16 (each value off by at most 2^-8 of itself, as
+// the output's own rounding: together 1.4 times the output's, 0.0025 against 0.0017 in norm);
+// float32 inputs round nothing.
 //
 // dq and dk/dv are two kernels that each recompute s (7 products instead of 5): the one-pass
-// form would add dq over workgroups by atomics, whose order changes results from run to run.
+// form would add dq over workgroups by atomics, whose order changes results from run to run,
+// or through a partial dq per key tile, whose traffic (4.3 GB written and read at 8192 rows of
+// 32 heads) outweighs the two products.
+//
+// What bounds it. The matrix instructions and, beside them, the exponentials: 8192 causal rows
+// of 32 heads of 128 over one key/value head, bf16: forward 603 us (912 TFLOP/s), dq 821 (1004),
+// dk and dv 1388 (792), where a large library product reaches 1095 TFLOP/s on the same card
+// (its clock falls under that load) and HBM traffic is a few percent. Few query tokens: the
+// stream of keys and values, 131072 keys of 8 heads in 104 us, 5.2 TB/s (a large copy 5.1).
+// Tried and left out: the two waves of a SIMD in turns (one in matrix instructions while the
+// other has its exponentials, two barriers a step): forward 615 -> 580 us, but 43 -> 46 at three
+// short records and both backward kernels slower; 8 waves per forward workgroup (7% slower at
+// short records); scores of the next step before the current step's exponentials in the forward.
 
 #include <math.h>
 
@@ -363,132 +375,136 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
     const Group group = a.groups[blockIdx.x / a.kv_heads];
     const int kv_head = blockIdx.x % a.kv_heads;
     for (int piece = 0; piece < group.count; ++piece) {
-    const Item item = a.items[group.first + piece];
-    const Record rec = a.records[item.record];
-    const int lane = fresh_lane(), wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
+        const Item item = a.items[group.first + piece];
+        const Record rec = a.records[item.record];
+        const int lane = fresh_lane(), wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
 
-    const RowOf row(a, rec, kv_head, (int64_t)item.begin + wave * kWaveCols + (lane & 31));
-    int least, most;
-    wave_limits(row, least, most);
-    uint4 qf[Tile<T, DP>::kFrags];
-    row_fragments<T, DP>(a.q + row.token * a.q_token + row.head * a.q_head, qf, row.valid, chunks, lane);
+        const RowOf row(a, rec, kv_head, (int64_t)item.begin + wave * kWaveCols + (lane & 31));
+        int least, most;
+        wave_limits(row, least, most);
+        uint4 qf[Tile<T, DP>::kFrags];
+        row_fragments<T, DP>(a.q + row.token * a.q_token + row.head * a.q_head, qf, row.valid, chunks, lane);
 
-    const char *k0 = a.k + rec.k_start * a.k_token + kv_head * a.k_head;
-    const char *v0 = a.v + rec.k_start * a.v_token + kv_head * a.v_head;
-    Stage<T, DP, KT, 64 * WAVES> ks, vs;
-    auto load = [&](int key) {
-        const int left = (int)rec.k_len - key;
-        auto valid = [&](int r) { return r < left; };
-        ks.load(k0 + key * a.k_token, chunks, [&](int p) { return (uint32_t)ks.row_of(p) * (uint32_t)a.k_token; }, valid);
-        vs.load(v0 + key * a.v_token, chunks, [&](int p) { return (uint32_t)vs.row_of(p) * (uint32_t)a.v_token; }, valid);
-    };
+        const char *k0 = a.k + rec.k_start * a.k_token + kv_head * a.k_head;
+        const char *v0 = a.v + rec.k_start * a.v_token + kv_head * a.v_head;
+        Stage<T, DP, KT, 64 * WAVES> ks, vs;
+        auto load = [&](int key) {
+            const int left = (int)rec.k_len - key;
+            auto valid = [&](int r) { return r < left; };
+            ks.load(k0 + key * a.k_token, chunks,
+                    [&](int p) { return (uint32_t)ks.row_of(p) * (uint32_t)a.k_token; }, valid);
+            vs.load(v0 + key * a.v_token, chunks,
+                    [&](int p) { return (uint32_t)vs.row_of(p) * (uint32_t)a.v_token; }, valid);
+        };
 
-    f32x16 o[DP / 32];
+        f32x16 o[DP / 32];
 #pragma unroll
-    for (int n = 0; n < DP / 32; ++n) o[n] = splat(0.0f);
-    Running run;
-    if (item.lo < item.hi) {
-        load(item.lo);
-        ks.store(sk[0]);
-        vs.store(sv[0]);
-    }
-    __syncthreads();
-    Lanes<T, DP> at(lane);
-    auto step = [&](int key, auto stage) {
-        constexpr int buf = decltype(stage)::value;
-        at.refresh();
-        const bool more = key + KT < item.hi;
-        if (more) load(key + KT);
-        if (key < most) {
-            f32x16 s[KT / 32];
+        for (int n = 0; n < DP / 32; ++n) o[n] = splat(0.0f);
+        Running run;
+        if (item.lo < item.hi) {
+            load(item.lo);
+            ks.store(sk[0]);
+            vs.store(sv[0]);
+        }
+        __syncthreads();
+        Lanes<T, DP> at(lane);
+        auto step = [&](int key, auto stage) {
+            constexpr int buf = decltype(stage)::value;
+            at.refresh();
+            const bool more = key + KT < item.hi;
+            if (more) load(key + KT);
+            if (key < most) {
+                f32x16 s[KT / 32];
 #pragma unroll
-            for (int t = 0; t < KT / 32; ++t) {
-                s[t] = splat(0.0f);
-                scores<T, DP>(s[t], lds_of(sk) + buf * (uint32_t)sizeof(sk[0]), 32 * t, qf, at);
-            }
-            if (key + KT > least) {
-                const int left = row.limit - key - 4 * (lane >> 5);
+                for (int t = 0; t < KT / 32; ++t) {
+                    s[t] = splat(0.0f);
+                    scores<T, DP>(s[t], lds_of(sk) + buf * (uint32_t)sizeof(sk[0]), 32 * t, qf, at);
+                }
+                if (key + KT > least) {
+                    const int left = row.limit - key - 4 * (lane >> 5);
+#pragma unroll
+                    for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            s[t][i] = 32 * t + 8 * (i >> 2) + (i & 3) < left ? s[t][i] : -INFINITY;
+                }
+                float top = s[0][0];
 #pragma unroll
                 for (int t = 0; t < KT / 32; ++t)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s[t][i] = 32 * t + 8 * (i >> 2) + (i & 3) < left ? s[t][i] : -INFINITY;
-            }
-            float top = s[0][0];
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
+                top = fmaxf(top, other_half(top)) * a.scale2;
+                // The reference moves only when a row's maximum has grown by more than 2^8: p then
+                // stays below 2^8, o and the sum are exact in that scale, and most tiles skip the
+                // rescaling of o.
+                if (__any(top > run.m2 + 8.0f)) {
+                    const float grown = fmaxf(run.m2, top);
+                    const float shrink = grown == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run.m2 - grown);
+                    run.m2 = grown;
+                    run.sum *= shrink;
 #pragma unroll
-            for (int t = 0; t < KT / 32; ++t)
+                    for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
-            top = fmaxf(top, other_half(top)) * a.scale2;
-            // The reference moves only when a row's maximum has grown by more than 2^8: p then
-            // stays below 2^8, o and the sum are exact in that scale, and most tiles skip the
-            // rescaling of o.
-            if (__any(top > run.m2 + 8.0f)) {
-                const float grown = fmaxf(run.m2, top);
-                const float shrink = grown == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run.m2 - grown);
-                run.m2 = grown;
-                run.sum *= shrink;
-#pragma unroll
-                for (int n = 0; n < DP / 32; ++n)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[n][i] *= shrink;
-            }
-            const float ref = run.m2 == -INFINITY ? 0.0f : run.m2;
-#pragma unroll
-            for (int t = 0; t < KT / 32; ++t) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.scale2, -ref));
-                    run.sum += s[t][i];
+                        for (int i = 0; i < 16; ++i) o[n][i] *= shrink;
                 }
-                outer<T, DP>(o, lds_of(sv) + buf * (uint32_t)sizeof(sv[0]), 32 * t, s[t], at);
+                const float ref = run.m2 == -INFINITY ? 0.0f : run.m2;
+#pragma unroll
+                for (int t = 0; t < KT / 32; ++t) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.scale2, -ref));
+                        run.sum += s[t][i];
+                    }
+                    outer<T, DP>(o, lds_of(sv) + buf * (uint32_t)sizeof(sv[0]), 32 * t, s[t], at);
+                }
             }
+            if (more) {
+                ks.store(sk[buf ^ 1]);
+                vs.store(sv[buf ^ 1]);
+            }
+            __syncthreads();
+        };
+        for (int key = item.lo; key < item.hi; key += 2 * KT) {
+            step(key, std::integral_constant<int, 0>());
+            if (key + KT < item.hi) step(key + KT, std::integral_constant<int, 1>());
         }
-        if (more) {
-            ks.store(sk[buf ^ 1]);
-            vs.store(sv[buf ^ 1]);
-        }
-        __syncthreads();
-    };
-    for (int key = item.lo; key < item.hi; key += 2 * KT) {
-        step(key, std::integral_constant<int, 0>());
-        if (key + KT < item.hi) step(key + KT, std::integral_constant<int, 1>());
-    }
 
-    const float sum = run.sum + other_half(run.sum);
-    const int d0 = 4 * (lane >> 5);
-    if (!row.valid) continue;
-    if (item.slot < 0) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        char *dst = a.dst0 + row.token * a.o_token + row.head * a.o_head;
+        const float sum = run.sum + other_half(run.sum);
+        const int d0 = 4 * (lane >> 5);
+        if (!row.valid) continue;
+        if (item.slot < 0) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            char *dst = a.dst0 + row.token * a.o_token + row.head * a.o_head;
 #pragma unroll
-        for (int n = 0; n < DP / 32; ++n)
+            for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int d = 32 * n + 2 * i + d0;
-                if (d < a.head_dim)
-                    store4<T>(dst, d, o[n][i] * inv, o[n][i + 1] * inv, o[n][i + 2] * inv, o[n][i + 3] * inv);
-            }
-        if (a.stats && lane < 32)
-            a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : run.m2 + __builtin_amdgcn_logf(sum);
-    } else {
-        const int64_t at = ((int64_t)item.slot * a.kv_heads + kv_head) * (32 * WAVES) + wave * kWaveCols + (lane & 31);
-        float *dst = a.part0 + at * DP;
+                for (int i = 0; i < 16; i += 4) {
+                    const int d = 32 * n + 2 * i + d0;
+                    if (d < a.head_dim)
+                        store4<T>(dst, d, o[n][i] * inv, o[n][i + 1] * inv, o[n][i + 2] * inv, o[n][i + 3] * inv);
+                }
+            if (a.stats && lane < 32)
+                a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : run.m2 + __builtin_amdgcn_logf(sum);
+        } else {
+            const int64_t at = ((int64_t)item.slot * a.kv_heads + kv_head) * (32 * WAVES) + wave * kWaveCols + (lane & 31);
+            float *dst = a.part0 + at * DP;
 #pragma unroll
-        for (int n = 0; n < DP / 32; ++n)
+            for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<float4 *>(dst + 32 * n + 2 * i + d0) =
-                    make_float4(o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3]);
-        if (lane < 32) *reinterpret_cast<float2 *>(a.part1 + 2 * at) = make_float2(run.m2, sum);
-    }
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<float4 *>(dst + 32 * n + 2 * i + d0) =
+                        make_float4(o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3]);
+            if (lane < 32) *reinterpret_cast<float2 *>(a.part1 + 2 * at) = make_float2(run.m2, sum);
+        }
     }
 }
 
 // Joins the key ranges of split rows: with M = max_s m_s, o = sum_s 2^(m_s - M) o_s over
 // sum_s 2^(m_s - M) sum_s. DP / 4 threads per row and part; parts past the fourth of a row are
 // shared out over up to 8 such teams, whose sums are added in order.
-__host__ __device__ __forceinline__ int join_teams(int parts) { return parts <= 4 ? 1 : parts <= 8 ? 2 : parts <= 16 ? 4 : 8; }
+__host__ __device__ __forceinline__ int join_teams(int parts) {
+    return parts <= 4 ? 1 : parts <= 8 ? 2 : parts <= 16 ? 4 : 8;
+}
 __host__ __device__ __forceinline__ int join_rows(int parts, int dp) { return kThreads / (dp / 4) / join_teams(parts); }
 
 template <typename T, int DP>
@@ -542,7 +558,8 @@ __global__ __launch_bounds__(kThreads) void attention_join(AttnParams a, const I
     if (4 * lane < a.head_dim)
         store4<T>(a.dst0 + row.token * a.o_token + row.head * a.o_head, 4 * lane, acc.x * inv, acc.y * inv, acc.z * inv,
                   acc.w * inv);
-    if (a.stats && lane == 0) a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+    if (a.stats && lane == 0)
+        a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
 // Sum of the parts of one row or key, in order, for four elements.
@@ -584,109 +601,111 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
     const Group group = a.groups[blockIdx.x / a.kv_heads];
     const int kv_head = blockIdx.x % a.kv_heads;
     for (int piece = 0; piece < group.count; ++piece) {
-    const Item item = a.items[group.first + piece];
-    const Record rec = a.records[item.record];
-    const int lane = fresh_lane(), wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
+        const Item item = a.items[group.first + piece];
+        const Record rec = a.records[item.record];
+        const int lane = fresh_lane(), wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
 
-    const RowOf row(a, rec, kv_head, (int64_t)item.begin + wave * kWaveCols + (lane & 31));
-    int least, most;
-    wave_limits(row, least, most);
-    most = min(most, item.hi);
-    uint4 qf[Tile<T, DP>::kFrags], gf[Tile<T, DP>::kFrags];
-    row_fragments<T, DP>(a.dout + row.token * a.do_token + row.head * a.do_head, gf, row.valid, chunks, lane);
-    row_fragments<T, DP>(a.out + row.token * a.o_token + row.head * a.o_head, qf, row.valid, chunks, lane);
-    float delta = 0.0f;
+        const RowOf row(a, rec, kv_head, (int64_t)item.begin + wave * kWaveCols + (lane & 31));
+        int least, most;
+        wave_limits(row, least, most);
+        most = min(most, item.hi);
+        uint4 qf[Tile<T, DP>::kFrags], gf[Tile<T, DP>::kFrags];
+        row_fragments<T, DP>(a.dout + row.token * a.do_token + row.head * a.do_head, gf, row.valid, chunks, lane);
+        row_fragments<T, DP>(a.out + row.token * a.o_token + row.head * a.o_head, qf, row.valid, chunks, lane);
+        float delta = 0.0f;
 #pragma unroll
-    for (int s = 0; s < Tile<T, DP>::kFrags; ++s) delta = dot_chunk<T>(gf[s], qf[s], delta);
-    delta += other_half(delta);
-    float lse = INFINITY;
-    if (row.valid) {
-        const int64_t at = row.token * a.heads + row.head;
-        lse = a.stats[at];
-        if (lane < 32 && item.lo == 0) a.delta[at] = delta;
-    }
-    row_fragments<T, DP>(a.q + row.token * a.q_token + row.head * a.q_head, qf, row.valid, chunks, lane);
-
-    const char *k0 = a.k + rec.k_start * a.k_token + kv_head * a.k_head;
-    const char *v0 = a.v + rec.k_start * a.v_token + kv_head * a.v_head;
-    Stage<T, DP, kStep, 64 * WAVES> ks, vs;
-    auto load = [&](int key) {
-        const int left = (int)rec.k_len - key;
-        auto valid = [&](int r) { return r < left; };
-        ks.load(k0 + key * a.k_token, chunks, [&](int p) { return (uint32_t)ks.row_of(p) * (uint32_t)a.k_token; }, valid);
-        vs.load(v0 + key * a.v_token, chunks, [&](int p) { return (uint32_t)vs.row_of(p) * (uint32_t)a.v_token; }, valid);
-    };
-    auto store = [&](int buf) {
-        ks.store(sk[buf]);
-        vs.store(sv[buf]);
-    };
-
-    f32x16 o[DP / 32], s, g;
-#pragma unroll
-    for (int n = 0; n < DP / 32; ++n) o[n] = splat(0.0f);
-    if (item.lo < item.hi) {
-        load(item.lo);
-        store(0);
-        if (item.lo + kStep < item.hi) {
-            load(item.lo + kStep);
-            store(1);
-            if (item.lo + 2 * kStep < item.hi) load(item.lo + 2 * kStep);
+        for (int s = 0; s < Tile<T, DP>::kFrags; ++s) delta = dot_chunk<T>(gf[s], qf[s], delta);
+        delta += other_half(delta);
+        float lse = INFINITY;
+        if (row.valid) {
+            const int64_t at = row.token * a.heads + row.head;
+            lse = a.stats[at];
+            if (lane < 32 && item.lo == 0) a.delta[at] = delta;
         }
-    }
-    __syncthreads();
-    Lanes<T, DP> at(lane);
-    auto both = [&](int buf) {
-        s = splat(0.0f);
-        g = splat(-delta);
-        scores<T, DP>(s, lds_of(sk) + buf * (uint32_t)sizeof(sk[0]), 0, qf, at);
-        scores<T, DP>(g, lds_of(sv) + buf * (uint32_t)sizeof(sv[0]), 0, gf, at);
-    };
-    if (item.lo < most) both(0);
-    by_stage(item.lo, item.hi, [&](int key, auto now_, auto next_, auto then_) {
-        constexpr int now = decltype(now_)::value, next = decltype(next_)::value, then = decltype(then_)::value;
-        if (key + 2 * kStep < item.hi) {
-            store(then);
-            if (key + 3 * kStep < item.hi) load(key + 3 * kStep);
-        }
-        if (key < most) {
-            at.refresh();
-            f32x16 ds;
+        row_fragments<T, DP>(a.q + row.token * a.q_token + row.head * a.q_head, qf, row.valid, chunks, lane);
+
+        const char *k0 = a.k + rec.k_start * a.k_token + kv_head * a.k_head;
+        const char *v0 = a.v + rec.k_start * a.v_token + kv_head * a.v_head;
+        Stage<T, DP, kStep, 64 * WAVES> ks, vs;
+        auto load = [&](int key) {
+            const int left = (int)rec.k_len - key;
+            auto valid = [&](int r) { return r < left; };
+            ks.load(k0 + key * a.k_token, chunks,
+                    [&](int p) { return (uint32_t)ks.row_of(p) * (uint32_t)a.k_token; }, valid);
+            vs.load(v0 + key * a.v_token, chunks,
+                    [&](int p) { return (uint32_t)vs.row_of(p) * (uint32_t)a.v_token; }, valid);
+        };
+        auto store = [&](int buf) {
+            ks.store(sk[buf]);
+            vs.store(sv[buf]);
+        };
+
+        f32x16 o[DP / 32], s, g;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                ds[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse)) * g[i];
-            if (key + kStep > least) {
-                const int left = row.limit - key - 4 * (lane >> 5);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) ds[i] = 8 * (i >> 2) + (i & 3) < left ? ds[i] : 0.0f;
+        for (int n = 0; n < DP / 32; ++n) o[n] = splat(0.0f);
+        if (item.lo < item.hi) {
+            load(item.lo);
+            store(0);
+            if (item.lo + kStep < item.hi) {
+                load(item.lo + kStep);
+                store(1);
+                if (item.lo + 2 * kStep < item.hi) load(item.lo + 2 * kStep);
             }
-            if (key + kStep < most) both(next);
-            outer<T, DP>(o, lds_of(sk) + now * (uint32_t)sizeof(sk[0]), 0, ds, at);
         }
         __syncthreads();
-    });
-    if (!row.valid) continue;
-    const int d0 = 4 * (lane >> 5);
-    if (item.slot < 0) {
-        char *dst = a.dst0 + row.token * a.d_token + (int64_t)row.head * a.head_dim * (int)sizeof(T);
-#pragma unroll
-        for (int n = 0; n < DP / 32; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int d = 32 * n + 2 * i + d0;
-                if (d < a.head_dim)
-                    store4<T>(dst, d, o[n][i] * a.scale, o[n][i + 1] * a.scale, o[n][i + 2] * a.scale,
-                              o[n][i + 3] * a.scale);
+        Lanes<T, DP> at(lane);
+        auto both = [&](int buf) {
+            s = splat(0.0f);
+            g = splat(-delta);
+            scores<T, DP>(s, lds_of(sk) + buf * (uint32_t)sizeof(sk[0]), 0, qf, at);
+            scores<T, DP>(g, lds_of(sv) + buf * (uint32_t)sizeof(sv[0]), 0, gf, at);
+        };
+        if (item.lo < most) both(0);
+        by_stage(item.lo, item.hi, [&](int key, auto now_, auto next_, auto then_) {
+            constexpr int now = decltype(now_)::value, next = decltype(next_)::value, then = decltype(then_)::value;
+            if (key + 2 * kStep < item.hi) {
+                store(then);
+                if (key + 3 * kStep < item.hi) load(key + 3 * kStep);
             }
-    } else {
-        float *dst = a.part0 + (((int64_t)item.slot * a.kv_heads + kv_head) * (32 * WAVES) + wave * kWaveCols +
-                                (lane & 31)) * DP;
+            if (key < most) {
+                at.refresh();
+                f32x16 ds;
 #pragma unroll
-        for (int n = 0; n < DP / 32; ++n)
+                for (int i = 0; i < 16; ++i)
+                    ds[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse)) * g[i];
+                if (key + kStep > least) {
+                    const int left = row.limit - key - 4 * (lane >> 5);
 #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<float4 *>(dst + 32 * n + 2 * i + d0) =
-                    make_float4(o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3]);
-    }
+                    for (int i = 0; i < 16; ++i) ds[i] = 8 * (i >> 2) + (i & 3) < left ? ds[i] : 0.0f;
+                }
+                if (key + kStep < most) both(next);
+                outer<T, DP>(o, lds_of(sk) + now * (uint32_t)sizeof(sk[0]), 0, ds, at);
+            }
+            __syncthreads();
+        });
+        if (!row.valid) continue;
+        const int d0 = 4 * (lane >> 5);
+        if (item.slot < 0) {
+            char *dst = a.dst0 + row.token * a.d_token + (int64_t)row.head * a.head_dim * (int)sizeof(T);
+#pragma unroll
+            for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const int d = 32 * n + 2 * i + d0;
+                    if (d < a.head_dim)
+                        store4<T>(dst, d, o[n][i] * a.scale, o[n][i + 1] * a.scale, o[n][i + 2] * a.scale,
+                                  o[n][i + 3] * a.scale);
+                }
+        } else {
+            float *dst = a.part0 + (((int64_t)item.slot * a.kv_heads + kv_head) * (32 * WAVES) + wave * kWaveCols +
+                                    (lane & 31)) * DP;
+#pragma unroll
+            for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<float4 *>(dst + 32 * n + 2 * i + d0) =
+                        make_float4(o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3]);
+        }
     }
 }
 
@@ -709,8 +728,8 @@ __global__ __launch_bounds__(kThreads) void attention_dq_join(AttnParams a, cons
 // other do . v - delta, ds = p (do . v - delta) with the first one's p through LDS (lane by
 // lane: both hold the same layout) and dk += ds^T q. Each then holds one operand of keys and
 // one accumulator, which leaves room for two waves per SIMD; a single wave with both needs
-// 490 registers and ran at 25% of the matrix instructions' rate (2633 against ... us at 8192
-// rows of 32 heads of 128).
+// 490 registers and ran at 25% of the matrix instructions' rate (2633 us at 8192 rows of 32
+// heads, this form 1936 with the same shares of work, 1388 with even ones).
 constexpr int kKeyWaves = 8;
 
 template <typename T, int DP>
@@ -723,177 +742,179 @@ __global__ __launch_bounds__(64 * kKeyWaves, sizeof(T) == 2 && DP == 64 ? 4 : 2)
     const Group group = a.groups[blockIdx.x / a.kv_heads];
     const int kv_head = blockIdx.x % a.kv_heads;
     for (int piece = 0; piece < group.count; ++piece) {
-    const Item item = a.items[group.first + piece];
-    const Record rec = a.records[item.record];
-    const int lane = fresh_lane(), wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
-    const int pair = wave & 3;                // waves w and w + 4 run on one SIMD
-    const bool for_dv = wave < kKeyWaves / 2;
+        const Item item = a.items[group.first + piece];
+        const Record rec = a.records[item.record];
+        const int lane = fresh_lane(), wave = wave_index(), chunks = a.head_dim * (int)sizeof(T) / 16;
+        const int pair = wave & 3;                // waves w and w + 4 run on one SIMD
+        const bool for_dv = wave < kKeyWaves / 2;
 
-    const int key0 = item.begin + pair * kWaveCols, key = key0 + (lane & 31);
-    const bool valid = key < rec.k_len;
-    const int64_t kv = rec.k_start + (valid ? key : 0);
-    uint4 frag[Tile<T, DP>::kFrags];
-    row_fragments<T, DP>(for_dv ? a.k + kv * a.k_token + kv_head * a.k_head : a.v + kv * a.v_token + kv_head * a.v_head,
-                         frag, valid, chunks, lane);
+        const int key0 = item.begin + pair * kWaveCols, key = key0 + (lane & 31);
+        const bool valid = key < rec.k_len;
+        const int64_t kv = rec.k_start + (valid ? key : 0);
+        uint4 frag[Tile<T, DP>::kFrags];
+        row_fragments<T, DP>(for_dv ? a.k + kv * a.k_token + kv_head * a.k_head : a.v + kv * a.v_token + kv_head * a.v_head,
+                             frag, valid, chunks, lane);
 
-    const int nrows = (int)(rec.q_len * a.group);
-    // Row r sees key j when r >= first(j); tokens before key j - (keys - queries) do not.
-    auto first = [&](int j) -> int64_t {
-        const int64_t t = a.causal ? j - (rec.k_len - rec.q_len) : 0;
-        return t < 0 ? 0 : t * a.group;
-    };
-    const int64_t mine = first(key), wave_first = first(key0), wave_last = first(key0 + kWaveCols - 1);
+        const int nrows = (int)(rec.q_len * a.group);
+        // Row r sees key j when r >= first(j); tokens before key j - (keys - queries) do not.
+        auto first = [&](int j) -> int64_t {
+            const int64_t t = a.causal ? j - (rec.k_len - rec.q_len) : 0;
+            return t < 0 ? 0 : t * a.group;
+        };
+        const int64_t mine = first(key), wave_first = first(key0), wave_last = first(key0 + kWaveCols - 1);
 
-    Stage<T, DP, kStep, kAll> qs, gs;
-    float stat_r = 0.0f;
-    // A group that divides the step makes a row's token and head the same in every step; the
-    // others are divided out each time.
-    const bool regular = kStep % a.group == 0;
-    const int stat_row = (int)threadIdx.x % kStep;
-    struct Place {
-        uint32_t q, g;
-        int32_t stat;
-    };
-    auto place = [&](int row, uint32_t base) -> Place {   // row after the first token of the step
-        const uint32_t r = base + (uint32_t)row, t = div_group(a, r), h = r - t * (uint32_t)a.group;
-        return {t * (uint32_t)a.q_token + h * (uint32_t)a.q_head, t * (uint32_t)a.do_token + h * (uint32_t)a.do_head,
-                (int32_t)(t * (uint32_t)a.heads + h)};
-    };
-    constexpr int kLoads = Stage<T, DP, kStep, kAll>::kLoads;
-    Place fixed[kLoads];
+        Stage<T, DP, kStep, kAll> qs, gs;
+        float stat_r = 0.0f;
+        // A group that divides the step makes a row's token and head the same in every step; the
+        // others are divided out each time.
+        const bool regular = kStep % a.group == 0;
+        const int stat_row = (int)threadIdx.x % kStep;
+        struct Place {
+            uint32_t q, g;
+            int32_t stat;
+        };
+        auto place = [&](int row, uint32_t base) -> Place {   // row after the first token of the step
+            const uint32_t r = base + (uint32_t)row, t = div_group(a, r), h = r - t * (uint32_t)a.group;
+            return {t * (uint32_t)a.q_token + h * (uint32_t)a.q_head, t * (uint32_t)a.do_token + h * (uint32_t)a.do_head,
+                    (int32_t)(t * (uint32_t)a.heads + h)};
+        };
+        constexpr int kLoads = Stage<T, DP, kStep, kAll>::kLoads;
+        Place fixed[kLoads];
 #pragma unroll
-    for (int p = 0; p < kLoads; ++p) fixed[p] = place(qs.row_of(p), 0);
-    const int32_t fixed_stat = place(stat_row, 0).stat;
-    auto load = [&](int r0) {
-        const uint32_t t0 = div_group(a, (uint32_t)r0), base = (uint32_t)r0 - t0 * (uint32_t)a.group;
-        const int64_t token = rec.q_start + t0;
-        const int left = nrows - r0;
-        Place at[kLoads];
-        int32_t stat = fixed_stat;
+        for (int p = 0; p < kLoads; ++p) fixed[p] = place(qs.row_of(p), 0);
+        const int32_t fixed_stat = place(stat_row, 0).stat;
+        auto load = [&](int r0) {
+            const uint32_t t0 = div_group(a, (uint32_t)r0), base = (uint32_t)r0 - t0 * (uint32_t)a.group;
+            const int64_t token = rec.q_start + t0;
+            const int left = nrows - r0;
+            Place at[kLoads];
+            int32_t stat = fixed_stat;
 #pragma unroll
-        for (int p = 0; p < kLoads; ++p) at[p] = fixed[p];
-        if (!regular) {
+            for (int p = 0; p < kLoads; ++p) at[p] = fixed[p];
+            if (!regular) {
 #pragma unroll
-            for (int p = 0; p < kLoads; ++p) at[p] = place(qs.row_of(p), base);
-            stat = place(stat_row, base).stat;
-        }
-        auto exists = [&](int row) { return row < left; };
-        qs.load(a.q + token * a.q_token + (int64_t)kv_head * a.group * a.q_head, chunks, [&](int p) { return at[p].q; },
-                exists);
-        gs.load(a.dout + token * a.do_token + (int64_t)kv_head * a.group * a.do_head, chunks,
-                [&](int p) { return at[p].g; }, exists);
-        if (wave == 0) {   // lanes 0 - 31 the statistics, 32 - 63 delta; rows behind the last: p = 0
-            const float *from = (lane < kStep ? a.stats : a.delta) + token * a.heads + kv_head * a.group;
-            stat_r = stat_row < left ? from[stat] : lane < kStep ? INFINITY : 0.0f;
-        }
-    };
-    auto store = [&](int buf) {
-        qs.store(st[0][buf]);
-        gs.store(st[1][buf]);
-        if (wave == 0) sstat[lane < kStep ? 0 : 1][buf][stat_row] = -stat_r;
-    };
+                for (int p = 0; p < kLoads; ++p) at[p] = place(qs.row_of(p), base);
+                stat = place(stat_row, base).stat;
+            }
+            auto exists = [&](int row) { return row < left; };
+            qs.load(a.q + token * a.q_token + (int64_t)kv_head * a.group * a.q_head, chunks, [&](int p) { return at[p].q; },
+                    exists);
+            gs.load(a.dout + token * a.do_token + (int64_t)kv_head * a.group * a.do_head, chunks,
+                    [&](int p) { return at[p].g; }, exists);
+            if (wave == 0) {   // lanes 0 - 31 the statistics, 32 - 63 delta; rows behind the last: p = 0
+                const float *from = (lane < kStep ? a.stats : a.delta) + token * a.heads + kv_head * a.group;
+                stat_r = stat_row < left ? from[stat] : lane < kStep ? INFINITY : 0.0f;
+            }
+        };
+        auto store = [&](int buf) {
+            qs.store(st[0][buf]);
+            gs.store(st[1][buf]);
+            if (wave == 0) sstat[lane < kStep ? 0 : 1][buf][stat_row] = -stat_r;
+        };
 
-    f32x16 acc[DP / 32], s = splat(0.0f);
+        f32x16 acc[DP / 32], s = splat(0.0f);
 #pragma unroll
-    for (int n = 0; n < DP / 32; ++n) acc[n] = splat(0.0f);
-    // Both roles run the same reads, from places of their own: scores with q, from zero, and the
-    // second product with dout, or the other way round and from -delta.
-    constexpr uint32_t kOther = sizeof(st[0]), kStage = sizeof(st[0][0]), kStat = sizeof(sstat[0][0]);
-    Lanes<T, DP> at(lane);
-    at.shift(for_dv ? 0 : kOther, for_dv ? kOther : 0);
-    const uint32_t start = 16 * (lane >> 5) + (for_dv ? lds_of(szero) : lds_of(sstat) + kStages * kStat);
-    const uint32_t start_step = for_dv ? 0 : kStat;
-    if (threadIdx.x < kStep) szero[threadIdx.x] = 0.0f;
-    // Probabilities (for dv, shared) or do . v - delta of the rows at r0 in stage `buf`.
-    auto make = [&](int r0, int buf, int turn) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f32x4 v = __builtin_bit_cast(f32x4, lds_read16(start + buf * start_step + 32 * i));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * i + e] = v[e];
-        }
-        scores<T, DP>(s, lds_of(st) + buf * kStage, 0, frag, at);
-        if (for_dv) {
+        for (int n = 0; n < DP / 32; ++n) acc[n] = splat(0.0f);
+        // Both roles run the same reads, from places of their own: scores with q, from zero, and the
+        // second product with dout, or the other way round and from -delta.
+        constexpr uint32_t kOther = sizeof(st[0]), kStage = sizeof(st[0][0]), kStat = sizeof(sstat[0][0]);
+        Lanes<T, DP> at(lane);
+        at.shift(for_dv ? 0 : kOther, for_dv ? kOther : 0);
+        const uint32_t start = 16 * (lane >> 5) + (for_dv ? lds_of(szero) : lds_of(sstat) + kStages * kStat);
+        const uint32_t start_step = for_dv ? 0 : kStat, own_stat = lds_of(sstat) + 16 * (lane >> 5);
+        if (threadIdx.x < kStep) szero[threadIdx.x] = 0.0f;
+        // Probabilities (for dv, shared) or do . v - delta of the rows at r0 in stage `buf`.
+        auto make = [&](int r0, int buf, int turn) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x4 v = __builtin_bit_cast(f32x4, lds_read16(lds_of(sstat) + buf * kStat + 16 * (lane >> 5) + 32 * i));
+                const f32x4 v = __builtin_bit_cast(f32x4, lds_read16(start + buf * start_step + 32 * i));
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    s[4 * i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + e], a.scale2, v[e]));
+                for (int e = 0; e < 4; ++e) s[4 * i + e] = v[e];
             }
-            if (r0 < wave_last) {
-                const int hidden = (int)(mine < nrows ? mine : nrows) - r0 - 4 * (lane >> 5);   // rows below do not see the key
+            scores<T, DP>(s, lds_of(st) + buf * kStage, 0, frag, at);
+            if (for_dv) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) >= hidden ? s[i] : 0.0f;
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 v = __builtin_bit_cast(f32x4, lds_read16(own_stat + buf * kStat + 32 * i));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[4 * i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + e], a.scale2, v[e]));
+                }
+                if (r0 < wave_last) {
+                    // rows below `hidden` do not see the key
+                    const int hidden = (int)(mine < nrows ? mine : nrows) - r0 - 4 * (lane >> 5);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) >= hidden ? s[i] : 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    sp[turn][pair][i][lane] = f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sp[turn][pair][i][lane] = f32x4{s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]};
-        }
-    };
-    if (item.lo < item.hi) {
-        load(item.lo);
-        store(0);
-        if (item.lo + kStep < item.hi) {
-            load(item.lo + kStep);
-            store(1);
-            if (item.lo + 2 * kStep < item.hi) load(item.lo + 2 * kStep);
-        }
-    }
-    __syncthreads();
-    int turn = 0;
-    if (item.lo < item.hi && item.lo + kStep > wave_first) make(item.lo, 0, 0);
-    __syncthreads();
-    by_stage(item.lo, item.hi, [&](int r0, auto now_, auto next_, auto then_) {
-        constexpr int now = decltype(now_)::value, next = decltype(next_)::value, then = decltype(then_)::value;
-        if (r0 + 2 * kStep < item.hi) {
-            store(then);
-            if (r0 + 3 * kStep < item.hi) load(r0 + 3 * kStep);
-        }
-        at.refresh();
-        const bool seen = r0 + kStep > wave_first, more = r0 + kStep < item.hi && r0 + 2 * kStep > wave_first;
-        f32x16 z = s;
-        if (seen && !for_dv) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f32x4 p = sp[turn][pair][i][lane];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) z[4 * i + e] *= p[e];
-            }
-            if (r0 < wave_last) {   // 0 x inf
-                const int hidden = (int)(mine < nrows ? mine : nrows) - r0 - 4 * (lane >> 5);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) z[i] = 8 * (i >> 2) + (i & 3) >= hidden ? z[i] : 0.0f;
+        };
+        if (item.lo < item.hi) {
+            load(item.lo);
+            store(0);
+            if (item.lo + kStep < item.hi) {
+                load(item.lo + kStep);
+                store(1);
+                if (item.lo + 2 * kStep < item.hi) load(item.lo + 2 * kStep);
             }
         }
-        if (more) make(r0 + kStep, next, turn ^ 1);
-        if (seen) outer<T, DP>(acc, lds_of(st) + now * kStage, 0, z, at);
         __syncthreads();
-        turn ^= 1;
-    });
-    const int d0 = 4 * (lane >> 5);
-    const float scale = for_dv ? 1.0f : a.scale;
-    if (item.slot < 0) {
-        if (!valid) continue;
-        char *dst = (for_dv ? a.dst1 : a.dst0) + kv * a.d_token + (int64_t)kv_head * a.head_dim * (int)sizeof(T);
-#pragma unroll
-        for (int n = 0; n < DP / 32; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int d = 32 * n + 2 * i + d0;
-                if (d < a.head_dim)
-                    store4<T>(dst, d, acc[n][i] * scale, acc[n][i + 1] * scale, acc[n][i + 2] * scale,
-                              acc[n][i + 3] * scale);
+        int turn = 0;
+        if (item.lo < item.hi && item.lo + kStep > wave_first) make(item.lo, 0, 0);
+        __syncthreads();
+        by_stage(item.lo, item.hi, [&](int r0, auto now_, auto next_, auto then_) {
+            constexpr int now = decltype(now_)::value, next = decltype(next_)::value, then = decltype(then_)::value;
+            if (r0 + 2 * kStep < item.hi) {
+                store(then);
+                if (r0 + 3 * kStep < item.hi) load(r0 + 3 * kStep);
             }
-    } else {
-        float *dst = (for_dv ? a.part1 : a.part0) +
-                     (((int64_t)item.slot * a.kv_heads + kv_head) * kTile + pair * kWaveCols + (lane & 31)) * DP;
+            at.refresh();
+            const bool seen = r0 + kStep > wave_first, more = r0 + kStep < item.hi && r0 + 2 * kStep > wave_first;
+            f32x16 z = s;
+            if (seen && !for_dv) {
 #pragma unroll
-        for (int n = 0; n < DP / 32; ++n)
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 p = sp[turn][pair][i][lane];
 #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<float4 *>(dst + 32 * n + 2 * i + d0) =
-                    make_float4(acc[n][i], acc[n][i + 1], acc[n][i + 2], acc[n][i + 3]);
-    }
+                    for (int e = 0; e < 4; ++e) z[4 * i + e] *= p[e];
+                }
+                if (r0 < wave_last) {   // 0 x inf
+                    const int hidden = (int)(mine < nrows ? mine : nrows) - r0 - 4 * (lane >> 5);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) z[i] = 8 * (i >> 2) + (i & 3) >= hidden ? z[i] : 0.0f;
+                }
+            }
+            if (more) make(r0 + kStep, next, turn ^ 1);
+            if (seen) outer<T, DP>(acc, lds_of(st) + now * kStage, 0, z, at);
+            __syncthreads();
+            turn ^= 1;
+        });
+        const int d0 = 4 * (lane >> 5);
+        const float scale = for_dv ? 1.0f : a.scale;
+        if (item.slot < 0) {
+            if (!valid) continue;
+            char *dst = (for_dv ? a.dst1 : a.dst0) + kv * a.d_token + (int64_t)kv_head * a.head_dim * (int)sizeof(T);
+#pragma unroll
+            for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const int d = 32 * n + 2 * i + d0;
+                    if (d < a.head_dim)
+                        store4<T>(dst, d, acc[n][i] * scale, acc[n][i + 1] * scale, acc[n][i + 2] * scale,
+                                  acc[n][i + 3] * scale);
+                }
+        } else {
+            float *dst = (for_dv ? a.part1 : a.part0) +
+                         (((int64_t)item.slot * a.kv_heads + kv_head) * kTile + pair * kWaveCols + (lane & 31)) * DP;
+#pragma unroll
+            for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<float4 *>(dst + 32 * n + 2 * i + d0) =
+                        make_float4(acc[n][i], acc[n][i + 1], acc[n][i + 2], acc[n][i + 3]);
+        }
     }
 }
 
@@ -985,8 +1006,10 @@ int status_of_last_launch() {
 
 template <typename F>
 int by_type(int dtype, int dp, F f) {
-    if (dtype == CT_BF16) return dp == 64 ? f((uint16_t)0, std::integral_constant<int, 64>()) : f((uint16_t)0, std::integral_constant<int, 128>());
-    return dp == 64 ? f(0.0f, std::integral_constant<int, 64>()) : f(0.0f, std::integral_constant<int, 128>());
+    typedef std::integral_constant<int, 64> Narrow;
+    typedef std::integral_constant<int, 128> Wide;
+    if (dtype == CT_BF16) return dp == 64 ? f((uint16_t)0, Narrow()) : f((uint16_t)0, Wide());
+    return dp == 64 ? f(0.0f, Narrow()) : f(0.0f, Wide());
 }
 
 int64_t parts_per_item(int32_t pass, int dp) {   // floats
@@ -1051,7 +1074,8 @@ void make_plan(int32_t pass, const Record *rec, int64_t n, int64_t kv_heads, int
     std::vector<Item> tiles;
     int64_t work = 0, longest = 0;
     for (int64_t i = 0; i < n; ++i) {
-        const int64_t rows = rec[i].q_len * group, span = keys ? rec[i].k_len : rows, shift = rec[i].k_len - rec[i].q_len;
+        const int64_t rows = rec[i].q_len * group, shift = rec[i].k_len - rec[i].q_len;
+        const int64_t span = keys ? rec[i].k_len : rows;
         for (int64_t b = 0; b < span; b += tile) {
             Item it = {};
             it.record = (int32_t)i;
@@ -1117,7 +1141,8 @@ void make_plan(int32_t pass, const Record *rec, int64_t n, int64_t kv_heads, int
         for (int32_t k = 0; k < g.count; ++k) c += units_of(plan.pieces[(size_t)(g.first + k)]) + fixed;
         return c;
     };
-    std::stable_sort(plan.groups.begin(), plan.groups.end(), [&](const Group &x, const Group &y) { return cost(x) > cost(y); });
+    std::stable_sort(plan.groups.begin(), plan.groups.end(),
+                     [&](const Group &x, const Group &y) { return cost(x) > cost(y); });
 }
 
 // counts: pieces, joins, partials, workgroups.

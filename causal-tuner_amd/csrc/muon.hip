@@ -14,6 +14,15 @@
 // over three (float32 steps on the whole matrix: 4e-6 and 6e-6). G, P and the products
 // between them are therefore double (v_mfma_f64_16x16x4, which runs at half of float32's rate
 // on a fifth of the work); only the last product, of the final P_{n-1} ... P_0 and M, is float32.
+// Keeping P_{n-1} ... P_0 in float32 too would lose a factor of three in those cases.
+//
+// What bounds it, two layers' adapters of rank 256 (72M elements, 855 us a step): the Gram
+// pass 255 us (double matrix instructions, 66% of what a large library product reaches, and 12
+// bytes an element), the 14 launches of r x r products 24 us each (their operands' way from
+// L2, half of it, and double matrix instructions), the last product 314 us (16 bytes an
+// element at 3.7 TB/s, with float32 matrix instructions under it). Small sets: the launches.
+// Tried and left out: 64 x 64 tiles in the r x r products (the same at 24 matrices, 20% slower
+// at 12), k-steps of 32 rows in flight instead of 16 (more registers, 3% slower).
 //
 // The Muon step (Jordan et al., Muon: an optimizer for hidden layers; torch.optim.Muon's
 // arguments): m = mu m + (1 - mu) g, M = nesterov ? mu m + (1 - mu) g : m, and
@@ -722,7 +731,8 @@ __device__ __forceinline__ void apply_slab(const Matrix &m, const Item &it, cons
 #pragma unroll
             for (int p = 0; p < kUnits; ++p) {
                 const int u = p * kApplyThreads + tid;
-                const int s = TALL ? u % (kShort / 4) * 4 : u / (kLong / 4), l = TALL ? u / (kShort / 4) : u % (kLong / 4) * 4;
+                const int s = TALL ? u % (kShort / 4) * 4 : u / (kLong / 4);
+                const int l = TALL ? u / (kShort / 4) : u % (kLong / 4) * 4;
                 const int64_t at = TALL ? (col0 + l) * r + k0 + s : (int64_t)(k0 + s) * m.cols + col0 + l;
                 const int64_t left = TALL ? (col0 + l < width ? r - k0 - s : 0) : (k0 + s < r ? width - col0 - l : 0);
                 float4 v = make_float4(0, 0, 0, 0);
@@ -744,7 +754,8 @@ __device__ __forceinline__ void apply_slab(const Matrix &m, const Item &it, cons
             __syncthreads();
             if (row >= rp) continue;
             const int depth = rp - k0 < kShort ? rp - k0 : kShort;
-            const float4 *w = reinterpret_cast<const float4 *>(q) + ((int64_t)(k0 / 8) * rp + row + (lane & 31)) * 2 + half;
+            const float4 *w =
+                reinterpret_cast<const float4 *>(q) + ((int64_t)(k0 / 8) * rp + row + (lane & 31)) * 2 + half;
 #pragma unroll 2
             for (int s = 0; s < depth; s += 8) {
                 const float4 w4 = w[(int64_t)(s / 8) * rp * 2];
@@ -758,7 +769,8 @@ __device__ __forceinline__ void apply_slab(const Matrix &m, const Item &it, cons
                         xv[0] = x4.x; xv[1] = x4.y; xv[2] = x4.z; xv[3] = x4.w;
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) xv[e] = sx[(s + 4 * half + e) * kPitch + part + 32 * t + (lane & 31)];
+                        for (int e = 0; e < 4; ++e)
+                            xv[e] = sx[(s + 4 * half + e) * kPitch + part + 32 * t + (lane & 31)];
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
@@ -892,8 +904,9 @@ int64_t gram_cap(const std::vector<Shape> &shapes) {
 // A matrix's items and its number of partial Gram matrices.
 void plan_matrix(int32_t index, const Shape &s, int64_t cap, std::vector<Item> (&items)[kKinds], int32_t &splits) {
     const bool one_pass = s.r <= kOnePass;
+    const int64_t blocks = cdiv(s.r, kGramTile) * (cdiv(s.r, kGramTile) + 1) / 2;
     const int64_t parts = one_pass ? cdiv(s.width, gram_step(s, cap))
-                                   : std::max<int64_t>(1, std::min<int64_t>(cdiv(s.width, 512), 32));
+                                   : std::max<int64_t>(1, std::min<int64_t>(cdiv(s.width, 512), 1024 / blocks));
     const int64_t step = cdiv(cdiv(s.width, parts), kChunk) * kChunk;   // even parts
     const int64_t count = cdiv(s.width, step);
     auto range = [&](int64_t k, int32_t i, int32_t j) -> Item {
@@ -1033,8 +1046,8 @@ extern "C" int ct_muon(const ct_muon_matrix *matrices, int64_t count, const int3
         muon_join<<<grid(kItemsJoin), dim3(kThreads), 0, stream>>>(mats, items[kItemsJoin], h, ws);
         if (!ok()) return status;
         auto stage = [&](const StageOp &op0, const StageOp *op1) {
-            muon_stage<<<grid(kItemsStage, op1 ? 2 : 1), dim3(kStageThreads), 0, stream>>>(mats, items[kItemsStage], h, ws,
-                                                                                     op0, op1 ? *op1 : op0);
+            muon_stage<<<grid(kItemsStage, op1 ? 2 : 1), dim3(kStageThreads), 0, stream>>>(
+                mats, items[kItemsStage], h, ws, op0, op1 ? *op1 : op0);
             return ok();
         };
         int q = kQ;   // the product of the P so far; the first P is the first Q
