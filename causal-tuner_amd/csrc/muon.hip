@@ -16,11 +16,12 @@
 // on a fifth of the work); only the last product, of the final P_{n-1} ... P_0 and M, is float32.
 // Keeping P_{n-1} ... P_0 in float32 too would lose a factor of three in those cases.
 //
-// What bounds it, two layers' adapters of rank 256 (72M elements, 855 us a step): the Gram
-// pass 255 us (double matrix instructions, 66% of what a large library product reaches, and 12
-// bytes an element), the 14 launches of r x r products 24 us each (their operands' way from
-// L2, half of it, and double matrix instructions), the last product 314 us (16 bytes an
-// element at 3.7 TB/s, with float32 matrix instructions under it). Small sets: the launches.
+// What bounds it, two layers' adapters of rank 256 (36M elements, 754 us a step): the Gram
+// pass 229 us (double matrix instructions, 73% of its cycles at a clock that they pull down to
+// about 1.9 GHz; 12 bytes an element), the 14 launches of r x r products 24 us each (their
+// operands' way from L2, half of it, and double matrix instructions), the last product 240 us
+// (float32 matrix instructions, 62% of its cycles; 16 bytes an element, 2.4 TB/s, which alone
+// take 170). Small sets: the launches.
 // Tried and left out: 64 x 64 tiles in the r x r products (the same at 24 matrices, 20% slower
 // at 12), k-steps of 32 rows in flight instead of 16 (more registers, 3% slower).
 //
@@ -70,6 +71,22 @@ struct Hyper {
     double a, b, c, eps;
 };
 
+// Pointers that come out of memory may be of any kind to the compiler, and its flat loads are
+// waited for by every wait for LDS. These say that they are global: the Gram pass of two layers'
+// adapters went from 250 us to 230 by that alone.
+typedef float Float4 __attribute__((ext_vector_type(4)));
+typedef uint32_t Uint2 __attribute__((ext_vector_type(2)));
+template <typename V>
+__device__ __forceinline__ V from_global(const void *p) {
+    typedef const __attribute__((address_space(1))) V *Global;
+    return *(Global)(uintptr_t)p;
+}
+template <typename V>
+__device__ __forceinline__ void to_global(void *p, V v) {
+    typedef __attribute__((address_space(1))) V *Global;
+    *(Global)(uintptr_t)p = v;
+}
+
 __host__ __device__ __forceinline__ int64_t least(int64_t x, int64_t y) { return x < y ? x : y; }
 __device__ __forceinline__ int short_side(const Matrix &m) { return (int)least(m.rows, m.cols); }
 __host__ __device__ __forceinline__ int padded(int r) { return (r + kPad - 1) / kPad * kPad; }
@@ -107,19 +124,31 @@ __device__ __forceinline__ int64_t final_at(int rp, int row, int k) {
 
 template <typename T>
 __device__ __forceinline__ float load_elem(const void *p, int64_t i) {
-    if constexpr (sizeof(T) == 2) return bf16_to_f32(static_cast<const uint16_t *>(p)[i]);
-    else return static_cast<const float *>(p)[i];
+    if constexpr (sizeof(T) == 2) return bf16_to_f32(from_global<uint16_t>(static_cast<const uint16_t *>(p) + i));
+    else return from_global<float>(static_cast<const float *>(p) + i);
 }
-// Four elements from a multiple of four.
+// Four elements from a multiple of four, as they are stored; widened only when they are used,
+// since a load that is widened at once is waited for at once.
 template <typename T>
-__device__ __forceinline__ float4 load_four(const void *p, int64_t i) {
-    if constexpr (sizeof(T) == 2) {
-        const uint2 v = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i);
-        return make_float4(__builtin_bit_cast(float, v.x << 16), __builtin_bit_cast(float, v.x & 0xffff0000u),
-                           __builtin_bit_cast(float, v.y << 16), __builtin_bit_cast(float, v.y & 0xffff0000u));
-    } else {
-        return *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+struct Stored;
+template <>
+struct Stored<float> {
+    using four = Float4;
+    static __device__ __forceinline__ Float4 widen(Float4 v) { return v; }
+    static __device__ __forceinline__ float widen(float v) { return v; }
+};
+template <>
+struct Stored<uint16_t> {
+    using four = Uint2;
+    static __device__ __forceinline__ Float4 widen(Uint2 v) {
+        return {__builtin_bit_cast(float, v.x << 16), __builtin_bit_cast(float, v.x & 0xffff0000u),
+                __builtin_bit_cast(float, v.y << 16), __builtin_bit_cast(float, v.y & 0xffff0000u)};
     }
+    static __device__ __forceinline__ float widen(uint16_t v) { return bf16_to_f32(v); }
+};
+template <typename T>
+__device__ __forceinline__ typename Stored<T>::four load_four(const void *p, int64_t i) {
+    return from_global<typename Stored<T>::four>(static_cast<const T *>(p) + i);
 }
 
 // M from the gradient and the updated momentum.
@@ -129,7 +158,7 @@ __device__ __forceinline__ float combine(const Hyper &h, float g, float m) {
 template <typename T>
 __device__ __forceinline__ float source(const Matrix &m, const Hyper &h, int64_t i) {
     const float g = load_elem<T>(m.grad, i);
-    return h.step ? combine(h, g, m.momentum[i]) : g;
+    return h.step ? combine(h, g, load_elem<float>(m.momentum, i)) : g;
 }
 
 // Whether groups of four along a row can be loaded at once.
@@ -169,8 +198,14 @@ __device__ __forceinline__ f64x4 mfma_f64(double a, double b, f64x4 c) {
 constexpr int kGramThreads = 512;
 constexpr int kGramLds = 2 * kChunk * (kOnePass + 16);   // doubles: two stages, 139 KB
 
+template <typename T>
 struct Four {
-    float4 g, m;
+    typename Stored<T>::four g;
+    Float4 m;
+    __device__ __forceinline__ void set(int e, const T *p) {
+        if constexpr (sizeof(T) == 2) g[e / 2] |= (uint32_t)from_global<uint16_t>(p) << 16 * (e % 2);
+        else g[e] = from_global<float>(p);
+    }
 };
 
 template <typename T, int NT, bool TALL>
@@ -190,7 +225,7 @@ __device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, c
     const bool four = by_four<T>(m, h.step);
     const int64_t cols = m.cols;
     f64x4 acc[kMost] = {};
-    Four held[kPasses];
+    Four<T> held[kPasses];
 
     // A unit is four elements along a stored row; a thread's units are `gap` rows apart.
     constexpr int kRowUnits = TALL ? kRows / 4 : kChunk / 4, kGap = kGramThreads / kRowUnits;
@@ -207,20 +242,19 @@ __device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, c
     auto load = [&](int k0) {
 #pragma unroll
         for (int p = 0; p < kPasses; ++p) {
-            held[p] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+            held[p] = {};
             if (!active) continue;
             const int64_t at = at0 + p * gap;
             const int left = left_of(p, k0);
             if (four && left >= 4) {
                 held[p].g = load_four<T>(m.grad, at);
-                if (h.step) held[p].m = *reinterpret_cast<const float4 *>(m.momentum + at);
+                if (h.step) held[p].m = load_four<float>(m.momentum, at);
             } else {
-                float *g = &held[p].g.x, *v = &held[p].m.x;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (e < left) {
-                        g[e] = load_elem<T>(m.grad, at + e);
-                        if (h.step) v[e] = m.momentum[at + e];
+                        held[p].set(e, static_cast<const T *>(m.grad) + at + e);
+                        if (h.step) held[p].m[e] = load_elem<float>(m.momentum, at + e);
                     }
             }
         }
@@ -229,18 +263,18 @@ __device__ __forceinline__ void gram_one_pass(const Matrix &m, const Item &it, c
 #pragma unroll
         for (int p = 0; p < kPasses; ++p) {
             if (!active) continue;
-            float *g = &held[p].g.x, *v = &held[p].m.x;
+            Float4 g = Stored<T>::widen(held[p].g), v = held[p].m;
             if (h.step) {
                 const int64_t at = at0 + p * gap;
                 const int left = left_of(p, k0);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(h.mu, v[e], h.rest * g[e]);
                 if (four && left >= 4) {
-                    *reinterpret_cast<float4 *>(m.momentum + at) = held[p].m;
+                    to_global<Float4>(m.momentum + at, v);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (e < left) m.momentum[at + e] = v[e];
+                        if (e < left) to_global<float>(m.momentum + at + e, v[e]);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) g[e] = combine(h, g[e], v[e]);
@@ -405,7 +439,7 @@ __global__ __launch_bounds__(kThreads) void muon_momentum(const Matrix *matrices
     const Matrix m = matrices[it.matrix];
     const int r = short_side(m);
     for (int64_t i = (int64_t)it.lo * r + threadIdx.x; i < (int64_t)it.hi * r; i += kThreads)
-        m.momentum[i] = __builtin_fmaf(h.mu, m.momentum[i], h.rest * load_elem<T>(m.grad, i));
+        to_global<float>(m.momentum + i, __builtin_fmaf(h.mu, load_elem<float>(m.momentum, i), h.rest * load_elem<T>(m.grad, i)));
 }
 
 // One 64 x 64 tile (i >= j) of M M^T over the columns lo .. hi - 1: 4 waves of 32 x 32.
@@ -705,122 +739,262 @@ __global__ __launch_bounds__(kStageThreads) void muon_stage(const Matrix *matric
 
 // ------------------------------------------------------------------ the last product
 // Q M by 8 waves: each takes 32 rows of the short side and 64 elements of the long side
-// (v_mfma_f32_32x32x2, 2 x 32), so a workgroup covers 64, 128, 256 or 512 elements of the long
-// side with short sides up to 256, 128, 64 or 32. Its part of M (combined from gradient and
-// momentum on the way) stays in LDS, Q comes from L2 in the order that final_at gives it.
-// Short sides past 256 go in blocks of 256 rows and 256 of the reduction.
+// (v_mfma_f32_32x32x2, 2 x 32), so a slab covers 64, 128, 256 or 512 elements of the long side
+// with short sides up to 256, 128, 64 or 32. Its part of M (combined from gradient and momentum
+// on the way) lies in LDS, Q comes from L2 in the order that final_at gives it.
+// One workgroup per CU runs through an even share of all slabs, of several matrices if it has
+// to. Loads return in the order they were asked for, so a slab's product is cut into groups of
+// 32 of the reduction, and each group asks first for the next group's Q, then for a part of
+// the next slab's gradient and momentum and of its own parameters: those have a group's
+// products (1.7 us) to come in before anything waits behind them. Two layers' adapters of rank
+// 256 take 240 us; a slab per workgroup, two workgroups per CU with nothing asked for ahead,
+// took 302. Short sides past 256 go slab by slab, in blocks of 256 rows and 256 of the reduction.
 constexpr int kApplyThreads = 512;
+constexpr int kApplyLds = 18432;   // floats: 256 x 72, 128 x 136, 64 x 264, 32 x 520 and their transposes
 
 __host__ __device__ __forceinline__ int apply_blocks(int r) { return r <= 32 ? 1 : r <= 64 ? 2 : r <= 128 ? 4 : 8; }
 
-template <typename T, int NB, bool TALL>
-__device__ __forceinline__ void apply_slab(const Matrix &m, const Item &it, const Hyper &h, double *ws, float *sx) {
+// acc[t] += Q[32 rows, 32] M[32, 2 x 32 elements of the long side]; q: what the lane has of Q.
+template <int PITCH, bool TALL>
+__device__ __forceinline__ void apply_product(f32x16 (&acc)[2], const float4 (&q)[4], const float *sx, int part, int lane) {
+    const int half = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int s = 8 * i + 4 * half;
+        const float qv[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int l = part + 32 * t + (lane & 31);
+            float xv[4];
+            if constexpr (TALL) {
+                const float4 x4 = *reinterpret_cast<const float4 *>(sx + l * PITCH + s);
+                xv[0] = x4.x; xv[1] = x4.y; xv[2] = x4.z; xv[3] = x4.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) xv[e] = sx[(s + e) * PITCH + l];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                acc[t] = TALL ? __builtin_amdgcn_mfma_f32_32x32x2f32(xv[e], qv[e], acc[t], 0, 0, 0)
+                              : __builtin_amdgcn_mfma_f32_32x32x2f32(qv[e], xv[e], acc[t], 0, 0, 0);
+        }
+    }
+}
+
+// Where a lane's results go: register i is `8 (i / 4) + i % 4` rows of the stored matrix below
+// the lane's first, of which `limit` exist; a parameter that does not exist reads another.
+template <typename T, bool TALL>
+struct ApplyPlace {
+    T *param;
+    int64_t stride;
+    int limit;
+    __device__ __forceinline__ ApplyPlace(const Matrix &m, int r, int64_t width, int row, int64_t col, int lane) {
+        const int half = lane >> 5, s = row + (TALL ? lane & 31 : 4 * half);
+        const int64_t l = col + (TALL ? 4 * half : lane & 31);
+        stride = TALL ? r : m.cols;
+        const int64_t below = TALL ? (s < r ? width - l : 0) : (l < width ? r - s : 0);
+        limit = below > 32 ? 32 : below < 0 ? 0 : (int)below;
+        param = static_cast<T *>(m.param) + (limit ? (TALL ? l * r + s : (int64_t)s * m.cols + l) : 0);
+    }
+    __device__ static __forceinline__ int down(int i) { return 8 * (i >> 2) + (i & 3); }
+    __device__ __forceinline__ T load(int i) const {
+        const int last = limit > 1 ? limit - 1 : 0;
+        return from_global<T>(param + (uint64_t)(uint32_t)(down(i) < last ? down(i) : last) * (uint32_t)stride);
+    }
+    // acc = old keep - lr adjust acc
+    __device__ static __forceinline__ void update(f32x16 &acc, const T (&old)[16], const Hyper &h, const Matrix &m) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            acc[i] = __builtin_fmaf(-h.lr * m.adjust, acc[i], Stored<T>::widen(old[i]) * h.keep);
+    }
+    __device__ __forceinline__ void store(const f32x16 &v) const {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (down(i) >= limit) continue;
+            if constexpr (sizeof(T) == 2) to_global<uint16_t>(param + down(i) * stride, bf16_bits(v[i]));
+            else to_global<float>(param + down(i) * stride, v[i]);
+        }
+    }
+};
+
+template <typename T, int NB, bool TALL, bool STEP>
+__device__ __forceinline__ void apply_run(const Matrix &m, const Item &it, const Hyper &h, double *ws, float *lds) {
     constexpr int kLong = 64 * (8 / NB), kShort = 32 * NB;
     constexpr int kPitch = TALL ? kShort + 4 : kLong + 8;
-    constexpr int kUnits = kLong * kShort / 4 / kApplyThreads;   // 8
-    const int r = short_side(m), rp = padded(r), tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-    const int block = wave % NB, part = wave / NB * 64;
-    const int64_t width = TALL ? m.rows : m.cols, col0 = it.lo;
-    const bool four = by_four<T>(m, h.step);
-    const float *q = final_q(m, ws);
-    for (int r0 = 0; r0 < rp; r0 += kShort) {
-        const int row = r0 + 32 * block;   // this wave's short rows
+    constexpr int kUnits = kLong * kShort / 4 / kApplyThreads;   // 8, of four elements along a stored row
+    constexpr int kRowUnits = TALL ? kShort / 4 : kLong / 4, kGap = kApplyThreads / kRowUnits;
+    static_assert(kPitch * (TALL ? kLong : kShort) <= kApplyLds && kUnits == 8, "LDS");
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));   // keeps the variants' addresses apart: shared ones spill
+    const int r = short_side(m), rp = padded(r), lane = tid & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int row = 32 * (wave % NB), part = wave / NB * 64;
+    const int64_t width = TALL ? m.rows : m.cols;
+    const bool four = by_four<T>(m, STEP);
+    const int along = tid % kRowUnits * 4, across = tid / kRowUnits;
+    Four<T> held[kUnits];
+    // Past the matrix's end its last elements come instead: Q has zeros for the short side's
+    // (whose groups past rp are left out), the long side's results are not stored.
+    auto fetch = [&](int p, int64_t col0) {
+        const int line = across + p * kGap;
+        const int64_t left = width - col0;
+        const int down = TALL ? (int)least(line, left - 1) : least(line, r - 1);
+        const int right = TALL ? (int)least(along, r - 4) : (int)least(along, left - 4);
+        const int64_t at = (uint64_t)(uint32_t)down * (uint32_t)m.cols + (TALL ? col0 * m.cols : col0) + right;
+        held[p].g = load_four<T>(m.grad, at);
+        if constexpr (STEP) held[p].m = load_four<float>(m.momentum, at);
+    };
+    // Q of this wave's rows, group by group; a wave past the last row reads the last ones'.
+    const float4 *q = reinterpret_cast<const float4 *>(final_q(m, ws)) + (row < rp ? row : rp - 32) * 2;
+    unsigned q_lane = (lane & 31) * 2 + half;
+    int q_step = rp * 2;
+    auto q_at = [&](int group, int i) { return (q + (4 * group + i) * q_step)[q_lane]; };
+    float4 now[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) now[i] = q_at(0, i);
+    auto keep = [&](int p, float *sx) {
+        Float4 x = Stored<T>::widen(held[p].g);
+        if constexpr (STEP)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = combine(h, x[e], held[p].m[e]);
+        *reinterpret_cast<Float4 *>(sx + (across + p * kGap) * kPitch + along) = x;
+    };
+    if (four) {
+#pragma unroll
+        for (int p = 0; p < kUnits; ++p) fetch(p, it.lo);
+#pragma unroll
+        for (int p = 0; p < kUnits; ++p) keep(p, lds);
+    }
+    float *sx = lds, *other = lds + kApplyLds;
+    for (int64_t col0 = it.lo; col0 < it.hi; col0 += kLong) {
+        if (!four) {
+#pragma unroll 4
+            for (int u = tid; u < kLong * kShort; u += kApplyThreads) {
+                const int s = TALL ? u % kShort : u / kLong, l = TALL ? u / kShort : u % kLong;
+                const int64_t at = TALL ? (col0 + l) * r + s : s * m.cols + col0 + l;
+                sx[TALL ? l * kPitch + s : s * kPitch + l] = s < r && col0 + l < width ? source<T>(m, h, at) : 0.0f;
+            }
+        }
+        __syncthreads();
+        const bool more = four && col0 + kLong < it.hi;
+        const ApplyPlace<T, TALL> first(m, r, width, row, col0 + part, lane);
+        const ApplyPlace<T, TALL> second(m, r, width, row, col0 + part + 32, lane);
+        T old[2][16];
+        f32x16 acc[2] = {};
+#pragma unroll
+        for (int group = 0; group < NB; ++group) {
+            float4 ahead[4];
+            const int next = 32 * (group + 1) < rp ? group + 1 : 0;
+            asm volatile("" : "+v"(q_lane), "+s"(q_step));   // nor are the addresses kept from slab to slab
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ahead[i] = q_at(next, i);
+#pragma unroll
+            for (int p = 0; p < kUnits; ++p) {   // over the first three quarters of the groups
+                if (p * 3 * NB / 32 != group) continue;
+                if (more) fetch(p, col0 + kLong);
+                if constexpr (STEP)
+#pragma unroll
+                    for (int i = 2 * p; i < 2 * p + 2; ++i) {
+                        old[0][i] = first.load(i);
+                        old[1][i] = second.load(i);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (row < rp && 32 * group < rp)
+                apply_product<kPitch, TALL>(acc, now, sx + 32 * group * (TALL ? 1 : kPitch), part, lane);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int p = 0; p < kUnits; ++p)   // what has had a group's time or two
+                if (group == least(NB - 1, p * 3 * NB / 32 + NB / 4) && more) keep(p, other);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) now[i] = ahead[i];
+        }
+        if constexpr (STEP) {
+            first.update(acc[0], old[0], h, m);
+            second.update(acc[1], old[1], h, m);
+        }
+        first.store(acc[0]);
+        second.store(acc[1]);
+        float *swap = sx;
+        sx = other;
+        other = swap;
+    }
+}
+
+// Slabs of a matrix whose short side is past 256.
+template <typename T, bool TALL, bool STEP>
+__device__ __forceinline__ void apply_blocked(const Matrix &m, const Item &it, const Hyper &h, double *ws, float *sx) {
+    constexpr int kLong = 64, kShort = 256, kPitch = TALL ? kShort + 4 : kLong + 8;
+    const int r = short_side(m), rp = padded(r), tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t width = TALL ? m.rows : m.cols;
+    const int blocks = (rp + kShort - 1) / kShort;
+    for (int64_t n = 0; n < (it.hi - it.lo + kLong - 1) / kLong * blocks; ++n) {
+        const int64_t col0 = it.lo + n / blocks * kLong;
+        const int row = (int)(n % blocks) * kShort + 32 * wave;
         f32x16 acc[2] = {};
         for (int k0 = 0; k0 < rp; k0 += kShort) {
             __syncthreads();
-#pragma unroll
-            for (int p = 0; p < kUnits; ++p) {
-                const int u = p * kApplyThreads + tid;
-                const int s = TALL ? u % (kShort / 4) * 4 : u / (kLong / 4);
-                const int l = TALL ? u / (kShort / 4) : u % (kLong / 4) * 4;
-                const int64_t at = TALL ? (col0 + l) * r + k0 + s : (int64_t)(k0 + s) * m.cols + col0 + l;
-                const int64_t left = TALL ? (col0 + l < width ? r - k0 - s : 0) : (k0 + s < r ? width - col0 - l : 0);
-                float4 v = make_float4(0, 0, 0, 0);
-                if (four && left >= 4) {
-                    v = load_four<T>(m.grad, at);
-                    if (h.step) {
-                        const float4 b = *reinterpret_cast<const float4 *>(m.momentum + at);
-                        v = make_float4(combine(h, v.x, b.x), combine(h, v.y, b.y), combine(h, v.z, b.z),
-                                        combine(h, v.w, b.w));
-                    }
-                } else {
-                    float *x = &v.x;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (e < left) x[e] = source<T>(m, h, at + e);
-                }
-                *reinterpret_cast<float4 *>(sx + (TALL ? l * kPitch + s : s * kPitch + l)) = v;
+#pragma unroll 4
+            for (int u = tid; u < kLong * kShort; u += kApplyThreads) {
+                const int s = TALL ? u % kShort : u / kLong, l = TALL ? u / kShort : u % kLong;
+                const bool inside = k0 + s < r && col0 + l < width;
+                const int64_t at = TALL ? (col0 + l) * r + k0 + s : (k0 + s) * m.cols + col0 + l;
+                sx[TALL ? l * kPitch + s : s * kPitch + l] = inside ? source<T>(m, h, at) : 0.0f;
             }
             __syncthreads();
             if (row >= rp) continue;
-            const int depth = rp - k0 < kShort ? rp - k0 : kShort;
-            const float4 *w =
-                reinterpret_cast<const float4 *>(q) + ((int64_t)(k0 / 8) * rp + row + (lane & 31)) * 2 + half;
-#pragma unroll 2
-            for (int s = 0; s < depth; s += 8) {
-                const float4 w4 = w[(int64_t)(s / 8) * rp * 2];
-                const float wv[4] = {w4.x, w4.y, w4.z, w4.w};
+            const float4 *q = reinterpret_cast<const float4 *>(final_q(m, ws)) + (row + (lane & 31)) * 2 + (lane >> 5);
+            for (int s = 0; s < kShort && k0 + s < rp; s += 32) {
+                float4 now[4];
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    float xv[4];
-                    if constexpr (TALL) {
-                        const float4 x4 = *reinterpret_cast<const float4 *>(
-                            sx + (part + 32 * t + (lane & 31)) * kPitch + s + 4 * half);
-                        xv[0] = x4.x; xv[1] = x4.y; xv[2] = x4.z; xv[3] = x4.w;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            xv[e] = sx[(s + 4 * half + e) * kPitch + part + 32 * t + (lane & 31)];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        acc[t] = TALL ? __builtin_amdgcn_mfma_f32_32x32x2f32(xv[e], wv[e], acc[t], 0, 0, 0)
-                                      : __builtin_amdgcn_mfma_f32_32x32x2f32(wv[e], xv[e], acc[t], 0, 0, 0);
-                }
+                for (int i = 0; i < 4; ++i) now[i] = q[((int64_t)(k0 + s) / 8 + i) * rp * 2];
+                apply_product<kPitch, TALL>(acc, now, sx + s * (TALL ? 1 : kPitch), 0, lane);
             }
         }
         if (row >= rp) continue;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            // register i is `8 (i / 4) + i % 4` rows of the stored matrix below the lane's first
-            const int s = row + (TALL ? lane & 31 : 4 * half);
-            const int64_t l = col0 + part + 32 * t + (TALL ? 4 * half : lane & 31);
-            const int64_t stride = TALL ? r : m.cols, at = TALL ? l * r + s : (int64_t)s * m.cols + l;
-            const int64_t below = TALL ? (s < r ? width - l : 0) : (l < width ? r - s : 0);
-            const int limit = below > 32 ? 32 : (int)below;
-            T *lane_param = static_cast<T *>(m.param) + at;
+            const ApplyPlace<T, TALL> place(m, r, width, row, col0 + 32 * t, lane);
+            if constexpr (STEP) {
+                T old[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int down = 8 * (i >> 2) + (i & 3);
-                if (down >= limit) continue;
-                T *dst = lane_param + down * stride;
-                float v = acc[t][i];
-                if (h.step) v = __builtin_fmaf(-h.lr * m.adjust, v, load_elem<T>(dst, 0) * h.keep);
-                if constexpr (sizeof(T) == 2) *dst = bf16_bits(v);
-                else *dst = v;
+                for (int i = 0; i < 16; ++i) old[i] = place.load(i);
+                place.update(acc[t], old, h, m);
             }
+            place.store(acc[t]);
         }
     }
 }
 
-template <typename T, bool TALL>
-__device__ __forceinline__ void apply_by_size(const Matrix &m, const Item &it, const Hyper &h, double *ws, float *sx) {
+template <typename T, bool TALL, bool STEP>
+__device__ __forceinline__ void apply_by_size(const Matrix &m, const Item &it, const Hyper &h, double *ws, float *lds) {
+    if (short_side(m) > 256) return apply_blocked<T, TALL, STEP>(m, it, h, ws, lds);
     switch (apply_blocks(short_side(m))) {
-        case 1: return apply_slab<T, 1, TALL>(m, it, h, ws, sx);
-        case 2: return apply_slab<T, 2, TALL>(m, it, h, ws, sx);
-        case 4: return apply_slab<T, 4, TALL>(m, it, h, ws, sx);
-        default: return apply_slab<T, 8, TALL>(m, it, h, ws, sx);
+        case 1: return apply_run<T, 1, TALL, STEP>(m, it, h, ws, lds);
+        case 2: return apply_run<T, 2, TALL, STEP>(m, it, h, ws, lds);
+        case 4: return apply_run<T, 4, TALL, STEP>(m, it, h, ws, lds);
+        default: return apply_run<T, 8, TALL, STEP>(m, it, h, ws, lds);
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kApplyThreads, 4) void muon_apply(const Matrix *matrices, const Item *items, Hyper h,
+// An item's slot names the item that the same workgroup takes next, if any; those have pad0 = 1.
+template <typename T, bool STEP>
+__global__ __launch_bounds__(kApplyThreads, 2) void muon_apply(const Matrix *matrices, const Item *items, Hyper h,
                                                               double *ws) {
-    __shared__ __align__(16) float sx[18432];   // 256 x 72, 128 x 136, 64 x 264, 32 x 520 and their transposes
-    const Item it = items[blockIdx.x];
-    const Matrix m = matrices[it.matrix];
-    if (m.rows > m.cols) apply_by_size<T, true>(m, it, h, ws, sx);
-    else apply_by_size<T, false>(m, it, h, ws, sx);
+    __shared__ __align__(16) float lds[2 * kApplyLds];
+    Item it = items[blockIdx.x];
+    if (it.pad0) return;
+    for (;;) {
+        const Matrix m = matrices[it.matrix];
+        if (m.rows > m.cols) apply_by_size<T, true, STEP>(m, it, h, ws, lds);
+        else apply_by_size<T, false, STEP>(m, it, h, ws, lds);
+        if (!it.slot) break;
+        it = items[it.slot];
+        __syncthreads();
+    }
 }
 
 // ------------------------------------------------------------------ host side
@@ -901,6 +1075,45 @@ int64_t gram_cap(const std::vector<Shape> &shapes) {
     return high;
 }
 
+// The last product's slabs in even shares, one per CU. A slab of a short side past 256 costs
+// its blocks' products.
+void share_slabs(const std::vector<Shape> &shapes, std::vector<Item> &items) {
+    int64_t total = 0, slabs = 0, done = 0, last = -1;
+    auto length = [](const Shape &s) -> int64_t { return 64 * (8 / apply_blocks(s.r)); };
+    auto cost = [](const Shape &s) { return cdiv(s.r, 256) * cdiv(s.r, 256); };
+    for (const Shape &s : shapes) {
+        slabs += cdiv(s.width, length(s));
+        total += cdiv(s.width, length(s)) * cost(s);
+    }
+    const int64_t shares = std::min(slabs, kGroupsWanted);
+    std::vector<Item> more;
+    std::vector<int32_t> owner;   // of each in `more`: the share it belongs to
+    for (size_t i = 0; i < shapes.size(); ++i) {
+        const Shape &s = shapes[i];
+        const int64_t slab = length(s), count = cdiv(s.width, slab);
+        for (int64_t c = 0, n; c < count; c += n) {
+            const int64_t share = done * shares / total, end = cdiv((share + 1) * total, shares);
+            n = std::min(count - c, cdiv(end - done, cost(s)));
+            const Item it = {(int32_t)i, 0, 0, (int32_t)(c * slab), (int32_t)std::min(s.width, (c + n) * slab), 0, share == last, 0};
+            if (it.pad0) {
+                more.push_back(it);
+                owner.push_back((int32_t)items.size() - 1);
+            } else {
+                items.push_back(it);
+            }
+            last = share;
+            done += n * cost(s);
+        }
+    }
+    const int32_t firsts = (int32_t)items.size();
+    for (size_t k = 0; k < more.size(); ++k) {
+        const int32_t index = firsts + (int32_t)k;
+        if (k && owner[k - 1] == owner[k]) items.back().slot = index;
+        else items[(size_t)owner[k]].slot = index;
+        items.push_back(more[k]);
+    }
+}
+
 // A matrix's items and its number of partial Gram matrices.
 void plan_matrix(int32_t index, const Shape &s, int64_t cap, std::vector<Item> (&items)[kKinds], int32_t &splits) {
     const bool one_pass = s.r <= kOnePass;
@@ -931,9 +1144,6 @@ void plan_matrix(int32_t index, const Shape &s, int64_t cap, std::vector<Item> (
         for (int a = 0; a < s.rp / kPad; ++a)
             for (int b = 0; b <= a; ++b) items[kItemsStage].push_back({index, a, b, 0, 0, 0, 0, 0});
     }
-    const int64_t slab = 64 * (8 / apply_blocks(s.r));
-    for (int64_t c = 0; c < s.width; c += slab)
-        items[kItemsApply].push_back({index, 0, 0, (int32_t)c, (int32_t)std::min(s.width, c + slab), 0, 0, 0});
 }
 
 }  // namespace
@@ -965,6 +1175,7 @@ extern "C" int ct_muon_plan(ct_muon_matrix *matrices, int64_t count, int32_t *en
             matrices[i].scratch = doubles;
             doubles += scratch_doubles(s);
         }
+        share_slabs(shapes, items[kItemsApply]);
         by_xcd(items[kItemsStage]);
         int64_t size = 0;
         for (int k = 0; k < kKinds; ++k) {
@@ -1065,7 +1276,8 @@ extern "C" int ct_muon(const ct_muon_matrix *matrices, int64_t count, const int3
             if (!first) q = next;
         }
     }
-    const auto kernel = half ? muon_apply<uint16_t> : muon_apply<float>;
+    const auto kernel = half ? (h.step ? muon_apply<uint16_t, true> : muon_apply<uint16_t, false>)
+                             : (h.step ? muon_apply<float, true> : muon_apply<float, false>);
     kernel<<<grid(kItemsApply), dim3(kApplyThreads), 0, stream>>>(mats, items[kItemsApply], h, ws);
     return status_of_last_launch();
 }

@@ -50,7 +50,7 @@ def _matrix(shape, dtype, decades=None, seed=0):
 
 
 SHAPES = [(1, 1), (1, 7), (5, 1), (3, 3), (16, 1024), (1024, 16), (31, 33), (33, 31), (64, 64), (65, 200), (130, 1111),
-          (2049, 64), (255, 257), (256, 4096), (4100, 128), (8, 3001), (300, 513), (700, 290)]
+          (2049, 64), (100, 300), (300, 100), (40, 516), (516, 252), (160, 640), (255, 257), (256, 4096), (4100, 128), (8, 3001), (300, 513), (700, 290)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -96,6 +96,17 @@ def test_zero_tiny_and_infinite_matrices():
     assert not x.any()
     _check(y, tiny)
     assert torch.isnan(z).all()
+
+
+def test_more_matrices_than_workgroups():
+    """Workgroups of the last product go from one matrix to the next, of other sizes, kinds and
+    alignments."""
+    from causal_tuner.optim import orthogonalize
+    sizes = [(8, 20), (100, 36), (5, 7), (40, 516), (1, 1), (260, 270), (33, 31), (1030, 24), (70, 200)]
+    matrices = [_matrix(sizes[i % len(sizes)], torch.float32, seed=i) for i in range(330)]
+    matrices[1::11] = [m.new_empty(m.numel() + 1)[1:].view(m.shape).copy_(m) for m in matrices[1::11]]
+    for m, got in zip(matrices, orthogonalize(matrices)):
+        _check(got, m)
 
 
 @pytest.mark.parametrize("steps,coefficients", [(1, (2.0, -1.5, 0.5)), (2, (A, B, C)), (3, (1.875, -1.25, 0.375)),
