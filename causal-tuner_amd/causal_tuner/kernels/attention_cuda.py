@@ -232,14 +232,14 @@ class _PackedAttention(torch.autograd.Function):
 
 
 def _host_attention(q, k, v, layout, causal, scale):
-    """The same in torch operations, record by record in float32."""
-    group = q.shape[1] // k.shape[1]
+    """The same in torch operations, record by record in float32 (float64 for its tensors)."""
+    group, wide = q.shape[1] // k.shape[1], torch.promote_types(q.dtype, torch.float32)
     out = q.new_zeros(q.shape)
     for (qa, qb), (ka, kb) in zip(layout.records, layout.key_records):
         if qa == qb or ka == kb:
             continue
-        query = q[qa:qb].float().transpose(0, 1)
-        key, value = (t[ka:kb].float().repeat_interleave(group, 1).transpose(0, 1) for t in (k, v))
+        query = q[qa:qb].to(wide).transpose(0, 1)
+        key, value = (t[ka:kb].to(wide).repeat_interleave(group, 1).transpose(0, 1) for t in (k, v))
         s = (query @ key.transpose(1, 2)) * scale
         hidden = torch.zeros(qb - qa, kb - ka, dtype=torch.bool)
         if causal:
@@ -270,13 +270,15 @@ def packed_attention(q, k, v, records, *, causal=True, scale=None):
         raise ValueError(f"packed_attention: {heads} heads of {head_dim} do not share {kv_heads} of {key_dim}")
     if not q.dtype == k.dtype == v.dtype:
         raise ValueError("packed_attention: mismatched element types")
+    if not q.is_floating_point():
+        raise ValueError("packed_attention: tensors of a floating type required")
     if not q.device == k.device == v.device:
         raise ValueError("packed_attention: q, k and v are on different devices")
     if head_dim == 0:
         raise ValueError("packed_attention: heads of no channels")
     scale = head_dim ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"packed_attention: scale {scale} is not a positive number")
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:   # of float32's normal range, log2(e) times it too
+        raise ValueError(f"packed_attention: scale {scale} is not a positive float32 number up to 2^126")
     layout = records if isinstance(records, AttentionLayout) else AttentionLayout(records, q.device)
     if layout.tokens > tokens or layout.key_tokens > key_tokens:
         raise ValueError(f"packed_attention: records reach to {layout.tokens} queries and {layout.key_tokens} keys, "

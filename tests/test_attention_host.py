@@ -31,6 +31,14 @@ def test_list_of_records_and_batch_dimension():
     check((out[0],), *reference(q[0], k[0], v[0], [(0, 4), (4, 9)], [(0, 4), (4, 9)], True, 0.3))
 
 
+def test_host_path_in_double():
+    """Double tensors are worked on in double: against differences, with a shared head and queries
+    that see no key."""
+    q, k, v = (torch.randn(n, h, 3, dtype=torch.float64, requires_grad=True) for n, h in ((7, 4), (6, 2), (6, 2)))
+    layout = AttentionLayout([(0, 4), (4, 7)], "cpu", key_records=[(0, 2), (2, 6)])
+    assert torch.autograd.gradcheck(lambda *t: packed_attention(*t, layout), (q, k, v))
+
+
 def test_refusals():
     with pytest.raises(ValueError, match="overlap"):
         AttentionLayout([(0, 5), (4, 8)], "cpu")
@@ -44,7 +52,8 @@ def test_refusals():
     bad = [(q, torch.zeros(5, 3, 8), torch.zeros(5, 3, 8), {}), (q, torch.zeros(5, 2, 16), torch.zeros(5, 2, 16), {}),
            (q, k, torch.zeros(6, 2, 8), {}), (q[0], k, k, {}), (q, k.double(), k.double(), {}),
            (q, torch.zeros(5, 0, 8), torch.zeros(5, 0, 8), {}), (q, k, k, {"scale": 0.0}), (q, k, k, {"scale": -1.0}),
-           (q, k, k, {"scale": float("nan")}), (q, k, k, {"scale": float("inf")}),
+           (q, k, k, {"scale": float("nan")}), (q, k, k, {"scale": float("inf")}), (q, k, k, {"scale": 1e-60}),
+           (q, k, k, {"scale": 3e38}), (q.int(), k.int(), k.int(), {}),
            (torch.zeros(5, 4, 0), torch.zeros(5, 2, 0), torch.zeros(5, 2, 0), {})]
     for a, b, c, options in bad:
         with pytest.raises(ValueError):
