@@ -238,7 +238,8 @@ class FusedMuon(torch.optim.Optimizer):
     Each step: momentum = mu momentum + (1 - mu) grad, M = mu momentum + (1 - mu) grad (nesterov)
     or momentum, param = param (1 - lr weight_decay) - lr adjust orthogonalize(M), with adjust =
     sqrt(max(1, rows / cols)) ("original", the default) or 0.2 sqrt(max(rows, cols))
-    ("match_rms_adamw")."""
+    ("match_rms_adamw"). A step can be captured into a graph after a first one outside; the
+    graph keeps the learning rate and the other numbers that it was captured with."""
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
                  ns_coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, ns_steps=5, adjust_lr_fn=None):
@@ -275,6 +276,9 @@ class FusedMuon(torch.optim.Optimizer):
     def _buffer_of(self, p):
         state = self.state[p]
         if "momentum_buffer" not in state:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("FusedMuon: a parameter's first step makes its momentum_buffer and cannot be captured "
+                                   "(every replay would clear it); run a step before the capture")
             state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
         buffer = state["momentum_buffer"]
         if (buffer.dtype != torch.float32 or buffer.shape != p.shape or buffer.device != p.device

@@ -623,8 +623,9 @@ typedef struct ct_muon_options {
  * cut into workgroups' shares: 32-byte entries of CT_MUON_KINDS kinds, counts[0 ..
  * CT_MUON_KINDS - 1] of them one kind after the other, and the bytes of workspace. With
  * entries = null only counts, the table and workspace_bytes are written. The caller copies the
- * entries to the device (16-byte aligned); they hold for every call with these shapes. Empty matrices are refused: the caller leaves them out. ct_muon reads the
- * host table while it runs and passes it to the device in kernel arguments.
+ * entries to the device (16-byte aligned); they hold for every call with these shapes. Empty
+ * matrices are refused: the caller leaves them out. ct_muon reads the host table while it runs
+ * and passes it to the device in kernel arguments.
  */
 int ct_muon_plan(ct_muon_matrix *matrices, int64_t count, int32_t *entries, int64_t capacity, int64_t *counts,
                  int64_t *workspace_bytes);

@@ -209,6 +209,13 @@ def test_captured_steps_replay():
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             orthogonalize(torch.ones(11, 13, device="cuda"))
     torch.cuda.synchronize()
+    fresh = torch.nn.Parameter(params[0].detach().clone())   # of a known shape, but without a buffer
+    fresh.grad = torch.ones_like(fresh)
+    orthogonalize(fresh.grad)
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            FusedMuon([fresh]).step()
+    torch.cuda.synchronize()
     _check(orthogonalize(params[0].detach()), params[0].detach())
 
 
