@@ -62,7 +62,7 @@ class Attention(ctypes.Structure):
     _fields_ = [
         ("q", _P), ("k", _P), ("v", _P), ("q_token", _I64), ("q_head", _I64), ("k_token", _I64), ("k_head", _I64),
         ("v_token", _I64), ("v_head", _I64), ("records", _P), ("heads", _I32), ("kv_heads", _I32),
-        ("head_dim", _I32), ("dtype", _I32), ("causal", _I32), ("scale", ctypes.c_float),
+        ("head_dim", _I32), ("dtype", _I32), ("causal", _I32), ("scale", ctypes.c_float), ("rest", _P),
     ]
 
 

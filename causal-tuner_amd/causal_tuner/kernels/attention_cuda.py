@@ -14,7 +14,8 @@ queries are then the last of them (causal: query i of L_q sees keys 0 .. i + L_k
 form of a prompt that continues a cache and, with one query per record, of writing answers
 token by token. A query that sees no key gives zeros, and no gradient. The scores, their
 statistics and every sum are float32; the probabilities and their gradients are rounded to
-bf16 for bf16 inputs. Repeated calls, backward included, are bit-identical.
+bf16 for bf16 inputs, whose backward keeps the output's rounding error, a tensor of the output's
+size. Repeated calls, backward included, are bit-identical.
 
 A masked score counts as minus infinity whatever it holds, and rows of no record are never
 read. Inside a record, a key or value that is not finite makes NaN of every row whose tile of
@@ -153,17 +154,17 @@ def _strided(t, tokens_at_once, heads):
     return t
 
 
-def _operands(q, k, v, tables, causal, scale):
+def _operands(q, k, v, tables, causal, scale, rest):
     q_token, q_head, _ = q.stride()
     k_token, k_head, _ = k.stride()
     v_token, v_head, _ = v.stride()
     return _native.Attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), q_token, q_head, k_token, k_head, v_token, v_head,
                              tables.records, q.shape[1], k.shape[1], q.shape[2], _native.dtype_code(q.dtype), causal,
-                             scale)
+                             scale, _native.ptr(rest))
 
 
 def _forward(q, k, v, layout, causal, scale, keep_stats):
-    """(q, k, v as the kernels read them, out, stats or None)."""
+    """(q, k, v as the kernels read them, out, its rounding error or None, stats or None)."""
     tokens, heads, head_dim = q.shape
     kv_heads = k.shape[1]
     group = heads // kv_heads
@@ -171,6 +172,7 @@ def _forward(q, k, v, layout, causal, scale, keep_stats):
     work = layout.tokens and layout.key_tokens   # else there is nothing but zeros
     fresh = torch.empty if work and layout.whole and layout.tokens == tokens else torch.zeros
     out = fresh((tokens, heads, head_dim), dtype=q.dtype, device=q.device)
+    rest = torch.empty_like(out) if keep_stats and q.dtype == torch.bfloat16 else None
     stats = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if keep_stats else None
     if work:
         tables = layout.tables(heads, kv_heads, head_dim, q.dtype, causal)
@@ -180,10 +182,10 @@ def _forward(q, k, v, layout, causal, scale, keep_stats):
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         with _native.device_of(q):
             status = _native.library().ct_attention_forward(
-                _operands(q, k, v, tables, causal, scale), plan.entries, plan.counts, out.data_ptr(),
+                _operands(q, k, v, tables, causal, scale, rest), plan.entries, plan.counts, out.data_ptr(),
                 _native.ptr(stats), _native.ptr(workspace), nbytes, stream)
         _native.check(status, "ct_attention_forward")
-    return q, k, v, out, stats
+    return q, k, v, out, rest, stats
 
 
 class _PackedAttention(torch.autograd.Function):
@@ -191,15 +193,15 @@ class _PackedAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, layout, causal, scale):
-        q, k, v, out, stats = _forward(q, k, v, layout, causal, scale, True)
-        ctx.save_for_backward(q, k, v, out, stats)
+        q, k, v, out, rest, stats = _forward(q, k, v, layout, causal, scale, True)
+        ctx.save_for_backward(q, k, v, out, rest, stats)
         ctx.layout, ctx.causal, ctx.scale = layout, causal, scale
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, stats = ctx.saved_tensors
+        q, k, v, out, rest, stats = ctx.saved_tensors
         layout, causal, scale = ctx.layout, ctx.causal, ctx.scale
         if not layout.keys_disjoint:
             raise RuntimeError("packed_attention: key_records that overlap have no backward")
@@ -224,7 +226,7 @@ class _PackedAttention(torch.autograd.Function):
             dout_token, dout_head, _ = dout.stride()
             with _native.device_of(q):
                 status = _native.library().ct_attention_backward(
-                    _operands(q, k, v, tables, causal, scale), rows.entries, rows.counts, keys.entries, keys.counts,
+                    _operands(q, k, v, tables, causal, scale, rest), rows.entries, rows.counts, keys.entries, keys.counts,
                     out.data_ptr(), stats.data_ptr(), dout.data_ptr(), dout_token, dout_head, at, dq.data_ptr(),
                     dk.data_ptr(), dv.data_ptr(), at + delta if nbytes else None, nbytes, stream)
             _native.check(status, "ct_attention_backward")

@@ -23,8 +23,11 @@
 //
 // Rounding. Scores, statistics, delta and all sums are fp32. bf16 inputs round p and ds to
 // bf16 for the second products, which take bf16 (each value off by at most 2^-8 of itself, as
-// the output's own rounding: together 1.4 times the output's, 0.0025 against 0.0017 in norm);
-// float32 inputs round nothing.
+// the output's own rounding: together 1.4 times the output's, 0.0024 against 0.0017 in norm);
+// float32 inputs round nothing. Where a row sees few keys, do . v and delta nearly cancel, and
+// a delta from the rounded output made dq and dk 0.005 off (records of one to four tokens): the
+// output is divided by the sum of the p that entered its product (lse keeps the exact one), and
+// for a backward the forward keeps the output's rounding error in bf16 as well (`rest`).
 //
 // dq and dk/dv are two kernels that each recompute s (7 products instead of 5): the one-pass
 // form would add dq over workgroups by atomics, whose order changes results from run to run,
@@ -32,10 +35,11 @@
 // 32 heads) outweighs the two products.
 //
 // What bounds it. The matrix instructions and, beside them, the exponentials: 8192 causal rows
-// of 32 heads of 128 over one key/value head, bf16: forward 603 us (912 TFLOP/s), dq 821 (1004),
-// dk and dv 1388 (792), where a large library product reaches 1095 TFLOP/s on the same card
-// (its clock falls under that load) and HBM traffic is a few percent. Few query tokens: the
-// stream of keys and values, 131072 keys of 8 heads in 104 us, 5.2 TB/s (a large copy 5.1).
+// of 32 heads of 128 over one key/value head, bf16: forward 608 us (905 TFLOP/s; 598 without
+// the second sum and `rest`), dq 831 (992), dk and dv 1388 (792), where a large library product
+// reaches 1095 TFLOP/s on the same card (its clock falls under that load) and HBM traffic is a
+// few percent. Few query tokens: the stream of keys and values, 131072 keys of 8 heads in 104
+// us, 5.2 TB/s (a large copy 5.1).
 // Tried and left out: the two waves of a SIMD in turns (one in matrix instructions while the
 // other has its exponentials, two barriers a step): forward 615 -> 580 us, but 43 -> 46 at three
 // short records and both backward kernels slower; 8 waves per forward workgroup (7% slower at
@@ -86,6 +90,7 @@ struct AttnParams {
     const Item *items;
     const Group *groups;
     char *dst0, *dst1;    // out | dq | dk, dv
+    char *rest;           // out's rounding error, as out, or null
     int64_t d_token;      // bytes between tokens of dst0 and dst1
     float *stats;         // [tokens, heads] lse * log2(e), +inf where a row sees no key
     float *delta;         // [tokens, heads]
@@ -195,11 +200,18 @@ __device__ __forceinline__ void scores(f32x16 &acc, uint32_t tile, int row0, con
     }
 }
 
+// sum + the two values of a pair rounded to bf16 (v_dot2_f32_bf16).
+__device__ __forceinline__ float add_pair(uint32_t pair, float sum) {
+    const bf16x2_v ones = {(__bf16)1.0f, (__bf16)1.0f};
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, pair), ones, sum, false);
+}
+
 // acc[b][d, col] += sum_row tile[row0 + row][32 b + d] * p[row, col], p as `scores` leaves it:
-// register i of lane half h is row 8 (i / 4) + 4 h + i % 4.
+// register i of lane half h is row 8 (i / 4) + 4 h + i % 4. `taken`: the sum of the lane's p as
+// they enter the product.
 template <typename T, int DP>
 __device__ __forceinline__ void outer(f32x16 (&acc)[DP / 32], uint32_t tile, int row0, const f32x16 &p,
-                                      const Lanes<T, DP> &at) {
+                                      const Lanes<T, DP> &at, float *taken = nullptr) {
     const uint32_t base = tile + row0 * Tile<T, DP>::kBytes;
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -209,6 +221,7 @@ __device__ __forceinline__ void outer(f32x16 (&acc)[DP / 32], uint32_t tile, int
             b.y = pack_bf16x2(p[8 * s + 2], p[8 * s + 3]);
             b.z = pack_bf16x2(p[8 * s + 4], p[8 * s + 5]);
             b.w = pack_bf16x2(p[8 * s + 6], p[8 * s + 7]);
+            if (taken) *taken = add_pair(b.w, add_pair(b.z, add_pair(b.y, add_pair(b.x, *taken))));
 #pragma unroll
             for (int n = 0; n < DP / 32; ++n) {
                 const uint2 l2 = lds_read_transposed(at.col[2 * n] + base + 16 * s * Tile<T, DP>::kBytes);
@@ -307,6 +320,13 @@ __device__ __forceinline__ void store4(char *row, int d, float x, float y, float
     else
         *reinterpret_cast<float4 *>(row + 4 * d) = make_float4(x, y, z, w);
 }
+// What that rounding left of them.
+template <typename T>
+__device__ __forceinline__ void store4_rest(char *row, int d, float x, float y, float z, float w) {
+    if constexpr (sizeof(T) == 2)
+        store4<T>(row, d, x - bf16_to_f32(bf16_bits(x)), y - bf16_to_f32(bf16_bits(y)), z - bf16_to_f32(bf16_bits(z)),
+                  w - bf16_to_f32(bf16_bits(w)));
+}
 
 // ------------------------------------------------------------------ rows of a forward or dq tile
 struct RowOf {
@@ -361,7 +381,7 @@ __device__ __forceinline__ void by_stage(int from, int to, F f) {
 // Running softmax of a wave's 32 rows over their keys; m2 is the reference exponent of base
 // 2 that p and the sums are relative to.
 struct Running {
-    float m2 = -INFINITY, sum = 0.0f;
+    float m2 = -INFINITY, sum = 0.0f, taken = 0.0f;   // taken: the sum of p as rounded for the product
 };
 
 // ------------------------------------------------------------------ forward
@@ -442,6 +462,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
                     const float shrink = grown == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run.m2 - grown);
                     run.m2 = grown;
                     run.sum *= shrink;
+                    run.taken *= shrink;
 #pragma unroll
                     for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
@@ -455,7 +476,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
                         s[t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.scale2, -ref));
                         run.sum += s[t][i];
                     }
-                    outer<T, DP>(o, lds_of(sv) + buf * (uint32_t)sizeof(sv[0]), 32 * t, s[t], at);
+                    outer<T, DP>(o, lds_of(sv) + buf * (uint32_t)sizeof(sv[0]), 32 * t, s[t], at, &run.taken);
                 }
             }
             if (more) {
@@ -470,30 +491,35 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
         }
 
         const float sum = run.sum + other_half(run.sum);
+        const float taken = sizeof(T) == 2 ? run.taken + other_half(run.taken) : sum;
         const int d0 = 4 * (lane >> 5);
         if (!row.valid) continue;
         if (item.slot < 0) {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            char *dst = a.dst0 + row.token * a.o_token + row.head * a.o_head;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / taken;
+            const int64_t at = row.token * a.o_token + row.head * a.o_head;
+            char *dst = a.dst0 + at;
 #pragma unroll
             for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
                     const int d = 32 * n + 2 * i + d0;
-                    if (d < a.head_dim)
-                        store4<T>(dst, d, o[n][i] * inv, o[n][i + 1] * inv, o[n][i + 2] * inv, o[n][i + 3] * inv);
+                    if (d >= a.head_dim) continue;
+                    const float x = o[n][i] * inv, y = o[n][i + 1] * inv, z = o[n][i + 2] * inv, w = o[n][i + 3] * inv;
+                    store4<T>(dst, d, x, y, z, w);
+                    if (a.rest) store4_rest<T>(a.rest + at, d, x, y, z, w);
                 }
             if (a.stats && lane < 32)
                 a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : run.m2 + __builtin_amdgcn_logf(sum);
         } else {
             const int64_t at = ((int64_t)item.slot * a.kv_heads + kv_head) * (32 * WAVES) + wave * kWaveCols + (lane & 31);
             float *dst = a.part0 + at * DP;
+            const float scale = sum == 0.0f ? 0.0f : sum / taken;   // joined with the exact sums as weights
 #pragma unroll
             for (int n = 0; n < DP / 32; ++n)
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
                     *reinterpret_cast<float4 *>(dst + 32 * n + 2 * i + d0) =
-                        make_float4(o[n][i], o[n][i + 1], o[n][i + 2], o[n][i + 3]);
+                        make_float4(o[n][i] * scale, o[n][i + 1] * scale, o[n][i + 2] * scale, o[n][i + 3] * scale);
             if (lane < 32) *reinterpret_cast<float2 *>(a.part1 + 2 * at) = make_float2(run.m2, sum);
         }
     }
@@ -555,9 +581,12 @@ __global__ __launch_bounds__(kThreads) void attention_join(AttnParams a, const I
     const Record rec = a.records[join.record];
     const RowOf row(a, rec, kv_head, (int64_t)join.begin + r);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (4 * lane < a.head_dim)
-        store4<T>(a.dst0 + row.token * a.o_token + row.head * a.o_head, 4 * lane, acc.x * inv, acc.y * inv, acc.z * inv,
-                  acc.w * inv);
+    const int64_t at = row.token * a.o_token + row.head * a.o_head;
+    acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if (4 * lane < a.head_dim) {
+        store4<T>(a.dst0 + at, 4 * lane, acc.x, acc.y, acc.z, acc.w);
+        if (a.rest) store4_rest<T>(a.rest + at, 4 * lane, acc.x, acc.y, acc.z, acc.w);
+    }
     if (a.stats && lane == 0)
         a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
@@ -615,6 +644,11 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
         float delta = 0.0f;
 #pragma unroll
         for (int s = 0; s < Tile<T, DP>::kFrags; ++s) delta = dot_chunk<T>(gf[s], qf[s], delta);
+        if (sizeof(T) == 2 && a.rest) {
+            row_fragments<T, DP>(a.rest + row.token * a.o_token + row.head * a.o_head, qf, row.valid, chunks, lane);
+#pragma unroll
+            for (int s = 0; s < Tile<T, DP>::kFrags; ++s) delta = dot_chunk<T>(gf[s], qf[s], delta);
+        }
         delta += other_half(delta);
         float lse = INFINITY;
         if (row.valid) {
@@ -987,6 +1021,8 @@ int fill_params(const ct_attention *c, AttnParams &a) {
     a.causal = c->causal ? 1 : 0;
     a.scale = c->scale;
     a.scale2 = c->scale * kLog2e;
+    a.rest = c->dtype == CT_BF16 ? (char *)c->rest : nullptr;
+    if ((uintptr_t)a.rest % 16) return -CT_EINVAL_POINTER;
     // r / group for r < 2^31: with 2^s >= group and M = floor(2^(31+s) / group) + 1,
     // r M / 2^(31+s) exceeds r / group by less than 1 / group.
     int s = 0;

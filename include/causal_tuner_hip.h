@@ -544,6 +544,8 @@ typedef struct ct_attention {
     int32_t dtype;
     int32_t causal;
     float scale;
+    void *rest;       /* bf16 [tokens, heads, head_dim] contiguous: what out's rounding left, written by
+                         the forward, read by the backward; null: not kept. Unused for CT_F32 */
 } ct_attention;
 
 #define CT_ATTENTION_FORWARD 0  /* ct_attention_forward */

@@ -6,8 +6,10 @@ With u half a step of the tensors' type, e = 2^-24 and g = n e for a float32 sum
 
 * a score is off by at most S = g_d |scale| sum |q||k| + 2 e |s| in its exponent, so p by
   S + max_j S relative (numerator and normalizer), plus u where it is rounded to bf16;
-* o = sum p v gains g_n + u (its own rounding);
-* delta = do . o uses the rounded o: its error is |do| . bound(o) + g_d |do| . |o|;
+* o = sum p v / sum p, both of the rounded p, gains g_n + u (its own rounding); a rounding of
+  p_j by r_j, |r_j| <= u, moves it by sum p_j r_j (v_j - o), at most u (sum p |v| + |o|);
+* delta = do . o uses o and, for bf16, its rounding error, itself rounded to bf16 (off by u^2 |o|);
+  its error is |do| . (the bound of that o) + g_d |do| . |o|;
 * ds = p (do . v - delta) adds p times those errors and g_d |do| . |v|, and u |ds| where rounded;
 * dq, dk, dv are sums of such terms, rounded once."""
 
@@ -54,14 +56,15 @@ def reference(q, k, v, records, key_records, causal, scale, dout=None):
             off = torch.where(seen, off, torch.zeros_like(off))
             dp_rel = off + off.amax(-1, keepdim=True) + 2 * gn + pu
             o = p @ value
-            bo = (p * dp_rel) @ value.abs() + 2 * gn * (p @ value.abs())
+            bo = (p * dp_rel) @ value.abs() + 2 * gn * (p @ value.abs()) + pu * o.abs()
+            taken = bo + (u * u if pu else u) * (o.abs() + bo)   # of what delta is made from
             bo = bo + u * (o.abs() + bo)
             values[0][qa:qb, h], bounds[0][qa:qb, h] = o, bo
             if dout is None:
                 continue
             g = dout[qa:qb, h]
             delta = (g * o).sum(-1, keepdim=True)
-            b_delta = (g.abs() * bo).sum(-1, keepdim=True) + gd * (g.abs() * o.abs()).sum(-1, keepdim=True)
+            b_delta = (g.abs() * taken).sum(-1, keepdim=True) + gd * (g.abs() * o.abs()).sum(-1, keepdim=True)
             part = g @ value.T - delta
             ds = p * part
             b_ds = ds.abs() * (dp_rel + 4 * E32) + p * (1 + dp_rel) * (

@@ -61,6 +61,22 @@ def test_queries_that_see_no_key(dtype):
     assert not out[70:79].any() and not dk[10:22].any() and not dv[10:22].any()
 
 
+def test_gradients_of_short_records_in_norm():
+    """Where a row sees few keys, do . v - delta nearly cancels. ds, the results and the p behind
+    delta are each rounded to bf16: uniform errors of at most half a step, 2^-8 / sqrt(3) in root
+    mean square, together 2^-8 in norm; delta from the rounded output alone gives 0.0047."""
+    from causal_tuner.kernels.attention_cuda import AttentionLayout
+    sizes = [1 + i % 4 for i in range(300)]
+    records = records_of(sizes)
+    q, k, v, dout = _tensors(sum(sizes), sum(sizes), 8, 8, 128, torch.bfloat16)
+    got = _run(q, k, v, dout, AttentionLayout(records, "cuda"))
+    want, _ = reference(q, k, v, records, records, True, 128 ** -0.5, dout)
+    for x, y in zip(got, want):
+        assert (x.double() - y).norm() <= 2.0 ** -8 * y.norm()
+    lone = [a for a, b in records if b - a == 1]   # one key: p = 1, ds = 0
+    assert got[1][lone].abs().max() < 1e-4
+
+
 @pytest.mark.parametrize("dtype,length,heads,kv_heads,dim", [
     (torch.bfloat16, 1500, 4, 1, 128), (torch.bfloat16, 1111, 4, 4, 64), (torch.float32, 700, 3, 1, 128)])
 def test_long_records(dtype, length, heads, kv_heads, dim):
