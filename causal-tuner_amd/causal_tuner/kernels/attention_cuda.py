@@ -173,7 +173,7 @@ def _forward(q, k, v, layout, causal, scale, keep_stats):
     fresh = torch.empty if work and layout.whole and layout.tokens == tokens else torch.zeros
     out = fresh((tokens, heads, head_dim), dtype=q.dtype, device=q.device)
     rest = torch.empty_like(out) if keep_stats and q.dtype == torch.bfloat16 else None
-    stats = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if keep_stats else None
+    stats = torch.empty((tokens, heads, 2), dtype=torch.float32, device=q.device) if keep_stats else None
     if work:
         tables = layout.tables(heads, kv_heads, head_dim, q.dtype, causal)
         plan, stream = tables.forward, _native.stream_of(q)
@@ -218,17 +218,17 @@ class _PackedAttention(torch.autograd.Function):
             tables = layout.tables(heads, kv_heads, head_dim, dtype, causal)
             rows, keys, stream = tables.rows, tables.keys, _native.stream_of(q)
             tables.use(stream)
-            # delta, then the partial results of one pass after the other
-            delta = -(-4 * tokens * heads // 256) * 256
+            # the rows' terms, then the partial results of one pass after the other
+            terms = -(-16 * tokens * heads // 256) * 256
             nbytes = max(rows.workspace, keys.workspace)
-            scratch = torch.empty(max(delta + nbytes, 1), dtype=torch.uint8, device=device)
+            scratch = torch.empty(max(terms + nbytes, 1), dtype=torch.uint8, device=device)
             at = scratch.data_ptr()
             dout_token, dout_head, _ = dout.stride()
             with _native.device_of(q):
                 status = _native.library().ct_attention_backward(
                     _operands(q, k, v, tables, causal, scale, rest), rows.entries, rows.counts, keys.entries, keys.counts,
                     out.data_ptr(), stats.data_ptr(), dout.data_ptr(), dout_token, dout_head, at, dq.data_ptr(),
-                    dk.data_ptr(), dv.data_ptr(), at + delta if nbytes else None, nbytes, stream)
+                    dk.data_ptr(), dv.data_ptr(), at + terms if nbytes else None, nbytes, stream)
             _native.check(status, "ct_attention_backward")
         return dq, dk, dv, None, None, None
 

@@ -92,8 +92,8 @@ struct AttnParams {
     char *dst0, *dst1;    // out | dq | dk, dv
     char *rest;           // out's rounding error, as out, or null
     int64_t d_token;      // bytes between tokens of dst0 and dst1
-    float *stats;         // [tokens, heads] lse * log2(e), +inf where a row sees no key
-    float *delta;         // [tokens, heads]
+    float2 *stats;        // [tokens, heads] Running's m and log2 of the sum (+inf where a row sees no key)
+    float4 *terms;        // [tokens, heads] what dq leaves of a row for dk and dv: sstat's three, 1 where far
     float *part0, *part1; // split partials
     int32_t heads, kv_heads, group, head_dim, causal;
     uint32_t magic;       // r / group = (r * magic) >> shift for r < 2^31
@@ -378,11 +378,25 @@ __device__ __forceinline__ void by_stage(int from, int to, F f) {
     }
 }
 
-// Running softmax of a wave's 32 rows over their keys; m2 is the reference exponent of base
-// 2 that p and the sums are relative to.
+// Exponents scale2 (s - m) are one fused multiply-add of s with a rounded scale2 m, or in the
+// backward with scale2 m + log2 of the sum. Past this size of scale2 m the rounding would show:
+// p a factor of up to 2^(2^-24 scale2 m) off in the backward, and from 2^31 on p out of float32's
+// range everywhere. Such rows' scores have m subtracted first, which is exact near m; for all
+// rows that would cost 3% of the forward (632 us instead of 610 at 8192 rows of 32 heads).
+constexpr float kFar = 64.0f;
+
+__device__ __forceinline__ bool is_far(float m, float scale2) { return fabsf(m * scale2) > kFar; }
+
+// Running softmax of a wave's 32 rows over their keys; m is the score that p and the sums are
+// relative to, p = 2^(scale2 (s - m)).
 struct Running {
-    float m2 = -INFINITY, sum = 0.0f, taken = 0.0f;   // taken: the sum of p as rounded for the product
+    float m = -INFINITY, sum = 0.0f, taken = 0.0f;   // taken: the sum of p as rounded for the product
 };
+
+// What the backward needs of a row, apart: their sum would lose the logarithm where m is large.
+__device__ __forceinline__ float2 row_stats(float m, float sum) {
+    return sum == 0.0f ? make_float2(0.0f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(sum));
+}
 
 // ------------------------------------------------------------------ forward
 template <typename T>
@@ -453,14 +467,14 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
                 for (int t = 0; t < KT / 32; ++t)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
-                top = fmaxf(top, other_half(top)) * a.scale2;
+                top = fmaxf(top, other_half(top));
                 // The reference moves only when a row's maximum has grown by more than 2^8: p then
                 // stays below 2^8, o and the sum are exact in that scale, and most tiles skip the
                 // rescaling of o.
-                if (__any(top > run.m2 + 8.0f)) {
-                    const float grown = fmaxf(run.m2, top);
-                    const float shrink = grown == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(run.m2 - grown);
-                    run.m2 = grown;
+                if (__any((top - run.m) * a.scale2 > 8.0f)) {
+                    const float grown = fmaxf(run.m, top);
+                    const float shrink = grown == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((run.m - grown) * a.scale2);
+                    run.m = grown;
                     run.sum *= shrink;
                     run.taken *= shrink;
 #pragma unroll
@@ -468,7 +482,15 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[n][i] *= shrink;
                 }
-                const float ref = run.m2 == -INFINITY ? 0.0f : run.m2;
+                const float m = run.m == -INFINITY ? 0.0f : run.m;
+                float ref = m * a.scale2;
+                if (__any(is_far(m, a.scale2))) {
+                    ref = 0.0f;
+#pragma unroll
+                    for (int t = 0; t < KT / 32; ++t)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[t][i] -= m;
+                }
 #pragma unroll
                 for (int t = 0; t < KT / 32; ++t) {
 #pragma unroll
@@ -509,7 +531,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
                     if (a.rest) store4_rest<T>(a.rest + at, d, x, y, z, w);
                 }
             if (a.stats && lane < 32)
-                a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : run.m2 + __builtin_amdgcn_logf(sum);
+                a.stats[row.token * a.heads + row.head] = row_stats(run.m, sum);
         } else {
             const int64_t at = ((int64_t)item.slot * a.kv_heads + kv_head) * (32 * WAVES) + wave * kWaveCols + (lane & 31);
             float *dst = a.part0 + at * DP;
@@ -520,7 +542,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
                 for (int i = 0; i < 16; i += 4)
                     *reinterpret_cast<float4 *>(dst + 32 * n + 2 * i + d0) =
                         make_float4(o[n][i] * scale, o[n][i + 1] * scale, o[n][i + 2] * scale, o[n][i + 3] * scale);
-            if (lane < 32) *reinterpret_cast<float2 *>(a.part1 + 2 * at) = make_float2(run.m2, sum);
+            if (lane < 32) *reinterpret_cast<float2 *>(a.part1 + 2 * at) = make_float2(run.m, sum);
         }
     }
 }
@@ -556,7 +578,7 @@ __global__ __launch_bounds__(kThreads) void attention_join(AttnParams a, const I
         const int64_t at = first + s * step;
         const float2 ms = *reinterpret_cast<const float2 *>(a.part1 + 2 * at);
         const float4 x = *reinterpret_cast<const float4 *>(a.part0 + at * DP + 4 * lane);
-        const float w = __builtin_amdgcn_exp2f(ms.x - ref);
+        const float w = __builtin_amdgcn_exp2f((ms.x - ref) * a.scale2);
         sum = __builtin_fmaf(w, ms.y, sum);
         acc.x = __builtin_fmaf(w, x.x, acc.x);
         acc.y = __builtin_fmaf(w, x.y, acc.y);
@@ -588,7 +610,7 @@ __global__ __launch_bounds__(kThreads) void attention_join(AttnParams a, const I
         if (a.rest) store4_rest<T>(a.rest + at, 4 * lane, acc.x, acc.y, acc.z, acc.w);
     }
     if (a.stats && lane == 0)
-        a.stats[row.token * a.heads + row.head] = sum == 0.0f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+        a.stats[row.token * a.heads + row.head] = row_stats(top, sum);
 }
 
 // Sum of the parts of one row or key, in order, for four elements.
@@ -606,7 +628,7 @@ __device__ __forceinline__ float4 sum_parts(const float *part, int64_t at, int64
     return v;
 }
 
-// ------------------------------------------------------------------ dq (and delta)
+// ------------------------------------------------------------------ dq (and the rows' terms)
 template <typename T>
 __device__ __forceinline__ float dot_chunk(const uint4 &x, const uint4 &y, float acc) {
     const uint32_t p[4] = {x.x, x.y, x.z, x.w}, q[4] = {y.x, y.y, y.z, y.w};
@@ -650,12 +672,20 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
             for (int s = 0; s < Tile<T, DP>::kFrags; ++s) delta = dot_chunk<T>(gf[s], qf[s], delta);
         }
         delta += other_half(delta);
-        float lse = INFINITY;
+        float m = 0.0f, lse = INFINITY;
         if (row.valid) {
             const int64_t at = row.token * a.heads + row.head;
-            lse = a.stats[at];
-            if (lane < 32 && item.lo == 0) a.delta[at] = delta;
+            const float2 stats = a.stats[at];
+            m = stats.x;
+            lse = stats.y;
         }
+        if (row.valid && lane < 32 && item.lo == 0) {
+            const bool far = is_far(m, a.scale2);
+            a.terms[row.token * a.heads + row.head] =
+                make_float4(far ? m : 0.0f, far ? -lse : -__builtin_fmaf(m, a.scale2, lse), -delta, far ? 1.0f : 0.0f);
+        }
+        const bool far = __any(is_far(m, a.scale2));
+        if (!far) lse = __builtin_fmaf(m, a.scale2, lse);
         row_fragments<T, DP>(a.q + row.token * a.q_token + row.head * a.q_head, qf, row.valid, chunks, lane);
 
         const char *k0 = a.k + rec.k_start * a.k_token + kv_head * a.k_head;
@@ -703,6 +733,11 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
             }
             if (key < most) {
                 at.refresh();
+                if (far) {
+                    const float m = row.valid ? a.stats[row.token * a.heads + row.head].x : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] -= m;
+                }
                 f32x16 ds;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
@@ -770,7 +805,8 @@ template <typename T, int DP>
 __global__ __launch_bounds__(64 * kKeyWaves, sizeof(T) == 2 && DP == 64 ? 4 : 2) void attention_dkv(AttnParams a) {
     constexpr int kUnits = kStep * Tile<T, DP>::kChunks, kAll = 64 * kKeyWaves;
     __shared__ uint4 st[2][kStages][kUnits];                     // q, dout
-    __shared__ __align__(16) float sstat[2][kStages][kStep];   // -lse, -delta
+    __shared__ __align__(16) float sstat[3][kStages][kStep];   // m of far rows, -lse (far: -log2 sum), -delta
+    __shared__ int sfar[kStages];                               // whether any row is far
     __shared__ __align__(16) float szero[kStep];
     __shared__ f32x4 sp[2][kKeyWaves / 2][4][64];
     const Group group = a.groups[blockIdx.x / a.kv_heads];
@@ -798,7 +834,7 @@ __global__ __launch_bounds__(64 * kKeyWaves, sizeof(T) == 2 && DP == 64 ? 4 : 2)
         const int64_t mine = first(key), wave_first = first(key0), wave_last = first(key0 + kWaveCols - 1);
 
         Stage<T, DP, kStep, kAll> qs, gs;
-        float stat_r = 0.0f;
+        float4 stat_r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         // A group that divides the step makes a row's token and head the same in every step; the
         // others are divided out each time.
         const bool regular = kStep % a.group == 0;
@@ -835,15 +871,22 @@ __global__ __launch_bounds__(64 * kKeyWaves, sizeof(T) == 2 && DP == 64 ? 4 : 2)
                     exists);
             gs.load(a.dout + token * a.do_token + (int64_t)kv_head * a.group * a.do_head, chunks,
                     [&](int p) { return at[p].g; }, exists);
-            if (wave == 0) {   // lanes 0 - 31 the statistics, 32 - 63 delta; rows behind the last: p = 0
-                const float *from = (lane < kStep ? a.stats : a.delta) + token * a.heads + kv_head * a.group;
-                stat_r = stat_row < left ? from[stat] : lane < kStep ? INFINITY : 0.0f;
-            }
+            if (wave == kKeyWaves / 2 && lane < kStep)   // rows behind the last: p = 0
+                stat_r = stat_row < left ? a.terms[token * a.heads + kv_head * a.group + stat]
+                                         : make_float4(0.0f, -INFINITY, 0.0f, 0.0f);
         };
         auto store = [&](int buf) {
             qs.store(st[0][buf]);
             gs.store(st[1][buf]);
-            if (wave == 0) sstat[lane < kStep ? 0 : 1][buf][stat_row] = -stat_r;
+            if (wave == kKeyWaves / 2) {
+                const bool any = __any(stat_r.w != 0.0f);
+                if (lane < kStep) {
+                    sstat[0][buf][lane] = stat_r.x;
+                    sstat[1][buf][lane] = stat_r.y;
+                    sstat[2][buf][lane] = stat_r.z;
+                }
+                if (lane == 0) sfar[buf] = any;
+            }
         };
 
         f32x16 acc[DP / 32], s = splat(0.0f);
@@ -854,7 +897,7 @@ __global__ __launch_bounds__(64 * kKeyWaves, sizeof(T) == 2 && DP == 64 ? 4 : 2)
         constexpr uint32_t kOther = sizeof(st[0]), kStage = sizeof(st[0][0]), kStat = sizeof(sstat[0][0]);
         Lanes<T, DP> at(lane);
         at.shift(for_dv ? 0 : kOther, for_dv ? kOther : 0);
-        const uint32_t start = 16 * (lane >> 5) + (for_dv ? lds_of(szero) : lds_of(sstat) + kStages * kStat);
+        const uint32_t start = 16 * (lane >> 5) + (for_dv ? lds_of(szero) : lds_of(sstat) + 2 * kStages * kStat);
         const uint32_t start_step = for_dv ? 0 : kStat, own_stat = lds_of(sstat) + 16 * (lane >> 5);
         if (threadIdx.x < kStep) szero[threadIdx.x] = 0.0f;
         // Probabilities (for dv, shared) or do . v - delta of the rows at r0 in stage `buf`.
@@ -867,9 +910,17 @@ __global__ __launch_bounds__(64 * kKeyWaves, sizeof(T) == 2 && DP == 64 ? 4 : 2)
             }
             scores<T, DP>(s, lds_of(st) + buf * kStage, 0, frag, at);
             if (for_dv) {
+                if (__builtin_amdgcn_readfirstlane(sfar[buf])) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const f32x4 m = __builtin_bit_cast(f32x4, lds_read16(own_stat + buf * kStat + 32 * i));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[4 * i + e] -= m[e];
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const f32x4 v = __builtin_bit_cast(f32x4, lds_read16(own_stat + buf * kStat + 32 * i));
+                    const f32x4 v = __builtin_bit_cast(f32x4, lds_read16(own_stat + (kStages + buf) * kStat + 32 * i));
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         s[4 * i + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + e], a.scale2, v[e]));
@@ -1252,13 +1303,14 @@ extern "C" int ct_attention_forward(const ct_attention *c, const int32_t *plan, 
     const int64_t joins = counts[1], slots = counts[2], groups = counts[3];
     if (groups == 0) return 0;
     if (!plan || !out || (uintptr_t)plan % 16 || (uintptr_t)out % 16) return -CT_EINVAL_POINTER;
+    if ((uintptr_t)stats % 8) return -CT_EINVAL_POINTER;
     if (slots && (!workspace || (uintptr_t)workspace % 16 ||
                   workspace_bytes < ct_attention_workspace(CT_ATTENTION_FORWARD, slots, c->kv_heads, c->head_dim)))
         return -CT_EINVAL_WORKSPACE;
     const int dp = padded_dim(c->head_dim);
     set_plan(a, plan, counts);
     a.dst0 = (char *)out;
-    a.stats = stats;
+    a.stats = (float2 *)stats;
     a.part0 = (float *)workspace;
     a.part1 = a.part0 + slots * c->kv_heads * kRowTile * dp;
     return by_type(c->dtype, dp, [&](auto type, auto dim) {
@@ -1277,7 +1329,7 @@ extern "C" int ct_attention_forward(const ct_attention *c, const int32_t *plan, 
 extern "C" int ct_attention_backward(const ct_attention *c, const int32_t *row_plan, const int64_t *row_counts,
                                      const int32_t *key_plan, const int64_t *key_counts, const void *out,
                                      const float *stats, const void *dout, int64_t dout_token, int64_t dout_head,
-                                     float *delta, void *dq, void *dk, void *dv, void *workspace,
+                                     float *terms, void *dq, void *dk, void *dv, void *workspace,
                                      int64_t workspace_bytes, hipStream_t stream) {
     AttnParams a;
     if (const int status = fill_params(c, a)) return status;
@@ -1286,8 +1338,9 @@ extern "C" int ct_attention_backward(const ct_attention *c, const int32_t *row_p
     const int64_t rows = row_counts[3], keys = key_counts[3], row_slots = row_counts[2], key_slots = key_counts[2];
     const int64_t size = c->dtype == CT_BF16 ? 2 : 4;
     if (rows) {
-        if (!row_plan || !out || !stats || !dout || !delta || !dq ||
-            ((uintptr_t)row_plan | (uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq) % 16)
+        if (!row_plan || !out || !stats || !dout || !terms || !dq ||
+            ((uintptr_t)row_plan | (uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)terms) % 16 ||
+            (uintptr_t)stats % 8)
             return -CT_EINVAL_POINTER;
         if (dout_token < 0 || dout_head < 0 || dout_token * size % 16 || dout_head * size % 16 ||
             dout_token > (int64_t)1 << 40 || dout_head > (int64_t)1 << 40)
@@ -1305,14 +1358,14 @@ extern "C" int ct_attention_backward(const ct_attention *c, const int32_t *row_p
     a.dout = (const char *)dout;
     a.do_token = dout_token * size;
     a.do_head = dout_head * size;
-    a.stats = const_cast<float *>(stats);
-    a.delta = delta;
+    a.stats = (float2 *)const_cast<float *>(stats);
+    a.terms = (float4 *)terms;
     return by_type(c->dtype, dp, [&](auto type, auto dim) {
         typedef decltype(type) T;
         constexpr int DP = decltype(dim)::value;
         AttnParams r = a;
         r.part0 = (float *)workspace;
-        if (rows) {   // dq first: it leaves delta for the other kernel
+        if (rows) {   // dq first: it leaves the rows' terms for the other kernel
             set_plan(r, row_plan, row_counts);
             r.dst0 = (char *)dq;
             r.d_token = a.o_token;

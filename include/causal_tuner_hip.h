@@ -568,8 +568,9 @@ int ct_attention_plan(int32_t pass, const int64_t *records, int64_t n_records, i
 int64_t ct_attention_workspace(int32_t pass, int64_t slots, int32_t kv_heads, int32_t head_dim);
 
 /*
- * out [tokens, heads, head_dim] contiguous; stats float32 [tokens, heads] for the backward (null:
- * none): log2 of the softmax's denominator with its maximum (+inf for a query that sees no key).
+ * out [tokens, heads, head_dim] contiguous; stats float32 [tokens, heads, 2], 8-byte aligned, for
+ * the backward (null: none): the score q . k that the row's probabilities are relative to, and log2
+ * of their sum (0 and +inf for a query that sees no key).
  * Rows of no record are left as they are.
  */
 int ct_attention_forward(const ct_attention *attention, const int32_t *plan, const int64_t *counts, void *out,
@@ -577,14 +578,14 @@ int ct_attention_forward(const ct_attention *attention, const int32_t *plan, con
 
 /*
  * dq [tokens, heads, head_dim], dk and dv [key tokens, kv_heads, head_dim], contiguous, from
- * dout (strides as for q), the forward's out and stats; delta float32 [tokens, heads] is
- * scratch. The probabilities are recomputed; sums run in a fixed order, so repeated calls are
+ * dout (strides as for q), the forward's out and stats; terms float32 [tokens, heads, 4], 16-byte
+ * aligned, is scratch. The probabilities are recomputed; sums run in a fixed order, so repeated calls are
  * bit-identical. Rows of no record are left as they are. row_plan and key_plan are the plans
  * of CT_ATTENTION_ROWS and CT_ATTENTION_KEYS.
  */
 int ct_attention_backward(const ct_attention *attention, const int32_t *row_plan, const int64_t *row_counts,
                           const int32_t *key_plan, const int64_t *key_counts, const void *out, const float *stats,
-                          const void *dout, int64_t dout_token, int64_t dout_head, float *delta, void *dq, void *dk,
+                          const void *dout, int64_t dout_token, int64_t dout_head, float *terms, void *dq, void *dk,
                           void *dv, void *workspace, int64_t workspace_bytes, hipStream_t stream);
 
 /*

@@ -302,3 +302,36 @@ def test_device_refusals():
         packed_attention(make(2, 64), make(1, 64), make(1, 64), AttentionLayout([(0, 4)], "cpu"))
     with pytest.raises(ValueError, match="different devices"):
         packed_attention(make(2, 64), make(1, 64).cpu(), make(1, 64), layout)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("sizes,key_sizes", [([200], [200]), ([1, 3], [700, 900])])
+@pytest.mark.parametrize("exponent", [14, 16, 24, 34, 100])
+def test_scores_of_any_size(exponent, sizes, key_sizes, dtype):
+    """Scores s = +-2^exponent k / 8 of whole k, so that each row's softmax is 1 at its largest
+    score or 1/2 at two equal ones and 0 elsewhere: a float32 sum of m and log2 of the
+    denominator would lose the latter from scores of 2^16 on. v and dout are -1, 0 or 1, so all
+    sums and ds = (dp_1 - dp_2) / 4 are exact; what is left is the results' rounding and the last
+    places of the exponential and the logarithm."""
+    from causal_tuner.kernels.attention_cuda import AttentionLayout
+    tokens, key_tokens, heads, dim = sum(sizes), sum(key_sizes), 4, 64
+    records, keys = records_of(sizes), records_of(key_sizes)
+    g = torch.Generator().manual_seed(exponent)
+    if len(sizes) == 1:
+        number = torch.arange(key_tokens) // 2 + 1
+    else:
+        number = torch.randint(1, 100, (key_tokens,), generator=g)
+        for start, _ in keys:
+            number[[start + 5, start + 420]], number[[start + 7, start + 555]] = 200, 0
+    q = torch.zeros(tokens, heads, dim)
+    q[:, :, 0] = 2.0 ** exponent * torch.tensor([1.0, -1.0, 1.0, -1.0])
+    k = torch.zeros(key_tokens, 1, dim)
+    k[:, 0, 0] = number
+    v, dout = (torch.randint(-1, 2, s, generator=g).float() for s in ((key_tokens, 1, dim), (tokens, heads, dim)))
+    leaves = [t.to("cuda", dtype).requires_grad_(True) for t in (q, k, v)]
+    got = _run(*leaves, dout.to("cuda", dtype), AttentionLayout(records, "cuda", key_records=keys))
+    want, _ = reference(*leaves, records, keys, True, 0.125, dout.cuda())
+    assert not want[1].any() and want[2].any()
+    u = torch.finfo(dtype).eps / 2
+    for name, x, y in zip(("out", "dq", "dk", "dv"), got, want):
+        assert ((x.double() - y).abs() <= (u + 8 * 2.0 ** -24) * y.abs()).all(), name
