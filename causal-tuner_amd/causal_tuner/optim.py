@@ -199,7 +199,11 @@ def orthogonalize(matrices, *, coefficients=(3.4445, -4.7750, 2.0315), steps=5, 
 
     `matrices` is a 2-D tensor or a list of them, float32 or bfloat16 on the device (any
     shapes and strides, types and devices mixed); returns new contiguous tensors of the same
-    shapes and types, one or a list. Empty matrices come back empty, zero ones zero."""
+    shapes and types, one or a list. Empty matrices come back empty, zero ones zero.
+
+    A direction that M does not have grows from rounding noise by a per step, as in any iteration
+    in 32 bits: matrices of low rank are 2e-5 off after 5 steps of the default coefficients, 1e-2
+    after 10 and about 0.1 however many follow; those of full rank stay within 2e-7."""
     coefficients, steps, eps = _muon_numbers(coefficients, steps, eps)
     single = isinstance(matrices, torch.Tensor)
     inputs = [matrices] if single else list(matrices)

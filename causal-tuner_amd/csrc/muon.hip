@@ -16,6 +16,16 @@
 // on a fifth of the work); only the last product, of the final P_{n-1} ... P_0 and M, is float32.
 // Keeping P_{n-1} ... P_0 in float32 too would lose a factor of three in those cases.
 //
+// Every G is positive semidefinite, and G <- P G P keeps it so, but roundings of 1e-16 make the
+// zero eigenvalues of a matrix of low rank negative. A step multiplies those by (a + b l + c l^2)^2,
+// which grows with |l| where it falls for the positive ones: from 14 steps on (a^28 = 1e15) they
+// ran away, at 20 the result was NaN. So each G gets gram_floor(r) = 2^-50 r on its diagonal, more
+// than its roundings (2^-53 sqrt(r) times 40 at most: |P|^2 < 12, |G| < 1.5, two products) and less
+// than shows: after 5 steps 1e-8 of what small singular values become. With it the result's error
+// for a matrix of low rank is that of float32 steps on the whole matrix, since Q grows by a = 3.4 a
+// step where M has nothing and its own rounding (2^-24) reaches M's rows: 2e-5 after 5 steps, 1e-2
+// after 10, and a tenth from 14 on, where the floor ends Q's growth (float32 steps: 1 and more).
+//
 // What bounds it, two layers' adapters of rank 256 (36M elements, 754 us a step): the Gram
 // pass 229 us (double matrix instructions, 73% of its cycles at a clock that they pull down to
 // about 1.9 GHz; 12 bytes an element), the 14 launches of r x r products 24 us each (their
@@ -91,6 +101,9 @@ __host__ __device__ __forceinline__ int64_t least(int64_t x, int64_t y) { return
 __device__ __forceinline__ int short_side(const Matrix &m) { return (int)least(m.rows, m.cols); }
 __host__ __device__ __forceinline__ int padded(int r) { return (r + kPad - 1) / kPad * kPad; }
 __host__ __device__ __forceinline__ int tiles16(int r) { return (r + 15) / 16; }
+
+// What every G has on its diagonal on top.
+__device__ __forceinline__ double gram_floor(int r) { return padded(r) * 0x1p-50; }
 
 // A partial Gram matrix: the squared norms of its part of M (one, or one per 64 rows), then
 // the 16 x 16 tiles (i, j), i >= j, row by row.
@@ -539,7 +552,8 @@ __global__ __launch_bounds__(kThreads) void muon_join(const Matrix *matrices, co
         g[i * rp + j] = g[j * rp + i] = 0.0;
         return;
     }
-    const double v = join_tile(m, ws, it.i, it.j, threadIdx.x) * (inv * inv);
+    double v = join_tile(m, ws, it.i, it.j, threadIdx.x) * (inv * inv);
+    if (i == j && i < short_side(m)) v += gram_floor(short_side(m));
     if (i >= j) g[i * rp + j] = g[j * rp + i] = v;
 }
 
@@ -576,13 +590,14 @@ __global__ __launch_bounds__(kSmallThreads) void muon_small(const Matrix *matric
         for (int x = 0; x < kMost; ++x) {
             const int t = (x * kSmallThreads + tid) >> 8, i = tile_row(t), j = t - i * (i + 1) / 2;
             const int row = i * 16 + ((tid & 255) >> 4), col = j * 16 + (tid & 15);
-            if (t < count && row >= col) sg[at(row, col)] = sg[at(col, row)] = v[x] * (inv * inv);
+            if (t < count && row >= col)
+                sg[at(row, col)] = sg[at(col, row)] = v[x] * (inv * inv) + (row == col && row < r ? gram_floor(r) : 0.0);
         }
     }
     __syncthreads();
 
-    // dst = left right, or a I + b left + c left right; dst may be an operand.
-    auto product = [&](const double *left, const double *right, double *dst, bool polynomial) {
+    // dst = left right + diagonal I, or a I + b left + c left right; dst may be an operand.
+    auto product = [&](const double *left, const double *right, double *dst, bool polynomial, double diagonal = 0.0) {
         f64x4 result[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -605,12 +620,11 @@ __global__ __launch_bounds__(kSmallThreads) void muon_small(const Matrix *matric
                     odd = mfma_f64(p[u + 1], q[u + 1], odd);
                 }
             result[x] = even + odd;
-            if (polynomial) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int row = 16 * i + 4 * e + (lane >> 4), col = 16 * j + (lane & 15);
-                    result[x][e] = h.c * result[x][e] + h.b * left[at(row, col)] + (row == col && row < r ? h.a : 0.0);
-                }
+            for (int e = 0; e < 4; ++e) {
+                const int row = 16 * i + 4 * e + (lane >> 4), col = 16 * j + (lane & 15);
+                if (polynomial) result[x][e] = h.c * result[x][e] + h.b * left[at(row, col)];
+                if (row == col && row < r) result[x][e] += polynomial ? h.a : diagonal;
             }
         }
         __syncthreads();
@@ -632,7 +646,7 @@ __global__ __launch_bounds__(kSmallThreads) void muon_small(const Matrix *matric
         product(sg, sg, p, true);
         if (i + 1 < steps) product(p, sg, st, false);
         if (i) product(p, sq, sq, false);
-        if (i + 1 < steps) product(p, st, sg, false);
+        if (i + 1 < steps) product(p, st, sg, false, gram_floor(r));
     }
     const int rp = padded(r);
     float *final = final_q(m, ws);
@@ -718,6 +732,8 @@ __global__ __launch_bounds__(kStageThreads) void muon_stage(const Matrix *matric
             const int i = it.i * kPad + row, j = it.j * kPad + col;
             v = h.c * v + h.b * g[(int64_t)i * rp + j];
             if (i == j && i < r) v += h.a;
+        } else if (op.dst == kG && it.i == it.j && row == col && it.i * kPad + row < r) {
+            v += gram_floor(r);
         }
         return v;
     };

@@ -598,7 +598,9 @@ int ct_attention_backward(const ct_attention *attention, const int32_t *row_plan
  *   grad : momentum, param = param (1 - lr weight_decay) - lr adjust X_steps.
  * param and grad are [rows, cols] contiguous of `dtype` (CT_F32 or CT_BF16), momentum float32.
  * The iteration runs in double on the short side's Gram matrix, the last product in float32;
- * results are rounded once. Sums run in a fixed order.
+ * results are rounded once. Sums run in a fixed order. The Gram matrix has 2^-50 times its
+ * (padded) size on its diagonal in every step, which keeps its roundings from making it indefinite:
+ * any number of steps stays bounded for matrices of any rank.
  */
 #define CT_MUON_KINDS 7
 

@@ -250,3 +250,66 @@ def test_device_refusals():
     optimizer.state[p]["momentum_buffer"] = torch.zeros(6, 4, device="cuda", dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="momentum_buffer"):
         optimizer.step()
+
+
+def _low_rank(shape, rank, dtype, seed=0):
+    """(matrix of whole numbers, exact in `dtype`; its factors in float64)."""
+    g = torch.Generator().manual_seed(seed)
+    left, right = (torch.randint(-2, 3, s, generator=g).double() for s in ((shape[0], rank), (rank, shape[1])))
+    return (left @ right).to("cuda", dtype), left.cuda(), right.cuda()
+
+
+def _low_rank_reference(left, right, steps, coefficients):
+    """The iteration in the factors' small core, where no direction is empty: (X, Q, X_0)."""
+    a, b, c = coefficients
+    u, x = torch.linalg.qr(left)
+    v, y = torch.linalg.qr(right.T)
+    x = x @ y.T
+    x = x0 = x / x.norm()
+    eye = torch.eye(len(x), dtype=x.dtype, device=x.device)
+    q = eye
+    for _ in range(steps):
+        g = x @ x.T
+        p = a * eye + b * g + c * (g @ g)
+        x, q = p @ x, p @ q
+    whole = torch.eye(len(u), dtype=x.dtype, device=x.device)
+    return u @ x @ v.T, a ** steps * (whole - u @ u.T) + u @ q @ u.T, u @ x0 @ v.T
+
+
+@pytest.mark.parametrize("steps,coefficients", [(5, (A, B, C)), (10, (A, B, C)), (20, (A, B, C)), (100, (A, B, C)),
+                                                (20, (1.5, -0.5, 0.0)), (100, (1.5, -0.5, 0.0))])
+@pytest.mark.parametrize("shape,rank", [((7, 60), 1), ((16, 300), 2), ((500, 64), 8), ((200, 700), 8), ((700, 130), 3),
+                                        ((300, 520), 4)])
+def test_matrices_of_low_rank(shape, rank, steps, coefficients):
+    """Directions that M does not have stay small for as many steps as are accepted. Q grows by a
+    a step there, and each of its entries and each of the product's r sums is rounded in float32:
+    the elementwise bound of this file's head, until a^steps reaches 2^20. From there on Q's norm is
+    at most q = 2 / sqrt(2^-50 r) (a direction's value, at most 1.3, over the floor's root), and the
+    error in norm e q (1 + sqrt(rank) + sqrt(r)): Q is q off the identity of the empty directions by
+    its rounding e, by e sqrt(rank) off its part in the others, and r terms are added."""
+    from causal_tuner.optim import orthogonalize
+    m, left, right = _low_rank(shape, rank, torch.float32)
+    got = orthogonalize(m, steps=steps, coefficients=coefficients)
+    assert torch.isfinite(got).all()
+    if shape[0] > shape[1]:
+        got, left, right = got.T, right.T, left.T
+    want, q, x0 = _low_rank_reference(left, right, steps, coefficients)
+    r = min(shape)
+    if coefficients[0] ** steps <= 2.0 ** 20:
+        bound = 2 * (r + 4) * E32 * (q.abs() @ x0.abs())
+        assert ((got.double() - want).abs() <= bound + E32 * want.abs()).all()
+    else:
+        most = 2 / (2.0 ** -50 * (-(-r // 32) * 32)) ** 0.5
+        assert (got.double() - want).norm() <= E32 * most * (1 + rank ** 0.5 + r ** 0.5)
+
+
+def test_muon_steps_of_low_rank_stay_finite():
+    from causal_tuner.optim import FusedMuon
+    shapes = [(64, 500), (200, 700), (16, 30)]
+    params = [torch.nn.Parameter(_matrix(s, torch.bfloat16, seed=i) * 20) for i, s in enumerate(shapes)]
+    before = [p.detach().clone() for p in params]
+    for p, s in zip(params, shapes):
+        p.grad = _low_rank(s, 2, torch.bfloat16)[0]
+    FusedMuon(params, lr=0.02, weight_decay=0.0, ns_steps=100).step()
+    for p, old in zip(params, before):
+        assert torch.isfinite(p).all() and (p - old).norm() <= 0.02 * 3 * len(p) ** 0.5
