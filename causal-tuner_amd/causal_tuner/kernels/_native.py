@@ -11,6 +11,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 DEFAULT_LIBRARY = os.path.normpath(os.path.join(_HERE, "..", "..", "lib", "libcausal_tuner_hip.so"))
@@ -225,6 +226,13 @@ def device_of(tensor):
 
 def ptr(tensor):
     return None if tensor is None else tensor.data_ptr()
+
+
+def refuse_tangents(name, *tensors):
+    """Raises where a tensor carries a forward-mode derivative: a kernel that is called outside
+    an autograd Function would drop it without a word."""
+    if any(unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name}: the HIP kernels have no forward-mode derivative")
 
 
 def dtype_code(dtype):

@@ -203,6 +203,7 @@ class _PackedAttention(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, out, rest, stats = ctx.saved_tensors
         layout, causal, scale = ctx.layout, ctx.causal, ctx.scale
+        _native.refuse_tangents("packed_attention", dout)
         if not layout.keys_disjoint:
             raise RuntimeError("packed_attention: key_records that overlap have no backward")
         tokens, heads, head_dim = q.shape
@@ -259,7 +260,8 @@ def packed_attention(q, k, v, records, *, causal=True, scale=None):
     dtype, H a multiple of H_kv, D a multiple of 8 up to 128, bf16 or float32 on the device, any
     strides (other than those of whole 16-byte pieces are copied first). `records` is an
     `AttentionLayout` or, for a single call, a list of (start, stop) spans. `scale` defaults to
-    D ** -0.5. Returns a tensor of q's shape, differentiable in q, k and v."""
+    D ** -0.5. Returns a tensor of q's shape, differentiable in q, k and v
+    (once, in reverse; host tensors in every way that torch offers)."""
     if q.dim() == 4 and q.shape[0] == 1 and k.dim() == 4 and k.shape[0] == 1 and v.dim() == 4 and v.shape[0] == 1:
         return packed_attention(q[0], k[0], v[0], records, causal=causal, scale=scale)[None]
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
@@ -294,6 +296,7 @@ def packed_attention(q, k, v, records, *, causal=True, scale=None):
         raise NotImplementedError("packed_attention: the HIP kernels take bfloat16 or float32")
     if head_dim % 8 or head_dim > 128:
         raise ValueError(f"packed_attention: head_dim {head_dim} is not a multiple of 8 up to 128")
+    _native.refuse_tangents("packed_attention", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _PackedAttention.apply(q, k, v, layout, causal, scale)
     return _forward(q, k, v, layout, causal, scale, False)[3]

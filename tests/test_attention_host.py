@@ -156,3 +156,14 @@ def test_abi_refusals():
     assert lib.ct_attention_forward(ctypes.byref(_native.Attention(**good)), 256, counts, 256, None, None, 0, None) == -5
     counts[0] = -1
     assert forward() == -2
+
+
+def test_host_tangents():
+    """Host tensors carry forward-mode derivatives: against differences."""
+    from torch.autograd import forward_ad
+    q, k, v = (torch.randn(6, h, 4, dtype=torch.float64) for h in (4, 2, 2))
+    along, h = torch.randn_like(k), 1e-6
+    with forward_ad.dual_level():
+        tangent = forward_ad.unpack_dual(packed_attention(q, forward_ad.make_dual(k, along), v, [(0, 6)])).tangent
+    up, down = (packed_attention(q, k + s * h * along, v, [(0, 6)]) for s in (1, -1))
+    torch.testing.assert_close(tangent, (up - down) / (2 * h), rtol=1e-6, atol=1e-8)

@@ -335,3 +335,26 @@ def test_scores_of_any_size(exponent, sizes, key_sizes, dtype):
     u = torch.finfo(dtype).eps / 2
     for name, x, y in zip(("out", "dq", "dk", "dv"), got, want):
         assert ((x.double() - y).abs() <= (u + 8 * 2.0 ** -24) * y.abs()).all(), name
+
+
+def test_forward_mode_derivatives_are_refused():
+    """Not dropped: with and without a gradient asked for, and of the upstream gradient."""
+    from torch.autograd import forward_ad
+    from causal_tuner.kernels.attention_cuda import AttentionLayout, packed_attention
+    q, k, v, dout = _tensors(20, 20, 2, 1, 64, torch.float32, grad=False)
+    layout = AttentionLayout([(0, 20)], "cuda")
+    want = packed_attention(q, k, v, layout)
+    with forward_ad.dual_level():
+        for i in range(3):
+            operands = [q, k, v]
+            operands[i] = forward_ad.make_dual(operands[i], torch.ones_like(operands[i]))
+            for mode in (torch.no_grad, torch.enable_grad):
+                with mode(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    packed_attention(*operands, layout)
+        assert torch.equal(packed_attention(q, k, v, layout), want)
+        leaf = q.clone().requires_grad_(True)
+        out = packed_attention(leaf, k, v, layout)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(out, leaf, forward_ad.make_dual(dout, dout))
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda t: packed_attention(t, k, v, layout), (q,), (q,))
