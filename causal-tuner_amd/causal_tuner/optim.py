@@ -199,7 +199,8 @@ def orthogonalize(matrices, *, coefficients=(3.4445, -4.7750, 2.0315), steps=5, 
 
     `matrices` is a 2-D tensor or a list of them, float32 or bfloat16 on the device (any
     shapes and strides, types and devices mixed); returns new contiguous tensors of the same
-    shapes and types, one or a list. Empty matrices come back empty, zero ones zero.
+    shapes and types, one or a list, that carry no gradient. Empty matrices come back empty, zero
+    ones zero (where eps is not zero).
 
     A direction that M does not have grows from rounding noise by a per step, as in any iteration
     in 32 bits: matrices of low rank are 2e-5 off after 5 steps of the default coefficients, 1e-2
@@ -218,6 +219,7 @@ def orthogonalize(matrices, *, coefficients=(3.4445, -4.7750, 2.0315), steps=5, 
         if not m.is_cuda:
             results.append(_newton_schulz(m, coefficients, steps, eps) if m.numel() else m.clone())
             continue
+        _native.refuse_tangents("orthogonalize", m)
         results.append(torch.empty(m.shape, dtype=m.dtype, device=m.device))
         if m.numel():
             buckets.setdefault((m.device, m.dtype), []).append(index)

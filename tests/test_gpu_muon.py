@@ -313,3 +313,18 @@ def test_muon_steps_of_low_rank_stay_finite():
     FusedMuon(params, lr=0.02, weight_decay=0.0, ns_steps=100).step()
     for p, old in zip(params, before):
         assert torch.isfinite(p).all() and (p - old).norm() <= 0.02 * 3 * len(p) ** 0.5
+
+
+def test_forward_mode_derivatives_are_refused():
+    """Not dropped: host matrices carry them."""
+    from torch.autograd import forward_ad
+    from causal_tuner.optim import orthogonalize
+    m = _matrix((20, 30), torch.float32)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(m, torch.ones_like(m))
+        for given in (dual, [m, dual]):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                orthogonalize(given)
+        host = orthogonalize(forward_ad.make_dual(m.cpu(), torch.ones(20, 30)))
+        assert forward_ad.unpack_dual(host).tangent.any()
+    _check(orthogonalize(m), m)
