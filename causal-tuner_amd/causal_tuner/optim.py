@@ -249,24 +249,33 @@ class FusedMuon(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True,
                  ns_coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, ns_steps=5, adjust_lr_fn=None):
-        if not 0.0 <= float(lr):
-            raise ValueError(f"Invalid learning rate: {lr}")
-        if not 0.0 <= momentum <= 1.0:
-            raise ValueError(f"Invalid momentum value: {momentum}")
-        if not 0.0 <= weight_decay:
-            raise ValueError(f"Invalid weight_decay value: {weight_decay}")
-        if adjust_lr_fn not in (None, "original", "match_rms_adamw"):
-            raise ValueError(f"Invalid learning rate adjustment: {adjust_lr_fn}")
-        _muon_numbers(ns_coefficients, ns_steps, eps)
         super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
                                       ns_coefficients=ns_coefficients, eps=eps, ns_steps=ns_steps,
                                       adjust_lr_fn=adjust_lr_fn))
 
-    def add_param_group(self, param_group):
-        super().add_param_group(param_group)
-        for p in self.param_groups[-1]["params"]:
+    @staticmethod
+    def _check_group(group):
+        if not 0.0 <= float(group["lr"]):
+            raise ValueError(f"Invalid learning rate: {group['lr']}")
+        if not 0.0 <= group["momentum"] <= 1.0:
+            raise ValueError(f"Invalid momentum value: {group['momentum']}")
+        if not 0.0 <= group["weight_decay"]:
+            raise ValueError(f"Invalid weight_decay value: {group['weight_decay']}")
+        if group["adjust_lr_fn"] not in (None, "original", "match_rms_adamw"):
+            raise ValueError(f"Invalid learning rate adjustment: {group['adjust_lr_fn']}")
+        _muon_numbers(group["ns_coefficients"], group["ns_steps"], group["eps"])
+        for p in group["params"]:
             if p.dim() != 2:
                 raise ValueError(f"FusedMuon takes matrices only, not a parameter of shape {tuple(p.shape)}")
+
+    def add_param_group(self, param_group):
+        """Adds a group, or raises and leaves the optimizer as it was."""
+        super().add_param_group(param_group)
+        try:
+            self._check_group(self.param_groups[-1])
+        except Exception:
+            self.param_groups.pop()
+            raise
 
     def load_state_dict(self, state_dict):
         """Loads a state dict (this class's or torch.optim.Muon's); the buffers stay float32,

@@ -123,3 +123,21 @@ def test_abi_refusals():
     assert call(ws=None) == -5 and call(n=8) == -5
     assert call(o=_native.MuonOptions(steps=0)) == -2 and call(o=_native.MuonOptions(steps=101)) == -2
     assert call(o=_native.MuonOptions(steps=5, update=1)) == -1   # no momentum
+
+
+def test_groups_of_their_own_are_checked_and_refused_ones_left_out():
+    make = lambda *s: torch.nn.Parameter(torch.zeros(*s))  # noqa: E731
+    first = make(3, 4)
+    optimizer = FusedMuon([first], lr=0.1)
+    for group in ({"params": [make(3, 4), make(3)]}, {"params": [make(3, 4)], "lr": -1.0},
+                  {"params": [make(3, 4)], "momentum": 2.0}, {"params": [make(3, 4)], "weight_decay": -1.0},
+                  {"params": [make(3, 4)], "adjust_lr_fn": "else"}, {"params": [make(3, 4)], "ns_steps": 0},
+                  {"params": [make(3, 4)], "eps": -1.0}):
+        with pytest.raises(ValueError):
+            optimizer.add_param_group(group)
+        assert len(optimizer.param_groups) == 1 and optimizer.param_groups[0]["params"] == [first]
+        with pytest.raises(ValueError):
+            FusedMuon([group])
+    second = make(4, 3)
+    optimizer.add_param_group({"params": (p for p in [second]), "adjust_lr_fn": "match_rms_adamw"})
+    assert optimizer.param_groups[1]["params"] == [second] and optimizer.param_groups[1]["lr"] == 0.1
