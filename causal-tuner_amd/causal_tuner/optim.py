@@ -167,6 +167,15 @@ def _muon_plan(shapes, device):
     return _MuonPlan(shapes, device)
 
 
+_MUON_SHORT, _MUON_LONG = 16384, 1 << 30   # sides of a matrix that ct_muon_plan takes
+
+
+def _refuse_large(name, shape):
+    if min(shape) > _MUON_SHORT or max(shape) > _MUON_LONG:
+        raise NotImplementedError(f"{name}: the HIP kernels take matrices up to {_MUON_SHORT} x {_MUON_LONG}, "
+                                  f"not {tuple(shape)}")
+
+
 def _muon_numbers(coefficients, steps, eps):
     """Checked (a, b, c), steps and eps of the iteration."""
     a, b, c = (float(x) for x in coefficients)
@@ -198,7 +207,7 @@ def orthogonalize(matrices, *, coefficients=(3.4445, -4.7750, 2.0315), steps=5, 
     transposed matrix where it has more rows than columns).
 
     `matrices` is a 2-D tensor or a list of them, float32 or bfloat16 on the device (any
-    shapes and strides, types and devices mixed); returns new contiguous tensors of the same
+    strides, types and devices mixed, shorter sides up to 16384, longer ones up to 2^30); returns new contiguous tensors of the same
     shapes and types, one or a list, that carry no gradient. Empty matrices come back empty, zero
     ones zero (where eps is not zero).
 
@@ -220,6 +229,7 @@ def orthogonalize(matrices, *, coefficients=(3.4445, -4.7750, 2.0315), steps=5, 
             results.append(_newton_schulz(m, coefficients, steps, eps) if m.numel() else m.clone())
             continue
         _native.refuse_tangents("orthogonalize", m)
+        _refuse_large("orthogonalize", m.shape)
         results.append(torch.empty(m.shape, dtype=m.dtype, device=m.device))
         if m.numel():
             buckets.setdefault((m.device, m.dtype), []).append(index)
@@ -239,7 +249,7 @@ def _adjusted(adjust_lr_fn, rows, cols):
 
 
 class FusedMuon(torch.optim.Optimizer):
-    """Muon over matrices on the device; torch.optim.Muon's arguments.
+    """Muon over matrices on the device (shorter sides up to 16384); torch.optim.Muon's arguments.
 
     Each step: momentum = mu momentum + (1 - mu) grad, M = mu momentum + (1 - mu) grad (nesterov)
     or momentum, param = param (1 - lr weight_decay) - lr adjust orthogonalize(M), with adjust =
@@ -320,6 +330,7 @@ class FusedMuon(torch.optim.Optimizer):
                 if p.grad.dtype != p.dtype or not p.is_contiguous() or not p.grad.is_contiguous():
                     raise NotImplementedError("FusedMuon: contiguous gradients of the parameter's dtype required")
                 if p.numel():
+                    _refuse_large("FusedMuon", p.shape)
                     buckets.setdefault((p.device, p.dtype), []).append((p, self._buffer_of(p)))
             options = _native.MuonOptions(
                 lr=float(group["lr"]), weight_decay=float(group["weight_decay"]), momentum=float(group["momentum"]),

@@ -629,7 +629,8 @@ typedef struct ct_muon_options {
  * CT_MUON_KINDS - 1] of them one kind after the other, and the bytes of workspace. With
  * entries = null only counts, the table and workspace_bytes are written. The caller copies the
  * entries to the device (16-byte aligned); they hold for every call with these shapes. Empty
- * matrices are refused: the caller leaves them out. ct_muon reads the host table while it runs
+ * matrices are refused (the caller leaves them out), and so are shorter sides past 16384 and
+ * longer ones past 2^30. ct_muon reads the host table while it runs
  * and passes it to the device in kernel arguments.
  */
 int ct_muon_plan(ct_muon_matrix *matrices, int64_t count, int32_t *entries, int64_t capacity, int64_t *counts,

@@ -328,3 +328,16 @@ def test_forward_mode_derivatives_are_refused():
         host = orthogonalize(forward_ad.make_dual(m.cpu(), torch.ones(20, 30)))
         assert forward_ad.unpack_dual(host).tangent.any()
     _check(orthogonalize(m), m)
+
+
+def test_sides_past_the_kernels_are_refused_by_name():
+    from causal_tuner.optim import FusedMuon, orthogonalize
+    for shape in ((16385, 16400), (1, (1 << 30) + 1)):
+        with pytest.raises(NotImplementedError, match="up to 16384"):
+            orthogonalize(torch.ones(1, 1, device="cuda", dtype=torch.bfloat16).expand(*shape))
+    p = torch.nn.Parameter(torch.zeros(16385, 16385, device="cuda", dtype=torch.bfloat16))
+    p.grad = torch.zeros_like(p)
+    optimizer = FusedMuon([p])
+    with pytest.raises(NotImplementedError, match="up to 16384"):
+        optimizer.step()
+    assert not optimizer.state[p]

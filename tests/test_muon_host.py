@@ -141,3 +141,20 @@ def test_groups_of_their_own_are_checked_and_refused_ones_left_out():
     second = make(4, 3)
     optimizer.add_param_group({"params": (p for p in [second]), "adjust_lr_fn": "match_rms_adamw"})
     assert optimizer.param_groups[1]["params"] == [second] and optimizer.param_groups[1]["lr"] == 0.1
+
+
+def test_the_largest_sides():
+    """The sizes that the Python calls refuse by name are those that ct_muon_plan refuses."""
+    from causal_tuner.optim import _refuse_large
+    lib = _native.library()
+    counts, nbytes = (ctypes.c_int64 * _native.CT_MUON_KINDS)(), ctypes.c_int64()
+    table = (_native.MuonMatrix * 1)()
+    for shape, fits in (((16384, 16384), True), ((16385, 16385), False), ((1, 1 << 30), True), ((1 << 30, 1), True),
+                        ((1, (1 << 30) + 1), False), (((1 << 30) + 1, 1), False), ((16384, 20000), True)):
+        table[0].rows, table[0].cols = shape
+        assert lib.ct_muon_plan(table, 1, None, 0, counts, ctypes.byref(nbytes)) == (0 if fits else -2), shape
+        if fits:
+            _refuse_large("orthogonalize", shape)
+        else:
+            with pytest.raises(NotImplementedError, match="up to 16384"):
+                _refuse_large("orthogonalize", shape)
