@@ -101,6 +101,9 @@ class AttentionLayout:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.tokens = max((stop for _, stop in self.records), default=0)
         self.key_tokens = max((stop for _, stop in self.key_records), default=0)
+        # whether the records follow one another, each with its own rows as keys
+        filled = [r for r in self.records if r[0] < r[1]]
+        self.in_order = self.key_records == self.records and filled == sorted(filled)
         # whether every row of the spans' range belongs to a record
         self.whole = sum(b - a for a, b in self.records) == self.tokens
         self.keys_whole = self.keys_disjoint and sum(b - a for a, b in self.key_records) == self.key_tokens

@@ -86,9 +86,12 @@ def packed_records(records, config, device):
     """`records` as the layers take them: for the packed kernels their layout, made once for all
     layers, otherwise the spans themselves."""
     from ..kernels.attention_cuda import AttentionLayout
+    given = isinstance(records, AttentionLayout)
+    if given and records.key_records != records.records:
+        raise ValueError("a decoder's records attend to themselves: a layout with other key_records")
     if config.attention != "packed":
-        return getattr(records, "records", records)
-    return records if isinstance(records, AttentionLayout) else AttentionLayout(records, device)
+        return records.records if given else records
+    return records if given else AttentionLayout(records, device)
 
 
 def _attention(q, k, v, records, config):
@@ -96,8 +99,8 @@ def _attention(q, k, v, records, config):
     if config.attention == "packed":
         from ..kernels.attention_cuda import packed_attention
         layout = packed_records(records, config, q.device)
-        if not layout.whole or layout.tokens != q.shape[1]:
-            raise ValueError("records must cover the sequence")
+        if not layout.whole or not layout.in_order or layout.tokens != q.shape[1]:
+            raise ValueError("records must cover the sequence in order")
         return packed_attention(q, k, v, layout)
     from torch.nn.attention import SDPBackend, sdpa_kernel
     records = packed_records(records, config, q.device)

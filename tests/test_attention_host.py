@@ -167,3 +167,24 @@ def test_host_tangents():
         tangent = forward_ad.unpack_dual(packed_attention(q, forward_ad.make_dual(k, along), v, [(0, 6)])).tangent
     up, down = (packed_attention(q, k + s * h * along, v, [(0, 6)]) for s in (1, -1))
     torch.testing.assert_close(tangent, (up - down) / (2 * h), rtol=1e-6, atol=1e-8)
+
+
+def test_decoder_records():
+    """The decoder's positions restart at each record as listed: records out of order or with keys
+    of others are refused, not attended to with other rows' positions."""
+    from causal_tuner.modeling import decoder
+    config = decoder.DecoderConfig(hidden_size=16, num_attention_heads=2, head_dim=8, intermediate_size=16,
+                                   num_hidden_layers=1, vocab_size=10, attention="packed")
+    plain = decoder.DecoderConfig(**{**vars(config), "attention": "sdpa"})
+    q, k, v = torch.randn(1, 9, 2, 8), torch.randn(1, 9, 1, 8), torch.randn(1, 9, 1, 8)
+    want = packed_attention(q, k, v, [(0, 4), (4, 4), (4, 9)])
+    for records in ([(0, 4), (4, 4), (4, 9)], [(0, 4), (4, 9), (0, 0)], AttentionLayout([(0, 4), (4, 9)], "cpu")):
+        assert torch.equal(decoder._attention(q, k, v, records, config), want)
+    for records in ([(4, 9), (0, 4)], [(0, 4), (4, 8)], [(0, 4), (5, 9)]):
+        with pytest.raises(ValueError, match="cover the sequence"):
+            decoder._attention(q, k, v, records, config)
+    others = AttentionLayout([(0, 4), (4, 9)], "cpu", key_records=[(0, 4), (0, 9)])
+    for c in (config, plain):
+        with pytest.raises(ValueError, match="key_records"):
+            decoder._attention(q, k, v, others, c)
+        assert decoder.packed_records([(0, 9)], c, "cpu") is not None
