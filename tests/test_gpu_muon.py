@@ -341,3 +341,46 @@ def test_sides_past_the_kernels_are_refused_by_name():
     with pytest.raises(NotImplementedError, match="up to 16384"):
         optimizer.step()
     assert not optimizer.state[p]
+
+
+def _shifted(t, by):
+    """The same tensor `by` elements into its storage: contiguous, at no 16-byte boundary."""
+    return t.new_empty(t.numel() + by)[by:].view(t.shape).copy_(t)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_muon_steps_of_every_kind_of_matrix(dtype, offset):
+    """Two steps of one list: short sides of each of the Gram and last products' sizes up to 256 and
+    past it, wide and tall, rows of four elements or not, and all of them at an odd element of
+    their storage (parameter, gradient and momentum)."""
+    from causal_tuner.optim import FusedMuon
+    shapes = [(256, 300), (300, 256), (256, 1030), (200, 333), (333, 201), (129, 132), (300, 513), (513, 290), (290, 516),
+              (33, 31), (1, 7), (7, 1), (60, 2051), (1030, 1100), (12, 20), (100, 64), (4, 4100)]
+    params = [torch.nn.Parameter(_shifted(_matrix(s, dtype, seed=i) * 20, offset)) for i, s in enumerate(shapes)]
+    lr, decay, mu = 0.02, 0.1, 0.9
+    optimizer = FusedMuon(params, lr=lr, weight_decay=decay, momentum=mu)
+    for i, (p, s) in enumerate(zip(params, shapes)):
+        optimizer.state[p]["momentum_buffer"] = _shifted(_matrix(s, torch.float32, seed=50 + i), offset)
+    u = torch.finfo(dtype).eps / 2
+    for step in range(2):
+        before = [p.detach().double() for p in params]
+        held = [optimizer.state[p]["momentum_buffer"].double() for p in params]
+        for i, p in enumerate(params):
+            p.grad = _shifted(_matrix(shapes[i], dtype, seed=100 * step + i + 7), offset)
+        kept = [p.grad.clone() for p in params]
+        optimizer.step()
+        for p, old, m, g in zip(params, before, held, kept):
+            assert torch.equal(p.grad, g)
+            buffer = optimizer.state[p]["momentum_buffer"]
+            g = g.double()
+            want = mu * m + (1 - mu) * g
+            assert ((buffer.double() - want).abs() <= 4 * E32 * (mu * m.abs() + (1 - mu) * g.abs())).all(), tuple(p.shape)
+            m = buffer.double()   # from here on with what the optimizer holds
+            direction, bound = _reference(mu * m + (1 - mu) * g)
+            rows, cols = p.shape
+            factor = lr * max(1.0, rows / cols) ** 0.5
+            want = old * (1 - lr * decay) - factor * direction
+            allowed = factor * (bound + 3 * E32 * A ** 5 + 4 * E32 * direction.abs()) + 4 * E32 * old.abs()
+            over = (p.double() - want).abs() - allowed - u * (want.abs() + allowed)
+            assert over.max() <= 0, f"{tuple(p.shape)}: {over.max()} over a bound of {allowed.max()}"
