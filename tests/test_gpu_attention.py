@@ -358,3 +358,13 @@ def test_forward_mode_derivatives_are_refused():
             torch.autograd.grad(out, leaf, forward_ad.make_dual(dout, dout))
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda t: packed_attention(t, k, v, layout), (q,), (q,))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,dim,sizes,key_sizes", [
+    (24, 1, 64, [1, 70, 129], [1, 70, 129]), (32, 1, 128, [65, 40], [65, 40]), (33, 1, 64, [9, 50], [30, 50]),
+    (48, 1, 128, [33, 3, 60], [33, 3, 60]), (72, 2, 40, [21, 30], [21, 45]), (130, 1, 64, [5, 17], [5, 80]),
+    (64, 64, 16, [40], [40])])
+def test_many_heads_to_a_key_value_head(heads, kv_heads, dim, sizes, key_sizes, dtype):
+    """Groups as large as a step of 32 rows, which they divide, and past it; past a tile of 128."""
+    _case(sizes, key_sizes, heads, kv_heads, dim, dtype, True)
