@@ -61,6 +61,7 @@ typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
 constexpr int kThreads = 256;   // 4 waves
 constexpr int kWaveCols = 32;   // rows (forward, dq) or keys (dk, dv) per wave
 constexpr int kTile = 128;      // per workgroup
+constexpr int kRowWaves = 4, kRowTile = kWaveCols * kRowWaves;   // of a forward or dq workgroup
 constexpr int kEntry = 8;       // int32 per plan entry
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -357,11 +358,13 @@ __device__ __forceinline__ void wave_limits(const RowOf &row, int &least, int &m
     most = __builtin_amdgcn_readfirstlane(most);
 }
 
-// ------------------------------------------------------------------ the key loop
-// Forward and dq run over 32-key steps, dk/dv over 32-row steps, all in one rhythm: step t
-// multiplies with tile t (the second products) while it makes the scores of tile t + 1, so
-// that a wave always has matrix instructions beside its exponentials; tile t + 2 goes from
-// registers to LDS and tile t + 3 from memory to registers. Three LDS stages, one barrier a step.
+// ------------------------------------------------------------------ the main loops
+// dq runs over 32-key steps and dk/dv over 32-row steps in one rhythm: step t multiplies with
+// tile t (the second products) while it makes the scores of tile t + 1, so that a wave always
+// has matrix instructions beside its exponentials; tile t + 2 goes from registers to LDS and
+// tile t + 3 from memory to registers. Three LDS stages, one barrier a step. The forward, which
+// has no registers for a second set of scores, runs over tiles of kKeyTile keys in two stages: a
+// tile's scores, its exponentials, its products, while the next one comes in.
 constexpr int kStep = 32, kStages = 3;
 
 // Runs f(stage, next, then) over consecutive steps with the stages as constants, so that LDS
@@ -402,8 +405,8 @@ __device__ __forceinline__ float2 row_stats(float m, float sum) {
 template <typename T>
 constexpr int kKeyTile = sizeof(T) == 2 ? 64 : 32;
 
-template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) void attention_forward(AttnParams a) {
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 || DP == 64 ? 2 : 1) void attention_forward(AttnParams a) {
     constexpr int KT = kKeyTile<T>, kUnits = KT * Tile<T, DP>::kChunks;
     __shared__ uint4 sk[2][kUnits], sv[2][kUnits];
     const Group group = a.groups[blockIdx.x / a.kv_heads];
@@ -421,7 +424,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
 
         const char *k0 = a.k + rec.k_start * a.k_token + kv_head * a.k_head;
         const char *v0 = a.v + rec.k_start * a.v_token + kv_head * a.v_head;
-        Stage<T, DP, KT, 64 * WAVES> ks, vs;
+        Stage<T, DP, KT, 64 * kRowWaves> ks, vs;
         auto load = [&](int key) {
             const int left = (int)rec.k_len - key;
             auto valid = [&](int r) { return r < left; };
@@ -533,7 +536,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
             if (a.stats && lane < 32)
                 a.stats[row.token * a.heads + row.head] = row_stats(run.m, sum);
         } else {
-            const int64_t at = ((int64_t)item.slot * a.kv_heads + kv_head) * (32 * WAVES) + wave * kWaveCols + (lane & 31);
+            const int64_t at = ((int64_t)item.slot * a.kv_heads + kv_head) * kRowTile + wave * kWaveCols + (lane & 31);
             float *dst = a.part0 + at * DP;
             const float scale = sum == 0.0f ? 0.0f : sum / taken;   // joined with the exact sums as weights
 #pragma unroll
@@ -645,8 +648,8 @@ __device__ __forceinline__ float dot_chunk(const uint4 &x, const uint4 &y, float
     return acc;
 }
 
-template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) void attention_dq(AttnParams a) {
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * kRowWaves, sizeof(T) == 2 || DP == 64 ? 2 : 1) void attention_dq(AttnParams a) {
     constexpr int kUnits = kStep * Tile<T, DP>::kChunks;
     __shared__ uint4 sk[kStages][kUnits], sv[kStages][kUnits];
     const Group group = a.groups[blockIdx.x / a.kv_heads];
@@ -690,7 +693,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
 
         const char *k0 = a.k + rec.k_start * a.k_token + kv_head * a.k_head;
         const char *v0 = a.v + rec.k_start * a.v_token + kv_head * a.v_head;
-        Stage<T, DP, kStep, 64 * WAVES> ks, vs;
+        Stage<T, DP, kStep, 64 * kRowWaves> ks, vs;
         auto load = [&](int key) {
             const int left = (int)rec.k_len - key;
             auto valid = [&](int r) { return r < left; };
@@ -766,7 +769,7 @@ __global__ __launch_bounds__(64 * WAVES, sizeof(T) == 2 || DP == 64 ? 2 : 1) voi
                                   o[n][i + 3] * a.scale);
                 }
         } else {
-            float *dst = a.part0 + (((int64_t)item.slot * a.kv_heads + kv_head) * (32 * WAVES) + wave * kWaveCols +
+            float *dst = a.part0 + (((int64_t)item.slot * a.kv_heads + kv_head) * kRowTile + wave * kWaveCols +
                                     (lane & 31)) * DP;
 #pragma unroll
             for (int n = 0; n < DP / 32; ++n)
@@ -1019,10 +1022,6 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_join(AttnParams a, con
 }
 
 // ------------------------------------------------------------------ host side
-#ifndef RW
-#define RW 4
-#endif
-constexpr int kRowWaves = RW, kRowTile = 32 * kRowWaves;
 constexpr int64_t kMaxRows = 0x7fffffff - 2 * kTile;
 
 // A piece's fixed cost (its rows' or keys' load, its result's store) in units of kUnit.
@@ -1316,7 +1315,7 @@ extern "C" int ct_attention_forward(const ct_attention *c, const int32_t *plan, 
     return by_type(c->dtype, dp, [&](auto type, auto dim) {
         typedef decltype(type) T;
         constexpr int DP = decltype(dim)::value;
-        attention_forward<T, DP, kRowWaves>
+        attention_forward<T, DP>
             <<<dim3((unsigned)(groups * c->kv_heads)), dim3(64 * kRowWaves), 0, stream>>>(a);
         if (const int status = status_of_last_launch()) return status;
         if (!joins) return 0;
@@ -1369,7 +1368,7 @@ extern "C" int ct_attention_backward(const ct_attention *c, const int32_t *row_p
             set_plan(r, row_plan, row_counts);
             r.dst0 = (char *)dq;
             r.d_token = a.o_token;
-            attention_dq<T, DP, kRowWaves>
+            attention_dq<T, DP>
                 <<<dim3((unsigned)(rows * c->kv_heads)), dim3(64 * kRowWaves), 0, stream>>>(r);
             if (const int status = status_of_last_launch()) return status;
             if (row_counts[1]) {

@@ -666,7 +666,7 @@ struct StageOp {
 // One 32 x 32 tile (i >= j) of left right, both symmetric and commuting, so their product is
 // symmetric too and the tile's mirror image is its transpose. kMakeP: a I + b G + c G G. Each
 // of the 8 waves takes an eighth of the reduction over the whole tile (one load per product
-// instead of two) straight from L2, all loads of up to 8 k-steps in flight at once, operand
+// instead of two) straight from L2, all loads of up to kSteps k-steps in flight at once, operand
 // rows read along k's rows (symmetry), and the sums are added in LDS in order.
 constexpr int kStageThreads = 512;
 
