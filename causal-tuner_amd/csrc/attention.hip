@@ -2,7 +2,7 @@
 // probabilities. Per record and head, with query i and key j of the record,
 //   s_ij = scale q_i . k_j          visible: j < limit_i = keys (plain) or
 //                                   min(keys, i + 1 + keys - queries) (causal)
-//   p_ij = exp(s_ij - lse_i),  lse_i = log sum_j exp(s_ij),  o_i = sum_j p_ij v_j
+//   p_ij = exp(s_ij - m_i) / l_i,  m_i = max_j s_ij,  l_i = sum_j exp(s_ij - m_i),  o_i = sum_j p_ij v_j
 //   delta_i = do_i . o_i,  ds_ij = p_ij (do_i . v_j - delta_i)
 //   dv_j = sum_i p_ij do_i,  dk_j = scale sum_i ds_ij q_i,  dq_i = scale sum_j ds_ij k_j
 // (the place of the reference's kernels/attention.py:58-93, which calls a library).
@@ -26,7 +26,7 @@
 // the output's own rounding: together 1.4 times the output's, 0.0024 against 0.0017 in norm);
 // float32 inputs round nothing. Where a row sees few keys, do . v and delta nearly cancel, and
 // a delta from the rounded output made dq and dk 0.005 off (records of one to four tokens): the
-// output is divided by the sum of the p that entered its product (lse keeps the exact one), and
+// output is divided by the sum of the p that entered its product (the backward has the exact one), and
 // for a backward the forward keeps the output's rounding error in bf16 as well (`rest`).
 //
 // dq and dk/dv are two kernels that each recompute s (7 products instead of 5): the one-pass
@@ -35,11 +35,11 @@
 // 32 heads) outweighs the two products.
 //
 // What bounds it. The matrix instructions and, beside them, the exponentials: 8192 causal rows
-// of 32 heads of 128 over one key/value head, bf16: forward 608 us (905 TFLOP/s; 598 without
-// the second sum and `rest`), dq 831 (992), dk and dv 1388 (792), where a large library product
-// reaches 1095 TFLOP/s on the same card (its clock falls under that load) and HBM traffic is a
-// few percent. Few query tokens: the stream of keys and values, 131072 keys of 8 heads in 104
-// us, 5.2 TB/s (a large copy 5.1).
+// of 32 heads of 128 over one key/value head, bf16: forward 613 us (897 TFLOP/s; 10 us of it for
+// the second sum and `rest`), dq 782 (1055), dk and dv 1351 (814), with the matrix instructions
+// busy 42, 52 and 35% of the SIMDs' cycles. Large library products reach 1100 to 1600 on the same
+// card by size and layout; HBM traffic is a few percent. Few query tokens: the stream of keys and
+// values, 131072 keys of 8 heads in 103 us, 5.2 TB/s (a large copy 5.2).
 // Tried and left out: the two waves of a SIMD in turns (one in matrix instructions while the
 // other has its exponentials, two barriers a step): forward 615 -> 580 us, but 43 -> 46 at three
 // short records and both backward kernels slower; 8 waves per forward workgroup (7% slower at
@@ -1024,7 +1024,12 @@ __global__ __launch_bounds__(kThreads) void attention_dkv_join(AttnParams a, con
 // ------------------------------------------------------------------ host side
 constexpr int64_t kMaxRows = 0x7fffffff - 2 * kTile;
 
-// A piece's fixed cost (its rows' or keys' load, its result's store) in units of kUnit.
+// A piece's fixed cost (its rows' or keys' load, its result's store) in units of kUnit: the
+// smaller it is, the more pieces and partials there are. Measured, three records of 3421 tokens of
+// 16 heads, forward: 53 us with kRowFixed = 1, 43 with 3, 40 with 6, which takes 51 instead of 50 at
+// 24 tokens of one row. kKeyFixed = 3, 6 and 12: the same within 1%. Two float32 records of 833 rows
+// of 8 heads, forward and backward: 85 us with kF32Fixed = 1, 111 with 3, 176 with 6; its few rows
+// are short of workgroups, not of joins.
 constexpr int64_t kRowFixed = 3, kKeyFixed = 6, kF32Fixed = 1;
 constexpr int64_t kMaxPitch = (int64_t)1 << 24;   // bytes between tokens of k and v
 

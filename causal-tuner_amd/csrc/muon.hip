@@ -26,12 +26,14 @@
 // step where M has nothing and its own rounding (2^-24) reaches M's rows: 2e-5 after 5 steps, 1e-2
 // after 10, and a tenth from 14 on, where the floor ends Q's growth (float32 steps: 1 and more).
 //
-// What bounds it, two layers' adapters of rank 256 (36M elements, 754 us a step): the Gram
-// pass 229 us (double matrix instructions, 73% of its cycles at a clock that they pull down to
-// about 1.9 GHz; 12 bytes an element), the 14 launches of r x r products 24 us each (their
-// operands' way from L2, half of it, and double matrix instructions), the last product 240 us
-// (float32 matrix instructions, 62% of its cycles; 16 bytes an element, 2.4 TB/s, which alone
-// take 170). Small sets: the launches.
+// What bounds it, two layers' adapters of rank 256 (36M elements, 749 us a step): the Gram
+// pass 206 us (double matrix instructions, 70% of its cycles at a clock that they pull down to
+// about 1.9 GHz; 12 bytes an element), the 14 launches of r x r products 22 us each (their
+// operands' way from L2, half of it, and double matrix instructions, 45%), the last product 214 us
+// (float32 matrix instructions, 62% of its cycles; 16 bytes an element, 2.7 TB/s, which alone
+// take 170). Small sets: the launches. Whole models: every matrix has its own scratch, 949 MB for
+// 24 layers of width 2048, and the launches go through it past the caches (338 us a layer, 264
+// at 4 layers).
 // Tried and left out: 64 x 64 tiles in the r x r products (the same at 24 matrices, 20% slower
 // at 12), k-steps of 32 rows in flight instead of 16 (more registers, 3% slower).
 //
@@ -763,8 +765,8 @@ __global__ __launch_bounds__(kStageThreads) void muon_stage(const Matrix *matric
 // 32 of the reduction, and each group asks first for the next group's Q, then for a part of
 // the next slab's gradient and momentum and of its own parameters: those have a group's
 // products (1.7 us) to come in before anything waits behind them. Two layers' adapters of rank
-// 256 take 240 us; a slab per workgroup, two workgroups per CU with nothing asked for ahead,
-// took 302. Short sides past 256 go slab by slab, in blocks of 256 rows and 256 of the reduction.
+// 256 took 240 us (five passes, a cold card); a slab per workgroup, two workgroups per CU with
+// nothing asked for ahead, 302. Short sides past 256 go slab by slab, in blocks of 256 rows and 256 of the reduction.
 constexpr int kApplyThreads = 512;
 constexpr int kApplyLds = 18432;   // floats: 256 x 72, 128 x 136, 64 x 264, 32 x 520 and their transposes
 
