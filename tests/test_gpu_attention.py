@@ -306,15 +306,16 @@ def test_device_refusals():
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("sizes,key_sizes", [([200], [200]), ([1, 3], [700, 900])])
+@pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("exponent", [14, 16, 24, 34, 100])
-def test_scores_of_any_size(exponent, sizes, key_sizes, dtype):
+def test_scores_of_any_size(exponent, dim, sizes, key_sizes, dtype):
     """Scores s = +-2^exponent k / 8 of whole k, so that each row's softmax is 1 at its largest
     score or 1/2 at two equal ones and 0 elsewhere: a float32 sum of m and log2 of the
     denominator would lose the latter from scores of 2^16 on. v and dout are -1, 0 or 1, so all
-    sums and ds = (dp_1 - dp_2) / 4 are exact; what is left is the results' rounding and the last
+    sums and ds = (dp_1 - dp_2) / 4 (at most 8 bits) are exact; what is left is the results' rounding and the last
     places of the exponential and the logarithm."""
     from causal_tuner.kernels.attention_cuda import AttentionLayout
-    tokens, key_tokens, heads, dim = sum(sizes), sum(key_sizes), 4, 64
+    tokens, key_tokens, heads = sum(sizes), sum(key_sizes), 4
     records, keys = records_of(sizes), records_of(key_sizes)
     g = torch.Generator().manual_seed(exponent)
     if len(sizes) == 1:
@@ -329,7 +330,7 @@ def test_scores_of_any_size(exponent, sizes, key_sizes, dtype):
     k[:, 0, 0] = number
     v, dout = (torch.randint(-1, 2, s, generator=g).float() for s in ((key_tokens, 1, dim), (tokens, heads, dim)))
     leaves = [t.to("cuda", dtype).requires_grad_(True) for t in (q, k, v)]
-    got = _run(*leaves, dout.to("cuda", dtype), AttentionLayout(records, "cuda", key_records=keys))
+    got = _run(*leaves, dout.to("cuda", dtype), AttentionLayout(records, "cuda", key_records=keys), scale=0.125)
     want, _ = reference(*leaves, records, keys, True, 0.125, dout.cuda())
     assert not want[1].any() and want[2].any()
     u = torch.finfo(dtype).eps / 2
