@@ -206,11 +206,11 @@ def orthogonalize(matrices, *, coefficients=(3.4445, -4.7750, 2.0315), steps=5, 
     X = M / max(|M|, eps), then `steps` times X = a X + (b A + c A^2) X with A = X X^T (of the
     transposed matrix where it has more rows than columns).
 
-    `matrices` is a 2-D tensor or a list of them, float32 or bfloat16 on the device (any
-    strides, types and devices mixed, shorter sides up to 16384, longer ones up to 2^30); returns new contiguous tensors of the same
-    shapes and types, one or a list, that carry no gradient. Empty matrices come back empty, zero
-    ones zero (where eps is not zero); device matrices need max(|M|, eps) of 1e-35, below which
-    float32 factors 1 / |M| overflow.
+    `matrices` is a 2-D tensor or a list of them, float32 or bfloat16 on the device (any strides,
+    types and devices mixed, shorter sides up to 16384, longer ones up to 2^30); returns new
+    contiguous tensors of the same shapes and types, one or a list, that carry no gradient. Empty
+    matrices come back empty, zero ones zero (where eps is not zero); device matrices need
+    max(|M|, eps) of 1e-35, below which float32 factors 1 / |M| overflow.
 
     A direction that M does not have grows from rounding noise by a per step, as in any iteration
     in 32 bits: matrices of low rank are 2e-5 off after 5 steps of the default coefficients, 1e-2
