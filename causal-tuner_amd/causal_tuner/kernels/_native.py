@@ -70,6 +70,18 @@ class Attention(ctypes.Structure):
 _ATT = ctypes.POINTER(Attention)
 
 
+class HeadLoss(ctypes.Structure):
+    """Mirror of `ct_head_loss`: the operands of the loss over a vocabulary walked in pieces."""
+
+    _fields_ = [(name, _P) for name in ("hidden", "head", "rows", "indices", "values", "log_normalizer", "weights")] + [
+        (name, _I64) for name in ("ld_hidden", "ld_head", "ld_indices", "ld_values", "tokens", "hidden_width", "count",
+                                  "width", "vocab")] + [
+        ("entries", _I32), ("dtype", _I32), ("temperature", ctypes.c_double)]
+
+
+_HEAD = ctypes.POINTER(HeadLoss)
+
+
 CT_MUON_KINDS = 7  # kinds of plan entries of ct_muon_plan
 
 
@@ -142,6 +154,14 @@ _SIGNATURES = {
                                              _P]),
     "ct_muon_plan": (ctypes.c_int, [_MUON, _I64, _P, _I64, _P, _P]),
     "ct_muon": (ctypes.c_int, [_MUON, _I64, _P, _P, _I32, ctypes.POINTER(MuonOptions), _P, _I64, _I64, _P]),
+    "ct_head_loss_kept": (_I64, [_I64, _I64, _I64, _I32, _I32, _I32]),
+    "ct_head_loss_workspace": (_I64, [_I64, _I64, _I64, _I32, _I32, _I32]),
+    "ct_head_loss_forward": (ctypes.c_int, [_HEAD, _P, _I32, _P, _I64, _P, _I64, _P]),
+    "ct_head_loss_backward": (ctypes.c_int, [_HEAD, _P, _P, _I32, _I64, _P, _I64, _I64, _I32, _P, _I64, _I64, _I32, _P,
+                                             _I64, _P]),
+    "ct_layer_norm_forward": (ctypes.c_int, [_P, _I32, _P, _P, _I32, _P, _P, _P, _I64, _I64, ctypes.c_double, _P]),
+    "ct_layer_norm_backward_workspace": (_I64, [_I64, _I64, _I32, _I32]),
+    "ct_layer_norm_backward": (ctypes.c_int, [_P, _I32, _P, _I32, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _P]),
     "ct_profile_begin": (ctypes.c_int, [_I32, _I32]),
     "ct_profile_read": (ctypes.c_int, [_I32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_I64),
                                        ctypes.POINTER(ctypes.c_double)]),

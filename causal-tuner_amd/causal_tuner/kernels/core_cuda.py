@@ -6,6 +6,8 @@ kernels ct_rms_forward / ct_rms_backward with the reference's rounding points, i
 private-gradient reuse (the input gradient written over the incoming gradient) and its
 output reconstruction mode (the backward reads the output and the weight instead of x).
 
+`layer_norm_device` is layer normalization on ct_layer_norm_forward / ct_layer_norm_backward, behind
+`modeling.norm.layer_norm` (the reference has none).
 
 Same operator API as the reference: `rotate_owned_qk` (core_cuda.py:192-200) rotates the
 q and k outputs of a projection group in place, `inverse_rope_tile` (203-208) writes the
@@ -64,6 +66,82 @@ class RMS(torch.autograd.Function):
                     _native.stream_of(x))
             _native.check(status, "ct_rms_backward")
         return (result, dw, None, None, None)[:len(ctx.needs_input_grad)]
+
+
+def _layer_norm(x, weight, bias, eps, keep):
+    """(x as the kernel reads it, y, mean, rstd); mean and rstd None unless kept."""
+    x = x.contiguous()
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        weight, bias = weight.float(), bias.float()   # one type for both: float32 holds either
+    if weight is not None:
+        weight = weight.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    vector = weight if weight is not None else bias
+    y, width = torch.empty_like(x), x.shape[-1]
+    rows = x.numel() // width
+    mean = rstd = None
+    if keep:
+        mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32)
+    with _native.device_of(x):
+        status = _native.library().ct_layer_norm_forward(
+            x.data_ptr(), _native.dtype_code(x.dtype), _native.ptr(weight), _native.ptr(bias),
+            _native.CT_F32 if vector is None else _native.dtype_code(vector.dtype), y.data_ptr(), _native.ptr(mean),
+            _native.ptr(rstd), rows, width, eps, _native.stream_of(x))
+    _native.check(status, "ct_layer_norm_forward")
+    return x, y, mean, rstd
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        x, y, mean, rstd = _layer_norm(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, mean, rstd = ctx.saved_tensors
+        _native.refuse_tangents("layer_norm", grad)
+        grad, width, rows = grad.contiguous(), x.shape[-1], len(mean)
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = torch.empty_like(x) if need_x else None
+        # both sums are made in the weight's dtype; a bias of a wider one takes float32
+        dtype = weight.dtype if weight is not None else ctx.bias_dtype or torch.float32
+        if need_b and ctx.bias_dtype != dtype:
+            dtype = torch.float32
+        dw = torch.empty(width, device=x.device, dtype=dtype) if need_w else None
+        db = torch.empty(width, device=x.device, dtype=dtype) if need_b else None
+        if weight is not None:
+            weight = weight.to(dtype).contiguous()   # a wider type holds the same values
+        lib, code = _native.library(), _native.dtype_code(x.dtype)
+        nbytes = lib.ct_layer_norm_backward_workspace(rows, width, code, int(need_w or need_b))
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        with _native.device_of(x):
+            status = lib.ct_layer_norm_backward(
+                x.data_ptr(), code, _native.ptr(weight), _native.dtype_code(dtype), mean.data_ptr(), rstd.data_ptr(),
+                grad.data_ptr(), _native.ptr(dx), _native.ptr(dw), _native.ptr(db), rows, width, _native.ptr(workspace),
+                nbytes, _native.stream_of(x))
+        _native.check(status, "ct_layer_norm_backward")
+        if dw is not None:
+            dw = dw.to(ctx.saved_tensors[1].dtype)
+        if db is not None:
+            db = db.to(ctx.bias_dtype)
+        return dx, dw, db, None
+
+
+def layer_norm_device(x, weight, bias, eps):
+    """`modeling.norm.layer_norm` of device tensors, its arguments checked there."""
+    if x.dtype not in _native.DTYPE_CODES or any(t is not None and t.dtype not in _native.DTYPE_CODES
+                                                 for t in (weight, bias)):
+        raise NotImplementedError("layer_norm: the HIP kernels take bfloat16, float16 or float32")
+    given = [t for t in (x, weight, bias) if t is not None]
+    _native.refuse_tangents("layer_norm", *given)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return _layer_norm(x, weight, bias, eps, False)[1]
 
 
 def _token_pitch(t, tokens, width):

@@ -1,4 +1,5 @@
-"""Projection + weighted cross-entropy without ever holding the sequence's logits.
+"""Projection + weighted cross-entropy without ever holding the sequence's logits, and
+distillation from a teacher's top logits in the same way (`distillation_loss`).
 
 Interface of the reference's kernels/loss.py (`active_rows` 6-16, `row_count` 19-20,
 `projection_loss` 23-66) and of its host autograd function `ProjectionLoss`
@@ -43,7 +44,7 @@ def _check_backend(implementation, cut_chunk_size, head):
         if head.requires_grad:
             raise ValueError("cut cannot guarantee FP32 head-gradient accumulation; use fused")
         raise RuntimeError("The cut backend requires cut-cross-entropy")
-    if implementation != "fused":
+    if implementation not in ("fused", "streamed"):
         raise ValueError("Unsupported projection-loss backend")
     if cut_chunk_size:
         raise ValueError("cut_chunk_size applies only to the cut backend")
@@ -54,7 +55,13 @@ def projection_loss(hidden, head, targets, weights, *, token_budget=128, compute
     """sum_i weights[i] * CE(hidden[i] head^T, targets[i]) over the supervised rows, with at
     most `token_budget` rows of logits at a time. `reuse_hidden` lets the gradient of
     `hidden` take over its storage (an exclusive contiguous non-leaf tensor). `rows` is a
-    precomputed `active_rows` selection."""
+    precomputed `active_rows` selection.
+
+    `implementation="streamed"` takes all rows at once and walks the vocabulary in pieces instead
+    (`head_loss_cuda`): no logits are held, so `token_budget` plays no part; the statistics and
+    the loss come from unrounded float32 logits, and every gradient is rounded once, after the
+    upstream scale. bf16 and float32; `reuse_hidden` belongs to the fused path. With `rows` given
+    it can be captured into a graph."""
     if token_budget <= 0:
         raise ValueError("loss_token_budget must be positive")
     selection = active_rows(weights, hidden.device) if rows is None else rows
@@ -62,10 +69,17 @@ def projection_loss(hidden, head, targets, weights, *, token_budget=128, compute
         # The logits GEMM is the BLAS library's: its bf16 reductions stay in fp32.
         torch.backends.cuda.matmul.allow_bf16_reduced_precision_reduction = False
     _check_backend(implementation, cut_chunk_size, head)
+    if implementation == "streamed":
+        if reuse_hidden:
+            raise ValueError("reuse_hidden applies only to the fused backend")
+        _check_rows(hidden, head, weights, {"targets": targets})
     if not hidden.is_cuda:
         return ProjectionLoss.apply(hidden, head, targets, weights, token_budget, compute_dtype, selection)
     if not torch.is_grad_enabled():
         hidden, head = hidden.detach(), head.detach()
+    if implementation == "streamed":
+        from .head_loss_cuda import streamed_loss
+        return streamed_loss(hidden, head, weights, selection, compute_dtype, targets.reshape(-1, 1))
     if reuse_hidden and hidden.requires_grad:
         shared = hidden.is_leaf or hidden._base is not None or not hidden.is_contiguous()
         if shared:
@@ -74,6 +88,82 @@ def projection_loss(hidden, head, targets, weights, *, token_budget=128, compute
     total, _ = FusedProjectionLoss.apply(hidden, head, targets, weights, token_budget, compute_dtype,
                                          reuse_hidden, selection)
     return total
+
+
+def _check_rows(hidden, head, weights, tables):
+    """One row of every table and one weight per row of hidden, all on its device."""
+    if hidden.dim() < 1 or head.dim() != 2 or hidden.shape[-1] != head.shape[1] or head.numel() == 0:
+        raise ValueError(f"hidden {tuple(hidden.shape)} and head {tuple(head.shape)} do not give logits")
+    tokens = hidden.numel() // hidden.shape[-1]
+    if weights.numel() != tokens:
+        raise ValueError(f"{weights.numel()} weights for {tokens} rows of hidden")
+    for name, table in tables.items():
+        if table.numel() != tokens * (table.shape[-1] if name in ("indices", "values") else 1):
+            raise ValueError(f"{name} {tuple(table.shape)} for {tokens} rows of hidden")
+    for name, table in {"head": head, **tables}.items():
+        if table.device != hidden.device:
+            raise ValueError(f"{name} is on {table.device}, hidden on {hidden.device}")
+
+
+def distillation_loss(hidden, head, indices, values, weights, *, temperature=1.0, log_normalizer=None,
+                      compute_dtype=torch.bfloat16, rows=None):
+    """Distillation from a teacher's top logits: over the supervised rows,
+
+        sum_i weights[i] * sum_k q_ik (log q_ik - log p_i[indices[i, k]]),
+        p_i = softmax(hidden[i] head^T / temperature) over the whole vocabulary,
+        q_i = softmax(values[i] / temperature) over the row's entries, or, with `log_normalizer`
+              (the teacher's own log sum exp of its logits / temperature, one per row),
+              exp(values[i] / temperature - log_normalizer[i]), whose sum may be below one.
+
+    `indices` and `values` are [..., K], K up to 1024, one row per row of hidden. Lists may differ in length:
+    an index outside [0, vocab) (-1, say) is no entry, whatever its value; a value of -inf is an
+    entry without mass; an index given twice counts once, with the sum of both probabilities; a row
+    without entries has no loss and no gradient. The factor temperature^2 that keeps the gradient's size,
+    or a share beside another loss, belongs into `weights`. The vocabulary is walked in pieces
+    as `projection_loss(implementation="streamed")` does, on the same kernels; gradients reach
+    hidden and head, not the teacher. `rows` as in `projection_loss`."""
+    if indices.dim() < 1 or indices.shape != values.shape:
+        raise ValueError(f"indices {tuple(indices.shape)} and values {tuple(values.shape)} differ")
+    if not 1 <= indices.shape[-1] <= 1024:
+        raise ValueError(f"{indices.shape[-1]} entries per row: 1 to 1024 are taken")
+    if indices.is_floating_point() or not values.is_floating_point():
+        raise ValueError("indices are whole numbers, values floating")
+    temperature = float(temperature)
+    if not 2.0 ** -60 <= temperature <= 2.0 ** 60:
+        raise ValueError(f"temperature {temperature} is not a positive number between 2^-60 and 2^60")
+    tables = {"indices": indices, "values": values}
+    if log_normalizer is not None:
+        tables["log_normalizer"] = log_normalizer
+    _check_rows(hidden, head, weights, tables)
+    if any(t is not None and t.requires_grad for t in (values, log_normalizer)):
+        raise ValueError("the teacher's values get no gradient: detach them")
+    selection = active_rows(weights, hidden.device) if rows is None else rows
+    entries = indices.shape[-1]
+    indices, values = indices.reshape(-1, entries), values.reshape(-1, entries)
+    log_normalizer = None if log_normalizer is None else log_normalizer.flatten()
+    if not hidden.is_cuda:
+        return _host_distillation(hidden, head, indices, values, weights, temperature, log_normalizer, compute_dtype,
+                                  selection)
+    if not torch.is_grad_enabled():
+        hidden, head = hidden.detach(), head.detach()
+    from .head_loss_cuda import streamed_loss
+    return streamed_loss(hidden, head, weights, selection, compute_dtype, indices, values, log_normalizer, temperature)
+
+
+def _host_distillation(hidden, head, indices, values, weights, temperature, log_normalizer, compute_dtype, selection):
+    """The same in torch operations, float32 (float64 for its tensors) from the logits on."""
+    h = hidden.reshape(-1, hidden.shape[-1])[selection].to(compute_dtype)
+    wide = torch.promote_types(compute_dtype, torch.float32)
+    log_p = torch.log_softmax(F.linear(h, head.to(compute_dtype)).to(wide) / temperature, -1)
+    index, scale = indices[selection], weights.flatten()[selection].to(wide)
+    teacher = (values[selection].to(wide) / temperature).masked_fill((index < 0) | (index >= len(head)), -float("inf"))
+    if log_normalizer is None:
+        # a row without any mass has no entries
+        log_q = teacher - torch.logsumexp(teacher, -1, keepdim=True).clamp_min(torch.finfo(wide).min)
+    else:
+        log_q = teacher - log_normalizer[selection].to(wide)[:, None]
+    q = torch.zeros_like(log_p).scatter_add_(1, index.clamp(0, len(head) - 1), log_q.exp())
+    return (scale[:, None] * torch.where(q != 0, q * (torch.where(q != 0, q, 1).log() - log_p), 0)).sum()
 
 
 def _host_tiles(selection, tile):

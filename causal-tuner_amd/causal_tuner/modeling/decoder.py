@@ -5,9 +5,10 @@ to what one training step of packed records needs.
 Every projection is a `Projection` with a frozen NF4 base and a unit-scale LoRA adapter,
 driven through the reference's group operators: q/k/v share their input in
 `project_group` with the partial RoPE applied to q and k (`rotary=`), o_proj adds the
-residual, the MLP is `tiled_lora_mlp` with the residual; RMSNorm runs the HIP kernels,
-and the loss is `projection_loss` over the supervised rows. Attention is causal within each
-packed record, the single key/value head shared by the query heads: PyTorch-ROCm's
+residual, the MLP is `tiled_lora_mlp` with the residual; RMSNorm runs the HIP kernels (layer
+norms with `DecoderConfig(norm="layer")`), and the loss is `projection_loss` over the supervised
+rows, or `distillation_loss` from a teacher's top logits. Attention is causal within each packed
+record, the single key/value head shared by the query heads: PyTorch-ROCm's
 scaled-dot-product attention (memory-efficient backend, flash as the deterministic
 choice) or, with `DecoderConfig(attention="packed")`, the HIP kernels of
 `kernels.attention_cuda.packed_attention`, which are deterministic. The MLP cache budget
@@ -26,7 +27,7 @@ from torch.nn import functional as F
 
 from .lora import Projection
 from .mlp import MLP
-from .norm import RMSNorm
+from .norm import LayerNorm, RMSNorm
 
 
 @dataclass
@@ -41,8 +42,11 @@ class DecoderConfig:
     partial_rotary_factor: float = 0.5
     rms_norm_eps: float = 1e-6
     attention: str = "sdpa"   # or "packed"
+    norm: str = "rms"         # or "layer"
 
     def __post_init__(self):
+        if self.norm not in ("rms", "layer"):
+            raise ValueError(f"norm is 'rms' or 'layer', not {self.norm!r}")
         if self.attention not in ("sdpa", "packed"):
             raise ValueError(f"attention is 'sdpa' or 'packed', not {self.attention!r}")
 
@@ -142,15 +146,27 @@ class Attention(nn.Module):
         return project_group((self.o_proj,), y, residual=residual)[0]
 
 
+class _FrozenLayerNorm(LayerNorm):
+    """A layer norm in a pre-norm's place: its input gradient is always its own."""
+
+    def forward(self, x, *, reuse_grad=False):
+        return super().forward(x)
+
+
+def _norm(config, device):
+    kind = RMSNorm if config.norm == "rms" else _FrozenLayerNorm
+    return kind(config.hidden_size, config.rms_norm_eps, torch.bfloat16, device)
+
+
 class Layer(nn.Module):
     def __init__(self, config, *, rank, device=None):
         super().__init__()
         self.self_attn = Attention(config, rank=rank, device=device)
         self.mlp = MLP(config.hidden_size, config.intermediate_size, rank=rank, device=device)
-        self.input_layernorm = RMSNorm(config.hidden_size, config.rms_norm_eps, torch.bfloat16, device)
-        self.post_attention_layernorm = RMSNorm(config.hidden_size, config.rms_norm_eps, torch.bfloat16, device)
+        self.input_layernorm = _norm(config, device)
+        self.post_attention_layernorm = _norm(config, device)
         for norm in (self.input_layernorm, self.post_attention_layernorm):
-            norm.weight.requires_grad_(False)
+            norm.requires_grad_(False)
 
     def forward(self, x, cosine, sine, records):
         from ..kernels.mlp_cuda import tiled_lora_mlp
@@ -159,7 +175,8 @@ class Layer(nn.Module):
 
 
 class Decoder(nn.Module):
-    """Embedding, layers, final norm and a frozen head; `loss` returns the weighted CE sum."""
+    """Embedding, layers, final norm and a frozen head; `loss` returns the weighted CE sum,
+    `distillation_loss` the weighted divergence from a teacher's top logits."""
 
     def __init__(self, config, *, rank, device=None):
         super().__init__()
@@ -167,7 +184,7 @@ class Decoder(nn.Module):
         self.embed_tokens = nn.Embedding(config.vocab_size, config.hidden_size, dtype=torch.bfloat16, device=device)
         self.layers = nn.ModuleList([Layer(config, rank=rank, device=device)
                                      for _ in range(config.num_hidden_layers)])
-        self.norm = RMSNorm(config.hidden_size, config.rms_norm_eps, torch.bfloat16, device)
+        self.norm = _norm(config, device)
         self.lm_head = nn.Linear(config.hidden_size, config.vocab_size, bias=False, dtype=torch.bfloat16,
                                  device=device)
         for name, parameter in self.named_parameters():
@@ -206,7 +223,17 @@ class Decoder(nn.Module):
                 x = layer(x, cosine, sine, records)
         return self.norm(x)
 
-    def loss(self, ids, targets, weights, records, *, token_budget=128, mlp_cache_bytes=0, projection_bytes=0):
+    def loss(self, ids, targets, weights, records, *, token_budget=128, mlp_cache_bytes=0, projection_bytes=0,
+             implementation="fused"):
         from ..kernels.loss import projection_loss
         hidden = self.hidden(ids, records, mlp_cache_bytes=mlp_cache_bytes, projection_bytes=projection_bytes)
-        return projection_loss(hidden, self.lm_head.weight, targets, weights, token_budget=token_budget)
+        return projection_loss(hidden, self.lm_head.weight, targets, weights, token_budget=token_budget,
+                               implementation=implementation)
+
+    def distillation_loss(self, ids, indices, values, weights, records, *, temperature=1.0, log_normalizer=None,
+                          mlp_cache_bytes=0, projection_bytes=0):
+        """`kernels.loss.distillation_loss` of the final hidden states."""
+        from ..kernels.loss import distillation_loss
+        hidden = self.hidden(ids, records, mlp_cache_bytes=mlp_cache_bytes, projection_bytes=projection_bytes)
+        return distillation_loss(hidden, self.lm_head.weight, indices, values, weights, temperature=temperature,
+                                 log_normalizer=log_normalizer)

@@ -1,4 +1,5 @@
-"""The decoder's RMSNorm module (interface of the reference's modeling/model.py:38-64).
+"""The decoder's RMSNorm module (interface of the reference's modeling/model.py:38-64), and layer
+normalization beside it (`layer_norm`, `LayerNorm`), which the reference's decoder has not.
 
 Device inputs run `kernels.core_cuda.RMS` (HIP kernels); host inputs the plain formula in
 fp32, rounded to the input dtype and multiplied by the weight in that dtype.
@@ -52,3 +53,52 @@ class RMSNorm(nn.Module):
         from ..kernels.core_cuda import RMS
         reconstruct = bool(reuse_grad and torch.is_grad_enabled() and self._can_reconstruct(x.dtype))
         return RMS.apply(x, self.weight, self.eps, reuse_grad, reconstruct)
+
+
+def _host_layer_norm(x, weight, bias, eps):
+    wide = x.to(torch.promote_types(x.dtype, torch.float32))
+    centred = wide - wide.mean(-1, keepdim=True)
+    y = centred * torch.rsqrt(centred.square().mean(-1, keepdim=True) + eps)
+    y = y if weight is None else y * weight.to(y.dtype)
+    y = y if bias is None else y + bias.to(y.dtype)
+    return y.to(x.dtype)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension, in float32 and
+    rounded once to x's dtype. x is bf16, f16 or float32 on the device; weight and bias, each optional, are
+    vectors of its width, of any of these types. Differentiable in all three (once, in reverse; host
+    tensors in every way that torch offers); the gradients of weight and bias are summed over the
+    rows in a fixed order."""
+    width = x.shape[-1] if x.dim() else 0
+    if not width:
+        raise ValueError("layer_norm: rows of no width")
+    if not x.is_floating_point():
+        raise ValueError("layer_norm: a tensor of a floating type required")
+    for name, vector in (("weight", weight), ("bias", bias)):
+        if vector is None:
+            continue
+        if vector.shape != (width,):
+            raise ValueError(f"layer_norm: {name} {tuple(vector.shape)} for rows of {width}")
+        if vector.device != x.device:
+            raise ValueError(f"layer_norm: {name} is on {vector.device}, x on {x.device}")
+    eps = float(eps)
+    if not 0 <= eps < float("inf"):
+        raise ValueError(f"layer_norm: eps {eps} is negative or not finite")
+    if not x.is_cuda:
+        return _host_layer_norm(x, weight, bias, eps)
+    from ..kernels.core_cuda import layer_norm_device
+    return layer_norm_device(x, weight, bias, eps)
+
+
+class LayerNorm(nn.Module):
+    """`layer_norm` with its own weight (ones) and bias (zeros, or None)."""
+
+    def __init__(self, size, eps, dtype, device, *, bias=True):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(size, dtype=dtype, device=device))
+        self.bias = nn.Parameter(torch.zeros(size, dtype=dtype, device=device)) if bias else None
+        self.eps = eps
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)

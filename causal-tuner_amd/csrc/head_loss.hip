@@ -1,0 +1,1307 @@
+// The head's loss over a large vocabulary, walked in pieces, gfx950: cross-entropy to one label,
+// or to a teacher's top entries, of softmax(h W^T / T) without the logits ever being held.
+//
+// With l_iv = h_i . w_v / T, Z_i = sum_v exp(l_iv), a row's targets (v_k, q_k), k < K, distinct and
+// sorted, mass Q = sum_k q_k and entropy term H = sum_k q_k log q_k:
+//
+//   loss  = sum_i c_i (H_i + sum_k q_ik (log Z_i - l_iv_k))
+//   dh_i  = c_i / T (Q_i / Z_i sum_v exp(l_iv) w_v - sum_k q_ik w_v_k)
+//   dW_v  = sum_i c_i / T (Q_i exp(l_iv) / Z_i - q_iv) h_i
+//
+// A hard label is K = 1, q = 1, H = 0. The hidden gradient is attention with the head as keys and
+// values, so the forward makes it in the same sweep over the vocabulary, piece by piece: one
+// product writes E = 2^(l log2 e - c), rounded to the inputs' type, beside the sums of a running
+// softmax; the next adds E W_piece to a float32 accumulator per row; Z divides at the end. The
+// targets' own terms are left out of E and of the sums, and their coefficients Q p_k - q_k formed in
+// double from their logits and the others' sum: for a label of probability near one, 1 - p is not the
+// difference of two roundings. The backward adds them in float32. The head's gradient needs the
+// finished Z: the backward forms the logits of a piece again, E becomes the derivative itself, and
+// a second product multiplies it with the hidden rows.
+//
+// bf16. Both products run on v_mfma_f32_16x16x32_bf16 with one operand, the left one of every
+// product, stored in the order in which the lanes take it ("packed": 1 KB per 16 rows x 32
+// reduction indices, lane l's 16 bytes at 16 l), so that it goes from global memory to registers
+// with whole-line loads and never through LDS; only the other operand is staged there. The logits
+// kernel writes E packed for the product that follows straight from its accumulators: a lane holds
+// 4 + 4 values of one row, which become one 16-byte unit. That fixes the order of the reduction
+// indices inside a block of 32 (unit q holds indices 4 q .. + 3 and 16 + 4 q .. + 3), and the
+// product that follows reads its LDS tile in that order.
+//
+// float32. The products are ct_gemm_f32's over a piece of logits in the workspace, with a row pass
+// between them.
+//
+// Every sum runs in a fixed order: repeated calls are bit-identical.
+
+#include <math.h>
+
+#include "gemm_common.hpp"
+
+namespace ct {
+namespace {
+
+constexpr int kStep = 64;              // reduction indices per step of a product
+constexpr int kUnit = 128;             // vocabulary entries per (row, unit) pair of statistics
+constexpr int kMaxEntries = 1024;
+constexpr int64_t kMaxWidth = 65536, kMaxVocab = (int64_t{1} << 31) - 1024, kMaxRows = int64_t{1} << 30;
+// E of one piece, in bytes: what two passes over it can share through the 256 MB last-level cache.
+constexpr int64_t kPieceBytes = int64_t{256} << 20;
+constexpr float kNone = -3e38f;        // the shift of a row or unit without a finite logit
+constexpr int kNoEntry = 0x7fffffff;
+
+__host__ __device__ constexpr int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// ------------------------------------------------------------------------- plan of a call
+struct Plan {
+    int64_t rows, width, vocab, entries;
+    int dtype, bp, bl;      // a workgroup's packed rows and vocabulary entries (or columns)
+    int64_t rows_pad, width_pad, units;
+    int64_t piece, pieces;  // vocabulary entries per piece of the sweep
+    int splits;             // of the hidden gradient's reduction
+};
+
+// Workgroups' worth of work in whole rounds: how many splits of a reduction of `steps` leave the
+// fewest compute units idle, each further split paying for another pass over the sums.
+int splits_for(int64_t tiles, int64_t slots, int64_t steps) {
+    int best = 1;
+    double most = 0;
+    for (int s = 1; s <= 64 && s <= (steps + 3) / 4; ++s) {
+        const double work = (double)tiles * s, rounds = (double)((int64_t)(work + slots - 1) / slots);
+        const double gain = work / (rounds * slots) - 0.02 * (s - 1) * (tiles >= 32 ? 1 : 0.1);
+        if (gain > most + 1e-9) {
+            most = gain;
+            best = s;
+        }
+    }
+    return best;
+}
+
+Plan plan_of(int64_t rows, int64_t width, int64_t vocab, int64_t entries, int dtype) {
+    Plan p{};
+    p.rows = rows;
+    p.width = width;
+    p.vocab = vocab;
+    p.entries = entries;
+    p.dtype = dtype;
+    p.bp = rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    p.bl = p.bp == 64 ? 128 : 256;
+    p.rows_pad = up(rows, p.bp);
+    p.width_pad = up(width, kStep);
+    p.units = cdiv(vocab, kUnit);
+    const int64_t element = dtype == CT_F32 ? 4 : 2;
+    int64_t most = kPieceBytes / (p.rows_pad * element) / 256 * 256;
+    if (most < 1024) most = 1024;
+    p.pieces = cdiv(vocab, most);
+    p.piece = up(cdiv(vocab, p.pieces), 256);
+    p.pieces = cdiv(vocab, p.piece);
+    p.splits = 1;
+    if (dtype == CT_BF16) {
+        const int64_t tiles = p.rows_pad / p.bp * cdiv(width, p.bl);
+        p.splits = splits_for(tiles, p.bp == 256 ? 256 : 512, p.piece / kStep);
+    }
+    return p;
+}
+
+// What a call keeps for its backward, and its scratch: regions of one buffer each.
+struct Regions {
+    int64_t at = 0;
+    int64_t take(int64_t bytes) {
+        const int64_t start = at;
+        at += up(bytes, 256);
+        return start;
+    }
+};
+struct Kept {
+    int64_t index, q, chosen, first, shift, total, weight, mass, entropy, sums, bytes;
+};
+Kept kept_of(const Plan &p, bool hidden_grad) {
+    Regions r;
+    Kept k{};
+    k.index = r.take(p.rows * p.entries * 4);
+    k.q = r.take(p.rows * p.entries * 4);
+    k.chosen = r.take(p.rows * p.entries * 4);       // the targets' logits, later their coefficients
+    k.first = r.take(p.rows_pad * (p.units + 1) * 2);
+    k.shift = r.take(p.rows_pad * 4);                // c
+    k.total = r.take(p.rows_pad * 4);                // Z 2^-c
+    k.weight = r.take(p.rows_pad * 4);
+    k.mass = r.take(p.rows_pad * 4);
+    k.entropy = r.take(p.rows_pad * 4);
+    k.sums = r.take(hidden_grad ? (int64_t)p.splits * p.rows * p.width * 4 : 0);
+    k.bytes = r.at;
+    return k;
+}
+struct Scratch {
+    int64_t packed, plain, piece, stats, factor, inverse, near, losses, bytes;
+};
+// sweep 0: statistics alone, 1: with the hidden gradient's sums, 2: the head's gradient.
+Scratch scratch_of(const Plan &p, int sweep) {
+    Regions r;
+    Scratch s{};
+    const bool wide = p.dtype == CT_F32;
+    s.packed = r.take(wide ? 0 : p.rows_pad * p.width_pad * 2);
+    s.plain = r.take(wide ? p.rows * p.width * 4 : sweep == 2 ? p.rows * p.width * 2 : 0);
+    s.piece = r.take(wide ? p.rows * p.piece * 4 : sweep ? p.rows_pad * p.piece * 2 : 0);
+    s.stats = r.take(wide || sweep == 2 ? 0 : (sweep ? p.piece / kUnit : up(p.units, 2)) * p.rows_pad * 8);
+    s.factor = r.take(p.rows_pad * 4);
+    s.inverse = r.take(p.rows_pad * 4);
+    s.near = r.take(p.rows_pad * 4);
+    s.losses = r.take(p.rows * 8);
+    s.bytes = r.at;
+    return s;
+}
+
+// ------------------------------------------------------------------------- targets
+struct Targets {
+    const int64_t *rows;       // which rows of the tables, or null
+    int64_t tokens;            // rows of the tables
+    const int64_t *indices;    // [*, entries], row pitch ld
+    const float *values;       // the teacher's logits, or null: hard labels
+    const float *normalizer;   // the teacher's log normalizer per row, or null
+    const float *weights;
+    int64_t ld_indices, ld_values;
+};
+
+// A float sum over the workgroup, in a fixed order.
+template <int THREADS>
+__device__ __forceinline__ float block_sum(float v, float *lds) {
+    lds[threadIdx.x] = v;
+    __syncthreads();
+    for (int h = THREADS / 2; h > 0; h >>= 1) {
+        if (threadIdx.x < h) lds[threadIdx.x] += lds[threadIdx.x + h];
+        __syncthreads();
+    }
+    const float sum = lds[0];
+    __syncthreads();
+    return sum;
+}
+template <int THREADS>
+__device__ __forceinline__ float block_max(float v, float *lds) {
+    lds[threadIdx.x] = v;
+    __syncthreads();
+    for (int h = THREADS / 2; h > 0; h >>= 1) {
+        if (threadIdx.x < h) lds[threadIdx.x] = fmaxf(lds[threadIdx.x], lds[threadIdx.x + h]);
+        __syncthreads();
+    }
+    const float top = lds[0];
+    __syncthreads();
+    return top;
+}
+
+// One workgroup per row: q of its entries, sorted by index with equal indices joined, the entries
+// outside the vocabulary dropped; `first` [row][unit] counts the entries before each unit. Rows of
+// the padding get no entries and no weight.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void targets_kernel(Targets t, int64_t rows, int entries, int64_t vocab,
+                                                          int64_t units, double inverse_t, int *__restrict__ index,
+                                                          float *__restrict__ q_out, float *__restrict__ chosen,
+                                                          uint16_t *__restrict__ first, float *__restrict__ weight,
+                                                          float *__restrict__ mass, float *__restrict__ entropy,
+                                                          float *__restrict__ shift, float *__restrict__ total) {
+    __shared__ uint64_t key[kMaxEntries];
+    __shared__ float value[kMaxEntries], lds[THREADS];
+    __shared__ int sorted[kMaxEntries], kept;
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    if (tid == 0) {
+        shift[row] = kNone;
+        total[row] = 0.f;
+    }
+    const int64_t from = row < rows && t.rows ? t.rows[row] : row;
+    if (row >= rows || from < 0 || from >= t.tokens) {
+        if (row < rows)
+            for (int e = tid; e < entries; e += THREADS) {
+                index[row * entries + e] = kNoEntry;
+                q_out[row * entries + e] = chosen[row * entries + e] = 0.f;
+            }
+        for (int64_t u = tid; u <= units; u += THREADS) first[row * (units + 1) + u] = 0;
+        if (tid == 0) weight[row] = mass[row] = entropy[row] = 0.f;
+        return;
+    }
+    if (!t.values) {  // one hard label
+        const int64_t label = t.indices[from * t.ld_indices];
+        const bool there = label >= 0 && label < vocab;
+        for (int64_t u = tid; u <= units; u += THREADS)
+            first[row * (units + 1) + u] = there && label < u * kUnit ? 1 : 0;
+        if (tid == 0) {
+            index[row] = there ? (int)label : kNoEntry;
+            q_out[row] = there ? 1.f : 0.f;
+            chosen[row] = 0.f;
+            weight[row] = t.weights[from];
+            mass[row] = 1.f;
+            entropy[row] = 0.f;
+        }
+        return;
+    }
+    int size = 1;
+    while (size < entries) size <<= 1;
+    float top = -INFINITY;
+    for (int e = tid; e < size; e += THREADS) {
+        uint64_t k = ~uint64_t{0};
+        if (e < entries) {
+            const int64_t at = t.indices[from * t.ld_indices + e];
+            if (at >= 0 && at < vocab) {
+                k = (uint64_t)at << 32 | (uint32_t)e;
+                const float v = (float)((double)t.values[from * t.ld_values + e] * inverse_t);
+                value[e] = v;
+                top = fmaxf(top, v);
+            }
+        }
+        key[e] = k;
+    }
+    if (t.normalizer) {
+        top = t.normalizer[from];
+    } else {
+        top = block_max<THREADS>(top, lds);
+        if (top == -INFINITY) top = 0.f;   // no entry holds any mass
+    }
+    __syncthreads();
+    float sum = 0.f;
+    for (int e = tid; e < entries; e += THREADS)
+        if (key[e] != ~uint64_t{0}) {
+            value[e] = value[e] - top;
+            sum += expf(value[e]);
+        }
+    sum = block_sum<THREADS>(sum, lds);
+    const float norm = t.normalizer || sum == 0.f ? 0.f : logf(sum);
+    for (int width = 2; width <= size; width <<= 1)   // bitonic, ascending
+        for (int stride = width / 2; stride > 0; stride >>= 1) {
+            __syncthreads();
+            for (int e = tid; e < size; e += THREADS) {
+                const int other = e ^ stride;
+                if (other > e) {
+                    const uint64_t a = key[e], b = key[other];
+                    if ((a > b) == ((e & width) == 0)) {
+                        key[e] = b;
+                        key[other] = a;
+                    }
+                }
+            }
+        }
+    __syncthreads();
+    // The first of equal indices takes their sum; its place is the count of firsts before it.
+    if (tid == 0) {
+        int n = 0;
+        for (int e = 0; e < size && key[e] != ~uint64_t{0}; ++e)
+            if (e == 0 || (key[e] >> 32) != (key[e - 1] >> 32)) sorted[n++] = e;
+        kept = n;
+    }
+    __syncthreads();
+    float held = 0.f, ent = 0.f;
+    for (int n = tid; n < entries; n += THREADS) {
+        const int64_t to = row * entries + n;
+        chosen[to] = 0.f;
+        if (n >= kept) {
+            index[to] = kNoEntry;
+            q_out[to] = 0.f;
+            continue;
+        }
+        const int e = sorted[n], at = (int)(key[e] >> 32);
+        const int next = n + 1 < kept ? sorted[n + 1] : size;
+        float log_q = value[(uint32_t)key[e]] - norm, q = expf(log_q);
+        bool joined = false;
+        for (int m = e + 1; m < next && (int)(key[m] >> 32) == at && key[m] != ~uint64_t{0}; ++m) {
+            q += expf(value[(uint32_t)key[m]] - norm);
+            joined = true;
+        }
+        if (joined) log_q = logf(q);
+        index[to] = at;
+        q_out[to] = q;
+        held += q;
+        if (q != 0.f) ent += q * log_q;
+    }
+    held = block_sum<THREADS>(held, lds);
+    ent = block_sum<THREADS>(ent, lds);
+    if (tid == 0) {
+        weight[row] = t.weights[from];
+        mass[row] = held;
+        entropy[row] = ent;
+    }
+    for (int64_t u = tid; u <= units; u += THREADS) {
+        int lo = 0, hi = kept;   // entries with an index below u * kUnit
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if ((int64_t)(key[sorted[mid]] >> 32) < u * kUnit) lo = mid + 1;
+            else hi = mid;
+        }
+        first[row * (units + 1) + u] = (uint16_t)lo;
+    }
+}
+
+// ------------------------------------------------------------------------- packing
+// The row of `hidden` that row i of the loss is, or -1.
+struct Source {
+    const void *x;
+    const int64_t *rows;
+    int64_t ld, count, tokens, width;   // width: columns of x, zeros past them
+    __device__ __forceinline__ int64_t row(int64_t i) const {
+        if (i >= count) return -1;
+        const int64_t r = rows ? rows[i] : i;
+        return r >= 0 && r < tokens ? r : -1;
+    }
+};
+
+// Hidden rows in the order of a product's packed operand, zeros past the rows and the width.
+template <bool VEC>
+__global__ __launch_bounds__(256) void pack_rows(Source src, int64_t blocks, uint4 *__restrict__ out, int64_t units) {
+    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (u >= units) return;
+    const int lane = (int)(u & 63);
+    const int64_t block = u >> 6, kb = block % blocks, row = src.row(block / blocks * 16 + (lane & 15));
+    const int64_t k = kb * 32 + (lane >> 4) * 8;
+    const uint16_t *x = static_cast<const uint16_t *>(src.x) + row * src.ld;
+    uint4 v = zero4();
+    if (row >= 0) {
+        if constexpr (VEC) {
+            if (k < src.width) v = *reinterpret_cast<const uint4 *>(x + k);
+        } else {
+            uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (k + i < src.width) w[i / 2] |= (uint32_t)x[k + i] << (16 * (i & 1));
+            v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    out[u] = v;
+}
+
+// The same rows one after the other, `pitch` columns each.
+template <class T>
+__global__ __launch_bounds__(256) void gather_rows(Source src, T *__restrict__ out, int64_t pitch) {
+    const int64_t row = src.row(blockIdx.x);
+    const T *x = static_cast<const T *>(src.x) + row * src.ld;
+    for (int64_t c = threadIdx.x; c < pitch; c += 256)
+        out[blockIdx.x * pitch + c] = row >= 0 && c < src.width ? x[c] : T(0);
+}
+
+// ------------------------------------------------------------------------- the product's core
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+// Workgroup `id` of np x nl tiles: each of the 8 XCDs walks a contiguous range, in groups of four
+// packed tiles that share the other operand's tile in its L2.
+__device__ __forceinline__ void tile_of(int64_t id, int64_t np, int64_t nl, int64_t &tp, int64_t &tl) {
+    const int64_t total = np * nl, share = total / 8, more = total % 8, x = id & 7, i = id >> 3;
+    const int64_t t = x < more ? x * (share + 1) + i : more * (share + 1) + (x - more) * share + i;
+    const int64_t size = 4 * nl, group = t / size, at = t - group * size;
+    const int64_t count = np - group * 4 < 4 ? np - group * 4 : 4;
+    tp = group * 4 + at % count;
+    tl = at / count;
+}
+
+// acc[f][j] += fragment f of the staged operand x fragment j of the packed one, over reduction
+// steps [beg, end). WP x WL waves, each of PF x LF fragments of 16. KT: the staged operand is
+// stored with the reduction index as its row (as values in attention are), in LDS too, and its
+// fragments come from transposing reads; else its rows are reduction-contiguous. SWAP: the staged
+// operand is the MFMA's first, so a lane holds four of its consecutive rows for one packed row;
+// otherwise four packed rows for one of the staged ones.
+template <int WP, int WL, int PF, bool KT, bool SWAP>
+struct Core {
+    static constexpr int LF = 8, BP = WP * PF * 16, BL = WL * LF * 16, THREADS = 64 * WP * WL;
+    static constexpr int kPer = BL * 8 / THREADS;   // 16-byte units of a stage per thread
+    static constexpr int kStage = BL * 8;           // units per stage
+
+    const char *base;      // the staged operand at step 0 ...
+    int64_t bytes, advance;  // ... the bytes from there to its end, and from one step to the next
+    uint32_t off[kPer];
+    int k[kPer];           // KC: the unit's first index of a step; KT: its row
+    int limit;             // of k
+    const uint4 *a;        // the wave's packed rows at step 0
+    int64_t a_row;         // units between two blocks of packed rows
+
+    // base: the staged operand at the tile's first row (KC) or column (KT); `extent` its rows from
+    // there (KC) or columns (KT), `depth` the reduction's extent.
+    __device__ __forceinline__ void init(const uint16_t *first, int64_t ld, int64_t extent, int64_t depth,
+                                         const uint4 *packed, int64_t block, int64_t blocks) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wp = wave % WP;
+        limit = (int)depth;
+        base = reinterpret_cast<const char *>(first);
+        if constexpr (KT) {
+            bytes = ((depth - 1) * ld + (extent < BL ? up(extent, 8) : BL)) * 2;   // rows are whole units
+            advance = kStep * ld * 2;
+        } else {
+            bytes = (((extent < BL ? extent : BL) - 1) * ld + depth) * 2;
+            advance = kStep * 2;
+        }
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) {
+            const int u = tid + c * THREADS;
+            if constexpr (KT) {
+                const int row = u / (BL / 8), chunk = u % (BL / 8);
+                off[c] = chunk * 8 < extent ? (uint32_t)((row * ld + chunk * 8) * 2) : kOOB;
+                k[c] = row;
+            } else {
+                const int row = u >> 3, chunk = u & 7;
+                off[c] = row < extent ? (uint32_t)((row * ld + chunk * 8) * 2) : kOOB;
+                k[c] = chunk * 8;
+            }
+        }
+        a = packed + (block + wp * PF) * blocks * 64 + lane;
+        a_row = blocks * 64;
+    }
+    __device__ __forceinline__ void load_b(int step, uint4 (&r)[kPer]) const {
+        // a descriptor per step: offsets stay within a step, whatever the operand's size
+        const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(base + step * advance, bytes - step * advance);
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) r[c] = buf_load16(rsrc, step * kStep + k[c] < limit ? off[c] : kOOB);
+    }
+    __device__ __forceinline__ void load_a(int step, uint4 (&f)[2][PF]) const {
+#pragma unroll
+        for (int j = 0; j < PF; ++j)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) f[ks][j] = a[j * a_row + (int64_t)(step * 2 + ks) * 64];
+    }
+    __device__ __forceinline__ static void store_b(uint4 *stage, const uint4 (&r)[kPer]) {
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) {
+            const int u = threadIdx.x + c * THREADS;
+            if constexpr (KT) {
+                const int row = u / (BL / 8), chunk = u % (BL / 8);
+                stage[row * (BL / 8) + ((chunk >> 1 ^ (row & 7)) << 1 | (chunk & 1))] = r[c];
+            } else {
+                stage[slot(u >> 3, u & 7)] = r[c];
+            }
+        }
+    }
+    __device__ __forceinline__ static uint4 fragment(const uint4 *stage, int f, int ks, int wl, int lane) {
+        const int c0 = (wl * LF + f) * 16;
+        if constexpr (KT) {
+            const int j = lane & 15, row = 4 * (lane >> 4) + (j >> 2);
+            const __attribute__((address_space(3))) char *p =
+                (const __attribute__((address_space(3))) char *)stage + (ks * 32 + row) * (BL * 2) +
+                ((c0 >> 4 ^ (row & 7)) << 5) + ((j & 3) << 3);
+            const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)p);
+            const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(p + 16 * (BL * 2)));
+            const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+            return make_uint4(l2.x, l2.y, h2.x, h2.y);
+        } else {
+            return stage[slot(c0 + (lane & 15), ks * 4 + (lane >> 4))];
+        }
+    }
+    // One step: stage `cur` and the fragments `af` are multiplied while `b` (the next step's) goes
+    // to stage `nxt`, the one after it is loaded into b and the next step's fragments into `an`.
+    __device__ __forceinline__ void step(int t, const uint4 *cur, uint4 *nxt, const uint4 (&af)[2][PF],
+                                         uint4 (&an)[2][PF], uint4 (&b)[kPer], int last, f32x4 (&acc)[LF][PF], int wl,
+                                         int lane) const {
+        load_a(t + 1 < last ? t + 1 : t, an);
+        store_b(nxt, b);
+        load_b(t + 2, b);
+#pragma unroll
+        for (int f = 0; f < LF; ++f) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const uint4 lf = fragment(cur, f, ks, wl, lane);
+#pragma unroll
+                for (int j = 0; j < PF; ++j)
+                    acc[f][j] = SWAP ? mfma16x16x32(lf, af[ks][j], acc[f][j]) : mfma16x16x32(af[ks][j], lf, acc[f][j]);
+            }
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ void run(int beg, int end, uint4 *s0, uint4 *s1, f32x4 (&acc)[LF][PF]) const {
+        const int lane = threadIdx.x & 63, wl = (threadIdx.x >> 6) / WP;
+#pragma unroll
+        for (int f = 0; f < LF; ++f)
+#pragma unroll
+            for (int j = 0; j < PF; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (beg >= end) return;
+        uint4 b[kPer], a0[2][PF], a1[2][PF];
+        load_b(beg, b);
+        load_a(beg, a0);
+        store_b(s0, b);
+        load_b(beg + 1, b);
+        __syncthreads();
+        int t = beg;
+        for (; t + 1 < end; t += 2) {
+            step(t, s0, s1, a0, a1, b, end, acc, wl, lane);
+            step(t + 1, s1, s0, a1, a0, b, end, acc, wl, lane);
+        }
+        if (t < end) step(t, s0, s1, a0, a1, b, end, acc, wl, lane);
+    }
+};
+
+// ------------------------------------------------------------------------- logits of a piece
+enum { STATS = 0, EXP = 1, GRAD = 2 };
+
+struct LogitsParams {
+    const uint16_t *head;
+    int64_t ld, width, vocab;
+    const uint4 *packed;       // hidden rows
+    int64_t blocks;            // of 32 along the width
+    int64_t v0, v1;            // the piece's entries
+    int64_t np, nl;            // tiles
+    float scale;               // log2(e) / T
+    uint4 *piece;              // EXP: E, GRAD: the derivative, packed
+    int64_t piece_blocks;      // EXP: of 32 entries; GRAD: of 32 rows
+    float2 *stats;             // [unit of the piece][row]
+    int64_t rows_pad, rows;
+    const int *index;
+    const uint16_t *first;
+    float *chosen;             // the targets' logits (written); GRAD: their coefficients (read)
+    int entries;
+    int64_t units;
+    const float *shift, *factor, *inverse;   // GRAD: of row_factors
+};
+
+// The shift of a unit whose largest scaled logit is `top` (a whole number): one of ..., -128, -32,
+// 64, ..., at most 80 below it and less than 16 above, so that units whose largest logits lie within
+// 33 of zero share theirs and nothing is rescaled. E reaches 2^80, and holds what is down to 2^-110 of
+// the unit's maximum.
+__device__ __forceinline__ float shift_of(float top) {
+    return fabsf(top) < 1e6f ? 96.f * ceilf((top - 48.f) * (1.f / 96.f)) - 32.f : top;
+}
+
+// A wave's entries: which of its 64 (or 16 PF) rows x 128 vocabulary entries are targets, as bits in
+// LDS [row][4], one lane per row.
+template <int ROWS>
+__device__ __forceinline__ void mark_targets(const LogitsParams &p, int64_t row0, int64_t unit, uint32_t *bits, int lane) {
+    if (lane < ROWS) {
+        uint32_t w[4] = {0, 0, 0, 0};
+        const int64_t row = row0 + lane;
+        if (row < p.rows && unit < p.units) {
+            const uint16_t *at = p.first + row * (p.units + 1) + unit;
+            for (int e = at[0]; e < at[1]; ++e) {
+                const int v = p.index[row * p.entries + e] & (kUnit - 1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (v >> 5 == i) w[i] |= 1u << (v & 31);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bits[lane * 4 + i] = w[i];
+    }
+}
+
+// The place among a row's sorted entries of the one at `bit` (0 .. 127) of unit `unit`.
+__device__ __forceinline__ int64_t place_of(const LogitsParams &p, int64_t row, int64_t unit, const uint32_t *bits, int bit) {
+    int n = p.first[row * (p.units + 1) + unit];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i <= bit >> 5) n += __builtin_popcount(i < bit >> 5 ? bits[i] : bits[i] & ((1u << (bit & 31)) - 1));
+    return row * p.entries + n;
+}
+
+template <int WP, int WL, int PF, int MODE>
+__global__ __launch_bounds__(64 * WP * WL) void logits_kernel(const LogitsParams p) {
+    using C = Core<WP, WL, PF, false, MODE != GRAD>;
+    __shared__ uint4 s0[C::kStage], s1[C::kStage];
+    __shared__ uint32_t marks[WP * WL][PF * 16 * 4];
+    int64_t tp, tl;
+    tile_of(blockIdx.x, p.np, p.nl, tp, tl);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wp = wave % WP, wl = wave / WP, q = lane >> 4;
+    const int64_t v0 = p.v0 + tl * C::BL, left = p.v1 - v0;
+    C core;
+    core.init(p.head + v0 * p.ld, p.ld, left, p.width, p.packed, tp * (C::BP / 16), p.blocks);
+    f32x4 acc[C::LF][PF];
+    core.run(0, (int)(p.blocks / 2), s0, s1, acc);
+
+    const int64_t row0 = tp * C::BP + wp * PF * 16, u0 = v0 + wl * kUnit, unit = u0 / kUnit;
+    uint32_t *bits = marks[wave];
+    mark_targets<PF * 16>(p, row0, unit, bits, lane);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the lanes read each other's marks
+    const int valid = (int)(p.v1 - u0 < kUnit ? (p.v1 > u0 ? p.v1 - u0 : 0) : kUnit);
+
+    if constexpr (MODE == GRAD) {
+        // lane: entry l % 16 of fragment f, rows 4 q + i of packed fragment j
+#pragma unroll
+        for (int jj = 0; jj < PF; ++jj) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int local = jj * 16 + 4 * q + i;
+                const int64_t row = row0 + local;
+                const float c = p.shift[row], factor = p.factor[row];
+#pragma unroll
+                for (int f = 0; f < C::LF; ++f) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][jj][i], p.scale, -c)) * factor;
+                    acc[f][jj][i] = 16 * f + (lane & 15) < valid ? e : 0.f;
+                }
+                const uint4 m = *reinterpret_cast<const uint4 *>(bits + local * 4);
+                const uint32_t w[4] = {m.x, m.y, m.z, m.w};
+                if (__builtin_amdgcn_ballot_w64(((w[0] | w[1] | w[2] | w[3]) >> (lane & 15) & 0x00010001u) != 0)) {
+                    const float inverse = p.inverse[row];   // 0 past the rows, which have no targets
+#pragma unroll
+                    for (int f = 0; f < C::LF; ++f) {
+                        const int bit = 16 * f + (lane & 15);
+                        if (w[f >> 1] >> (bit & 31) & 1)
+                            acc[f][jj][i] = inverse * p.chosen[place_of(p, row, unit, bits + local * 4, bit)];
+                    }
+                }
+            }
+        }
+        static_assert(PF == 1 || PF % 2 == 0, "pairs of packed fragments");
+        if constexpr (PF % 2 == 0) {
+#pragma unroll
+            for (int jj = 0; jj < PF; jj += 2)
+#pragma unroll
+                for (int f = 0; f < C::LF; ++f) {
+                    const f32x4 x = acc[f][jj], y = acc[f][jj + 1];
+                    p.piece[(((u0 - p.v0) / 16 + f) * p.piece_blocks + row0 / 32 + jj / 2) * 64 + lane] =
+                        make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(y[0], y[1]),
+                                   pack_bf16x2(y[2], y[3]));
+                }
+        } else {   // half a unit: the other half is the wave's that holds the next 16 rows
+#pragma unroll
+            for (int f = 0; f < C::LF; ++f) {
+                const f32x4 x = acc[f][0];
+                uint4 *to = p.piece + (((u0 - p.v0) / 16 + f) * p.piece_blocks + row0 / 32) * 64 + lane;
+                reinterpret_cast<uint2 *>(to)[(row0 / 16) & 1] = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+            }
+        }
+    } else {
+        // lane: row l % 16 of packed fragment j, entries 4 q + i of fragment f
+        if (valid < kUnit) {
+#pragma unroll
+            for (int f = 0; f < C::LF; ++f)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (16 * f + 4 * q + i >= valid)
+#pragma unroll
+                        for (int j = 0; j < PF; ++j) acc[f][j][i] = -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < PF; ++j) {
+            const int local = j * 16 + (lane & 15);
+            const int64_t row = row0 + local;
+            const uint4 m = *reinterpret_cast<const uint4 *>(bits + local * 4);
+            const uint32_t w[4] = {m.x, m.y, m.z, m.w};
+            float top = acc[0][j][0];
+#pragma unroll
+            for (int f = 0; f < C::LF; ++f)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, acc[f][j][i]);
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            // exponents are taken relative to the unit's own maximum, where they are exact to their
+            // own size, and brought to the shift by a power of two
+            const float near = fmaxf(ceilf(top * p.scale), kNone), c = shift_of(near);
+            const float by = near == c ? 1.f : ldexpf(1.f, (int)(near - c));
+            float sum = 0.f;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {   // 32 entries: two fragments
+                float e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[2 * g + i / 4][j][i % 4], p.scale, -near));
+                }
+                const uint32_t mine = w[g] >> (4 * q) & 0x000f000fu;
+                if (mine) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (mine >> (16 * (i / 4) + i % 4) & 1) {
+                            p.chosen[place_of(p, row, unit, bits + local * 4, 32 * g + 16 * (i / 4) + 4 * q + i % 4)] =
+                                acc[2 * g + i / 4][j][i % 4];
+                            e[i] = 0.f;
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    sum += e[i];
+                    e[i] *= by;
+                }
+                if constexpr (MODE == EXP)
+                    p.piece[((row0 / 16 + j) * p.piece_blocks + (u0 - p.v0) / 32 + g) * 64 + lane] =
+                        make_uint4(pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]),
+                                   pack_bf16x2(e[6], e[7]));
+            }
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            if (q == 0) p.stats[(u0 - p.v0) / kUnit * p.rows_pad + row] = make_float2(c, sum * by);
+        }
+    }
+}
+
+// The units' statistics of a piece joined to the rows': 16 rows x 16 groups of units a workgroup.
+// A row's shift becomes the largest of its own and the units'; E of a unit with another shift is
+// brought to it, and `factor` is what the sums of the pieces before are brought to it with.
+__global__ __launch_bounds__(256) void join_kernel(const float2 *__restrict__ stats, int units, int64_t rows_pad,
+                                                   float *__restrict__ shift, float *__restrict__ total,
+                                                   float *__restrict__ factor, uint4 *piece, int64_t piece_blocks) {
+    __shared__ float part[16][17];
+    const int r = threadIdx.x & 15, g = threadIdx.x >> 4;
+    const int64_t row = (int64_t)blockIdx.x * 16 + r;
+    const float2 *at = stats + row;
+    float c = kNone;
+    for (int u = g; u < units; u += 16) c = fmaxf(c, at[u * rows_pad].x);
+    part[g][r] = c;
+    __syncthreads();
+    const float before = shift[row], held = total[row];
+    c = before;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) c = fmaxf(c, part[i][r]);
+    __syncthreads();
+    float sum = 0.f;
+    for (int u = g; u < units; u += 16) {
+        const float2 s = at[u * rows_pad];
+        if (s.x == c) {
+            sum += s.y;
+            continue;
+        }
+        const float by = __builtin_amdgcn_exp2f(s.x - c);
+        sum += s.y * by;
+        if (!piece) continue;
+        for (int i = 0; i < kUnit / 8; ++i) {   // the row's 16 units of 16 bytes
+            uint4 *e = piece + (row / 16 * piece_blocks + u * (kUnit / 32) + i / 4) * 64 + (i % 4) * 16 + r;
+            uint4 v = *e;
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                w[j] = pack_bf16x2(bf16_to_f32((uint16_t)(w[j] & 0xffffu)) * by, bf16_to_f32((uint16_t)(w[j] >> 16)) * by);
+            *e = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    part[g][r] = sum;
+    __syncthreads();
+    if (g == 0) {
+        const float by = before == c ? 1.f : __builtin_amdgcn_exp2f(before - c);
+        sum = held * by;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += part[i][r];
+        total[row] = sum;
+        shift[row] = c;
+        factor[row] = by;
+    }
+}
+
+// ------------------------------------------------------------------------- the second product
+struct ProductParams {
+    const uint16_t *b;         // [depth, cols]
+    int64_t ld, depth, cols;
+    const uint4 *packed;       // [rows, depth]
+    int64_t blocks;
+    int64_t np, nl;
+    int64_t rows;
+    void *out;
+    int64_t ldo, slab;         // elements between two splits' outputs
+    int steps_per_split, steps;
+    const float *factor;       // per row: out = factor out + sum; null: out = sum
+    int vec;
+};
+
+// out[row, col] (= factor out +) sum_k packed(row, k) b[k, col], one split of the reduction per z.
+template <int WP, int WL, int PF, int OUT>
+__global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductParams p) {
+    using C = Core<WP, WL, PF, true, true>;
+    __shared__ uint4 s0[C::kStage], s1[C::kStage];
+    int64_t tp, tl;
+    tile_of(blockIdx.x, p.np, p.nl, tp, tl);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wp = wave % WP, wl = wave / WP, q = lane >> 4;
+    const int beg = blockIdx.y * p.steps_per_split;
+    const int end = beg + p.steps_per_split < p.steps ? beg + p.steps_per_split : p.steps;
+    // the split's own range of the staged operand, so that offsets stay within 32 bits
+    C core;
+    const int64_t k0 = (int64_t)beg * kStep;
+    core.init(p.b + k0 * p.ld + tl * C::BL, p.ld, p.cols - tl * C::BL, p.depth - k0, p.packed + (int64_t)beg * 128,
+              tp * (C::BP / 16), p.blocks);
+    f32x4 acc[C::LF][PF];
+    core.run(0, end - beg, s0, s1, acc);
+#pragma unroll
+    for (int j = 0; j < PF; ++j) {
+        const int64_t row = tp * C::BP + (wp * PF + j) * 16 + (lane & 15);
+        if (row >= p.rows) continue;
+        const float factor = p.factor ? p.factor[row] : 0.f;
+#pragma unroll
+        for (int f = 0; f < C::LF; ++f) {
+            const int64_t col = tl * C::BL + (wl * C::LF + f) * 16 + 4 * q;
+            if (col >= p.cols) continue;
+            f32x4 v = acc[f][j];
+            if constexpr (OUT == CT_F32) {
+                float *o = static_cast<float *>(p.out) + blockIdx.y * p.slab + row * p.ldo + col;
+                if (p.vec && col + 4 <= p.cols) {
+                    if (p.factor) {
+                        const float4 old = *reinterpret_cast<const float4 *>(o);
+                        v[0] += factor * old.x;
+                        v[1] += factor * old.y;
+                        v[2] += factor * old.z;
+                        v[3] += factor * old.w;
+                    }
+                    *reinterpret_cast<float4 *>(o) = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+                    for (int i = 0; i < 4; ++i)
+                        if (col + i < p.cols) o[i] = p.factor ? v[i] + factor * o[i] : v[i];
+                }
+            } else {
+                uint16_t *o = static_cast<uint16_t *>(p.out) + row * p.ldo + col;
+                if (p.vec && col + 4 <= p.cols) {
+                    *reinterpret_cast<uint2 *>(o) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+                } else {
+                    for (int i = 0; i < 4; ++i)
+                        if (col + i < p.cols) o[i] = bf16_bits(v[i]);
+                }
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------- float32 row passes
+// One workgroup per row of a piece of float32 logits: the running maximum and sum; with `sums` the
+// logits become E (0 at the row's targets) and the row of the sums so far is brought to its shift.
+__global__ __launch_bounds__(256) void rows_exp_f32(float *__restrict__ logits, int64_t ld, int64_t v0, int64_t cols,
+                                                    float scale, float *__restrict__ shift, float *__restrict__ total,
+                                                    const int *__restrict__ index, const uint16_t *__restrict__ first,
+                                                    float *__restrict__ chosen, int entries, int64_t units, float *sums,
+                                                    int64_t width) {
+    __shared__ float lds[256];
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    float *l = logits + row * ld;
+    float top = -INFINITY;
+    for (int64_t c = tid; c < cols; c += 256) top = fmaxf(top, l[c]);
+    top = block_max<256>(top, lds);
+    const float before = shift[row], held = total[row];
+    const float c = fmaxf(before, fmaxf(ceilf(top * scale), kNone));
+    // pieces start at multiples of 256: whole units
+    const int e0 = first[row * (units + 1) + v0 / kUnit], e1 = first[row * (units + 1) + cdiv(v0 + cols, kUnit)];
+    for (int e = e0 + tid; e < e1; e += 256) {
+        float *at = l + index[row * entries + e] - v0;
+        chosen[row * entries + e] = *at;
+        *at = -INFINITY;
+    }
+    __syncthreads();
+    float sum = 0.f;
+    for (int64_t i = tid; i < cols; i += 256) {
+        const float e = exp2f(__builtin_fmaf(l[i], scale, -c));
+        sum += e;
+        if (sums) l[i] = e;
+    }
+    sum = block_sum<256>(sum, lds);
+    const float by = before == c ? 1.f : exp2f(before - c);
+    if (sums && by != 1.f && v0 > 0)
+        for (int64_t i = tid; i < width; i += 256) sums[row * width + i] *= by;
+    if (tid == 0) {
+        total[row] = held * by + sum;
+        shift[row] = c;
+    }
+}
+
+__global__ __launch_bounds__(256) void rows_grad_f32(float *__restrict__ logits, int64_t ld, int64_t v0, int64_t cols,
+                                                     float scale, const float *__restrict__ shift,
+                                                     const float *__restrict__ factor, const float *__restrict__ inverse,
+                                                     const int *__restrict__ index, const uint16_t *__restrict__ first,
+                                                     const float *__restrict__ coefficient, int entries, int64_t units) {
+    const int64_t row = blockIdx.x;
+    float *l = logits + row * ld;
+    const float c = shift[row], f = factor[row];
+    for (int64_t i = threadIdx.x; i < cols; i += 256) l[i] = exp2f(__builtin_fmaf(l[i], scale, -c)) * f;
+    __syncthreads();
+    const int e0 = first[row * (units + 1) + v0 / kUnit], e1 = first[row * (units + 1) + cdiv(v0 + cols, kUnit)];
+    for (int e = e0 + (int)threadIdx.x; e < e1; e += 256)
+        l[index[row * entries + e] - v0] = inverse[row] * coefficient[row * entries + e];
+}
+
+// ------------------------------------------------------------------------- the ends
+// A row's loss, the coefficients Q p_k - q_k of its targets in place of their logits, and Z with the
+// targets' own terms in place of the others' sum. In double, from the targets' exponentials and the
+// others' sum: log p_k = -log1p((Z - e_k) / e_k), Q p_k - q_k = (Q - q_k) - Q (Z - e_k) / Z.
+__global__ __launch_bounds__(64) void row_loss(const float *__restrict__ shift, float *__restrict__ total,
+                                               const float *__restrict__ weight, const float *__restrict__ mass,
+                                               const float *__restrict__ entropy, const int *__restrict__ index,
+                                               const float *__restrict__ q, float *__restrict__ chosen, int64_t rows,
+                                               int entries, double inverse_t, int hard, double *__restrict__ losses) {
+    const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x;
+    const double c = shift[row], others = total[row], held = mass[row], ln2 = 0.693147180559945309417;
+    const auto exponent = [&](int64_t at) { return (double)chosen[at] * inverse_t - c * ln2; };
+    double own = 0;
+    for (int e = lane; e < entries; e += 64)
+        if (index[row * entries + e] != kNoEntry) own += exp(exponent(row * entries + e));
+    for (int o = 32; o > 0; o >>= 1) own += __shfl_xor(own, o, 64);
+    const double z = others + own;
+    double sum = 0;
+    for (int e = lane; e < entries; e += 64) {
+        const int64_t at = row * entries + e;
+        const double qk = q[at];
+        if (index[at] == kNoEntry) {
+            if (hard) sum += log(z) + c * ln2;   // a label outside the vocabulary: the row's loss is log Z
+            chosen[at] = 0.f;
+            continue;
+        }
+        const double x = exponent(at), ek = exp(x);
+        // exact where the row has one target, which `own` then is
+        const double rest = entries == 1 || own == ek ? others : others + (own - ek);
+        if (qk != 0.0) sum += qk * (ek > 0 ? log1p(rest / ek) : log(z) - x);
+        chosen[at] = (float)((held - qk) - held * (rest / z));
+    }
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) {
+        losses[row] = held == 0.0 && !hard ? 0.0 : (double)weight[row] * (sum + (double)entropy[row]);
+        total[row] = (float)z;
+    }
+}
+
+__global__ __launch_bounds__(1024) void total_loss(const double *__restrict__ losses, int64_t rows, float *__restrict__ loss) {
+    __shared__ double lds[1024];
+    double sum = 0;
+    for (int64_t i = threadIdx.x; i < rows; i += 1024) sum += losses[i];
+    lds[threadIdx.x] = sum;
+    __syncthreads();
+    for (int h = 512; h > 0; h >>= 1) {
+        if (threadIdx.x < h) lds[threadIdx.x] += lds[threadIdx.x + h];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *loss = (float)lds[0];
+}
+
+// What the derivative of a row is made with, 0 in the padding: inverse = c_i u / T, and
+// near + log2 of (factor / inverse) = log2 (Q_i / Z_i) with a whole number `near` as close to log2 Z_i
+// as that allows, so that probabilities down to 2^-126 are held.
+__global__ __launch_bounds__(256) void row_factors(const float *__restrict__ weight, const float *__restrict__ mass,
+                                                   const float *__restrict__ shift, const float *__restrict__ total,
+                                                   const float *__restrict__ upstream, float inverse_t, int64_t rows,
+                                                   int64_t rows_pad, float *__restrict__ near, float *__restrict__ factor,
+                                                   float *__restrict__ inverse) {
+    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (row >= rows_pad) return;
+    const float f = row < rows ? weight[row] * *upstream * inverse_t : 0.f;
+    int size = 0;
+    const float z = frexpf(total[row], &size);
+    inverse[row] = f;
+    near[row] = shift[row] + (float)size;
+    factor[row] = row < rows && mass[row] != 0.f ? f * mass[row] / z : 0.f;
+}
+
+// dh_i = u c_i / T (Q_i / Z_i sums_i + sum_k coefficient_k w_v_k), the splits' sums in order. One
+// workgroup per row and 2048 columns.
+template <int IN, int OUT>
+__global__ __launch_bounds__(256) void hidden_grad_kernel(const float *__restrict__ sums, int splits, int64_t slab,
+                                                          int64_t width, const float *__restrict__ weight,
+                                                          const float *__restrict__ mass, const float *__restrict__ total,
+                                                          const float *__restrict__ upstream, float inverse_t,
+                                                          const int *__restrict__ index,
+                                                          const float *__restrict__ coefficient, int entries,
+                                                          const void *__restrict__ head, int64_t ld,
+                                                          const int64_t *__restrict__ rows, int64_t tokens,
+                                                          void *__restrict__ out, int64_t ldo, int64_t out_width) {
+    const int64_t row = blockIdx.x, to = rows ? rows[row] : row;
+    if (to < 0 || to >= tokens) return;
+    const float held = mass[row], f = weight[row] * *upstream * inverse_t;
+    const float by = held != 0.f ? held / total[row] : 0.f;
+    for (int64_t c = (int64_t)blockIdx.y * 2048 + threadIdx.x; c < out_width && c < (int64_t)(blockIdx.y + 1) * 2048; c += 256) {
+        float sum = 0.f;
+        for (int s = 0; s < splits; ++s) sum += sums[s * slab + row * width + c];
+        sum *= by;
+        for (int e = 0; e < entries; ++e) {
+            const int v = index[row * entries + e];
+            if (v == kNoEntry) break;
+            const float w = IN == CT_F32 ? static_cast<const float *>(head)[v * ld + c]
+                                         : bf16_to_f32(static_cast<const uint16_t *>(head)[v * ld + c]);
+            sum += coefficient[row * entries + e] * w;
+        }
+        sum = held != 0.f ? sum * f : 0.f;
+        if constexpr (OUT == CT_F32) static_cast<float *>(out)[to * ldo + c] = sum;
+        else static_cast<uint16_t *>(out)[to * ldo + c] = bf16_bits(sum);
+    }
+}
+
+template <class T>
+T *at(void *base, int64_t offset) {
+    return reinterpret_cast<T *>(static_cast<char *>(base) + offset);
+}
+
+template <int MODE>
+hipError_t launch_logits(const Plan &pl, const LogitsParams &p, hipStream_t s) {
+    const dim3 grid((unsigned)(p.np * p.nl));
+    if (pl.bp == 64) logits_kernel<4, 1, 1, MODE><<<grid, dim3(256), 0, s>>>(p);
+    else if (pl.bp == 128) logits_kernel<4, 2, 2, MODE><<<grid, dim3(512), 0, s>>>(p);
+    else logits_kernel<4, 2, 4, MODE><<<grid, dim3(512), 0, s>>>(p);
+    return hipGetLastError();
+}
+template <int OUT>
+hipError_t launch_product(int bp, const ProductParams &p, int splits, hipStream_t s) {
+    const dim3 grid((unsigned)(p.np * p.nl), (unsigned)splits);
+    if (bp == 64) product_kernel<4, 1, 1, OUT><<<grid, dim3(256), 0, s>>>(p);
+    else if (bp == 128) product_kernel<4, 2, 2, OUT><<<grid, dim3(512), 0, s>>>(p);
+    else product_kernel<4, 2, 4, OUT><<<grid, dim3(512), 0, s>>>(p);
+    return hipGetLastError();
+}
+
+int check(const ct_head_loss *a, bool hidden) {
+    if (!a) return -CT_EINVAL_POINTER;
+    if (a->dtype != CT_BF16 && a->dtype != CT_F32) return -CT_EINVAL_DTYPE;
+    if (a->count < 0 || a->count > kMaxRows || a->width <= 0 || a->width > kMaxWidth || a->vocab <= 0 ||
+        a->vocab > kMaxVocab || a->entries < 1 || a->entries > kMaxEntries)
+        return -CT_EINVAL_SHAPE;
+    if (a->tokens < 0 || (!a->rows && a->tokens < a->count)) return -CT_EINVAL_SHAPE;
+    if (a->hidden_width <= 0 || a->hidden_width > a->width || a->ld_hidden < a->hidden_width || a->ld_head < a->width)
+        return -CT_EINVAL_SHAPE;
+    if (!a->values && a->entries != 1) return -CT_EINVAL_SHAPE;
+    if (a->ld_indices < a->entries || (a->values && a->ld_values < a->entries)) return -CT_EINVAL_SHAPE;
+    if (!(a->temperature > 0)) return -CT_EINVAL_SHAPE;
+    if (a->count && ((hidden && !a->hidden) || !a->head || !a->indices || !a->weights)) return -CT_EINVAL_POINTER;
+    if (a->dtype == CT_BF16 && (a->width % 8 || a->ld_head % 8)) return -CT_EINVAL_SHAPE;
+    if (a->dtype == CT_BF16 && reinterpret_cast<uintptr_t>(a->head) % 16) return -CT_EINVAL_POINTER;
+    return 0;
+}
+Source source(const ct_head_loss *a) { return Source{a->hidden, a->rows, a->ld_hidden, a->count, a->tokens, a->hidden_width}; }
+// Whether the hidden rows can be read as they lie: [count, width] rows, for bf16 in 16-byte units.
+bool in_place(const ct_head_loss *a) {
+    if (a->rows || a->hidden_width != a->width) return false;
+    return a->dtype == CT_F32 || (a->ld_hidden % 8 == 0 && reinterpret_cast<uintptr_t>(a->hidden) % 16 == 0);
+}
+int check_sizes(int64_t count, int64_t width, int64_t vocab, int32_t entries, int32_t dtype) {
+    if (dtype != CT_BF16 && dtype != CT_F32) return -CT_EINVAL_DTYPE;
+    return count < 0 || count > kMaxRows || width <= 0 || width > kMaxWidth || vocab <= 0 || vocab > kMaxVocab ||
+                   entries < 1 || entries > kMaxEntries
+               ? -CT_EINVAL_SHAPE
+               : 0;
+}
+#define CT_TRY(call)                            \
+    do {                                        \
+        const hipError_t e_ = (call);           \
+        if (e_ != hipSuccess) return (int)e_;   \
+    } while (0)
+
+LogitsParams logits_params(const ct_head_loss *a, const Plan &pl, const Kept &k, const Scratch &sc, void *kept, void *ws) {
+    LogitsParams p{};
+    p.head = static_cast<const uint16_t *>(a->head);
+    p.ld = a->ld_head;
+    p.width = pl.width;
+    p.vocab = pl.vocab;
+    p.packed = at<const uint4>(ws, sc.packed);
+    p.blocks = pl.width_pad / 32;
+    p.np = pl.rows_pad / pl.bp;
+    p.scale = (float)(1.4426950408889634074 / a->temperature);
+    p.piece = at<uint4>(ws, sc.piece);
+    p.stats = at<float2>(ws, sc.stats);
+    p.rows_pad = pl.rows_pad;
+    p.rows = pl.rows;
+    p.index = at<int>(kept, k.index);
+    p.first = at<uint16_t>(kept, k.first);
+    p.chosen = at<float>(kept, k.chosen);
+    p.entries = (int)pl.entries;
+    p.units = pl.units;
+    return p;
+}
+
+hipError_t pack_hidden(const ct_head_loss *a, const Plan &pl, void *packed, hipStream_t stream) {
+    const int64_t units = pl.rows_pad / 16 * (pl.width_pad / 32) * 64;
+    const Source src = source(a);
+    const bool vec = a->hidden_width % 8 == 0 && a->ld_hidden % 8 == 0 && reinterpret_cast<uintptr_t>(a->hidden) % 16 == 0;
+    const dim3 grid((unsigned)cdiv(units, 256));
+    if (vec) pack_rows<true><<<grid, dim3(256), 0, stream>>>(src, pl.width_pad / 32, static_cast<uint4 *>(packed), units);
+    else pack_rows<false><<<grid, dim3(256), 0, stream>>>(src, pl.width_pad / 32, static_cast<uint4 *>(packed), units);
+    return hipGetLastError();
+}
+// The loss's rows one after the other: as they lie, or gathered into `to`.
+hipError_t plain_hidden(const ct_head_loss *a, const Plan &pl, void *to, const void **hidden, int64_t *ld, hipStream_t stream) {
+    if (in_place(a)) {
+        *hidden = a->hidden;
+        *ld = a->ld_hidden;
+        return hipSuccess;
+    }
+    *hidden = to;
+    *ld = pl.width;
+    const dim3 grid((unsigned)pl.rows);
+    if (a->dtype == CT_F32) gather_rows<float><<<grid, dim3(256), 0, stream>>>(source(a), static_cast<float *>(to), pl.width);
+    else gather_rows<uint16_t><<<grid, dim3(256), 0, stream>>>(source(a), static_cast<uint16_t *>(to), pl.width);
+    return hipGetLastError();
+}
+
+}  // namespace
+}  // namespace ct
+
+using namespace ct;
+
+extern "C" int64_t ct_head_loss_kept(int64_t count, int64_t width, int64_t vocab, int32_t entries, int32_t dtype,
+                                     int32_t hidden_grad) {
+    if (check_sizes(count, width, vocab, entries, dtype) || count == 0) return 0;
+    return kept_of(plan_of(count, width, vocab, entries, dtype), hidden_grad != 0).bytes;
+}
+
+extern "C" int64_t ct_head_loss_workspace(int64_t count, int64_t width, int64_t vocab, int32_t entries, int32_t dtype,
+                                          int32_t pass) {
+    if (check_sizes(count, width, vocab, entries, dtype) || count == 0 || pass < 0 || pass > 2) return 0;
+    return scratch_of(plan_of(count, width, vocab, entries, dtype), pass).bytes;
+}
+
+extern "C" int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t hidden_grad, void *kept,
+                                    int64_t kept_bytes, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
+    if (const int bad = check(a, true)) return bad;
+    if (!loss) return -CT_EINVAL_POINTER;
+    if (a->count == 0) {
+        total_loss<<<dim3(1), dim3(1024), 0, stream>>>(nullptr, 0, loss);
+        return (int)hipGetLastError();
+    }
+    const Plan pl = plan_of(a->count, a->width, a->vocab, a->entries, a->dtype);
+    const Kept k = kept_of(pl, hidden_grad != 0);
+    const Scratch sc = scratch_of(pl, hidden_grad ? 1 : 0);
+    if (!kept || kept_bytes < k.bytes || !workspace || workspace_bytes < sc.bytes ||
+        reinterpret_cast<uintptr_t>(kept) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16)
+        return -CT_EINVAL_WORKSPACE;
+    const double inverse_t = 1.0 / a->temperature;
+    float *shift = at<float>(kept, k.shift), *total = at<float>(kept, k.total), *sums = at<float>(kept, k.sums);
+    float *factor = at<float>(workspace, sc.factor);
+    const Targets t{a->rows, a->tokens, a->indices, a->values, a->log_normalizer, a->weights, a->ld_indices, a->ld_values};
+    const auto targets = [&](auto kernel, int threads) {
+        kernel<<<dim3((unsigned)pl.rows_pad), dim3(threads), 0, stream>>>(
+            t, pl.rows, (int)pl.entries, pl.vocab, pl.units, inverse_t, at<int>(kept, k.index), at<float>(kept, k.q),
+            at<float>(kept, k.chosen), at<uint16_t>(kept, k.first), at<float>(kept, k.weight), at<float>(kept, k.mass),
+            at<float>(kept, k.entropy), shift, total);
+    };
+    if (pl.entries <= 64) targets(targets_kernel<64>, 64);
+    else targets(targets_kernel<256>, 256);
+    CT_TRY(hipGetLastError());
+
+    if (pl.dtype == CT_F32) {
+        const float scale = (float)(1.4426950408889634074 / a->temperature);
+        float *piece = at<float>(workspace, sc.piece);
+        const float *head = static_cast<const float *>(a->head);
+        const void *hidden;
+        int64_t ld;
+        CT_TRY(plain_hidden(a, pl, at<void>(workspace, sc.plain), &hidden, &ld, stream));
+        for (int64_t v0 = 0; v0 < pl.vocab; v0 += pl.piece) {
+            const int64_t cols = pl.vocab - v0 < pl.piece ? pl.vocab - v0 : pl.piece;
+            if (const int bad = ct_gemm_f32(static_cast<const float *>(hidden), ld, 0, head + v0 * a->ld_head, a->ld_head, 1, piece, pl.piece,
+                                            0, nullptr, pl.rows, cols, pl.width, stream))
+                return bad;
+            rows_exp_f32<<<dim3((unsigned)pl.rows), dim3(256), 0, stream>>>(
+                piece, pl.piece, v0, cols, scale, shift, total, at<int>(kept, k.index), at<uint16_t>(kept, k.first),
+                at<float>(kept, k.chosen), (int)pl.entries, pl.units, hidden_grad ? sums : nullptr, pl.width);
+            CT_TRY(hipGetLastError());
+            if (!hidden_grad) continue;
+            if (const int bad = ct_gemm_f32(piece, pl.piece, 0, head + v0 * a->ld_head, a->ld_head, 0, sums, pl.width, v0 > 0,
+                                            nullptr, pl.rows, pl.width, cols, stream))
+                return bad;
+        }
+    } else {
+        CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), stream));
+        LogitsParams p = logits_params(a, pl, k, sc, kept, workspace);
+        const int64_t piece = hidden_grad ? pl.piece : pl.vocab;
+        for (int64_t v0 = 0; v0 < pl.vocab; v0 += piece) {
+            const int64_t cols = pl.vocab - v0 < piece ? pl.vocab - v0 : piece;
+            p.v0 = v0;
+            p.v1 = v0 + cols;
+            p.nl = cdiv(cols, pl.bl);
+            p.piece_blocks = up(cols, pl.bl) / 32;
+            CT_TRY(hidden_grad ? launch_logits<EXP>(pl, p, stream) : launch_logits<STATS>(pl, p, stream));
+            join_kernel<<<dim3((unsigned)(pl.rows_pad / 16)), dim3(256), 0, stream>>>(
+                p.stats, (int)cdiv(cols, kUnit), pl.rows_pad, shift, total, factor, hidden_grad ? p.piece : nullptr,
+                p.piece_blocks);
+            CT_TRY(hipGetLastError());
+            if (!hidden_grad) continue;
+            ProductParams g{};
+            g.b = p.head + v0 * p.ld;
+            g.ld = p.ld;
+            g.depth = cols;
+            g.cols = pl.width;
+            g.packed = p.piece;
+            g.blocks = p.piece_blocks;
+            g.np = p.np;
+            g.nl = cdiv(pl.width, pl.bl);
+            g.rows = pl.rows;
+            g.out = sums;
+            g.ldo = pl.width;
+            g.slab = pl.rows * pl.width;
+            g.steps = (int)cdiv(cols, kStep);
+            g.steps_per_split = (int)cdiv(g.steps, pl.splits);
+            g.factor = v0 ? factor : nullptr;
+            g.vec = pl.width % 4 == 0;
+            CT_TRY(launch_product<CT_F32>(pl.bp, g, pl.splits, stream));
+        }
+    }
+    row_loss<<<dim3((unsigned)pl.rows), dim3(64), 0, stream>>>(
+        shift, total, at<float>(kept, k.weight), at<float>(kept, k.mass), at<float>(kept, k.entropy),
+        at<int>(kept, k.index), at<float>(kept, k.q), at<float>(kept, k.chosen), pl.rows, (int)pl.entries, inverse_t,
+        a->values == nullptr, at<double>(workspace, sc.losses));
+    CT_TRY(hipGetLastError());
+    total_loss<<<dim3(1), dim3(1024), 0, stream>>>(at<double>(workspace, sc.losses), pl.rows, loss);
+    return (int)hipGetLastError();
+}
+
+extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstream, const void *kept_in, int32_t hidden_grad,
+                                     int64_t kept_bytes, void *d_hidden, int64_t ld_d_hidden, int64_t d_hidden_width,
+                                     int32_t d_hidden_dtype, void *d_head, int64_t ld_d_head, int64_t d_head_width,
+                                     int32_t d_head_dtype, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
+    if (const int bad = check(a, d_head != nullptr)) return bad;
+    if (a->count == 0) return 0;
+    if (!upstream) return -CT_EINVAL_POINTER;
+    const Plan pl = plan_of(a->count, a->width, a->vocab, a->entries, a->dtype);
+    const Kept k = kept_of(pl, hidden_grad != 0);
+    void *kept = const_cast<void *>(kept_in);
+    if (!kept || kept_bytes < k.bytes || reinterpret_cast<uintptr_t>(kept) % 16) return -CT_EINVAL_WORKSPACE;
+    const float inverse_t = (float)(1.0 / a->temperature);
+    if (d_hidden) {
+        if (!hidden_grad) return -CT_EINVAL_WORKSPACE;
+        if (d_hidden_dtype != CT_F32 && d_hidden_dtype != CT_BF16) return -CT_EINVAL_DTYPE;
+        if (d_hidden_width < 0 || d_hidden_width > pl.width || ld_d_hidden < d_hidden_width) return -CT_EINVAL_SHAPE;
+        const auto run = [&](auto kernel) {
+            kernel<<<dim3((unsigned)pl.rows, (unsigned)cdiv(d_hidden_width, 2048)), dim3(256), 0, stream>>>(
+                at<const float>(kept, k.sums), pl.splits, pl.rows * pl.width, pl.width, at<const float>(kept, k.weight),
+                at<const float>(kept, k.mass), at<const float>(kept, k.total), upstream, inverse_t,
+                at<const int>(kept, k.index), at<const float>(kept, k.chosen), (int)pl.entries, a->head, a->ld_head, a->rows, a->tokens,
+                d_hidden, ld_d_hidden, d_hidden_width);
+        };
+        if (pl.dtype == CT_F32) {
+            if (d_hidden_dtype == CT_F32) run(hidden_grad_kernel<CT_F32, CT_F32>);
+            else run(hidden_grad_kernel<CT_F32, CT_BF16>);
+        } else {
+            if (d_hidden_dtype == CT_F32) run(hidden_grad_kernel<CT_BF16, CT_F32>);
+            else run(hidden_grad_kernel<CT_BF16, CT_BF16>);
+        }
+        CT_TRY(hipGetLastError());
+    }
+    if (!d_head) return 0;
+    if (d_head_dtype != CT_F32 && d_head_dtype != CT_BF16) return -CT_EINVAL_DTYPE;
+    if (pl.dtype == CT_F32 && d_head_dtype != CT_F32) return -CT_EINVAL_DTYPE;
+    if (d_head_width < 0 || d_head_width > pl.width || ld_d_head < d_head_width) return -CT_EINVAL_SHAPE;
+    const Scratch sc = scratch_of(pl, 2);
+    if (!workspace || workspace_bytes < sc.bytes || reinterpret_cast<uintptr_t>(workspace) % 16) return -CT_EINVAL_WORKSPACE;
+    float *factor = at<float>(workspace, sc.factor);
+    float *inverse = at<float>(workspace, sc.inverse), *near = at<float>(workspace, sc.near);
+    row_factors<<<dim3((unsigned)cdiv(pl.rows_pad, 256)), dim3(256), 0, stream>>>(
+        at<const float>(kept, k.weight), at<const float>(kept, k.mass), at<const float>(kept, k.shift),
+        at<const float>(kept, k.total), upstream, inverse_t, pl.rows, pl.rows_pad, near, factor, inverse);
+    CT_TRY(hipGetLastError());
+    if (pl.dtype == CT_F32) {
+        const float scale = (float)(1.4426950408889634074 / a->temperature);
+        float *piece = at<float>(workspace, sc.piece), *out = static_cast<float *>(d_head);
+        const float *head = static_cast<const float *>(a->head);
+        const void *hidden;
+        int64_t ld;
+        CT_TRY(plain_hidden(a, pl, at<void>(workspace, sc.plain), &hidden, &ld, stream));
+        for (int64_t v0 = 0; v0 < pl.vocab; v0 += pl.piece) {
+            const int64_t cols = pl.vocab - v0 < pl.piece ? pl.vocab - v0 : pl.piece;
+            if (const int bad = ct_gemm_f32(static_cast<const float *>(hidden), ld, 0, head + v0 * a->ld_head, a->ld_head, 1, piece, pl.piece,
+                                            0, nullptr, pl.rows, cols, pl.width, stream))
+                return bad;
+            rows_grad_f32<<<dim3((unsigned)pl.rows), dim3(256), 0, stream>>>(
+                piece, pl.piece, v0, cols, scale, near, factor, inverse, at<int>(kept, k.index),
+                at<uint16_t>(kept, k.first), at<float>(kept, k.chosen), (int)pl.entries, pl.units);
+            CT_TRY(hipGetLastError());
+            if (const int bad = ct_gemm_f32(piece, pl.piece, 1, static_cast<const float *>(hidden), ld, 0, out + v0 * ld_d_head, ld_d_head, 0,
+                                            nullptr, cols, d_head_width, pl.rows, stream))
+                return bad;
+        }
+        return 0;
+    }
+    CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), stream));
+    const void *hidden;
+    int64_t ld;
+    CT_TRY(plain_hidden(a, pl, at<void>(workspace, sc.plain), &hidden, &ld, stream));
+    LogitsParams p = logits_params(a, pl, k, sc, kept, workspace);
+    p.shift = near;
+    p.factor = factor;
+    p.inverse = inverse;
+    p.piece_blocks = pl.rows_pad / 32;
+    for (int64_t v0 = 0; v0 < pl.vocab; v0 += pl.piece) {
+        const int64_t cols = pl.vocab - v0 < pl.piece ? pl.vocab - v0 : pl.piece;
+        p.v0 = v0;
+        p.v1 = v0 + cols;
+        p.nl = cdiv(cols, pl.bl);
+        CT_TRY(launch_logits<GRAD>(pl, p, stream));
+        ProductParams g{};
+        g.b = static_cast<const uint16_t *>(hidden);
+        g.ld = ld;
+        g.depth = pl.rows;
+        g.cols = d_head_width;
+        g.packed = p.piece;
+        g.blocks = p.piece_blocks;
+        g.np = cdiv(cols, pl.bp);
+        g.nl = cdiv(d_head_width, pl.bl);
+        g.rows = cols;
+        g.out = static_cast<char *>(d_head) + v0 * ld_d_head * (d_head_dtype == CT_F32 ? 4 : 2);
+        g.ldo = ld_d_head;
+        g.steps = g.steps_per_split = (int)cdiv(pl.rows, kStep);
+        g.vec = ld_d_head % 4 == 0 && reinterpret_cast<uintptr_t>(d_head) % 16 == 0;
+        CT_TRY(d_head_dtype == CT_F32 ? launch_product<CT_F32>(pl.bp, g, 1, stream)
+                                      : launch_product<CT_BF16>(pl.bp, g, 1, stream));
+    }
+    return 0;
+}

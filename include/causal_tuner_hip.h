@@ -640,6 +640,84 @@ int ct_muon(const ct_muon_matrix *matrices, int64_t count, const int32_t *plan, 
             int64_t workspace_needed, hipStream_t stream);
 
 /*
+ * The head's loss over a vocabulary walked in pieces, the logits never held: the streamed form of
+ * the reference's chunked projection loss (kernels/loss.py:23-66), and distillation from a
+ * teacher's top entries, which the reference has not. With l_iv = hidden_i . head_v / temperature,
+ * log p_iv = l_iv - log sum_v exp(l_iv), and the targets (v_k, q_k) of row i:
+ *   loss = sum_i weights_i sum_k q_k (log q_k - log p_iv_k)
+ * hidden [tokens, hidden_width], zeros past its columns, and head [vocab, width] of dtype (CT_BF16 or
+ * CT_F32). Row i < count of the loss is row rows[i] of hidden, of the targets and of the weights
+ * (rows null: row i); a row outside [0, tokens) has no loss. No row may be given twice.
+ * values null: hard labels, entries = 1, q = 1 (a label outside the vocabulary leaves log sum exp).
+ * Otherwise values float32 [*, entries] are the teacher's logits at indices [*, entries] and
+ * q = softmax(values / temperature) over a row's entries, or with log_normalizer float32 [*]
+ * q = exp(values / temperature - log_normalizer). An index outside [0, vocab) is no entry,
+ * an index given twice counts once with the sum of both, and a row without entries has no loss.
+ * bf16: width and ld_head multiples of 8, head 16-byte aligned.
+ */
+typedef struct ct_head_loss {
+    const void *hidden;
+    const void *head;
+    const int64_t *rows;
+    const int64_t *indices;
+    const float *values;
+    const float *log_normalizer;
+    const float *weights;
+    int64_t ld_hidden;
+    int64_t ld_head;
+    int64_t ld_indices;
+    int64_t ld_values;
+    int64_t tokens;
+    int64_t hidden_width;
+    int64_t count;
+    int64_t width;
+    int64_t vocab;
+    int32_t entries;
+    int32_t dtype;
+    double temperature;
+} ct_head_loss;
+
+/* Bytes of what a forward keeps for its backward (16-byte aligned, as the workspace); with
+ * hidden_grad, the gradient's unscaled float32 sums are among them. */
+int64_t ct_head_loss_kept(int64_t count, int64_t width, int64_t vocab, int32_t entries, int32_t dtype,
+                          int32_t hidden_grad);
+/* Bytes of workspace: pass 0 the forward, 1 the forward with hidden_grad, 2 a backward with d_head. */
+int64_t ct_head_loss_workspace(int64_t count, int64_t width, int64_t vocab, int32_t entries, int32_t dtype,
+                               int32_t pass);
+/* loss float32 [1]. With hidden_grad the same sweep sums the hidden rows' gradient. */
+int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t hidden_grad, void *kept, int64_t kept_bytes,
+                         void *workspace, int64_t workspace_bytes, hipStream_t stream);
+/*
+ * The gradients times upstream (float32 [1]), each rounded once: d_hidden [tokens, ..] (null: none;
+ * kept from a forward with hidden_grad), whose row rows[i] is written from row i of the loss, other
+ * rows left as they are; d_head [vocab, ..] (null: none), from logits formed again piece by piece. CT_F32 or
+ * CT_BF16 (d_head of float32 operands CT_F32); the first d_*_width columns are written. The
+ * derivative of bf16 operands is rounded to bf16 for the head's product. hidden (not read without
+ * d_head), hidden_grad and kept as the forward had them. Deterministic; kept is left as it is.
+ */
+int ct_head_loss_backward(const ct_head_loss *a, const float *upstream, const void *kept, int32_t hidden_grad,
+                          int64_t kept_bytes, void *d_hidden, int64_t ld_d_hidden, int64_t d_hidden_width,
+                          int32_t d_hidden_dtype, void *d_head, int64_t ld_d_head, int64_t d_head_width,
+                          int32_t d_head_dtype, void *workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Row-wise layer normalization, beside ct_rms_*. x, y [rows, width] of x_dtype (contiguous), w and
+ * bias [width] of w_dtype (either may be null), mean and rstd fp32 [rows] (both null: not kept).
+ *   forward:  mean = sum(x) / width, rstd = 1 / sqrt(sum((x - mean)^2) / width + eps),
+ *             y = (x - mean) rstd w + bias, rounded once
+ *   backward: g = dy w, n = (x - mean) rstd,
+ *             dx = rstd (g - sum(g) / width - n sum(g n) / width), dw = sum dy n, dbias = sum dy
+ * All in fp32; any of dx, dw and dbias may be null. dx may be dy itself. Deterministic: fixed
+ * reduction orders, the rows' in groups whose partial sums the workspace holds.
+ */
+int ct_layer_norm_forward(const void *x, int32_t x_dtype, const void *w, const void *bias, int32_t w_dtype, void *y,
+                          float *mean, float *rstd, int64_t rows, int64_t width, double eps, hipStream_t stream);
+int64_t ct_layer_norm_backward_workspace(int64_t rows, int64_t width, int32_t x_dtype, int32_t weight_grad);
+int ct_layer_norm_backward(const void *x, int32_t x_dtype, const void *w, int32_t w_dtype, const float *mean,
+                           const float *rstd, const void *dy, void *dx, void *dw, void *dbias, int64_t rows,
+                           int64_t width, void *workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/*
  * Kernel timing for benchmarks; no counterpart in the reference (which publishes no kernel
  * timings). ct_profile_begin enables the families in `families` and creates `capacity`
  * HIP event pairs; each later launch of an enabled family is bracketed by one pair
