@@ -57,6 +57,7 @@ struct Plan {
     int64_t rows_pad, width_pad, units;
     int64_t piece, pieces;  // vocabulary entries per piece of the sweep
     int splits;             // of the hidden gradient's reduction
+    bool turned;            // the second products read their staged operand transposed
 };
 
 // Workgroups' worth of work in whole rounds: how many splits of a reduction of `steps` leave the
@@ -94,9 +95,10 @@ Plan plan_of(int64_t rows, int64_t width, int64_t vocab, int64_t entries, int dt
     p.piece = up(cdiv(vocab, p.pieces), 256);
     p.pieces = cdiv(vocab, p.piece);
     p.splits = 1;
+    p.turned = dtype == CT_BF16 && p.bp == 256;
     if (dtype == CT_BF16) {
         const int64_t tiles = p.rows_pad / p.bp * cdiv(width, p.bl);
-        p.splits = splits_for(tiles, p.bp == 256 ? 256 : 512, p.piece / kStep);
+        p.splits = splits_for(tiles, p.bp == 64 ? 512 : 256, p.piece / kStep);
     }
     return p;
 }
@@ -130,7 +132,7 @@ Kept kept_of(const Plan &p, bool hidden_grad) {
     return k;
 }
 struct Scratch {
-    int64_t packed, plain, piece, stats, factor, inverse, near, losses, bytes;
+    int64_t packed, plain, piece, turned, stats, factor, inverse, near, losses, bytes;
 };
 // sweep 0: statistics alone, 1: with the hidden gradient's sums, 2: the head's gradient.
 Scratch scratch_of(const Plan &p, int sweep) {
@@ -140,6 +142,7 @@ Scratch scratch_of(const Plan &p, int sweep) {
     s.packed = r.take(wide ? 0 : p.rows_pad * p.width_pad * 2);
     s.plain = r.take(wide ? p.rows * p.width * 4 : sweep == 2 ? p.rows * p.width * 2 : 0);
     s.piece = r.take(wide ? p.rows * p.piece * 4 : sweep ? p.rows_pad * p.piece * 2 : 0);
+    s.turned = r.take(p.turned && sweep ? p.width * 2 * (sweep == 1 ? p.piece : up(p.rows, kStep)) : 0);
     s.stats = r.take(wide || sweep == 2 ? 0 : (sweep ? p.piece / kUnit : up(p.units, 2)) * p.rows_pad * 8);
     s.factor = r.take(p.rows_pad * 4);
     s.inverse = r.take(p.rows_pad * 4);
@@ -372,6 +375,34 @@ __global__ __launch_bounds__(256) void gather_rows(Source src, T *__restrict__ o
         out[blockIdx.x * pitch + c] = row >= 0 && c < src.width ? x[c] : T(0);
 }
 
+// out [cols][pitch] = x [rows][cols] transposed, the indices inside each block of 32 rows in the
+// order of the second product (unit q: 4 q .. + 3, 16 + 4 q .. + 3), zeros past the rows. A workgroup takes 64 x 64.
+__global__ __launch_bounds__(256) void transpose_rows(const uint16_t *__restrict__ x, int64_t ld, int64_t rows, int64_t cols,
+                                                      uint16_t *__restrict__ out, int64_t pitch) {
+    __shared__ uint16_t tile[64][72];
+    const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int u = threadIdx.x + i * 256, r = u >> 3, c = (u & 7) * 8;
+        uint4 v = zero4();
+        if (r0 + r < rows && c0 + c < cols) v = *reinterpret_cast<const uint4 *>(x + (r0 + r) * ld + c0 + c);
+        *reinterpret_cast<uint4 *>(&tile[r][c]) = v;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int u = threadIdx.x + i * 256, c = u >> 3, unit = u & 7, from = (unit >> 2) * 32 + (unit & 3) * 4;
+        if (c0 + c >= cols) continue;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = from + (j >> 1) * 16 + (j & 1) * 2;
+            w[j] = (uint32_t)tile[r][c] | (uint32_t)tile[r + 1][c] << 16;
+        }
+        *reinterpret_cast<uint4 *>(out + (c0 + c) * pitch + r0 + unit * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
 // ------------------------------------------------------------------------- the product's core
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
@@ -387,134 +418,153 @@ __device__ __forceinline__ void tile_of(int64_t id, int64_t np, int64_t nl, int6
     tl = at / count;
 }
 
-// acc[f][j] += fragment f of the staged operand x fragment j of the packed one, over reduction
-// steps [beg, end). WP x WL waves, each of PF x LF fragments of 16. KT: the staged operand is
-// stored with the reduction index as its row (as values in attention are), in LDS too, and its
-// fragments come from transposing reads; else its rows are reduction-contiguous. SWAP: the staged
-// operand is the MFMA's first, so a lane holds four of its consecutive rows for one packed row;
-// otherwise four packed rows for one of the staged ones.
+// acc[f][j] += fragment f of the staged operand x fragment j of the packed one, over the reduction.
+// WP x WL waves, each of PF x LF fragments of 16. KT: the staged operand is stored with the reduction
+// index as its row (as values in attention are), in LDS too, and its fragments come from transposing
+// reads; else its rows are reduction-contiguous. SWAP: the staged operand is the MFMA's first, so a
+// lane holds four of its consecutive rows for one packed row; otherwise four packed rows for one of
+// the staged ones.
+//
+// A step of 64 indices runs column by column (a fragment of the staged operand against all packed
+// ones), the order of everything in it fixed: a column's fragments are read two columns ahead, the
+// first two of the next step's at the end of this one, which its third stage allows; the stores of
+// the tile after next and the loads of the one behind it lie between the columns. With the stores
+// first in the step, as the order of the code suggests, all waves wait behind them after each barrier.
 template <int WP, int WL, int PF, bool KT, bool SWAP>
 struct Core {
     static constexpr int LF = 8, BP = WP * PF * 16, BL = WL * LF * 16, THREADS = 64 * WP * WL;
     static constexpr int kPer = BL * 8 / THREADS;   // 16-byte units of a stage per thread
     static constexpr int kStage = BL * 8;           // units per stage
+    static constexpr int kRows = KT ? THREADS / (BL / 8) : THREADS / 8;   // rows between a thread's units
+    static_assert(kRows % 16 == 0, "a thread's units differ by immediate offsets");
 
-    const char *base;      // the staged operand at step 0 ...
+    const char *base;        // the staged operand at step 0 ...
     int64_t bytes, advance;  // ... the bytes from there to its end, and from one step to the next
-    uint32_t off[kPer];
-    int k[kPer];           // KC: the unit's first index of a step; KT: its row
-    int limit;             // of k
-    const uint4 *a;        // the wave's packed rows at step 0
-    int64_t a_row;         // units between two blocks of packed rows
+    uint32_t off, pitch;     // of the thread's first unit, and between its units
+    int k, limit;            // KC: the unit's first index of a step, and the depth
+    const uint4 *a;          // the wave's packed rows at step 0
+    int64_t a_row;           // units between two blocks of packed rows
+    int steps, store_at, read_at;
 
-    // base: the staged operand at the tile's first row (KC) or column (KT); `extent` its rows from
+    // first: the staged operand at the tile's first row (KC) or column (KT); `extent` its rows from
     // there (KC) or columns (KT), `depth` the reduction's extent.
     __device__ __forceinline__ void init(const uint16_t *first, int64_t ld, int64_t extent, int64_t depth,
-                                         const uint4 *packed, int64_t block, int64_t blocks) {
-        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wp = wave % WP;
-        limit = (int)depth;
+                                         const uint4 *packed, int64_t block, int64_t blocks, int wave) {
+        const int tid = threadIdx.x, lane = tid & 63, wp = wave % WP, wl = wave / WP;
         base = reinterpret_cast<const char *>(first);
+        limit = (int)depth;
+        steps = (int)cdiv(depth, kStep);
+        pitch = (uint32_t)(kRows * ld * 2);
         if constexpr (KT) {
+            const int row = tid / (BL / 8), chunk = tid % (BL / 8), j = lane & 15, from = 4 * (lane >> 4) + (j >> 2);
             bytes = ((depth - 1) * ld + (extent < BL ? up(extent, 8) : BL)) * 2;   // rows are whole units
             advance = kStep * ld * 2;
+            off = chunk * 8 < extent ? (uint32_t)((row * ld + chunk * 8) * 2) : kOOB;
+            k = 0;
+            store_at = row * (BL / 8) + ((chunk >> 1 ^ (row & 7)) << 1 | (chunk & 1));
+            read_at = from * (BL * 2) + ((wl * LF ^ (from & 7)) << 5) + ((j & 3) << 3);
         } else {
-            bytes = (((extent < BL ? extent : BL) - 1) * ld + depth) * 2;
+            const int row = tid >> 3, chunk = tid & 7;
+            // rows are whole units; those past the extent lie behind the last
+            bytes = (((extent < BL ? extent : BL) - 1) * ld + up(depth, 8)) * 2;
             advance = kStep * 2;
-        }
-#pragma unroll
-        for (int c = 0; c < kPer; ++c) {
-            const int u = tid + c * THREADS;
-            if constexpr (KT) {
-                const int row = u / (BL / 8), chunk = u % (BL / 8);
-                off[c] = chunk * 8 < extent ? (uint32_t)((row * ld + chunk * 8) * 2) : kOOB;
-                k[c] = row;
-            } else {
-                const int row = u >> 3, chunk = u & 7;
-                off[c] = row < extent ? (uint32_t)((row * ld + chunk * 8) * 2) : kOOB;
-                k[c] = chunk * 8;
-            }
+            off = (uint32_t)((row * ld + chunk * 8) * 2);
+            k = chunk * 8;
+            store_at = slot(row, chunk);
+            read_at = slot(wl * LF * 16 + (lane & 15), lane >> 4);
         }
         a = packed + (block + wp * PF) * blocks * 64 + lane;
         a_row = blocks * 64;
     }
-    __device__ __forceinline__ void load_b(int step, uint4 (&r)[kPer]) const {
+    __device__ __forceinline__ void load_b(int t, uint4 (&r)[kPer]) const {
         // a descriptor per step: offsets stay within a step, whatever the operand's size
-        const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(base + step * advance, bytes - step * advance);
+        const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(base + t * advance, t < steps ? bytes - t * advance : 0);
+        const uint32_t from = KT || t * kStep + k < limit ? off : kOOB;
 #pragma unroll
-        for (int c = 0; c < kPer; ++c) r[c] = buf_load16(rsrc, step * kStep + k[c] < limit ? off[c] : kOOB);
+        for (int c = 0; c < kPer; ++c) r[c] = buf_load16(rsrc, from + c * pitch);
     }
-    __device__ __forceinline__ void load_a(int step, uint4 (&f)[2][PF]) const {
+    __device__ __forceinline__ void load_a(int t, uint4 (&f)[2][PF]) const {
+        const uint4 *at = a + (int64_t)(t < steps ? t : steps - 1) * 128;
 #pragma unroll
         for (int j = 0; j < PF; ++j)
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) f[ks][j] = a[j * a_row + (int64_t)(step * 2 + ks) * 64];
+            for (int ks = 0; ks < 2; ++ks) f[ks][j] = at[j * a_row + ks * 64];
     }
-    __device__ __forceinline__ static void store_b(uint4 *stage, const uint4 (&r)[kPer]) {
+    __device__ __forceinline__ void store_b(uint4 *stage, const uint4 (&r)[kPer]) const {
 #pragma unroll
-        for (int c = 0; c < kPer; ++c) {
-            const int u = threadIdx.x + c * THREADS;
+        for (int c = 0; c < kPer; ++c) stage[store_at + c * kRows * (KT ? BL / 8 : 8)] = r[c];
+    }
+    __device__ __forceinline__ void read(const uint4 *stage, int f, uint4 (&lf)[2]) const {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
             if constexpr (KT) {
-                const int row = u / (BL / 8), chunk = u % (BL / 8);
-                stage[row * (BL / 8) + ((chunk >> 1 ^ (row & 7)) << 1 | (chunk & 1))] = r[c];
+                const __attribute__((address_space(3))) char *p =
+                    (const __attribute__((address_space(3))) char *)stage + (read_at ^ f << 5) + ks * 32 * (BL * 2);
+                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)p);
+                const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(p + 16 * (BL * 2)));
+                const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+                lf[ks] = make_uint4(l2.x, l2.y, h2.x, h2.y);
             } else {
-                stage[slot(u >> 3, u & 7)] = r[c];
+                lf[ks] = stage[(read_at ^ ks << 2) + f * 128];
             }
         }
     }
-    __device__ __forceinline__ static uint4 fragment(const uint4 *stage, int f, int ks, int wl, int lane) {
-        const int c0 = (wl * LF + f) * 16;
-        if constexpr (KT) {
-            const int j = lane & 15, row = 4 * (lane >> 4) + (j >> 2);
-            const __attribute__((address_space(3))) char *p =
-                (const __attribute__((address_space(3))) char *)stage + (ks * 32 + row) * (BL * 2) +
-                ((c0 >> 4 ^ (row & 7)) << 5) + ((j & 3) << 3);
-            const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)p);
-            const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(p + 16 * (BL * 2)));
-            const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-            return make_uint4(l2.x, l2.y, h2.x, h2.y);
-        } else {
-            return stage[slot(c0 + (lane & 15), ks * 4 + (lane >> 4))];
-        }
-    }
-    // One step: stage `cur` and the fragments `af` are multiplied while `b` (the next step's) goes
-    // to stage `nxt`, the one after it is loaded into b and the next step's fragments into `an`.
-    __device__ __forceinline__ void step(int t, const uint4 *cur, uint4 *nxt, const uint4 (&af)[2][PF],
-                                         uint4 (&an)[2][PF], uint4 (&b)[kPer], int last, f32x4 (&acc)[LF][PF], int wl,
-                                         int lane) const {
-        load_a(t + 1 < last ? t + 1 : t, an);
-        store_b(nxt, b);
-        load_b(t + 2, b);
+    template <int F>
+    __device__ __forceinline__ void columns(int t, const uint4 *cur, const uint4 *nxt, uint4 *wr, const uint4 (&af)[2][PF],
+                                            uint4 (&an)[2][PF], uint4 (&b)[kPer], uint4 (&lf)[3][2],
+                                            f32x4 (&acc)[LF][PF]) const {
+        if constexpr (F < LF) {
+            read(F + 2 < LF ? cur : nxt, (F + 2) % LF, lf[(F + 2) % 3]);
+            if constexpr (F == 0) load_a(t + 1, an);
+            if constexpr (F == 2) store_b(wr, b);
+            if constexpr (F == 3) load_b(t + 3, b);
 #pragma unroll
-        for (int f = 0; f < LF; ++f) {
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                const uint4 lf = fragment(cur, f, ks, wl, lane);
+            for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int j = 0; j < PF; ++j)
-                    acc[f][j] = SWAP ? mfma16x16x32(lf, af[ks][j], acc[f][j]) : mfma16x16x32(af[ks][j], lf, acc[f][j]);
-            }
+                    acc[F][j] = SWAP ? mfma16x16x32(lf[F % 3][ks], af[ks][j], acc[F][j])
+                                     : mfma16x16x32(af[ks][j], lf[F % 3][ks], acc[F][j]);
+            __builtin_amdgcn_sched_barrier(0);
+            columns<F + 1>(t, cur, nxt, wr, af, an, b, lf, acc);
         }
+    }
+    // LF is not a multiple of 3: the fragments read ahead move to their places of the next step
+    __device__ __forceinline__ void step(int t, uint4 *stages, int &at, const uint4 (&af)[2][PF], uint4 (&an)[2][PF],
+                                         uint4 (&b)[kPer], uint4 (&lf)[3][2], f32x4 (&acc)[LF][PF]) const {
+        const int next = at == 2 * kStage ? 0 : at + kStage, after = next == 2 * kStage ? 0 : next + kStage;
+        columns<0>(t, stages + at, stages + next, stages + after, af, an, b, lf, acc);
+        static_assert(LF % 3 == 2, "the places of the next step's first two columns");
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            const uint4 x = lf[2][ks], y = lf[0][ks];
+            lf[0][ks] = x;
+            lf[1][ks] = y;
+        }
+        at = next;
         __syncthreads();
     }
-    __device__ __forceinline__ void run(int beg, int end, uint4 *s0, uint4 *s1, f32x4 (&acc)[LF][PF]) const {
-        const int lane = threadIdx.x & 63, wl = (threadIdx.x >> 6) / WP;
+    __device__ __forceinline__ void run(uint4 *stages, f32x4 (&acc)[LF][PF]) const {
 #pragma unroll
         for (int f = 0; f < LF; ++f)
 #pragma unroll
             for (int j = 0; j < PF; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (beg >= end) return;
-        uint4 b[kPer], a0[2][PF], a1[2][PF];
-        load_b(beg, b);
-        load_a(beg, a0);
-        store_b(s0, b);
-        load_b(beg + 1, b);
+        if (steps <= 0) return;
+        uint4 b[kPer], more[kPer], a0[2][PF], a1[2][PF], lf[3][2];
+        load_b(0, b);
+        load_b(1, more);
+        load_a(0, a0);
+        store_b(stages, b);
+        store_b(stages + kStage, more);
+        load_b(2, b);
         __syncthreads();
-        int t = beg;
-        for (; t + 1 < end; t += 2) {
-            step(t, s0, s1, a0, a1, b, end, acc, wl, lane);
-            step(t + 1, s1, s0, a1, a0, b, end, acc, wl, lane);
+        read(stages, 0, lf[0]);
+        read(stages, 1, lf[1]);
+        int t = 0, at = 0;
+        for (; t + 1 < steps; t += 2) {
+            step(t, stages, at, a0, a1, b, lf, acc);
+            step(t + 1, stages, at, a1, a0, b, lf, acc);
         }
-        if (t < end) step(t, s0, s1, a0, a1, b, end, acc, wl, lane);
+        if (t < steps) step(t, stages, at, a0, a1, b, lf, acc);
     }
 };
 
@@ -582,16 +632,17 @@ __device__ __forceinline__ int64_t place_of(const LogitsParams &p, int64_t row, 
 template <int WP, int WL, int PF, int MODE>
 __global__ __launch_bounds__(64 * WP * WL) void logits_kernel(const LogitsParams p) {
     using C = Core<WP, WL, PF, false, MODE != GRAD>;
-    __shared__ uint4 s0[C::kStage], s1[C::kStage];
+    __shared__ uint4 stages[3 * C::kStage];
     __shared__ uint32_t marks[WP * WL][PF * 16 * 4];
     int64_t tp, tl;
     tile_of(blockIdx.x, p.np, p.nl, tp, tl);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wp = wave % WP, wl = wave / WP, q = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wp = wave % WP, wl = wave / WP, q = lane >> 4;
     const int64_t v0 = p.v0 + tl * C::BL, left = p.v1 - v0;
     C core;
-    core.init(p.head + v0 * p.ld, p.ld, left, p.width, p.packed, tp * (C::BP / 16), p.blocks);
+    core.init(p.head + v0 * p.ld, p.ld, left, p.width, p.packed, tp * (C::BP / 16), p.blocks, wave);
     f32x4 acc[C::LF][PF];
-    core.run(0, (int)(p.blocks / 2), s0, s1, acc);
+    core.run(stages, acc);
 
     const int64_t row0 = tp * C::BP + wp * PF * 16, u0 = v0 + wl * kUnit, unit = u0 / kUnit;
     uint32_t *bits = marks[wave];
@@ -708,27 +759,27 @@ __global__ __launch_bounds__(64 * WP * WL) void logits_kernel(const LogitsParams
     }
 }
 
-// The units' statistics of a piece joined to the rows': 16 rows x 16 groups of units a workgroup.
+// The units' statistics of a piece joined to the rows': 16 rows x 64 groups of units a workgroup.
 // A row's shift becomes the largest of its own and the units'; E of a unit with another shift is
 // brought to it, and `factor` is what the sums of the pieces before are brought to it with.
-__global__ __launch_bounds__(256) void join_kernel(const float2 *__restrict__ stats, int units, int64_t rows_pad,
+__global__ __launch_bounds__(1024) void join_kernel(const float2 *__restrict__ stats, int units, int64_t rows_pad,
                                                    float *__restrict__ shift, float *__restrict__ total,
                                                    float *__restrict__ factor, uint4 *piece, int64_t piece_blocks) {
-    __shared__ float part[16][17];
+    __shared__ float part[64][17];
     const int r = threadIdx.x & 15, g = threadIdx.x >> 4;
     const int64_t row = (int64_t)blockIdx.x * 16 + r;
     const float2 *at = stats + row;
     float c = kNone;
-    for (int u = g; u < units; u += 16) c = fmaxf(c, at[u * rows_pad].x);
+    for (int u = g; u < units; u += 64) c = fmaxf(c, at[u * rows_pad].x);
     part[g][r] = c;
     __syncthreads();
     const float before = shift[row], held = total[row];
     c = before;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) c = fmaxf(c, part[i][r]);
+    for (int i = 0; i < 64; ++i) c = fmaxf(c, part[i][r]);
     __syncthreads();
     float sum = 0.f;
-    for (int u = g; u < units; u += 16) {
+    for (int u = g; u < units; u += 64) {
         const float2 s = at[u * rows_pad];
         if (s.x == c) {
             sum += s.y;
@@ -753,7 +804,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float2 *__restrict__ st
         const float by = before == c ? 1.f : __builtin_amdgcn_exp2f(before - c);
         sum = held * by;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum += part[i][r];
+        for (int i = 0; i < 64; ++i) sum += part[i][r];
         total[row] = sum;
         shift[row] = c;
         factor[row] = by;
@@ -762,8 +813,9 @@ __global__ __launch_bounds__(256) void join_kernel(const float2 *__restrict__ st
 
 // ------------------------------------------------------------------------- the second product
 struct ProductParams {
-    const uint16_t *b;         // [depth, cols]
+    const uint16_t *b;         // KT: [depth, cols], else its transpose
     int64_t ld, depth, cols;
+    bool kt;
     const uint4 *packed;       // [rows, depth]
     int64_t blocks;
     int64_t np, nl;
@@ -775,23 +827,25 @@ struct ProductParams {
     int vec;
 };
 
-// out[row, col] (= factor out +) sum_k packed(row, k) b[k, col], one split of the reduction per z.
-template <int WP, int WL, int PF, int OUT>
+// out[row, col] (= factor out +) sum_k packed(row, k) b(k, col), one split of the reduction per y.
+template <int WP, int WL, int PF, bool KT, int OUT>
 __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductParams p) {
-    using C = Core<WP, WL, PF, true, true>;
-    __shared__ uint4 s0[C::kStage], s1[C::kStage];
+    using C = Core<WP, WL, PF, KT, true>;
+    __shared__ uint4 stages[3 * C::kStage];
     int64_t tp, tl;
     tile_of(blockIdx.x, p.np, p.nl, tp, tl);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wp = wave % WP, wl = wave / WP, q = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wp = wave % WP, wl = wave / WP, q = lane >> 4;
     const int beg = blockIdx.y * p.steps_per_split;
     const int end = beg + p.steps_per_split < p.steps ? beg + p.steps_per_split : p.steps;
     // the split's own range of the staged operand, so that offsets stay within 32 bits
     C core;
     const int64_t k0 = (int64_t)beg * kStep;
-    core.init(p.b + k0 * p.ld + tl * C::BL, p.ld, p.cols - tl * C::BL, p.depth - k0, p.packed + (int64_t)beg * 128,
-              tp * (C::BP / 16), p.blocks);
+    const int64_t depth = (end < p.steps ? (int64_t)end * kStep : p.depth) - k0;   // none: an empty split
+    core.init(p.b + (KT ? k0 * p.ld + tl * C::BL : tl * C::BL * p.ld + k0), p.ld, p.cols - tl * C::BL, depth,
+              p.packed + (int64_t)beg * 128, tp * (C::BP / 16), p.blocks, wave);
     f32x4 acc[C::LF][PF];
-    core.run(0, end - beg, s0, s1, acc);
+    core.run(stages, acc);
 #pragma unroll
     for (int j = 0; j < PF; ++j) {
         const int64_t row = tp * C::BP + (wp * PF + j) * 16 + (lane & 15);
@@ -957,9 +1011,10 @@ __global__ __launch_bounds__(256) void row_factors(const float *__restrict__ wei
     factor[row] = row < rows && mass[row] != 0.f ? f * mass[row] / z : 0.f;
 }
 
-// dh_i = u c_i / T (Q_i / Z_i sums_i + sum_k coefficient_k w_v_k), the splits' sums in order. One
-// workgroup per row and 2048 columns.
-template <int IN, int OUT>
+// dh_i = u c_i / T (Q_i / Z_i sums_i + sum_k coefficient_k w_v_k). A workgroup takes a row and 512
+// columns; its four waves share the splits' sums and the targets, every fourth each, and are joined
+// in order. Bound by the targets' rows of the head: K x width per row of the loss, from the caches.
+template <int IN, int OUT, bool VEC>
 __global__ __launch_bounds__(256) void hidden_grad_kernel(const float *__restrict__ sums, int splits, int64_t slab,
                                                           int64_t width, const float *__restrict__ weight,
                                                           const float *__restrict__ mass, const float *__restrict__ total,
@@ -969,25 +1024,65 @@ __global__ __launch_bounds__(256) void hidden_grad_kernel(const float *__restric
                                                           const void *__restrict__ head, int64_t ld,
                                                           const int64_t *__restrict__ rows, int64_t tokens,
                                                           void *__restrict__ out, int64_t ldo, int64_t out_width) {
+    __shared__ float lds[4][512];
     const int64_t row = blockIdx.x, to = rows ? rows[row] : row;
     if (to < 0 || to >= tokens) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const float held = mass[row], f = weight[row] * *upstream * inverse_t;
     const float by = held != 0.f ? held / total[row] : 0.f;
-    for (int64_t c = (int64_t)blockIdx.y * 2048 + threadIdx.x; c < out_width && c < (int64_t)(blockIdx.y + 1) * 2048; c += 256) {
-        float sum = 0.f;
-        for (int s = 0; s < splits; ++s) sum += sums[s * slab + row * width + c];
-        sum *= by;
-        for (int e = 0; e < entries; ++e) {
-            const int v = index[row * entries + e];
-            if (v == kNoEntry) break;
-            const float w = IN == CT_F32 ? static_cast<const float *>(head)[v * ld + c]
-                                         : bf16_to_f32(static_cast<const uint16_t *>(head)[v * ld + c]);
-            sum += coefficient[row * entries + e] * w;
+    const int64_t c0 = (int64_t)blockIdx.y * 512 + lane * 8;
+    const auto in = [&](int i) { return VEC ? c0 < width : c0 + i < width; };
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s = wave; s < splits; s += 4) {
+        const float *p = sums + s * slab + row * width + c0;
+        if constexpr (VEC) {
+            if (in(0)) {
+                const float4 x = *reinterpret_cast<const float4 *>(p), y = *reinterpret_cast<const float4 *>(p + 4);
+                v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (in(i)) v[i] += p[i];
         }
-        sum = held != 0.f ? sum * f : 0.f;
-        if constexpr (OUT == CT_F32) static_cast<float *>(out)[to * ldo + c] = sum;
-        else static_cast<uint16_t *>(out)[to * ldo + c] = bf16_bits(sum);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= by;
+    const int *at = index + row * entries;
+    const float *k = coefficient + row * entries;
+#pragma unroll 8
+    for (int e = wave; e < entries; e += 4) {
+        const int vocab = at[e];
+        if (vocab == kNoEntry) continue;
+        const float by_k = k[e];
+        if constexpr (IN == CT_F32) {
+            const float *w = static_cast<const float *>(head) + vocab * ld + c0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (in(i)) v[i] += by_k * w[i];
+        } else if (in(0)) {   // rows of whole units
+            const uint4 x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(head) + vocab * ld + c0);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] += by_k * bf16_to_f32((uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lds[wave][lane * 8 + i] = v[i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 512; c += 256) {
+        const int64_t col = (int64_t)blockIdx.y * 512 + c;
+        if (col >= out_width) break;
+        const float sum = held != 0.f ? (lds[0][c] + lds[1][c] + lds[2][c] + lds[3][c]) * f : 0.f;
+        if constexpr (OUT == CT_F32) static_cast<float *>(out)[to * ldo + col] = sum;
+        else static_cast<uint16_t *>(out)[to * ldo + col] = bf16_bits(sum);
+    }
+}
+
+hipError_t transpose(const uint16_t *x, int64_t ld, int64_t rows, int64_t cols, uint16_t *out, int64_t pitch, hipStream_t s) {
+    transpose_rows<<<dim3((unsigned)cdiv(rows, 64), (unsigned)cdiv(cols, 64)), dim3(256), 0, s>>>(x, ld, rows, cols, out, pitch);
+    return hipGetLastError();
 }
 
 template <class T>
@@ -1003,13 +1098,17 @@ hipError_t launch_logits(const Plan &pl, const LogitsParams &p, hipStream_t s) {
     else logits_kernel<4, 2, 4, MODE><<<grid, dim3(512), 0, s>>>(p);
     return hipGetLastError();
 }
-template <int OUT>
+template <int OUT, bool KT>
 hipError_t launch_product(int bp, const ProductParams &p, int splits, hipStream_t s) {
     const dim3 grid((unsigned)(p.np * p.nl), (unsigned)splits);
-    if (bp == 64) product_kernel<4, 1, 1, OUT><<<grid, dim3(256), 0, s>>>(p);
-    else if (bp == 128) product_kernel<4, 2, 2, OUT><<<grid, dim3(512), 0, s>>>(p);
-    else product_kernel<4, 2, 4, OUT><<<grid, dim3(512), 0, s>>>(p);
+    if (bp == 64) product_kernel<4, 1, 1, KT, OUT><<<grid, dim3(256), 0, s>>>(p);
+    else if (bp == 128 || KT) product_kernel<4, 2, 2, KT, OUT><<<grid, dim3(512), 0, s>>>(p);
+    else product_kernel<4, 2, 4, KT, OUT><<<grid, dim3(512), 0, s>>>(p);
     return hipGetLastError();
+}
+template <int OUT>
+hipError_t launch_product(int bp, const ProductParams &p, int splits, hipStream_t s) {
+    return p.kt ? launch_product<OUT, true>(bp, p, splits, s) : launch_product<OUT, false>(bp, p, splits, s);
 }
 
 int check(const ct_head_loss *a, bool hidden) {
@@ -1171,7 +1270,7 @@ extern "C" int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t 
             p.nl = cdiv(cols, pl.bl);
             p.piece_blocks = up(cols, pl.bl) / 32;
             CT_TRY(hidden_grad ? launch_logits<EXP>(pl, p, stream) : launch_logits<STATS>(pl, p, stream));
-            join_kernel<<<dim3((unsigned)(pl.rows_pad / 16)), dim3(256), 0, stream>>>(
+            join_kernel<<<dim3((unsigned)(pl.rows_pad / 16)), dim3(1024), 0, stream>>>(
                 p.stats, (int)cdiv(cols, kUnit), pl.rows_pad, shift, total, factor, hidden_grad ? p.piece : nullptr,
                 p.piece_blocks);
             CT_TRY(hipGetLastError());
@@ -1179,7 +1278,14 @@ extern "C" int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t 
             ProductParams g{};
             g.b = p.head + v0 * p.ld;
             g.ld = p.ld;
-            g.depth = cols;
+            g.kt = !pl.turned;
+            if (pl.turned) {
+                uint16_t *turned = at<uint16_t>(workspace, sc.turned);
+                CT_TRY(transpose(g.b, g.ld, cols, pl.width, turned, pl.piece, stream));
+                g.b = turned;
+                g.ld = pl.piece;
+            }
+            g.depth = pl.turned ? up(cols, kStep) : cols;   // turned rows end with a whole step, in their order
             g.cols = pl.width;
             g.packed = p.piece;
             g.blocks = p.piece_blocks;
@@ -1222,18 +1328,22 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
         if (d_hidden_dtype != CT_F32 && d_hidden_dtype != CT_BF16) return -CT_EINVAL_DTYPE;
         if (d_hidden_width < 0 || d_hidden_width > pl.width || ld_d_hidden < d_hidden_width) return -CT_EINVAL_SHAPE;
         const auto run = [&](auto kernel) {
-            kernel<<<dim3((unsigned)pl.rows, (unsigned)cdiv(d_hidden_width, 2048)), dim3(256), 0, stream>>>(
+            kernel<<<dim3((unsigned)pl.rows, (unsigned)cdiv(d_hidden_width, 512)), dim3(256), 0, stream>>>(
                 at<const float>(kept, k.sums), pl.splits, pl.rows * pl.width, pl.width, at<const float>(kept, k.weight),
                 at<const float>(kept, k.mass), at<const float>(kept, k.total), upstream, inverse_t,
                 at<const int>(kept, k.index), at<const float>(kept, k.chosen), (int)pl.entries, a->head, a->ld_head, a->rows, a->tokens,
                 d_hidden, ld_d_hidden, d_hidden_width);
         };
-        if (pl.dtype == CT_F32) {
-            if (d_hidden_dtype == CT_F32) run(hidden_grad_kernel<CT_F32, CT_F32>);
-            else run(hidden_grad_kernel<CT_F32, CT_BF16>);
+        const bool vec = pl.width % 8 == 0;
+        if (pl.dtype == CT_BF16) {
+            if (d_hidden_dtype == CT_F32) run(hidden_grad_kernel<CT_BF16, CT_F32, true>);
+            else run(hidden_grad_kernel<CT_BF16, CT_BF16, true>);
+        } else if (d_hidden_dtype == CT_F32) {
+            if (vec) run(hidden_grad_kernel<CT_F32, CT_F32, true>);
+            else run(hidden_grad_kernel<CT_F32, CT_F32, false>);
         } else {
-            if (d_hidden_dtype == CT_F32) run(hidden_grad_kernel<CT_BF16, CT_F32>);
-            else run(hidden_grad_kernel<CT_BF16, CT_BF16>);
+            if (vec) run(hidden_grad_kernel<CT_F32, CT_BF16, true>);
+            else run(hidden_grad_kernel<CT_F32, CT_BF16, false>);
         }
         CT_TRY(hipGetLastError());
     }
@@ -1280,6 +1390,12 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
     p.factor = factor;
     p.inverse = inverse;
     p.piece_blocks = pl.rows_pad / 32;
+    if (pl.turned) {
+        uint16_t *turned = at<uint16_t>(workspace, sc.turned);
+        CT_TRY(transpose(static_cast<const uint16_t *>(hidden), ld, pl.rows, pl.width, turned, up(pl.rows, kStep), stream));
+        hidden = turned;
+        ld = up(pl.rows, kStep);
+    }
     for (int64_t v0 = 0; v0 < pl.vocab; v0 += pl.piece) {
         const int64_t cols = pl.vocab - v0 < pl.piece ? pl.vocab - v0 : pl.piece;
         p.v0 = v0;
@@ -1289,7 +1405,8 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
         ProductParams g{};
         g.b = static_cast<const uint16_t *>(hidden);
         g.ld = ld;
-        g.depth = pl.rows;
+        g.kt = !pl.turned;
+        g.depth = pl.turned ? up(pl.rows, kStep) : pl.rows;
         g.cols = d_head_width;
         g.packed = p.piece;
         g.blocks = p.piece_blocks;
