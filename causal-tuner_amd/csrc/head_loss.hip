@@ -27,8 +27,9 @@
 // indices inside a block of 32 (unit q holds indices 4 q .. + 3 and 16 + 4 q .. + 3), and the
 // product that follows reads its LDS tile in that order.
 //
-// float32. The products are ct_gemm_f32's over a piece of logits in the workspace, with a row pass
-// between them.
+// float32. Operands are split into three bf16 terms, which hold them exactly, and take the same
+// kernels (Core, TRI). Up to 64 rows, where reading the head bounds and splitting it would cost more,
+// the products are ct_gemm_f32's over a piece of logits in the workspace, with a row pass between them.
 //
 // Every sum runs in a fixed order: repeated calls are bit-identical.
 
@@ -42,6 +43,7 @@ namespace {
 constexpr int kStep = 64;              // reduction indices per step of a product
 constexpr int kUnit = 128;             // vocabulary entries per (row, unit) pair of statistics
 constexpr int kMaxEntries = 1024;
+constexpr int64_t kFewRows = 64;       // float32: up to here on ct_gemm_f32
 constexpr int64_t kMaxWidth = 65536, kMaxVocab = (int64_t{1} << 31) - 1024, kMaxRows = int64_t{1} << 30;
 // E of one piece, in bytes: what two passes over it can share through the 256 MB last-level cache.
 constexpr int64_t kPieceBytes = int64_t{256} << 20;
@@ -58,6 +60,8 @@ struct Plan {
     int64_t piece, pieces;  // vocabulary entries per piece of the sweep
     int splits;             // of the hidden gradient's reduction
     bool turned;            // the second products read their staged operand transposed
+    bool tri;               // float32 in three bf16 terms
+    int terms;
 };
 
 // Workgroups' worth of work in whole rounds: how many splits of a reduction of `steps` leave the
@@ -88,15 +92,17 @@ Plan plan_of(int64_t rows, int64_t width, int64_t vocab, int64_t entries, int dt
     p.rows_pad = up(rows, p.bp);
     p.width_pad = up(width, kStep);
     p.units = cdiv(vocab, kUnit);
-    const int64_t element = dtype == CT_F32 ? 4 : 2;
+    p.tri = dtype == CT_F32 && rows > kFewRows;
+    p.terms = p.tri ? 3 : 1;
+    const int64_t element = p.tri ? 6 : dtype == CT_F32 ? 4 : 2;
     int64_t most = kPieceBytes / (p.rows_pad * element) / 256 * 256;
     if (most < 1024) most = 1024;
     p.pieces = cdiv(vocab, most);
     p.piece = up(cdiv(vocab, p.pieces), 256);
     p.pieces = cdiv(vocab, p.piece);
     p.splits = 1;
-    p.turned = dtype == CT_BF16 && p.bp == 256;
-    if (dtype == CT_BF16) {
+    p.turned = p.tri || (dtype == CT_BF16 && p.bp == 256);
+    if (dtype == CT_BF16 || p.tri) {
         const int64_t tiles = p.rows_pad / p.bp * cdiv(width, p.bl);
         p.splits = splits_for(tiles, p.bp == 64 ? 512 : 256, p.piece / kStep);
     }
@@ -132,18 +138,20 @@ Kept kept_of(const Plan &p, bool hidden_grad) {
     return k;
 }
 struct Scratch {
-    int64_t packed, plain, piece, turned, stats, factor, inverse, near, losses, bytes;
+    int64_t packed, plain, piece, turned, split, stats, factor, inverse, near, losses, bytes;
 };
 // sweep 0: statistics alone, 1: with the hidden gradient's sums, 2: the head's gradient.
 Scratch scratch_of(const Plan &p, int sweep) {
     Regions r;
     Scratch s{};
-    const bool wide = p.dtype == CT_F32;
-    s.packed = r.take(wide ? 0 : p.rows_pad * p.width_pad * 2);
-    s.plain = r.take(wide ? p.rows * p.width * 4 : sweep == 2 ? p.rows * p.width * 2 : 0);
-    s.piece = r.take(wide ? p.rows * p.piece * 4 : sweep ? p.rows_pad * p.piece * 2 : 0);
-    s.turned = r.take(p.turned && sweep ? p.width * 2 * (sweep == 1 ? p.piece : up(p.rows, kStep)) : 0);
-    s.stats = r.take(wide || sweep == 2 ? 0 : (sweep ? p.piece / kUnit : up(p.units, 2)) * p.rows_pad * 8);
+    const bool gemm = p.dtype == CT_F32 && !p.tri;
+    const int64_t terms = 2 * p.terms, piece = sweep || p.tri ? p.piece : up(p.units, 2) * kUnit;
+    s.packed = r.take(gemm ? 0 : p.rows_pad * p.width_pad * terms);
+    s.plain = r.take(gemm || (p.tri && sweep == 2) ? p.rows * p.width * 4 : sweep == 2 ? p.rows * p.width * 2 : 0);
+    s.piece = r.take(gemm ? p.rows * p.piece * 4 : sweep ? p.rows_pad * p.piece * terms : 0);
+    s.turned = r.take(p.turned && sweep ? p.width * terms * (sweep == 1 ? p.piece : up(p.rows, kStep)) : 0);
+    s.split = r.take(p.tri ? p.piece * up(p.width, 8) * terms : 0);
+    s.stats = r.take(gemm || sweep == 2 ? 0 : piece / kUnit * p.rows_pad * 8);
     s.factor = r.take(p.rows_pad * 4);
     s.inverse = r.take(p.rows_pad * 4);
     s.near = r.take(p.rows_pad * 4);
@@ -342,6 +350,55 @@ struct Source {
     }
 };
 
+// A float32 value as the sum of three bf16 terms, exact for values of 2^-100 and more: 8 bits of the
+// significand each.
+__device__ __forceinline__ void split3(float v, float (&t)[3]) {
+    t[0] = bf16_to_f32(bf16_bits(v));
+    t[1] = bf16_to_f32(bf16_bits(v - t[0]));
+    t[2] = v - t[0] - t[1];
+}
+// Eight of them, term by term, as 16-byte units.
+__device__ __forceinline__ void split_unit(const float (&v)[8], uint4 (&out)[3]) {
+    float t[8][3];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) split3(v[i], t[i]);
+#pragma unroll
+    for (int s = 0; s < 3; ++s)
+        out[s] = make_uint4(pack_bf16x2(t[0][s], t[1][s]), pack_bf16x2(t[2][s], t[3][s]), pack_bf16x2(t[4][s], t[5][s]),
+                            pack_bf16x2(t[6][s], t[7][s]));
+}
+
+// pack_rows below for float32 rows: three packed operands, `units` apart.
+__global__ __launch_bounds__(256) void pack_split(Source src, int64_t blocks, uint4 *__restrict__ out, int64_t units) {
+    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (u >= units) return;
+    const int lane = (int)(u & 63);
+    const int64_t block = u >> 6, kb = block % blocks, row = src.row(block / blocks * 16 + (lane & 15));
+    const int64_t k = kb * 32 + (lane >> 4) * 8;
+    const float *x = static_cast<const float *>(src.x) + row * src.ld;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = row >= 0 && k + i < src.width ? x[k + i] : 0.f;
+    uint4 t[3];
+    split_unit(v, t);
+#pragma unroll
+    for (int s = 0; s < 3; ++s) out[u + s * units] = t[s];
+}
+
+// float32 rows [rows][cols] as three bf16 arrays of `pitch` columns, `apart` units between them.
+__global__ __launch_bounds__(256) void split_rows(const float *__restrict__ x, int64_t ld, int64_t rows, int64_t cols,
+                                                  uint4 *__restrict__ out, int64_t pitch, int64_t apart) {
+    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x, per = pitch / 8, row = u / per, c = u % per * 8;
+    if (row >= rows) return;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? x[row * ld + c + i] : 0.f;
+    uint4 t[3];
+    split_unit(v, t);
+#pragma unroll
+    for (int s = 0; s < 3; ++s) out[u + s * apart] = t[s];
+}
+
 // Hidden rows in the order of a product's packed operand, zeros past the rows and the width.
 template <bool VEC>
 __global__ __launch_bounds__(256) void pack_rows(Source src, int64_t blocks, uint4 *__restrict__ out, int64_t units) {
@@ -376,30 +433,50 @@ __global__ __launch_bounds__(256) void gather_rows(Source src, T *__restrict__ o
 }
 
 // out [cols][pitch] = x [rows][cols] transposed, the indices inside each block of 32 rows in the
-// order of the second product (unit q: 4 q .. + 3, 16 + 4 q .. + 3), zeros past the rows. A workgroup takes 64 x 64.
-__global__ __launch_bounds__(256) void transpose_rows(const uint16_t *__restrict__ x, int64_t ld, int64_t rows, int64_t cols,
-                                                      uint16_t *__restrict__ out, int64_t pitch) {
-    __shared__ uint16_t tile[64][72];
+// order of the second product (unit q: 4 q .. + 3, 16 + 4 q .. + 3), zeros past the rows. A workgroup
+// takes 64 x 64. float32: three bf16 arrays, `apart` units between them.
+template <class T>
+__global__ __launch_bounds__(256) void transpose_rows(const T *__restrict__ x, int64_t ld, int64_t rows, int64_t cols,
+                                                      uint4 *__restrict__ out, int64_t pitch, int64_t apart) {
+    constexpr int PER = 16 / sizeof(T), UNITS = 64 * 64 / PER;
+    __shared__ T tile[64][64 + PER];
     const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int u = threadIdx.x + i * 256, r = u >> 3, c = (u & 7) * 8;
-        uint4 v = zero4();
-        if (r0 + r < rows && c0 + c < cols) v = *reinterpret_cast<const uint4 *>(x + (r0 + r) * ld + c0 + c);
-        *reinterpret_cast<uint4 *>(&tile[r][c]) = v;
+    for (int i = 0; i < UNITS / 256; ++i) {
+        const int u = threadIdx.x + i * 256, r = u / (64 / PER), c = u % (64 / PER) * PER;
+        if constexpr (sizeof(T) == 2) {   // rows of whole units
+            uint4 v = zero4();
+            if (r0 + r < rows && c0 + c < cols) v = *reinterpret_cast<const uint4 *>(x + (r0 + r) * ld + c0 + c);
+            *reinterpret_cast<uint4 *>(&tile[r][c]) = v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < PER; ++e)
+                tile[r][c + e] = r0 + r < rows && c0 + c + e < cols ? x[(r0 + r) * ld + c0 + c + e] : 0.f;
+        }
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int u = threadIdx.x + i * 256, c = u >> 3, unit = u & 7, from = (unit >> 2) * 32 + (unit & 3) * 4;
         if (c0 + c >= cols) continue;
-        uint32_t w[4];
+        uint4 *to = out + ((c0 + c) * pitch + r0) / 8 + unit;
+        if constexpr (sizeof(T) == 2) {
+            uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = from + (j >> 1) * 16 + (j & 1) * 2;
-            w[j] = (uint32_t)tile[r][c] | (uint32_t)tile[r + 1][c] << 16;
+            for (int j = 0; j < 4; ++j) {
+                const int r = from + (j >> 1) * 16 + (j & 1) * 2;
+                w[j] = (uint32_t)tile[r][c] | (uint32_t)tile[r + 1][c] << 16;
+            }
+            *to = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = tile[from + (j >> 2) * 16 + (j & 3)][c];
+            uint4 t[3];
+            split_unit(v, t);
+#pragma unroll
+            for (int s = 0; s < 3; ++s) to[s * apart] = t[s];
         }
-        *reinterpret_cast<uint4 *>(out + (c0 + c) * pitch + r0 + unit * 8) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -426,13 +503,20 @@ __device__ __forceinline__ void tile_of(int64_t id, int64_t np, int64_t nl, int6
 // the staged ones.
 //
 // A step of 64 indices runs column by column (a fragment of the staged operand against all packed
-// ones), the order of everything in it fixed: a column's fragments are read two columns ahead, the
-// first two of the next step's at the end of this one, which its third stage allows; the stores of
-// the tile after next and the loads of the one behind it lie between the columns. With the stores
-// first in the step, as the order of the code suggests, all waves wait behind them after each barrier.
-template <int WP, int WL, int PF, bool KT, bool SWAP>
+// ones), the order of everything in it fixed: a column's fragments are read three columns ahead, the
+// first three of the next step's at the end of this one, which its third stage allows; the loads and
+// the stores of the tiles to come lie one by one between the columns. (In one run each, all waves queue
+// behind them: 3% slower.) Eight waves side by side along the packed rows read no packed row twice;
+// 4 x 2 waves, with half the LDS reads and twice the packed loads, are 6% slower, two workgroups of four
+// waves per CU 9%.
+//
+// TRI: float32 operands as three bf16 terms each (split3). The reduction runs over six products of
+// the terms, the small ones first; the three left out are below 2^-26 of the whole, and every
+// product of two terms is exact in float32. Six bf16 products are faster than one float32 product
+// on this card's matrix units (v_mfma_f32_16x16x4_f32, a sixteenth of the bf16 rate).
+template <int WP, int WL, int PF, int LF, bool KT, bool SWAP, bool TRI = false>
 struct Core {
-    static constexpr int LF = 8, BP = WP * PF * 16, BL = WL * LF * 16, THREADS = 64 * WP * WL;
+    static constexpr int BP = WP * PF * 16, BL = WL * LF * 16, THREADS = 64 * WP * WL;
     static constexpr int kPer = BL * 8 / THREADS;   // 16-byte units of a stage per thread
     static constexpr int kStage = BL * 8;           // units per stage
     static constexpr int kRows = KT ? THREADS / (BL / 8) : THREADS / 8;   // rows between a thread's units
@@ -445,6 +529,9 @@ struct Core {
     const uint4 *a;          // the wave's packed rows at step 0
     int64_t a_row;           // units between two blocks of packed rows
     int steps, store_at, read_at;
+    uint32_t part;           // TRI: 2^32 / the steps of one product of terms, rounded up
+    int one;                 // TRI: those steps
+    int64_t b_apart, a_apart;  // TRI: bytes, and units, between two terms
 
     // first: the staged operand at the tile's first row (KC) or column (KT); `extent` its rows from
     // there (KC) or columns (KT), `depth` the reduction's extent.
@@ -476,30 +563,47 @@ struct Core {
         a = packed + (block + wp * PF) * blocks * 64 + lane;
         a_row = blocks * 64;
     }
+    __device__ __forceinline__ void terms(int64_t b_units, int64_t a_units) {
+        one = steps;
+        part = one > 1 ? 0xffffffffu / (uint32_t)one + 1 : 0;
+        steps *= 6;
+        b_apart = b_units * 16;
+        a_apart = a_units;
+    }
+    // The product of terms that step t belongs to, and the step in it. Of the packed operand the terms
+    // 2 1 0 1 0 0, of the staged one 0 1 2 0 1 0.
+    __device__ __forceinline__ int product(int t, int &at) const {
+        const int s = one > 1 ? (int)__umulhi((uint32_t)t, part) : t;
+        at = t - s * one;
+        return s;
+    }
+    // The thread's unit C of step t, its fragment I, and the unit's place in a stage.
+    template <int C>
     __device__ __forceinline__ void load_b(int t, uint4 (&r)[kPer]) const {
+        const char *from = base;
+        int at = t;
+        if constexpr (TRI) from += (0x124 >> 2 * product(t, at) & 3) * b_apart;
         // a descriptor per step: offsets stay within a step, whatever the operand's size
-        const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(base + t * advance, t < steps ? bytes - t * advance : 0);
-        const uint32_t from = KT || t * kStep + k < limit ? off : kOOB;
-#pragma unroll
-        for (int c = 0; c < kPer; ++c) r[c] = buf_load16(rsrc, from + c * pitch);
+        const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(from + at * advance, t < steps ? bytes - at * advance : 0);
+        r[C] = buf_load16(rsrc, (KT || at * kStep + k < limit ? off : kOOB) + C * pitch);
     }
+    template <int I>
     __device__ __forceinline__ void load_a(int t, uint4 (&f)[2][PF]) const {
-        const uint4 *at = a + (int64_t)(t < steps ? t : steps - 1) * 128;
-#pragma unroll
-        for (int j = 0; j < PF; ++j)
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) f[ks][j] = at[j * a_row + ks * 64];
+        const uint4 *from = a;
+        int at = t < steps ? t : steps - 1;
+        if constexpr (TRI) from += (0x46 >> 2 * product(at, at) & 3) * a_apart;
+        f[I & 1][I >> 1] = from[(int64_t)at * 128 + (I >> 1) * a_row + (I & 1) * 64];
     }
+    template <int C>
     __device__ __forceinline__ void store_b(uint4 *stage, const uint4 (&r)[kPer]) const {
-#pragma unroll
-        for (int c = 0; c < kPer; ++c) stage[store_at + c * kRows * (KT ? BL / 8 : 8)] = r[c];
+        stage[store_at + C * kRows * (KT ? BL / 8 : 8)] = r[C];
     }
     __device__ __forceinline__ void read(const uint4 *stage, int f, uint4 (&lf)[2]) const {
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if constexpr (KT) {
                 const __attribute__((address_space(3))) char *p =
-                    (const __attribute__((address_space(3))) char *)stage + (read_at ^ f << 5) + ks * 32 * (BL * 2);
+                    (const __attribute__((address_space(3))) char *)stage + (read_at ^ (f & 7) << 5) + (f >> 3) * 256 + ks * 32 * (BL * 2);
                 const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)p);
                 const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(p + 16 * (BL * 2)));
                 const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
@@ -511,37 +615,45 @@ struct Core {
     }
     template <int F>
     __device__ __forceinline__ void columns(int t, const uint4 *cur, const uint4 *nxt, uint4 *wr, const uint4 (&af)[2][PF],
-                                            uint4 (&an)[2][PF], uint4 (&b)[kPer], uint4 (&lf)[3][2],
+                                            uint4 (&an)[2][PF], uint4 (&b)[kPer], uint4 (&lf)[4][2],
                                             f32x4 (&acc)[LF][PF]) const {
         if constexpr (F < LF) {
-            read(F + 2 < LF ? cur : nxt, (F + 2) % LF, lf[(F + 2) % 3]);
-            if constexpr (F == 0) load_a(t + 1, an);
-            if constexpr (F == 2) store_b(wr, b);
-            if constexpr (F == 3) load_b(t + 3, b);
+            read(F + 3 < LF ? cur : nxt, (F + 3) % LF, lf[(F + 3) % 4]);
+            if constexpr (F % (LF / 8) == 0 && F / (LF / 8) < 2 * PF) load_a<F / (LF / 8)>(t + 1, an);
+            if constexpr (F % (LF / 4) == LF / 8 - 1) store_b<F / (LF / 4)>(wr, b);
+            if constexpr (F % (LF / 4) == LF / 4 - 1) load_b<F / (LF / 4)>(t + 3, b);
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int j = 0; j < PF; ++j)
-                    acc[F][j] = SWAP ? mfma16x16x32(lf[F % 3][ks], af[ks][j], acc[F][j])
-                                     : mfma16x16x32(af[ks][j], lf[F % 3][ks], acc[F][j]);
+                    acc[F][j] = SWAP ? mfma16x16x32(lf[F % 4][ks], af[ks][j], acc[F][j])
+                                     : mfma16x16x32(af[ks][j], lf[F % 4][ks], acc[F][j]);
             __builtin_amdgcn_sched_barrier(0);
             columns<F + 1>(t, cur, nxt, wr, af, an, b, lf, acc);
         }
     }
-    // LF is not a multiple of 3: the fragments read ahead move to their places of the next step
     __device__ __forceinline__ void step(int t, uint4 *stages, int &at, const uint4 (&af)[2][PF], uint4 (&an)[2][PF],
-                                         uint4 (&b)[kPer], uint4 (&lf)[3][2], f32x4 (&acc)[LF][PF]) const {
+                                         uint4 (&b)[kPer], uint4 (&lf)[4][2], f32x4 (&acc)[LF][PF]) const {
         const int next = at == 2 * kStage ? 0 : at + kStage, after = next == 2 * kStage ? 0 : next + kStage;
         columns<0>(t, stages + at, stages + next, stages + after, af, an, b, lf, acc);
-        static_assert(LF % 3 == 2, "the places of the next step's first two columns");
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            const uint4 x = lf[2][ks], y = lf[0][ks];
-            lf[0][ks] = x;
-            lf[1][ks] = y;
-        }
+        static_assert(LF % 4 == 0, "the next step's first columns are in their places");
         at = next;
         __syncthreads();
+    }
+    template <int I>
+    __device__ __forceinline__ void first(uint4 *stages, uint4 (&b)[kPer], uint4 (&more)[kPer], uint4 (&af)[2][PF]) const {
+        static_assert(kPer == 4 && 2 * PF <= 8, "spread over the columns");
+        if constexpr (I < 4) {
+            load_b<I>(0, b);
+            load_b<I>(1, more);
+        } else if constexpr (I < 12) {
+            if constexpr (I - 4 < 2 * PF) load_a<I - 4>(0, af);
+        } else if constexpr (I < 16) {
+            store_b<I - 12>(stages, b);
+            store_b<I - 12>(stages + kStage, more);
+            load_b<I - 12>(2, b);
+        }
+        if constexpr (I < 15) first<I + 1>(stages, b, more, af);
     }
     __device__ __forceinline__ void run(uint4 *stages, f32x4 (&acc)[LF][PF]) const {
 #pragma unroll
@@ -549,16 +661,12 @@ struct Core {
 #pragma unroll
             for (int j = 0; j < PF; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (steps <= 0) return;
-        uint4 b[kPer], more[kPer], a0[2][PF], a1[2][PF], lf[3][2];
-        load_b(0, b);
-        load_b(1, more);
-        load_a(0, a0);
-        store_b(stages, b);
-        store_b(stages + kStage, more);
-        load_b(2, b);
+        uint4 b[kPer], more[kPer], a0[2][PF], a1[2][PF], lf[4][2];
+        first<0>(stages, b, more, a0);
         __syncthreads();
         read(stages, 0, lf[0]);
         read(stages, 1, lf[1]);
+        read(stages, 2, lf[2]);
         int t = 0, at = 0;
         for (; t + 1 < steps; t += 2) {
             step(t, stages, at, a0, a1, b, lf, acc);
@@ -572,8 +680,9 @@ struct Core {
 enum { STATS = 0, EXP = 1, GRAD = 2 };
 
 struct LogitsParams {
-    const uint16_t *head;
+    const uint16_t *head;      // from v0 on
     int64_t ld, width, vocab;
+    int64_t head_apart, packed_apart, piece_apart;   // TRI: units between two terms
     const uint4 *packed;       // hidden rows
     int64_t blocks;            // of 32 along the width
     int64_t v0, v1;            // the piece's entries
@@ -599,13 +708,26 @@ __device__ __forceinline__ float shift_of(float top) {
     return fabsf(top) < 1e6f ? 96.f * ceilf((top - 48.f) * (1.f / 96.f)) - 32.f : top;
 }
 
-// A wave's entries: which of its 64 (or 16 PF) rows x 128 vocabulary entries are targets, as bits in
-// LDS [row][4], one lane per row.
-template <int ROWS>
-__device__ __forceinline__ void mark_targets(const LogitsParams &p, int64_t row0, int64_t unit, uint32_t *bits, int lane) {
-    if (lane < ROWS) {
+template <bool TRI>
+__device__ __forceinline__ void store_unit(uint4 *to, int64_t apart, const float (&v)[8]) {
+    if constexpr (TRI) {
+        uint4 t[3];
+        split_unit(v, t);
+#pragma unroll
+        for (int s = 0; s < 3; ++s) to[s * apart] = t[s];
+    } else {
+        *to = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    }
+}
+
+// Which of a wave's rows x units of 128 vocabulary entries are targets, as bits in LDS [row][unit][4],
+// a lane per row and unit.
+template <int ROWS, int UNITS>
+__device__ __forceinline__ void mark_targets(const LogitsParams &p, int64_t row0, int64_t unit0, uint32_t *bits, int lane) {
+    static_assert(ROWS * UNITS <= 64, "a lane each");
+    if (lane < ROWS * UNITS) {
         uint32_t w[4] = {0, 0, 0, 0};
-        const int64_t row = row0 + lane;
+        const int64_t row = row0 + lane / UNITS, unit = unit0 + lane % UNITS;
         if (row < p.rows && unit < p.units) {
             const uint16_t *at = p.first + row * (p.units + 1) + unit;
             for (int e = at[0]; e < at[1]; ++e) {
@@ -615,8 +737,7 @@ __device__ __forceinline__ void mark_targets(const LogitsParams &p, int64_t row0
                     if (v >> 5 == i) w[i] |= 1u << (v & 31);
             }
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) bits[lane * 4 + i] = w[i];
+        *reinterpret_cast<uint4 *>(bits + lane * 4) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -629,132 +750,139 @@ __device__ __forceinline__ int64_t place_of(const LogitsParams &p, int64_t row, 
     return row * p.entries + n;
 }
 
-template <int WP, int WL, int PF, int MODE>
+template <int WP, int WL, int PF, int LF, int MODE, bool TRI>
 __global__ __launch_bounds__(64 * WP * WL) void logits_kernel(const LogitsParams p) {
-    using C = Core<WP, WL, PF, false, MODE != GRAD>;
+    using C = Core<WP, WL, PF, LF, false, MODE != GRAD, TRI>;
+    constexpr int UNITS = LF / 8;   // of a wave
     __shared__ uint4 stages[3 * C::kStage];
-    __shared__ uint32_t marks[WP * WL][PF * 16 * 4];
+    __shared__ uint4 marks[WP * WL][PF * 16 * UNITS];
     int64_t tp, tl;
     tile_of(blockIdx.x, p.np, p.nl, tp, tl);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wp = wave % WP, wl = wave / WP, q = lane >> 4;
     const int64_t v0 = p.v0 + tl * C::BL, left = p.v1 - v0;
+    const int64_t row0 = tp * C::BP + wp * PF * 16;
+    uint32_t *wave_bits = reinterpret_cast<uint32_t *>(marks[wave]);
+    mark_targets<PF * 16, UNITS>(p, row0, (v0 + wl * LF * 16) / kUnit, wave_bits, lane);
     C core;
-    core.init(p.head + v0 * p.ld, p.ld, left, p.width, p.packed, tp * (C::BP / 16), p.blocks, wave);
-    f32x4 acc[C::LF][PF];
+    core.init(p.head + (v0 - p.v0) * p.ld, p.ld, left, p.width, p.packed, tp * (C::BP / 16), p.blocks, wave);
+    if constexpr (TRI) core.terms(p.head_apart, p.packed_apart);
+    f32x4 acc[LF][PF];
     core.run(stages, acc);
 
-    const int64_t row0 = tp * C::BP + wp * PF * 16, u0 = v0 + wl * kUnit, unit = u0 / kUnit;
-    uint32_t *bits = marks[wave];
-    mark_targets<PF * 16>(p, row0, unit, bits, lane);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the lanes read each other's marks
-    const int valid = (int)(p.v1 - u0 < kUnit ? (p.v1 > u0 ? p.v1 - u0 : 0) : kUnit);
 
-    if constexpr (MODE == GRAD) {
-        // lane: entry l % 16 of fragment f, rows 4 q + i of packed fragment j
 #pragma unroll
-        for (int jj = 0; jj < PF; ++jj) {
+    for (int u = 0; u < UNITS; ++u) {
+        const int64_t u0 = v0 + (wl * UNITS + u) * kUnit, unit = u0 / kUnit;
+        const int valid = (int)(p.v1 - u0 < kUnit ? (p.v1 > u0 ? p.v1 - u0 : 0) : kUnit);
+        if constexpr (MODE == GRAD) {
+            // lane: entry l % 16 of fragment f, rows 4 q + i of packed fragment j
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int local = jj * 16 + 4 * q + i;
-                const int64_t row = row0 + local;
-                const float c = p.shift[row], factor = p.factor[row];
+            for (int j = 0; j < PF; ++j) {
 #pragma unroll
-                for (int f = 0; f < C::LF; ++f) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[f][jj][i], p.scale, -c)) * factor;
-                    acc[f][jj][i] = 16 * f + (lane & 15) < valid ? e : 0.f;
-                }
-                const uint4 m = *reinterpret_cast<const uint4 *>(bits + local * 4);
-                const uint32_t w[4] = {m.x, m.y, m.z, m.w};
-                if (__builtin_amdgcn_ballot_w64(((w[0] | w[1] | w[2] | w[3]) >> (lane & 15) & 0x00010001u) != 0)) {
-                    const float inverse = p.inverse[row];   // 0 past the rows, which have no targets
+                for (int i = 0; i < 4; ++i) {
+                    const int local = j * 16 + 4 * q + i;
+                    const int64_t row = row0 + local;
+                    const float c = p.shift[row], factor = p.factor[row];
 #pragma unroll
-                    for (int f = 0; f < C::LF; ++f) {
-                        const int bit = 16 * f + (lane & 15);
-                        if (w[f >> 1] >> (bit & 31) & 1)
-                            acc[f][jj][i] = inverse * p.chosen[place_of(p, row, unit, bits + local * 4, bit)];
+                    for (int f = 0; f < 8; ++f) {
+                        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[8 * u + f][j][i], p.scale, -c)) * factor;
+                        acc[8 * u + f][j][i] = 16 * f + (lane & 15) < valid ? e : 0.f;
+                    }
+                    const uint32_t *bits = wave_bits + (local * UNITS + u) * 4;
+                    const uint4 m = *reinterpret_cast<const uint4 *>(bits);
+                    const uint32_t w[4] = {m.x, m.y, m.z, m.w};
+                    if (__builtin_amdgcn_ballot_w64(((w[0] | w[1] | w[2] | w[3]) >> (lane & 15) & 0x00010001u) != 0)) {
+                        const float inverse = p.inverse[row];   // 0 past the rows, which have no targets
+#pragma unroll
+                        for (int f = 0; f < 8; ++f) {
+                            const int bit = 16 * f + (lane & 15);
+                            if (w[f >> 1] >> (bit & 31) & 1)
+                                acc[8 * u + f][j][i] = inverse * p.chosen[place_of(p, row, unit, bits, bit)];
+                        }
                     }
                 }
             }
-        }
-        static_assert(PF == 1 || PF % 2 == 0, "pairs of packed fragments");
-        if constexpr (PF % 2 == 0) {
 #pragma unroll
-            for (int jj = 0; jj < PF; jj += 2)
-#pragma unroll
-                for (int f = 0; f < C::LF; ++f) {
-                    const f32x4 x = acc[f][jj], y = acc[f][jj + 1];
-                    p.piece[(((u0 - p.v0) / 16 + f) * p.piece_blocks + row0 / 32 + jj / 2) * 64 + lane] =
-                        make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(y[0], y[1]),
-                                   pack_bf16x2(y[2], y[3]));
-                }
-        } else {   // half a unit: the other half is the wave's that holds the next 16 rows
-#pragma unroll
-            for (int f = 0; f < C::LF; ++f) {
-                const f32x4 x = acc[f][0];
+            for (int f = 0; f < 8; ++f) {
                 uint4 *to = p.piece + (((u0 - p.v0) / 16 + f) * p.piece_blocks + row0 / 32) * 64 + lane;
-                reinterpret_cast<uint2 *>(to)[(row0 / 16) & 1] = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
-            }
-        }
-    } else {
-        // lane: row l % 16 of packed fragment j, entries 4 q + i of fragment f
-        if (valid < kUnit) {
+                if constexpr (PF == 1) {   // half a unit: the other half is the wave's that holds the next 16 rows
+                    const f32x4 x = acc[8 * u + f][0];
+                    const float v[8] = {x[0], x[1], x[2], x[3]};
+                    uint4 t[3];
+                    if constexpr (TRI) split_unit(v, t);
+                    else t[0] = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), 0, 0);
 #pragma unroll
-            for (int f = 0; f < C::LF; ++f)
+                    for (int s = 0; s < (TRI ? 3 : 1); ++s)
+                        reinterpret_cast<uint2 *>(to + s * p.piece_apart)[(row0 / 16) & 1] = make_uint2(t[s].x, t[s].y);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (16 * f + 4 * q + i >= valid)
-#pragma unroll
-                        for (int j = 0; j < PF; ++j) acc[f][j][i] = -INFINITY;
-        }
-#pragma unroll
-        for (int j = 0; j < PF; ++j) {
-            const int local = j * 16 + (lane & 15);
-            const int64_t row = row0 + local;
-            const uint4 m = *reinterpret_cast<const uint4 *>(bits + local * 4);
-            const uint32_t w[4] = {m.x, m.y, m.z, m.w};
-            float top = acc[0][j][0];
-#pragma unroll
-            for (int f = 0; f < C::LF; ++f)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, acc[f][j][i]);
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            // exponents are taken relative to the unit's own maximum, where they are exact to their
-            // own size, and brought to the shift by a power of two
-            const float near = fmaxf(ceilf(top * p.scale), kNone), c = shift_of(near);
-            const float by = near == c ? 1.f : ldexpf(1.f, (int)(near - c));
-            float sum = 0.f;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {   // 32 entries: two fragments
-                float e[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[2 * g + i / 4][j][i % 4], p.scale, -near));
+                    for (int j = 0; j < PF; j += 2) {
+                        const f32x4 x = acc[8 * u + f][j], y = acc[8 * u + f][j + 1];
+                        store_unit<TRI>(to + j / 2 * 64, p.piece_apart, {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
+                    }
                 }
-                const uint32_t mine = w[g] >> (4 * q) & 0x000f000fu;
-                if (mine) {
+            }
+        } else {
+            // lane: row l % 16 of packed fragment j, entries 4 q + i of fragment f
+            if (valid < kUnit) {
+#pragma unroll
+                for (int f = 0; f < 8; ++f)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (16 * f + 4 * q + i >= valid)
+#pragma unroll
+                            for (int j = 0; j < PF; ++j) acc[8 * u + f][j][i] = -INFINITY;
+            }
+#pragma unroll
+            for (int j = 0; j < PF; ++j) {
+                const int local = j * 16 + (lane & 15);
+                const int64_t row = row0 + local;
+                const uint32_t *bits = wave_bits + (local * UNITS + u) * 4;
+                const uint4 m = *reinterpret_cast<const uint4 *>(bits);
+                const uint32_t w[4] = {m.x, m.y, m.z, m.w};
+                float top = acc[8 * u][j][0];
+#pragma unroll
+                for (int f = 0; f < 8; ++f)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = fmaxf(top, acc[8 * u + f][j][i]);
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                // exponents are taken relative to the unit's own maximum, where they are exact to
+                // their own size, and brought to the shift by a power of two
+                const float near = fmaxf(ceilf(top * p.scale), kNone), c = shift_of(near);
+                const float by = near == c ? 1.f : ldexpf(1.f, (int)(near - c));
+                float sum = 0.f;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {   // 32 entries: two fragments
+                    float e[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (mine >> (16 * (i / 4) + i % 4) & 1) {
-                            p.chosen[place_of(p, row, unit, bits + local * 4, 32 * g + 16 * (i / 4) + 4 * q + i % 4)] =
-                                acc[2 * g + i / 4][j][i % 4];
-                            e[i] = 0.f;
-                        }
-                }
+                        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[8 * u + 2 * g + i / 4][j][i % 4], p.scale, -near));
+                    const uint32_t mine = w[g] >> (4 * q) & 0x000f000fu;
+                    if (mine) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    sum += e[i];
-                    e[i] *= by;
+                        for (int i = 0; i < 8; ++i)
+                            if (mine >> (16 * (i / 4) + i % 4) & 1) {
+                                p.chosen[place_of(p, row, unit, bits, 32 * g + 16 * (i / 4) + 4 * q + i % 4)] =
+                                    acc[8 * u + 2 * g + i / 4][j][i % 4];
+                                e[i] = 0.f;
+                            }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        sum += e[i];
+                        e[i] *= by;
+                    }
+                    if constexpr (MODE == EXP)
+                        store_unit<TRI>(p.piece + ((row0 / 16 + j) * p.piece_blocks + (u0 - p.v0) / 32 + g) * 64 + lane,
+                                        p.piece_apart, e);
                 }
-                if constexpr (MODE == EXP)
-                    p.piece[((row0 / 16 + j) * p.piece_blocks + (u0 - p.v0) / 32 + g) * 64 + lane] =
-                        make_uint4(pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]),
-                                   pack_bf16x2(e[6], e[7]));
+                sum += __shfl_xor(sum, 16, 64);
+                sum += __shfl_xor(sum, 32, 64);
+                if (q == 0) p.stats[(u0 - p.v0) / kUnit * p.rows_pad + row] = make_float2(c, sum * by);
             }
-            sum += __shfl_xor(sum, 16, 64);
-            sum += __shfl_xor(sum, 32, 64);
-            if (q == 0) p.stats[(u0 - p.v0) / kUnit * p.rows_pad + row] = make_float2(c, sum * by);
         }
     }
 }
@@ -764,7 +892,8 @@ __global__ __launch_bounds__(64 * WP * WL) void logits_kernel(const LogitsParams
 // brought to it, and `factor` is what the sums of the pieces before are brought to it with.
 __global__ __launch_bounds__(1024) void join_kernel(const float2 *__restrict__ stats, int units, int64_t rows_pad,
                                                    float *__restrict__ shift, float *__restrict__ total,
-                                                   float *__restrict__ factor, uint4 *piece, int64_t piece_blocks) {
+                                                   float *__restrict__ factor, uint4 *piece, int64_t piece_blocks,
+                                                    int terms, int64_t apart) {
     __shared__ float part[64][17];
     const int r = threadIdx.x & 15, g = threadIdx.x >> 4;
     const int64_t row = (int64_t)blockIdx.x * 16 + r;
@@ -788,8 +917,8 @@ __global__ __launch_bounds__(1024) void join_kernel(const float2 *__restrict__ s
         const float by = __builtin_amdgcn_exp2f(s.x - c);
         sum += s.y * by;
         if (!piece) continue;
-        for (int i = 0; i < kUnit / 8; ++i) {   // the row's 16 units of 16 bytes
-            uint4 *e = piece + (row / 16 * piece_blocks + u * (kUnit / 32) + i / 4) * 64 + (i % 4) * 16 + r;
+        for (int i = 0; i < kUnit / 8 * terms; ++i) {   // the row's 16 units of 16 bytes, term by term
+            uint4 *e = piece + i / 16 * apart + (row / 16 * piece_blocks + u * (kUnit / 32) + i % 16 / 4) * 64 + i % 4 * 16 + r;
             uint4 v = *e;
             uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -817,7 +946,7 @@ struct ProductParams {
     int64_t ld, depth, cols;
     bool kt;
     const uint4 *packed;       // [rows, depth]
-    int64_t blocks;
+    int64_t blocks, b_apart, packed_apart;   // TRI: units between two terms
     int64_t np, nl;
     int64_t rows;
     void *out;
@@ -828,9 +957,9 @@ struct ProductParams {
 };
 
 // out[row, col] (= factor out +) sum_k packed(row, k) b(k, col), one split of the reduction per y.
-template <int WP, int WL, int PF, bool KT, int OUT>
+template <int WP, int WL, int PF, int LF, bool KT, int OUT, bool TRI>
 __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductParams p) {
-    using C = Core<WP, WL, PF, KT, true>;
+    using C = Core<WP, WL, PF, LF, KT, true, TRI>;
     __shared__ uint4 stages[3 * C::kStage];
     int64_t tp, tl;
     tile_of(blockIdx.x, p.np, p.nl, tp, tl);
@@ -844,7 +973,8 @@ __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductPara
     const int64_t depth = (end < p.steps ? (int64_t)end * kStep : p.depth) - k0;   // none: an empty split
     core.init(p.b + (KT ? k0 * p.ld + tl * C::BL : tl * C::BL * p.ld + k0), p.ld, p.cols - tl * C::BL, depth,
               p.packed + (int64_t)beg * 128, tp * (C::BP / 16), p.blocks, wave);
-    f32x4 acc[C::LF][PF];
+    if constexpr (TRI) core.terms(p.b_apart, p.packed_apart);
+    f32x4 acc[LF][PF];
     core.run(stages, acc);
 #pragma unroll
     for (int j = 0; j < PF; ++j) {
@@ -852,8 +982,8 @@ __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductPara
         if (row >= p.rows) continue;
         const float factor = p.factor ? p.factor[row] : 0.f;
 #pragma unroll
-        for (int f = 0; f < C::LF; ++f) {
-            const int64_t col = tl * C::BL + (wl * C::LF + f) * 16 + 4 * q;
+        for (int f = 0; f < LF; ++f) {
+            const int64_t col = tl * C::BL + (wl * LF + f) * 16 + 4 * q;
             if (col >= p.cols) continue;
             f32x4 v = acc[f][j];
             if constexpr (OUT == CT_F32) {
@@ -1080,8 +1210,15 @@ __global__ __launch_bounds__(256) void hidden_grad_kernel(const float *__restric
     }
 }
 
-hipError_t transpose(const uint16_t *x, int64_t ld, int64_t rows, int64_t cols, uint16_t *out, int64_t pitch, hipStream_t s) {
-    transpose_rows<<<dim3((unsigned)cdiv(rows, 64), (unsigned)cdiv(cols, 64)), dim3(256), 0, s>>>(x, ld, rows, cols, out, pitch);
+// The term arrays of float32 rows lie `terms_apart` 16-byte units apart.
+hipError_t transpose(const void *x, int dtype, int64_t ld, int64_t rows, int64_t cols, void *out, int64_t pitch,
+                     hipStream_t s) {
+    const dim3 grid((unsigned)cdiv(rows, 64), (unsigned)cdiv(cols, 64));
+    uint4 *to = static_cast<uint4 *>(out);
+    if (dtype == CT_F32)
+        transpose_rows<<<grid, dim3(256), 0, s>>>(static_cast<const float *>(x), ld, rows, cols, to, pitch, cols * pitch / 8);
+    else
+        transpose_rows<<<grid, dim3(256), 0, s>>>(static_cast<const uint16_t *>(x), ld, rows, cols, to, pitch, (int64_t)0);
     return hipGetLastError();
 }
 
@@ -1093,22 +1230,30 @@ T *at(void *base, int64_t offset) {
 template <int MODE>
 hipError_t launch_logits(const Plan &pl, const LogitsParams &p, hipStream_t s) {
     const dim3 grid((unsigned)(p.np * p.nl));
-    if (pl.bp == 64) logits_kernel<4, 1, 1, MODE><<<grid, dim3(256), 0, s>>>(p);
-    else if (pl.bp == 128) logits_kernel<4, 2, 2, MODE><<<grid, dim3(512), 0, s>>>(p);
-    else logits_kernel<4, 2, 4, MODE><<<grid, dim3(512), 0, s>>>(p);
+    if (pl.bp == 64) logits_kernel<4, 1, 1, 8, MODE, false><<<grid, dim3(256), 0, s>>>(p);
+    else if (pl.bp == 128 && pl.tri) logits_kernel<8, 1, 1, 16, MODE, true><<<grid, dim3(512), 0, s>>>(p);
+    else if (pl.bp == 128) logits_kernel<8, 1, 1, 16, MODE, false><<<grid, dim3(512), 0, s>>>(p);
+    else if (pl.tri) logits_kernel<8, 1, 2, 16, MODE, true><<<grid, dim3(512), 0, s>>>(p);
+    else logits_kernel<8, 1, 2, 16, MODE, false><<<grid, dim3(512), 0, s>>>(p);
     return hipGetLastError();
 }
-template <int OUT, bool KT>
+template <int OUT, bool KT, bool TRI>
 hipError_t launch_product(int bp, const ProductParams &p, int splits, hipStream_t s) {
     const dim3 grid((unsigned)(p.np * p.nl), (unsigned)splits);
-    if (bp == 64) product_kernel<4, 1, 1, KT, OUT><<<grid, dim3(256), 0, s>>>(p);
-    else if (bp == 128 || KT) product_kernel<4, 2, 2, KT, OUT><<<grid, dim3(512), 0, s>>>(p);
-    else product_kernel<4, 2, 4, KT, OUT><<<grid, dim3(512), 0, s>>>(p);
+    if constexpr (KT) {
+        if (bp == 64) product_kernel<4, 1, 1, 8, true, OUT, false><<<grid, dim3(256), 0, s>>>(p);
+        else product_kernel<8, 1, 1, 16, true, OUT, false><<<grid, dim3(512), 0, s>>>(p);
+    } else {
+        if (bp == 128) product_kernel<8, 1, 1, 16, false, OUT, TRI><<<grid, dim3(512), 0, s>>>(p);
+        else product_kernel<8, 1, 2, 16, false, OUT, TRI><<<grid, dim3(512), 0, s>>>(p);
+    }
     return hipGetLastError();
 }
 template <int OUT>
-hipError_t launch_product(int bp, const ProductParams &p, int splits, hipStream_t s) {
-    return p.kt ? launch_product<OUT, true>(bp, p, splits, s) : launch_product<OUT, false>(bp, p, splits, s);
+hipError_t launch_product(const Plan &pl, const ProductParams &p, int splits, hipStream_t s) {
+    if constexpr (OUT == CT_F32)
+        if (pl.tri) return launch_product<OUT, false, true>(pl.bp, p, splits, s);
+    return p.kt ? launch_product<OUT, true, false>(pl.bp, p, splits, s) : launch_product<OUT, false, false>(pl.bp, p, splits, s);
 }
 
 int check(const ct_head_loss *a, bool hidden) {
@@ -1149,9 +1294,11 @@ int check_sizes(int64_t count, int64_t width, int64_t vocab, int32_t entries, in
 
 LogitsParams logits_params(const ct_head_loss *a, const Plan &pl, const Kept &k, const Scratch &sc, void *kept, void *ws) {
     LogitsParams p{};
-    p.head = static_cast<const uint16_t *>(a->head);
-    p.ld = a->ld_head;
-    p.width = pl.width;
+    p.ld = pl.tri ? up(pl.width, 8) : a->ld_head;
+    p.width = up(pl.width, 8);
+    p.head_apart = pl.piece * p.ld / 8;
+    p.packed_apart = pl.rows_pad * pl.width_pad / 8;
+    p.piece_apart = pl.rows_pad * pl.piece / 8;
     p.vocab = pl.vocab;
     p.packed = at<const uint4>(ws, sc.packed);
     p.blocks = pl.width_pad / 32;
@@ -1172,10 +1319,33 @@ LogitsParams logits_params(const ct_head_loss *a, const Plan &pl, const Kept &k,
 hipError_t pack_hidden(const ct_head_loss *a, const Plan &pl, void *packed, hipStream_t stream) {
     const int64_t units = pl.rows_pad / 16 * (pl.width_pad / 32) * 64;
     const Source src = source(a);
+    if (pl.tri) {
+        pack_split<<<dim3((unsigned)cdiv(units, 256)), dim3(256), 0, stream>>>(src, pl.width_pad / 32,
+                                                                              static_cast<uint4 *>(packed), units);
+        return hipGetLastError();
+    }
     const bool vec = a->hidden_width % 8 == 0 && a->ld_hidden % 8 == 0 && reinterpret_cast<uintptr_t>(a->hidden) % 16 == 0;
     const dim3 grid((unsigned)cdiv(units, 256));
     if (vec) pack_rows<true><<<grid, dim3(256), 0, stream>>>(src, pl.width_pad / 32, static_cast<uint4 *>(packed), units);
     else pack_rows<false><<<grid, dim3(256), 0, stream>>>(src, pl.width_pad / 32, static_cast<uint4 *>(packed), units);
+    return hipGetLastError();
+}
+// The piece of the head that starts at entry v0, as the logits kernel stages it: in place, or float32
+// rows in their three terms.
+hipError_t head_piece(const ct_head_loss *a, const Plan &pl, LogitsParams &p, int64_t v0, int64_t cols, void *split,
+                      hipStream_t stream) {
+    p.v0 = v0;
+    p.v1 = v0 + cols;
+    p.nl = cdiv(cols, pl.bl);
+    if (!pl.tri) {
+        p.head = static_cast<const uint16_t *>(a->head) + v0 * a->ld_head;
+        return hipSuccess;
+    }
+    p.head = static_cast<const uint16_t *>(split);
+    const int64_t units = cols * (p.ld / 8);
+    split_rows<<<dim3((unsigned)cdiv(units, 256)), dim3(256), 0, stream>>>(
+        static_cast<const float *>(a->head) + v0 * a->ld_head, a->ld_head, cols, pl.width, static_cast<uint4 *>(split), p.ld,
+        p.head_apart);
     return hipGetLastError();
 }
 // The loss's rows one after the other: as they lie, or gathered into `to`.
@@ -1238,7 +1408,7 @@ extern "C" int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t 
     else targets(targets_kernel<256>, 256);
     CT_TRY(hipGetLastError());
 
-    if (pl.dtype == CT_F32) {
+    if (pl.dtype == CT_F32 && !pl.tri) {
         const float scale = (float)(1.4426950408889634074 / a->temperature);
         float *piece = at<float>(workspace, sc.piece);
         const float *head = static_cast<const float *>(a->head);
@@ -1262,29 +1432,30 @@ extern "C" int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t 
     } else {
         CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), stream));
         LogitsParams p = logits_params(a, pl, k, sc, kept, workspace);
-        const int64_t piece = hidden_grad ? pl.piece : pl.vocab;
+        const int64_t piece = hidden_grad || pl.tri ? pl.piece : pl.vocab;
         for (int64_t v0 = 0; v0 < pl.vocab; v0 += piece) {
             const int64_t cols = pl.vocab - v0 < piece ? pl.vocab - v0 : piece;
-            p.v0 = v0;
-            p.v1 = v0 + cols;
-            p.nl = cdiv(cols, pl.bl);
-            p.piece_blocks = up(cols, pl.bl) / 32;
+            CT_TRY(head_piece(a, pl, p, v0, cols, at<void>(workspace, sc.split), stream));
+            p.piece_blocks = pl.piece / 32;
             CT_TRY(hidden_grad ? launch_logits<EXP>(pl, p, stream) : launch_logits<STATS>(pl, p, stream));
             join_kernel<<<dim3((unsigned)(pl.rows_pad / 16)), dim3(1024), 0, stream>>>(
                 p.stats, (int)cdiv(cols, kUnit), pl.rows_pad, shift, total, factor, hidden_grad ? p.piece : nullptr,
-                p.piece_blocks);
+                p.piece_blocks, pl.terms, p.piece_apart);
             CT_TRY(hipGetLastError());
             if (!hidden_grad) continue;
             ProductParams g{};
-            g.b = p.head + v0 * p.ld;
+            g.b = p.head;
             g.ld = p.ld;
             g.kt = !pl.turned;
             if (pl.turned) {
                 uint16_t *turned = at<uint16_t>(workspace, sc.turned);
-                CT_TRY(transpose(g.b, g.ld, cols, pl.width, turned, pl.piece, stream));
+                const void *from = static_cast<const char *>(a->head) + v0 * a->ld_head * (pl.tri ? 4 : 2);
+                CT_TRY(transpose(from, pl.dtype, a->ld_head, cols, pl.width, turned, pl.piece, stream));
                 g.b = turned;
                 g.ld = pl.piece;
             }
+            g.b_apart = pl.width * pl.piece / 8;
+            g.packed_apart = p.piece_apart;
             g.depth = pl.turned ? up(cols, kStep) : cols;   // turned rows end with a whole step, in their order
             g.cols = pl.width;
             g.packed = p.piece;
@@ -1299,7 +1470,7 @@ extern "C" int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t 
             g.steps_per_split = (int)cdiv(g.steps, pl.splits);
             g.factor = v0 ? factor : nullptr;
             g.vec = pl.width % 4 == 0;
-            CT_TRY(launch_product<CT_F32>(pl.bp, g, pl.splits, stream));
+            CT_TRY(launch_product<CT_F32>(pl, g, pl.splits, stream));
         }
     }
     row_loss<<<dim3((unsigned)pl.rows), dim3(64), 0, stream>>>(
@@ -1359,7 +1530,7 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
         at<const float>(kept, k.weight), at<const float>(kept, k.mass), at<const float>(kept, k.shift),
         at<const float>(kept, k.total), upstream, inverse_t, pl.rows, pl.rows_pad, near, factor, inverse);
     CT_TRY(hipGetLastError());
-    if (pl.dtype == CT_F32) {
+    if (pl.dtype == CT_F32 && !pl.tri) {
         const float scale = (float)(1.4426950408889634074 / a->temperature);
         float *piece = at<float>(workspace, sc.piece), *out = static_cast<float *>(d_head);
         const float *head = static_cast<const float *>(a->head);
@@ -1392,20 +1563,20 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
     p.piece_blocks = pl.rows_pad / 32;
     if (pl.turned) {
         uint16_t *turned = at<uint16_t>(workspace, sc.turned);
-        CT_TRY(transpose(static_cast<const uint16_t *>(hidden), ld, pl.rows, pl.width, turned, up(pl.rows, kStep), stream));
+        CT_TRY(transpose(hidden, pl.dtype, ld, pl.rows, pl.width, turned, up(pl.rows, kStep), stream));
         hidden = turned;
         ld = up(pl.rows, kStep);
     }
     for (int64_t v0 = 0; v0 < pl.vocab; v0 += pl.piece) {
         const int64_t cols = pl.vocab - v0 < pl.piece ? pl.vocab - v0 : pl.piece;
-        p.v0 = v0;
-        p.v1 = v0 + cols;
-        p.nl = cdiv(cols, pl.bl);
+        CT_TRY(head_piece(a, pl, p, v0, cols, at<void>(workspace, sc.split), stream));
         CT_TRY(launch_logits<GRAD>(pl, p, stream));
         ProductParams g{};
         g.b = static_cast<const uint16_t *>(hidden);
         g.ld = ld;
         g.kt = !pl.turned;
+        g.b_apart = pl.width * up(pl.rows, kStep) / 8;
+        g.packed_apart = p.piece_apart;
         g.depth = pl.turned ? up(pl.rows, kStep) : pl.rows;
         g.cols = d_head_width;
         g.packed = p.piece;
@@ -1417,8 +1588,8 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
         g.ldo = ld_d_head;
         g.steps = g.steps_per_split = (int)cdiv(pl.rows, kStep);
         g.vec = ld_d_head % 4 == 0 && reinterpret_cast<uintptr_t>(d_head) % 16 == 0;
-        CT_TRY(d_head_dtype == CT_F32 ? launch_product<CT_F32>(pl.bp, g, 1, stream)
-                                      : launch_product<CT_BF16>(pl.bp, g, 1, stream));
+        CT_TRY(d_head_dtype == CT_F32 ? launch_product<CT_F32>(pl, g, 1, stream)
+                                      : launch_product<CT_BF16>(pl, g, 1, stream));
     }
     return 0;
 }
