@@ -28,8 +28,7 @@
 // product that follows reads its LDS tile in that order.
 //
 // float32. Operands are split into three bf16 terms, which hold them exactly, and take the same
-// kernels (Core, TRI). Up to 64 rows, where reading the head bounds and splitting it would cost more,
-// the products are ct_gemm_f32's over a piece of logits in the workspace, with a row pass between them.
+// kernels (Core, TRI).
 //
 // Every sum runs in a fixed order: repeated calls are bit-identical.
 
@@ -43,7 +42,10 @@ namespace {
 constexpr int kStep = 64;              // reduction indices per step of a product
 constexpr int kUnit = 128;             // vocabulary entries per (row, unit) pair of statistics
 constexpr int kMaxEntries = 1024;
-constexpr int64_t kFewRows = 64;       // float32: up to here on ct_gemm_f32
+// bf16: up to so many rows, where reading the head bounds, the exponentials (twice as many: the
+// derivative) are kept in two bf16 terms. One rounding, by up to 2^-8, of the one or two large values
+// that a row has would show in the gradients of few rows; of many rows they average.
+constexpr int64_t kTwoTerms = 128;
 constexpr int64_t kMaxWidth = 65536, kMaxVocab = (int64_t{1} << 31) - 1024, kMaxRows = int64_t{1} << 30;
 // E of one piece, in bytes: what two passes over it can share through the 256 MB last-level cache.
 constexpr int64_t kPieceBytes = int64_t{256} << 20;
@@ -61,7 +63,7 @@ struct Plan {
     int splits;             // of the hidden gradient's reduction
     bool turned;            // the second products read their staged operand transposed
     bool tri;               // float32 in three bf16 terms
-    int terms;
+    int terms[3];           // bf16 terms of a piece's values, by sweep
 };
 
 // Workgroups' worth of work in whole rounds: how many splits of a reduction of `steps` leave the
@@ -92,20 +94,19 @@ Plan plan_of(int64_t rows, int64_t width, int64_t vocab, int64_t entries, int dt
     p.rows_pad = up(rows, p.bp);
     p.width_pad = up(width, kStep);
     p.units = cdiv(vocab, kUnit);
-    p.tri = dtype == CT_F32 && rows > kFewRows;
-    p.terms = p.tri ? 3 : 1;
-    const int64_t element = p.tri ? 6 : dtype == CT_F32 ? 4 : 2;
+    p.tri = dtype == CT_F32;
+    p.terms[0] = 1;
+    p.terms[1] = p.tri ? 3 : rows <= kTwoTerms ? 2 : 1;
+    p.terms[2] = p.tri ? 3 : rows <= 2 * kTwoTerms ? 2 : 1;
+    const int64_t element = 2 * p.terms[2];
     int64_t most = kPieceBytes / (p.rows_pad * element) / 256 * 256;
     if (most < 1024) most = 1024;
     p.pieces = cdiv(vocab, most);
     p.piece = up(cdiv(vocab, p.pieces), 256);
     p.pieces = cdiv(vocab, p.piece);
-    p.splits = 1;
-    p.turned = p.tri || (dtype == CT_BF16 && p.bp == 256);
-    if (dtype == CT_BF16 || p.tri) {
-        const int64_t tiles = p.rows_pad / p.bp * cdiv(width, p.bl);
-        p.splits = splits_for(tiles, p.bp == 64 ? 512 : 256, p.piece / kStep);
-    }
+    p.turned = p.tri ? p.bp > 64 : p.bp == 256;
+    const int64_t tiles = p.rows_pad / p.bp * cdiv(width, p.bl);
+    p.splits = splits_for(tiles, p.bp == 64 ? 512 : 256, p.piece / kStep);
     return p;
 }
 
@@ -144,14 +145,15 @@ struct Scratch {
 Scratch scratch_of(const Plan &p, int sweep) {
     Regions r;
     Scratch s{};
-    const bool gemm = p.dtype == CT_F32 && !p.tri;
-    const int64_t terms = 2 * p.terms, piece = sweep || p.tri ? p.piece : up(p.units, 2) * kUnit;
-    s.packed = r.take(gemm ? 0 : p.rows_pad * p.width_pad * terms);
-    s.plain = r.take(gemm || (p.tri && sweep == 2) ? p.rows * p.width * 4 : sweep == 2 ? p.rows * p.width * 2 : 0);
-    s.piece = r.take(gemm ? p.rows * p.piece * 4 : sweep ? p.rows_pad * p.piece * terms : 0);
-    s.turned = r.take(p.turned && sweep ? p.width * terms * (sweep == 1 ? p.piece : up(p.rows, kStep)) : 0);
-    s.split = r.take(p.tri ? p.piece * up(p.width, 8) * terms : 0);
-    s.stats = r.take(gemm || sweep == 2 ? 0 : piece / kUnit * p.rows_pad * 8);
+    const int64_t terms = p.tri ? 6 : 2, pitch = up(p.width, 8), steps = up(p.rows, kStep);
+    const int64_t piece = sweep || p.tri ? p.piece : up(p.units, 2) * kUnit;
+    s.packed = r.take(p.rows_pad * p.width_pad * terms);
+    s.plain = r.take(sweep == 2 ? p.rows * p.width * (p.tri ? 4 : 2) : 0);
+    s.piece = r.take(sweep ? p.rows_pad * p.piece * 2 * p.terms[sweep] : 0);
+    s.turned = r.take(sweep == 0 ? 0 : p.turned ? p.width * terms * (sweep == 1 ? p.piece : steps)
+                                                : p.tri && sweep == 2 ? p.rows * pitch * terms : 0);
+    s.split = r.take(p.tri ? p.piece * pitch * terms : 0);
+    s.stats = r.take(sweep == 2 ? 0 : piece / kUnit * p.rows_pad * 8);
     s.factor = r.take(p.rows_pad * 4);
     s.inverse = r.take(p.rows_pad * 4);
     s.near = r.take(p.rows_pad * 4);
@@ -350,22 +352,22 @@ struct Source {
     }
 };
 
-// A float32 value as the sum of three bf16 terms, exact for values of 2^-100 and more: 8 bits of the
-// significand each.
-__device__ __forceinline__ void split3(float v, float (&t)[3]) {
-    t[0] = bf16_to_f32(bf16_bits(v));
-    t[1] = bf16_to_f32(bf16_bits(v - t[0]));
-    t[2] = v - t[0] - t[1];
-}
-// Eight of them, term by term, as 16-byte units.
-__device__ __forceinline__ void split_unit(const float (&v)[8], uint4 (&out)[3]) {
-    float t[8][3];
+// Eight float32 values as sums of bf16 terms, 8 bits of the significand each, term by term as 16-byte
+// units: three terms hold values of 2^-100 and more exactly.
+template <int TERMS>
+__device__ __forceinline__ void split_unit(const float (&v)[8], uint4 (&out)[TERMS]) {
+    float rest[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) split3(v[i], t[i]);
+    for (int i = 0; i < 8; ++i) rest[i] = v[i];
 #pragma unroll
-    for (int s = 0; s < 3; ++s)
-        out[s] = make_uint4(pack_bf16x2(t[0][s], t[1][s]), pack_bf16x2(t[2][s], t[3][s]), pack_bf16x2(t[4][s], t[5][s]),
-                            pack_bf16x2(t[6][s], t[7][s]));
+    for (int s = 0; s < TERMS; ++s) {
+        out[s] = make_uint4(pack_bf16x2(rest[0], rest[1]), pack_bf16x2(rest[2], rest[3]), pack_bf16x2(rest[4], rest[5]),
+                            pack_bf16x2(rest[6], rest[7]));
+        if (s + 1 == TERMS) break;
+        const uint32_t w[4] = {out[s].x, out[s].y, out[s].z, out[s].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rest[i] -= bf16_to_f32((uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu));
+    }
 }
 
 // pack_rows below for float32 rows: three packed operands, `units` apart.
@@ -380,21 +382,30 @@ __global__ __launch_bounds__(256) void pack_split(Source src, int64_t blocks, ui
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = row >= 0 && k + i < src.width ? x[k + i] : 0.f;
     uint4 t[3];
-    split_unit(v, t);
+    split_unit<3>(v, t);
 #pragma unroll
     for (int s = 0; s < 3; ++s) out[u + s * units] = t[s];
 }
 
 // float32 rows [rows][cols] as three bf16 arrays of `pitch` columns, `apart` units between them.
+template <bool PAIRS>
 __global__ __launch_bounds__(256) void split_rows(const float *__restrict__ x, int64_t ld, int64_t rows, int64_t cols,
                                                   uint4 *__restrict__ out, int64_t pitch, int64_t apart) {
     const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x, per = pitch / 8, row = u / per, c = u % per * 8;
     if (row >= rows) return;
     float v[8];
+    if (PAIRS && c + 8 <= cols) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? x[row * ld + c + i] : 0.f;
+        for (int i = 0; i < 8; i += 2) {
+            const float2 f = *reinterpret_cast<const float2 *>(x + row * ld + c + i);
+            v[i] = f.x, v[i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? x[row * ld + c + i] : 0.f;
+    }
     uint4 t[3];
-    split_unit(v, t);
+    split_unit<3>(v, t);
 #pragma unroll
     for (int s = 0; s < 3; ++s) out[u + s * apart] = t[s];
 }
@@ -473,7 +484,7 @@ __global__ __launch_bounds__(256) void transpose_rows(const T *__restrict__ x, i
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = tile[from + (j >> 2) * 16 + (j & 3)][c];
             uint4 t[3];
-            split_unit(v, t);
+            split_unit<3>(v, t);
 #pragma unroll
             for (int s = 0; s < 3; ++s) to[s * apart] = t[s];
         }
@@ -510,12 +521,15 @@ __device__ __forceinline__ void tile_of(int64_t id, int64_t np, int64_t nl, int6
 // 4 x 2 waves, with half the LDS reads and twice the packed loads, are 6% slower, two workgroups of four
 // waves per CU 9%.
 //
-// TRI: float32 operands as three bf16 terms each (split3). The reduction runs over six products of
+// TERMS 2: the packed operand is the sum of two bf16 terms, both multiplied with each staged fragment.
+// TERMS 3 (TRI): float32 operands as three bf16 terms each (split3). The reduction runs over six products of
 // the terms, the small ones first; the three left out are below 2^-26 of the whole, and every
 // product of two terms is exact in float32. Six bf16 products are faster than one float32 product
 // on this card's matrix units (v_mfma_f32_16x16x4_f32, a sixteenth of the bf16 rate).
-template <int WP, int WL, int PF, int LF, bool KT, bool SWAP, bool TRI = false>
+template <int WP, int WL, int PF, int LF, bool KT, bool SWAP, int TERMS = 1>
 struct Core {
+    static constexpr bool TRI = TERMS == 3;
+    static constexpr int KS = TERMS == 2 ? 4 : 2;   // packed fragments of a step
     static constexpr int BP = WP * PF * 16, BL = WL * LF * 16, THREADS = 64 * WP * WL;
     static constexpr int kPer = BL * 8 / THREADS;   // 16-byte units of a stage per thread
     static constexpr int kStage = BL * 8;           // units per stage
@@ -531,7 +545,7 @@ struct Core {
     int steps, store_at, read_at;
     uint32_t part;           // TRI: 2^32 / the steps of one product of terms, rounded up
     int one;                 // TRI: those steps
-    int64_t b_apart, a_apart;  // TRI: bytes, and units, between two terms
+    int64_t b_apart, a_apart = 0;  // bytes, and units, between two terms
 
     // first: the staged operand at the tile's first row (KC) or column (KT); `extent` its rows from
     // there (KC) or columns (KT), `depth` the reduction's extent.
@@ -564,11 +578,12 @@ struct Core {
         a_row = blocks * 64;
     }
     __device__ __forceinline__ void terms(int64_t b_units, int64_t a_units) {
+        a_apart = a_units;
+        if constexpr (!TRI) return;
         one = steps;
         part = one > 1 ? 0xffffffffu / (uint32_t)one + 1 : 0;
         steps *= 6;
         b_apart = b_units * 16;
-        a_apart = a_units;
     }
     // The product of terms that step t belongs to, and the step in it. Of the packed operand the terms
     // 2 1 0 1 0 0, of the staged one 0 1 2 0 1 0.
@@ -588,11 +603,11 @@ struct Core {
         r[C] = buf_load16(rsrc, (KT || at * kStep + k < limit ? off : kOOB) + C * pitch);
     }
     template <int I>
-    __device__ __forceinline__ void load_a(int t, uint4 (&f)[2][PF]) const {
+    __device__ __forceinline__ void load_a(int t, uint4 (&f)[KS][PF]) const {
         const uint4 *from = a;
         int at = t < steps ? t : steps - 1;
         if constexpr (TRI) from += (0x46 >> 2 * product(at, at) & 3) * a_apart;
-        f[I & 1][I >> 1] = from[(int64_t)at * 128 + (I >> 1) * a_row + (I & 1) * 64];
+        f[I % KS][I / KS] = from[(I % KS >> 1) * a_apart + (int64_t)at * 128 + I / KS * a_row + (I & 1) * 64];
     }
     template <int C>
     __device__ __forceinline__ void store_b(uint4 *stage, const uint4 (&r)[kPer]) const {
@@ -614,25 +629,25 @@ struct Core {
         }
     }
     template <int F>
-    __device__ __forceinline__ void columns(int t, const uint4 *cur, const uint4 *nxt, uint4 *wr, const uint4 (&af)[2][PF],
-                                            uint4 (&an)[2][PF], uint4 (&b)[kPer], uint4 (&lf)[4][2],
+    __device__ __forceinline__ void columns(int t, const uint4 *cur, const uint4 *nxt, uint4 *wr, const uint4 (&af)[KS][PF],
+                                            uint4 (&an)[KS][PF], uint4 (&b)[kPer], uint4 (&lf)[4][2],
                                             f32x4 (&acc)[LF][PF]) const {
         if constexpr (F < LF) {
             read(F + 3 < LF ? cur : nxt, (F + 3) % LF, lf[(F + 3) % 4]);
-            if constexpr (F % (LF / 8) == 0 && F / (LF / 8) < 2 * PF) load_a<F / (LF / 8)>(t + 1, an);
+            if constexpr (F % (LF / 8) == 0 && F / (LF / 8) < KS * PF) load_a<F / (LF / 8)>(t + 1, an);
             if constexpr (F % (LF / 4) == LF / 8 - 1) store_b<F / (LF / 4)>(wr, b);
             if constexpr (F % (LF / 4) == LF / 4 - 1) load_b<F / (LF / 4)>(t + 3, b);
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
+            for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int j = 0; j < PF; ++j)
-                    acc[F][j] = SWAP ? mfma16x16x32(lf[F % 4][ks], af[ks][j], acc[F][j])
-                                     : mfma16x16x32(af[ks][j], lf[F % 4][ks], acc[F][j]);
+                    acc[F][j] = SWAP ? mfma16x16x32(lf[F % 4][ks & 1], af[ks][j], acc[F][j])
+                                     : mfma16x16x32(af[ks][j], lf[F % 4][ks & 1], acc[F][j]);
             __builtin_amdgcn_sched_barrier(0);
             columns<F + 1>(t, cur, nxt, wr, af, an, b, lf, acc);
         }
     }
-    __device__ __forceinline__ void step(int t, uint4 *stages, int &at, const uint4 (&af)[2][PF], uint4 (&an)[2][PF],
+    __device__ __forceinline__ void step(int t, uint4 *stages, int &at, const uint4 (&af)[KS][PF], uint4 (&an)[KS][PF],
                                          uint4 (&b)[kPer], uint4 (&lf)[4][2], f32x4 (&acc)[LF][PF]) const {
         const int next = at == 2 * kStage ? 0 : at + kStage, after = next == 2 * kStage ? 0 : next + kStage;
         columns<0>(t, stages + at, stages + next, stages + after, af, an, b, lf, acc);
@@ -641,13 +656,13 @@ struct Core {
         __syncthreads();
     }
     template <int I>
-    __device__ __forceinline__ void first(uint4 *stages, uint4 (&b)[kPer], uint4 (&more)[kPer], uint4 (&af)[2][PF]) const {
-        static_assert(kPer == 4 && 2 * PF <= 8, "spread over the columns");
+    __device__ __forceinline__ void first(uint4 *stages, uint4 (&b)[kPer], uint4 (&more)[kPer], uint4 (&af)[KS][PF]) const {
+        static_assert(kPer == 4 && KS * PF <= 8, "spread over the columns");
         if constexpr (I < 4) {
             load_b<I>(0, b);
             load_b<I>(1, more);
         } else if constexpr (I < 12) {
-            if constexpr (I - 4 < 2 * PF) load_a<I - 4>(0, af);
+            if constexpr (I - 4 < KS * PF) load_a<I - 4>(0, af);
         } else if constexpr (I < 16) {
             store_b<I - 12>(stages, b);
             store_b<I - 12>(stages + kStage, more);
@@ -661,7 +676,7 @@ struct Core {
 #pragma unroll
             for (int j = 0; j < PF; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (steps <= 0) return;
-        uint4 b[kPer], more[kPer], a0[2][PF], a1[2][PF], lf[4][2];
+        uint4 b[kPer], more[kPer], a0[KS][PF], a1[KS][PF], lf[4][2];
         first<0>(stages, b, more, a0);
         __syncthreads();
         read(stages, 0, lf[0]);
@@ -682,7 +697,7 @@ enum { STATS = 0, EXP = 1, GRAD = 2 };
 struct LogitsParams {
     const uint16_t *head;      // from v0 on
     int64_t ld, width, vocab;
-    int64_t head_apart, packed_apart, piece_apart;   // TRI: units between two terms
+    int64_t head_apart, packed_apart, piece_apart;   // units between two terms
     const uint4 *packed;       // hidden rows
     int64_t blocks;            // of 32 along the width
     int64_t v0, v1;            // the piece's entries
@@ -708,16 +723,12 @@ __device__ __forceinline__ float shift_of(float top) {
     return fabsf(top) < 1e6f ? 96.f * ceilf((top - 48.f) * (1.f / 96.f)) - 32.f : top;
 }
 
-template <bool TRI>
+template <int TERMS>
 __device__ __forceinline__ void store_unit(uint4 *to, int64_t apart, const float (&v)[8]) {
-    if constexpr (TRI) {
-        uint4 t[3];
-        split_unit(v, t);
+    uint4 t[TERMS];
+    split_unit(v, t);
 #pragma unroll
-        for (int s = 0; s < 3; ++s) to[s * apart] = t[s];
-    } else {
-        *to = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-    }
+    for (int s = 0; s < TERMS; ++s) to[s * apart] = t[s];
 }
 
 // Which of a wave's rows x units of 128 vocabulary entries are targets, as bits in LDS [row][unit][4],
@@ -750,9 +761,10 @@ __device__ __forceinline__ int64_t place_of(const LogitsParams &p, int64_t row, 
     return row * p.entries + n;
 }
 
-template <int WP, int WL, int PF, int LF, int MODE, bool TRI>
+template <int WP, int WL, int PF, int LF, int MODE, int TERMS>
 __global__ __launch_bounds__(64 * WP * WL) void logits_kernel(const LogitsParams p) {
-    using C = Core<WP, WL, PF, LF, false, MODE != GRAD, TRI>;
+    constexpr bool TRI = TERMS == 3;
+    using C = Core<WP, WL, PF, LF, false, MODE != GRAD, TRI ? 3 : 1>;
     constexpr int UNITS = LF / 8;   // of a wave
     __shared__ uint4 stages[3 * C::kStage];
     __shared__ uint4 marks[WP * WL][PF * 16 * UNITS];
@@ -809,18 +821,16 @@ __global__ __launch_bounds__(64 * WP * WL) void logits_kernel(const LogitsParams
                 uint4 *to = p.piece + (((u0 - p.v0) / 16 + f) * p.piece_blocks + row0 / 32) * 64 + lane;
                 if constexpr (PF == 1) {   // half a unit: the other half is the wave's that holds the next 16 rows
                     const f32x4 x = acc[8 * u + f][0];
-                    const float v[8] = {x[0], x[1], x[2], x[3]};
-                    uint4 t[3];
-                    if constexpr (TRI) split_unit(v, t);
-                    else t[0] = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), 0, 0);
+                    uint4 t[TERMS];
+                    split_unit({x[0], x[1], x[2], x[3]}, t);
 #pragma unroll
-                    for (int s = 0; s < (TRI ? 3 : 1); ++s)
+                    for (int s = 0; s < TERMS; ++s)
                         reinterpret_cast<uint2 *>(to + s * p.piece_apart)[(row0 / 16) & 1] = make_uint2(t[s].x, t[s].y);
                 } else {
 #pragma unroll
                     for (int j = 0; j < PF; j += 2) {
                         const f32x4 x = acc[8 * u + f][j], y = acc[8 * u + f][j + 1];
-                        store_unit<TRI>(to + j / 2 * 64, p.piece_apart, {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
+                        store_unit<TERMS>(to + j / 2 * 64, p.piece_apart, {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
                     }
                 }
             }
@@ -876,7 +886,7 @@ __global__ __launch_bounds__(64 * WP * WL) void logits_kernel(const LogitsParams
                         e[i] *= by;
                     }
                     if constexpr (MODE == EXP)
-                        store_unit<TRI>(p.piece + ((row0 / 16 + j) * p.piece_blocks + (u0 - p.v0) / 32 + g) * 64 + lane,
+                        store_unit<TERMS>(p.piece + ((row0 / 16 + j) * p.piece_blocks + (u0 - p.v0) / 32 + g) * 64 + lane,
                                         p.piece_apart, e);
                 }
                 sum += __shfl_xor(sum, 16, 64);
@@ -946,7 +956,7 @@ struct ProductParams {
     int64_t ld, depth, cols;
     bool kt;
     const uint4 *packed;       // [rows, depth]
-    int64_t blocks, b_apart, packed_apart;   // TRI: units between two terms
+    int64_t blocks, b_apart, packed_apart;   // units between two terms
     int64_t np, nl;
     int64_t rows;
     void *out;
@@ -957,9 +967,9 @@ struct ProductParams {
 };
 
 // out[row, col] (= factor out +) sum_k packed(row, k) b(k, col), one split of the reduction per y.
-template <int WP, int WL, int PF, int LF, bool KT, int OUT, bool TRI>
+template <int WP, int WL, int PF, int LF, bool KT, int OUT, int TERMS>
 __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductParams p) {
-    using C = Core<WP, WL, PF, LF, KT, true, TRI>;
+    using C = Core<WP, WL, PF, LF, KT, true, TERMS>;
     __shared__ uint4 stages[3 * C::kStage];
     int64_t tp, tl;
     tile_of(blockIdx.x, p.np, p.nl, tp, tl);
@@ -973,7 +983,7 @@ __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductPara
     const int64_t depth = (end < p.steps ? (int64_t)end * kStep : p.depth) - k0;   // none: an empty split
     core.init(p.b + (KT ? k0 * p.ld + tl * C::BL : tl * C::BL * p.ld + k0), p.ld, p.cols - tl * C::BL, depth,
               p.packed + (int64_t)beg * 128, tp * (C::BP / 16), p.blocks, wave);
-    if constexpr (TRI) core.terms(p.b_apart, p.packed_apart);
+    if constexpr (TERMS > 1) core.terms(p.b_apart, p.packed_apart);
     f32x4 acc[LF][PF];
     core.run(stages, acc);
 #pragma unroll
@@ -1012,62 +1022,6 @@ __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductPara
             }
         }
     }
-}
-
-// ------------------------------------------------------------------------- float32 row passes
-// One workgroup per row of a piece of float32 logits: the running maximum and sum; with `sums` the
-// logits become E (0 at the row's targets) and the row of the sums so far is brought to its shift.
-__global__ __launch_bounds__(256) void rows_exp_f32(float *__restrict__ logits, int64_t ld, int64_t v0, int64_t cols,
-                                                    float scale, float *__restrict__ shift, float *__restrict__ total,
-                                                    const int *__restrict__ index, const uint16_t *__restrict__ first,
-                                                    float *__restrict__ chosen, int entries, int64_t units, float *sums,
-                                                    int64_t width) {
-    __shared__ float lds[256];
-    const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x;
-    float *l = logits + row * ld;
-    float top = -INFINITY;
-    for (int64_t c = tid; c < cols; c += 256) top = fmaxf(top, l[c]);
-    top = block_max<256>(top, lds);
-    const float before = shift[row], held = total[row];
-    const float c = fmaxf(before, fmaxf(ceilf(top * scale), kNone));
-    // pieces start at multiples of 256: whole units
-    const int e0 = first[row * (units + 1) + v0 / kUnit], e1 = first[row * (units + 1) + cdiv(v0 + cols, kUnit)];
-    for (int e = e0 + tid; e < e1; e += 256) {
-        float *at = l + index[row * entries + e] - v0;
-        chosen[row * entries + e] = *at;
-        *at = -INFINITY;
-    }
-    __syncthreads();
-    float sum = 0.f;
-    for (int64_t i = tid; i < cols; i += 256) {
-        const float e = exp2f(__builtin_fmaf(l[i], scale, -c));
-        sum += e;
-        if (sums) l[i] = e;
-    }
-    sum = block_sum<256>(sum, lds);
-    const float by = before == c ? 1.f : exp2f(before - c);
-    if (sums && by != 1.f && v0 > 0)
-        for (int64_t i = tid; i < width; i += 256) sums[row * width + i] *= by;
-    if (tid == 0) {
-        total[row] = held * by + sum;
-        shift[row] = c;
-    }
-}
-
-__global__ __launch_bounds__(256) void rows_grad_f32(float *__restrict__ logits, int64_t ld, int64_t v0, int64_t cols,
-                                                     float scale, const float *__restrict__ shift,
-                                                     const float *__restrict__ factor, const float *__restrict__ inverse,
-                                                     const int *__restrict__ index, const uint16_t *__restrict__ first,
-                                                     const float *__restrict__ coefficient, int entries, int64_t units) {
-    const int64_t row = blockIdx.x;
-    float *l = logits + row * ld;
-    const float c = shift[row], f = factor[row];
-    for (int64_t i = threadIdx.x; i < cols; i += 256) l[i] = exp2f(__builtin_fmaf(l[i], scale, -c)) * f;
-    __syncthreads();
-    const int e0 = first[row * (units + 1) + v0 / kUnit], e1 = first[row * (units + 1) + cdiv(v0 + cols, kUnit)];
-    for (int e = e0 + (int)threadIdx.x; e < e1; e += 256)
-        l[index[row * entries + e] - v0] = inverse[row] * coefficient[row * entries + e];
 }
 
 // ------------------------------------------------------------------------- the ends
@@ -1189,7 +1143,7 @@ __global__ __launch_bounds__(256) void hidden_grad_kernel(const float *__restric
             const float *w = static_cast<const float *>(head) + vocab * ld + c0;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (in(i)) v[i] += by_k * w[i];
+                if (VEC ? c0 < width : c0 + i < width) v[i] += by_k * w[i];
         } else if (in(0)) {   // rows of whole units
             const uint4 x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(head) + vocab * ld + c0);
             const uint32_t w[4] = {x.x, x.y, x.z, x.w};
@@ -1227,33 +1181,42 @@ T *at(void *base, int64_t offset) {
     return reinterpret_cast<T *>(static_cast<char *>(base) + offset);
 }
 
-template <int MODE>
+template <int MODE, int TERMS>
 hipError_t launch_logits(const Plan &pl, const LogitsParams &p, hipStream_t s) {
     const dim3 grid((unsigned)(p.np * p.nl));
-    if (pl.bp == 64) logits_kernel<4, 1, 1, 8, MODE, false><<<grid, dim3(256), 0, s>>>(p);
-    else if (pl.bp == 128 && pl.tri) logits_kernel<8, 1, 1, 16, MODE, true><<<grid, dim3(512), 0, s>>>(p);
-    else if (pl.bp == 128) logits_kernel<8, 1, 1, 16, MODE, false><<<grid, dim3(512), 0, s>>>(p);
-    else if (pl.tri) logits_kernel<8, 1, 2, 16, MODE, true><<<grid, dim3(512), 0, s>>>(p);
-    else logits_kernel<8, 1, 2, 16, MODE, false><<<grid, dim3(512), 0, s>>>(p);
+    if (pl.bp == 64) logits_kernel<4, 1, 1, 8, MODE, TERMS><<<grid, dim3(256), 0, s>>>(p);
+    if (pl.bp == 128) logits_kernel<8, 1, 1, 16, MODE, TERMS><<<grid, dim3(512), 0, s>>>(p);
+    if constexpr (MODE == GRAD || TERMS != 2)   // E of so many rows is one term or three
+        if (pl.bp == 256) logits_kernel<8, 1, 2, 16, MODE, TERMS><<<grid, dim3(512), 0, s>>>(p);
     return hipGetLastError();
 }
-template <int OUT, bool KT, bool TRI>
+template <int MODE>
+hipError_t launch_logits(const Plan &pl, const LogitsParams &p, hipStream_t s) {
+    if (pl.tri) return launch_logits<MODE, 3>(pl, p, s);
+    if constexpr (MODE != STATS)
+        if (pl.terms[MODE] == 2) return launch_logits<MODE, 2>(pl, p, s);
+    return launch_logits<MODE, 1>(pl, p, s);
+}
+template <int OUT, bool KT, int TERMS>
 hipError_t launch_product(int bp, const ProductParams &p, int splits, hipStream_t s) {
     const dim3 grid((unsigned)(p.np * p.nl), (unsigned)splits);
-    if constexpr (KT) {
-        if (bp == 64) product_kernel<4, 1, 1, 8, true, OUT, false><<<grid, dim3(256), 0, s>>>(p);
-        else product_kernel<8, 1, 1, 16, true, OUT, false><<<grid, dim3(512), 0, s>>>(p);
+    if (bp == 64) {
+        if constexpr (KT) product_kernel<4, 1, 1, 8, true, OUT, TERMS><<<grid, dim3(256), 0, s>>>(p);
+    } else if (bp == 128) {
+        if constexpr (!KT || TERMS < 3) product_kernel<8, 1, 1, 16, KT, OUT, TERMS><<<grid, dim3(512), 0, s>>>(p);
     } else {
-        if (bp == 128) product_kernel<8, 1, 1, 16, false, OUT, TRI><<<grid, dim3(512), 0, s>>>(p);
-        else product_kernel<8, 1, 2, 16, false, OUT, TRI><<<grid, dim3(512), 0, s>>>(p);
+        if constexpr (!KT && TERMS != 2) product_kernel<8, 1, 2, 16, false, OUT, TERMS><<<grid, dim3(512), 0, s>>>(p);
     }
     return hipGetLastError();
 }
+// Packed operands of two terms take the narrower tiles: the wider ones have no registers for them.
 template <int OUT>
-hipError_t launch_product(const Plan &pl, const ProductParams &p, int splits, hipStream_t s) {
+hipError_t launch_product(int bp, int terms, const ProductParams &p, int splits, hipStream_t s) {
     if constexpr (OUT == CT_F32)
-        if (pl.tri) return launch_product<OUT, false, true>(pl.bp, p, splits, s);
-    return p.kt ? launch_product<OUT, true, false>(pl.bp, p, splits, s) : launch_product<OUT, false, false>(pl.bp, p, splits, s);
+        if (terms == 3)
+            return p.kt ? launch_product<OUT, true, 3>(bp, p, splits, s) : launch_product<OUT, false, 3>(bp, p, splits, s);
+    if (p.kt) return terms == 2 ? launch_product<OUT, true, 2>(bp, p, splits, s) : launch_product<OUT, true, 1>(bp, p, splits, s);
+    return terms == 2 ? launch_product<OUT, false, 2>(bp, p, splits, s) : launch_product<OUT, false, 1>(bp, p, splits, s);
 }
 
 int check(const ct_head_loss *a, bool hidden) {
@@ -1330,6 +1293,14 @@ hipError_t pack_hidden(const ct_head_loss *a, const Plan &pl, void *packed, hipS
     else pack_rows<false><<<grid, dim3(256), 0, stream>>>(src, pl.width_pad / 32, static_cast<uint4 *>(packed), units);
     return hipGetLastError();
 }
+hipError_t split_terms(const float *x, int64_t ld, int64_t rows, int64_t cols, uint4 *out, int64_t pitch, int64_t apart,
+                       hipStream_t s) {
+    const dim3 grid((unsigned)cdiv(rows * (pitch / 8), 256));
+    const bool pairs = ld % 2 == 0 && reinterpret_cast<uintptr_t>(x) % 8 == 0;
+    if (pairs) split_rows<true><<<grid, dim3(256), 0, s>>>(x, ld, rows, cols, out, pitch, apart);
+    else split_rows<false><<<grid, dim3(256), 0, s>>>(x, ld, rows, cols, out, pitch, apart);
+    return hipGetLastError();
+}
 // The piece of the head that starts at entry v0, as the logits kernel stages it: in place, or float32
 // rows in their three terms.
 hipError_t head_piece(const ct_head_loss *a, const Plan &pl, LogitsParams &p, int64_t v0, int64_t cols, void *split,
@@ -1342,11 +1313,8 @@ hipError_t head_piece(const ct_head_loss *a, const Plan &pl, LogitsParams &p, in
         return hipSuccess;
     }
     p.head = static_cast<const uint16_t *>(split);
-    const int64_t units = cols * (p.ld / 8);
-    split_rows<<<dim3((unsigned)cdiv(units, 256)), dim3(256), 0, stream>>>(
-        static_cast<const float *>(a->head) + v0 * a->ld_head, a->ld_head, cols, pl.width, static_cast<uint4 *>(split), p.ld,
-        p.head_apart);
-    return hipGetLastError();
+    return split_terms(static_cast<const float *>(a->head) + v0 * a->ld_head, a->ld_head, cols, pl.width,
+                       static_cast<uint4 *>(split), p.ld, p.head_apart, stream);
 }
 // The loss's rows one after the other: as they lie, or gathered into `to`.
 hipError_t plain_hidden(const ct_head_loss *a, const Plan &pl, void *to, const void **hidden, int64_t *ld, hipStream_t stream) {
@@ -1408,70 +1376,47 @@ extern "C" int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t 
     else targets(targets_kernel<256>, 256);
     CT_TRY(hipGetLastError());
 
-    if (pl.dtype == CT_F32 && !pl.tri) {
-        const float scale = (float)(1.4426950408889634074 / a->temperature);
-        float *piece = at<float>(workspace, sc.piece);
-        const float *head = static_cast<const float *>(a->head);
-        const void *hidden;
-        int64_t ld;
-        CT_TRY(plain_hidden(a, pl, at<void>(workspace, sc.plain), &hidden, &ld, stream));
-        for (int64_t v0 = 0; v0 < pl.vocab; v0 += pl.piece) {
-            const int64_t cols = pl.vocab - v0 < pl.piece ? pl.vocab - v0 : pl.piece;
-            if (const int bad = ct_gemm_f32(static_cast<const float *>(hidden), ld, 0, head + v0 * a->ld_head, a->ld_head, 1, piece, pl.piece,
-                                            0, nullptr, pl.rows, cols, pl.width, stream))
-                return bad;
-            rows_exp_f32<<<dim3((unsigned)pl.rows), dim3(256), 0, stream>>>(
-                piece, pl.piece, v0, cols, scale, shift, total, at<int>(kept, k.index), at<uint16_t>(kept, k.first),
-                at<float>(kept, k.chosen), (int)pl.entries, pl.units, hidden_grad ? sums : nullptr, pl.width);
-            CT_TRY(hipGetLastError());
-            if (!hidden_grad) continue;
-            if (const int bad = ct_gemm_f32(piece, pl.piece, 0, head + v0 * a->ld_head, a->ld_head, 0, sums, pl.width, v0 > 0,
-                                            nullptr, pl.rows, pl.width, cols, stream))
-                return bad;
+    CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), stream));
+    LogitsParams p = logits_params(a, pl, k, sc, kept, workspace);
+    const int64_t piece = hidden_grad || pl.tri ? pl.piece : pl.vocab;
+    for (int64_t v0 = 0; v0 < pl.vocab; v0 += piece) {
+        const int64_t cols = pl.vocab - v0 < piece ? pl.vocab - v0 : piece;
+        CT_TRY(head_piece(a, pl, p, v0, cols, at<void>(workspace, sc.split), stream));
+        p.piece_blocks = pl.piece / 32;
+        CT_TRY(hidden_grad ? launch_logits<EXP>(pl, p, stream) : launch_logits<STATS>(pl, p, stream));
+        join_kernel<<<dim3((unsigned)(pl.rows_pad / 16)), dim3(1024), 0, stream>>>(
+            p.stats, (int)cdiv(cols, kUnit), pl.rows_pad, shift, total, factor, hidden_grad ? p.piece : nullptr,
+            p.piece_blocks, pl.terms[hidden_grad ? 1 : 0], p.piece_apart);
+        CT_TRY(hipGetLastError());
+        if (!hidden_grad) continue;
+        ProductParams g{};
+        g.b = p.head;
+        g.ld = p.ld;
+        g.kt = !pl.turned;
+        if (pl.turned) {
+            uint16_t *turned = at<uint16_t>(workspace, sc.turned);
+            const void *from = static_cast<const char *>(a->head) + v0 * a->ld_head * (pl.tri ? 4 : 2);
+            CT_TRY(transpose(from, pl.dtype, a->ld_head, cols, pl.width, turned, pl.piece, stream));
+            g.b = turned;
+            g.ld = pl.piece;
         }
-    } else {
-        CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), stream));
-        LogitsParams p = logits_params(a, pl, k, sc, kept, workspace);
-        const int64_t piece = hidden_grad || pl.tri ? pl.piece : pl.vocab;
-        for (int64_t v0 = 0; v0 < pl.vocab; v0 += piece) {
-            const int64_t cols = pl.vocab - v0 < piece ? pl.vocab - v0 : piece;
-            CT_TRY(head_piece(a, pl, p, v0, cols, at<void>(workspace, sc.split), stream));
-            p.piece_blocks = pl.piece / 32;
-            CT_TRY(hidden_grad ? launch_logits<EXP>(pl, p, stream) : launch_logits<STATS>(pl, p, stream));
-            join_kernel<<<dim3((unsigned)(pl.rows_pad / 16)), dim3(1024), 0, stream>>>(
-                p.stats, (int)cdiv(cols, kUnit), pl.rows_pad, shift, total, factor, hidden_grad ? p.piece : nullptr,
-                p.piece_blocks, pl.terms, p.piece_apart);
-            CT_TRY(hipGetLastError());
-            if (!hidden_grad) continue;
-            ProductParams g{};
-            g.b = p.head;
-            g.ld = p.ld;
-            g.kt = !pl.turned;
-            if (pl.turned) {
-                uint16_t *turned = at<uint16_t>(workspace, sc.turned);
-                const void *from = static_cast<const char *>(a->head) + v0 * a->ld_head * (pl.tri ? 4 : 2);
-                CT_TRY(transpose(from, pl.dtype, a->ld_head, cols, pl.width, turned, pl.piece, stream));
-                g.b = turned;
-                g.ld = pl.piece;
-            }
-            g.b_apart = pl.width * pl.piece / 8;
-            g.packed_apart = p.piece_apart;
-            g.depth = pl.turned ? up(cols, kStep) : cols;   // turned rows end with a whole step, in their order
-            g.cols = pl.width;
-            g.packed = p.piece;
-            g.blocks = p.piece_blocks;
-            g.np = p.np;
-            g.nl = cdiv(pl.width, pl.bl);
-            g.rows = pl.rows;
-            g.out = sums;
-            g.ldo = pl.width;
-            g.slab = pl.rows * pl.width;
-            g.steps = (int)cdiv(cols, kStep);
-            g.steps_per_split = (int)cdiv(g.steps, pl.splits);
-            g.factor = v0 ? factor : nullptr;
-            g.vec = pl.width % 4 == 0;
-            CT_TRY(launch_product<CT_F32>(pl, g, pl.splits, stream));
-        }
+        g.b_apart = pl.turned ? pl.width * pl.piece / 8 : p.head_apart;
+        g.packed_apart = p.piece_apart;
+        g.depth = pl.turned ? up(cols, kStep) : cols;   // turned rows end with a whole step, in their order
+        g.cols = pl.width;
+        g.packed = p.piece;
+        g.blocks = p.piece_blocks;
+        g.np = p.np;
+        g.nl = cdiv(pl.width, pl.bl);
+        g.rows = pl.rows;
+        g.out = sums;
+        g.ldo = pl.width;
+        g.slab = pl.rows * pl.width;
+        g.steps = (int)cdiv(cols, kStep);
+        g.steps_per_split = (int)cdiv(g.steps, pl.splits);
+        g.factor = v0 ? factor : nullptr;
+        g.vec = pl.width % 4 == 0;
+        CT_TRY(launch_product<CT_F32>(pl.bp, pl.terms[1], g, pl.splits, stream));
     }
     row_loss<<<dim3((unsigned)pl.rows), dim3(64), 0, stream>>>(
         shift, total, at<float>(kept, k.weight), at<float>(kept, k.mass), at<float>(kept, k.entropy),
@@ -1530,28 +1475,6 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
         at<const float>(kept, k.weight), at<const float>(kept, k.mass), at<const float>(kept, k.shift),
         at<const float>(kept, k.total), upstream, inverse_t, pl.rows, pl.rows_pad, near, factor, inverse);
     CT_TRY(hipGetLastError());
-    if (pl.dtype == CT_F32 && !pl.tri) {
-        const float scale = (float)(1.4426950408889634074 / a->temperature);
-        float *piece = at<float>(workspace, sc.piece), *out = static_cast<float *>(d_head);
-        const float *head = static_cast<const float *>(a->head);
-        const void *hidden;
-        int64_t ld;
-        CT_TRY(plain_hidden(a, pl, at<void>(workspace, sc.plain), &hidden, &ld, stream));
-        for (int64_t v0 = 0; v0 < pl.vocab; v0 += pl.piece) {
-            const int64_t cols = pl.vocab - v0 < pl.piece ? pl.vocab - v0 : pl.piece;
-            if (const int bad = ct_gemm_f32(static_cast<const float *>(hidden), ld, 0, head + v0 * a->ld_head, a->ld_head, 1, piece, pl.piece,
-                                            0, nullptr, pl.rows, cols, pl.width, stream))
-                return bad;
-            rows_grad_f32<<<dim3((unsigned)pl.rows), dim3(256), 0, stream>>>(
-                piece, pl.piece, v0, cols, scale, near, factor, inverse, at<int>(kept, k.index),
-                at<uint16_t>(kept, k.first), at<float>(kept, k.chosen), (int)pl.entries, pl.units);
-            CT_TRY(hipGetLastError());
-            if (const int bad = ct_gemm_f32(piece, pl.piece, 1, static_cast<const float *>(hidden), ld, 0, out + v0 * ld_d_head, ld_d_head, 0,
-                                            nullptr, cols, d_head_width, pl.rows, stream))
-                return bad;
-        }
-        return 0;
-    }
     CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), stream));
     const void *hidden;
     int64_t ld;
@@ -1561,8 +1484,18 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
     p.factor = factor;
     p.inverse = inverse;
     p.piece_blocks = pl.rows_pad / 32;
+    int64_t apart = 0;
+    if (pl.tri && !pl.turned) {
+        uint4 *terms = at<uint4>(workspace, sc.turned);
+        const int64_t pitch = up(pl.width, 8);
+        apart = pl.rows * pitch / 8;
+        CT_TRY(split_terms(static_cast<const float *>(hidden), ld, pl.rows, pl.width, terms, pitch, apart, stream));
+        hidden = terms;
+        ld = pitch;
+    }
     if (pl.turned) {
         uint16_t *turned = at<uint16_t>(workspace, sc.turned);
+        apart = pl.width * up(pl.rows, kStep) / 8;
         CT_TRY(transpose(hidden, pl.dtype, ld, pl.rows, pl.width, turned, up(pl.rows, kStep), stream));
         hidden = turned;
         ld = up(pl.rows, kStep);
@@ -1575,21 +1508,22 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
         g.b = static_cast<const uint16_t *>(hidden);
         g.ld = ld;
         g.kt = !pl.turned;
-        g.b_apart = pl.width * up(pl.rows, kStep) / 8;
+        g.b_apart = apart;
         g.packed_apart = p.piece_apart;
         g.depth = pl.turned ? up(pl.rows, kStep) : pl.rows;
         g.cols = d_head_width;
         g.packed = p.piece;
         g.blocks = p.piece_blocks;
-        g.np = cdiv(cols, pl.bp);
+        const int bp = pl.terms[2] == 2 && pl.bp == 256 ? 128 : pl.bp;
+        g.np = cdiv(cols, bp);
         g.nl = cdiv(d_head_width, pl.bl);
         g.rows = cols;
         g.out = static_cast<char *>(d_head) + v0 * ld_d_head * (d_head_dtype == CT_F32 ? 4 : 2);
         g.ldo = ld_d_head;
         g.steps = g.steps_per_split = (int)cdiv(pl.rows, kStep);
         g.vec = ld_d_head % 4 == 0 && reinterpret_cast<uintptr_t>(d_head) % 16 == 0;
-        CT_TRY(d_head_dtype == CT_F32 ? launch_product<CT_F32>(pl, g, 1, stream)
-                                      : launch_product<CT_BF16>(pl, g, 1, stream));
+        CT_TRY(d_head_dtype == CT_F32 ? launch_product<CT_F32>(bp, pl.terms[2], g, 1, stream)
+                                      : launch_product<CT_BF16>(bp, pl.terms[2], g, 1, stream));
     }
     return 0;
 }
