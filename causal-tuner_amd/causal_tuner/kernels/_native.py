@@ -11,6 +11,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.forward_ad import unpack_dual
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -251,6 +252,8 @@ def ptr(tensor):
 def refuse_tangents(name, *tensors):
     """Raises where a tensor carries a forward-mode derivative: a kernel that is called outside
     an autograd Function would drop it without a word."""
+    if getattr(forward_ad, "_current_level", 0) < 0:
+        return   # no forward-mode level is open
     if any(unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{name}: the HIP kernels have no forward-mode derivative")
 

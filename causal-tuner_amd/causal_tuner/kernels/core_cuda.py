@@ -69,7 +69,7 @@ class RMS(torch.autograd.Function):
 
 
 def _layer_norm(x, weight, bias, eps, keep):
-    """(x as the kernel reads it, y, mean, rstd); mean and rstd None unless kept."""
+    """(x as the kernel reads it, y, mean and rstd [2, rows]; None unless kept)."""
     x = x.contiguous()
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         weight, bias = weight.float(), bias.float()   # one type for both: float32 holds either
@@ -80,55 +80,64 @@ def _layer_norm(x, weight, bias, eps, keep):
     vector = weight if weight is not None else bias
     y, width = torch.empty_like(x), x.shape[-1]
     rows = x.numel() // width
-    mean = rstd = None
+    stats = mean = rstd = None
     if keep:
-        mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32)
+        stats = torch.empty((2, rows), device=x.device, dtype=torch.float32)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * rows
     with _native.device_of(x):
         status = _native.library().ct_layer_norm_forward(
             x.data_ptr(), _native.dtype_code(x.dtype), _native.ptr(weight), _native.ptr(bias),
-            _native.CT_F32 if vector is None else _native.dtype_code(vector.dtype), y.data_ptr(), _native.ptr(mean),
-            _native.ptr(rstd), rows, width, eps, _native.stream_of(x))
+            _native.CT_F32 if vector is None else _native.dtype_code(vector.dtype), y.data_ptr(), mean, rstd, rows, width,
+            eps, _native.stream_of(x))
     _native.check(status, "ct_layer_norm_forward")
-    return x, y, mean, rstd
+    return x, y, stats
 
 
 class _LayerNorm(torch.autograd.Function):
+    """What the backward needs besides the tensors is worked out in the forward: the backward runs on
+    autograd's device thread, where Python is several times slower."""
+
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        x, y, mean, rstd = _layer_norm(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        ctx.bias_dtype = None if bias is None else bias.dtype
+        x, y, stats = _layer_norm(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        kept = None if weight is None else weight.dtype
+        given = None if bias is None else bias.dtype
+        # both sums are made in the weight's dtype; beside a bias of another one, in float32
+        dtype = kept if given is None or given == kept else given if kept is None else torch.float32
+        rows, width, code = stats.shape[1], x.shape[-1], _native.dtype_code(x.dtype)
+        lib, sums = _native.library(), need_w or need_b
+        ctx.plan = (lib.ct_layer_norm_backward, code, dtype, _native.CT_F32 if dtype is None else _native.dtype_code(dtype),
+                    kept, given, rows, width, lib.ct_layer_norm_backward_workspace(rows, width, code, 1) if sums else 0)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, weight, mean, rstd = ctx.saved_tensors
+        x, weight, stats = ctx.saved_tensors
+        call, code, dtype, w_code, kept, given, rows, width, nbytes = ctx.plan
         _native.refuse_tangents("layer_norm", grad)
-        grad, width, rows = grad.contiguous(), x.shape[-1], len(mean)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        grad, device = grad.contiguous(), x.device
         dx = torch.empty_like(x) if need_x else None
-        # both sums are made in the weight's dtype; a bias of a wider one takes float32
-        dtype = weight.dtype if weight is not None else ctx.bias_dtype or torch.float32
-        if need_b and ctx.bias_dtype != dtype:
-            dtype = torch.float32
-        dw = torch.empty(width, device=x.device, dtype=dtype) if need_w else None
-        db = torch.empty(width, device=x.device, dtype=dtype) if need_b else None
+        dw = torch.empty(width, device=device, dtype=dtype) if need_w else None
+        db = torch.empty(width, device=device, dtype=dtype) if need_b else None
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         if weight is not None:
             weight = weight.to(dtype).contiguous()   # a wider type holds the same values
-        lib, code = _native.library(), _native.dtype_code(x.dtype)
-        nbytes = lib.ct_layer_norm_backward_workspace(rows, width, code, int(need_w or need_b))
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-        with _native.device_of(x):
-            status = lib.ct_layer_norm_backward(
-                x.data_ptr(), code, _native.ptr(weight), _native.dtype_code(dtype), mean.data_ptr(), rstd.data_ptr(),
-                grad.data_ptr(), _native.ptr(dx), _native.ptr(dw), _native.ptr(db), rows, width, _native.ptr(workspace),
-                nbytes, _native.stream_of(x))
-        _native.check(status, "ct_layer_norm_backward")
-        if dw is not None:
-            dw = dw.to(ctx.saved_tensors[1].dtype)
-        if db is not None:
-            db = db.to(ctx.bias_dtype)
+        mean = stats.data_ptr()
+        # autograd has made the tensors' device current
+        status = call(x.data_ptr(), code, _native.ptr(weight), w_code, mean, mean + 4 * rows, grad.data_ptr(),
+                      _native.ptr(dx), _native.ptr(dw), _native.ptr(db), rows, width, _native.ptr(workspace), nbytes,
+                      _native.stream_of(x))
+        if status:
+            _native.check(status, "ct_layer_norm_backward")
+        if need_w and kept != dtype:
+            dw = dw.to(kept)
+        if need_b and given != dtype:
+            db = db.to(given)
         return dx, dw, db, None
 
 

@@ -49,80 +49,84 @@ def _workspace(nbytes, device):
     return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
 
 
-class _Call:
-    """The C call's operands, and the tensors they point into."""
-
-    def __init__(self, hidden, matrix, tables, first, rows, count, temperature):
-        indices, values, normalizer, weights = tables
-        self.held = (hidden, matrix, tables, rows)
-        size = hidden.element_size()
-        shift = lambda t, pitch: None if t is None else t.data_ptr() + first * pitch * t.element_size()  # noqa: E731
-        entries = indices.shape[1]
-        self.c = _native.HeadLoss(
-            hidden=hidden.data_ptr() + first * hidden.stride(0) * size, head=matrix.data_ptr(), rows=_native.ptr(rows),
-            indices=shift(indices, entries), values=shift(values, entries), log_normalizer=shift(normalizer, 1),
-            weights=shift(weights, 1), ld_hidden=max(hidden.stride(0), hidden.shape[1]), ld_head=matrix.stride(0),
-            ld_indices=entries, ld_values=entries, tokens=len(hidden) - first, hidden_width=hidden.shape[1], count=count,
-            width=matrix.shape[1], vocab=len(matrix), entries=entries, dtype=_native.dtype_code(matrix.dtype),
-            temperature=temperature)
-        self.sizes = (count, matrix.shape[1], len(matrix), entries, self.c.dtype)
-
-
 class StreamedHeadLoss(torch.autograd.Function):
+    """What the backward needs besides the tensors is worked out in the forward: the backward runs on
+    autograd's device thread, where Python is several times slower."""
+
     @staticmethod
     def forward(ctx, hidden, head, tables, selection, compute_dtype, temperature):
         need_hidden, need_head = ctx.needs_input_grad[:2]
         h, matrix = _plain_rows(hidden.to(compute_dtype)), _aligned_head(head.to(compute_dtype))
-        first, rows, count = _rows_of(selection, len(h), h.device)
-        call = _Call(h, matrix, tables, first, rows, count, temperature)
-        lib = _native.library()
-        loss = torch.empty((), dtype=torch.float32, device=h.device)
-        kept = _workspace(lib.ct_head_loss_kept(*call.sizes, int(need_hidden)), h.device)
-        scratch = _workspace(lib.ct_head_loss_workspace(*call.sizes, int(need_hidden)), h.device)
-        with _native.device_of(h):
-            status = lib.ct_head_loss_forward(call.c, loss.data_ptr(), int(need_hidden), kept.data_ptr(), kept.numel(),
-                                              scratch.data_ptr(), scratch.numel(), _native.stream_of(h))
-        _native.check(status, "ct_head_loss_forward")
+        tokens, device = len(h), h.device
+        first, rows, count = _rows_of(selection, tokens, device)
         indices, values, normalizer, weights = tables
-        ctx.save_for_backward(h if need_head else None, matrix, kept, indices, values, normalizer, weights, rows)
-        ctx.call = (first, count, temperature, need_hidden, hidden.shape, hidden.dtype, head.shape, head.dtype)
+        entries, (vocab, width) = indices.shape[1], matrix.shape
+        skip = first * entries
+        ld, code = h.stride(0), _native.dtype_code(compute_dtype)
+        call = _native.HeadLoss(
+            h.data_ptr() + first * ld * h.element_size(), matrix.data_ptr(), _native.ptr(rows),
+            indices.data_ptr() + 8 * skip, None if values is None else values.data_ptr() + 4 * skip,
+            None if normalizer is None else normalizer.data_ptr() + 4 * first, weights.data_ptr() + 4 * first,
+            max(ld, h.shape[1]), matrix.stride(0), entries, entries, tokens - first, h.shape[1], count, width, vocab,
+            entries, code, temperature)
+        lib, sizes, sums = _native.library(), (count, width, vocab, entries, code), int(need_hidden)
+        loss = torch.empty((), dtype=torch.float32, device=device)
+        kept_bytes = lib.ct_head_loss_kept(*sizes, sums)
+        kept = _workspace(kept_bytes, device)
+        scratch = _workspace(lib.ct_head_loss_workspace(*sizes, sums), device)
+        with _native.device_of(h):
+            status = lib.ct_head_loss_forward(call, loss.data_ptr(), sums, kept.data_ptr(), kept_bytes, scratch.data_ptr(),
+                                              scratch.numel(), _native.stream_of(h))
+        _native.check(status, "ct_head_loss_forward")
+        if need_hidden or need_head:
+            ctx.save_for_backward(h if need_head else None, matrix, kept, rows)
+            d_hidden = (hidden.shape, hidden.dtype, rows is None and count == tokens)
+            d_head = (head.shape, head.dtype, lib.ct_head_loss_workspace(*sizes, 2)) if need_head else None
+            # the targets are in what is kept
+            call.indices = call.values = call.log_normalizer = call.weights = None
+            ctx.plan = (lib.ct_head_loss_backward, call, first, count, sums, kept_bytes, code, d_hidden, d_head)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, upstream):
-        h, matrix, kept, indices, values, normalizer, weights, rows = ctx.saved_tensors
-        first, count, temperature, kept_sums, hidden_shape, hidden_dtype, head_shape, head_dtype = ctx.call
-        _native.refuse_tangents("projection_loss", upstream)
-        device, width = matrix.device, head_shape[1]
-        tokens = hidden_shape[:-1].numel()
-        d_hidden = d_head = hidden_out = head_out = None
-        if ctx.needs_input_grad[0]:
-            dtype = hidden_dtype if hidden_dtype == torch.bfloat16 else torch.float32
-            fresh = torch.empty if rows is None and count == tokens else torch.zeros
-            d_hidden = fresh((tokens, width), dtype=dtype, device=device)
-            hidden_out = d_hidden[first:]
-        if ctx.needs_input_grad[1]:
-            narrow = head_dtype == torch.bfloat16 and matrix.dtype == torch.bfloat16
-            fresh = torch.empty if count else torch.zeros
-            d_head = head_out = fresh(head_shape, dtype=torch.bfloat16 if narrow else torch.float32, device=device)
+        h, matrix, kept, rows = ctx.saved_tensors
+        backward, call, first, count, sums, kept_bytes, code, hidden_plan, head_plan = ctx.plan
+        _native.refuse_tangents("streamed head loss", upstream)
+        need_hidden, need_head = ctx.needs_input_grad[:2]
+        device = matrix.device
+        d_hidden = d_head = scratch = None
+        hidden_at = head_at = scratch_at = None
+        width = hidden_code = head_code = scratch_bytes = 0
+        if need_hidden:
+            shape, dtype, whole = hidden_plan
+            width = shape[-1]
+            wide = torch.bfloat16 if dtype == torch.bfloat16 else torch.float32
+            d_hidden = (torch.empty if whole else torch.zeros)(shape, dtype=wide, device=device)
+            hidden_code = _native.dtype_code(wide)
+            hidden_at = d_hidden.data_ptr() + first * width * d_hidden.element_size()
+        if need_head:
+            shape, head_dtype, scratch_bytes = head_plan
+            width = shape[1]
+            wide = torch.bfloat16 if code == _native.CT_BF16 and head_dtype == torch.bfloat16 else torch.float32
+            d_head = (torch.empty if count else torch.zeros)(shape, dtype=wide, device=device)
+            head_code, head_at = _native.dtype_code(wide), d_head.data_ptr()
+            scratch = _workspace(scratch_bytes, device)
+            scratch_at = scratch.data_ptr()
         if count:
-            # without the head's gradient the hidden rows are not read: any rows stand for them
-            rows_in = h if h is not None else d_hidden
-            call = _Call(rows_in, matrix, (indices, values, normalizer, weights), first, rows, count, temperature)
-            upstream = upstream.to(torch.float32)
-            lib = _native.library()
-            scratch = _workspace(lib.ct_head_loss_workspace(*call.sizes, 2) if d_head is not None else 0, device)
-            code = lambda t: _native.CT_F32 if t is None else _native.dtype_code(t.dtype)  # noqa: E731
-            with _native.device_of(matrix):
-                status = lib.ct_head_loss_backward(
-                    call.c, upstream.data_ptr(), kept.data_ptr(), int(kept_sums), kept.numel(), _native.ptr(hidden_out),
-                    width, width, code(d_hidden), _native.ptr(head_out), width, width, code(d_head), scratch.data_ptr(),
-                    scratch.numel(), _native.stream_of(matrix))
-            _native.check(status, "ct_head_loss_backward")
-        if d_hidden is not None:
-            d_hidden = d_hidden.to(hidden_dtype).reshape(hidden_shape)
-        if d_head is not None:
+            # a tensor that was saved may have come back in another place
+            call = _native.HeadLoss.from_buffer_copy(call)
+            call.head, call.rows = matrix.data_ptr(), _native.ptr(rows)
+            call.hidden = None if h is None else h.data_ptr() + first * h.stride(0) * h.element_size()
+            # autograd has made the tensors' device current
+            status = backward(call, upstream.to(torch.float32).data_ptr(), kept.data_ptr(), sums, kept_bytes, hidden_at, width,
+                              width, hidden_code, head_at, width, width, head_code, scratch_at, scratch_bytes,
+                              _native.stream_of(matrix))
+            if status:
+                _native.check(status, "ct_head_loss_backward")
+        if need_hidden and d_hidden.dtype != hidden_plan[1]:
+            d_hidden = d_hidden.to(hidden_plan[1])
+        if need_head and d_head.dtype != head_dtype:
             d_head = d_head.to(head_dtype)
         return d_hidden, d_head, None, None, None, None
 

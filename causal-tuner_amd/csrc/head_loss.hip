@@ -1219,7 +1219,8 @@ hipError_t launch_product(int bp, int terms, const ProductParams &p, int splits,
     return terms == 2 ? launch_product<OUT, false, 2>(bp, p, splits, s) : launch_product<OUT, false, 1>(bp, p, splits, s);
 }
 
-int check(const ct_head_loss *a, bool hidden) {
+// forward: the targets are read from the tables; later they are in what is kept.
+int check(const ct_head_loss *a, bool hidden, bool forward) {
     if (!a) return -CT_EINVAL_POINTER;
     if (a->dtype != CT_BF16 && a->dtype != CT_F32) return -CT_EINVAL_DTYPE;
     if (a->count < 0 || a->count > kMaxRows || a->width <= 0 || a->width > kMaxWidth || a->vocab <= 0 ||
@@ -1228,10 +1229,11 @@ int check(const ct_head_loss *a, bool hidden) {
     if (a->tokens < 0 || (!a->rows && a->tokens < a->count)) return -CT_EINVAL_SHAPE;
     if (a->hidden_width <= 0 || a->hidden_width > a->width || a->ld_hidden < a->hidden_width || a->ld_head < a->width)
         return -CT_EINVAL_SHAPE;
-    if (!a->values && a->entries != 1) return -CT_EINVAL_SHAPE;
-    if (a->ld_indices < a->entries || (a->values && a->ld_values < a->entries)) return -CT_EINVAL_SHAPE;
+    if (forward && !a->values && a->entries != 1) return -CT_EINVAL_SHAPE;
+    if (forward && (a->ld_indices < a->entries || (a->values && a->ld_values < a->entries))) return -CT_EINVAL_SHAPE;
     if (!(a->temperature > 0)) return -CT_EINVAL_SHAPE;
-    if (a->count && ((hidden && !a->hidden) || !a->head || !a->indices || !a->weights)) return -CT_EINVAL_POINTER;
+    if (a->count && ((hidden && !a->hidden) || !a->head)) return -CT_EINVAL_POINTER;
+    if (a->count && forward && (!a->indices || !a->weights)) return -CT_EINVAL_POINTER;
     if (a->dtype == CT_BF16 && (a->width % 8 || a->ld_head % 8)) return -CT_EINVAL_SHAPE;
     if (a->dtype == CT_BF16 && reinterpret_cast<uintptr_t>(a->head) % 16) return -CT_EINVAL_POINTER;
     return 0;
@@ -1350,7 +1352,7 @@ extern "C" int64_t ct_head_loss_workspace(int64_t count, int64_t width, int64_t 
 
 extern "C" int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t hidden_grad, void *kept,
                                     int64_t kept_bytes, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
-    if (const int bad = check(a, true)) return bad;
+    if (const int bad = check(a, true, true)) return bad;
     if (!loss) return -CT_EINVAL_POINTER;
     if (a->count == 0) {
         total_loss<<<dim3(1), dim3(1024), 0, stream>>>(nullptr, 0, loss);
@@ -1431,7 +1433,7 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
                                      int64_t kept_bytes, void *d_hidden, int64_t ld_d_hidden, int64_t d_hidden_width,
                                      int32_t d_hidden_dtype, void *d_head, int64_t ld_d_head, int64_t d_head_width,
                                      int32_t d_head_dtype, void *workspace, int64_t workspace_bytes, hipStream_t stream) {
-    if (const int bad = check(a, d_head != nullptr)) return bad;
+    if (const int bad = check(a, d_head != nullptr, false)) return bad;
     if (a->count == 0) return 0;
     if (!upstream) return -CT_EINVAL_POINTER;
     const Plan pl = plan_of(a->count, a->width, a->vocab, a->entries, a->dtype);

@@ -693,7 +693,8 @@ int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t hidden_grad
  * rows left as they are; d_head [vocab, ..] (null: none), from logits formed again piece by piece. CT_F32 or
  * CT_BF16 (d_head of float32 operands CT_F32); the first d_*_width columns are written. The
  * derivative of bf16 operands is rounded to bf16 for the head's product. hidden (not read without
- * d_head), hidden_grad and kept as the forward had them. Deterministic; kept is left as it is.
+ * d_head), head, rows, the sizes, hidden_grad and kept as the forward had them; the targets' tables are
+ * not read again. Deterministic; kept is left as it is.
  */
 int ct_head_loss_backward(const ct_head_loss *a, const float *upstream, const void *kept, int32_t hidden_grad,
                           int64_t kept_bytes, void *d_hidden, int64_t ld_d_hidden, int64_t d_hidden_width,
