@@ -47,8 +47,10 @@ constexpr int kMaxEntries = 1024;
 // that a row has would show in the gradients of few rows; of many rows they average.
 constexpr int64_t kTwoTerms = 128;
 constexpr int64_t kMaxWidth = 65536, kMaxVocab = (int64_t{1} << 31) - 1024, kMaxRows = int64_t{1} << 30;
-// E of one piece, in bytes: what two passes over it can share through the 256 MB last-level cache.
-constexpr int64_t kPieceBytes = int64_t{256} << 20;
+// Values of one piece, in bytes, whatever the batch and the vocabulary. Larger pieces read and write the
+// float32 sums less often (16384 tokens, of 49152 entries: 128 MB 6.25 ms, 256 MB 5.75, 512 MB 5.54, 1 GB
+// 5.47), smaller ones stay in the 256 MB last-level cache, which pays for less than that.
+constexpr int64_t kPieceBytes = int64_t{512} << 20;
 constexpr float kNone = -3e38f;        // the shift of a row or unit without a finite logit
 constexpr int kNoEntry = 0x7fffffff;
 
@@ -59,7 +61,7 @@ struct Plan {
     int64_t rows, width, vocab, entries;
     int dtype, bp, bl;      // a workgroup's packed rows and vocabulary entries (or columns)
     int64_t rows_pad, width_pad, units;
-    int64_t piece, pieces;  // vocabulary entries per piece of the sweep
+    int64_t piece;          // vocabulary entries per piece of the sweep
     int splits;             // of the hidden gradient's reduction
     bool turned;            // the second products read their staged operand transposed
     bool tri;               // float32 in three bf16 terms
@@ -77,6 +79,24 @@ int splits_for(int64_t tiles, int64_t slots, int64_t steps) {
         if (gain > most + 1e-9) {
             most = gain;
             best = s;
+        }
+    }
+    return best;
+}
+
+// Of `all` columns of tiles, how many make a piece: at most `most`, such that the rounds of
+// workgroups over all pieces are fewest, each further piece paying for a pass over the sums. (2665
+// rows and 192 columns of 11 tiles each: pieces of 186 and 6 columns run 9 rounds, two of 96 each 10.)
+int64_t piece_for(int64_t all, int64_t most, int64_t rows, int64_t slots) {
+    if (all <= most) return all;
+    int64_t best = most;
+    double least = 1e30;
+    for (int64_t n = most; n > most / 2; --n) {
+        const int64_t whole = all / n, rest = all % n;
+        const double cost = (double)(whole * cdiv(n * rows, slots) + cdiv(rest * rows, slots)) + 0.5 * (whole + (rest > 0));
+        if (cost < least - 1e-9) {
+            least = cost;
+            best = n;
         }
     }
     return best;
@@ -101,9 +121,7 @@ Plan plan_of(int64_t rows, int64_t width, int64_t vocab, int64_t entries, int dt
     const int64_t element = 2 * p.terms[2];
     int64_t most = kPieceBytes / (p.rows_pad * element) / 256 * 256;
     if (most < 1024) most = 1024;
-    p.pieces = cdiv(vocab, most);
-    p.piece = up(cdiv(vocab, p.pieces), 256);
-    p.pieces = cdiv(vocab, p.piece);
+    p.piece = piece_for(cdiv(vocab, 256), most / 256, p.rows_pad / p.bp * (p.bp == 64 ? 2 : 1), p.bp == 64 ? 512 : 256) * 256;
     p.turned = p.tri ? p.bp > 64 : p.bp == 256;
     const int64_t tiles = p.rows_pad / p.bp * cdiv(width, p.bl);
     p.splits = splits_for(tiles, p.bp == 64 ? 512 : 256, p.piece / kStep);
@@ -202,16 +220,16 @@ __device__ __forceinline__ float block_max(float v, float *lds) {
 // One workgroup per row: q of its entries, sorted by index with equal indices joined, the entries
 // outside the vocabulary dropped; `first` [row][unit] counts the entries before each unit. Rows of
 // the padding get no entries and no weight.
-template <int THREADS>
+template <int THREADS, int MOST>
 __global__ __launch_bounds__(THREADS) void targets_kernel(Targets t, int64_t rows, int entries, int64_t vocab,
                                                           int64_t units, double inverse_t, int *__restrict__ index,
                                                           float *__restrict__ q_out, float *__restrict__ chosen,
                                                           uint16_t *__restrict__ first, float *__restrict__ weight,
                                                           float *__restrict__ mass, float *__restrict__ entropy,
                                                           float *__restrict__ shift, float *__restrict__ total) {
-    __shared__ uint64_t key[kMaxEntries];
-    __shared__ float value[kMaxEntries], lds[THREADS];
-    __shared__ int sorted[kMaxEntries], kept;
+    __shared__ uint64_t key[MOST];
+    __shared__ float value[MOST], lds[THREADS];
+    __shared__ int sorted[MOST], kept;
     const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
     if (tid == 0) {
@@ -291,11 +309,16 @@ __global__ __launch_bounds__(THREADS) void targets_kernel(Targets t, int64_t row
         }
     __syncthreads();
     // The first of equal indices takes their sum; its place is the count of firsts before it.
-    if (tid == 0) {
+    if (tid < 64) {
         int n = 0;
-        for (int e = 0; e < size && key[e] != ~uint64_t{0}; ++e)
-            if (e == 0 || (key[e] >> 32) != (key[e - 1] >> 32)) sorted[n++] = e;
-        kept = n;
+        for (int base = 0; base < size; base += 64) {
+            const int e = base + tid;
+            const bool is = e < size && key[e] != ~uint64_t{0} && (e == 0 || (key[e] >> 32) != (key[e - 1] >> 32));
+            const uint64_t all = __builtin_amdgcn_ballot_w64(is);
+            if (is) sorted[n + __builtin_popcountll(all & ((uint64_t{1} << tid) - 1))] = e;
+            n += __builtin_popcountll(all);
+        }
+        if (tid == 0) kept = n;
     }
     __syncthreads();
     float held = 0.f, ent = 0.f;
@@ -515,7 +538,8 @@ __device__ __forceinline__ void tile_of(int64_t id, int64_t np, int64_t nl, int6
 //
 // A step of 64 indices runs column by column (a fragment of the staged operand against all packed
 // ones), the order of everything in it fixed: a column's fragments are read three columns ahead, the
-// first three of the next step's at the end of this one, which its third stage allows; the loads and
+// first three of the next step's at the end of this one, which its third stage allows, and the packed
+// fragments loaded two steps ahead; the loads and
 // the stores of the tiles to come lie one by one between the columns. (In one run each, all waves queue
 // behind them: 3% slower.) Eight waves side by side along the packed rows read no packed row twice;
 // 4 x 2 waves, with half the LDS reads and twice the packed loads, are 6% slower, two workgroups of four
@@ -634,7 +658,7 @@ struct Core {
                                             f32x4 (&acc)[LF][PF]) const {
         if constexpr (F < LF) {
             read(F + 3 < LF ? cur : nxt, (F + 3) % LF, lf[(F + 3) % 4]);
-            if constexpr (F % (LF / 8) == 0 && F / (LF / 8) < KS * PF) load_a<F / (LF / 8)>(t + 1, an);
+            if constexpr (F % (LF / 8) == 0 && F / (LF / 8) < KS * PF) load_a<F / (LF / 8)>(t + 2, an);
             if constexpr (F % (LF / 4) == LF / 8 - 1) store_b<F / (LF / 4)>(wr, b);
             if constexpr (F % (LF / 4) == LF / 4 - 1) load_b<F / (LF / 4)>(t + 3, b);
 #pragma unroll
@@ -656,19 +680,19 @@ struct Core {
         __syncthreads();
     }
     template <int I>
-    __device__ __forceinline__ void first(uint4 *stages, uint4 (&b)[kPer], uint4 (&more)[kPer], uint4 (&af)[KS][PF]) const {
+    __device__ __forceinline__ void first(uint4 *stages, uint4 (&b)[kPer], uint4 (&more)[kPer], uint4 (&af)[KS][PF], uint4 (&ag)[KS][PF]) const {
         static_assert(kPer == 4 && KS * PF <= 8, "spread over the columns");
         if constexpr (I < 4) {
             load_b<I>(0, b);
             load_b<I>(1, more);
         } else if constexpr (I < 12) {
-            if constexpr (I - 4 < KS * PF) load_a<I - 4>(0, af);
+            if constexpr (I - 4 < KS * PF) { load_a<I - 4>(0, af); load_a<I - 4>(1, ag); }
         } else if constexpr (I < 16) {
             store_b<I - 12>(stages, b);
             store_b<I - 12>(stages + kStage, more);
             load_b<I - 12>(2, b);
         }
-        if constexpr (I < 15) first<I + 1>(stages, b, more, af);
+        if constexpr (I < 15) first<I + 1>(stages, b, more, af, ag);
     }
     __device__ __forceinline__ void run(uint4 *stages, f32x4 (&acc)[LF][PF]) const {
 #pragma unroll
@@ -676,18 +700,20 @@ struct Core {
 #pragma unroll
             for (int j = 0; j < PF; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (steps <= 0) return;
-        uint4 b[kPer], more[kPer], a0[KS][PF], a1[KS][PF], lf[4][2];
-        first<0>(stages, b, more, a0);
+        uint4 b[kPer], more[kPer], a0[KS][PF], a1[KS][PF], a2[KS][PF], lf[4][2];
+        first<0>(stages, b, more, a0, a1);
         __syncthreads();
         read(stages, 0, lf[0]);
         read(stages, 1, lf[1]);
         read(stages, 2, lf[2]);
         int t = 0, at = 0;
-        for (; t + 1 < steps; t += 2) {
-            step(t, stages, at, a0, a1, b, lf, acc);
+        for (; t + 2 < steps; t += 3) {
+            step(t, stages, at, a0, a2, b, lf, acc);
             step(t + 1, stages, at, a1, a0, b, lf, acc);
+            step(t + 2, stages, at, a2, a1, b, lf, acc);
         }
-        if (t < steps) step(t, stages, at, a0, a1, b, lf, acc);
+        if (t < steps) step(t, stages, at, a0, a2, b, lf, acc);
+        if (t + 1 < steps) step(t + 1, stages, at, a1, a0, b, lf, acc);
     }
 };
 
@@ -1374,8 +1400,8 @@ extern "C" int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t 
             at<float>(kept, k.chosen), at<uint16_t>(kept, k.first), at<float>(kept, k.weight), at<float>(kept, k.mass),
             at<float>(kept, k.entropy), shift, total);
     };
-    if (pl.entries <= 64) targets(targets_kernel<64>, 64);
-    else targets(targets_kernel<256>, 256);
+    if (pl.entries <= 64) targets(targets_kernel<64, 64>, 64);
+    else targets(targets_kernel<256, kMaxEntries>, 256);
     CT_TRY(hipGetLastError());
 
     CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), stream));
