@@ -378,25 +378,27 @@ __global__ __launch_bounds__(256) void columns_wide(const void *__restrict__ x, 
 
 bool aligned(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// The team and chunks per thread that hold a row of `units` chunks: the smallest of these.
-
+// The smallest of the teams and chunks per thread that hold a row. Rows that 16-byte accesses do not fit
+// (chunks of one element) take many chunks to a thread, so that as many bytes are under way:
+// 30000 x 1023 float32 on teams of 256 and 1024 with one to four chunks ran at 3.3 TB/s forward and 2.3 backward.
 struct Shape {
     int team, chunks;   // team 0: rows wider than the registers
 };
-Shape forward_shape(int64_t units) {
-    for (const Shape s : {Shape{64, 1}, Shape{64, 2}, Shape{64, 4}, Shape{256, 2}, Shape{256, 4}, Shape{1024, 2},
-                          Shape{1024, 8}})
+template <int N>
+Shape smallest(const Shape (&shapes)[N], int64_t units) {
+    for (const Shape s : shapes)
         if (units <= (int64_t)s.team * s.chunks) return s;
     return Shape{0, 0};
 }
-Shape backward_shape(int64_t units) {
-    for (const Shape s : {Shape{64, 1}, Shape{64, 2}, Shape{256, 1}, Shape{256, 2}, Shape{1024, 1}, Shape{1024, 2}})
-        if (units <= (int64_t)s.team * s.chunks) return s;
-    return Shape{0, 0};
-}
+constexpr Shape kForwardWide[] = {{64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {1024, 2}, {1024, 8}};
+constexpr Shape kForwardSingle[] = {{64, 1}, {64, 4}, {64, 16}, {256, 16}, {1024, 16}};
+constexpr Shape kBackwardWide[] = {{64, 1}, {64, 2}, {256, 1}, {256, 2}, {1024, 1}, {1024, 2}};
+constexpr Shape kBackwardSingle[] = {{64, 1}, {64, 4}, {64, 16}, {256, 16}, {1024, 16}};
+Shape forward_shape(int64_t units, bool vec) { return vec ? smallest(kForwardWide, units) : smallest(kForwardSingle, units); }
+Shape backward_shape(int64_t units, bool vec) { return vec ? smallest(kBackwardWide, units) : smallest(kBackwardSingle, units); }
 int64_t backward_teams(Shape s, int64_t rows) {
     if (s.team == 0) return rows < 64 ? rows : 64;
-    const int64_t per = s.team == 64 ? 4 : 1, most = s.team == 1024 ? 256 : 512;   // workgroups
+    const int64_t per = s.team == 64 ? 4 : 1, most = s.team == 1024 ? 256 : 512;   // workgroups (twice as many: 12% slower)
     const int64_t blocks = cdiv(rows, per);
     return (blocks < most ? blocks : most) * per;
 }
@@ -407,17 +409,29 @@ int64_t units_of(int64_t width, int dtype, bool vec) {
 template <int DT, int E>
 hipError_t launch_forward(const void *x, const void *w, const void *bias, int w_dtype, void *y, float *mean, float *rstd,
                           int64_t rows, int64_t width, float eps, hipStream_t stream) {
-    const Shape s = forward_shape(cdiv(width, E));
-    const auto run = [&](auto kernel, int threads, int64_t blocks) {
-        kernel<<<dim3((unsigned)blocks), dim3(threads), 0, stream>>>(x, w, bias, w_dtype, y, mean, rstd, rows, width, eps);
+    const Shape s = forward_shape(cdiv(width, E), E > 1);
+    const auto is = [&](int team, int chunks) { return s.team == team && s.chunks == chunks; };
+    const auto run = [&](auto kernel) {
+        kernel<<<dim3((unsigned)(s.team == 64 ? cdiv(rows, 4) : rows)), dim3(s.team > 256 ? s.team : 256), 0, stream>>>(
+            x, w, bias, w_dtype, y, mean, rstd, rows, width, eps);
     };
-    if (s.team == 64 && s.chunks == 1) run(forward_kernel<DT, E, 64, 1>, 256, cdiv(rows, 4));
-    else if (s.team == 64 && s.chunks == 2) run(forward_kernel<DT, E, 64, 2>, 256, cdiv(rows, 4));
-    else if (s.team == 64) run(forward_kernel<DT, E, 64, 4>, 256, cdiv(rows, 4));
-    else if (s.team == 256 && s.chunks == 2) run(forward_kernel<DT, E, 256, 2>, 256, rows);
-    else if (s.team == 256) run(forward_kernel<DT, E, 256, 4>, 256, rows);
-    else if (s.team == 1024 && s.chunks == 2) run(forward_kernel<DT, E, 1024, 2>, 1024, rows);
-    else if (s.team == 1024) run(forward_kernel<DT, E, 1024, 8>, 1024, rows);
+    if (is(64, 1)) run(forward_kernel<DT, E, 64, 1>);
+    else if (is(64, 4)) run(forward_kernel<DT, E, 64, 4>);
+    else if (s.team && E > 1) {
+        if constexpr (E > 1) {
+            if (is(64, 2)) run(forward_kernel<DT, E, 64, 2>);
+            else if (is(256, 2)) run(forward_kernel<DT, E, 256, 2>);
+            else if (is(256, 4)) run(forward_kernel<DT, E, 256, 4>);
+            else if (is(1024, 2)) run(forward_kernel<DT, E, 1024, 2>);
+            else run(forward_kernel<DT, E, 1024, 8>);
+        }
+    } else if (s.team) {
+        if constexpr (E == 1) {
+            if (is(64, 16)) run(forward_kernel<DT, E, 64, 16>);
+            else if (is(256, 16)) run(forward_kernel<DT, E, 256, 16>);
+            else run(forward_kernel<DT, E, 1024, 16>);
+        }
+    }
     else forward_wide<DT><<<dim3((unsigned)rows), dim3(1024), 0, stream>>>(x, w, bias, w_dtype, y, mean, rstd, width, eps);
     return hipGetLastError();
 }
@@ -425,16 +439,29 @@ hipError_t launch_forward(const void *x, const void *w, const void *bias, int w_
 template <int DT, int E>
 hipError_t launch_backward(const void *x, const void *w, int w_dtype, const float *mean, const float *rstd, const void *dy,
                            void *dx, float *partial, int64_t teams, int64_t rows, int64_t width, hipStream_t stream) {
-    const Shape s = backward_shape(cdiv(width, E));
-    const auto run = [&](auto kernel, int threads, int64_t blocks) {
-        kernel<<<dim3((unsigned)blocks), dim3(threads), 0, stream>>>(x, w, w_dtype, mean, rstd, dy, dx, partial, rows, width);
+    const Shape s = backward_shape(cdiv(width, E), E > 1);
+    const auto is = [&](int team, int chunks) { return s.team == team && s.chunks == chunks; };
+    const auto run = [&](auto kernel) {
+        kernel<<<dim3((unsigned)(s.team == 64 ? teams / 4 : teams)), dim3(s.team > 256 ? s.team : 256), 0, stream>>>(
+            x, w, w_dtype, mean, rstd, dy, dx, partial, rows, width);
     };
-    if (s.team == 64 && s.chunks == 1) run(backward_kernel<DT, E, 64, 1>, 256, teams / 4);
-    else if (s.team == 64) run(backward_kernel<DT, E, 64, 2>, 256, teams / 4);
-    else if (s.team == 256 && s.chunks == 1) run(backward_kernel<DT, E, 256, 1>, 256, teams);
-    else if (s.team == 256) run(backward_kernel<DT, E, 256, 2>, 256, teams);
-    else if (s.team == 1024 && s.chunks == 1) run(backward_kernel<DT, E, 1024, 1>, 1024, teams);
-    else if (s.team == 1024) run(backward_kernel<DT, E, 1024, 2>, 1024, teams);
+    if (is(64, 1)) run(backward_kernel<DT, E, 64, 1>);
+    else if (s.team && E > 1) {
+        if constexpr (E > 1) {
+            if (is(64, 2)) run(backward_kernel<DT, E, 64, 2>);
+            else if (is(256, 1)) run(backward_kernel<DT, E, 256, 1>);
+            else if (is(256, 2)) run(backward_kernel<DT, E, 256, 2>);
+            else if (is(1024, 1)) run(backward_kernel<DT, E, 1024, 1>);
+            else run(backward_kernel<DT, E, 1024, 2>);
+        }
+    } else if (s.team) {
+        if constexpr (E == 1) {
+            if (is(64, 4)) run(backward_kernel<DT, E, 64, 4>);
+            else if (is(64, 16)) run(backward_kernel<DT, E, 64, 16>);
+            else if (is(256, 16)) run(backward_kernel<DT, E, 256, 16>);
+            else run(backward_kernel<DT, E, 1024, 16>);
+        }
+    }
     else {
         if (dx) backward_wide<DT><<<dim3((unsigned)rows), dim3(1024), 0, stream>>>(x, w, w_dtype, mean, rstd, dy, dx, width);
         hipError_t e = hipGetLastError();
@@ -471,8 +498,8 @@ extern "C" int ct_layer_norm_forward(const void *x, int32_t x_dtype, const void 
 // The larger of the two counts of teams that the call may take, by its pointers' alignment.
 extern "C" int64_t ct_layer_norm_backward_workspace(int64_t rows, int64_t width, int32_t x_dtype, int32_t weight_grad) {
     if (rows <= 0 || width <= 0 || !weight_grad || !known(x_dtype)) return 0;
-    const int64_t a = backward_teams(backward_shape(units_of(width, x_dtype, true)), rows);
-    const int64_t b = backward_teams(backward_shape(units_of(width, x_dtype, false)), rows);
+    const int64_t a = backward_teams(backward_shape(units_of(width, x_dtype, true), true), rows);
+    const int64_t b = backward_teams(backward_shape(units_of(width, x_dtype, false), false), rows);
     return (a > b ? a : b) * 2 * width * (int64_t)sizeof(float);
 }
 
@@ -491,7 +518,7 @@ extern "C" int ct_layer_norm_backward(const void *x, int32_t x_dtype, const void
             return -CT_EINVAL_WORKSPACE;
         if (!grad) partial = nullptr;
         const bool vec = aligned(x) && aligned(dy) && aligned(dx) && aligned(w) && width % (x_dtype == CT_F32 ? 4 : 8) == 0;
-        teams = backward_teams(backward_shape(units_of(width, x_dtype, vec)), rows);
+        teams = backward_teams(backward_shape(units_of(width, x_dtype, vec), vec), rows);
         const auto run = [&](auto launch) {
             return launch(x, w, w_dtype, mean, rstd, dy, dx, partial, teams, rows, width, stream);
         };
