@@ -15,6 +15,12 @@ from . import _native
 from .loss import row_count
 
 
+_MAX_PITCH = 1 << 20     # elements between two rows
+_MAX_WIDTH = 1 << 16
+_MAX_VOCAB = (1 << 31) - 1024
+_MAX_ROWS = 1 << 30
+
+
 def _rows_of(selection, tokens, device):
     """(first row, row indices or None, count) of a selection."""
     if isinstance(selection, slice):
@@ -27,22 +33,26 @@ def _rows_of(selection, tokens, device):
     return 0, selection.to(device, torch.int64).contiguous(), row_count(selection)
 
 
+def _plain(t):
+    """Whether t's rows have unit stride and a pitch that the kernels take."""
+    return t.stride(1) == 1 and t.shape[1] <= t.stride(0) <= _MAX_PITCH
+
+
 def _aligned_head(head):
     """`head` with unit-stride rows that start at 16-byte boundaries, bf16 widths a multiple of 8:
     itself, or a copy padded with zeros."""
-    if head.dtype != torch.bfloat16:
-        return head if head.stride(1) == 1 and head.stride(0) >= head.shape[1] else head.contiguous()
-    pad = -head.shape[1] % 8
-    if pad:
-        return torch.nn.functional.pad(head, (0, pad))
-    if head.stride(1) != 1 or head.stride(0) % 8 or head.stride(0) < head.shape[1] or head.data_ptr() % 16:
-        return head.clone(memory_format=torch.contiguous_format)
-    return head
+    if head.dtype == torch.bfloat16:
+        pad = -head.shape[1] % 8
+        if pad:
+            return torch.nn.functional.pad(head, (0, pad))
+        if head.stride(0) % 8 or head.data_ptr() % 16:
+            return head.clone(memory_format=torch.contiguous_format)
+    return head if _plain(head) else head.clone(memory_format=torch.contiguous_format)
 
 
 def _plain_rows(hidden):
     h = hidden.reshape(-1, hidden.shape[-1])
-    return h if h.stride(1) == 1 and h.stride(0) >= h.shape[1] else h.contiguous()
+    return h if _plain(h) else h.clone(memory_format=torch.contiguous_format)
 
 
 def _workspace(nbytes, device):
@@ -136,6 +146,9 @@ def streamed_loss(hidden, head, weights, selection, compute_dtype, indices, valu
     """The loss of device tensors: hard labels `indices` [tokens, 1], or a teacher's entries."""
     if compute_dtype not in (torch.bfloat16, torch.float32):
         raise NotImplementedError("streamed head loss: the HIP kernels compute in bfloat16 or float32")
+    if head.shape[1] > _MAX_WIDTH or len(head) > _MAX_VOCAB or weights.numel() > _MAX_ROWS:
+        raise ValueError(f"streamed head loss: {weights.numel()} rows, head {tuple(head.shape)}; the HIP kernels take up to "
+                         f"{_MAX_ROWS} rows, {_MAX_VOCAB} entries and a width of {_MAX_WIDTH}")
     _native.refuse_tangents("streamed head loss", hidden, head)
     device = hidden.device
     wide = lambda t: None if t is None else t.to(device, torch.float32).contiguous()  # noqa: E731

@@ -72,6 +72,8 @@ def projection_loss(hidden, head, targets, weights, *, token_budget=128, compute
     if implementation == "streamed":
         if reuse_hidden:
             raise ValueError("reuse_hidden applies only to the fused backend")
+        if targets.is_floating_point():
+            raise ValueError("targets are whole numbers")
         _check_rows(hidden, head, weights, {"targets": targets})
     if not hidden.is_cuda:
         return ProjectionLoss.apply(hidden, head, targets, weights, token_budget, compute_dtype, selection)

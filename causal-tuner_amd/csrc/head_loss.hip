@@ -46,6 +46,7 @@ constexpr int kMaxEntries = 1024;
 // derivative) are kept in two bf16 terms. One rounding, by up to 2^-8, of the one or two large values
 // that a row has would show in the gradients of few rows; of many rows they average.
 constexpr int64_t kTwoTerms = 128;
+constexpr int64_t kMaxPitch = 1 << 20;   // a tile's offsets stay below 2^31
 constexpr int64_t kMaxWidth = 65536, kMaxVocab = (int64_t{1} << 31) - 1024, kMaxRows = int64_t{1} << 30;
 // Values of one piece, in bytes, whatever the batch and the vocabulary. Larger pieces read and write the
 // float32 sums less often (16384 tokens, of 49152 entries: 128 MB 6.25 ms, 256 MB 5.75, 512 MB 5.54, 1 GB
@@ -1253,7 +1254,8 @@ int check(const ct_head_loss *a, bool hidden, bool forward) {
         a->vocab > kMaxVocab || a->entries < 1 || a->entries > kMaxEntries)
         return -CT_EINVAL_SHAPE;
     if (a->tokens < 0 || (!a->rows && a->tokens < a->count)) return -CT_EINVAL_SHAPE;
-    if (a->hidden_width <= 0 || a->hidden_width > a->width || a->ld_hidden < a->hidden_width || a->ld_head < a->width)
+    if (a->hidden_width <= 0 || a->hidden_width > a->width || a->ld_hidden < a->hidden_width || a->ld_head < a->width ||
+        a->ld_hidden > kMaxPitch || a->ld_head > kMaxPitch)
         return -CT_EINVAL_SHAPE;
     if (forward && !a->values && a->entries != 1) return -CT_EINVAL_SHAPE;
     if (forward && (a->ld_indices < a->entries || (a->values && a->ld_values < a->entries))) return -CT_EINVAL_SHAPE;

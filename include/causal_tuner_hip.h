@@ -653,7 +653,8 @@ int ct_muon(const ct_muon_matrix *matrices, int64_t count, const int32_t *plan, 
  * q = softmax(values / temperature) over a row's entries, or with log_normalizer float32 [*]
  * q = exp(values / temperature - log_normalizer). An index outside [0, vocab) is no entry,
  * an index given twice counts once with the sum of both, and a row without entries has no loss.
- * bf16: width and ld_head multiples of 8, head 16-byte aligned.
+ * bf16: width and ld_head multiples of 8, head 16-byte aligned. Pitches of hidden and head up to 2^20,
+ * width up to 65536, entries up to 1024.
  */
 typedef struct ct_head_loss {
     const void *hidden;

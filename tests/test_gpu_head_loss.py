@@ -114,6 +114,47 @@ def test_many_pieces(teacher):
     _check(loss, hidden, head, indices, values, weights, BF16)
 
 
+@pytest.mark.parametrize("dtype,rows,vocab", [(BF16, 4100, 70001), (F32, 2100, 45001)])
+@pytest.mark.parametrize("order", [1, -1])
+def test_maxima_that_move_between_pieces(order, dtype, rows, vocab):
+    """The sums of the pieces before are brought to a larger shift, or later units to theirs."""
+    hidden, head, labels, weights = _inputs(rows, 64, vocab, dtype)
+    with torch.no_grad():
+        size = torch.linspace(0.2, 40.0, vocab, device="cuda")[:, None]
+        head.mul_(size if order > 0 else size.flip(0))
+    weights = weights / rows
+    _check(_streamed(hidden, head, labels, weights, dtype), hidden, head, labels[:, None], None, weights, dtype)
+
+
+def test_offsets_past_32_bits():
+    """A head of 2.3e9 values, nearly all rows zero, so that what they add is known: logits of 0 and no
+    gradient of the hidden rows."""
+    vocab, width, rows = 140000, 16384, 3
+    filled = torch.tensor([0, 1, vocab // 2, vocab - 2, vocab - 1], device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    hidden = torch.randn(rows, width, device="cuda", generator=g).to(BF16).requires_grad_()
+    head = torch.zeros(vocab, width, device="cuda", dtype=BF16)
+    head[filled] = (torch.randn(5, width, device="cuda", generator=g) * 0.1).to(BF16)
+    head.requires_grad_()
+    labels = torch.tensor([vocab - 1, 0, vocab - 2], device="cuda")
+    weights = torch.tensor([1.0, 0.5, 2.0], device="cuda")
+    loss = _streamed(hidden, head, labels, weights, BF16)
+    dh, dw = _grads(loss, hidden, head)
+    h, w, c = hidden.detach().double(), head.detach()[filled].double(), weights.double()[:, None]
+    logits = h @ w.T
+    z = logits.exp().sum(-1, keepdim=True) + (vocab - 5)
+    q = (filled == labels[:, None]).double()
+    d = c * (logits.exp() / z - q)
+    # logits are float32 chains of 16384 products: 2^-10 of a few dozen; the results are rounded to bf16
+    assert abs(loss.item() - (c * (z.log() - (q * logits).sum(-1, keepdim=True))).sum().item()) < 0.05
+    assert ((dh.double() - d @ w).norm(dim=-1) <= 2e-2 * (d @ w).norm(dim=-1)).all()
+    want = d.T @ h
+    assert ((dw[filled].double() - want).norm(dim=-1) <= 2e-2 * want.norm(dim=-1)).all()
+    other = (c / z).T @ h   # of a row of zeros
+    for row in (2, vocab // 2 + 1, vocab - 3):
+        assert (dw[row].double() - other[0]).norm() <= 2e-2 * other.norm()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("scale", [1e-3, 40.0, 400.0])
 def test_logits_of_any_size(scale, dtype):
@@ -213,7 +254,10 @@ def test_strides_and_alignments():
         wide_w = torch.randn(700, 141, device="cuda").to(BF16)
         wide_h[:, 1, 3:139], wide_w[:, 5:] = base_h, base_w
         column = base_w.detach().T.contiguous().T
-    views = [(wide_h.detach()[:, 1, 3:139], wide_w.detach()[:, 5:]), (base_h.detach()[:, :], column),
+        far_h, far_w = (torch.empty(n, 1 << 20 | 8, device="cuda", dtype=BF16)[:, 8:144] for n in (90, 700))
+        far_h.copy_(base_h)
+        far_w.copy_(base_w)
+    views = [(far_h, far_w), (wide_h.detach()[:, 1, 3:139], wide_w.detach()[:, 5:]), (base_h.detach()[:, :], column),
              (base_h.detach().T.contiguous().T, base_w.detach())]
     loss = _streamed(base_h, base_w, labels, weights, BF16)
     want = (loss.detach(), *_grads(loss, base_h, base_w))
@@ -335,6 +379,12 @@ def test_refusals():
         _streamed(hidden, head, labels.cpu(), weights, BF16)
     with pytest.raises(ValueError, match="indices"):
         distillation_loss(hidden, head, labels[:, None].cpu(), torch.zeros(4, 1), weights)
+    with pytest.raises(ValueError, match="width"):
+        _streamed(hidden.new_zeros(4, 65544), hidden.new_zeros(2, 65544), labels, weights, BF16)
+    for rows in (torch.ones(4, dtype=torch.bool, device="cuda"), torch.zeros(2, 1, dtype=torch.int64, device="cuda"),
+                 slice(0, 4, 2)):
+        with pytest.raises(ValueError, match="rows"):
+            _streamed(hidden, head, labels, weights, BF16, rows=rows)
     loss = _streamed(hidden, head, labels, weights, BF16)
     grad, = torch.autograd.grad(loss, hidden, create_graph=True)
     with pytest.raises(RuntimeError):

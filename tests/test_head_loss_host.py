@@ -110,6 +110,8 @@ def test_refusals():
         projection_loss(hidden, head, targets, weights, implementation="streamed", reuse_hidden=True)
     with pytest.raises(ValueError, match="targets"):
         projection_loss(hidden, head, targets[:5], weights, implementation="streamed")
+    with pytest.raises(ValueError, match="whole numbers"):
+        projection_loss(hidden, head, targets.float(), weights, implementation="streamed")
     with pytest.raises(ValueError, match="positive"):
         projection_loss(hidden, head, targets, weights, implementation="streamed", token_budget=0)
 
@@ -126,7 +128,8 @@ def test_library_refuses_bad_operands_on_the_host():
                        (dict(vocab=1 << 31), -2), (dict(entries=0), -2), (dict(entries=1025, values=256), -2),
                        (dict(entries=2), -2), (dict(tokens=3), -2), (dict(ld_head=63), -2), (dict(ld_hidden=63), -2),
                        (dict(hidden_width=65), -2), (dict(temperature=0.0), -2), (dict(temperature=math.nan), -2),
-                       (dict(dtype=_native.CT_F16), -3), (dict(values=256, ld_values=0), -2)]:
+                       (dict(dtype=_native.CT_F16), -3), (dict(ld_head=1 << 21), -2),
+                       (dict(ld_hidden=1 << 21), -2), (dict(width=1 << 17, ld_head=1 << 17), -2), (dict(values=256, ld_values=0), -2)]:
         assert forward(**kw) == status, kw
     sizes = (4, 64, 100, 1, _native.CT_BF16)
     kept, scratch = lib.ct_head_loss_kept(*sizes, 1), lib.ct_head_loss_workspace(*sizes, 1)
