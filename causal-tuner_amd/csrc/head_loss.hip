@@ -67,6 +67,7 @@ struct Plan {
     bool turned;            // the second products read their staged operand transposed
     bool tri;               // float32 in three bf16 terms
     int terms[3];           // bf16 terms of a piece's values, by sweep
+    int chunks;             // of the logits' reduction; more than one: logits in memory, exponentials by row
 };
 
 // Workgroups' worth of work in whole rounds: how many splits of a reduction of `steps` leave the
@@ -103,6 +104,15 @@ int64_t piece_for(int64_t all, int64_t most, int64_t rows, int64_t slots) {
     return best;
 }
 
+// A small vocabulary's logits are a few tiles, each a chain of the width's steps. Where they leave more
+// than half of the compute units idle and the chain is worth cutting, it is cut: the logits, at most
+// 128 tiles of them, go through memory. (18 rows x 328 entries x 3496, float32: 1.15 ms in one chain.)
+int chunks_for(int64_t tiles, int64_t steps) {
+    if (tiles > 128 || steps < 8) return 1;
+    const int64_t idle = cdiv(256, tiles), most = steps / 4;
+    return (int)(idle < most ? idle : most);
+}
+
 Plan plan_of(int64_t rows, int64_t width, int64_t vocab, int64_t entries, int dtype) {
     Plan p{};
     p.rows = rows;
@@ -126,6 +136,7 @@ Plan plan_of(int64_t rows, int64_t width, int64_t vocab, int64_t entries, int dt
     p.turned = p.tri ? p.bp > 64 : p.bp == 256;
     const int64_t tiles = p.rows_pad / p.bp * cdiv(width, p.bl);
     p.splits = splits_for(tiles, p.bp == 64 ? 512 : 256, p.piece / kStep);
+    p.chunks = chunks_for(p.rows_pad / p.bp * cdiv(vocab, p.bl), p.width_pad / kStep);
     return p;
 }
 
@@ -158,7 +169,7 @@ Kept kept_of(const Plan &p, bool hidden_grad) {
     return k;
 }
 struct Scratch {
-    int64_t packed, plain, piece, turned, split, stats, factor, inverse, near, losses, bytes;
+    int64_t packed, plain, piece, turned, split, logits, stats, factor, inverse, near, losses, bytes;
 };
 // sweep 0: statistics alone, 1: with the hidden gradient's sums, 2: the head's gradient.
 Scratch scratch_of(const Plan &p, int sweep) {
@@ -172,7 +183,8 @@ Scratch scratch_of(const Plan &p, int sweep) {
     s.turned = r.take(sweep == 0 ? 0 : p.turned ? p.width * terms * (sweep == 1 ? p.piece : steps)
                                                 : p.tri && sweep == 2 ? p.rows * pitch * terms : 0);
     s.split = r.take(p.tri ? p.piece * pitch * terms : 0);
-    s.stats = r.take(sweep == 2 ? 0 : piece / kUnit * p.rows_pad * 8);
+    s.logits = r.take(p.chunks > 1 ? p.chunks * p.rows * p.vocab * 4 : 0);
+    s.stats = r.take(sweep == 2 || p.chunks > 1 ? 0 : piece / kUnit * p.rows_pad * 8);
     s.factor = r.take(p.rows_pad * 4);
     s.inverse = r.take(p.rows_pad * 4);
     s.near = r.take(p.rows_pad * 4);
@@ -1051,6 +1063,100 @@ __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductPara
     }
 }
 
+// ------------------------------------------------------------------------- logits in memory
+struct RowParams {
+    float *logits;             // [chunks][rows][vocab], summed into the first
+    int chunks;
+    int64_t slab, rows, vocab;
+    float scale;
+    float *shift, *total;
+    const int *index;
+    const uint16_t *first;
+    float *chosen;
+    int entries;
+    int64_t units;
+    uint4 *piece;
+    int64_t piece_blocks, piece_apart;
+    const float *near, *factor, *inverse;
+};
+
+// What logits_kernel<EXP> and join_kernel do, a workgroup per row; zeros past the vocabulary up to a
+// whole step of the product that follows. TERMS 0: the statistics alone.
+template <int TERMS>
+__global__ __launch_bounds__(256) void rows_exp(const RowParams p) {
+    __shared__ float lds[256];
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    float *l = p.logits + row * p.vocab;
+    float top = -INFINITY;
+    for (int64_t v = tid; v < p.vocab; v += 256) {
+        float x = l[v];
+        for (int s = 1; s < p.chunks; ++s) x += l[s * p.slab + v];
+        l[v] = x;
+        top = fmaxf(top, x);
+    }
+    top = block_max<256>(top, lds);
+    const float c = fmaxf(ceilf(top * p.scale), kNone);
+    const int n = p.first[row * (p.units + 1) + p.units];
+    for (int e = tid; e < n; e += 256) {
+        float *at = l + p.index[row * p.entries + e];
+        p.chosen[row * p.entries + e] = *at;
+        *at = -INFINITY;
+    }
+    __syncthreads();
+    float sum = 0.f;
+    for (int64_t u = tid; u < up(p.vocab, kStep) / 8; u += 256) {   // 32 entries: four units
+        const int64_t block = u >> 2;
+        const int q = (int)(u & 3);
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int64_t v = block * 32 + (i >> 2) * 16 + q * 4 + (i & 3);
+            e[i] = v < p.vocab ? __builtin_amdgcn_exp2f(__builtin_fmaf(l[v], p.scale, -c)) : 0.f;
+            sum += e[i];
+        }
+        if constexpr (TERMS > 0)
+            store_unit<TERMS>(p.piece + ((row >> 4) * p.piece_blocks + block) * 64 + q * 16 + (row & 15), p.piece_apart, e);
+    }
+    sum = block_sum<256>(sum, lds);
+    if (tid == 0) {
+        p.shift[row] = c;
+        p.total[row] = sum;
+    }
+}
+
+// What logits_kernel<GRAD> does, a workgroup per row; zeros in the rows of the padding.
+template <int TERMS>
+__global__ __launch_bounds__(256) void rows_grad(const RowParams p) {
+    const int64_t row = blockIdx.x;
+    const int in = (int)(row & 31);
+    uint16_t *out = reinterpret_cast<uint16_t *>(p.piece) +
+                    ((row >> 5) * 64 + (in & 15) / 4 * 16) * 8 + (in & 3) + (in >> 4) * 4;
+    const auto put = [&](int64_t v, float d) {
+#pragma unroll
+        for (int s = 0; s < TERMS; ++s) {
+            const uint16_t bits = bf16_bits(d);
+            out[s * p.piece_apart * 8 + ((v >> 4) * p.piece_blocks * 64 + (v & 15)) * 8] = bits;
+            d -= bf16_to_f32(bits);
+        }
+    };
+    if (row >= p.rows) {
+        for (int64_t v = threadIdx.x; v < p.vocab; v += 256) put(v, 0.f);
+        return;
+    }
+    const float *l = p.logits + row * p.vocab;
+    const float c = p.near[row], f = p.factor[row];
+    for (int64_t v = threadIdx.x; v < p.vocab; v += 256) {
+        float x = l[v];
+        for (int s = 1; s < p.chunks; ++s) x += l[s * p.slab + v];
+        put(v, __builtin_amdgcn_exp2f(__builtin_fmaf(x, p.scale, -c)) * f);
+    }
+    __syncthreads();
+    const int n = p.first[row * (p.units + 1) + p.units];
+    for (int e = (int)threadIdx.x; e < n; e += 256)
+        put(p.index[row * p.entries + e], p.inverse[row] * p.chosen[row * p.entries + e]);
+}
+
 // ------------------------------------------------------------------------- the ends
 // A row's loss, the coefficients Q p_k - q_k of its targets in place of their logits, and Z with the
 // targets' own terms in place of the others' sum. In double, from the targets' exponentials and the
@@ -1228,7 +1334,8 @@ template <int OUT, bool KT, int TERMS>
 hipError_t launch_product(int bp, const ProductParams &p, int splits, hipStream_t s) {
     const dim3 grid((unsigned)(p.np * p.nl), (unsigned)splits);
     if (bp == 64) {
-        if constexpr (KT) product_kernel<4, 1, 1, 8, true, OUT, TERMS><<<grid, dim3(256), 0, s>>>(p);
+        if constexpr (KT || (OUT == CT_F32 && TERMS != 2))
+            product_kernel<4, 1, 1, 8, KT, OUT, TERMS><<<grid, dim3(256), 0, s>>>(p);
     } else if (bp == 128) {
         if constexpr (!KT || TERMS < 3) product_kernel<8, 1, 1, 16, KT, OUT, TERMS><<<grid, dim3(512), 0, s>>>(p);
     } else {
@@ -1307,6 +1414,43 @@ LogitsParams logits_params(const ct_head_loss *a, const Plan &pl, const Kept &k,
     p.entries = (int)pl.entries;
     p.units = pl.units;
     return p;
+}
+
+// The logits of the whole vocabulary in memory, in chunks of their reduction, and the row pass's operands.
+hipError_t logits_in_memory(const Plan &pl, const LogitsParams &p, void *ws, const Scratch &sc, RowParams &r, hipStream_t s) {
+    ProductParams g{};
+    g.b = p.head;
+    g.ld = p.ld;
+    g.depth = p.width;
+    g.cols = pl.vocab;
+    g.packed = p.packed;
+    g.blocks = p.blocks;
+    g.b_apart = p.head_apart;
+    g.packed_apart = p.packed_apart;
+    g.np = p.np;
+    g.nl = cdiv(pl.vocab, pl.bl);
+    g.rows = pl.rows;
+    g.out = at<float>(ws, sc.logits);
+    g.ldo = pl.vocab;
+    g.slab = pl.rows * pl.vocab;
+    g.steps = (int)cdiv(p.width, kStep);
+    g.steps_per_split = (int)cdiv(g.steps, pl.chunks);
+    g.vec = pl.vocab % 4 == 0;
+    r.logits = at<float>(ws, sc.logits);
+    r.chunks = pl.chunks;
+    r.slab = g.slab;
+    r.rows = pl.rows;
+    r.vocab = pl.vocab;
+    r.scale = p.scale;
+    r.index = p.index;
+    r.first = p.first;
+    r.chosen = p.chosen;
+    r.entries = p.entries;
+    r.units = p.units;
+    r.piece = p.piece;
+    r.piece_blocks = p.piece_blocks;
+    r.piece_apart = p.piece_apart;
+    return launch_product<CT_F32>(pl.bp, pl.tri ? 3 : 1, g, pl.chunks, s);
 }
 
 hipError_t pack_hidden(const ct_head_loss *a, const Plan &pl, void *packed, hipStream_t stream) {
@@ -1413,10 +1557,23 @@ extern "C" int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t 
         const int64_t cols = pl.vocab - v0 < piece ? pl.vocab - v0 : piece;
         CT_TRY(head_piece(a, pl, p, v0, cols, at<void>(workspace, sc.split), stream));
         p.piece_blocks = pl.piece / 32;
-        CT_TRY(hidden_grad ? launch_logits<EXP>(pl, p, stream) : launch_logits<STATS>(pl, p, stream));
-        join_kernel<<<dim3((unsigned)(pl.rows_pad / 16)), dim3(1024), 0, stream>>>(
-            p.stats, (int)cdiv(cols, kUnit), pl.rows_pad, shift, total, factor, hidden_grad ? p.piece : nullptr,
-            p.piece_blocks, pl.terms[hidden_grad ? 1 : 0], p.piece_apart);
+        if (pl.chunks > 1) {
+            RowParams r{};
+            CT_TRY(logits_in_memory(pl, p, workspace, sc, r, stream));
+            r.shift = shift;
+            r.total = total;
+            const dim3 grid((unsigned)pl.rows);
+            const int terms = hidden_grad ? pl.terms[1] : 0;
+            if (terms == 0) rows_exp<0><<<grid, dim3(256), 0, stream>>>(r);
+            else if (terms == 1) rows_exp<1><<<grid, dim3(256), 0, stream>>>(r);
+            else if (terms == 2) rows_exp<2><<<grid, dim3(256), 0, stream>>>(r);
+            else rows_exp<3><<<grid, dim3(256), 0, stream>>>(r);
+        } else {
+            CT_TRY(hidden_grad ? launch_logits<EXP>(pl, p, stream) : launch_logits<STATS>(pl, p, stream));
+            join_kernel<<<dim3((unsigned)(pl.rows_pad / 16)), dim3(1024), 0, stream>>>(
+                p.stats, (int)cdiv(cols, kUnit), pl.rows_pad, shift, total, factor, hidden_grad ? p.piece : nullptr,
+                p.piece_blocks, pl.terms[hidden_grad ? 1 : 0], p.piece_apart);
+        }
         CT_TRY(hipGetLastError());
         if (!hidden_grad) continue;
         ProductParams g{};
@@ -1533,7 +1690,20 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
     for (int64_t v0 = 0; v0 < pl.vocab; v0 += pl.piece) {
         const int64_t cols = pl.vocab - v0 < pl.piece ? pl.vocab - v0 : pl.piece;
         CT_TRY(head_piece(a, pl, p, v0, cols, at<void>(workspace, sc.split), stream));
-        CT_TRY(launch_logits<GRAD>(pl, p, stream));
+        if (pl.chunks > 1) {
+            RowParams r{};
+            CT_TRY(logits_in_memory(pl, p, workspace, sc, r, stream));
+            r.near = near;
+            r.factor = factor;
+            r.inverse = inverse;
+            const dim3 grid((unsigned)pl.rows_pad);
+            if (pl.terms[2] == 1) rows_grad<1><<<grid, dim3(256), 0, stream>>>(r);
+            else if (pl.terms[2] == 2) rows_grad<2><<<grid, dim3(256), 0, stream>>>(r);
+            else rows_grad<3><<<grid, dim3(256), 0, stream>>>(r);
+            CT_TRY(hipGetLastError());
+        } else {
+            CT_TRY(launch_logits<GRAD>(pl, p, stream));
+        }
         ProductParams g{};
         g.b = static_cast<const uint16_t *>(hidden);
         g.ld = ld;

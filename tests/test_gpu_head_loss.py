@@ -61,7 +61,9 @@ def _streamed(hidden, head, labels, weights, dtype, **kw):
 
 
 SIZES = [(1, 64, 1), (1, 8, 2), (1, 512, 4099), (2, 72, 127), (17, 64, 128), (63, 200, 129), (64, 128, 1000),
-         (65, 64, 255), (128, 136, 257), (129, 256, 513), (255, 64, 1025), (257, 512, 4099), (600, 320, 777)]
+         (65, 64, 255), (128, 136, 257), (129, 256, 513), (255, 64, 1025), (257, 512, 4099), (600, 320, 777),
+         # wide rows and few entries: the logits' reduction in chunks
+         (1, 4096, 300), (18, 2056, 328), (70, 1032, 129), (140, 2048, 500), (300, 1031, 1000), (700, 520, 64)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -82,7 +84,7 @@ def test_widths_that_fill_no_vector(width, dtype):
 @pytest.mark.parametrize("normalizer", [False, True])
 @pytest.mark.parametrize("rows,width,vocab,entries,temperature", [
     (1, 64, 300, 1, 1.0), (3, 64, 17, 40, 2.0), (33, 72, 1000, 8, 0.5), (100, 128, 4099, 64, 2.0), (130, 64, 513, 65, 4.0),
-    (300, 256, 2050, 128, 1.0), (20, 64, 5000, 1024, 1.0)])
+    (300, 256, 2050, 128, 1.0), (20, 64, 5000, 1024, 1.0), (33, 1024, 700, 30, 2.0), (260, 777, 90, 100, 0.5)])
 def test_teacher(rows, width, vocab, entries, temperature, normalizer, dtype):
     from causal_tuner.kernels.loss import distillation_loss
     hidden, head, _, weights = _inputs(rows, width, vocab, dtype)
