@@ -180,9 +180,8 @@ Scratch scratch_of(const Plan &p, int sweep) {
     s.packed = r.take(p.rows_pad * p.width_pad * terms);
     s.plain = r.take(sweep == 2 ? p.rows * p.width * (p.tri ? 4 : 2) : 0);
     s.piece = r.take(sweep ? p.rows_pad * p.piece * 2 * p.terms[sweep] : 0);
-    s.turned = r.take(sweep == 0 ? 0 : p.turned ? p.width * terms * (sweep == 1 ? p.piece : steps)
-                                                : p.tri && sweep == 2 ? p.rows * pitch * terms : 0);
-    s.split = r.take(p.tri ? p.piece * pitch * terms : 0);
+    s.turned = r.take(sweep && p.turned ? p.width * terms * (sweep == 1 ? p.piece : steps) : 0);
+    s.split = r.take(p.tri && p.turned ? p.piece * pitch * terms : 0);
     s.logits = r.take(p.chunks > 1 ? p.chunks * p.rows * p.vocab * 4 : 0);
     s.stats = r.take(sweep == 2 || p.chunks > 1 ? 0 : piece / kUnit * p.rows_pad * 8);
     s.factor = r.take(p.rows_pad * 4);
@@ -562,14 +561,20 @@ __device__ __forceinline__ void tile_of(int64_t id, int64_t np, int64_t nl, int6
 // TERMS 3 (TRI): float32 operands as three bf16 terms each (split3). The reduction runs over six products of
 // the terms, the small ones first; the three left out are below 2^-26 of the whole, and every
 // product of two terms is exact in float32. Six bf16 products are faster than one float32 product
-// on this card's matrix units (v_mfma_f32_16x16x4_f32, a sixteenth of the bf16 rate).
+// on this card's matrix units (v_mfma_f32_16x16x4_f32, a sixteenth of the bf16 rate). The packed
+// operand's terms, and on the wide tiles the staged one's, lie in memory one after the other (TRI, six
+// passes over the reduction); the narrow tile, for few rows, which reading the staged operand bounds,
+// takes it as float32, splits it on the way to LDS and makes the six products of a step together
+// (FUSED: 3 rows x 60000 x 2000 1.70 ms with the terms in memory).
 template <int WP, int WL, int PF, int LF, bool KT, bool SWAP, int TERMS = 1>
 struct Core {
-    static constexpr bool TRI = TERMS == 3;
-    static constexpr int KS = TERMS == 2 ? 4 : 2;   // packed fragments of a step
+    static constexpr bool FUSED = TERMS == 3 && PF == 1 && LF == 8, TRI = TERMS == 3 && !FUSED;
+    static constexpr int KS = TERMS == 2 ? 4 : FUSED ? 6 : 2;   // packed fragments of a step
+    static constexpr int ES = FUSED ? 4 : 2, ST = FUSED ? 3 : 1;   // bytes of a staged value, terms in LDS
     static constexpr int BP = WP * PF * 16, BL = WL * LF * 16, THREADS = 64 * WP * WL;
-    static constexpr int kPer = BL * 8 / THREADS;   // 16-byte units of a stage per thread
-    static constexpr int kStage = BL * 8;           // units per stage
+    static constexpr int kPer = BL * 8 / THREADS;   // units (8 values) of a stage per thread
+    static constexpr int kRaw = kPer * ES / 2;      // 16-byte loads of them
+    static constexpr int kTerm = BL * 8, kStage = kTerm * ST;   // 16-byte units in LDS
     static constexpr int kRows = KT ? THREADS / (BL / 8) : THREADS / 8;   // rows between a thread's units
     static_assert(kRows % 16 == 0, "a thread's units differ by immediate offsets");
 
@@ -586,27 +591,28 @@ struct Core {
 
     // first: the staged operand at the tile's first row (KC) or column (KT); `extent` its rows from
     // there (KC) or columns (KT), `depth` the reduction's extent.
-    __device__ __forceinline__ void init(const uint16_t *first, int64_t ld, int64_t extent, int64_t depth,
+    __device__ __forceinline__ void init(const void *first, int64_t ld, int64_t extent, int64_t depth,
                                          const uint4 *packed, int64_t block, int64_t blocks, int wave) {
         const int tid = threadIdx.x, lane = tid & 63, wp = wave % WP, wl = wave / WP;
-        base = reinterpret_cast<const char *>(first);
+        base = static_cast<const char *>(first);
         limit = (int)depth;
         steps = (int)cdiv(depth, kStep);
-        pitch = (uint32_t)(kRows * ld * 2);
+        pitch = (uint32_t)(kRows * ld * ES);
         if constexpr (KT) {
             const int row = tid / (BL / 8), chunk = tid % (BL / 8), j = lane & 15, from = 4 * (lane >> 4) + (j >> 2);
-            bytes = ((depth - 1) * ld + (extent < BL ? up(extent, 8) : BL)) * 2;   // rows are whole units
-            advance = kStep * ld * 2;
-            off = chunk * 8 < extent ? (uint32_t)((row * ld + chunk * 8) * 2) : kOOB;
+            // bf16 rows are whole units
+            bytes = ((depth - 1) * ld + (extent < BL ? FUSED ? extent : up(extent, 8) : BL)) * ES;
+            advance = kStep * ld * ES;
+            off = chunk * 8 < extent ? (uint32_t)((row * ld + chunk * 8) * ES) : kOOB;
             k = 0;
             store_at = row * (BL / 8) + ((chunk >> 1 ^ (row & 7)) << 1 | (chunk & 1));
             read_at = from * (BL * 2) + ((wl * LF ^ (from & 7)) << 5) + ((j & 3) << 3);
         } else {
             const int row = tid >> 3, chunk = tid & 7;
-            // rows are whole units; those past the extent lie behind the last
-            bytes = (((extent < BL ? extent : BL) - 1) * ld + up(depth, 8)) * 2;
-            advance = kStep * 2;
-            off = (uint32_t)((row * ld + chunk * 8) * 2);
+            // bf16 rows are whole units; rows past the extent lie behind the last
+            bytes = (((extent < BL ? extent : BL) - 1) * ld + (FUSED ? depth : up(depth, 8))) * ES;
+            advance = kStep * ES;
+            off = (uint32_t)((row * ld + chunk * 8) * ES);
             k = chunk * 8;
             store_at = slot(row, chunk);
             read_at = slot(wl * LF * 16 + (lane & 15), lane >> 4);
@@ -631,13 +637,19 @@ struct Core {
     }
     // The thread's unit C of step t, its fragment I, and the unit's place in a stage.
     template <int C>
-    __device__ __forceinline__ void load_b(int t, uint4 (&r)[kPer]) const {
+    __device__ __forceinline__ void load_b(int t, uint4 (&r)[kRaw]) const {
         const char *from = base;
         int at = t;
         if constexpr (TRI) from += (0x124 >> 2 * product(t, at) & 3) * b_apart;
         // a descriptor per step: offsets stay within a step, whatever the operand's size
         const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(from + at * advance, t < steps ? bytes - at * advance : 0);
-        r[C] = buf_load16(rsrc, (KT || at * kStep + k < limit ? off : kOOB) + C * pitch);
+        const uint32_t to = (KT || at * kStep + k < limit ? off : kOOB) + C * pitch;
+        if constexpr (FUSED) {
+            r[2 * C] = buf_load16(rsrc, to);
+            r[2 * C + 1] = buf_load16(rsrc, to + 16);
+        } else {
+            r[C] = buf_load16(rsrc, to);
+        }
     }
     template <int I>
     __device__ __forceinline__ void load_a(int t, uint4 (&f)[KS][PF]) const {
@@ -647,45 +659,65 @@ struct Core {
         f[I % KS][I / KS] = from[(I % KS >> 1) * a_apart + (int64_t)at * 128 + I / KS * a_row + (I & 1) * 64];
     }
     template <int C>
-    __device__ __forceinline__ void store_b(uint4 *stage, const uint4 (&r)[kPer]) const {
-        stage[store_at + C * kRows * (KT ? BL / 8 : 8)] = r[C];
-    }
-    __device__ __forceinline__ void read(const uint4 *stage, int f, uint4 (&lf)[2]) const {
+    __device__ __forceinline__ void store_b(int t, uint4 *stage, const uint4 (&r)[kRaw]) const {
+        const int to = store_at + C * kRows * (KT ? BL / 8 : 8);
+        if constexpr (FUSED) {
+            const uint32_t w[8] = {r[2 * C].x, r[2 * C].y, r[2 * C].z, r[2 * C].w,
+                                   r[2 * C + 1].x, r[2 * C + 1].y, r[2 * C + 1].z, r[2 * C + 1].w};
+            float v[8];
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
+            for (int i = 0; i < 8; ++i)   // a row's last unit reaches into the next row
+                v[i] = KT || t * kStep + k + i < limit ? __builtin_bit_cast(float, w[i]) : 0.f;
+            uint4 terms[3];
+            split_unit<3>(v, terms);
+#pragma unroll
+            for (int s = 0; s < 3; ++s) stage[to + s * kTerm] = terms[s];
+        } else {
+            stage[to] = r[C];
+        }
+    }
+    __device__ __forceinline__ void read(const uint4 *stages, int f, uint4 (&lf)[2 * ST]) const {
+#pragma unroll
+        for (int i = 0; i < 2 * ST; ++i) {
+            const int ks = i & 1;
+            const uint4 *stage = stages + (i >> 1) * kTerm;
             if constexpr (KT) {
                 const __attribute__((address_space(3))) char *p =
                     (const __attribute__((address_space(3))) char *)stage + (read_at ^ (f & 7) << 5) + (f >> 3) * 256 + ks * 32 * (BL * 2);
                 const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)p);
                 const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)(p + 16 * (BL * 2)));
                 const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-                lf[ks] = make_uint4(l2.x, l2.y, h2.x, h2.y);
+                lf[i] = make_uint4(l2.x, l2.y, h2.x, h2.y);
             } else {
-                lf[ks] = stage[(read_at ^ ks << 2) + f * 128];
+                lf[i] = stage[(read_at ^ ks << 2) + f * 128];
             }
         }
     }
     template <int F>
     __device__ __forceinline__ void columns(int t, const uint4 *cur, const uint4 *nxt, uint4 *wr, const uint4 (&af)[KS][PF],
-                                            uint4 (&an)[KS][PF], uint4 (&b)[kPer], uint4 (&lf)[4][2],
+                                            uint4 (&an)[KS][PF], uint4 (&b)[kRaw], uint4 (&lf)[4][2 * ST],
                                             f32x4 (&acc)[LF][PF]) const {
         if constexpr (F < LF) {
             read(F + 3 < LF ? cur : nxt, (F + 3) % LF, lf[(F + 3) % 4]);
             if constexpr (F % (LF / 8) == 0 && F / (LF / 8) < KS * PF) load_a<F / (LF / 8)>(t + 2, an);
-            if constexpr (F % (LF / 4) == LF / 8 - 1) store_b<F / (LF / 4)>(wr, b);
+            if constexpr (F % (LF / 4) == LF / 8 - 1) store_b<F / (LF / 4)>(t + 2, wr, b);
             if constexpr (F % (LF / 4) == LF / 4 - 1) load_b<F / (LF / 4)>(t + 3, b);
+            // FUSED: of the packed operand the terms 2 1 0 1 0 0, of the staged one 0 1 2 0 1 0
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
+            for (int m = 0; m < (FUSED ? 12 : KS); ++m) {
+                const int x = FUSED ? (0x46 >> m / 2 * 2 & 3) * 2 + (m & 1) : m;
+                const int y = FUSED ? (0x124 >> m / 2 * 2 & 3) * 2 + (m & 1) : m & 1;
 #pragma unroll
                 for (int j = 0; j < PF; ++j)
-                    acc[F][j] = SWAP ? mfma16x16x32(lf[F % 4][ks & 1], af[ks][j], acc[F][j])
-                                     : mfma16x16x32(af[ks][j], lf[F % 4][ks & 1], acc[F][j]);
+                    acc[F][j] = SWAP ? mfma16x16x32(lf[F % 4][y], af[x][j], acc[F][j])
+                                     : mfma16x16x32(af[x][j], lf[F % 4][y], acc[F][j]);
+            }
             __builtin_amdgcn_sched_barrier(0);
             columns<F + 1>(t, cur, nxt, wr, af, an, b, lf, acc);
         }
     }
     __device__ __forceinline__ void step(int t, uint4 *stages, int &at, const uint4 (&af)[KS][PF], uint4 (&an)[KS][PF],
-                                         uint4 (&b)[kPer], uint4 (&lf)[4][2], f32x4 (&acc)[LF][PF]) const {
+                                         uint4 (&b)[kRaw], uint4 (&lf)[4][2 * ST], f32x4 (&acc)[LF][PF]) const {
         const int next = at == 2 * kStage ? 0 : at + kStage, after = next == 2 * kStage ? 0 : next + kStage;
         columns<0>(t, stages + at, stages + next, stages + after, af, an, b, lf, acc);
         static_assert(LF % 4 == 0, "the next step's first columns are in their places");
@@ -693,7 +725,7 @@ struct Core {
         __syncthreads();
     }
     template <int I>
-    __device__ __forceinline__ void first(uint4 *stages, uint4 (&b)[kPer], uint4 (&more)[kPer], uint4 (&af)[KS][PF], uint4 (&ag)[KS][PF]) const {
+    __device__ __forceinline__ void first(uint4 *stages, uint4 (&b)[kRaw], uint4 (&more)[kRaw], uint4 (&af)[KS][PF], uint4 (&ag)[KS][PF]) const {
         static_assert(kPer == 4 && KS * PF <= 8, "spread over the columns");
         if constexpr (I < 4) {
             load_b<I>(0, b);
@@ -701,8 +733,8 @@ struct Core {
         } else if constexpr (I < 12) {
             if constexpr (I - 4 < KS * PF) { load_a<I - 4>(0, af); load_a<I - 4>(1, ag); }
         } else if constexpr (I < 16) {
-            store_b<I - 12>(stages, b);
-            store_b<I - 12>(stages + kStage, more);
+            store_b<I - 12>(0, stages, b);
+            store_b<I - 12>(1, stages + kStage, more);
             load_b<I - 12>(2, b);
         }
         if constexpr (I < 15) first<I + 1>(stages, b, more, af, ag);
@@ -713,7 +745,7 @@ struct Core {
 #pragma unroll
             for (int j = 0; j < PF; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (steps <= 0) return;
-        uint4 b[kPer], more[kPer], a0[KS][PF], a1[KS][PF], a2[KS][PF], lf[4][2];
+        uint4 b[kRaw], more[kRaw], a0[KS][PF], a1[KS][PF], a2[KS][PF], lf[4][2 * ST];
         first<0>(stages, b, more, a0, a1);
         __syncthreads();
         read(stages, 0, lf[0]);
@@ -734,7 +766,7 @@ struct Core {
 enum { STATS = 0, EXP = 1, GRAD = 2 };
 
 struct LogitsParams {
-    const uint16_t *head;      // from v0 on
+    const void *head;          // from v0 on
     int64_t ld, width, vocab;
     int64_t head_apart, packed_apart, piece_apart;   // units between two terms
     const uint4 *packed;       // hidden rows
@@ -816,7 +848,7 @@ __global__ __launch_bounds__(64 * WP * WL) void logits_kernel(const LogitsParams
     uint32_t *wave_bits = reinterpret_cast<uint32_t *>(marks[wave]);
     mark_targets<PF * 16, UNITS>(p, row0, (v0 + wl * LF * 16) / kUnit, wave_bits, lane);
     C core;
-    core.init(p.head + (v0 - p.v0) * p.ld, p.ld, left, p.width, p.packed, tp * (C::BP / 16), p.blocks, wave);
+    core.init(static_cast<const char *>(p.head) + (v0 - p.v0) * p.ld * C::ES, p.ld, left, p.width, p.packed, tp * (C::BP / 16), p.blocks, wave);
     if constexpr (TRI) core.terms(p.head_apart, p.packed_apart);
     f32x4 acc[LF][PF];
     core.run(stages, acc);
@@ -991,7 +1023,7 @@ __global__ __launch_bounds__(1024) void join_kernel(const float2 *__restrict__ s
 
 // ------------------------------------------------------------------------- the second product
 struct ProductParams {
-    const uint16_t *b;         // KT: [depth, cols], else its transpose
+    const void *b;             // KT: [depth, cols], else its transpose
     int64_t ld, depth, cols;
     bool kt;
     const uint4 *packed;       // [rows, depth]
@@ -1020,7 +1052,7 @@ __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductPara
     C core;
     const int64_t k0 = (int64_t)beg * kStep;
     const int64_t depth = (end < p.steps ? (int64_t)end * kStep : p.depth) - k0;   // none: an empty split
-    core.init(p.b + (KT ? k0 * p.ld + tl * C::BL : tl * C::BL * p.ld + k0), p.ld, p.cols - tl * C::BL, depth,
+    core.init(static_cast<const char *>(p.b) + (KT ? k0 * p.ld + tl * C::BL : tl * C::BL * p.ld + k0) * C::ES, p.ld, p.cols - tl * C::BL, depth,
               p.packed + (int64_t)beg * 128, tp * (C::BP / 16), p.blocks, wave);
     if constexpr (TERMS > 1) core.terms(p.b_apart, p.packed_apart);
     f32x4 acc[LF][PF];
@@ -1394,8 +1426,8 @@ int check_sizes(int64_t count, int64_t width, int64_t vocab, int32_t entries, in
 
 LogitsParams logits_params(const ct_head_loss *a, const Plan &pl, const Kept &k, const Scratch &sc, void *kept, void *ws) {
     LogitsParams p{};
-    p.ld = pl.tri ? up(pl.width, 8) : a->ld_head;
-    p.width = up(pl.width, 8);
+    p.ld = pl.tri && pl.turned ? up(pl.width, 8) : a->ld_head;
+    p.width = pl.tri && !pl.turned ? pl.width : up(pl.width, 8);
     p.head_apart = pl.piece * p.ld / 8;
     p.packed_apart = pl.rows_pad * pl.width_pad / 8;
     p.piece_apart = pl.rows_pad * pl.piece / 8;
@@ -1475,18 +1507,18 @@ hipError_t split_terms(const float *x, int64_t ld, int64_t rows, int64_t cols, u
     else split_rows<false><<<grid, dim3(256), 0, s>>>(x, ld, rows, cols, out, pitch, apart);
     return hipGetLastError();
 }
-// The piece of the head that starts at entry v0, as the logits kernel stages it: in place, or float32
-// rows in their three terms.
+// The piece of the head that starts at entry v0, as the logits kernel stages it: in place, or on the
+// wide tiles float32 rows in their three terms.
 hipError_t head_piece(const ct_head_loss *a, const Plan &pl, LogitsParams &p, int64_t v0, int64_t cols, void *split,
                       hipStream_t stream) {
     p.v0 = v0;
     p.v1 = v0 + cols;
     p.nl = cdiv(cols, pl.bl);
-    if (!pl.tri) {
-        p.head = static_cast<const uint16_t *>(a->head) + v0 * a->ld_head;
+    if (!pl.tri || !pl.turned) {
+        p.head = static_cast<const char *>(a->head) + v0 * a->ld_head * (pl.tri ? 4 : 2);
         return hipSuccess;
     }
-    p.head = static_cast<const uint16_t *>(split);
+    p.head = split;
     return split_terms(static_cast<const float *>(a->head) + v0 * a->ld_head, a->ld_head, cols, pl.width,
                        static_cast<uint4 *>(split), p.ld, p.head_apart, stream);
 }
@@ -1672,14 +1704,6 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
     p.inverse = inverse;
     p.piece_blocks = pl.rows_pad / 32;
     int64_t apart = 0;
-    if (pl.tri && !pl.turned) {
-        uint4 *terms = at<uint4>(workspace, sc.turned);
-        const int64_t pitch = up(pl.width, 8);
-        apart = pl.rows * pitch / 8;
-        CT_TRY(split_terms(static_cast<const float *>(hidden), ld, pl.rows, pl.width, terms, pitch, apart, stream));
-        hidden = terms;
-        ld = pitch;
-    }
     if (pl.turned) {
         uint16_t *turned = at<uint16_t>(workspace, sc.turned);
         apart = pl.width * up(pl.rows, kStep) / 8;
@@ -1705,7 +1729,7 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
             CT_TRY(launch_logits<GRAD>(pl, p, stream));
         }
         ProductParams g{};
-        g.b = static_cast<const uint16_t *>(hidden);
+        g.b = hidden;
         g.ld = ld;
         g.kt = !pl.turned;
         g.b_apart = apart;
