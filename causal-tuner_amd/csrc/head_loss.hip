@@ -34,6 +34,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "gemm_common.hpp"
 
 namespace ct {
@@ -135,7 +137,7 @@ Plan plan_of(int64_t rows, int64_t width, int64_t vocab, int64_t entries, int dt
     p.piece = piece_for(cdiv(vocab, 256), most / 256, p.rows_pad / p.bp * (p.bp == 64 ? 2 : 1), p.bp == 64 ? 512 : 256) * 256;
     p.turned = p.tri ? p.bp > 64 : p.bp == 256;
     const int64_t tiles = p.rows_pad / p.bp * cdiv(width, p.bl);
-    p.splits = splits_for(tiles, p.bp == 64 ? 512 : 256, p.piece / kStep);
+    p.splits = splits_for(tiles, p.bp == 64 && !p.tri ? 512 : 256, p.piece / kStep);
     p.chunks = chunks_for(p.rows_pad / p.bp * cdiv(vocab, p.bl), p.width_pad / kStep);
     return p;
 }
@@ -1260,10 +1262,12 @@ __global__ __launch_bounds__(256) void row_factors(const float *__restrict__ wei
     factor[row] = row < rows && mass[row] != 0.f ? f * mass[row] / z : 0.f;
 }
 
-// dh_i = u c_i / T (Q_i / Z_i sums_i + sum_k coefficient_k w_v_k). A workgroup takes a row and 512
-// columns; its four waves share the splits' sums and the targets, every fourth each, and are joined
-// in order. Bound by the targets' rows of the head: K x width per row of the loss, from the caches.
-template <int IN, int OUT, bool VEC>
+// dh_i = u c_i / T (Q_i / Z_i sums_i + sum_k coefficient_k w_v_k). A wave takes a row and 512 columns,
+// four waves of a workgroup 2048; where there are many splits or targets (SHARE) the four take the
+// same 512 columns, every fourth split and target each, and are joined in order. Bound by the sums and
+// by the targets' rows of the head, K x width per row of the loss, from the caches (8192 rows of 64 x
+// 2048: 255 us, 8.4 TB/s).
+template <int IN, int OUT, bool VEC, bool SHARE>
 __global__ __launch_bounds__(256) void hidden_grad_kernel(const float *__restrict__ sums, int splits, int64_t slab,
                                                           int64_t width, const float *__restrict__ weight,
                                                           const float *__restrict__ mass, const float *__restrict__ total,
@@ -1272,17 +1276,19 @@ __global__ __launch_bounds__(256) void hidden_grad_kernel(const float *__restric
                                                           const float *__restrict__ coefficient, int entries,
                                                           const void *__restrict__ head, int64_t ld,
                                                           const int64_t *__restrict__ rows, int64_t tokens,
-                                                          void *__restrict__ out, int64_t ldo, int64_t out_width) {
-    __shared__ float lds[4][512];
+                                                          void *__restrict__ out, int64_t ldo, int64_t out_width, int whole) {
+    __shared__ float lds[SHARE ? 4 : 1][512];
     const int64_t row = blockIdx.x, to = rows ? rows[row] : row;
     if (to < 0 || to >= tokens) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const float held = mass[row], f = weight[row] * *upstream * inverse_t;
     const float by = held != 0.f ? held / total[row] : 0.f;
-    const int64_t c0 = (int64_t)blockIdx.y * 512 + lane * 8;
+    const int64_t c0 = ((int64_t)blockIdx.y * (SHARE ? 1 : 4) + (SHARE ? 0 : wave)) * 512 + lane * 8;
+    constexpr int STEP = SHARE ? 4 : 1;
+    const int start = SHARE ? wave : 0;
     const auto in = [&](int i) { return VEC ? c0 < width : c0 + i < width; };
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s = wave; s < splits; s += 4) {
+    for (int s = start; s < splits; s += STEP) {
         const float *p = sums + s * slab + row * width + c0;
         if constexpr (VEC) {
             if (in(0)) {
@@ -1300,7 +1306,7 @@ __global__ __launch_bounds__(256) void hidden_grad_kernel(const float *__restric
     const int *at = index + row * entries;
     const float *k = coefficient + row * entries;
 #pragma unroll 8
-    for (int e = wave; e < entries; e += 4) {
+    for (int e = start; e < entries; e += STEP) {
         const int vocab = at[e];
         if (vocab == kNoEntry) continue;
         const float by_k = k[e];
@@ -1317,15 +1323,33 @@ __global__ __launch_bounds__(256) void hidden_grad_kernel(const float *__restric
                 v[i] += by_k * bf16_to_f32((uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu));
         }
     }
+    if constexpr (!SHARE) {
+        float o[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) lds[wave][lane * 8 + i] = v[i];
-    __syncthreads();
-    for (int c = threadIdx.x; c < 512; c += 256) {
-        const int64_t col = (int64_t)blockIdx.y * 512 + c;
-        if (col >= out_width) break;
-        const float sum = held != 0.f ? (lds[0][c] + lds[1][c] + lds[2][c] + lds[3][c]) * f : 0.f;
-        if constexpr (OUT == CT_F32) static_cast<float *>(out)[to * ldo + col] = sum;
-        else static_cast<uint16_t *>(out)[to * ldo + col] = bf16_bits(sum);
+        for (int i = 0; i < 8; ++i) o[i] = held != 0.f ? v[i] * f : 0.f;
+        if (OUT == CT_BF16 && whole && c0 + 8 <= out_width) {
+            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out) + to * ldo + c0) = make_uint4(
+                pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (c0 + i >= out_width) continue;
+            if constexpr (OUT == CT_F32) static_cast<float *>(out)[to * ldo + c0 + i] = o[i];
+            else static_cast<uint16_t *>(out)[to * ldo + c0 + i] = bf16_bits(o[i]);
+        }
+        return;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) lds[wave][lane * 8 + i] = v[i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < 512; c += 256) {
+            const int64_t col = (int64_t)blockIdx.y * 512 + c;
+            if (col >= out_width) break;
+            const float sum = held != 0.f ? (lds[0][c] + lds[1][c] + lds[2][c] + lds[3][c]) * f : 0.f;
+            if constexpr (OUT == CT_F32) static_cast<float *>(out)[to * ldo + col] = sum;
+            else static_cast<uint16_t *>(out)[to * ldo + col] = bf16_bits(sum);
+        }
     }
 }
 
@@ -1662,24 +1686,27 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
         if (!hidden_grad) return -CT_EINVAL_WORKSPACE;
         if (d_hidden_dtype != CT_F32 && d_hidden_dtype != CT_BF16) return -CT_EINVAL_DTYPE;
         if (d_hidden_width < 0 || d_hidden_width > pl.width || ld_d_hidden < d_hidden_width) return -CT_EINVAL_SHAPE;
+        const bool share = pl.splits + pl.entries > 4, vec = pl.width % 8 == 0;
+        const int whole = ld_d_hidden % 8 == 0 && reinterpret_cast<uintptr_t>(d_hidden) % 16 == 0;
         const auto run = [&](auto kernel) {
-            kernel<<<dim3((unsigned)pl.rows, (unsigned)cdiv(d_hidden_width, 512)), dim3(256), 0, stream>>>(
+            kernel<<<dim3((unsigned)pl.rows, (unsigned)cdiv(d_hidden_width, share ? 512 : 2048)), dim3(256), 0, stream>>>(
                 at<const float>(kept, k.sums), pl.splits, pl.rows * pl.width, pl.width, at<const float>(kept, k.weight),
                 at<const float>(kept, k.mass), at<const float>(kept, k.total), upstream, inverse_t,
-                at<const int>(kept, k.index), at<const float>(kept, k.chosen), (int)pl.entries, a->head, a->ld_head, a->rows, a->tokens,
-                d_hidden, ld_d_hidden, d_hidden_width);
+                at<const int>(kept, k.index), at<const float>(kept, k.chosen), (int)pl.entries, a->head, a->ld_head, a->rows,
+                a->tokens, d_hidden, ld_d_hidden, d_hidden_width, whole);
         };
-        const bool vec = pl.width % 8 == 0;
-        if (pl.dtype == CT_BF16) {
-            if (d_hidden_dtype == CT_F32) run(hidden_grad_kernel<CT_BF16, CT_F32, true>);
-            else run(hidden_grad_kernel<CT_BF16, CT_BF16, true>);
-        } else if (d_hidden_dtype == CT_F32) {
-            if (vec) run(hidden_grad_kernel<CT_F32, CT_F32, true>);
-            else run(hidden_grad_kernel<CT_F32, CT_F32, false>);
-        } else {
-            if (vec) run(hidden_grad_kernel<CT_F32, CT_BF16, true>);
-            else run(hidden_grad_kernel<CT_F32, CT_BF16, false>);
-        }
+        const auto pick = [&](auto in, auto out, auto wide) {
+            if (share) run(hidden_grad_kernel<decltype(in)::value, decltype(out)::value, decltype(wide)::value, true>);
+            else run(hidden_grad_kernel<decltype(in)::value, decltype(out)::value, decltype(wide)::value, false>);
+        };
+        const std::integral_constant<int, CT_F32> f32;
+        const std::integral_constant<int, CT_BF16> bf16;
+        const std::true_type yes;
+        const std::false_type no;
+        const bool narrow = d_hidden_dtype == CT_BF16;
+        if (pl.dtype == CT_BF16) narrow ? pick(bf16, bf16, yes) : pick(bf16, f32, yes);   // widths of whole units
+        else if (vec) narrow ? pick(f32, bf16, yes) : pick(f32, f32, yes);
+        else narrow ? pick(f32, bf16, no) : pick(f32, f32, no);
         CT_TRY(hipGetLastError());
     }
     if (!d_head) return 0;
