@@ -18,7 +18,8 @@ from .loss import row_count
 _MAX_PITCH = 1 << 20     # elements between two rows
 _MAX_WIDTH = 1 << 16
 _MAX_VOCAB = (1 << 31) - 1024
-_MAX_ROWS = 1 << 30
+_MAX_ROWS = (1 << 24) - 256
+_MAX_VALUES = (1 << 35) - 256    # of the padded rows
 
 
 def _rows_of(selection, tokens, device):
@@ -71,6 +72,9 @@ class StreamedHeadLoss(torch.autograd.Function):
         first, rows, count = _rows_of(selection, tokens, device)
         indices, values, normalizer, weights = tables
         entries, (vocab, width) = indices.shape[1], matrix.shape
+        if count > _MAX_ROWS or (count + 255) // 256 * 256 * ((width + 63) // 64 * 64) > _MAX_VALUES:
+            raise ValueError(f"streamed head loss: {count} rows of {width} values; the HIP kernels take up to {_MAX_ROWS} rows "
+                             f"and {_MAX_VALUES} values at once")
         skip = first * entries
         ld, code = h.stride(0), _native.dtype_code(compute_dtype)
         call = _native.HeadLoss(
@@ -146,9 +150,9 @@ def streamed_loss(hidden, head, weights, selection, compute_dtype, indices, valu
     """The loss of device tensors: hard labels `indices` [tokens, 1], or a teacher's entries."""
     if compute_dtype not in (torch.bfloat16, torch.float32):
         raise NotImplementedError("streamed head loss: the HIP kernels compute in bfloat16 or float32")
-    if head.shape[1] > _MAX_WIDTH or len(head) > _MAX_VOCAB or weights.numel() > _MAX_ROWS:
-        raise ValueError(f"streamed head loss: {weights.numel()} rows, head {tuple(head.shape)}; the HIP kernels take up to "
-                         f"{_MAX_ROWS} rows, {_MAX_VOCAB} entries and a width of {_MAX_WIDTH}")
+    if head.shape[1] > _MAX_WIDTH or len(head) > _MAX_VOCAB:
+        raise ValueError(f"streamed head loss: head {tuple(head.shape)}; the HIP kernels take up to {_MAX_VOCAB} entries and "
+                         f"a width of {_MAX_WIDTH}")
     _native.refuse_tangents("streamed head loss", hidden, head)
     device = hidden.device
     wide = lambda t: None if t is None else t.to(device, torch.float32).contiguous()  # noqa: E731

@@ -61,7 +61,7 @@ def projection_loss(hidden, head, targets, weights, *, token_budget=128, compute
     (`head_loss_cuda`): no logits are held, so `token_budget` plays no part; the statistics and
     the loss come from unrounded float32 logits, and every gradient is rounded once, after the
     upstream scale. bf16 and float32; `reuse_hidden` belongs to the fused path. With `rows` given
-    it can be captured into a graph."""
+    it can be captured into a graph. `rows` names each row at most once, counted from 0, in any order."""
     if token_budget <= 0:
         raise ValueError("loss_token_budget must be positive")
     selection = active_rows(weights, hidden.device) if rows is None else rows

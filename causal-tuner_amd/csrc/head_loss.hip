@@ -49,7 +49,9 @@ constexpr int kMaxEntries = 1024;
 // that a row has would show in the gradients of few rows; of many rows they average.
 constexpr int64_t kTwoTerms = 128;
 constexpr int64_t kMaxPitch = 1 << 20;   // a tile's offsets stay below 2^31
-constexpr int64_t kMaxWidth = 65536, kMaxVocab = (int64_t{1} << 31) - 1024, kMaxRows = int64_t{1} << 30;
+// A launch holds fewer than 2^32 threads: 256 per row, one per eight values of the padded rows.
+constexpr int64_t kMaxWidth = 65536, kMaxVocab = (int64_t{1} << 31) - 1024, kMaxRows = (int64_t{1} << 24) - 256;
+constexpr int64_t kMaxValues = (int64_t{1} << 35) - 256;
 // Values of one piece, in bytes, whatever the batch and the vocabulary. Larger pieces read and write the
 // float32 sums less often (16384 tokens, of 49152 entries: 128 MB 6.25 ms, 256 MB 5.75, 512 MB 5.54, 1 GB
 // 5.47), smaller ones stay in the 256 MB last-level cache, which pays for less than that.
@@ -142,6 +144,13 @@ Plan plan_of(int64_t rows, int64_t width, int64_t vocab, int64_t entries, int dt
     return p;
 }
 
+// Entries per piece of a sweep. Statistics alone: bounded by the pairs per row and unit.
+int64_t sweep_piece(const Plan &p, int sweep) {
+    if (sweep || p.tri) return p.piece;
+    const int64_t all = up(p.vocab, 2 * kUnit), most = kPieceBytes / (p.rows_pad * 8) / 2 * 2 * kUnit;
+    return all < most ? all : most;
+}
+
 // What a call keeps for its backward, and its scratch: regions of one buffer each.
 struct Regions {
     int64_t at = 0;
@@ -178,7 +187,7 @@ Scratch scratch_of(const Plan &p, int sweep) {
     Regions r;
     Scratch s{};
     const int64_t terms = p.tri ? 6 : 2, pitch = up(p.width, 8), steps = up(p.rows, kStep);
-    const int64_t piece = sweep || p.tri ? p.piece : up(p.units, 2) * kUnit;
+    const int64_t piece = sweep_piece(p, sweep);
     s.packed = r.take(p.rows_pad * p.width_pad * terms);
     s.plain = r.take(sweep == 2 ? p.rows * p.width * (p.tri ? 4 : 2) : 0);
     s.piece = r.take(sweep ? p.rows_pad * p.piece * 2 * p.terms[sweep] : 0);
@@ -1422,6 +1431,7 @@ int check(const ct_head_loss *a, bool hidden, bool forward) {
         return -CT_EINVAL_SHAPE;
     if (forward && !a->values && a->entries != 1) return -CT_EINVAL_SHAPE;
     if (forward && (a->ld_indices < a->entries || (a->values && a->ld_values < a->entries))) return -CT_EINVAL_SHAPE;
+    if (up(a->count, 256) * up(a->width, kStep) > kMaxValues) return -CT_EINVAL_SHAPE;
     if (!(a->temperature > 0)) return -CT_EINVAL_SHAPE;
     if (a->count && ((hidden && !a->hidden) || !a->head)) return -CT_EINVAL_POINTER;
     if (a->count && forward && (!a->indices || !a->weights)) return -CT_EINVAL_POINTER;
@@ -1438,7 +1448,7 @@ bool in_place(const ct_head_loss *a) {
 int check_sizes(int64_t count, int64_t width, int64_t vocab, int32_t entries, int32_t dtype) {
     if (dtype != CT_BF16 && dtype != CT_F32) return -CT_EINVAL_DTYPE;
     return count < 0 || count > kMaxRows || width <= 0 || width > kMaxWidth || vocab <= 0 || vocab > kMaxVocab ||
-                   entries < 1 || entries > kMaxEntries
+                   entries < 1 || entries > kMaxEntries || up(count, 256) * up(width, kStep) > kMaxValues
                ? -CT_EINVAL_SHAPE
                : 0;
 }
@@ -1608,7 +1618,7 @@ extern "C" int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t 
 
     CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), stream));
     LogitsParams p = logits_params(a, pl, k, sc, kept, workspace);
-    const int64_t piece = hidden_grad || pl.tri ? pl.piece : pl.vocab;
+    const int64_t piece = sweep_piece(pl, hidden_grad ? 1 : 0);
     for (int64_t v0 = 0; v0 < pl.vocab; v0 += piece) {
         const int64_t cols = pl.vocab - v0 < piece ? pl.vocab - v0 : piece;
         CT_TRY(head_piece(a, pl, p, v0, cols, at<void>(workspace, sc.split), stream));

@@ -487,11 +487,18 @@ extern "C" int ct_layer_norm_forward(const void *x, int32_t x_dtype, const void 
     if (rows == 0) return 0;
     if (!x || !y || !mean != !rstd) return -CT_EINVAL_POINTER;
     const bool vec = aligned(x) && aligned(y) && aligned(w) && aligned(bias) && width % (x_dtype == CT_F32 ? 4 : 8) == 0;
-    const auto run = [&](auto launch) { return launch(x, w, bias, w_dtype, y, mean, rstd, rows, width, (float)eps, stream); };
-    hipError_t e;
-    if (x_dtype == CT_F32) e = vec ? run(launch_forward<CT_F32, 4>) : run(launch_forward<CT_F32, 1>);
-    else if (x_dtype == CT_BF16) e = vec ? run(launch_forward<CT_BF16, 8>) : run(launch_forward<CT_BF16, 1>);
-    else e = vec ? run(launch_forward<CT_F16, 8>) : run(launch_forward<CT_F16, 1>);
+    hipError_t e = hipSuccess;
+    // A launch holds fewer than 2^32 threads, 1024 a row at most.
+    for (int64_t row = 0, most = 1 << 21; row < rows && e == hipSuccess; row += most) {
+        const int64_t count = rows - row < most ? rows - row : most, at = row * width * (x_dtype == CT_F32 ? 4 : 2);
+        const auto run = [&](auto launch) {
+            return launch(static_cast<const char *>(x) + at, w, bias, w_dtype, static_cast<char *>(y) + at,
+                          mean ? mean + row : nullptr, rstd ? rstd + row : nullptr, count, width, (float)eps, stream);
+        };
+        if (x_dtype == CT_F32) e = vec ? run(launch_forward<CT_F32, 4>) : run(launch_forward<CT_F32, 1>);
+        else if (x_dtype == CT_BF16) e = vec ? run(launch_forward<CT_BF16, 8>) : run(launch_forward<CT_BF16, 1>);
+        else e = vec ? run(launch_forward<CT_F16, 8>) : run(launch_forward<CT_F16, 1>);
+    }
     return (int)e;
 }
 

@@ -370,6 +370,22 @@ def test_other_stream_and_captured_replays():
             assert all(torch.equal(a, b) for a, b in zip(out, want)), turn
 
 
+def test_statistics_alone_in_pieces():
+    """Without gradients: so many rows that the units' statistics come to more than one piece, against
+    the same rows in parts. A unit's sum is the same in both; joining 71 of them in two orders differs
+    by at most 2 x 71 x 2^-24 < 2^-16 of Z, of the losses' mean (log 9000 and more) by less than 2^-19,
+    and the nine losses are rounded by 2^-24 each."""
+    rows, width, vocab = 1 << 20, 64, 9000   # 71 units of 8 bytes a row
+    hidden, head, labels, weights = _inputs(rows, width, vocab, BF16)
+    with torch.no_grad():
+        weights = weights.abs() / rows
+        whole = _streamed(hidden, head, labels, weights, BF16).double()
+        step = rows // 8
+        parts = sum(_streamed(hidden, head, labels, weights, BF16, rows=slice(i, i + step)).double()
+                    for i in range(0, rows, step))
+    assert abs(whole - parts) <= (2.0 ** -19 + 2.0 ** -22) * parts.abs()
+
+
 def test_refusals():
     from causal_tuner.kernels.loss import distillation_loss
     hidden, head, labels, weights = _inputs(4, 16, 30, BF16)
@@ -381,6 +397,9 @@ def test_refusals():
         _streamed(hidden, head, labels.cpu(), weights, BF16)
     with pytest.raises(ValueError, match="indices"):
         distillation_loss(hidden, head, labels[:, None].cpu(), torch.zeros(4, 1), weights)
+    with pytest.raises(ValueError, match="at once"):
+        tall = torch.zeros(1, 16, device="cuda", dtype=BF16).expand(1 << 24, 16)
+        _streamed(tall, head, labels[:1].expand(1 << 24), weights[:1].expand(1 << 24), BF16, rows=slice(0, 1 << 24))
     with pytest.raises(ValueError, match="width"):
         _streamed(hidden.new_zeros(4, 65544), hidden.new_zeros(2, 65544), labels, weights, BF16)
     for rows in (torch.ones(4, dtype=torch.bool, device="cuda"), torch.zeros(2, 1, dtype=torch.int64, device="cuda"),

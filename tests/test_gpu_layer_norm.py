@@ -225,6 +225,22 @@ def test_module_and_gradient_against_differences():
         assert abs((up - down) / (2 * step) - grad[at].item()) < 48 * 3 * UNIT * 4 / step + 2 * step ** 2
 
 
+def test_more_rows_than_one_launch_holds():
+    """2^26 + 5 rows, whose statistics and values are those that the rows have by themselves."""
+    from causal_tuner.modeling.norm import layer_norm
+    rows, width = (1 << 26) + 5, 8
+    x = torch.randn(1 << 20, width, device="cuda", dtype=BF16).repeat(65, 1)[:rows].requires_grad_()
+    weight, bias = torch.randn(2, width, device="cuda")
+    y = layer_norm(x, weight, bias)
+    dy = y.detach().roll(1, -1)
+    dx, = torch.autograd.grad(y, x, dy)
+    for first in (0, (1 << 21) - 3, (1 << 25) - 1, (1 << 26) - 2, rows - 7):
+        part = x.detach()[first:first + 7].clone().requires_grad_()
+        want = layer_norm(part, weight, bias)
+        assert torch.equal(y[first:first + 7], want), first
+        assert torch.equal(dx[first:first + 7], torch.autograd.grad(want, part, dy[first:first + 7])[0]), first
+
+
 def test_refusals():
     from causal_tuner.modeling.norm import layer_norm
     x, weight, bias, dy = _inputs(4, 16, F32, F32)
