@@ -10,7 +10,7 @@
 //
 // A hard label is K = 1, q = 1, H = 0. The hidden gradient is attention with the head as keys and
 // values, so the forward makes it in the same sweep over the vocabulary, piece by piece: one
-// product writes E = 2^(l log2 e - c), rounded to the inputs' type, beside the sums of a running
+// product writes E = 2^(l log2 e - c), in one to three bf16 terms, beside the float32 sums of a running
 // softmax; the next adds E W_piece to a float32 accumulator per row; Z divides at the end. The
 // targets' own terms are left out of E and of the sums, and their coefficients Q p_k - q_k formed in
 // double from their logits and the others' sum: for a label of probability near one, 1 - p is not the
@@ -29,6 +29,13 @@
 //
 // float32. Operands are split into three bf16 terms, which hold them exactly, and take the same
 // kernels (Core, TRI).
+//
+// Bound by the matrix units from some 300 rows on: 4 rows vocab width operations with the hidden
+// gradient, 8 with the head's too (2 of them the logits again, the price of not holding them). In bf16,
+// 49152 entries x 2048: 16384 rows with the hidden gradient 5.4 ms, 1.22 PFLOP/s (a library product of
+// such sizes alone runs at 1.26 to 1.55); 4001 rows with both gradients 2.7 ms, 1.18 PFLOP/s (logits 689
+// and 695, products 593 and 639 us). Of few rows by a read of the head for each product, from HBM and
+// in part from the last-level cache: one row, 201 MB, logits 33 us, product 46.
 //
 // Every sum runs in a fixed order: repeated calls are bit-identical.
 
@@ -491,7 +498,8 @@ __global__ __launch_bounds__(256) void gather_rows(Source src, T *__restrict__ o
 
 // out [cols][pitch] = x [rows][cols] transposed, the indices inside each block of 32 rows in the
 // order of the second product (unit q: 4 q .. + 3, 16 + 4 q .. + 3), zeros past the rows. A workgroup
-// takes 64 x 64. float32: three bf16 arrays, `apart` units between them.
+// takes 64 x 64. Bound by the copy (49152 x 2048 bf16: 74 us, 5.4 TB/s), which of more than 128 rows costs less
+// than the product's transposing reads from LDS. float32: three bf16 arrays, `apart` units between them.
 template <class T>
 __global__ __launch_bounds__(256) void transpose_rows(const T *__restrict__ x, int64_t ld, int64_t rows, int64_t cols,
                                                       uint4 *__restrict__ out, int64_t pitch, int64_t apart) {
@@ -778,7 +786,7 @@ enum { STATS = 0, EXP = 1, GRAD = 2 };
 
 struct LogitsParams {
     const void *head;          // from v0 on
-    int64_t ld, width, vocab;
+    int64_t ld, width;
     int64_t head_apart, packed_apart, piece_apart;   // units between two terms
     const uint4 *packed;       // hidden rows
     int64_t blocks;            // of 32 along the width
@@ -843,6 +851,12 @@ __device__ __forceinline__ int64_t place_of(const LogitsParams &p, int64_t row, 
     return row * p.entries + n;
 }
 
+// A tile's logits from Core, and from the accumulators what MODE asks for, so that no logit reaches
+// memory: the units' statistics (STATS), with E (EXP), or the derivative (GRAD), E and derivative in the
+// order in which the product that follows takes them. The orientation follows from that order: a lane
+// holds four entries of a row (EXP), or four rows of an entry (GRAD). 4001 rows x 49152 x 2048: 689 us,
+// 1.17 PFLOP/s, of which a fifth to a quarter are the exponentials and the stores behind the product's last step, which
+// workgroups that stay resident and overlap them did not hide (3% slower).
 template <int WP, int WL, int PF, int LF, int MODE, int TERMS>
 __global__ __launch_bounds__(64 * WP * WL) void logits_kernel(const LogitsParams p) {
     constexpr bool TRI = TERMS == 3;
@@ -979,7 +993,8 @@ __global__ __launch_bounds__(64 * WP * WL) void logits_kernel(const LogitsParams
     }
 }
 
-// The units' statistics of a piece joined to the rows': 16 rows x 64 groups of units a workgroup.
+// The units' statistics of a piece joined to the rows': 16 rows x 64 groups of units a workgroup, in
+// order (one row, 384 units: 6 us).
 // A row's shift becomes the largest of its own and the units'; E of a unit with another shift is
 // brought to it, and `factor` is what the sums of the pieces before are brought to it with.
 __global__ __launch_bounds__(1024) void join_kernel(const float2 *__restrict__ stats, int units, int64_t rows_pad,
@@ -1048,7 +1063,11 @@ struct ProductParams {
     int vec;
 };
 
-// out[row, col] (= factor out +) sum_k packed(row, k) b(k, col), one split of the reduction per y.
+// out[row, col] (= factor out +) sum_k packed(row, k) b(k, col), one split of the reduction per y, each
+// with an output of its own. Splits fill the compute units where the tiles alone do not (splits_for);
+// equal shares of all tiles' steps for each workgroup, which leave none idle, cost more than that: their
+// workgroups no longer read the same part of the head at once (2665 rows x 49152 x 2048, 11 x 8 tiles:
+// the whole call 1.10 ms with splits, 1.29 with shares). 4001 rows x 49152 x 2048: 593 us, 1.36 PFLOP/s.
 template <int WP, int WL, int PF, int LF, bool KT, int OUT, int TERMS>
 __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductParams p) {
     using C = Core<WP, WL, PF, LF, KT, true, TERMS>;
@@ -1465,7 +1484,6 @@ LogitsParams logits_params(const ct_head_loss *a, const Plan &pl, const Kept &k,
     p.head_apart = pl.piece * p.ld / 8;
     p.packed_apart = pl.rows_pad * pl.width_pad / 8;
     p.piece_apart = pl.rows_pad * pl.piece / 8;
-    p.vocab = pl.vocab;
     p.packed = at<const uint4>(ws, sc.packed);
     p.blocks = pl.width_pad / 32;
     p.np = pl.rows_pad / pl.bp;

