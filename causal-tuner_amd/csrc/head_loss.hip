@@ -549,11 +549,13 @@ __global__ __launch_bounds__(256) void transpose_rows(const T *__restrict__ x, i
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 
-// Workgroup `id` of np x nl tiles: each of the 8 XCDs walks a contiguous range, in groups of four
-// packed tiles that share the other operand's tile in its L2.
-__device__ __forceinline__ void tile_of(int64_t id, int64_t np, int64_t nl, int64_t &tp, int64_t &tl) {
-    const int64_t total = np * nl, share = total / 8, more = total % 8, x = id & 7, i = id >> 3;
-    const int64_t t = x < more ? x * (share + 1) + i : more * (share + 1) + (x - more) * share + i;
+// What workgroup `id` of `total` comes to when each of the 8 XCDs walks a contiguous range.
+__device__ __forceinline__ int64_t by_xcd(int64_t id, int64_t total) {
+    const int64_t share = total / 8, more = total % 8, x = id & 7, i = id >> 3;
+    return x < more ? x * (share + 1) + i : more * (share + 1) + (x - more) * share + i;
+}
+// Tile t of np x nl, in groups of four packed tiles that share the other operand's tile in an L2.
+__device__ __forceinline__ void tile_at(int64_t t, int64_t np, int64_t nl, int64_t &tp, int64_t &tl) {
     const int64_t size = 4 * nl, group = t / size, at = t - group * size;
     const int64_t count = np - group * 4 < 4 ? np - group * 4 : 4;
     tp = group * 4 + at % count;
@@ -865,7 +867,7 @@ __global__ __launch_bounds__(64 * WP * WL) void logits_kernel(const LogitsParams
     __shared__ uint4 stages[3 * C::kStage];
     __shared__ uint4 marks[WP * WL][PF * 16 * UNITS];
     int64_t tp, tl;
-    tile_of(blockIdx.x, p.np, p.nl, tp, tl);
+    tile_at(by_xcd(blockIdx.x, p.np * p.nl), p.np, p.nl, tp, tl);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wp = wave % WP, wl = wave / WP, q = lane >> 4;
     const int64_t v0 = p.v0 + tl * C::BL, left = p.v1 - v0;
@@ -1072,11 +1074,15 @@ template <int WP, int WL, int PF, int LF, bool KT, int OUT, int TERMS>
 __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductParams p) {
     using C = Core<WP, WL, PF, LF, KT, true, TERMS>;
     __shared__ uint4 stages[3 * C::kStage];
+    // an XCD takes all tiles of the same splits, which share what they read (257 rows x 32003 x 1000 with both
+    // gradients 232 -> 220 us, 500 x 32001 x 1022 in float32 1108 -> 1061 against tiles spread over the XCDs)
+    const int64_t tiles = p.np * p.nl, t = by_xcd(blockIdx.x + tiles * blockIdx.y, tiles * gridDim.y);
+    const int split = (int)(t / tiles);
     int64_t tp, tl;
-    tile_of(blockIdx.x, p.np, p.nl, tp, tl);
+    tile_at(t - split * tiles, p.np, p.nl, tp, tl);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wp = wave % WP, wl = wave / WP, q = lane >> 4;
-    const int beg = blockIdx.y * p.steps_per_split;
+    const int beg = split * p.steps_per_split;
     const int end = beg + p.steps_per_split < p.steps ? beg + p.steps_per_split : p.steps;
     // the split's own range of the staged operand, so that offsets stay within 32 bits
     C core;
@@ -1098,7 +1104,7 @@ __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductPara
             if (col >= p.cols) continue;
             f32x4 v = acc[f][j];
             if constexpr (OUT == CT_F32) {
-                float *o = static_cast<float *>(p.out) + blockIdx.y * p.slab + row * p.ldo + col;
+                float *o = static_cast<float *>(p.out) + split * p.slab + row * p.ldo + col;
                 if (p.vec && col + 4 <= p.cols) {
                     if (p.factor) {
                         const float4 old = *reinterpret_cast<const float4 *>(o);
