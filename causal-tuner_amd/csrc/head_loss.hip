@@ -32,10 +32,10 @@
 //
 // Bound by the matrix units from some 300 rows on: 4 rows vocab width operations with the hidden
 // gradient, 8 with the head's too (2 of them the logits again, the price of not holding them). In bf16,
-// 49152 entries x 2048: 16384 rows with the hidden gradient 5.4 ms, 1.22 PFLOP/s (a library product of
-// such sizes alone runs at 1.26 to 1.55); 4001 rows with both gradients 2.7 ms, 1.18 PFLOP/s (logits 689
-// and 695, products 593 and 639 us). Of few rows by a read of the head for each product, from HBM and
-// in part from the last-level cache: one row, 201 MB, logits 33 us, product 46.
+// 49152 entries x 2048: 16384 rows with the hidden gradient 5.5 ms, 1.19 PFLOP/s (a library product of
+// such sizes alone runs at 1.26 to 1.55); 4001 rows with both gradients 2.8 ms, 1.15 PFLOP/s (logits 706
+// and 713, products 623 and 660 us). Of few rows by a read of the head for each product, from HBM and
+// in part from the last-level cache: one row, 201 MB, logits 33 us, product 34.
 //
 // Every sum runs in a fixed order: repeated calls are bit-identical.
 
@@ -856,8 +856,8 @@ __device__ __forceinline__ int64_t place_of(const LogitsParams &p, int64_t row, 
 // A tile's logits from Core, and from the accumulators what MODE asks for, so that no logit reaches
 // memory: the units' statistics (STATS), with E (EXP), or the derivative (GRAD), E and derivative in the
 // order in which the product that follows takes them. The orientation follows from that order: a lane
-// holds four entries of a row (EXP), or four rows of an entry (GRAD). 4001 rows x 49152 x 2048: 689 us,
-// 1.17 PFLOP/s, of which a fifth to a quarter are the exponentials and the stores behind the product's last step, which
+// holds four entries of a row (EXP), or four rows of an entry (GRAD). 4001 rows x 49152 x 2048: 706 us,
+// 1.14 PFLOP/s, of which a fifth to a quarter are the exponentials and the stores behind the product's last step, which
 // workgroups that stay resident and overlap them did not hide (3% slower).
 template <int WP, int WL, int PF, int LF, int MODE, int TERMS>
 __global__ __launch_bounds__(64 * WP * WL) void logits_kernel(const LogitsParams p) {
@@ -1066,10 +1066,11 @@ struct ProductParams {
 };
 
 // out[row, col] (= factor out +) sum_k packed(row, k) b(k, col), one split of the reduction per y, each
-// with an output of its own. Splits fill the compute units where the tiles alone do not (splits_for);
+// with an output of its own, and an XCD with all tiles of a split (one row x 49152 x 2048: 34 us, 46 where a
+// split's tiles were spread over the XCDs). Splits fill the compute units where the tiles alone do not (splits_for);
 // equal shares of all tiles' steps for each workgroup, which leave none idle, cost more than that: their
 // workgroups no longer read the same part of the head at once (2665 rows x 49152 x 2048, 11 x 8 tiles:
-// the whole call 1.10 ms with splits, 1.29 with shares). 4001 rows x 49152 x 2048: 593 us, 1.36 PFLOP/s.
+// the whole call 1.10 ms with splits, 1.29 with shares). 4001 rows x 49152 x 2048: 623 us, 1.29 PFLOP/s.
 template <int WP, int WL, int PF, int LF, bool KT, int OUT, int TERMS>
 __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductParams p) {
     using C = Core<WP, WL, PF, LF, KT, true, TERMS>;
