@@ -131,12 +131,17 @@ Plan plan_of(int64_t rows, int64_t width, int64_t vocab, int64_t entries, int dt
     p.vocab = vocab;
     p.entries = entries;
     p.dtype = dtype;
-    p.bp = rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    p.tri = dtype == CT_F32;
+    // float32: the narrow tile, which splits the head on the way to LDS, up to where the wide ones' reuse
+    // pays for terms in memory and transposes (with both gradients, narrow and wide: 500 rows x 4000 x 1000 183
+    // and 386 us, 4000 x 2000 x 1000 540 and 1127, 500 x 32001 x 1022 1045 and 1070, 1000 x 16000 x 1000 980 and
+    // 894, 2000 x 16000 x 1024 1825 and 1590).
+    const bool narrow = rows <= 64 || (p.tri && (rows <= 512 || cdiv(rows, 64) * cdiv(vocab, 128) <= 1024));
+    p.bp = narrow ? 64 : rows <= 128 ? 128 : 256;
     p.bl = p.bp == 64 ? 128 : 256;
     p.rows_pad = up(rows, p.bp);
     p.width_pad = up(width, kStep);
     p.units = cdiv(vocab, kUnit);
-    p.tri = dtype == CT_F32;
     p.terms[0] = 1;
     p.terms[1] = p.tri ? 3 : rows <= kTwoTerms ? 2 : 1;
     p.terms[2] = p.tri ? 3 : rows <= 2 * kTwoTerms ? 2 : 1;
@@ -584,9 +589,9 @@ __device__ __forceinline__ void tile_at(int64_t t, int64_t np, int64_t nl, int64
 // product of two terms is exact in float32. Six bf16 products are faster than one float32 product
 // on this card's matrix units (v_mfma_f32_16x16x4_f32, a sixteenth of the bf16 rate). The packed
 // operand's terms, and on the wide tiles the staged one's, lie in memory one after the other (TRI, six
-// passes over the reduction); the narrow tile, for few rows, which reading the staged operand bounds,
-// takes it as float32, splits it on the way to LDS and makes the six products of a step together
-// (FUSED: 3 rows x 60000 x 2000 1.70 ms with the terms in memory).
+// passes over the reduction); the narrow tile, for few rows or tiles (plan_of), takes the staged one as
+// float32, splits it on the way to LDS and makes the six products of a step together (FUSED: 3 rows x
+// 60000 x 2000 0.78 ms, 1.70 with the terms in memory).
 template <int WP, int WL, int PF, int LF, bool KT, bool SWAP, int TERMS = 1>
 struct Core {
     static constexpr bool FUSED = TERMS == 3 && PF == 1 && LF == 8, TRI = TERMS == 3 && !FUSED;
@@ -1409,7 +1414,8 @@ template <int MODE, int TERMS>
 hipError_t launch_logits(const Plan &pl, const LogitsParams &p, hipStream_t s) {
     const dim3 grid((unsigned)(p.np * p.nl));
     if (pl.bp == 64) logits_kernel<4, 1, 1, 8, MODE, TERMS><<<grid, dim3(256), 0, s>>>(p);
-    if (pl.bp == 128) logits_kernel<8, 1, 1, 16, MODE, TERMS><<<grid, dim3(512), 0, s>>>(p);
+    if constexpr (TERMS != 3)   // float32 has the narrow tile there
+        if (pl.bp == 128) logits_kernel<8, 1, 1, 16, MODE, TERMS><<<grid, dim3(512), 0, s>>>(p);
     if constexpr (MODE == GRAD || TERMS != 2)   // E of so many rows is one term or three
         if (pl.bp == 256) logits_kernel<8, 1, 2, 16, MODE, TERMS><<<grid, dim3(512), 0, s>>>(p);
     return hipGetLastError();
@@ -1428,7 +1434,7 @@ hipError_t launch_product(int bp, const ProductParams &p, int splits, hipStream_
         if constexpr (KT || (OUT == CT_F32 && TERMS != 2))
             product_kernel<4, 1, 1, 8, KT, OUT, TERMS><<<grid, dim3(256), 0, s>>>(p);
     } else if (bp == 128) {
-        if constexpr (!KT || TERMS < 3) product_kernel<8, 1, 1, 16, KT, OUT, TERMS><<<grid, dim3(512), 0, s>>>(p);
+        if constexpr (TERMS < 3) product_kernel<8, 1, 1, 16, KT, OUT, TERMS><<<grid, dim3(512), 0, s>>>(p);
     } else {
         if constexpr (!KT && TERMS != 2) product_kernel<8, 1, 2, 16, false, OUT, TERMS><<<grid, dim3(512), 0, s>>>(p);
     }

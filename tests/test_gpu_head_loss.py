@@ -116,6 +116,18 @@ def test_many_pieces(teacher):
     _check(loss, hidden, head, indices, values, weights, BF16)
 
 
+@pytest.mark.parametrize("rows,width,vocab", [(513, 72, 14600), (600, 33, 13200), (1030, 264, 8200), (512, 72, 14600)])
+def test_float32_on_wide_and_narrow_tiles(rows, width, vocab):
+    """More tiles than the narrow one takes from 513 rows on, in terms that lie in memory; 512 rows beside it."""
+    from causal_tuner.kernels.loss import distillation_loss
+    hidden, head, labels, weights = _inputs(rows, width, vocab, F32)
+    weights = weights / rows
+    _check(_streamed(hidden, head, labels, weights, F32), hidden, head, labels[:, None], None, weights, F32)
+    indices, values = _teacher(rows, vocab, 20)
+    loss = distillation_loss(hidden, head, indices, values, weights, temperature=2.0, compute_dtype=F32)
+    _check(loss, hidden, head, indices, values, weights, F32, 2.0)
+
+
 @pytest.mark.parametrize("dtype,rows,vocab", [(BF16, 4100, 70001), (F32, 2100, 45001)])
 @pytest.mark.parametrize("order", [1, -1])
 def test_maxima_that_move_between_pieces(order, dtype, rows, vocab):
