@@ -1081,7 +1081,7 @@ __global__ __launch_bounds__(64 * WP * WL) void product_kernel(const ProductPara
     using C = Core<WP, WL, PF, LF, KT, true, TERMS>;
     __shared__ uint4 stages[3 * C::kStage];
     // an XCD takes all tiles of the same splits, which share what they read (257 rows x 32003 x 1000 with both
-    // gradients 232 -> 220 us, 500 x 32001 x 1022 in float32 1108 -> 1061 against tiles spread over the XCDs)
+    // gradients 220 us, 232 with a split's tiles spread over the XCDs)
     const int64_t tiles = p.np * p.nl, t = by_xcd(blockIdx.x + tiles * blockIdx.y, tiles * gridDim.y);
     const int split = (int)(t / tiles);
     int64_t tp, tl;
