@@ -128,10 +128,15 @@ class StreamedHeadLoss(torch.autograd.Function):
             scratch = _workspace(scratch_bytes, device)
             scratch_at = scratch.data_ptr()
         if count:
-            # a tensor that was saved may have come back in another place
+            # hooks on saved tensors (save_on_cpu) may have brought one back in another place and with other strides
             call = _native.HeadLoss.from_buffer_copy(call)
-            call.head, call.rows = matrix.data_ptr(), _native.ptr(rows)
-            call.hidden = None if h is None else h.data_ptr() + first * h.stride(0) * h.element_size()
+            matrix, kept = _aligned_head(matrix), kept.contiguous()
+            rows = None if rows is None else rows.contiguous()
+            call.head, call.ld_head, call.rows = matrix.data_ptr(), matrix.stride(0), _native.ptr(rows)
+            if h is not None:
+                h = h if _plain(h) else h.clone(memory_format=torch.contiguous_format)
+                call.hidden = h.data_ptr() + first * h.stride(0) * h.element_size()
+                call.ld_hidden = max(h.stride(0), h.shape[1])
             # autograd has made the tensors' device current
             status = backward(call, upstream.to(torch.float32).data_ptr(), kept.data_ptr(), sums, kept_bytes, hidden_at, width,
                               width, hidden_code, head_at, width, width, head_code, scratch_at, scratch_bytes,

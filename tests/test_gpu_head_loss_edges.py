@@ -1,0 +1,36 @@
+"""Calls of the streamed losses beside those of a plain training step: hooks on saved tensors, rows given
+twice, operands that must not be dropped."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _pitched(rows, width, pitch, dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    wide = torch.randn(rows, pitch, device="cuda", generator=g).to(dtype)
+    return wide[:, 8:8 + width].requires_grad_()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("frozen", [False, True])
+def test_saved_on_the_host(frozen, rows, dtype):
+    """Pitched views come back from save_on_cpu as dense ones, and the gradients are those of the views."""
+    from causal_tuner.kernels.loss import projection_loss
+    hidden, head = _pitched(rows, 72, 100 if dtype == F32 else 104, dtype, 1), _pitched(777, 72, 136, dtype, 2)
+    head.requires_grad_(not frozen)
+    labels = torch.randint(777, (rows,), device="cuda")
+    weights = torch.rand(rows, device="cuda") + 0.1
+    leaves = [t for t in (hidden, head) if t.requires_grad]
+
+    def step():
+        loss = projection_loss(hidden, head, labels, weights, implementation="streamed", compute_dtype=dtype)
+        return loss
+    want = torch.autograd.grad(step(), leaves)
+    with torch.autograd.graph.save_on_cpu():
+        loss = step()
+    for a, b in zip(torch.autograd.grad(loss, leaves), want):
+        assert torch.equal(a, b)
