@@ -121,6 +121,7 @@ class _LayerNorm(torch.autograd.Function):
         _native.refuse_tangents("layer_norm", grad)
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         grad, device = grad.contiguous(), x.device
+        x, stats = x.contiguous(), stats.contiguous()   # hooks on saved tensors may have given them other strides
         dx = torch.empty_like(x) if need_x else None
         dw = torch.empty(width, device=device, dtype=dtype) if need_w else None
         db = torch.empty(width, device=device, dtype=dtype) if need_b else None

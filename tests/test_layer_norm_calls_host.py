@@ -1,0 +1,61 @@
+"""What layer_norm hands to the library, on host tensors with the native calls stubbed."""
+
+import contextlib
+import ctypes
+import types
+
+import pytest
+import torch
+
+from causal_tuner.kernels import _native, core_cuda
+
+
+def _read(address, count):
+    return torch.tensor((ctypes.c_float * count).from_address(address)[:])
+
+
+def _write(address, values):
+    ctypes.memmove(address, values.contiguous().data_ptr(), values.numel() * 4)
+
+
+class _Library:
+    """float32 rows: y is x + 1, the statistics 2 and 3; the backward records what it is given."""
+
+    def ct_layer_norm_backward_workspace(self, *sizes):
+        return 64
+
+    def ct_layer_norm_forward(self, x, dtype, w, bias, w_dtype, y, mean, rstd, rows, width, eps, stream):
+        _write(y, _read(x, rows * width) + 1)
+        if mean:
+            _write(mean, torch.full((rows,), 2.0))
+            _write(rstd, torch.full((rows,), 3.0))
+        return 0
+
+    def ct_layer_norm_backward(self, x, dtype, w, w_dtype, mean, rstd, dy, dx, dw, dbias, rows, width, *rest):
+        self.x, self.w = _read(x, rows * width).reshape(rows, width), _read(w, width)
+        self.stats = _read(mean, rows), _read(rstd, rows)
+        self.dy = _read(dy, rows * width).reshape(rows, width)
+        return 0
+
+
+@pytest.fixture
+def library(monkeypatch):
+    stub = _Library()
+    monkeypatch.setattr(core_cuda, "_native", types.SimpleNamespace(**{
+        **vars(_native), "library": lambda: stub, "device_of": lambda t: contextlib.nullcontext(), "stream_of": lambda t: None}))
+    return stub
+
+
+def _strided(t):
+    """The same values, no two of them side by side."""
+    return t.new_full((*t.shape, 2), 9.0)[..., 0].copy_(t)
+
+
+def test_saved_tensors_come_back_with_other_strides(library):
+    x, weight = torch.randn(5, 6, requires_grad=True), torch.randn(6, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, _strided):
+        y = core_cuda.layer_norm_device(x, weight, None, 1e-5)
+    dy = torch.randn(5, 6)
+    y.backward(dy)
+    assert torch.equal(library.x, x.detach()) and torch.equal(library.w, weight.detach()) and torch.equal(library.dy, dy)
+    assert torch.equal(library.stats[0], torch.full((5,), 2.0)) and torch.equal(library.stats[1], torch.full((5,), 3.0))
