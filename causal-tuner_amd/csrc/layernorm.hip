@@ -465,11 +465,14 @@ hipError_t launch_backward(const void *x, const void *w, int w_dtype, const floa
         }
     }
     else {
+        // the columns' sums first: dx may be dy itself
+        if (partial) {
+            columns_wide<DT><<<dim3((unsigned)cdiv(width, 256), (unsigned)teams), dim3(256), 0, stream>>>(
+                x, dy, mean, rstd, partial, rows, width);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
         if (dx) backward_wide<DT><<<dim3((unsigned)rows), dim3(1024), 0, stream>>>(x, w, w_dtype, mean, rstd, dy, dx, width);
-        hipError_t e = hipGetLastError();
-        if (e != hipSuccess || !partial) return e;
-        columns_wide<DT><<<dim3((unsigned)cdiv(width, 256), (unsigned)teams), dim3(256), 0, stream>>>(
-            x, dy, mean, rstd, partial, rows, width);
     }
     return hipGetLastError();
 }
