@@ -44,6 +44,7 @@
 #include <type_traits>
 
 #include "gemm_common.hpp"
+#include "term_steps.hpp"
 
 namespace ct {
 namespace {
@@ -611,8 +612,8 @@ struct Core {
     const uint4 *a;          // the wave's packed rows at step 0
     int64_t a_row;           // units between two blocks of packed rows
     int steps, store_at, read_at;
-    uint32_t part;           // TRI: 2^32 / the steps of one product of terms, rounded up
-    int one;                 // TRI: those steps
+    int one;                 // TRI: the steps of one product of terms
+    TermDivisor part;        // TRI: the division by those
     int64_t b_apart, a_apart = 0;  // bytes, and units, between two terms
 
     // first: the staged operand at the tile's first row (KC) or column (KT); `extent` its rows from
@@ -650,16 +651,16 @@ struct Core {
         a_apart = a_units;
         if constexpr (!TRI) return;
         one = steps;
-        part = one > 1 ? 0xffffffffu / (uint32_t)one + 1 : 0;
+        part = term_divisor(one);
         steps *= 6;
         b_apart = b_units * 16;
     }
     // The product of terms that step t belongs to, and the step in it. Of the packed operand the terms
     // 2 1 0 1 0 0, of the staged one 0 1 2 0 1 0.
     __device__ __forceinline__ int product(int t, int &at) const {
-        const int s = one > 1 ? (int)__umulhi((uint32_t)t, part) : t;
-        at = t - s * one;
-        return s;
+        const TermStep step = term_step(t, one, part);
+        at = step.at;
+        return step.product;
     }
     // The thread's unit C of step t, its fragment I, and the unit's place in a stage.
     template <int C>

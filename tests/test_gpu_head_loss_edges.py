@@ -34,3 +34,25 @@ def test_saved_on_the_host(frozen, rows, dtype):
         loss = step()
     for a, b in zip(torch.autograd.grad(loss, leaves), want):
         assert torch.equal(a, b)
+
+
+def test_float32_head_gradient_of_very_many_rows():
+    """26992 steps of 64 rows: the first count whose last step a rounded reciprocal puts into a product of terms
+    that there is not. All rows but the last 64 are zero, so that the head's gradient is theirs."""
+    from causal_tuner.kernels.loss import projection_loss
+    rows, width, vocab = 26992 * 64, 72, 130
+    g = torch.Generator(device="cuda").manual_seed(1)
+    hidden = torch.zeros(rows, width, device="cuda")
+    hidden[-64:] = torch.randn(64, width, device="cuda", generator=g)
+    head = (torch.randn(vocab, width, device="cuda", generator=g) * 0.2).requires_grad_()
+    labels = torch.randint(vocab, (rows,), device="cuda", generator=g)
+    weights = torch.ones(rows, device="cuda")
+    loss = projection_loss(hidden, head, labels, weights, implementation="streamed", compute_dtype=F32, rows=slice(0, rows))
+    dw, = torch.autograd.grad(loss, head)
+    h = hidden[-64:].double()
+    d = torch.softmax(h @ head.detach().double().T, -1)
+    d[torch.arange(64), labels[-64:]] -= 1
+    # float32 throughout: a derivative within 2^-17 of its size and 2^-20 (a probability's error and the target's),
+    # then 64 products and sums
+    bound = (d.abs() * 2.0 ** -17 + 2.0 ** -20).T @ h.abs() * (1 + 64 * 2.0 ** -24)
+    assert ((dw.double() - d.T @ h).abs() <= bound).all()
