@@ -20,6 +20,7 @@ _MAX_WIDTH = 1 << 16
 _MAX_VOCAB = (1 << 31) - 1024
 _MAX_ROWS = (1 << 24) - 256
 _MAX_VALUES = (1 << 35) - 256    # of the padded rows
+_MAX_HEAD_ROWS = (1 << 22) - 64  # with the head's gradient
 
 
 def _rows_of(selection, tokens, device):
@@ -67,14 +68,18 @@ class StreamedHeadLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, head, tables, selection, compute_dtype, temperature):
         need_hidden, need_head = ctx.needs_input_grad[:2]
-        h, matrix = _plain_rows(hidden.to(compute_dtype)), _aligned_head(head.to(compute_dtype))
-        tokens, device = len(h), h.device
-        first, rows, count = _rows_of(selection, tokens, device)
         indices, values, normalizer, weights = tables
-        entries, (vocab, width) = indices.shape[1], matrix.shape
+        tokens, device, entries = len(indices), hidden.device, indices.shape[1]
+        first, rows, count = _rows_of(selection, tokens, device)
+        matrix = _aligned_head(head.to(compute_dtype))
+        vocab, width = matrix.shape
+        if need_head and count > _MAX_HEAD_ROWS:
+            raise ValueError(f"streamed head loss: {count} rows; the HIP kernels take up to {_MAX_HEAD_ROWS} at once with the "
+                             "head's gradient")
         if count > _MAX_ROWS or (count + 255) // 256 * 256 * ((width + 63) // 64 * 64) > _MAX_VALUES:
             raise ValueError(f"streamed head loss: {count} rows of {width} values; the HIP kernels take up to {_MAX_ROWS} rows "
                              f"and {_MAX_VALUES} values at once")
+        h = _plain_rows(hidden.to(compute_dtype))
         skip = first * entries
         ld, code = h.stride(0), _native.dtype_code(compute_dtype)
         call = _native.HeadLoss(

@@ -60,6 +60,9 @@ constexpr int64_t kMaxPitch = 1 << 20;   // a tile's offsets stay below 2^31
 // A launch holds fewer than 2^32 threads: 256 per row, one per eight values of the padded rows.
 constexpr int64_t kMaxWidth = 65536, kMaxVocab = (int64_t{1} << 31) - 1024, kMaxRows = (int64_t{1} << 24) - 256;
 constexpr int64_t kMaxValues = (int64_t{1} << 35) - 256;
+// Rows of a head gradient: transposed, they are the columns of a tile's 256 rows of bf16, up(rows, kStep) apart,
+// whose bytes a descriptor's 2^31 - 1 have to hold.
+constexpr int64_t kMaxHeadRows = (0x7fffffff / (256 * 2)) / kStep * kStep;
 // Values of one piece, in bytes, whatever the batch and the vocabulary. Larger pieces read and write the
 // float32 sums less often (16384 tokens, of 49152 entries: 128 MB 6.25 ms, 256 MB 5.75, 512 MB 5.54, 1 GB
 // 5.47), smaller ones stay in the 256 MB last-level cache, which pays for less than that.
@@ -1451,7 +1454,8 @@ hipError_t launch_product(int bp, int terms, const ProductParams &p, int splits,
     return terms == 2 ? launch_product<OUT, false, 2>(bp, p, splits, s) : launch_product<OUT, false, 1>(bp, p, splits, s);
 }
 
-// forward: the targets are read from the tables; later they are in what is kept.
+// hidden: the hidden rows are read (in a backward, for the head's gradient). forward: the targets are read
+// from the tables; later they are in what is kept.
 int check(const ct_head_loss *a, bool hidden, bool forward) {
     if (!a) return -CT_EINVAL_POINTER;
     if (a->dtype != CT_BF16 && a->dtype != CT_F32) return -CT_EINVAL_DTYPE;
@@ -1465,6 +1469,7 @@ int check(const ct_head_loss *a, bool hidden, bool forward) {
     if (forward && !a->values && a->entries != 1) return -CT_EINVAL_SHAPE;
     if (forward && (a->ld_indices < a->entries || (a->values && a->ld_values < a->entries))) return -CT_EINVAL_SHAPE;
     if (up(a->count, 256) * up(a->width, kStep) > kMaxValues) return -CT_EINVAL_SHAPE;
+    if (!forward && hidden && a->count > kMaxHeadRows) return -CT_EINVAL_SHAPE;
     if (!(a->temperature > 0)) return -CT_EINVAL_SHAPE;
     if (a->count && ((hidden && !a->hidden) || !a->head)) return -CT_EINVAL_POINTER;
     if (a->count && forward && (!a->indices || !a->weights)) return -CT_EINVAL_POINTER;
@@ -1616,7 +1621,9 @@ extern "C" int64_t ct_head_loss_kept(int64_t count, int64_t width, int64_t vocab
 
 extern "C" int64_t ct_head_loss_workspace(int64_t count, int64_t width, int64_t vocab, int32_t entries, int32_t dtype,
                                           int32_t pass) {
-    if (check_sizes(count, width, vocab, entries, dtype) || count == 0 || pass < 0 || pass > 2) return 0;
+    if (check_sizes(count, width, vocab, entries, dtype) || count == 0 || pass < 0 || pass > 2 ||
+        (pass == 2 && count > kMaxHeadRows))
+        return 0;
     return scratch_of(plan_of(count, width, vocab, entries, dtype), pass).bytes;
 }
 

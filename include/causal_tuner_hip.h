@@ -655,7 +655,7 @@ int ct_muon(const ct_muon_matrix *matrices, int64_t count, const int32_t *plan, 
  * an index given twice counts once with the sum of both, and a row without entries has no loss.
  * bf16: width and ld_head multiples of 8, head 16-byte aligned. Pitches of hidden and head up to 2^20,
  * width up to 65536, entries up to 1024, count below 2^24 - 255, and count x width, rounded up to 256 and
- * 64, below 2^35 - 255.
+ * 64, below 2^35 - 255; with d_head count up to 4194240.
  */
 typedef struct ct_head_loss {
     const void *hidden;

@@ -56,3 +56,26 @@ def test_float32_head_gradient_of_very_many_rows():
     # then 64 products and sums
     bound = (d.abs() * 2.0 ** -17 + 2.0 ** -20).T @ h.abs() * (1 + 64 * 2.0 ** -24)
     assert ((dw.double() - d.T @ h).abs() <= bound).all()
+
+
+def test_head_gradient_of_the_most_rows():
+    """2^22 - 64 rows, of 256 columns: the last column's last row lies just below the descriptor's end. Rows of zeros
+    but for the last 64, as above; the derivative rounded once to bf16, the gradient too."""
+    from causal_tuner.kernels.loss import projection_loss
+    rows, width, vocab = (1 << 22) - 64, 256, 130
+    g = torch.Generator(device="cuda").manual_seed(1)
+    hidden = torch.zeros(rows, width, device="cuda", dtype=BF16)
+    hidden[-64:] = torch.randn(64, width, device="cuda", generator=g).to(BF16)
+    head = (torch.randn(vocab, width, device="cuda", generator=g) * 0.1).to(BF16).requires_grad_()
+    labels = torch.randint(vocab, (rows,), device="cuda", generator=g)
+    run = lambda h, to: projection_loss(h, head, to, torch.ones(1, device="cuda").expand(len(h)), implementation="streamed",  # noqa: E731
+                                        rows=slice(0, len(h)))
+    dw, = torch.autograd.grad(run(hidden, labels), head)
+    h = hidden[-64:].double()
+    d = torch.softmax(h @ head.detach().double().T, -1)
+    d[torch.arange(64), labels[-64:]] -= 1
+    bound = (d.abs() * (2.0 ** -8 + 2.0 ** -16) + 2.0 ** -20).T @ h.abs()
+    want = d.T @ h
+    assert ((dw.double() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all()
+    with pytest.raises(ValueError, match="head's gradient"):
+        run(hidden[:1].expand(rows + 1, width), labels[:1].expand(rows + 1))

@@ -72,3 +72,34 @@ def test_saved_tensors_come_back_with_other_strides(dtype, rows, restore, librar
         assert (call.ld_hidden, call.ld_head) == (h.stride(0), w.stride(0)) == (width, width)
         assert call.head == w.data_ptr() and call.hidden == h.data_ptr() + first * width * size
     assert call.hidden and call.head % 16 == 0 and bool(call.rows) == isinstance(rows, torch.Tensor)
+
+
+@pytest.mark.parametrize("rows,refused", [((1 << 22) - 64, False), ((1 << 22) - 63, True)])
+def test_rows_of_a_head_gradient(rows, refused, library):
+    """More rows than a tile's offsets reach are refused by name before anything is laid out; a frozen head takes them."""
+    hidden, head = torch.zeros(1, 8).expand(rows, 8).requires_grad_(), torch.zeros(3, 8, requires_grad=True)
+    run = lambda w: head_loss_cuda.streamed_loss(hidden, w, torch.ones(1).expand(rows), slice(0, rows), torch.float32,  # noqa: E731
+                                                 torch.zeros(1, 1, dtype=torch.int64).expand(rows, 1))
+    if refused:
+        with pytest.raises(ValueError, match="head's gradient"):
+            run(head)
+        assert library.forward is None
+        run(head.detach())
+    else:
+        run(head)
+    assert library.forward.count == rows
+
+
+def test_library_refuses_a_head_gradient_of_more_rows():
+    lib = _native.library()
+    rows = (1 << 22) - 63
+    a = _native.HeadLoss(hidden=256, head=256, ld_hidden=64, ld_head=64, tokens=rows, hidden_width=64, count=rows, width=64,
+                         vocab=100, entries=1, dtype=_native.CT_BF16, temperature=1.0)
+    back = lambda d_hidden, d_head: lib.ct_head_loss_backward(a, 256, None, 1, 0, d_hidden, 64, 64, _native.CT_BF16, d_head, 64,  # noqa: E731
+                                                              64, _native.CT_BF16, 256, 1 << 40, None)
+    assert back(None, 256) == back(256, 256) == -2
+    assert back(256, None) == -5   # only the missing buffer
+    a.count -= 1
+    assert back(None, 256) == -5
+    sizes = (64, 100, 1, _native.CT_BF16, 2)
+    assert lib.ct_head_loss_workspace(rows, *sizes) == 0 < lib.ct_head_loss_workspace(rows - 1, *sizes)
