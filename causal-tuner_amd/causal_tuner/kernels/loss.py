@@ -60,8 +60,9 @@ def projection_loss(hidden, head, targets, weights, *, token_budget=128, compute
     `implementation="streamed"` takes all rows at once and walks the vocabulary in pieces instead
     (`head_loss_cuda`): no logits are held, so `token_budget` plays no part; the statistics and
     the loss come from unrounded float32 logits, and every gradient is rounded once, after the
-    upstream scale. bf16 and float32; `reuse_hidden` belongs to the fused path. With `rows` given
-    it can be captured into a graph. `rows` names each row at most once, counted from 0, in any order."""
+    upstream scale. bf16 and float32; `reuse_hidden` belongs to the fused path, and weights that ask for
+    a gradient are refused. With `rows` given it can be captured into a graph. `rows` names each row at
+    most once, counted from 0, in any order."""
     if token_budget <= 0:
         raise ValueError("loss_token_budget must be positive")
     selection = active_rows(weights, hidden.device) if rows is None else rows
@@ -102,6 +103,8 @@ def _check_rows(hidden, head, weights, tables):
     for name, table in tables.items():
         if table.numel() != tokens * (table.shape[-1] if name in ("indices", "values") else 1):
             raise ValueError(f"{name} {tuple(table.shape)} for {tokens} rows of hidden")
+    if weights.requires_grad and torch.is_grad_enabled():
+        raise ValueError("weights get no gradient: detach them")
     for name, table in {"head": head, **tables}.items():
         if table.device != hidden.device:
             raise ValueError(f"{name} is on {table.device}, hidden on {hidden.device}")
@@ -123,7 +126,8 @@ def distillation_loss(hidden, head, indices, values, weights, *, temperature=1.0
     without entries has no loss and no gradient. The factor temperature^2 that keeps the gradient's size,
     or a share beside another loss, belongs into `weights`. The vocabulary is walked in pieces
     as `projection_loss(implementation="streamed")` does, on the same kernels; gradients reach
-    hidden and head, not the teacher. `rows` as in `projection_loss`."""
+    hidden and head, not the teacher or the weights, which are refused where they ask for one. `rows`
+    as in `projection_loss`."""
     if indices.dim() < 1 or indices.shape != values.shape:
         raise ValueError(f"indices {tuple(indices.shape)} and values {tuple(values.shape)} differ")
     if not 1 <= indices.shape[-1] <= 1024:

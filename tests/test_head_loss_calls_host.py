@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from causal_tuner.kernels import _native, head_loss_cuda
+from causal_tuner.kernels.loss import distillation_loss, projection_loss
 
 
 class _Library:
@@ -103,3 +104,17 @@ def test_library_refuses_a_head_gradient_of_more_rows():
     assert back(None, 256) == -5
     sizes = (64, 100, 1, _native.CT_BF16, 2)
     assert lib.ct_head_loss_workspace(rows, *sizes) == 0 < lib.ct_head_loss_workspace(rows - 1, *sizes)
+
+
+def test_weights_that_ask_for_a_gradient_are_refused():
+    """On the host as on the device, where none is made: nothing is dropped without a word."""
+    hidden, head, weights = torch.randn(4, 8, requires_grad=True), torch.randn(9, 8), torch.rand(4, requires_grad=True)
+    indices, labels = torch.randint(9, (4, 3)), torch.randint(9, (4,))
+    calls = [lambda w: distillation_loss(hidden, head, indices, torch.randn(4, 3), w),
+             lambda w: projection_loss(hidden, head, labels, w, implementation="streamed")]
+    for call in calls:
+        with pytest.raises(ValueError, match="weights get no gradient"):
+            call(weights)
+        call(weights.detach())
+        with torch.no_grad():
+            call(weights)
