@@ -163,7 +163,7 @@ def streamed_loss(hidden, head, weights, selection, compute_dtype, indices, valu
     if head.shape[1] > _MAX_WIDTH or len(head) > _MAX_VOCAB:
         raise ValueError(f"streamed head loss: head {tuple(head.shape)}; the HIP kernels take up to {_MAX_VOCAB} entries and "
                          f"a width of {_MAX_WIDTH}")
-    _native.refuse_tangents("streamed head loss", hidden, head)
+    _native.refuse_tangents("streamed head loss", *(t for t in (hidden, head, weights, values, log_normalizer) if t is not None))
     device = hidden.device
     wide = lambda t: None if t is None else t.to(device, torch.float32).contiguous()  # noqa: E731
     tables = (indices.to(torch.int64).contiguous(), wide(values), wide(log_normalizer), wide(weights.flatten()))

@@ -5,6 +5,7 @@ import types
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from causal_tuner.kernels import _native, head_loss_cuda
 from causal_tuner.kernels.loss import distillation_loss, projection_loss
@@ -118,3 +119,18 @@ def test_weights_that_ask_for_a_gradient_are_refused():
         call(weights.detach())
         with torch.no_grad():
             call(weights)
+
+
+@pytest.mark.parametrize("which", ["hidden", "head", "weights", "values", "log_normalizer"])
+def test_forward_derivatives_are_refused(which, library):
+    given = dict(hidden=torch.randn(4, 8), head=torch.randn(9, 8), weights=torch.rand(4), values=torch.randn(4, 3),
+                 log_normalizer=torch.zeros(4))
+
+    def run(t):
+        return head_loss_cuda.streamed_loss(t["hidden"], t["head"], t["weights"], slice(0, 4), torch.float32,
+                                            torch.randint(9, (4, 3)), t["values"], t["log_normalizer"])
+    with forward_ad.dual_level():
+        run(given)
+        given[which] = forward_ad.make_dual(given[which], torch.ones_like(given[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            run(given)
