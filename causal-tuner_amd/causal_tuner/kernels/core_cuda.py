@@ -69,7 +69,7 @@ class RMS(torch.autograd.Function):
 
 
 def _layer_norm(x, weight, bias, eps, keep):
-    """(x as the kernel reads it, y, mean and rstd [2, rows]; None unless kept)."""
+    """(x as the kernel reads it, y, mean and rstd [2, rows] or None unless kept, rows, width)."""
     x = x.contiguous()
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         weight, bias = weight.float(), bias.float()   # one type for both: float32 holds either
@@ -78,8 +78,8 @@ def _layer_norm(x, weight, bias, eps, keep):
     if bias is not None:
         bias = bias.contiguous()
     vector = weight if weight is not None else bias
-    y, width = torch.empty_like(x), x.shape[-1]
-    rows = x.numel() // width
+    y, width = torch.empty_like(x), int(x.shape[-1])   # under a trace sizes are tensors
+    rows = int(x.numel()) // width
     stats = mean = rstd = None
     if keep:
         stats = torch.empty((2, rows), device=x.device, dtype=torch.float32)
@@ -91,7 +91,7 @@ def _layer_norm(x, weight, bias, eps, keep):
             _native.CT_F32 if vector is None else _native.dtype_code(vector.dtype), y.data_ptr(), mean, rstd, rows, width,
             eps, _native.stream_of(x))
     _native.check(status, "ct_layer_norm_forward")
-    return x, y, stats
+    return x, y, stats, rows, width
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -100,14 +100,14 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        x, y, stats = _layer_norm(x, weight, bias, eps, True)
+        x, y, stats, rows, width = _layer_norm(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, stats)
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         kept = None if weight is None else weight.dtype
         given = None if bias is None else bias.dtype
         # both sums are made in the weight's dtype; beside a bias of another one, in float32
         dtype = kept if given is None or given == kept else given if kept is None else torch.float32
-        rows, width, code = stats.shape[1], x.shape[-1], _native.dtype_code(x.dtype)
+        code = _native.dtype_code(x.dtype)
         lib, sums = _native.library(), need_w or need_b
         ctx.plan = (lib.ct_layer_norm_backward, code, dtype, _native.CT_F32 if dtype is None else _native.dtype_code(dtype),
                     kept, given, rows, width, lib.ct_layer_norm_backward_workspace(rows, width, code, 1) if sums else 0)
@@ -149,7 +149,8 @@ def layer_norm_device(x, weight, bias, eps):
         raise NotImplementedError("layer_norm: the HIP kernels take bfloat16, float16 or float32")
     given = [t for t in (x, weight, bias) if t is not None]
     _native.refuse_tangents("layer_norm", *given)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+    # without gradients the function is passed by, but not under a trace, which would record no call
+    if torch.jit.is_tracing() or (torch.is_grad_enabled() and any(t.requires_grad for t in given)):
         return _LayerNorm.apply(x, weight, bias, eps)
     return _layer_norm(x, weight, bias, eps, False)[1]
 

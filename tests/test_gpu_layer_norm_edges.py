@@ -36,3 +36,22 @@ def test_input_gradient_over_the_incoming_one(width, dtype):
         assert torch.equal(a, b), name
     # rows 2^-24 each, of sums of magnitudes of about 70 (dbias) in any order
     assert (apart[2] - dy.double().sum(0)).abs().max() <= rows * 2.0 ** -24 * dy.double().abs().sum(0).max()
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("grads", [False, True])
+def test_traced_calls(grads):
+    """A trace holds the call itself: new inputs, of other row counts too, with and without gradients."""
+    from causal_tuner.modeling.norm import LayerNorm
+    norm = LayerNorm(72, 1e-5, BF16, "cuda").requires_grad_(grads)
+    make = lambda n: torch.randn(n, 72, device="cuda").to(BF16).requires_grad_(grads)  # noqa: E731
+    with torch.set_grad_enabled(grads):
+        traced = torch.jit.trace(norm, (make(5),), check_trace=False)
+        for n in (5, 5, 9):
+            x = make(n)
+            got, want = traced(x), norm(x)
+            assert torch.equal(got, want)
+            if grads:
+                dy, leaves = torch.randn_like(want), (x, norm.weight, norm.bias)
+                for a, b in zip(torch.autograd.grad(got, leaves, dy), torch.autograd.grad(want, leaves, dy)):
+                    assert torch.equal(a, b)
