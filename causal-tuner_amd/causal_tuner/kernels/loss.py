@@ -62,7 +62,7 @@ def projection_loss(hidden, head, targets, weights, *, token_budget=128, compute
     the loss come from unrounded float32 logits, and every gradient is rounded once, after the
     upstream scale. bf16 and float32; `reuse_hidden` belongs to the fused path, and weights that ask for
     a gradient are refused. With `rows` given it can be captured into a graph. `rows` names each row at
-    most once, counted from 0, in any order."""
+    most once, counted from 0, in any order; a number that names no row has no loss."""
     if token_budget <= 0:
         raise ValueError("loss_token_budget must be positive")
     selection = active_rows(weights, hidden.device) if rows is None else rows
@@ -77,6 +77,8 @@ def projection_loss(hidden, head, targets, weights, *, token_budget=128, compute
             raise ValueError("targets are whole numbers")
         _check_rows(hidden, head, weights, {"targets": targets})
     if not hidden.is_cuda:
+        if implementation == "streamed":
+            selection = _named_rows(selection, weights.numel())
         return ProjectionLoss.apply(hidden, head, targets, weights, token_budget, compute_dtype, selection)
     if not torch.is_grad_enabled():
         hidden, head = hidden.detach(), head.detach()
@@ -91,6 +93,14 @@ def projection_loss(hidden, head, targets, weights, *, token_budget=128, compute
     total, _ = FusedProjectionLoss.apply(hidden, head, targets, weights, token_budget, compute_dtype,
                                          reuse_hidden, selection)
     return total
+
+
+def _named_rows(selection, tokens):
+    """Of row numbers on the host those that name a row, as the device's kernels take them: one outside [0, tokens)
+    has no loss."""
+    if isinstance(selection, slice):
+        return selection
+    return selection[(selection >= 0) & (selection < tokens)]
 
 
 def _check_rows(hidden, head, weights, tables):
@@ -158,6 +168,7 @@ def distillation_loss(hidden, head, indices, values, weights, *, temperature=1.0
 
 def _host_distillation(hidden, head, indices, values, weights, temperature, log_normalizer, compute_dtype, selection):
     """The same in torch operations, float32 (float64 for its tensors) from the logits on."""
+    selection = _named_rows(selection, len(indices))
     h = hidden.reshape(-1, hidden.shape[-1])[selection].to(compute_dtype)
     wide = torch.promote_types(compute_dtype, torch.float32)
     log_p = torch.log_softmax(F.linear(h, head.to(compute_dtype)).to(wide) / temperature, -1)
