@@ -61,8 +61,8 @@ def projection_loss(hidden, head, targets, weights, *, token_budget=128, compute
     (`head_loss_cuda`): no logits are held, so `token_budget` plays no part; the statistics and
     the loss come from unrounded float32 logits, and every gradient is rounded once, after the
     upstream scale. bf16 and float32; `reuse_hidden` belongs to the fused path, and weights that ask for
-    a gradient are refused. With `rows` given it can be captured into a graph. `rows` names each row at
-    most once, counted from 0, in any order; a number that names no row has no loss."""
+    a gradient are refused. With `rows` given it can be captured into a graph. `rows` are numbers
+    counted from 0, in any order: one given twice counts twice, one that names no row has no loss."""
     if token_budget <= 0:
         raise ValueError("loss_token_budget must be positive")
     selection = active_rows(weights, hidden.device) if rows is None else rows
@@ -78,7 +78,7 @@ def projection_loss(hidden, head, targets, weights, *, token_budget=128, compute
         _check_rows(hidden, head, weights, {"targets": targets})
     if not hidden.is_cuda:
         if implementation == "streamed":
-            selection = _named_rows(selection, weights.numel())
+            selection, weights = _counted_rows(_named_rows(selection, weights.numel()), weights)
         return ProjectionLoss.apply(hidden, head, targets, weights, token_budget, compute_dtype, selection)
     if not torch.is_grad_enabled():
         hidden, head = hidden.detach(), head.detach()
@@ -101,6 +101,18 @@ def _named_rows(selection, tokens):
     if isinstance(selection, slice):
         return selection
     return selection[(selection >= 0) & (selection < tokens)]
+
+
+def _counted_rows(selection, weights):
+    """Row numbers without repeats, the weights of repeated ones times their count."""
+    if isinstance(selection, slice):
+        return selection, weights
+    rows, times = selection.unique(return_counts=True)
+    if len(rows) == len(selection):
+        return selection, weights
+    weights = weights.flatten().clone()
+    weights[rows] *= times
+    return rows, weights
 
 
 def _check_rows(hidden, head, weights, tables):

@@ -177,8 +177,14 @@ struct Regions {
     }
 };
 struct Kept {
-    int64_t index, q, chosen, first, shift, total, weight, mass, entropy, sums, bytes;
+    int64_t index, q, chosen, first, shift, total, weight, mass, entropy, sums, slots, place, bytes;
 };
+// Slots of the table that counts how often a row is given: at most half of them are taken.
+int64_t slots_for(int64_t rows) {
+    int64_t n = 2;
+    while (n < 2 * rows) n *= 2;
+    return n;
+}
 Kept kept_of(const Plan &p, bool hidden_grad) {
     Regions r;
     Kept k{};
@@ -192,6 +198,8 @@ Kept kept_of(const Plan &p, bool hidden_grad) {
     k.mass = r.take(p.rows_pad * 4);
     k.entropy = r.take(p.rows_pad * 4);
     k.sums = r.take(hidden_grad ? (int64_t)p.splits * p.rows * p.width * 4 : 0);
+    k.slots = r.take(hidden_grad ? slots_for(p.rows) * 8 : 0);   // a row of the loss each, then how often it is given
+    k.place = r.take(hidden_grad ? p.rows * 4 : 0);              // a row's slot
     k.bytes = r.at;
     return k;
 }
@@ -230,6 +238,28 @@ struct Targets {
     int64_t ld_indices, ld_values;
 };
 
+// How often each row of the tables is given: a row of the loss finds the slot of its table row, whichever of the
+// equal ones claims it, and counts there. `slots` null: rows are not numbered.
+struct Repeats {
+    int *slots, *place;
+    int64_t size;   // a power of two; the counts follow the slots
+    // Thread u of a launch with at least `size` threads; before any call of `count`.
+    __device__ __forceinline__ void clear(int64_t u) const {
+        if (!slots || u >= size) return;
+        slots[u] = -1;
+        slots[size + u] = 0;
+    }
+    __device__ __forceinline__ void count(const int64_t *rows, int64_t row) const {
+        int64_t at = (int64_t)((uint64_t)rows[row] * 0x9e3779b97f4a7c15u >> 32) & (size - 1);
+        for (;; at = (at + 1) & (size - 1)) {   // ends: there are more slots than rows
+            const int held = atomicCAS(slots + at, -1, (int)row);
+            if (held == -1 || rows[held] == rows[row]) break;
+        }
+        atomicAdd(slots + size + at, 1);
+        place[row] = (int)at;
+    }
+};
+
 // A float sum over the workgroup, in a fixed order.
 template <int THREADS>
 __device__ __forceinline__ float block_sum(float v, float *lds) {
@@ -265,7 +295,8 @@ __global__ __launch_bounds__(THREADS) void targets_kernel(Targets t, int64_t row
                                                           float *__restrict__ q_out, float *__restrict__ chosen,
                                                           uint16_t *__restrict__ first, float *__restrict__ weight,
                                                           float *__restrict__ mass, float *__restrict__ entropy,
-                                                          float *__restrict__ shift, float *__restrict__ total) {
+                                                          float *__restrict__ shift, float *__restrict__ total,
+                                                          const Repeats repeats) {
     __shared__ uint64_t key[MOST];
     __shared__ float value[MOST], lds[THREADS];
     __shared__ int sorted[MOST], kept;
@@ -286,6 +317,7 @@ __global__ __launch_bounds__(THREADS) void targets_kernel(Targets t, int64_t row
         if (tid == 0) weight[row] = mass[row] = entropy[row] = 0.f;
         return;
     }
+    if (repeats.slots && tid == 0) repeats.count(t.rows, row);
     if (!t.values) {  // one hard label
         const int64_t label = t.indices[from * t.ld_indices];
         const bool there = label >= 0 && label < vocab;
@@ -433,9 +465,11 @@ __device__ __forceinline__ void split_unit(const float (&v)[8], uint4 (&out)[TER
 }
 
 // pack_rows below for float32 rows: three packed operands, `units` apart.
-__global__ __launch_bounds__(256) void pack_split(Source src, int64_t blocks, uint4 *__restrict__ out, int64_t units) {
+__global__ __launch_bounds__(256) void pack_split(Source src, int64_t blocks, uint4 *__restrict__ out, int64_t units,
+                                                  const Repeats repeats) {
     const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (u >= units) return;
+    repeats.clear(u);
     const int lane = (int)(u & 63);
     const int64_t block = u >> 6, kb = block % blocks, row = src.row(block / blocks * 16 + (lane & 15));
     const int64_t k = kb * 32 + (lane >> 4) * 8;
@@ -472,11 +506,14 @@ __global__ __launch_bounds__(256) void split_rows(const float *__restrict__ x, i
     for (int s = 0; s < 3; ++s) out[u + s * apart] = t[s];
 }
 
-// Hidden rows in the order of a product's packed operand, zeros past the rows and the width.
+// Hidden rows in the order of a product's packed operand, zeros past the rows and the width. On the way the
+// slots of `repeats` are cleared: eight units or more a row, four slots at most.
 template <bool VEC>
-__global__ __launch_bounds__(256) void pack_rows(Source src, int64_t blocks, uint4 *__restrict__ out, int64_t units) {
+__global__ __launch_bounds__(256) void pack_rows(Source src, int64_t blocks, uint4 *__restrict__ out, int64_t units,
+                                                 const Repeats repeats) {
     const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (u >= units) return;
+    repeats.clear(u);
     const int lane = (int)(u & 63);
     const int64_t block = u >> 6, kb = block % blocks, row = src.row(block / blocks * 16 + (lane & 15));
     const int64_t k = kb * 32 + (lane >> 4) * 8;
@@ -1306,7 +1343,8 @@ __global__ __launch_bounds__(256) void row_factors(const float *__restrict__ wei
     factor[row] = row < rows && mass[row] != 0.f ? f * mass[row] / z : 0.f;
 }
 
-// dh_i = u c_i / T (Q_i / Z_i sums_i + sum_k coefficient_k w_v_k). A wave takes a row and 512 columns,
+// dh_i = u c_i / T (Q_i / Z_i sums_i + sum_k coefficient_k w_v_k), times how often the row is given: rows of one
+// number are equal, and each of them writes that value. A wave takes a row and 512 columns,
 // four waves of a workgroup 2048; where there are many splits or targets (SHARE) the four take the
 // same 512 columns, every fourth split and target each, and are joined in order. Bound by the sums and
 // by the targets' rows of the head, K x width per row of the loss, from the caches (8192 rows of 64 x
@@ -1320,12 +1358,14 @@ __global__ __launch_bounds__(256) void hidden_grad_kernel(const float *__restric
                                                           const float *__restrict__ coefficient, int entries,
                                                           const void *__restrict__ head, int64_t ld,
                                                           const int64_t *__restrict__ rows, int64_t tokens,
-                                                          void *__restrict__ out, int64_t ldo, int64_t out_width, int whole) {
+                                                          void *__restrict__ out, int64_t ldo, int64_t out_width, int whole,
+                                                          const Repeats repeats) {
     __shared__ float lds[SHARE ? 4 : 1][512];
     const int64_t row = blockIdx.x, to = rows ? rows[row] : row;
     if (to < 0 || to >= tokens) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const float held = mass[row], f = weight[row] * *upstream * inverse_t;
+    const float times = repeats.slots ? (float)repeats.slots[repeats.size + repeats.place[row]] : 1.f;
+    const float held = mass[row], f = weight[row] * *upstream * inverse_t * times;
     const float by = held != 0.f ? held / total[row] : 0.f;
     const int64_t c0 = ((int64_t)blockIdx.y * (SHARE ? 1 : 4) + (SHARE ? 0 : wave)) * 512 + lane * 8;
     constexpr int STEP = SHARE ? 4 : 1;
@@ -1556,18 +1596,23 @@ hipError_t logits_in_memory(const Plan &pl, const LogitsParams &p, void *ws, con
     return launch_product<CT_F32>(pl.bp, pl.tri ? 3 : 1, g, pl.chunks, s);
 }
 
-hipError_t pack_hidden(const ct_head_loss *a, const Plan &pl, void *packed, hipStream_t stream) {
+Repeats repeats_of(const ct_head_loss *a, const Plan &pl, const Kept &k, void *kept, bool hidden_grad) {
+    if (!a->rows || !hidden_grad) return Repeats{nullptr, nullptr, 0};
+    return Repeats{at<int>(kept, k.slots), at<int>(kept, k.place), slots_for(pl.rows)};
+}
+
+hipError_t pack_hidden(const ct_head_loss *a, const Plan &pl, void *packed, const Repeats &cleared, hipStream_t stream) {
     const int64_t units = pl.rows_pad / 16 * (pl.width_pad / 32) * 64;
     const Source src = source(a);
     if (pl.tri) {
         pack_split<<<dim3((unsigned)cdiv(units, 256)), dim3(256), 0, stream>>>(src, pl.width_pad / 32,
-                                                                              static_cast<uint4 *>(packed), units);
+                                                                              static_cast<uint4 *>(packed), units, cleared);
         return hipGetLastError();
     }
     const bool vec = a->hidden_width % 8 == 0 && a->ld_hidden % 8 == 0 && reinterpret_cast<uintptr_t>(a->hidden) % 16 == 0;
     const dim3 grid((unsigned)cdiv(units, 256));
-    if (vec) pack_rows<true><<<grid, dim3(256), 0, stream>>>(src, pl.width_pad / 32, static_cast<uint4 *>(packed), units);
-    else pack_rows<false><<<grid, dim3(256), 0, stream>>>(src, pl.width_pad / 32, static_cast<uint4 *>(packed), units);
+    if (vec) pack_rows<true><<<grid, dim3(256), 0, stream>>>(src, pl.width_pad / 32, static_cast<uint4 *>(packed), units, cleared);
+    else pack_rows<false><<<grid, dim3(256), 0, stream>>>(src, pl.width_pad / 32, static_cast<uint4 *>(packed), units, cleared);
     return hipGetLastError();
 }
 hipError_t split_terms(const float *x, int64_t ld, int64_t rows, int64_t cols, uint4 *out, int64_t pitch, int64_t apart,
@@ -1645,17 +1690,18 @@ extern "C" int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t 
     float *shift = at<float>(kept, k.shift), *total = at<float>(kept, k.total), *sums = at<float>(kept, k.sums);
     float *factor = at<float>(workspace, sc.factor);
     const Targets t{a->rows, a->tokens, a->indices, a->values, a->log_normalizer, a->weights, a->ld_indices, a->ld_values};
+    const Repeats repeats = repeats_of(a, pl, k, kept, hidden_grad != 0);
     const auto targets = [&](auto kernel, int threads) {
         kernel<<<dim3((unsigned)pl.rows_pad), dim3(threads), 0, stream>>>(
             t, pl.rows, (int)pl.entries, pl.vocab, pl.units, inverse_t, at<int>(kept, k.index), at<float>(kept, k.q),
             at<float>(kept, k.chosen), at<uint16_t>(kept, k.first), at<float>(kept, k.weight), at<float>(kept, k.mass),
-            at<float>(kept, k.entropy), shift, total);
+            at<float>(kept, k.entropy), shift, total, repeats);
     };
+    CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), repeats, stream));   // clears the slots
     if (pl.entries <= 64) targets(targets_kernel<64, 64>, 64);
     else targets(targets_kernel<256, kMaxEntries>, 256);
     CT_TRY(hipGetLastError());
 
-    CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), stream));
     LogitsParams p = logits_params(a, pl, k, sc, kept, workspace);
     const int64_t piece = sweep_piece(pl, hidden_grad ? 1 : 0);
     for (int64_t v0 = 0; v0 < pl.vocab; v0 += piece) {
@@ -1742,7 +1788,7 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
                 at<const float>(kept, k.sums), pl.splits, pl.rows * pl.width, pl.width, at<const float>(kept, k.weight),
                 at<const float>(kept, k.mass), at<const float>(kept, k.total), upstream, inverse_t,
                 at<const int>(kept, k.index), at<const float>(kept, k.chosen), (int)pl.entries, a->head, a->ld_head, a->rows,
-                a->tokens, d_hidden, ld_d_hidden, d_hidden_width, whole);
+                a->tokens, d_hidden, ld_d_hidden, d_hidden_width, whole, repeats_of(a, pl, k, kept, true));
         };
         const auto pick = [&](auto in, auto out, auto wide) {
             if (share) run(hidden_grad_kernel<decltype(in)::value, decltype(out)::value, decltype(wide)::value, true>);
@@ -1770,7 +1816,7 @@ extern "C" int ct_head_loss_backward(const ct_head_loss *a, const float *upstrea
         at<const float>(kept, k.weight), at<const float>(kept, k.mass), at<const float>(kept, k.shift),
         at<const float>(kept, k.total), upstream, inverse_t, pl.rows, pl.rows_pad, near, factor, inverse);
     CT_TRY(hipGetLastError());
-    CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), stream));
+    CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), Repeats{nullptr, nullptr, 0}, stream));
     const void *hidden;
     int64_t ld;
     CT_TRY(plain_hidden(a, pl, at<void>(workspace, sc.plain), &hidden, &ld, stream));

@@ -647,7 +647,8 @@ int ct_muon(const ct_muon_matrix *matrices, int64_t count, const int32_t *plan, 
  *   loss = sum_i weights_i sum_k q_k (log q_k - log p_iv_k)
  * hidden [tokens, hidden_width], zeros past its columns, and head [vocab, width] of dtype (CT_BF16 or
  * CT_F32). Row i < count of the loss is row rows[i] of hidden, of the targets and of the weights
- * (rows null: row i); a row outside [0, tokens) has no loss. No row may be given twice.
+ * (rows null: row i); a row outside [0, tokens) has no loss, one given twice
+ * counts twice.
  * values null: hard labels, entries = 1, q = 1 (a label outside the vocabulary leaves log sum exp).
  * Otherwise values float32 [*, entries] are the teacher's logits at indices [*, entries] and
  * q = softmax(values / temperature) over a row's entries, or with log_normalizer float32 [*]

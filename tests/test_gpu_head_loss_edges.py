@@ -4,6 +4,8 @@ twice, operands that must not be dropped."""
 import pytest
 import torch
 
+from head_loss_reference import bounds, check, reference
+
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -79,3 +81,73 @@ def test_head_gradient_of_the_most_rows():
     assert ((dw.double() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all()
     with pytest.raises(ValueError, match="head's gradient"):
         run(hidden[:1].expand(rows + 1, width), labels[:1].expand(rows + 1))
+
+
+def _repeated(count, tokens, g):
+    """Row numbers with repeats, some outside the batch, and how often each row is given."""
+    rows = torch.randint(tokens, (count,), device="cuda", generator=g)
+    rows[::7] = -1 - rows[::7]
+    rows[3::11] = tokens + (rows[3::11] << 33)
+    inside = rows[(rows >= 0) & (rows < tokens)]
+    times = torch.bincount(inside, minlength=tokens)
+    return rows, times
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("count,tokens", [(2, 1), (40, 3), (130, 50), (900, 200), (1000, 100000)])
+@pytest.mark.parametrize("teacher", [False, True])
+def test_rows_given_twice_count_twice(teacher, count, tokens, dtype):
+    """As once with their weight times that count: within the bounds of those rows, and the same bits on each call."""
+    from causal_tuner.kernels.loss import distillation_loss, projection_loss
+    g = torch.Generator(device="cuda").manual_seed(count)
+    hidden = torch.randn(tokens, 72, device="cuda", generator=g).to(dtype).requires_grad_()
+    head = (torch.randn(333, 72, device="cuda", generator=g) * 0.3).to(dtype).requires_grad_()
+    weights = torch.rand(tokens, device="cuda", generator=g) + 0.1
+    labels = torch.randint(333, (tokens, 3 if teacher else 1), device="cuda", generator=g)
+    values = torch.randn(tokens, 3, device="cuda", generator=g)
+    rows, times = _repeated(count, tokens, g)
+
+    def run():
+        if teacher:
+            loss = distillation_loss(hidden, head, labels, values, weights, compute_dtype=dtype, rows=rows)
+        else:
+            loss = projection_loss(hidden, head, labels[:, 0], weights, implementation="streamed", compute_dtype=dtype, rows=rows)
+        return (loss.detach(), *torch.autograd.grad(loss, (hidden, head)))
+    got = run()
+    chosen = times.nonzero().flatten()
+    scaled = (weights * times)[chosen]
+    want = reference(hidden[chosen], head, labels[chosen], values[chosen] if teacher else None, scaled)
+    bound = bounds(want[3], scaled, dtype, dtype, dtype)
+    # the head's gradient sums as many terms as there are rows given, not as there are rows
+    more = count * 2.0 ** -24 * (want[3][8].abs().T @ hidden[chosen].detach().double().abs())
+    check("loss", got[0], want[0], bound[0])
+    check("dh", got[1][chosen], want[1], bound[1])
+    check("dW", got[2], want[2], bound[2] + more)
+    assert not got[1][times == 0].any()
+    assert all(torch.equal(a, b) for a, b in zip(got, run()))
+
+
+def test_captured_rows_that_change_between_replays():
+    """The count of each row is taken anew by every replay."""
+    from causal_tuner.kernels.loss import projection_loss
+    g = torch.Generator(device="cuda").manual_seed(5)
+    hidden = torch.randn(90, 64, device="cuda", generator=g).to(BF16).requires_grad_()
+    head = (torch.randn(500, 64, device="cuda", generator=g) * 0.3).to(BF16)
+    labels, weights = torch.randint(500, (90,), device="cuda", generator=g), torch.rand(90, device="cuda", generator=g) + 0.1
+    rows = torch.arange(70, device="cuda")
+
+    def step():
+        loss = projection_loss(hidden, head, labels, weights, implementation="streamed", rows=rows)
+        return (loss.detach(), *torch.autograd.grad(loss, (hidden,)))
+    want = step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for turn in range(4):
+        with torch.no_grad():
+            rows.copy_(_repeated(70, 90, g)[0] if turn % 2 else torch.randperm(90, device="cuda", generator=g)[:70])
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), turn

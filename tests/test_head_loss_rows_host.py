@@ -25,3 +25,13 @@ def test_numbers_outside_the_batch_have_no_loss(which):
     torch.testing.assert_close(got, want, rtol=0, atol=0)
     for a, b in zip(torch.autograd.grad(got, (hidden, head)), torch.autograd.grad(want, (hidden, head))):
         torch.testing.assert_close(a, b, rtol=0, atol=0)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_rows_given_twice_count_twice(which):
+    hidden, head, weights, calls = _calls()
+    got = calls[which](weights, torch.tensor([3, 0, 3, 5, 3, 0]))
+    want = calls[which](weights * torch.tensor([2., 0., 0., 3., 0., 1.]), None)
+    torch.testing.assert_close(got, want)
+    for a, b in zip(torch.autograd.grad(got, (hidden, head)), torch.autograd.grad(want, (hidden, head))):
+        torch.testing.assert_close(a, b)
