@@ -97,9 +97,12 @@ def projection_loss(hidden, head, targets, weights, *, token_budget=128, compute
 
 def _named_rows(selection, tokens):
     """Of row numbers on the host those that name a row, as the device's kernels take them: one outside [0, tokens)
-    has no loss."""
+    has no loss. A mask or a list is taken as its numbers."""
     if isinstance(selection, slice):
         return selection
+    selection = torch.as_tensor(selection)
+    if selection.dtype == torch.bool:
+        return selection.nonzero().flatten()
     return selection[(selection >= 0) & (selection < tokens)]
 
 

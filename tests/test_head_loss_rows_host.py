@@ -35,3 +35,18 @@ def test_rows_given_twice_count_twice(which):
     torch.testing.assert_close(got, want)
     for a, b in zip(torch.autograd.grad(got, (hidden, head)), torch.autograd.grad(want, (hidden, head))):
         torch.testing.assert_close(a, b)
+
+
+@pytest.mark.parametrize("tokens", [1, 6])
+@pytest.mark.parametrize("which", [0, 1])
+def test_masks_and_lists(which, tokens):
+    hidden, head, weights, calls = _calls(tokens)
+    numbers = [0] if tokens == 1 else [1, 3, 4]
+    mask = torch.zeros(tokens, dtype=torch.bool)
+    mask[numbers] = True
+    want = calls[which](weights, torch.tensor(numbers))
+    for rows in (mask, numbers):
+        got = calls[which](weights, rows)
+        torch.testing.assert_close(got, want, rtol=0, atol=0)
+        for a, b in zip(torch.autograd.grad(got, (hidden, head)), torch.autograd.grad(want, (hidden, head), retain_graph=True)):
+            torch.testing.assert_close(a, b, rtol=0, atol=0)
