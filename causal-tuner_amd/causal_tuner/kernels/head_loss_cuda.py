@@ -103,14 +103,15 @@ class StreamedHeadLoss(torch.autograd.Function):
             d_head = (head.shape, head.dtype, lib.ct_head_loss_workspace(*sizes, 2)) if need_head else None
             # the targets are in what is kept
             call.indices = call.values = call.log_normalizer = call.weights = None
-            ctx.plan = (lib.ct_head_loss_backward, call, first, count, sums, kept_bytes, code, d_hidden, d_head)
+            ctx.plan = (lib.ct_head_loss_backward, call, first, count, sums, kept_bytes, code, d_hidden, d_head,
+                        (matrix.stride(), h.stride()))
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, upstream):
         h, matrix, kept, rows = ctx.saved_tensors
-        backward, call, first, count, sums, kept_bytes, code, hidden_plan, head_plan = ctx.plan
+        backward, call, first, count, sums, kept_bytes, code, hidden_plan, head_plan, strides = ctx.plan
         _native.refuse_tangents("streamed head loss", upstream)
         need_hidden, need_head = ctx.needs_input_grad[:2]
         device = matrix.device
@@ -134,14 +135,17 @@ class StreamedHeadLoss(torch.autograd.Function):
             scratch_at = scratch.data_ptr()
         if count:
             # hooks on saved tensors (save_on_cpu) may have brought one back in another place and with other strides
+            if (matrix.stride() != strides[0] or matrix.data_ptr() % 16 or (h is not None and h.stride() != strides[1])
+                    or kept.stride(0) != 1 or (rows is not None and rows.stride(0) != 1)):
+                matrix, kept = _aligned_head(matrix), kept.contiguous()
+                h = None if h is None else _plain_rows(h)
+                rows = None if rows is None else rows.contiguous()
             call = _native.HeadLoss.from_buffer_copy(call)
-            matrix, kept = _aligned_head(matrix), kept.contiguous()
-            rows = None if rows is None else rows.contiguous()
             call.head, call.ld_head, call.rows = matrix.data_ptr(), matrix.stride(0), _native.ptr(rows)
             if h is not None:
-                h = h if _plain(h) else h.clone(memory_format=torch.contiguous_format)
-                call.hidden = h.data_ptr() + first * h.stride(0) * h.element_size()
-                call.ld_hidden = max(h.stride(0), h.shape[1])
+                ld = h.stride(0)
+                call.hidden = h.data_ptr() + first * ld * h.element_size()
+                call.ld_hidden = ld if ld > h.shape[1] else h.shape[1]
             # autograd has made the tensors' device current
             status = backward(call, upstream.to(torch.float32).data_ptr(), kept.data_ptr(), sums, kept_bytes, hidden_at, width,
                               width, hidden_code, head_at, width, width, head_code, scratch_at, scratch_bytes,
