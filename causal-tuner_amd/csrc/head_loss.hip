@@ -1697,10 +1697,13 @@ extern "C" int ct_head_loss_forward(const ct_head_loss *a, float *loss, int32_t 
             at<float>(kept, k.chosen), at<uint16_t>(kept, k.first), at<float>(kept, k.weight), at<float>(kept, k.mass),
             at<float>(kept, k.entropy), shift, total, repeats);
     };
-    CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), repeats, stream));   // clears the slots
+    // Numbered rows are packed first, which clears their slots. Others last: the first launch of a pass waits for
+    // what it reads, longer for the hidden rows than for the tables (one row: 2 us).
+    if (repeats.slots) CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), repeats, stream));
     if (pl.entries <= 64) targets(targets_kernel<64, 64>, 64);
     else targets(targets_kernel<256, kMaxEntries>, 256);
     CT_TRY(hipGetLastError());
+    if (!repeats.slots) CT_TRY(pack_hidden(a, pl, at<void>(workspace, sc.packed), repeats, stream));
 
     LogitsParams p = logits_params(a, pl, k, sc, kept, workspace);
     const int64_t piece = sweep_piece(pl, hidden_grad ? 1 : 0);
