@@ -250,11 +250,11 @@ def ptr(tensor):
 
 
 def refuse_tangents(name, *tensors):
-    """Raises where a tensor carries a forward-mode derivative: a kernel that is called outside
+    """Raises where a tensor (or None) carries a forward-mode derivative: a kernel that is called outside
     an autograd Function would drop it without a word."""
     if getattr(forward_ad, "_current_level", 0) < 0:
         return   # no forward-mode level is open
-    if any(unpack_dual(t).tangent is not None for t in tensors):
+    if any(t is not None and unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{name}: the HIP kernels have no forward-mode derivative")
 
 

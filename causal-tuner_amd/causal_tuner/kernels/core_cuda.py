@@ -68,6 +68,9 @@ class RMS(torch.autograd.Function):
         return (result, dw, None, None, None)[:len(ctx.needs_input_grad)]
 
 
+_is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+
+
 def _layer_norm(x, weight, bias, eps, keep):
     """(x as the kernel reads it, y, mean and rstd [2, rows] or None unless kept, rows, width)."""
     x = x.contiguous()
@@ -78,10 +81,11 @@ def _layer_norm(x, weight, bias, eps, keep):
     if bias is not None:
         bias = bias.contiguous()
     vector = weight if weight is not None else bias
-    y, width = torch.empty_like(x), int(x.shape[-1])   # under a trace sizes are tensors
-    rows = int(x.numel()) // width
+    y, width = torch.empty_like(x), x.shape[-1]
+    rows = x.numel() // width
     stats = mean = rstd = None
     if keep:
+        rows, width = int(rows), int(width)   # under a trace sizes are tensors
         stats = torch.empty((2, rows), device=x.device, dtype=torch.float32)
         mean = stats.data_ptr()
         rstd = mean + 4 * rows
@@ -150,7 +154,7 @@ def layer_norm_device(x, weight, bias, eps):
     given = [t for t in (x, weight, bias) if t is not None]
     _native.refuse_tangents("layer_norm", *given)
     # without gradients the function is passed by, but not under a trace, which would record no call
-    if torch.jit.is_tracing() or (torch.is_grad_enabled() and any(t.requires_grad for t in given)):
+    if _is_tracing() or (torch.is_grad_enabled() and any(t.requires_grad for t in given)):
         return _LayerNorm.apply(x, weight, bias, eps)
     return _layer_norm(x, weight, bias, eps, False)[1]
 

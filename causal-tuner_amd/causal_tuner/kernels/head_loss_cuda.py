@@ -134,18 +134,19 @@ class StreamedHeadLoss(torch.autograd.Function):
             scratch = _workspace(scratch_bytes, device)
             scratch_at = scratch.data_ptr()
         if count:
+            call, head_in = _native.HeadLoss.from_buffer_copy(call), matrix.data_ptr()
             # hooks on saved tensors (save_on_cpu) may have brought one back in another place and with other strides
-            if (matrix.stride() != strides[0] or matrix.data_ptr() % 16 or (h is not None and h.stride() != strides[1])
+            if (matrix.stride() != strides[0] or head_in % 16 or (h is not None and h.stride() != strides[1])
                     or kept.stride(0) != 1 or (rows is not None and rows.stride(0) != 1)):
                 matrix, kept = _aligned_head(matrix), kept.contiguous()
-                h = None if h is None else _plain_rows(h)
+                head_in, call.ld_head = matrix.data_ptr(), matrix.stride(0)
+                if h is not None:
+                    h = _plain_rows(h)
+                    call.ld_hidden = max(h.stride(0), h.shape[1])
                 rows = None if rows is None else rows.contiguous()
-            call = _native.HeadLoss.from_buffer_copy(call)
-            call.head, call.ld_head, call.rows = matrix.data_ptr(), matrix.stride(0), _native.ptr(rows)
+            call.head, call.rows = head_in, _native.ptr(rows)
             if h is not None:
-                ld = h.stride(0)
-                call.hidden = h.data_ptr() + first * ld * h.element_size()
-                call.ld_hidden = ld if ld > h.shape[1] else h.shape[1]
+                call.hidden = h.data_ptr() + first * h.stride(0) * h.element_size()
             # autograd has made the tensors' device current
             status = backward(call, upstream.to(torch.float32).data_ptr(), kept.data_ptr(), sums, kept_bytes, hidden_at, width,
                               width, hidden_code, head_at, width, width, head_code, scratch_at, scratch_bytes,
@@ -167,7 +168,7 @@ def streamed_loss(hidden, head, weights, selection, compute_dtype, indices, valu
     if head.shape[1] > _MAX_WIDTH or len(head) > _MAX_VOCAB:
         raise ValueError(f"streamed head loss: head {tuple(head.shape)}; the HIP kernels take up to {_MAX_VOCAB} entries and "
                          f"a width of {_MAX_WIDTH}")
-    _native.refuse_tangents("streamed head loss", *(t for t in (hidden, head, weights, values, log_normalizer) if t is not None))
+    _native.refuse_tangents("streamed head loss", hidden, head, weights, values, log_normalizer)
     device = hidden.device
     wide = lambda t: None if t is None else t.to(device, torch.float32).contiguous()  # noqa: E731
     tables = (indices.to(torch.int64).contiguous(), wide(values), wide(log_normalizer), wide(weights.flatten()))
