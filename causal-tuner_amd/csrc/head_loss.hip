@@ -1506,7 +1506,7 @@ int check(const ct_head_loss *a, bool hidden, bool forward) {
     if (a->hidden_width <= 0 || a->hidden_width > a->width || a->ld_hidden < a->hidden_width || a->ld_head < a->width ||
         a->ld_hidden > kMaxPitch || a->ld_head > kMaxPitch)
         return -CT_EINVAL_SHAPE;
-    if (forward && !a->values && a->entries != 1) return -CT_EINVAL_SHAPE;
+    if (a->count && forward && !a->values && a->entries != 1) return -CT_EINVAL_SHAPE;   // empty tables have no address
     if (forward && (a->ld_indices < a->entries || (a->values && a->ld_values < a->entries))) return -CT_EINVAL_SHAPE;
     if (up(a->count, 256) * up(a->width, kStep) > kMaxValues) return -CT_EINVAL_SHAPE;
     if (!forward && hidden && a->count > kMaxHeadRows) return -CT_EINVAL_SHAPE;

@@ -151,3 +151,86 @@ def test_captured_rows_that_change_between_replays():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), turn
+
+
+@pytest.mark.parametrize("frozen", [False, True])
+def test_under_a_checkpoint(frozen):
+    """The norm and the loss formed again in the backward: what is kept comes from the second forward."""
+    from torch.utils.checkpoint import checkpoint
+
+    from causal_tuner.kernels.loss import projection_loss
+    from causal_tuner.modeling.norm import LayerNorm
+    norm = LayerNorm(72, 1e-5, BF16, "cuda")
+    x, head = _pitched(90, 72, 104, BF16, 1), _pitched(500, 72, 136, BF16, 2)
+    head.requires_grad_(not frozen)
+    labels, weights = torch.randint(500, (90,), device="cuda"), torch.rand(90, device="cuda") + 0.1
+    rows = torch.tensor([3, 80, 3, 41], device="cuda")
+    leaves = [x, norm.weight, norm.bias] + ([] if frozen else [head])
+    step = lambda x, head: projection_loss(norm(x), head, labels, weights, implementation="streamed", rows=rows)  # noqa: E731
+    want = torch.autograd.grad(step(x, head), leaves)
+    got = torch.autograd.grad(checkpoint(step, x, head, use_reentrant=False), leaves)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("h_type,w_type,compute", [(torch.float16, F32, BF16), (BF16, F32, F32), (F32, BF16, F32),
+                                                   (torch.float16, BF16, F32), (torch.float64, F32, F32)])
+def test_types_beside_the_computed_one(h_type, w_type, compute):
+    """Operands of other types are brought to the computed one first; gradients come in their own."""
+    from causal_tuner.kernels.loss import projection_loss
+    g = torch.Generator(device="cuda").manual_seed(7)
+    hidden = torch.randn(2, 35, 40, device="cuda", generator=g).to(compute).to(h_type).requires_grad_()
+    head = (torch.randn(300, 40, device="cuda", generator=g) * 0.3).to(compute).to(w_type).requires_grad_()
+    labels = torch.randint(300, (2, 35), device="cuda", generator=g, dtype=torch.int32)
+    weights = torch.rand(2, 35, device="cuda", generator=g) + 0.1
+    loss = projection_loss(hidden, head, labels, weights, implementation="streamed", compute_dtype=compute)
+    dh, dw = torch.autograd.grad(loss, (hidden, head))
+    assert dh.dtype == h_type and dw.dtype == w_type and dh.shape == hidden.shape
+    h, w, flat = hidden.detach().reshape(-1, 40).to(compute), head.detach().to(compute), weights.flatten()
+    want = reference(h, w, labels.reshape(-1, 1).long(), None, flat)
+    bound = bounds(want[3], flat, compute, F32, F32)
+    half = {torch.float16: 2.0 ** -11, BF16: 2.0 ** -8, F32: 2.0 ** -24, torch.float64: 0.0}
+    check("loss", loss.detach(), want[0], bound[0])
+    # rounded to the leaf's type beside float32; float16's smallest step near zero is 2^-24
+    for name, got, exact, b, t in (("dh", dh.reshape(-1, 40), want[1], bound[1], h_type), ("dW", dw, want[2], bound[2], w_type)):
+        check(name, got, exact, b + half[t] * (exact.abs() + b) + (2.0 ** -25 if t == torch.float16 else 0.0))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_no_tokens(dtype):
+    from causal_tuner.kernels.loss import distillation_loss, projection_loss
+    hidden = torch.zeros(0, 40, device="cuda", dtype=dtype, requires_grad=True)
+    head = torch.randn(30, 40, device="cuda").to(dtype).requires_grad_()
+    none = torch.zeros(0, dtype=torch.int64, device="cuda")
+    weights, entries = torch.zeros(0, device="cuda"), torch.zeros(0, 3, dtype=torch.int64, device="cuda")
+    for loss in (projection_loss(hidden, head, none, weights, implementation="streamed", compute_dtype=dtype),
+                 distillation_loss(hidden, head, entries, entries.float(), weights, compute_dtype=dtype)):
+        dh, dw = torch.autograd.grad(loss, (hidden, head))
+        assert loss.item() == 0 and dh.shape == hidden.shape and not dw.any()
+
+
+def test_two_streams_at_once():
+    """Calls of two streams share no scratch memory: both run together and give what each gives alone."""
+    from causal_tuner.kernels.loss import projection_loss
+    g = torch.Generator(device="cuda").manual_seed(3)
+    cases = []
+    for rows in (300, 41):
+        hidden = torch.randn(rows, 256, device="cuda", generator=g).to(BF16).requires_grad_()
+        head = (torch.randn(9000, 256, device="cuda", generator=g) * 0.1).to(BF16).requires_grad_()
+        cases.append((hidden, head, torch.randint(9000, (rows,), device="cuda", generator=g),
+                      torch.rand(rows, device="cuda", generator=g) + 0.1, torch.arange(rows, device="cuda") // 2))
+
+    def step(hidden, head, labels, weights, rows):
+        loss = projection_loss(hidden, head, labels, weights, implementation="streamed", rows=rows)
+        return torch.autograd.grad(loss, (hidden, head))
+    want = [step(*case) for case in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for stream, case in zip(streams, cases):
+            with torch.cuda.stream(stream):
+                got.append(step(*case))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
