@@ -101,6 +101,8 @@ def _named_rows(selection, tokens):
     if isinstance(selection, slice):
         return selection
     selection = torch.as_tensor(selection)
+    if selection.numel() == 0:
+        return slice(0, 0)
     if selection.dtype == torch.bool:
         return selection.nonzero().flatten()
     return selection[(selection >= 0) & (selection < tokens)]

@@ -50,3 +50,12 @@ def test_masks_and_lists(which, tokens):
         torch.testing.assert_close(got, want, rtol=0, atol=0)
         for a, b in zip(torch.autograd.grad(got, (hidden, head)), torch.autograd.grad(want, (hidden, head), retain_graph=True)):
             torch.testing.assert_close(a, b, rtol=0, atol=0)
+
+
+@pytest.mark.parametrize("rows", [[], torch.zeros(0, dtype=torch.int64), torch.tensor([-1, 9])])
+@pytest.mark.parametrize("which", [0, 1])
+def test_no_rows(which, rows):
+    hidden, head, weights, calls = _calls()
+    loss = calls[which](weights, rows)
+    dh, dw = torch.autograd.grad(loss, (hidden, head))
+    assert loss.item() == 0 and not dh.any() and not dw.any()
